@@ -19,13 +19,19 @@ FJX_DTYPE_F32 = 0
 FJX_DTYPE_BF16 = 1
 FJX_OUTGOING = 0
 FJX_INCOMING = 1
+FJX_CODES_NONE = 0
+FJX_CODES_E4M3 = 1
+FJX_CODES_INT8 = 2
+FJX_SHARE_N = 1
+FJX_SHARE_M = 2
+FJX_SHARE_C = 4
 FJX_OK = 0
 FJX_ERR_INVALID = 1
 FJX_ERR_UNSUPPORTED = 2
 FJX_ERR_WORKSPACE = 3
 FJX_ERR_HIP = 4
 
-ABI_VERSION = 6
+ABI_VERSION = 7
 NOALLOC_SCRATCH_BYTES = 3 * 591 * 640 * 256
 
 _vp = ctypes.c_void_p
@@ -33,6 +39,8 @@ _i64 = ctypes.c_int64
 _i32 = ctypes.c_int32
 _f32 = ctypes.c_float
 _sz = ctypes.c_size_t
+_u64 = ctypes.c_uint64
+_i64x3 = _i64 * 3
 
 
 class TriMulArgs(ctypes.Structure):
@@ -102,6 +110,50 @@ class SingleAttentionArgs(ctypes.Structure):
     ]
 
 
+class DiffAttentionArgs(ctypes.Structure):
+    _fields_ = [
+        ("items", _i64), ("heads", _i64), ("kv_heads", _i64), ("nq", _i64), ("nk", _i64), ("head_dim", _i64),
+        ("bias_share", _i64), ("dtype", _i32), ("scale", _f32), ("lambda_init", _f32),
+        ("q", _vp), ("k", _vp), ("v", _vp), ("out", _vp),
+        ("q_strides", _i64x3), ("k_strides", _i64x3), ("v_strides", _i64x3), ("out_strides", _i64x3),
+        ("bias", _vp), ("bias_strides", _i64x3), ("mask", _vp), ("lambda_vectors", _vp), ("stats", _vp),
+        ("workspace", _vp), ("workspace_bytes", _sz),
+    ]
+
+
+class DiffAttentionBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("fwd", DiffAttentionArgs),
+        ("dout", _vp), ("dq", _vp), ("dk", _vp), ("dv", _vp),
+        ("dq_strides", _i64x3), ("dk_strides", _i64x3), ("dv_strides", _i64x3),
+        ("dbias", _vp), ("dbias_strides", _i64x3), ("dlambda", _vp),
+    ]
+
+
+class RmsNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", _i64), ("c", _i64), ("dtype", _i32), ("eps", _f32),
+        ("x", _vp), ("residual", _vp), ("weight", _vp), ("sum_out", _vp), ("out", _vp),
+        ("codes", _i32), ("group", _i64), ("scales", _vp),
+    ]
+
+
+class RmsNormBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", _i64), ("c", _i64), ("dtype", _i32), ("eps", _f32),
+        ("dy", _vp), ("h", _vp), ("weight", _vp), ("dh", _vp), ("dx", _vp), ("dweight", _vp),
+        ("workspace", _vp), ("workspace_bytes", _sz),
+    ]
+
+
+class DropoutArgs(ctypes.Structure):
+    _fields_ = [
+        ("batch", _i64), ("n", _i64), ("m", _i64), ("c", _i64), ("dtype", _i32), ("shared", _i32),
+        ("p", ctypes.c_double), ("seed", _u64), ("offset", _u64), ("step", _vp),
+        ("x", _vp), ("residual", _vp), ("out_mask", _vp), ("out", _vp),
+    ]
+
+
 # every symbol the header declares, with its ctypes signature
 SYMBOLS = {
     "fjx_trimul_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i32]),
@@ -116,6 +168,14 @@ SYMBOLS = {
     "fjx_pair_bias_size": (_sz, [_i64, _i64, _i64, _i32]),
     "fjx_single_attention_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i32]),
     "fjx_single_attention_fwd": (ctypes.c_int, [ctypes.POINTER(SingleAttentionArgs), _vp]),
+    "fjx_diff_attention_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64, _i32]),
+    "fjx_diff_attention_fwd": (ctypes.c_int, [ctypes.POINTER(DiffAttentionArgs), _vp]),
+    "fjx_diff_attention_bwd_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i64, _i32]),
+    "fjx_diff_attention_bwd": (ctypes.c_int, [ctypes.POINTER(DiffAttentionBwdArgs), _vp]),
+    "fjx_rms_norm_fwd": (ctypes.c_int, [ctypes.POINTER(RmsNormArgs), _vp]),
+    "fjx_rms_norm_bwd_workspace_size": (_sz, [_i64, _i64]),
+    "fjx_rms_norm_bwd": (ctypes.c_int, [ctypes.POINTER(RmsNormBwdArgs), _vp]),
+    "fjx_dropout_fwd": (ctypes.c_int, [ctypes.POINTER(DropoutArgs), _vp]),
     "fjx_last_error": (ctypes.c_char_p, []),
     "fjx_abi_version": (ctypes.c_int, []),
     "fjx_prof_enable": (ctypes.c_int, [ctypes.c_int]),

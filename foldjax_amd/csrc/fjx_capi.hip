@@ -11,6 +11,7 @@
 
 #include "fjx_tri.h"
 #include "fjx_common.hpp"
+#include "fjx_diffattn.hpp"
 #include "fjx_kernels.hpp"
 
 using namespace fjx;
@@ -58,13 +59,19 @@ enum KernelId {
   K_SINGLE_FLASH,
   K_SINGLE_OUT,
   K_SINGLE_TRANSITION,
+  K_DIFF_ATTENTION_FWD,
+  K_DIFF_ATTENTION_BWD,
+  K_RMS_NORM_FWD,
+  K_RMS_NORM_BWD,
+  K_DROPOUT,
   K_COUNT
 };
 const char* kKernelNames[K_COUNT] = {"trimul_prologue", "trimul_contract", "trimul_epilogue",
                                      "triattn_prologue", "triattn_flash", "triattn_epilogue",
                                      "triattn_core_prep", "transition",     "single_proj",
                                      "single_pair_bias", "single_flash",   "single_out",
-                                     "single_transition"};
+                                     "single_transition", "diff_attention_fwd", "diff_attention_bwd",
+                                     "rms_norm_fwd",     "rms_norm_bwd",   "dropout"};
 
 struct Prof {
   std::mutex mu;
@@ -1102,6 +1109,232 @@ int trimul_dispatch(const fjx_trimul_args* a, bool tight, hipStream_t st) {
   return a->dtype == FJX_DTYPE_BF16 ? trimul_run<bf16>(a, tight, st) : trimul_run<float>(a, tight, st);
 }
 
+// ------------------------------------------------- differential attention
+// How a forward call is cut: 64 query rows of a key/value head to a workgroup,
+// or 16 rows with the keys over its four waves (keywise), and the keys over
+// `splits` workgroups of `split_blocks` 128-key blocks each.
+struct DiffPlan {
+  bool keywise;
+  int splits;
+  int64_t split_blocks;
+  size_t part_o, part_ml;  // workspace bytes
+};
+DiffPlan diff_plan(int64_t items, int64_t heads, int64_t kv_heads, int64_t nq, int64_t nk, int64_t d) {
+  const int64_t rows = heads / kv_heads * nq;
+  DiffPlan p = {};
+  p.keywise = rows <= 16 || items * kv_heads * ((rows + 63) / 64) < 256;
+  p.splits = 1;
+  const int64_t blocks = p.keywise ? (nk + 127) / 128 : (nk + 63) / 64;
+  p.split_blocks = blocks;
+  if (p.keywise) {
+    const int64_t wgs = items * kv_heads * ((rows + 15) / 16);
+    const int64_t want = std::min<int64_t>((512 + wgs - 1) / wgs, blocks / 2);  // two blocks a split at least
+    if (want > 1) {
+      p.split_blocks = (blocks + want - 1) / want;
+      p.splits = (int)((blocks + p.split_blocks - 1) / p.split_blocks);
+    }
+  }
+  if (p.splits > 1) {
+    const size_t r = (size_t)items * heads * nq * p.splits * 2;
+    p.part_o = align_up(r * 2 * d * sizeof(float));
+    p.part_ml = align_up(r * 2 * sizeof(float));
+  }
+  return p;
+}
+
+// The bias gradient of shared planes: items of one chunk, so that the 64 x 64
+// tiles times the chunks are some workgroups a CU.
+struct DiffBwdPlan {
+  int chunks;
+  int64_t chunk_items;
+  size_t delta, part;
+};
+DiffBwdPlan diff_bwd_plan(int64_t items, int64_t heads, int64_t nq, int64_t nk, int64_t share, bool with_dbias) {
+  DiffBwdPlan p = {};
+  p.delta = align_up((size_t)items * 2 * heads * nq * sizeof(float));
+  if (with_dbias && share > 1) {
+    const int64_t planes = items / share;
+    const int64_t tiles = planes * heads * ((nq + 63) / 64) * ((nk + 63) / 64);
+    const int64_t want = std::max<int64_t>(1, std::min<int64_t>((1024 + tiles - 1) / tiles, share));
+    p.chunk_items = (share + want - 1) / want;
+    p.chunks = (int)((share + p.chunk_items - 1) / p.chunk_items);
+    p.part = align_up((size_t)p.chunks * planes * heads * nq * nk * sizeof(float));
+  }
+  return p;
+}
+
+// strides that the kernels' 16-byte accesses of rows take; `write`: axes longer
+// than one must not fall together
+bool diff_strides_ok(const int64_t* s, int64_t items, int64_t heads, int64_t n, size_t es, bool write) {
+  const int64_t len[3] = {items, heads, n};
+  for (int i = 0; i < 3; ++i)
+    if (len[i] > 1 && (s[i] < (write ? 1 : 0) || s[i] * (int64_t)es % 16)) return false;
+  return true;
+}
+
+int diff_check(const fjx_diff_attention_args* a, const char* fn, const void* out) {
+  if (a->items < 1 || a->heads < 1 || a->kv_heads < 1 || a->nq < 1 || a->nk < 1)
+    return fail(FJX_ERR_INVALID, "%s: items, heads, kv_heads, nq and nk must be >= 1", fn);
+  if (!dtype_ok(a->dtype)) return fail(FJX_ERR_INVALID, "%s: unknown dtype %d", fn, a->dtype);
+  if ((a->head_dim != 32 && a->head_dim != 64) || a->heads > 1024)
+    return fail(FJX_ERR_UNSUPPORTED, "%s: this build supports head_dim 32 and 64 and at most 1024 heads, got %lld and %lld",
+                fn, (long long)a->head_dim, (long long)a->heads);
+  if (a->heads % a->kv_heads)
+    return fail(FJX_ERR_INVALID, "%s: kv_heads must divide heads, got %lld and %lld", fn, (long long)a->kv_heads,
+                (long long)a->heads);
+  constexpr int64_t kLong = (int64_t)1 << 31;
+  if (a->nq >= kLong || a->nk >= kLong || a->items >= kLong)
+    return fail(FJX_ERR_UNSUPPORTED, "%s: items, nq and nk must be below 2^31", fn);
+  if (!a->q || !a->k || !a->v || !out || !a->lambda_vectors)
+    return fail(FJX_ERR_INVALID, "%s: a required pointer is NULL", fn);
+  if (!aligned16({a->q, a->k, a->v, out, a->lambda_vectors}))
+    return fail(FJX_ERR_INVALID, "%s: tensors must be 16-byte aligned", fn);
+  const size_t es = esize(a->dtype);
+  if (!diff_strides_ok(a->q_strides, a->items, 2 * a->heads, a->nq, es, false) ||
+      !diff_strides_ok(a->k_strides, a->items, 2 * a->kv_heads, a->nk, es, false) ||
+      !diff_strides_ok(a->v_strides, a->items, a->kv_heads, a->nk, es, false) ||
+      !diff_strides_ok(a->out_strides, a->items, a->heads, a->nq, es, out == a->out))
+    return fail(FJX_ERR_INVALID, "%s: strides must be multiples of 16 bytes, not negative (an output's: positive)", fn);
+  if (a->bias) {
+    if (a->bias_share < 1 || a->items % a->bias_share)
+      return fail(FJX_ERR_INVALID, "%s: bias_share must divide items, got %lld and %lld", fn, (long long)a->bias_share,
+                  (long long)a->items);
+    if (a->bias_strides[0] < 0 || a->bias_strides[1] < 0 || a->bias_strides[2] < 0 ||
+        reinterpret_cast<uintptr_t>(a->bias) % es)
+      return fail(FJX_ERR_INVALID, "%s: bias strides must be >= 0 and the bias aligned to its elements", fn);
+  }
+  // the longest launch: a workgroup takes 16 query rows or 64 keys of a head
+  const double blocks = (double)a->items * a->kv_heads *
+                        std::max((double)(a->heads / a->kv_heads) * a->nq / 16 + 1, (double)a->nk / 64 + 1);
+  if (blocks >= (1 << 23)) return fail(FJX_ERR_UNSUPPORTED, "%s: more rows than one launch takes", fn);
+  return FJX_OK;
+}
+
+template <typename T>
+DiffAttnParams<T> diff_params(const fjx_diff_attention_args* a) {
+  DiffAttnParams<T> p = {};
+  auto view = [](const void* ptr, const int64_t* s) { return HeadsView<const T>{static_cast<const T*>(ptr), s[0], s[1], s[2]}; };
+  p.q = view(a->q, a->q_strides);
+  p.k = view(a->k, a->k_strides);
+  p.v = view(a->v, a->v_strides);
+  p.bias = view(a->bias, a->bias_strides);
+  p.mask = a->mask;
+  p.lam = a->lambda_vectors;
+  p.items = a->items;
+  p.nq = a->nq;
+  p.nk = a->nk;
+  p.share = a->bias ? a->bias_share : 1;
+  p.heads = (int)a->heads;
+  p.group = (int)(a->heads / a->kv_heads);
+  p.scale = a->scale;
+  p.scale_log2 = a->scale * kLog2e;
+  p.init = a->lambda_init;
+  return p;
+}
+
+template <typename T>
+int diff_fwd_run(const fjx_diff_attention_args* a, const DiffPlan& plan, hipStream_t st) {
+  DiffAttnParams<T> p = diff_params<T>(a);
+  p.out = {static_cast<T*>(a->out), a->out_strides[0], a->out_strides[1], a->out_strides[2]};
+  p.stats = a->stats;
+  p.splits = plan.splits;
+  p.split_blocks = plan.split_blocks;
+  p.part_o = at<float>(a->workspace, 0);
+  p.part_ml = at<float>(a->workspace, plan.part_o);
+  return timed(K_DIFF_ATTENTION_FWD, st, "diff_attention_fwd",
+               [&] { launch_diffattn_fwd<T>(p, (int)a->head_dim, plan.keywise, st); });
+}
+
+template <typename T>
+int diff_bwd_run(const fjx_diff_attention_bwd_args* b, const DiffBwdPlan& plan, hipStream_t st) {
+  const fjx_diff_attention_args* a = &b->fwd;
+  DiffAttnParams<T> p = diff_params<T>(a);
+  auto view = [](void* ptr, const int64_t* s) { return HeadsView<T>{static_cast<T*>(ptr), s[0], s[1], s[2]}; };
+  p.dout = {static_cast<const T*>(b->dout), a->out_strides[0], a->out_strides[1], a->out_strides[2]};
+  p.dq = view(b->dq, b->dq_strides);
+  p.dk = view(b->dk, b->dk_strides);
+  p.dv = view(b->dv, b->dv_strides);
+  p.dbias = view(b->dbias, b->dbias_strides);
+  p.saved = a->stats;
+  p.dlam = b->dlambda;
+  p.delta = at<float>(a->workspace, 0);
+  p.part_bias = at<float>(a->workspace, plan.delta);
+  p.chunks = plan.chunks;
+  p.chunk_items = plan.chunk_items;
+  return timed(K_DIFF_ATTENTION_BWD, st, "diff_attention_bwd",
+               [&] { launch_diffattn_bwd<T>(p, (int)a->head_dim, st); });
+}
+
+// -------------------------------------------------------------- RMS norm
+template <typename T>
+int rms_norm_run(const fjx_rms_norm_args* a, hipStream_t st) {
+  RmsNormParams<T> p = {};
+  p.x = static_cast<const T*>(a->x);
+  p.residual = static_cast<const T*>(a->residual);
+  p.w = static_cast<const T*>(a->weight);
+  p.h = static_cast<T*>(a->sum_out);
+  p.y = a->codes ? nullptr : static_cast<T*>(a->out);
+  p.codes = a->out;
+  p.scales = a->scales;
+  p.rows = a->rows;
+  p.c = (int)a->c;
+  p.group = (int)(a->group ? a->group : a->c);
+  p.eps = a->eps;
+  return timed(K_RMS_NORM_FWD, st, "rms_norm_fwd", [&] { launch_rmsnorm<T>(p, a->codes, st); });
+}
+
+template <typename T>
+int rms_norm_bwd_run(const fjx_rms_norm_bwd_args* a, hipStream_t st) {
+  RmsNormBwdParams<T> p = {};
+  p.dy = static_cast<const T*>(a->dy);
+  p.h = static_cast<const T*>(a->h);
+  p.w = static_cast<const T*>(a->weight);
+  p.dh = static_cast<const T*>(a->dh);
+  p.dx = static_cast<T*>(a->dx);
+  p.part = static_cast<float*>(a->workspace);
+  p.rows = a->rows;
+  p.c = (int)a->c;
+  p.eps = a->eps;
+  return timed(K_RMS_NORM_BWD, st, "rms_norm_bwd", [&] { launch_rmsnorm_bwd<T>(p, a->dweight, st); });
+}
+
+int rms_norm_shape(const char* fn, int64_t rows, int64_t c, int32_t dtype) {
+  if (rows < 1) return fail(FJX_ERR_INVALID, "%s: rows must be >= 1", fn);
+  if (!dtype_ok(dtype)) return fail(FJX_ERR_INVALID, "%s: unknown dtype %d", fn, dtype);
+  if (c < 8 || c % 8 || c > 8192)
+    return fail(FJX_ERR_UNSUPPORTED, "%s: c must be a multiple of 8 in [8, 8192], got %lld", fn, (long long)c);
+  if (rows >= (int64_t)1 << 40) return fail(FJX_ERR_UNSUPPORTED, "%s: too many rows", fn);
+  return FJX_OK;
+}
+
+// --------------------------------------------------------------- dropout
+template <typename T>
+int dropout_run(const fjx_dropout_args* a, hipStream_t st) {
+  DropoutParams<T> p = {};
+  p.x = static_cast<const T*>(a->x);
+  p.residual = static_cast<const T*>(a->residual);
+  p.out_mask = static_cast<const T*>(a->out_mask);
+  p.out = static_cast<T*>(a->out);
+  p.j = a->m;
+  p.c = (int)a->c;
+  p.share_i = a->shared & FJX_SHARE_N;
+  p.share_j = a->shared & FJX_SHARE_M;
+  p.by_channel = !(a->shared & FJX_SHARE_C);
+  p.frees = a->batch * (p.share_i ? 1 : a->n) * (p.share_j ? 1 : a->m);
+  p.run = (p.share_i ? a->n : 1) * (p.share_j ? a->m : 1);
+  // 8 positions a thread along a run, so that the generator's ten rounds are
+  // shared, but half a million threads (the card's) before that
+  const int64_t threads = p.frees * (a->c / 8);
+  p.run_part = std::min<int64_t>(p.run, std::max<int64_t>(1, std::min<int64_t>(8, threads * p.run >> 19)));
+  p.parts = (p.run + p.run_part - 1) / p.run_part;
+  p.threshold = (uint32_t)(a->p * 4294967296.0);
+  p.scale = (float)(1.0 / (1.0 - a->p));
+  p.seed = a->seed;
+  p.offset = a->offset;
+  p.step = a->step;
+  return timed(K_DROPOUT, st, "dropout", [&] { launch_dropout<T>(p, st); });
+}
+
 }  // namespace
 
 extern "C" {
@@ -1289,6 +1522,120 @@ int fjx_single_attention_fwd(const fjx_single_attention_args* a, hipStream_t st)
   const bool bf = a->dtype == FJX_DTYPE_BF16, zbf = a->z_dtype == FJX_DTYPE_BF16;
   if (bf) return zbf ? single_run<bf16, bf16>(a, st) : single_run<bf16, float>(a, st);
   return zbf ? single_run<float, bf16>(a, st) : single_run<float, float>(a, st);
+}
+
+size_t fjx_diff_attention_workspace_size(int64_t items, int64_t heads, int64_t kv_heads, int64_t nq, int64_t nk,
+                                         int64_t head_dim, int32_t dtype) {
+  if (items < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || nq < 1 || nk < 1 || head_dim < 1 || !dtype_ok(dtype))
+    return 0;
+  const DiffPlan p = diff_plan(items, heads, kv_heads, nq, nk, head_dim);
+  return p.part_o + p.part_ml;
+}
+
+int fjx_diff_attention_fwd(const fjx_diff_attention_args* a, hipStream_t st) {
+  g_err.clear();
+  if (!a) return fail(FJX_ERR_INVALID, "fjx_diff_attention_fwd: args is NULL");
+  if (int rc = diff_check(a, "fjx_diff_attention_fwd", a->out)) return rc;
+  const DiffPlan plan = diff_plan(a->items, a->heads, a->kv_heads, a->nq, a->nk, a->head_dim);
+  const size_t need = plan.part_o + plan.part_ml;
+  if (need && (!a->workspace || a->workspace_bytes < need))
+    return fail(FJX_ERR_WORKSPACE, "fjx_diff_attention_fwd: workspace of %zu bytes needed, %zu given", need,
+                a->workspace_bytes);
+  if (need && !aligned16({a->workspace}))
+    return fail(FJX_ERR_INVALID, "fjx_diff_attention_fwd: the workspace must be 16-byte aligned");
+  return a->dtype == FJX_DTYPE_BF16 ? diff_fwd_run<bf16>(a, plan, st) : diff_fwd_run<float>(a, plan, st);
+}
+
+size_t fjx_diff_attention_bwd_workspace_size(int64_t items, int64_t heads, int64_t nq, int64_t nk, int64_t bias_share,
+                                             int32_t with_dbias) {
+  if (items < 1 || heads < 1 || nq < 1 || nk < 1 || (with_dbias && (bias_share < 1 || items % bias_share))) return 0;
+  const DiffBwdPlan p = diff_bwd_plan(items, heads, nq, nk, bias_share, with_dbias != 0);
+  return p.delta + p.part;
+}
+
+int fjx_diff_attention_bwd(const fjx_diff_attention_bwd_args* b, hipStream_t st) {
+  const char* fn = "fjx_diff_attention_bwd";
+  g_err.clear();
+  if (!b) return fail(FJX_ERR_INVALID, "%s: args is NULL", fn);
+  const fjx_diff_attention_args* a = &b->fwd;
+  if (int rc = diff_check(a, fn, b->dout)) return rc;
+  if (!b->dq || !b->dk || !b->dv || !b->dlambda || !a->stats) return fail(FJX_ERR_INVALID, "%s: a required pointer is NULL", fn);
+  if (!aligned16({b->dq, b->dk, b->dv})) return fail(FJX_ERR_INVALID, "%s: tensors must be 16-byte aligned", fn);
+  const size_t es = esize(a->dtype);
+  if (!diff_strides_ok(b->dq_strides, a->items, 2 * a->heads, a->nq, es, true) ||
+      !diff_strides_ok(b->dk_strides, a->items, 2 * a->kv_heads, a->nk, es, true) ||
+      !diff_strides_ok(b->dv_strides, a->items, a->kv_heads, a->nk, es, true))
+    return fail(FJX_ERR_INVALID, "%s: the gradients' strides must be positive multiples of 16 bytes", fn);
+  if (b->dbias) {
+    const int64_t len[3] = {a->bias ? a->items / a->bias_share : 0, a->heads, a->nq};
+    for (int i = 0; i < 3; ++i)
+      if (!a->bias || (len[i] > 1 && b->dbias_strides[i] < 1))
+        return fail(FJX_ERR_INVALID, "%s: dbias needs a bias and positive strides", fn);
+    if (reinterpret_cast<uintptr_t>(b->dbias) % es)
+      return fail(FJX_ERR_INVALID, "%s: dbias must be aligned to its elements", fn);
+  }
+  const DiffBwdPlan plan = diff_bwd_plan(a->items, a->heads, a->nq, a->nk, a->bias ? a->bias_share : 1, b->dbias != nullptr);
+  const double tiles = (double)std::max(plan.chunks, 1) * a->items * a->heads * (a->nq / 64 + 1.0) * (a->nk / 64 + 1.0) /
+                       (a->bias ? a->bias_share : a->items);
+  if (plan.chunks && tiles >= (1 << 23)) return fail(FJX_ERR_UNSUPPORTED, "%s: more bias than one launch takes", fn);
+  const size_t need = plan.delta + plan.part;
+  if (!a->workspace || a->workspace_bytes < need)
+    return fail(FJX_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", fn, need, a->workspace_bytes);
+  if (!aligned16({a->workspace})) return fail(FJX_ERR_INVALID, "%s: the workspace must be 16-byte aligned", fn);
+  return a->dtype == FJX_DTYPE_BF16 ? diff_bwd_run<bf16>(b, plan, st) : diff_bwd_run<float>(b, plan, st);
+}
+
+int fjx_rms_norm_fwd(const fjx_rms_norm_args* a, hipStream_t st) {
+  const char* fn = "fjx_rms_norm_fwd";
+  g_err.clear();
+  if (!a) return fail(FJX_ERR_INVALID, "%s: args is NULL", fn);
+  if (int rc = rms_norm_shape(fn, a->rows, a->c, a->dtype)) return rc;
+  if (a->codes < FJX_CODES_NONE || a->codes > FJX_CODES_INT8) return fail(FJX_ERR_INVALID, "%s: unknown codes %d", fn, a->codes);
+  if (!a->x || !a->weight || !a->out || (a->codes && !a->scales))
+    return fail(FJX_ERR_INVALID, "%s: a required pointer is NULL", fn);
+  if (a->codes && a->group && ((a->group != 32 && a->group != 64 && a->group != 128) || a->c % a->group))
+    return fail(FJX_ERR_UNSUPPORTED, "%s: group must be 0, 32, 64 or 128 and divide c, got %lld for c=%lld", fn,
+                (long long)a->group, (long long)a->c);
+  if (!aligned16({a->x, a->residual, a->weight, a->sum_out, a->out}))
+    return fail(FJX_ERR_INVALID, "%s: tensors must be 16-byte aligned", fn);
+  if (a->sum_out == a->out || (a->codes && (a->out == a->x || a->out == a->residual)))
+    return fail(FJX_ERR_INVALID, "%s: out must be a buffer of its own", fn);
+  return a->dtype == FJX_DTYPE_BF16 ? rms_norm_run<bf16>(a, st) : rms_norm_run<float>(a, st);
+}
+
+size_t fjx_rms_norm_bwd_workspace_size(int64_t rows, int64_t c) {
+  if (rows < 1 || c < 8 || c % 8 || c > 8192) return 0;
+  return align_up((size_t)rmsnorm_bwd_blocks(rows, (int)c) * c * sizeof(float));
+}
+
+int fjx_rms_norm_bwd(const fjx_rms_norm_bwd_args* a, hipStream_t st) {
+  const char* fn = "fjx_rms_norm_bwd";
+  g_err.clear();
+  if (!a) return fail(FJX_ERR_INVALID, "%s: args is NULL", fn);
+  if (int rc = rms_norm_shape(fn, a->rows, a->c, a->dtype)) return rc;
+  if (!a->dy || !a->h || !a->weight || !a->dx || !a->dweight) return fail(FJX_ERR_INVALID, "%s: a required pointer is NULL", fn);
+  if (!aligned16({a->dy, a->h, a->weight, a->dh, a->dx})) return fail(FJX_ERR_INVALID, "%s: tensors must be 16-byte aligned", fn);
+  const size_t need = fjx_rms_norm_bwd_workspace_size(a->rows, a->c);
+  if (!a->workspace || a->workspace_bytes < need)
+    return fail(FJX_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", fn, need, a->workspace_bytes);
+  return a->dtype == FJX_DTYPE_BF16 ? rms_norm_bwd_run<bf16>(a, st) : rms_norm_bwd_run<float>(a, st);
+}
+
+int fjx_dropout_fwd(const fjx_dropout_args* a, hipStream_t st) {
+  const char* fn = "fjx_dropout_fwd";
+  g_err.clear();
+  if (!a) return fail(FJX_ERR_INVALID, "%s: args is NULL", fn);
+  if (a->batch < 1 || a->n < 1 || a->m < 1) return fail(FJX_ERR_INVALID, "%s: batch, n and m must be >= 1", fn);
+  if (!dtype_ok(a->dtype)) return fail(FJX_ERR_INVALID, "%s: unknown dtype %d", fn, a->dtype);
+  if (a->c < 8 || a->c % 8 || a->c >= (int64_t)1 << 30)
+    return fail(FJX_ERR_UNSUPPORTED, "%s: c must be a multiple of 8 in [8, 2^30), got %lld", fn, (long long)a->c);
+  if (a->shared & ~7) return fail(FJX_ERR_INVALID, "%s: unknown shared axes %d", fn, a->shared);
+  if (!(a->p >= 0.0 && a->p < 1.0)) return fail(FJX_ERR_INVALID, "%s: p must be in [0, 1), got %g", fn, a->p);
+  if ((double)a->batch * a->n * a->m * a->c >= 0x1p50) return fail(FJX_ERR_UNSUPPORTED, "%s: too many elements", fn);
+  if (!a->x || !a->out) return fail(FJX_ERR_INVALID, "%s: a required pointer is NULL", fn);
+  if (!aligned16({a->x, a->residual, a->out})) return fail(FJX_ERR_INVALID, "%s: tensors must be 16-byte aligned", fn);
+  if (reinterpret_cast<uintptr_t>(a->step) % 8) return fail(FJX_ERR_INVALID, "%s: step must be 8-byte aligned", fn);
+  return a->dtype == FJX_DTYPE_BF16 ? dropout_run<bf16>(a, st) : dropout_run<float>(a, st);
 }
 
 int fjx_prof_enable(int on) {

@@ -1,0 +1,333 @@
+// Differential attention, forward: one pass over the keys with the running
+// maximum and sum of both softmaxes.
+#include "fjx_diffattn.hpp"
+
+namespace fjx {
+
+namespace {
+
+// A wave holds 16 query rows, lane l row l % 16 of them, and walks the keys in
+// tiles of 16: S_t^T = K_t Q_t^T leaves the lane 4 keys of its own row a tile
+// (keys 4 g + r, g = l / 16), so a row's maximum and sum are the lane's own
+// values and two lane swaps, and the weights of two tiles are the operand of
+// O_t^T = V^T P_t^T as they lie.
+//
+// The two outputs are subtracted at the end, where they may nearly cancel (two
+// maps that are almost the same, lambda near one), so a bf16 weight would be
+// rounded relative to a sum several times the result: weights go into the
+// product as two bf16 parts.
+// A weight may exceed 1 by up to 2^kSlack before the maximum is moved, which
+// saves the outputs' rescaling in all but the first blocks of a row.
+constexpr float kSlack = 8.f;
+
+// KEYWISE: the four waves share one 16-row tile and take 32 keys each of a
+// 128-key block, for calls with few rows; otherwise each has 16 rows of its own
+// and walks every 64-key block.
+template <typename T, int D, bool KEYWISE>
+__global__ __launch_bounds__(256) void diffattn_fwd_kernel(DiffAttnParams<T> P) {
+  constexpr int kRows = KEYWISE ? 128 : 64;    // keys of a block
+  constexpr int kNt = KEYWISE ? 2 : 4;         // key tiles of a wave in one
+  constexpr int kBufs = KEYWISE ? 1 : 2;
+  constexpr int kC = D / 32, kU = 2 * D / 16;  // k-steps of a score, tiles of 16 values
+  typedef typename Frag<T>::type F;
+  typedef DaTile<T, D, kRows> Tile;
+  constexpr size_t kMerge = 4 * 16 * 2 * (2 * D + 4) * sizeof(float);
+  constexpr size_t kBytes = kBufs * sizeof(Tile) > kMerge || !KEYWISE ? kBufs * sizeof(Tile) : kMerge;
+  __shared__ __attribute__((aligned(16))) unsigned char raw[kBytes];
+  __shared__ __attribute__((aligned(16))) float key_on[kBufs][kRows];
+  Tile* tiles = reinterpret_cast<Tile*>(raw);
+
+  const int t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int kvh = P.heads / P.group;
+  const int64_t rows = P.group * P.nq;  // of one key/value head
+  const int64_t row_blocks = KEYWISE ? (rows + 15) / 16 : (rows + 63) / 64;
+  int64_t id = xcd_order(blockIdx.x, gridDim.x);
+  if (id >= P.items * kvh * row_blocks * P.splits) return;
+  const int64_t rb = id % row_blocks;
+  id /= row_blocks;
+  const int split = (int)(id % P.splits);
+  id /= P.splits;
+  const int kv = (int)(id % kvh);
+  const int64_t item = id / kvh;
+
+  const int64_t row = KEYWISE ? rb * 16 + li : rb * 64 + 16 * wave + li;
+  const bool row_on = row < rows;
+  const int64_t row_c = row_on ? row : rows - 1;
+  const int hg = (int)(row_c / P.nq);
+  const int64_t qi = row_c - hg * P.nq;
+  const int head = kv * P.group + hg;
+
+  DaStage<T, D, kRows, 256> st;
+  st.init(P.k.p + item * P.k.item + 2 * kv * P.k.head, P.k.head, P.k.token, P.v.p + item * P.v.item + kv * P.v.head,
+          P.v.token, t);
+  const uint8_t* mask = P.mask ? P.mask + item * P.nk : nullptr;
+  const T* bias = P.bias.p ? P.bias.p + (item / P.share) * P.bias.item + head * P.bias.head + qi * P.bias.token : nullptr;
+
+  const int64_t blocks = (P.nk + kRows - 1) / kRows;
+  const int64_t blk0 = split * P.split_blocks;
+  const int64_t blk1 = blk0 + P.split_blocks < blocks ? blk0 + P.split_blocks : blocks;
+
+  st.load(blk0 * kRows, P.nk, mask);
+  F qf[2][kC];
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int c = 0; c < kC; ++c)
+      qf[m][c] = load8(P.q.p + item * P.q.item + (2 * head + m) * P.q.head + qi * P.q.token + 32 * c + 8 * lg);
+  const float lam = da_lambda<D>(P.lam, P.heads, head, P.init, lane);
+
+  // a key that takes part adds nothing, or lets the bias through: 0, or +inf
+  // for the minimum with the bias; one that does not is -inf either way (also
+  // against a NaN in the bias)
+  const float on = bias ? INFINITY : 0.f;
+  auto key_flags = [&](int64_t blk, int buf) {
+    if (t < kRows) {
+      const int64_t k = blk * kRows + t;
+      key_on[buf][t] = k < P.nk && (!mask || mask[k]) ? on : -INFINITY;
+    }
+  };
+  const int key_w = KEYWISE ? 32 * wave : 0;  // this wave's keys of a block
+  f32x4 bv[kNt];
+  auto load_bias = [&](int64_t blk) {
+    const int64_t k0 = blk * kRows + key_w + 4 * lg;
+    if ((blk + 1) * kRows <= P.nk) {
+#pragma unroll
+      for (int kt = 0; kt < kNt; ++kt) bv[kt] = load4_any(bias + k0 + 16 * kt);
+    } else {
+#pragma unroll
+      for (int kt = 0; kt < kNt; ++kt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) bv[kt][r] = k0 + 16 * kt + r < P.nk ? to_f32(bias[k0 + 16 * kt + r]) : 0.f;
+    }
+  };
+  if (bias && blk0 < blk1) load_bias(blk0);
+
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  f32x4 o[2][kU];
+#pragma unroll
+  for (int mp = 0; mp < 2; ++mp)
+#pragma unroll
+    for (int u = 0; u < kU; ++u) o[mp][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  st.store(tiles[0]);
+  key_flags(blk0, 0);
+  __syncthreads();
+
+  for (int64_t blk = blk0; blk < blk1; ++blk) {
+    const int buf = kBufs == 2 ? (int)(blk - blk0) & 1 : 0;
+    const Tile& tile = tiles[buf];
+    const bool more = blk + 1 < blk1;
+    f32x4 b[kNt];
+#pragma unroll
+    for (int kt = 0; kt < kNt; ++kt) {
+      b[kt] = *reinterpret_cast<const f32x4*>(&key_on[buf][key_w + 16 * kt + 4 * lg]);
+      if (bias) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) b[kt][r] = fminf(bv[kt][r] * kLog2e, b[kt][r]);
+      }
+    }
+    if (more) {
+      st.load((blk + 1) * kRows, P.nk, mask);
+      if (bias) load_bias(blk + 1);
+    }
+    F pf[2][kNt / 2][kParts<T>];
+#pragma unroll
+    for (int mp = 0; mp < 2; ++mp) {
+      f32x4 s[kNt];
+#pragma unroll
+      for (int kt = 0; kt < kNt; ++kt) {
+        s[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < kC; ++c) mma(s[kt], load8(&tile.a[mp][key_w + 16 * kt + li][32 * c + 8 * lg]), qf[mp][c]);
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int kt = 0; kt < kNt; ++kt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          s[kt][r] = fmaf(s[kt][r], P.scale_log2, b[kt][r]);
+          top = fmaxf(top, s[kt][r]);
+        }
+      top = group_max(top);
+      if (__builtin_amdgcn_ballot_w64(top > m[mp] + kSlack)) {
+        const float mn = fmaxf(m[mp], top);
+        const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[mp] - mn);
+        m[mp] = mn;
+        l[mp] *= alpha;
+#pragma unroll
+        for (int u = 0; u < kU; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[mp][u][r] *= alpha;
+      }
+      const float base = m[mp] == -INFINITY ? 0.f : m[mp];  // no key so far: every weight is 0
+      float p[kNt / 2][8];
+#pragma unroll
+      for (int kt = 0; kt < kNt; ++kt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float e = __builtin_amdgcn_exp2f(s[kt][r] - base);
+          l[mp] += e;
+          p[kt >> 1][4 * (kt & 1) + r] = e;
+        }
+#pragma unroll
+      for (int c = 0; c < kNt / 2; ++c) parts(p[c], pf[mp][c]);
+    }
+#pragma unroll
+    for (int c = 0; c < kNt / 2; ++c)
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        const F v = col_frag(&tile.b[0][0], Tile::kB, key_w + 32 * c, 16 * u, lane);
+        mma_parts(o[0][u], v, pf[0][c]);
+        mma_parts(o[1][u], v, pf[1][c]);
+      }
+    if (kBufs == 1) __syncthreads();
+    if (more) {
+      st.store(tiles[kBufs == 2 ? buf ^ 1 : 0]);
+      key_flags(blk + 1, kBufs == 2 ? buf ^ 1 : 0);
+    }
+    __syncthreads();
+  }
+  l[0] = group_sum(l[0]);
+  l[1] = group_sum(l[1]);
+
+  if constexpr (KEYWISE) {
+    // the waves' partial rows, on the largest of their maxima
+    float* ml = reinterpret_cast<float*>(raw);                 // [wave][map][row][2]
+    float* po = ml + 4 * 2 * 16 * 2;                           // [wave][map][row][2 D + 2]
+    constexpr int kPo = 2 * D + 2;
+    if (lg == 0)
+      for (int mp = 0; mp < 2; ++mp) {
+        ml[((wave * 2 + mp) * 16 + li) * 2] = m[mp];
+        ml[((wave * 2 + mp) * 16 + li) * 2 + 1] = l[mp];
+      }
+    __syncthreads();
+#pragma unroll
+    for (int mp = 0; mp < 2; ++mp) {
+      float mx = -INFINITY, ls = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) mx = fmaxf(mx, ml[((w * 2 + mp) * 16 + li) * 2]);
+      const float base = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        ls = fmaf(ml[((w * 2 + mp) * 16 + li) * 2 + 1], __builtin_amdgcn_exp2f(ml[((w * 2 + mp) * 16 + li) * 2] - base), ls);
+      const float alpha = __builtin_amdgcn_exp2f(m[mp] - base);
+#pragma unroll
+      for (int u = 0; u < kU; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) po[((wave * 2 + mp) * 16 + li) * kPo + 16 * u + 4 * lg + r] = o[mp][u][r] * alpha;
+      m[mp] = mx;
+      l[mp] = ls;
+    }
+    __syncthreads();
+    // each wave takes kU / 4 of the tiles of 16 values
+#pragma unroll
+    for (int mp = 0; mp < 2; ++mp)
+#pragma unroll
+      for (int u = 0; u < kU / 4; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float a = 0.f;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) a += po[((w * 2 + mp) * 16 + li) * kPo + 16 * (wave * (kU / 4) + u) + 4 * lg + r];
+          o[mp][u][r] = a;
+        }
+  }
+  if (!row_on) return;
+  constexpr int kOwn = KEYWISE ? kU / 4 : kU;
+  const int u0 = KEYWISE ? wave * kOwn : 0;
+  const bool first = lg == 0 && (!KEYWISE || wave == 0);
+  const int64_t at = item * P.heads * P.nq + (int64_t)head * P.nq + qi;
+  if (P.splits > 1) {
+    const int64_t base = (split * (P.items * P.heads * P.nq) + at) * 2;
+#pragma unroll
+    for (int mp = 0; mp < 2; ++mp) {
+      if (first) *reinterpret_cast<f32x2*>(P.part_ml + (base + mp) * 2) = f32x2{m[mp], l[mp]};
+#pragma unroll
+      for (int u = 0; u < kOwn; ++u)
+        *reinterpret_cast<f32x4*>(P.part_o + (base + mp) * (2 * D) + 16 * (u0 + u) + 4 * lg) = o[mp][u];
+    }
+    return;
+  }
+  float inv[2];
+#pragma unroll
+  for (int mp = 0; mp < 2; ++mp) {
+    inv[mp] = l[mp] == 0.f ? 0.f : 1.f / l[mp];  // a row without keys is zeros
+    if (first && P.stats)  // +inf for such a row: its weights are zeros in the backward pass as well
+      P.stats[(item * 2 * P.heads + 2 * head + mp) * P.nq + qi] = l[mp] == 0.f ? INFINITY : m[mp] + log2f(l[mp]);
+  }
+  inv[1] *= lam;
+  T* out = P.out.p + item * P.out.item + head * P.out.head + qi * P.out.token;
+#pragma unroll
+  for (int u = 0; u < kOwn; ++u) {
+    float v[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = o[0][u][r] * inv[0] - o[1][u][r] * inv[1];
+    store4f(out + 16 * (u0 + u) + 4 * lg, v);
+  }
+}
+
+// The splits of a row joined: a wave a row, lane l holding 2 D / 64 values.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void diffattn_join_kernel(DiffAttnParams<T> P) {
+  const int lane = threadIdx.x & 63;
+  const int64_t rows = P.items * P.heads * P.nq;
+  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (at >= rows) return;
+  const int64_t qi = at % P.nq, ih = at / P.nq;
+  const int head = (int)(ih % P.heads);
+  const int64_t item = ih / P.heads;
+  const float lam = da_lambda<D>(P.lam, P.heads, head, P.init, lane);
+  float res[2 * D / 64] = {};
+#pragma unroll
+  for (int mp = 0; mp < 2; ++mp) {
+    float mx = -INFINITY;
+    for (int s = lane; s < P.splits; s += 64) mx = fmaxf(mx, P.part_ml[((s * rows + at) * 2 + mp) * 2]);
+#pragma unroll
+    for (int x = 32; x >= 1; x >>= 1) mx = fmaxf(mx, shfl_xor(mx, x));
+    const float base = mx == -INFINITY ? 0.f : mx;
+    float l = 0.f, o[2 * D / 64] = {};
+#pragma unroll 4
+    for (int s = 0; s < P.splits; ++s) {
+      const int64_t i = (s * rows + at) * 2 + mp;
+      const f32x2 v = *reinterpret_cast<const f32x2*>(P.part_ml + i * 2);
+      const float w = __builtin_amdgcn_exp2f(v[0] - base);
+      l = fmaf(v[1], w, l);
+#pragma unroll
+      for (int j = 0; j < 2 * D / 64; ++j) o[j] = fmaf(P.part_o[i * (2 * D) + 64 * j + lane], w, o[j]);
+    }
+    const float inv = (l == 0.f ? 0.f : 1.f / l) * (mp ? -lam : 1.f);
+#pragma unroll
+    for (int j = 0; j < 2 * D / 64; ++j) res[j] = fmaf(o[j], inv, res[j]);
+    if (lane == 0 && P.stats) P.stats[(item * 2 * P.heads + 2 * head + mp) * P.nq + qi] = l == 0.f ? INFINITY : mx + log2f(l);
+  }
+  T* out = P.out.p + item * P.out.item + head * P.out.head + qi * P.out.token;
+#pragma unroll
+  for (int j = 0; j < 2 * D / 64; ++j) out[64 * j + lane] = from_f32<T>(res[j]);
+}
+
+template <typename T, int D>
+void fwd(const DiffAttnParams<T>& P, bool keywise, hipStream_t st) {
+  const int64_t rows = P.group * P.nq;
+  const int64_t blocks = P.items * (P.heads / P.group) * P.splits * (keywise ? (rows + 15) / 16 : (rows + 63) / 64);
+  const dim3 grid((unsigned)((blocks + 7) / 8 * 8));
+  if (keywise)
+    diffattn_fwd_kernel<T, D, true><<<grid, 256, 0, st>>>(P);
+  else
+    diffattn_fwd_kernel<T, D, false><<<grid, 256, 0, st>>>(P);
+  if (P.splits > 1) diffattn_join_kernel<T, D><<<(unsigned)((P.items * P.heads * P.nq + 3) / 4), 256, 0, st>>>(P);
+}
+
+}  // namespace
+
+template <typename T>
+void launch_diffattn_fwd(const DiffAttnParams<T>& P, int d, bool keywise, hipStream_t st) {
+  if (d == 32)
+    fwd<T, 32>(P, keywise, st);
+  else
+    fwd<T, 64>(P, keywise, st);
+}
+template void launch_diffattn_fwd<bf16>(const DiffAttnParams<bf16>&, int, bool, hipStream_t);
+template void launch_diffattn_fwd<float>(const DiffAttnParams<float>&, int, bool, hipStream_t);
+
+}  // namespace fjx

@@ -1,0 +1,215 @@
+// What the kernels of differential attention share: the staged tiles, their
+// fragments, the per-key masks and the weight of the second map.
+//
+//   S_t = scale q_t k_t^T + bias  (t = 1, 2),  P_t = softmax over the keys
+//   out = (P_1 - lambda P_2) v,  lambda_h = exp(a_1 . b_1) - exp(a_2 . b_2) + init
+//
+// The heads of one key/value head are worked on together: its query rows are
+// the nq queries of each of the heads / kv_heads query heads, one after the
+// other, so that a single token's heads fill one 16-row tile and read the
+// cache once. Scores are in log2 units: scale log2(e) and log2(e) are folded
+// into one fma, and a bias whose product with log2(e) leaves float32's range
+// (the types' lowest values) is -inf, as a masked key is.
+#pragma once
+
+#include "fjx_common.hpp"
+#include "fjx_kernels.hpp"
+
+namespace fjx {
+
+// strides in elements: item, head, token
+template <typename T>
+struct HeadsView {
+  T* p;
+  int64_t item, head, token;
+};
+
+template <typename T>
+struct DiffAttnParams {
+  HeadsView<const T> q, k, v;  // [items][2 H][nq][D], [items][2 Hk][nk][D], [items][Hk][nk][2 D]
+  HeadsView<T> out;            // [items][H][nq][2 D]
+  HeadsView<const T> bias;     // [items / share][H][nq][nk] (item: plane, token: query), or null
+  const uint8_t* mask;         // [items][nk] or null
+  const float* lam;            // [4][H][D]: a_1, b_1, a_2, b_2
+  float* stats;                // [items][2 H][nq] row statistics, or null
+  int64_t items, nq, nk, share;
+  int heads, group;            // query heads, and those of one key/value head
+  float scale_log2, init;
+  // keys split over workgroups: key blocks of one split, and the partial
+  // results [split][items][H nq rows][2 maps]: values [2 D], then (max, sum)
+  int splits;
+  int64_t split_blocks;
+  float* part_o;
+  float* part_ml;
+  // backward
+  HeadsView<const T> dout;     // [items][H][nq][2 D]
+  HeadsView<T> dq, dk, dv;
+  HeadsView<T> dbias;          // as bias, or null
+  const float* saved;          // the forward pass's stats
+  float* delta;                // [items][2 H][nq]: rowsum(P_t dP)
+  float* dlam;                 // [4][H][D]
+  float* part_bias;            // [chunks][planes][H][nq][nk] partial sums of dbias
+  int64_t chunk_items;         // items of one chunk
+  int chunks;
+  float scale;
+};
+
+constexpr int kDaKeys = 64;  // keys (or, for the keys' gradients, queries) of a staged block
+
+// one staged block: two tiles of D columns and one of 2 D, rows padded by 16
+// bytes so that 16 rows' 16-byte pieces fall on distinct banks
+template <typename T, int D, int ROWS>
+struct DaTile {
+  static constexpr int kA = D + 16 / (int)sizeof(T);      // row pitch of the two
+  static constexpr int kB = 2 * D + 16 / (int)sizeof(T);  // of the third
+  T a[2][ROWS][kA];
+  T b[ROWS][kB];
+};
+
+// 8 k-slots of a column operand: rows row0 + 4 g + 0..3 and row0 + 16 + 4 g +
+// 0..3 (g = lane / 16) of column col0 + lane % 16, the rows that a lane's
+// accumulators of two adjacent 16-row score tiles hold
+__device__ __forceinline__ bf16x8 col_frag(const bf16* tile, int pitch, int row0, int col0, int lane) {
+  // ds_read_b64_tr_b16: the 16 lanes of a group name 4 rows x 16 columns in
+  // row order, and lane i gets the 4 rows of column i
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  typedef short s16x8 __attribute__((ext_vector_type(8)));
+  typedef __attribute__((address_space(3))) s16x4 lds4;
+  const bf16* p = tile + (row0 + 4 * (lane >> 4) + ((lane >> 2) & 3)) * pitch + col0 + 4 * (lane & 3);
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p));
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 16 * pitch));
+  return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+__device__ __forceinline__ f32x8 col_frag(const float* tile, int pitch, int row0, int col0, int lane) {
+  const float* p = tile + (row0 + 4 * (lane >> 4)) * pitch + col0 + (lane & 15);
+  f32x8 v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    v[e] = p[e * pitch];
+    v[4 + e] = p[(16 + e) * pitch];
+  }
+  return v;
+}
+
+// A float32 operand that the kernel computed (weights, dS) as the matrix
+// instructions take it: itself, or two bf16 parts (16 bits; the high one cut,
+// not rounded: the low one holds what is left either way), whose products take
+// twice the matrix instructions. These run beside the exponentials and the
+// vector work that bound the kernels.
+template <typename T> constexpr int kParts = sizeof(T) == 2 ? 2 : 1;
+__device__ __forceinline__ void parts(const float* p, bf16x8 (&f)[2]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float hi = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, p[e]) & 0xffff0000u);
+    f[0][e] = static_cast<bf16>(hi);
+    f[1][e] = static_cast<bf16>(p[e] - hi);
+  }
+}
+__device__ __forceinline__ void parts(const float* p, f32x8 (&f)[1]) { f[0] = pack8<float>(p); }
+__device__ __forceinline__ void mma_parts(f32x4& o, const bf16x8& a, const bf16x8 (&p)[2]) {
+  mma(o, a, p[1]);
+  mma(o, a, p[0]);
+}
+__device__ __forceinline__ void mma_parts(f32x4& o, const f32x8& a, const f32x8 (&p)[1]) { mma(o, a, p[0]); }
+
+// 4 contiguous elements with element alignment only (rows of an odd length)
+__device__ __forceinline__ f32x4 load4_any(const bf16* p) {
+  typedef bf16x4 any4 __attribute__((aligned(2)));
+  const bf16x4 v = *reinterpret_cast<const any4*>(p);
+  return f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
+}
+__device__ __forceinline__ f32x4 load4_any(const float* p) {
+  typedef f32x4 any4 __attribute__((aligned(4)));
+  return *reinterpret_cast<const any4*>(p);
+}
+
+// max over the 4 lanes {l % 16 + 16 g}
+__device__ __forceinline__ float group_max(float x) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t a0 = a[0], a1 = a[1];
+  const uint32_t v = __builtin_bit_cast(uint32_t, fmaxf(__builtin_bit_cast(float, a0), __builtin_bit_cast(float, a1)));
+  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  const uint32_t b0 = b[0], b1 = b[1];
+  return fmaxf(__builtin_bit_cast(float, b0), __builtin_bit_cast(float, b1));
+}
+
+// lambda of `head`, the lane's own; the 4 lanes of a row take a quarter of
+// the two dot products each. e[0], e[1]: the two exponentials
+template <int D>
+__device__ __forceinline__ float da_lambda(const float* lam, int heads, int head, float init, int lane, float* e = nullptr) {
+  float dot[2] = {0.f, 0.f};
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const float* a = lam + ((int64_t)(2 * t) * heads + head) * D + (lane >> 4) * (D / 4);
+    const float* b = a + (int64_t)heads * D;
+#pragma unroll
+    for (int d = 0; d < D / 4; d += 4) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(a + d), y = *reinterpret_cast<const f32x4*>(b + d);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) dot[t] = fmaf(x[r], y[r], dot[t]);
+    }
+    dot[t] = group_sum(dot[t]);
+  }
+  const float e1 = expf(dot[0]), e2 = expf(dot[1]);
+  if (e) e[0] = e1, e[1] = e2;
+  return e1 - e2 + init;
+}
+
+// The pieces of one block that a thread moves from memory to LDS: 16 bytes
+// of a row at a time, the same columns of every `step`-th row. Rows past n,
+// and those that the mask takes out, are zeros: a weight of zero times what
+// padding holds there must stay zero.
+template <typename T, int D, int ROWS, int THREADS>
+struct DaStage {
+  static constexpr int kE = 16 / (int)sizeof(T);           // elements of a piece
+  static constexpr int kPa = D / kE;                       // pieces of a row of the first two
+  static constexpr int kPk = 4 * kPa;                      // pieces of a row in all
+  static constexpr int kStep = THREADS / kPk;              // rows between a thread's pieces
+  static constexpr int kN = ROWS / kStep;                  // pieces of a thread
+  static_assert(THREADS % kPk == 0 && ROWS % kStep == 0, "whole pieces");
+  u32x4 r[kN];
+  const T* src;
+  int64_t pitch;
+  int row, which, col;
+
+  // a, b: the rows' bases; a_head: elements between the two a tiles
+  __device__ __forceinline__ void init(const T* a, int64_t a_head, int64_t a_token, const T* b, int64_t b_token,
+                                       int t) {
+    const int in = t % kPk;
+    row = t / kPk;
+    which = in / kPa;  // 0, 1: the a tiles; 2, 3: the halves of b
+    col = (in % kPa) * kE + (which == 3 ? D : 0);
+    src = (which < 2 ? a + which * a_head : b) + col;
+    pitch = which < 2 ? a_token : b_token;
+  }
+  __device__ __forceinline__ void load(int64_t row0, int64_t n, const uint8_t* mask) {
+    bool on[kN];
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const int64_t x = row0 + row + i * kStep;
+      on[i] = x < n;
+      if (on[i] && mask) on[i] = mask[x] != 0;
+    }
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      r[i] = u32x4{0, 0, 0, 0};
+      if (on[i]) r[i] = *reinterpret_cast<const u32x4*>(src + (row0 + row + i * kStep) * pitch);
+    }
+  }
+  __device__ __forceinline__ void store(DaTile<T, D, ROWS>& tile) const {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const int x = row + i * kStep;
+      T* d = which < 2 ? &tile.a[which & 1][x][col] : &tile.b[x][col];
+      *reinterpret_cast<u32x4*>(d) = r[i];
+    }
+  }
+};
+
+// workgroups in an order that keeps neighbours (the tiles of one item, which
+// read the same keys) on one of the 8 XCDs, to which the hardware deals block
+// after block in turn; grids are multiples of 8 blocks
+__device__ __forceinline__ int64_t xcd_order(int64_t blk, int64_t blocks) { return (blk & 7) * (blocks >> 3) + (blk >> 3); }
+
+}  // namespace fjx

@@ -1,0 +1,602 @@
+// Differential attention, backward. With dP = dO v^T and
+//   D_t = rowsum(P_t dP),  dS_1 = P_1 (dP - D_1),  dS_2 = -lambda P_2 (dP - D_2):
+//   dq_t = scale dS_t k_t,  dk_t = scale dS_t^T q_t,  dv = (P_1 - lambda P_2)^T dO,
+//   dbias = dS_1 + dS_2,  dlambda = -sum D_2
+// The weights come again from the scores and the forward pass's row statistics
+// L_t = log2 sum 2^x: P_t = 2^(x - L_t). Every sum has one owner and one order:
+// no atomics, and the same bits each time.
+//
+// dS's rows sum to zero, so its products may cancel: like the weights it goes
+// into them as two bf16 parts, and a gradient is off by its own rounding. With
+// one part dq and dk were off by 1.4 times as much (1.5 at a few keys).
+#include "fjx_diffattn.hpp"
+
+namespace fjx {
+
+namespace {
+
+template <typename T>
+__device__ __forceinline__ void store4_any(T* p, const f32x4& v);
+template <>
+__device__ __forceinline__ void store4_any<bf16>(bf16* p, const f32x4& v) {
+  typedef bf16x4 any4 __attribute__((aligned(2)));
+  *reinterpret_cast<any4*>(p) = bf16x4{(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3]};
+}
+template <>
+__device__ __forceinline__ void store4_any<float>(float* p, const f32x4& v) {
+  typedef f32x4 any4 __attribute__((aligned(4)));
+  *reinterpret_cast<any4*>(p) = v;
+}
+
+// a bias's 4 keys of each of 4 tiles, from k0 + 4 g on
+template <typename T>
+__device__ __forceinline__ void bias_tile(const T* bias, int64_t k0, int64_t nk, bool whole, f32x4 (&bv)[4]) {
+  if (whole) {
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt) bv[kt] = load4_any(bias + k0 + 16 * kt);
+  } else {
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) bv[kt][r] = k0 + 16 * kt + r < nk ? to_f32(bias[k0 + 16 * kt + r]) : 0.f;
+  }
+}
+
+// scores of the wave's 16 rows and a block's 64 keys, one map, as weights
+template <typename T, int D>
+__device__ __forceinline__ void tile_weights(const DaTile<T, D, kDaKeys>& tile, int mp, const typename Frag<T>::type (&qf)[D / 32],
+                                             const f32x4 (&b)[4], float scale_log2, float L, int li, int lg,
+                                             f32x4 (&p)[4]) {
+#pragma unroll
+  for (int kt = 0; kt < 4; ++kt) {
+    p[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) mma(p[kt], load8(&tile.a[mp][16 * kt + li][32 * c + 8 * lg]), qf[c]);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) p[kt][r] = __builtin_amdgcn_exp2f(fmaf(p[kt][r], scale_log2, b[kt][r]) - L);
+  }
+}
+
+template <typename T, int D>
+__device__ __forceinline__ void tile_dp(const DaTile<T, D, kDaKeys>& tile, const typename Frag<T>::type (&dof)[2 * D / 32], int li,
+                                        int lg, f32x4 (&dp)[4]) {
+#pragma unroll
+  for (int kt = 0; kt < 4; ++kt) {
+    dp[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < 2 * D / 32; ++c) mma(dp[kt], load8(&tile.b[16 * kt + li][32 * c + 8 * lg]), dof[c]);
+  }
+}
+
+// dq, and D_t, and dbias where every item has a bias of its own. A wave holds
+// 16 query rows (lane l row l % 16) as in the forward pass and goes over the
+// keys twice: for D_t, then for dS_t.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void diffattn_dq_kernel(DiffAttnParams<T> P) {
+  constexpr int kC = D / 32, kU = D / 16;
+  typedef typename Frag<T>::type F;
+  typedef DaTile<T, D, kDaKeys> Tile;
+  __shared__ __attribute__((aligned(16))) Tile tiles[2];
+  __shared__ __attribute__((aligned(16))) float key_on[2][kDaKeys];
+
+  const int t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int kvh = P.heads / P.group;
+  const int64_t rows = P.group * P.nq;
+  const int64_t row_blocks = (rows + 63) / 64;
+  int64_t id = xcd_order(blockIdx.x, gridDim.x);
+  if (id >= P.items * kvh * row_blocks) return;
+  const int64_t rb = id % row_blocks;
+  id /= row_blocks;
+  const int kv = (int)(id % kvh);
+  const int64_t item = id / kvh;
+  const int64_t row = rb * 64 + 16 * wave + li;
+  const bool row_on = row < rows;
+  const int64_t row_c = row_on ? row : rows - 1;
+  const int hg = (int)(row_c / P.nq);
+  const int64_t qi = row_c - hg * P.nq;
+  const int head = kv * P.group + hg;
+
+  DaStage<T, D, kDaKeys, 256> st;
+  st.init(P.k.p + item * P.k.item + 2 * kv * P.k.head, P.k.head, P.k.token, P.v.p + item * P.v.item + kv * P.v.head,
+          P.v.token, t);
+  const uint8_t* mask = P.mask ? P.mask + item * P.nk : nullptr;
+  const int64_t plane = P.bias.p ? item / P.share : 0;
+  const T* bias = P.bias.p ? P.bias.p + plane * P.bias.item + head * P.bias.head + qi * P.bias.token : nullptr;
+  T* dbias = P.dbias.p && P.share == 1 && row_on
+                 ? P.dbias.p + plane * P.dbias.item + head * P.dbias.head + qi * P.dbias.token
+                 : nullptr;
+
+  st.load(0, P.nk, mask);
+  F qf[2][kC], dof[2 * kC];
+  float L[2];
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    L[m] = P.saved[(item * 2 * P.heads + 2 * head + m) * P.nq + qi];
+#pragma unroll
+    for (int c = 0; c < kC; ++c)
+      qf[m][c] = load8(P.q.p + item * P.q.item + (2 * head + m) * P.q.head + qi * P.q.token + 32 * c + 8 * lg);
+  }
+#pragma unroll
+  for (int c = 0; c < 2 * kC; ++c)
+    dof[c] = load8(P.dout.p + item * P.dout.item + head * P.dout.head + qi * P.dout.token + 32 * c + 8 * lg);
+  const float lam = da_lambda<D>(P.lam, P.heads, head, P.init, lane);
+  const float on = bias ? INFINITY : 0.f;
+  auto key_flags = [&](int64_t blk, int buf) {
+    if (t < kDaKeys) {
+      const int64_t k = blk * kDaKeys + t;
+      key_on[buf][t] = k < P.nk && (!mask || mask[k]) ? on : -INFINITY;
+    }
+  };
+  f32x4 bv[4];
+  const int64_t blocks = (P.nk + kDaKeys - 1) / kDaKeys;
+  if (bias) bias_tile(bias, 4 * lg, P.nk, kDaKeys <= P.nk, bv);
+
+  float Dt[2] = {0.f, 0.f};
+  f32x4 dq[2][kU];
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int u = 0; u < kU; ++u) dq[m][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  st.store(tiles[0]);
+  key_flags(0, 0);
+  __syncthreads();
+  int buf = 0;
+  for (int sweep = 0; sweep < 2; ++sweep) {
+    for (int64_t blk = 0; blk < blocks; ++blk, buf ^= 1) {
+      const Tile& tile = tiles[buf];
+      const bool more = sweep == 0 || blk + 1 < blocks;
+      const int64_t next = blk + 1 < blocks ? blk + 1 : 0;
+      f32x4 b[4];
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt) {
+        b[kt] = *reinterpret_cast<const f32x4*>(&key_on[buf][16 * kt + 4 * lg]);
+        if (bias) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) b[kt][r] = fminf(bv[kt][r] * kLog2e, b[kt][r]);
+        }
+      }
+      if (more) {
+        st.load(next * kDaKeys, P.nk, mask);
+        if (bias) bias_tile(bias, next * kDaKeys + 4 * lg, P.nk, (next + 1) * kDaKeys <= P.nk, bv);
+      }
+      f32x4 dp[4];
+      tile_dp<T, D>(tile, dof, li, lg, dp);
+      f32x4 both[4];
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        f32x4 p[4];
+        tile_weights<T, D>(tile, m, qf[m], b, P.scale_log2, L[m], li, lg, p);
+        if (sweep == 0) {
+#pragma unroll
+          for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) Dt[m] = fmaf(p[kt][r], dp[kt][r], Dt[m]);
+          continue;
+        }
+        const float by = m ? -lam : 1.f;
+        float ds[2][8];
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float x = p[kt][r] * by * (dp[kt][r] - Dt[m]);
+            ds[kt >> 1][4 * (kt & 1) + r] = x;
+            both[kt][r] = m ? both[kt][r] + x : x;
+          }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          F f[kParts<T>];
+          parts(ds[c], f);
+#pragma unroll
+          for (int u = 0; u < kU; ++u)
+            mma_parts(dq[m][u], col_frag(&tile.a[m][0][0], Tile::kA, 32 * c, 16 * u, lane), f);
+        }
+      }
+      if (sweep == 1 && dbias) {
+        const int64_t k0 = blk * kDaKeys + 4 * lg;
+        if ((blk + 1) * kDaKeys <= P.nk) {
+#pragma unroll
+          for (int kt = 0; kt < 4; ++kt) store4_any<T>(dbias + k0 + 16 * kt, both[kt]);
+        } else {
+#pragma unroll
+          for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (k0 + 16 * kt + r < P.nk) dbias[k0 + 16 * kt + r] = from_f32<T>(both[kt][r]);
+        }
+      }
+      if (more) {
+        st.store(tiles[buf ^ 1]);
+        key_flags(next, buf ^ 1);
+      }
+      __syncthreads();
+    }
+    if (sweep == 0) {
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        Dt[m] = group_sum(Dt[m]);
+        if (row_on && lg == 0) P.delta[(item * 2 * P.heads + 2 * head + m) * P.nq + qi] = Dt[m];
+      }
+    }
+  }
+  if (!row_on) return;
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    T* out = P.dq.p + item * P.dq.item + (2 * head + m) * P.dq.head + qi * P.dq.token;
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      float v[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] = dq[m][u][r] * P.scale;
+      store4f(out + 16 * u + 4 * lg, v);
+    }
+  }
+}
+
+// dk and dv: a wave owns 16 keys (lane l key l % 16, its k and v in registers)
+// and walks the query blocks of every head that shares them. S_t = Q_t K_t^T
+// leaves the lane 4 queries of its key a tile, the operand of dS_t^T Q_t and of
+// (P_1 - lambda P_2)^T dO as they lie.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void diffattn_dkv_kernel(DiffAttnParams<T> P) {
+  constexpr int kC = D / 32, kU = D / 16, kQ = kDaKeys;
+  typedef typename Frag<T>::type F;
+  typedef DaTile<T, D, kQ> Tile;
+  __shared__ __attribute__((aligned(16))) Tile tiles[2];
+  __shared__ __attribute__((aligned(16))) float row_stat[2][4][kQ];  // L_1, L_2, D_1, D_2
+
+  const int t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int kvh = P.heads / P.group;
+  const int64_t key_blocks = (P.nk + 63) / 64;
+  int64_t id = xcd_order(blockIdx.x, gridDim.x);
+  if (id >= P.items * kvh * key_blocks) return;
+  const int64_t kb = id % key_blocks;
+  id /= key_blocks;
+  const int kv = (int)(id % kvh);
+  const int64_t item = id / kvh;
+  const int64_t key = kb * 64 + 16 * wave + li;
+  const bool in = key < P.nk;
+  const bool part = in && (!P.mask || P.mask[item * P.nk + key]);
+
+  F kf[2][kC], vf[2 * kC];
+  F zero;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) zero[e] = from_f32<T>(0.f);
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int c = 0; c < kC; ++c)
+      kf[m][c] = part ? load8(P.k.p + item * P.k.item + (2 * kv + m) * P.k.head + key * P.k.token + 32 * c + 8 * lg) : zero;
+#pragma unroll
+  for (int c = 0; c < 2 * kC; ++c)
+    vf[c] = part ? load8(P.v.p + item * P.v.item + kv * P.v.head + key * P.v.token + 32 * c + 8 * lg) : zero;
+  const bool biased = P.bias.p != nullptr;
+  const float key_on = part ? (biased ? INFINITY : 0.f) : -INFINITY;
+  const int64_t plane = biased ? item / P.share : 0;
+  const T* bias = biased ? P.bias.p + plane * P.bias.item + (in ? key : 0) : nullptr;
+
+  const int64_t q_blocks = (P.nq + kQ - 1) / kQ;
+  DaStage<T, D, kQ, 256> st;
+  const int h0 = kv * P.group;
+  st.init(P.q.p + item * P.q.item + 2 * h0 * P.q.head, P.q.head, P.q.token, P.dout.p + item * P.dout.item + h0 * P.dout.head,
+          P.dout.token, t);
+  const int64_t head_step = st.which < 2 ? 2 * P.q.head : P.dout.head;
+  const T* src0 = st.src;
+  float stat;
+  auto fetch = [&](int hg, int64_t qb) {
+    st.src = src0 + hg * head_step;
+    st.load(qb * kQ, P.nq, nullptr);
+    const int which = t >> 6;
+    const int64_t q = qb * kQ + (t & 63);
+    const int64_t at = (item * 2 * P.heads + 2 * (h0 + hg) + (which & 1)) * P.nq + q;
+    stat = which < 2 ? INFINITY : 0.f;  // past the last query: weights of zero
+    if (q < P.nq) stat = which < 2 ? P.saved[at] : P.delta[at];
+  };
+  T bq[4][4];
+  auto fetch_bias = [&](int hg, int64_t qb) {
+    const T* p = bias + (h0 + hg) * P.bias.head;
+#pragma unroll
+    for (int qt = 0; qt < 4; ++qt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int64_t q = qb * kQ + 16 * qt + 4 * lg + r;
+        bq[qt][r] = p[(q < P.nq ? q : P.nq - 1) * P.bias.token];
+      }
+  };
+
+  f32x4 dk[2][kU], dv[2 * kU];
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int u = 0; u < kU; ++u) dk[m][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int u = 0; u < 2 * kU; ++u) dv[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  fetch(0, 0);
+  if (biased) fetch_bias(0, 0);
+  st.store(tiles[0]);
+  row_stat[0][t >> 6][t & 63] = stat;
+  __syncthreads();
+  int buf = 0;
+  for (int hg = 0; hg < P.group; ++hg) {
+    const float lam = da_lambda<D>(P.lam, P.heads, h0 + hg, P.init, lane);
+    for (int64_t qb = 0; qb < q_blocks; ++qb, buf ^= 1) {
+      const Tile& tile = tiles[buf];
+      const bool same = qb + 1 < q_blocks;
+      const bool more = same || hg + 1 < P.group;
+      float b[4][4];
+#pragma unroll
+      for (int qt = 0; qt < 4; ++qt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) b[qt][r] = biased ? fminf(to_f32(bq[qt][r]) * kLog2e, key_on) : key_on;
+      if (more) {
+        fetch(same ? hg : hg + 1, same ? qb + 1 : 0);
+        if (biased) fetch_bias(same ? hg : hg + 1, same ? qb + 1 : 0);
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float comb[8], ds[2][8];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int qt = 2 * c + j;
+          f32x4 s[2], dp = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            s[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int x = 0; x < kC; ++x) mma(s[m], load8(&tile.a[m][16 * qt + li][32 * x + 8 * lg]), kf[m][x]);
+          }
+#pragma unroll
+          for (int x = 0; x < 2 * kC; ++x) mma(dp, load8(&tile.b[16 * qt + li][32 * x + 8 * lg]), vf[x]);
+          f32x4 rs[4];
+#pragma unroll
+          for (int w = 0; w < 4; ++w) rs[w] = *reinterpret_cast<const f32x4*>(&row_stat[buf][w][16 * qt + 4 * lg]);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float p1 = __builtin_amdgcn_exp2f(fmaf(s[0][r], P.scale_log2, b[qt][r]) - rs[0][r]);
+            const float p2 = lam * __builtin_amdgcn_exp2f(fmaf(s[1][r], P.scale_log2, b[qt][r]) - rs[1][r]);
+            comb[4 * j + r] = p1 - p2;
+            ds[0][4 * j + r] = p1 * (dp[r] - rs[2][r]);
+            ds[1][4 * j + r] = p2 * (rs[3][r] - dp[r]);
+          }
+        }
+        F cf[kParts<T>], df0[kParts<T>], df1[kParts<T>];
+        parts(comb, cf);
+        parts(ds[0], df0);
+        parts(ds[1], df1);
+#pragma unroll
+        for (int u = 0; u < 2 * kU; ++u) mma_parts(dv[u], col_frag(&tile.b[0][0], Tile::kB, 32 * c, 16 * u, lane), cf);
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+          mma_parts(dk[0][u], col_frag(&tile.a[0][0][0], Tile::kA, 32 * c, 16 * u, lane), df0);
+          mma_parts(dk[1][u], col_frag(&tile.a[1][0][0], Tile::kA, 32 * c, 16 * u, lane), df1);
+        }
+      }
+      if (more) {
+        st.store(tiles[buf ^ 1]);
+        row_stat[buf ^ 1][t >> 6][t & 63] = stat;
+      }
+      __syncthreads();
+    }
+  }
+  if (!in) return;
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    T* out = P.dk.p + item * P.dk.item + (2 * kv + m) * P.dk.head + key * P.dk.token;
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      float v[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] = dk[m][u][r] * P.scale;
+      store4f(out + 16 * u + 4 * lg, v);
+    }
+  }
+  T* out = P.dv.p + item * P.dv.item + kv * P.dv.head + key * P.dv.token;
+#pragma unroll
+  for (int u = 0; u < 2 * kU; ++u) {
+    float v[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = dv[u][r];
+    store4f(out + 16 * u + 4 * lg, v);
+  }
+}
+
+// dbias of a plane that several items share (the rows of a triangle attention):
+// a workgroup owns 64 queries x 64 keys of one head and adds dS over the items
+// of its chunk in registers; the chunks' sums are added by diffattn_bias_sum.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void diffattn_dbias_kernel(DiffAttnParams<T> P) {
+  constexpr int kC = D / 32;
+  typedef typename Frag<T>::type F;
+  typedef DaTile<T, D, kDaKeys> Tile;
+  __shared__ __attribute__((aligned(16))) Tile tiles[2];
+  __shared__ __attribute__((aligned(16))) float key_on[2][kDaKeys];
+
+  const int t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int64_t planes = P.items / P.share;
+  const int64_t kbs = (P.nk + 63) / 64, qbs = (P.nq + 63) / 64;
+  int64_t id = xcd_order(blockIdx.x, gridDim.x);
+  if (id >= planes * P.heads * kbs * qbs * P.chunks) return;
+  const int64_t kb = id % kbs;
+  id /= kbs;
+  const int64_t qb = id % qbs;
+  id /= qbs;
+  const int head = (int)(id % P.heads);
+  id /= P.heads;
+  const int chunk = (int)(id % P.chunks);
+  const int64_t plane = id / P.chunks;
+  const int kv = head / P.group;
+  const int64_t qi = qb * 64 + 16 * wave + li;
+  const int64_t qc = qi < P.nq ? qi : P.nq - 1;
+  const int64_t i0 = plane * P.share + chunk * P.chunk_items;
+  const int64_t i1 = i0 + P.chunk_items < (plane + 1) * P.share ? i0 + P.chunk_items : (plane + 1) * P.share;
+
+  const float lam = da_lambda<D>(P.lam, P.heads, head, P.init, lane);
+  f32x4 raw_b[4];
+  bias_tile(P.bias.p + plane * P.bias.item + head * P.bias.head + qc * P.bias.token, kb * 64 + 4 * lg, P.nk,
+            (kb + 1) * 64 <= P.nk, raw_b);
+#pragma unroll
+  for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) raw_b[kt][r] *= kLog2e;
+
+  DaStage<T, D, kDaKeys, 256> st;
+  st.init(P.k.p + i0 * P.k.item + 2 * kv * P.k.head, P.k.head, P.k.token, P.v.p + i0 * P.v.item + kv * P.v.head,
+          P.v.token, t);
+  const int64_t item_step = st.which < 2 ? P.k.item : P.v.item;
+  F qf[2][kC], dof[2 * kC], qn[2][kC], don[2 * kC];
+  float rs[4], rn[4];
+  auto fetch = [&](int64_t item) {
+    st.load(kb * 64, P.nk, P.mask ? P.mask + item * P.nk : nullptr);
+    st.src += item_step;
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      const int64_t at = (item * 2 * P.heads + 2 * head + m) * P.nq + qc;
+      rn[m] = P.saved[at];
+      rn[2 + m] = P.delta[at];
+#pragma unroll
+      for (int c = 0; c < kC; ++c)
+        qn[m][c] = load8(P.q.p + item * P.q.item + (2 * head + m) * P.q.head + qc * P.q.token + 32 * c + 8 * lg);
+    }
+#pragma unroll
+    for (int c = 0; c < 2 * kC; ++c)
+      don[c] = load8(P.dout.p + item * P.dout.item + head * P.dout.head + qc * P.dout.token + 32 * c + 8 * lg);
+  };
+  auto key_flags = [&](int64_t item, int buf) {
+    if (t < kDaKeys) {
+      const int64_t k = kb * 64 + t;
+      key_on[buf][t] = k < P.nk && (!P.mask || P.mask[item * P.nk + k]) ? INFINITY : -INFINITY;
+    }
+  };
+  f32x4 acc[4];
+#pragma unroll
+  for (int kt = 0; kt < 4; ++kt) acc[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  fetch(i0);
+  st.store(tiles[0]);
+  key_flags(i0, 0);
+  __syncthreads();
+  int buf = 0;
+  for (int64_t item = i0; item < i1; ++item, buf ^= 1) {
+    const Tile& tile = tiles[buf];
+    const bool more = item + 1 < i1;
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int c = 0; c < kC; ++c) qf[m][c] = qn[m][c];
+#pragma unroll
+    for (int c = 0; c < 2 * kC; ++c) dof[c] = don[c];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) rs[w] = rn[w];
+    f32x4 b[4];
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt) {
+      b[kt] = *reinterpret_cast<const f32x4*>(&key_on[buf][16 * kt + 4 * lg]);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) b[kt][r] = fminf(raw_b[kt][r], b[kt][r]);
+    }
+    if (more) fetch(item + 1);
+    f32x4 dp[4];
+    tile_dp<T, D>(tile, dof, li, lg, dp);
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      f32x4 p[4];
+      tile_weights<T, D>(tile, m, qf[m], b, P.scale_log2, rs[m], li, lg, p);
+      const float by = m ? -lam : 1.f;
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[kt][r] = fmaf(p[kt][r] * by, dp[kt][r] - rs[2 + m], acc[kt][r]);
+    }
+    if (more) {
+      st.store(tiles[buf ^ 1]);
+      key_flags(item + 1, buf ^ 1);
+    }
+    __syncthreads();
+  }
+  if (qi >= P.nq) return;
+  float* out = P.part_bias + (((int64_t)chunk * planes + plane) * P.heads + head) * P.nq * P.nk + qi * P.nk;
+  const int64_t k0 = kb * 64 + 4 * lg;
+#pragma unroll
+  for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (k0 + 16 * kt + r < P.nk) out[k0 + 16 * kt + r] = acc[kt][r];
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void diffattn_bias_sum_kernel(DiffAttnParams<T> P) {
+  const int64_t per = P.items / P.share * P.heads * P.nq * P.nk;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < per; i += gridDim.x * 256ll) {
+    float s = 0.f;
+    for (int c = 0; c < P.chunks; ++c) s += P.part_bias[c * per + i];
+    const int64_t k = i % P.nk, q = i / P.nk % P.nq, ph = i / (P.nk * P.nq);
+    P.dbias.p[ph / P.heads * P.dbias.item + ph % P.heads * P.dbias.head + q * P.dbias.token + k] = from_f32<T>(s);
+  }
+}
+
+// dlambda_h = -sum over items and queries of D_2, and the four vectors'
+// gradients from it: one workgroup a head
+template <typename T, int D>
+__global__ __launch_bounds__(1024) void diffattn_dlam_kernel(DiffAttnParams<T> P) {
+  __shared__ float part[16];
+  const int t = threadIdx.x, head = blockIdx.x;
+  const int64_t n = P.items * P.nq;
+  float s = 0.f;
+  for (int64_t i = t; i < n; i += 1024) {
+    const int64_t item = i / P.nq;
+    s += P.delta[(item * 2 * P.heads + 2 * head + 1) * P.nq + i - item * P.nq];
+  }
+#pragma unroll
+  for (int x = 32; x >= 1; x >>= 1) s += shfl_xor(s, x);
+  if ((t & 63) == 0) part[t >> 6] = s;
+  __syncthreads();
+  if (t >= 64) return;
+  float dl = 0.f;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) dl -= part[w];
+  float e[2];
+  da_lambda<D>(P.lam, P.heads, head, P.init, t, e);
+  if (t < D) {
+    const int64_t st = (int64_t)P.heads * D, at = (int64_t)head * D + t;
+    const float g[2] = {dl * e[0], -dl * e[1]};
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      P.dlam[2 * m * st + at] = g[m] * P.lam[(2 * m + 1) * st + at];
+      P.dlam[(2 * m + 1) * st + at] = g[m] * P.lam[2 * m * st + at];
+    }
+  }
+}
+
+unsigned eights(int64_t blocks) { return (unsigned)((blocks + 7) / 8 * 8); }
+
+template <typename T, int D>
+void bwd(const DiffAttnParams<T>& P, hipStream_t st) {
+  const int64_t kvh = P.heads / P.group;
+  diffattn_dq_kernel<T, D><<<eights(P.items * kvh * ((P.group * P.nq + 63) / 64)), 256, 0, st>>>(P);
+  diffattn_dkv_kernel<T, D><<<eights(P.items * kvh * ((P.nk + 63) / 64)), 256, 0, st>>>(P);
+  if (P.dbias.p && P.share > 1) {
+    const int64_t planes = P.items / P.share;
+    diffattn_dbias_kernel<T, D><<<eights(planes * P.heads * P.chunks * ((P.nk + 63) / 64) * ((P.nq + 63) / 64)), 256, 0, st>>>(P);
+    const int64_t blocks = (planes * P.heads * P.nq * P.nk + 255) / 256;
+    diffattn_bias_sum_kernel<T><<<(unsigned)(blocks < 8192 ? blocks : 8192), 256, 0, st>>>(P);
+  }
+  diffattn_dlam_kernel<T, D><<<P.heads, 1024, 0, st>>>(P);
+}
+
+}  // namespace
+
+template <typename T>
+void launch_diffattn_bwd(const DiffAttnParams<T>& P, int d, hipStream_t st) {
+  if (d == 32)
+    bwd<T, 32>(P, st);
+  else
+    bwd<T, 64>(P, st);
+}
+template void launch_diffattn_bwd<bf16>(const DiffAttnParams<bf16>&, int, hipStream_t);
+template void launch_diffattn_bwd<float>(const DiffAttnParams<float>&, int, hipStream_t);
+
+}  // namespace fjx

@@ -1,0 +1,97 @@
+// Dropout from a counter-based generator, with the residual's addition; the
+// mask is never stored. Element i of the mask is kept where word i % 4 of
+// Philox 4x32-10 (Salmon, Moraes, Dror and Shaw, "Parallel random numbers: as
+// easy as 1, 2, 3", SC 2011) of the counter (i / 4, offset) under the key
+// `seed` is at least p 2^32.
+//
+// x is [B][I][J][C] and its mask may have one entry for all of I, J and C: a
+// thread draws the words of 8 channels once and uses them along the shared
+// positions, its "run".
+#include "fjx_common.hpp"
+#include "fjx_kernels.hpp"
+
+namespace fjx {
+
+namespace {
+
+struct Words {
+  uint32_t w[4];
+};
+__device__ __forceinline__ Words philox(uint64_t index, uint64_t offset, uint64_t seed) {
+  uint32_t c0 = (uint32_t)index, c1 = (uint32_t)(index >> 32), c2 = (uint32_t)offset, c3 = (uint32_t)(offset >> 32);
+  uint32_t k0 = (uint32_t)seed, k1 = (uint32_t)(seed >> 32);
+#pragma unroll
+  for (int r = 0; r < 10; ++r) {
+    const uint64_t a = (uint64_t)c0 * 0xD2511F53u, b = (uint64_t)c2 * 0xCD9E8D57u;
+    c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
+    c1 = (uint32_t)b;
+    c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+    c3 = (uint32_t)a;
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  return {{c0, c1, c2, c3}};
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void dropout_kernel(DropoutParams<T> P) {
+  const int64_t pieces = P.c / 8;
+  const int64_t id = (P.first + blockIdx.x) * 256 + threadIdx.x;
+  const int64_t per = P.frees * pieces;  // threads of one part of the runs
+  const int64_t part = id / per;
+  if (part >= P.parts) return;
+  const int64_t fp = id - part * per;
+  const int64_t f = fp / pieces;
+  const int ch = (int)(fp - f * pieces) * 8;
+  uint64_t offset = P.offset;
+  if (P.step) offset += *P.step;
+  uint32_t keep = 0;  // bit e: channel ch + e
+  if (P.by_channel) {
+    const uint64_t i = (uint64_t)f * P.c + ch;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const Words w = philox(i / 4 + j, offset, P.seed);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) keep |= (uint32_t)(w.w[e] >= P.threshold) << (4 * j + e);
+    }
+  } else {
+    const Words w = philox((uint64_t)f / 4, offset, P.seed);
+    const uint32_t lo = f & 1 ? w.w[1] : w.w[0], hi = f & 1 ? w.w[3] : w.w[2];
+    keep = (f & 2 ? hi : lo) >= P.threshold ? 0xffu : 0u;
+  }
+  // the first position of the run: free positions are (b, i, j) without the shared ones
+  int64_t pos = f * P.run;
+  if (P.share_i && !P.share_j) pos = f / P.j * P.run * P.j + f % P.j;
+  const int64_t step = P.share_i && !P.share_j ? P.j : 1;
+  const int64_t r1 = (part + 1) * P.run_part < P.run ? (part + 1) * P.run_part : P.run;
+#pragma unroll 4
+  for (int64_t r = part * P.run_part; r < r1; ++r) {
+    const int64_t p = pos + r * step;
+    const int64_t at = p * P.c + ch;
+    float x[8], o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    to_f32x8(load8(P.x + at), x);
+    if (P.residual) to_f32x8(load8(P.residual + at), o);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = keep >> e & 1 ? fmaf(x[e], P.scale, o[e]) : o[e];
+    if (P.out_mask && to_f32(P.out_mask[p]) == 0.f) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] = 0.f;
+    }
+    store8(P.out + at, pack8<T>(o));
+  }
+}
+
+}  // namespace
+
+template <typename T>
+void launch_dropout(const DropoutParams<T>& p, hipStream_t st) {
+  for_pieces((p.parts * p.frees * (p.c / 8) + 255) / 256, [&](int64_t first, unsigned blocks) {
+    DropoutParams<T> q = p;
+    q.first = first;
+    dropout_kernel<T><<<blocks, 256, 0, st>>>(q);
+  });
+}
+template void launch_dropout<bf16>(const DropoutParams<bf16>&, hipStream_t);
+template void launch_dropout<float>(const DropoutParams<float>&, hipStream_t);
+
+}  // namespace fjx

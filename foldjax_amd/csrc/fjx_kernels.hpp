@@ -279,6 +279,69 @@ void launch_flash_pipe(const FlashParams<bf16>& p, int64_t groups, int queries, 
 int probe_issue_mix(int mix, int waves_per_simd, int iters, float* ms, hipStream_t st);
 int probe_hbm_stream(int mode, int wgs_per_cu, int64_t bytes, float* ms, hipStream_t st);
 
+// RMS norm (fjx_rmsnorm.hip): c a multiple of 8 up to 8192
+template <typename T>
+struct RmsNormParams {
+  const T* x;         // [rows][c]
+  const T* residual;  // added to x, or null
+  const T* w;         // [c]
+  T* h;               // x + residual, or null (may be x or the residual)
+  T* y;               // the norm, or null with codes
+  void* codes;        // [rows][c] e4m3 or int8
+  float* scales;      // [rows][c / group]
+  int64_t rows;
+  int64_t first;      // block of this launch
+  int c, group;       // group: channels of one scale (32, 64 or 128, or c)
+  float eps;
+};
+template <typename T>
+struct RmsNormBwdParams {
+  const T* dy;
+  const T* h;
+  const T* w;
+  const T* dh;  // the sum's own gradient, or null
+  T* dx;        // may be dy or dh
+  float* part;  // [rmsnorm_bwd_blocks(rows, c)][c]
+  int64_t rows;
+  int c;
+  float eps;
+};
+// codes: 0 none, 1 e4m3, 2 int8
+template <typename T>
+void launch_rmsnorm(const RmsNormParams<T>& p, int codes, hipStream_t st);
+int rmsnorm_bwd_blocks(int64_t rows, int c);
+template <typename T>
+void launch_rmsnorm_bwd(const RmsNormBwdParams<T>& p, float* dw, hipStream_t st);
+
+// dropout (fjx_dropout.hip): `frees` mask positions in (b, i, j) order, each for
+// `run` positions of x (those along the shared axes), `run_part` of them a thread
+template <typename T>
+struct DropoutParams {
+  const T* x;         // [B][I][J][C], C a multiple of 8
+  const T* residual;  // or null
+  const T* out_mask;  // [B][I][J] or null
+  T* out;             // may be x or the residual
+  int64_t j, frees, run, run_part, parts;
+  int64_t first;      // block of this launch
+  int c;
+  bool share_i, share_j, by_channel;
+  uint32_t threshold;
+  float scale;
+  uint64_t seed, offset;
+  const uint64_t* step;  // added to the offset, or null
+};
+template <typename T>
+void launch_dropout(const DropoutParams<T>& p, hipStream_t st);
+
+// differential attention (fjx_diffattn.hip, fjx_diffattn_bwd.hip); the
+// parameters are in fjx_diffattn.hpp
+template <typename T>
+struct DiffAttnParams;
+template <typename T>
+void launch_diffattn_fwd(const DiffAttnParams<T>& P, int d, bool keywise, hipStream_t st);
+template <typename T>
+void launch_diffattn_bwd(const DiffAttnParams<T>& P, int d, hipStream_t st);
+
 // general-width paths (fjx_generic.hip); positions v = r*n + s of the virtual
 // grid read the original grid at s*n + r when t = 1
 template <typename T>

@@ -634,6 +634,393 @@ def triattn_core(
     return out.reshape(tuple(lead) + (rows, heads, n, d))
 
 
+def _launch(entry, args, x: torch.Tensor) -> None:
+    """``entry`` on the current stream of ``x``'s device, whichever device is
+    the current one."""
+    if torch.cuda.current_device() == x.get_device():
+        _lib.check(entry(ctypes.byref(args), _stream(x)))
+    else:
+        with torch.cuda.device(x.get_device()):
+            _lib.check(entry(ctypes.byref(args), _stream(x)))
+
+
+def _workspace(nbytes: int, x: torch.Tensor) -> torch.Tensor | None:
+    return torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+
+
+def _need_dtype(dtype: torch.dtype, **operands) -> None:
+    for name, t in operands.items():
+        if t is not None and t.dtype is not dtype:
+            raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+
+
+def _rows_ok(t: torch.Tensor) -> bool:
+    """Whether the kernels' 16-byte accesses can take ``t``'s rows as they lie."""
+    es = t.element_size()
+    return (t.stride(-1) == 1 and t.data_ptr() % 16 == 0
+            and all(n == 1 or (s > 0 and s * es % 16 == 0) for n, s in zip(t.shape[:-1], t.stride()[:-1])))
+
+
+def _items(t: torch.Tensor, tail: int) -> torch.Tensor:
+    """The axes before the last ``tail`` folded into one."""
+    return t if t.dim() == tail + 1 else t.reshape((-1,) + tuple(t.shape[t.dim() - tail:]))
+
+
+def _heads(t: torch.Tensor) -> torch.Tensor:
+    """[..., heads, tokens, width] as [items, heads, tokens, width] with rows
+    the kernels can take: a view wherever the strides allow one."""
+    t = _items(t, 3)
+    return t if _rows_ok(t) else t.clone(memory_format=torch.contiguous_format)
+
+
+def _strides3(t: torch.Tensor):
+    """Strides of the first three axes; an axis of one element has none."""
+    return _lib._i64x3(*(0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride()[:3])))
+
+
+def _diff_attention_args(q, k, v, lambda_vectors, lambda_init, scale, bias, mask):
+    """The checked argument block that both directions share, and the tensors
+    it points to (q, k, v and bias as [items or planes, heads, tokens, ...])."""
+    _same_device(q, k=k, v=v, lambda_vectors=lambda_vectors, bias=bias, mask=mask)
+    code = _code(q.dtype)
+    _need_dtype(q.dtype, k=k, v=v, bias=bias)
+    _need_dtype(torch.float32, lambda_vectors=lambda_vectors)
+    if q.dim() < 3 or k.dim() != q.dim() or v.dim() != q.dim():
+        raise ValueError(f"q, k and v must be [..., heads, tokens, width] of as many axes, got {tuple(q.shape)}, "
+                         f"{tuple(k.shape)}, {tuple(v.shape)}")
+    lead = tuple(q.shape[:-3])
+    h2, nq, d = (int(n) for n in q.shape[-3:])
+    hk2, nk = int(k.shape[-3]), int(k.shape[-2])
+    if h2 % 2 or hk2 % 2:
+        raise ValueError(f"q and k hold two maps a head: an even number of heads, got {h2} and {hk2}")
+    heads, kv_heads = h2 // 2, hk2 // 2
+    _need_shape("k", k, lead + (hk2, nk, d))
+    _need_shape("v", v, lead + (kv_heads, nk, 2 * d))
+    _need_shape("lambda_vectors", lambda_vectors, (4, heads, d))
+    q4, k4, v4 = _heads(q), _heads(k), _heads(v)
+    items = int(q4.shape[0])
+    lam = lambda_vectors.contiguous()
+    b4, share = None, 1
+    if bias is not None:
+        if bias.dim() < 3 or bias.dim() > q.dim() or tuple(bias.shape[-3:]) != (heads, nq, nk):
+            raise ValueError(f"bias must be [..., {heads}, {nq}, {nk}], got {tuple(bias.shape)}")
+        # planes for the leading items, then axes that share one
+        planes = (1,) * (len(lead) - bias.dim() + 3) + tuple(int(n) for n in bias.shape[:-3])
+        axis = len(lead)
+        while axis and planes[axis - 1] == 1:
+            axis -= 1
+            share *= lead[axis]
+        if planes[:axis] != lead[:axis]:
+            raise ValueError(f"bias must have one plane for each of q's leading axes {lead}, or share one over the last "
+                             f"of them, got {tuple(bias.shape[:-3])}")
+        b4 = _items(bias, 3)
+        if b4.stride(-1) != 1 and nk > 1 or min(b4.stride()) < 0:
+            b4 = b4.contiguous()
+    m2 = None
+    if mask is not None:
+        try:
+            m2 = torch.broadcast_to(mask, lead + (nk,))
+        except RuntimeError:
+            raise ValueError(f"mask of shape {tuple(mask.shape)} does not broadcast to {lead + (nk,)}") from None
+        m2 = (m2 if m2.dtype is torch.bool else m2.ne(0)).contiguous()
+    _dev(q)
+    a = _lib.DiffAttentionArgs(
+        items=items, heads=heads, kv_heads=kv_heads, nq=nq, nk=nk, head_dim=d, bias_share=share, dtype=code,
+        scale=float(scale), lambda_init=float(lambda_init), q=_ptr(q4), k=_ptr(k4), v=_ptr(v4),
+        q_strides=_strides3(q4), k_strides=_strides3(k4), v_strides=_strides3(v4),
+        bias=_ptr(b4), mask=_ptr(m2), lambda_vectors=_ptr(lam),
+    )
+    if b4 is not None:
+        a.bias_strides = _strides3(b4)
+    return a, (q4, k4, v4, b4, m2, lam), lead
+
+
+def diff_attention(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    lambda_vectors: torch.Tensor,
+    *,
+    lambda_init: float,
+    scale: float,
+    bias: torch.Tensor | None = None,
+    mask: torch.Tensor | None = None,
+    return_lse: bool = False,
+    out: torch.Tensor | None = None,
+):
+    """Differential attention (``fjx_diff_attention_fwd``): per head
+    ``(softmax(scale q_1 k_1^T + bias) - lambda softmax(scale q_2 k_2^T + bias)) v``
+    with ``lambda = exp(a_1 . b_1) - exp(a_2 . b_2) + lambda_init``.
+
+    q ``[..., 2 H, Q, D]`` and k ``[..., 2 Hk, K, D]``, heads 2 h and 2 h + 1
+    being the two maps of head h; v ``[..., Hk, K, 2 D]`` (Hk divides H: heads
+    may share keys and values); D 32 or 64. Any strides whose rows are whole
+    16-byte pieces are taken as they lie, others are copied.
+    ``lambda_vectors`` float32 ``[4, H, D]``: a_1, b_1, a_2, b_2. ``bias``
+    ``[..., H, Q, K]`` in q's dtype: a plane per leading index of q, or shared
+    over the last leading axes (1, or left out): ``[B, 1, H, J, J]`` for the
+    rows of a triangle attention. ``mask`` broadcasts to ``[..., K]``: 0 takes
+    a key out, whatever it holds. A bias of -inf, or of the dtype's lowest
+    value, takes a key out for one query (k and v finite there). A row without
+    keys is zeros.
+
+    Returns ``out`` ``[..., H, Q, 2 D]``; with ``return_lse`` also what
+    ``diff_attention_backward`` needs to know of the rows. ``out``: write into
+    this tensor (its rows whole 16-byte pieces, any order of the other axes)."""
+    a, (q4, *kept), lead = _diff_attention_args(q, k, v, lambda_vectors, lambda_init, scale, bias, mask)
+    shape = lead + (a.heads, a.nq, 2 * a.head_dim)
+    if out is None:
+        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+    else:
+        if out.shape != shape or out.dtype != q.dtype or out.device != q.device:
+            raise ValueError(f"out must be a {q.dtype} tensor of shape {shape} on {q.device}, "
+                             f"got {out.dtype} {tuple(out.shape)} on {out.device}")
+    o4 = out
+    if out.dim() != 4:
+        try:
+            o4 = out.view((a.items,) + shape[-3:])
+        except RuntimeError:
+            raise ValueError("out's leading axes must fold into one") from None
+    if not _rows_ok(o4):
+        raise ValueError("out must have rows of whole 16-byte pieces")
+    a.out, a.out_strides = _ptr(o4), _strides3(o4)
+    lse = None
+    if return_lse:
+        lse = torch.empty(lead + (2 * a.heads, a.nq), dtype=torch.float32, device=q.device)
+        a.stats = _ptr(lse)
+    lib = _lib.load()
+    nbytes = lib.fjx_diff_attention_workspace_size(a.items, a.heads, a.kv_heads, a.nq, a.nk, a.head_dim, a.dtype)
+    ws = _workspace(nbytes, q)
+    a.workspace, a.workspace_bytes = _ptr(ws), nbytes
+    _launch(lib.fjx_diff_attention_fwd, a, q)
+    return (out, lse) if return_lse else out
+
+
+def diff_attention_backward(
+    dout: torch.Tensor,
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    lambda_vectors: torch.Tensor,
+    lse: torch.Tensor,
+    *,
+    lambda_init: float,
+    scale: float,
+    bias: torch.Tensor | None = None,
+    mask: torch.Tensor | None = None,
+    bias_grad: bool = True,
+):
+    """Gradients of ``diff_attention`` (``fjx_diff_attention_bwd``) at the same
+    arguments, ``lse`` being what the forward call returned. Returns ``(dq, dk,
+    dv, dbias, dlambda)``: dq, dk, dv and dbias in the dtype and shape of q, k,
+    v and bias (dbias None without a bias or with ``bias_grad`` off; of a shared
+    plane the sum over the items, of shared heads' k and v the sum over the
+    query heads), dlambda float32 ``[4, H, D]``. The same bits each time."""
+    f, (q4, k4, v4, b4, *kept), lead = _diff_attention_args(q, k, v, lambda_vectors, lambda_init, scale, bias, mask)
+    _same_device(q, dout=dout, lse=lse)
+    _need_dtype(q.dtype, dout=dout)
+    _need_dtype(torch.float32, lse=lse)
+    _need_shape("dout", dout, lead + (f.heads, f.nq, 2 * f.head_dim))
+    _need_shape("lse", lse, lead + (2 * f.heads, f.nq))
+    do4 = _heads(dout)
+    lse = lse.contiguous()
+    f.out_strides, f.stats = _strides3(do4), _ptr(lse)
+    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    dlam = torch.empty_like(lambda_vectors, memory_format=torch.contiguous_format)
+    g = _lib.DiffAttentionBwdArgs(dout=_ptr(do4), dq=_ptr(dq), dk=_ptr(dk), dv=_ptr(dv), dlambda=_ptr(dlam))
+    g.dq_strides, g.dk_strides, g.dv_strides = (_strides3(_items(t, 3)) for t in (dq, dk, dv))
+    dbias = None
+    if bias is not None and bias_grad:
+        dbias = torch.empty(bias.shape, dtype=bias.dtype, device=bias.device)
+        g.dbias, g.dbias_strides = _ptr(dbias), _strides3(_items(dbias, 3))
+    lib = _lib.load()
+    nbytes = lib.fjx_diff_attention_bwd_workspace_size(f.items, f.heads, f.nq, f.nk, f.bias_share, dbias is not None)
+    ws = _workspace(nbytes, q)
+    f.workspace, f.workspace_bytes = _ptr(ws), nbytes
+    g.fwd = f
+    _launch(lib.fjx_diff_attention_bwd, g, q)
+    return dq, dk, dv, dbias, dlam
+
+
+_CODES = {None: (_lib.FJX_CODES_NONE, None), "e4m3": (_lib.FJX_CODES_E4M3, torch.float8_e4m3fn),
+          "int8": (_lib.FJX_CODES_INT8, torch.int8)}
+
+
+def rms_norm(
+    x: torch.Tensor,
+    weight: torch.Tensor,
+    *,
+    residual: torch.Tensor | None = None,
+    eps: float = 1e-6,
+    codes: str | None = None,
+    group: int = 0,
+    out: torch.Tensor | None = None,
+    sum_out: torch.Tensor | None = None,
+):
+    """Root-mean-square norm over the last axis (``fjx_rms_norm_fwd``):
+    ``h / sqrt(mean(h^2) + eps) * weight`` with ``h = x + residual``.
+
+    Returns ``y``, or ``(y, h)`` with a residual (h rounded to x's dtype, y of
+    the unrounded sum). ``codes`` ``"e4m3"`` or ``"int8"``: y in 8 bits with a
+    float32 scale a row, or every ``group`` channels (32, 64 or 128), and
+    ``(codes, scales)`` in y's place: ``(codes, scales)`` or ``(codes, scales,
+    h)``; ``y ~ codes * scale``, scales ``[..., 1]`` or ``[..., C / group]``.
+    ``out`` (without codes) and ``sum_out``: write y and h into these tensors
+    (x's shape and dtype, contiguous); each may be ``x`` or ``residual``."""
+    kind = _CODES.get(codes) if codes is None or isinstance(codes, str) else None
+    if kind is None:
+        raise ValueError(f"codes must be None, 'e4m3' or 'int8', got {codes!r}")
+    _same_device(x, weight=weight, residual=residual, out=out, sum_out=sum_out)
+    code = _code(x.dtype)
+    _need_dtype(x.dtype, weight=weight, residual=residual)
+    if x.dim() < 1:
+        raise ValueError("x must have a last axis to be normalised over")
+    c = int(x.shape[-1])
+    _need_shape("weight", weight, (c,))
+    if residual is not None:
+        _need_shape("residual", residual, x.shape)
+    elif sum_out is not None:
+        raise ValueError("sum_out needs a residual")
+    if group and codes is None:
+        raise ValueError("group needs codes")
+    _dev(x)
+    xf, res = x.contiguous(), None if residual is None else residual.contiguous()
+    scales = None
+    if codes is None:
+        y = _out_buffer(out, x, xf)
+    else:
+        if out is not None:
+            raise ValueError("out is for a norm without codes")
+        if group < 0 or (group and c % group):
+            raise ValueError(f"group must divide the {c} channels, got {group}")
+        y = torch.empty(x.shape, dtype=kind[1], device=x.device)
+        scales = torch.empty(tuple(x.shape[:-1]) + (c // group if group else 1,), dtype=torch.float32, device=x.device)
+    h = None if res is None else _out_buffer(sum_out, x, xf)
+    if h is not None and h.data_ptr() == y.data_ptr():
+        raise ValueError("out and sum_out must be two buffers")
+    w = weight.contiguous()
+    a = _lib.RmsNormArgs(rows=x.numel() // max(c, 1), c=c, dtype=code, eps=float(eps), x=_ptr(xf), residual=_ptr(res),
+                         weight=_ptr(w), sum_out=_ptr(h), out=_ptr(y), codes=kind[0], group=group, scales=_ptr(scales))
+    _launch(_lib.load().fjx_rms_norm_fwd, a, x)
+    got = (y,) if scales is None else (y, scales)
+    got = got if h is None else got + (h,)
+    return got if len(got) > 1 else y
+
+
+def rms_norm_backward(
+    dy: torch.Tensor,
+    h: torch.Tensor,
+    weight: torch.Tensor,
+    *,
+    dh: torch.Tensor | None = None,
+    eps: float = 1e-6,
+    out: torch.Tensor | None = None,
+):
+    """Gradients of ``rms_norm`` at the sum ``h`` it returned (x itself without
+    a residual): ``(dx, dweight)`` (``fjx_rms_norm_bwd``). dx is the residual's
+    gradient too and includes ``dh``, what reaches h from elsewhere; dweight is
+    float32, summed over the rows in one order. ``out``: write dx into this
+    tensor, which may be ``dy`` or ``dh``."""
+    _same_device(h, dy=dy, weight=weight, dh=dh, out=out)
+    code = _code(h.dtype)
+    _need_dtype(h.dtype, dy=dy, weight=weight, dh=dh)
+    if h.dim() < 1:
+        raise ValueError("h must have a last axis")
+    c = int(h.shape[-1])
+    _need_shape("weight", weight, (c,))
+    _need_shape("dy", dy, h.shape)
+    _need_shape("dh", dh, h.shape)
+    _dev(h)
+    hf, dyf = h.contiguous(), dy.contiguous()
+    dhf = None if dh is None else dh.contiguous()
+    w = weight.contiguous()
+    if out is not None and out.data_ptr() == h.data_ptr():
+        raise ValueError("out must not be h")
+    dx = _out_buffer(out, h, hf)
+    dw = torch.empty((c,), dtype=torch.float32, device=h.device)
+    lib = _lib.load()
+    rows = h.numel() // max(c, 1)
+    nbytes = lib.fjx_rms_norm_bwd_workspace_size(rows, c)
+    ws = _workspace(nbytes, h)
+    a = _lib.RmsNormBwdArgs(rows=rows, c=c, dtype=code, eps=float(eps), dy=_ptr(dyf), h=_ptr(hf), weight=_ptr(w),
+                            dh=_ptr(dhf), dx=_ptr(dx), dweight=_ptr(dw), workspace=_ptr(ws), workspace_bytes=nbytes)
+    _launch(lib.fjx_rms_norm_bwd, a, h)
+    return dx, dw
+
+
+_SHARE = {-3: _lib.FJX_SHARE_N, -2: _lib.FJX_SHARE_M, -1: _lib.FJX_SHARE_C}
+
+
+def dropout_add(
+    x: torch.Tensor,
+    *,
+    p: float,
+    seed: int,
+    offset: int = 0,
+    step: torch.Tensor | None = None,
+    residual: torch.Tensor | None = None,
+    shared: tuple[int, ...] = (),
+    out_mask: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """``residual + (kept ? x / (1 - p) : 0)``, times ``out_mask != 0`` per
+    position when that is given (``fjx_dropout_fwd``); without a residual the
+    dropped x alone. The last axis a multiple of 8.
+
+    The mask is drawn anew in every call that needs it and never stored: the
+    same ``seed`` (64 bits), ``offset`` (64 bits; one for each use of dropout)
+    and shape give the same one. ``shared``: the axes (-3, -2, -1) over which
+    one mask entry serves, as the Pairformer drops an update for all rows
+    (``(-3,)``) or for all columns (``(-2,)``). ``step``: an int64 tensor of
+    one element on x's device, read by the kernel and added to ``offset``: a
+    captured call then drops anew at each replay. ``out``: write into this
+    tensor, which may be ``x`` and/or ``residual``."""
+    _same_device(x, residual=residual, out_mask=out_mask, step=step, out=out)
+    code = _code(x.dtype)
+    _need_dtype(x.dtype, residual=residual)
+    if x.dim() < 1:
+        raise ValueError("x must have a last axis")
+    flags = 0
+    for axis in shared:
+        if axis not in _SHARE or x.dim() < -axis:
+            raise ValueError(f"shared must name axes of x among -3, -2 and -1, got {shared!r} for {tuple(x.shape)}")
+        flags |= _SHARE[axis]
+    if residual is not None:
+        _need_shape("residual", residual, x.shape)
+    for name, n in (("seed", seed), ("offset", offset)):
+        if not 0 <= n < 2**64:
+            raise ValueError(f"{name} must be in [0, 2^64), got {n}")
+    if step is not None and (step.dtype is not torch.int64 or step.numel() != 1):
+        raise ValueError(f"step must be an int64 tensor of one element, got {step.dtype} {tuple(step.shape)}")
+    _dev(x)
+    xf, res = x.contiguous(), None if residual is None else residual.contiguous()
+    om = _rows_of(out_mask, x.shape[:-1], x.dtype, "out_mask")
+    out = _out_buffer(out, x, xf)
+    n, m, c = (1, 1, *(int(v) for v in x.shape))[-3:]
+    a = _lib.DropoutArgs(batch=x.numel() // max(n * m * c, 1), n=n, m=m, c=c, dtype=code, shared=flags, p=float(p),
+                         seed=seed, offset=offset, step=_ptr(step), x=_ptr(xf), residual=_ptr(res), out_mask=_ptr(om),
+                         out=_ptr(out))
+    _launch(_lib.load().fjx_dropout_fwd, a, x)
+    return out
+
+
+def dropout_backward(
+    dout: torch.Tensor,
+    *,
+    p: float,
+    seed: int,
+    offset: int = 0,
+    step: torch.Tensor | None = None,
+    shared: tuple[int, ...] = (),
+    out_mask: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """The gradient of ``dropout_add``'s x: the same mask, drawn again, on the
+    output's gradient (the residual's gradient is ``dout`` itself, times
+    ``out_mask != 0``). ``step`` must hold what it held in the forward call."""
+    return dropout_add(dout, p=p, seed=seed, offset=offset, step=step, shared=shared, out_mask=out_mask, out=out)
+
+
 def _check_weights(x: torch.Tensor, w) -> None:
     """Every weight contiguous, in ``x``'s dtype and on its (cuda) device."""
     dtype, dev = x.dtype, x.get_device()

@@ -49,7 +49,7 @@
 extern "C" {
 #endif
 
-#define FJX_ABI_VERSION 6
+#define FJX_ABI_VERSION 7
 
 /* element types of activations, masks and weights */
 enum { FJX_DTYPE_F32 = 0, FJX_DTYPE_BF16 = 1 };
@@ -351,6 +351,173 @@ typedef struct fjx_single_attention_args {
 
 size_t fjx_single_attention_workspace_size(int64_t batch, int64_t n, int64_t c_s, int64_t heads, int32_t dtype);
 int fjx_single_attention_fwd(const fjx_single_attention_args* args, hipStream_t stream);
+
+/*
+ * Differential attention: the difference of two softmax maps over one set of
+ * values, the second weighted by a learned lambda per head. Beside
+ * fjx_triattn_core, with its pair bias; no counterpart in the reference.
+ *   x_t    = scale q_t k_t^T + bias          (t = 1, 2; the bias is the same for both)
+ *   P_t    = softmax of x_t over the keys that take part
+ *   out    = (P_1 - lambda P_2) v
+ *   lambda = exp(a_1 . b_1) - exp(a_2 . b_2) + lambda_init   per head
+ * Layouts: q [items, 2 heads, nq, head_dim] and k [items, 2 kv_heads, nk,
+ * head_dim], heads 2 h and 2 h + 1 being the two maps of head h; v [items,
+ * kv_heads, nk, 2 head_dim]; out [items, heads, nq, 2 head_dim]. Query heads
+ * heads / kv_heads * j and on share key/value head j. *_strides are {item,
+ * head, token} in elements, each a multiple of 16 bytes, the last axis
+ * contiguous, so that the projections' own token-major rows are taken as they
+ * lie. bias [items / bias_share, heads, nq, nk] (strides {plane, head, query},
+ * keys contiguous) serves bias_share consecutive items a plane: the rows of a
+ * triangle attention share one.
+ * A key takes part where mask ([items, nk] bytes, or NULL) is not 0 and the
+ * bias is above float32's lowest value / log2(e), about -2.36e38: -inf and the
+ * types' lowest values take a key out. A masked key's k, v and bias are never
+ * looked at (they may hold NaN), one that only the bias takes out needs finite
+ * k and v. A row without a key is zeros, with zero gradients.
+ * stats ([items, 2 heads, nq] fp32, or NULL): what the backward pass needs to
+ * know of a row. Supported: head_dim 32 or 64. Scores, weights and sums are fp32; the
+ * maps' weights enter the products with v as two bf16 parts (fp32: as they are).
+ */
+typedef struct fjx_diff_attention_args {
+  int64_t items;
+  int64_t heads;
+  int64_t kv_heads;     /* a divisor of heads */
+  int64_t nq;
+  int64_t nk;
+  int64_t head_dim;
+  int64_t bias_share;   /* a divisor of items; ignored without a bias */
+  int32_t dtype;        /* of q, k, v, bias and out */
+  float scale;
+  float lambda_init;
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  int64_t q_strides[3];
+  int64_t k_strides[3];
+  int64_t v_strides[3];
+  int64_t out_strides[3];
+  const void* bias;            /* or NULL; element alignment */
+  int64_t bias_strides[3];
+  const uint8_t* mask;         /* or NULL */
+  const float* lambda_vectors; /* [4, heads, head_dim]: a_1, b_1, a_2, b_2 */
+  float* stats;                /* or NULL */
+  void* workspace;             /* may be NULL when the size is 0 */
+  size_t workspace_bytes;
+} fjx_diff_attention_args;
+
+size_t fjx_diff_attention_workspace_size(int64_t items, int64_t heads, int64_t kv_heads, int64_t nq, int64_t nk,
+                                         int64_t head_dim, int32_t dtype);
+int fjx_diff_attention_fwd(const fjx_diff_attention_args* args, hipStream_t stream);
+
+/*
+ * The gradients of fjx_diff_attention_fwd. `fwd` holds that call's arguments
+ * (out is not read; its strides are dout's), with the stats it wrote. Every
+ * sum has one order: the same bits each time. dk and dv of a shared head are
+ * summed over its query heads, dbias over its plane's items.
+ */
+typedef struct fjx_diff_attention_bwd_args {
+  fjx_diff_attention_args fwd;
+  const void* dout;
+  void* dq;
+  void* dk;
+  void* dv;
+  int64_t dq_strides[3];
+  int64_t dk_strides[3];
+  int64_t dv_strides[3];
+  void* dbias;           /* or NULL (always without a bias) */
+  int64_t dbias_strides[3];
+  float* dlambda;        /* [4, heads, head_dim] */
+} fjx_diff_attention_bwd_args;
+
+/* with_dbias: whether dbias will be asked for */
+size_t fjx_diff_attention_bwd_workspace_size(int64_t items, int64_t heads, int64_t nq, int64_t nk, int64_t bias_share,
+                                             int32_t with_dbias);
+int fjx_diff_attention_bwd(const fjx_diff_attention_bwd_args* args, hipStream_t stream);
+
+/* 8-bit outputs of fjx_rms_norm_fwd */
+enum { FJX_CODES_NONE = 0, FJX_CODES_E4M3 = 1, FJX_CODES_INT8 = 2 };
+
+/*
+ * Root-mean-square norm of rows of c channels, with the residual's addition:
+ *   h = x + residual                        (x itself when residual is NULL)
+ *   y = h / sqrt(mean(h^2) + eps) * weight  (of the unrounded sum)
+ * h is written to sum_out when that is given. codes: y goes out in 8 bits
+ * instead, y ~ codes * scale with scale = max |y| / 448 (e4m3) or / 127 (int8)
+ * over a row, or over every `group` channels (32, 64 or 128, dividing c); a
+ * row or group whose values are all below 1e-30 is zeros with a scale of zero,
+ * one with a NaN has a NaN scale. No counterpart in the reference, whose norms
+ * are LayerNorms. c a multiple of 8 up to 8192.
+ */
+typedef struct fjx_rms_norm_args {
+  int64_t rows;
+  int64_t c;
+  int32_t dtype;         /* of x, residual, weight, sum_out and out */
+  float eps;
+  const void* x;         /* [rows, c] */
+  const void* residual;  /* [rows, c] or NULL */
+  const void* weight;    /* [c] */
+  void* sum_out;         /* [rows, c] or NULL; may be x or residual */
+  void* out;             /* [rows, c] (with codes: bytes); without codes it may be x or residual if sum_out is not */
+  int32_t codes;         /* FJX_CODES_* */
+  int64_t group;         /* 0: a scale a row */
+  float* scales;         /* [rows, c / group], with codes */
+} fjx_rms_norm_args;
+
+int fjx_rms_norm_fwd(const fjx_rms_norm_args* args, hipStream_t stream);
+
+/* The gradients at the stored sum h: dx (the residual's too) =
+ * rstd (dy w - n mean(dy w n)) + dh with n = h rstd, dweight = the sum of dy n
+ * over the rows, in one order. */
+typedef struct fjx_rms_norm_bwd_args {
+  int64_t rows;
+  int64_t c;
+  int32_t dtype;
+  float eps;
+  const void* dy;
+  const void* h;
+  const void* weight;
+  const void* dh;    /* the gradient that reaches the sum from elsewhere, or NULL */
+  void* dx;          /* may be dy or dh */
+  float* dweight;    /* [c] fp32 */
+  void* workspace;
+  size_t workspace_bytes;
+} fjx_rms_norm_bwd_args;
+
+size_t fjx_rms_norm_bwd_workspace_size(int64_t rows, int64_t c);
+int fjx_rms_norm_bwd(const fjx_rms_norm_bwd_args* args, hipStream_t stream);
+
+/*
+ * Dropout of x [batch, n, m, c] with the residual's addition:
+ *   out = residual + (kept ? x / (1 - p) : 0)   (* (out_mask != 0))
+ * The mask is never stored: its shape is x's with 1 for the axes in `shared`
+ * (FJX_SHARE_*: the Pairformer drops the pair track's updates with one mask
+ * for all rows, or for all columns after the ending node), and its element i
+ * is kept where word i % 4 of Philox 4x32-10 of the counter (i / 4, offset)
+ * under the key `seed` is at least p 2^32. `step` (a device value added to the
+ * offset) gives each replay of a captured call a mask of its own. The same
+ * call without a residual on the output's gradient is the backward pass.
+ */
+enum { FJX_SHARE_N = 1, FJX_SHARE_M = 2, FJX_SHARE_C = 4 };
+
+typedef struct fjx_dropout_args {
+  int64_t batch;
+  int64_t n;
+  int64_t m;
+  int64_t c;             /* a multiple of 8 */
+  int32_t dtype;
+  int32_t shared;        /* FJX_SHARE_* flags */
+  double p;              /* in [0, 1) */
+  uint64_t seed;
+  uint64_t offset;
+  const uint64_t* step;  /* device, or NULL */
+  const void* x;
+  const void* residual;  /* like x, or NULL */
+  const void* out_mask;  /* [batch, n, m], or NULL: see "Output masks" */
+  void* out;             /* like x; x, residual and out may be one buffer */
+} fjx_dropout_args;
+
+int fjx_dropout_fwd(const fjx_dropout_args* args, hipStream_t stream);
 
 /* Message for the last error on the calling thread ("" if none). */
 const char* fjx_last_error(void);
