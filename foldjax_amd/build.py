@@ -49,8 +49,12 @@ def _hipcc() -> str:
 # faster with max-ilp, the row kernels' tri-mul epilogue 4 % and tri-attn
 # epilogue 1 % faster with iterative-ilp (the prologues unchanged), the single
 # attention's flash kernel 27 % faster with iterative-ilp; the other files
-# measured no better or slower with either.
+# measured no better or slower with either. Differential attention's kernels
+# read every accumulator they make as well (a token against 16384 keys 33.7 ->
+# 31.5 us, the float32 gradients 3 % faster, the rest within 1 %).
 FILE_FLAGS = {
+    "fjx_diffattn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "fjx_diffattn_bwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "fjx_single_flash.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],
     "fjx_flash.hip": ["-fno-honor-nans", "-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "fjx_rowproj.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1", "-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],

@@ -1147,11 +1147,12 @@ DiffPlan diff_plan(int64_t items, int64_t heads, int64_t kv_heads, int64_t nq, i
 struct DiffBwdPlan {
   int chunks;
   int64_t chunk_items;
-  size_t delta, part;
+  size_t delta, lam, part;  // workspace bytes
 };
 DiffBwdPlan diff_bwd_plan(int64_t items, int64_t heads, int64_t nq, int64_t nk, int64_t share, bool with_dbias) {
   DiffBwdPlan p = {};
   p.delta = align_up((size_t)items * 2 * heads * nq * sizeof(float));
+  p.lam = align_up(diffattn_lam_floats(items, (int)heads, nq) * sizeof(float));
   if (with_dbias && share > 1) {
     const int64_t planes = items / share;
     const int64_t tiles = planes * heads * ((nq + 63) / 64) * ((nk + 63) / 64);
@@ -1182,6 +1183,8 @@ int diff_check(const fjx_diff_attention_args* a, const char* fn, const void* out
   if (a->heads % a->kv_heads)
     return fail(FJX_ERR_INVALID, "%s: kv_heads must divide heads, got %lld and %lld", fn, (long long)a->kv_heads,
                 (long long)a->heads);
+  if (!(a->scale >= 1e-30f && a->scale <= 1e30f))
+    return fail(FJX_ERR_INVALID, "%s: scale must be in [1e-30, 1e30], got %g", fn, (double)a->scale);
   constexpr int64_t kLong = (int64_t)1 << 31;
   if (a->nq >= kLong || a->nk >= kLong || a->items >= kLong)
     return fail(FJX_ERR_UNSUPPORTED, "%s: items, nq and nk must be below 2^31", fn);
@@ -1228,6 +1231,7 @@ DiffAttnParams<T> diff_params(const fjx_diff_attention_args* a) {
   p.group = (int)(a->heads / a->kv_heads);
   p.scale = a->scale;
   p.scale_log2 = a->scale * kLog2e;
+  p.inv_scale = 1.f / a->scale;
   p.init = a->lambda_init;
   return p;
 }
@@ -1258,7 +1262,8 @@ int diff_bwd_run(const fjx_diff_attention_bwd_args* b, const DiffBwdPlan& plan, 
   p.saved = a->stats;
   p.dlam = b->dlambda;
   p.delta = at<float>(a->workspace, 0);
-  p.part_bias = at<float>(a->workspace, plan.delta);
+  p.part_lam = plan.lam ? at<float>(a->workspace, plan.delta) : nullptr;
+  p.part_bias = at<float>(a->workspace, plan.delta + plan.lam);
   p.chunks = plan.chunks;
   p.chunk_items = plan.chunk_items;
   return timed(K_DIFF_ATTENTION_BWD, st, "diff_attention_bwd",
@@ -1550,7 +1555,7 @@ size_t fjx_diff_attention_bwd_workspace_size(int64_t items, int64_t heads, int64
                                              int32_t with_dbias) {
   if (items < 1 || heads < 1 || nq < 1 || nk < 1 || (with_dbias && (bias_share < 1 || items % bias_share))) return 0;
   const DiffBwdPlan p = diff_bwd_plan(items, heads, nq, nk, bias_share, with_dbias != 0);
-  return p.delta + p.part;
+  return p.delta + p.lam + p.part;
 }
 
 int fjx_diff_attention_bwd(const fjx_diff_attention_bwd_args* b, hipStream_t st) {
@@ -1578,7 +1583,7 @@ int fjx_diff_attention_bwd(const fjx_diff_attention_bwd_args* b, hipStream_t st)
   const double tiles = (double)std::max(plan.chunks, 1) * a->items * a->heads * (a->nq / 64 + 1.0) * (a->nk / 64 + 1.0) /
                        (a->bias ? a->bias_share : a->items);
   if (plan.chunks && tiles >= (1 << 23)) return fail(FJX_ERR_UNSUPPORTED, "%s: more bias than one launch takes", fn);
-  const size_t need = plan.delta + plan.part;
+  const size_t need = plan.delta + plan.lam + plan.part;
   if (!a->workspace || a->workspace_bytes < need)
     return fail(FJX_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", fn, need, a->workspace_bytes);
   if (!aligned16({a->workspace})) return fail(FJX_ERR_INVALID, "%s: the workspace must be 16-byte aligned", fn);

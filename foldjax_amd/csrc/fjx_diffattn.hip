@@ -24,7 +24,7 @@ constexpr float kSlack = 8.f;
 // 128-key block, for calls with few rows; otherwise each has 16 rows of its own
 // and walks every 64-key block.
 template <typename T, int D, bool KEYWISE>
-__global__ __launch_bounds__(256) void diffattn_fwd_kernel(DiffAttnParams<T> P) {
+__global__ __launch_bounds__(256, (kDaWaves<T, D> + (kDaWaves<T, D> > 1))) void diffattn_fwd_kernel(DiffAttnParams<T> P) {
   constexpr int kRows = KEYWISE ? 128 : 64;    // keys of a block
   constexpr int kNt = KEYWISE ? 2 : 4;         // key tiles of a wave in one
   constexpr int kBufs = KEYWISE ? 1 : 2;
@@ -34,28 +34,29 @@ __global__ __launch_bounds__(256) void diffattn_fwd_kernel(DiffAttnParams<T> P) 
   constexpr size_t kMerge = 4 * 16 * 2 * (2 * D + 4) * sizeof(float);
   constexpr size_t kBytes = kBufs * sizeof(Tile) > kMerge || !KEYWISE ? kBufs * sizeof(Tile) : kMerge;
   __shared__ __attribute__((aligned(16))) unsigned char raw[kBytes];
-  __shared__ __attribute__((aligned(16))) float key_on[kBufs][kRows];
+  __shared__ __attribute__((aligned(16))) KeyFlags<kRows> flags[3];  // of the block at hand and the next two
   Tile* tiles = reinterpret_cast<Tile*>(raw);
 
   const int t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int kvh = P.heads / P.group;
-  const int64_t rows = P.group * P.nq;  // of one key/value head
-  const int64_t row_blocks = KEYWISE ? (rows + 15) / 16 : (rows + 63) / 64;
-  int64_t id = xcd_order(blockIdx.x, gridDim.x);
-  if (id >= P.items * kvh * row_blocks * P.splits) return;
-  const int64_t rb = id % row_blocks;
+  // 32 bits from here to the item: a launch has fewer than 2^23 workgroups
+  const uint32_t nq = (uint32_t)P.nq, rows = P.group * nq;  // of one key/value head
+  const uint32_t row_blocks = KEYWISE ? (rows + 15) / 16 : (rows + 63) / 64;
+  uint32_t id = xcd_order(blockIdx.x, gridDim.x);
+  if (id >= (uint32_t)P.items * kvh * row_blocks * P.splits) return;
+  const uint32_t rb = id % row_blocks;
   id /= row_blocks;
-  const int split = (int)(id % P.splits);
-  id /= P.splits;
-  const int kv = (int)(id % kvh);
-  const int64_t item = id / kvh;
+  const uint32_t split = id % (uint32_t)P.splits;
+  id /= (uint32_t)P.splits;
+  const int kv = id % (uint32_t)kvh;
+  const int64_t item = id / (uint32_t)kvh;
 
-  const int64_t row = KEYWISE ? rb * 16 + li : rb * 64 + 16 * wave + li;
+  const uint32_t row = KEYWISE ? rb * 16 + li : rb * 64 + 16 * wave + li;
   const bool row_on = row < rows;
-  const int64_t row_c = row_on ? row : rows - 1;
-  const int hg = (int)(row_c / P.nq);
-  const int64_t qi = row_c - hg * P.nq;
+  const uint32_t row_c = row_on ? row : rows - 1;
+  const int hg = row_c / nq;
+  const int64_t qi = row_c - hg * nq;
   const int head = kv * P.group + hg;
 
   DaStage<T, D, kRows, 256> st;
@@ -68,7 +69,6 @@ __global__ __launch_bounds__(256) void diffattn_fwd_kernel(DiffAttnParams<T> P) 
   const int64_t blk0 = split * P.split_blocks;
   const int64_t blk1 = blk0 + P.split_blocks < blocks ? blk0 + P.split_blocks : blocks;
 
-  st.load(blk0 * kRows, P.nk, mask);
   F qf[2][kC];
 #pragma unroll
   for (int m = 0; m < 2; ++m)
@@ -77,101 +77,109 @@ __global__ __launch_bounds__(256) void diffattn_fwd_kernel(DiffAttnParams<T> P) 
       qf[m][c] = load8(P.q.p + item * P.q.item + (2 * head + m) * P.q.head + qi * P.q.token + 32 * c + 8 * lg);
   const float lam = da_lambda<D>(P.lam, P.heads, head, P.init, lane);
 
-  // a key that takes part adds nothing, or lets the bias through: 0, or +inf
-  // for the minimum with the bias; one that does not is -inf either way (also
-  // against a NaN in the bias)
-  const float on = bias ? INFINITY : 0.f;
-  auto key_flags = [&](int64_t blk, int buf) {
+  auto key_flags = [&](int64_t blk, int at) {
     if (t < kRows) {
       const int64_t k = blk * kRows + t;
-      key_on[buf][t] = k < P.nk && (!mask || mask[k]) ? on : -INFINITY;
+      flags[at].set(t, k < P.nk && (!mask || mask[k]));
     }
   };
   const int key_w = KEYWISE ? 32 * wave : 0;  // this wave's keys of a block
-  f32x4 bv[kNt];
+  typename Quad<T>::type bv[kNt];
   auto load_bias = [&](int64_t blk) {
-    const int64_t k0 = blk * kRows + key_w + 4 * lg;
-    if ((blk + 1) * kRows <= P.nk) {
-#pragma unroll
-      for (int kt = 0; kt < kNt; ++kt) bv[kt] = load4_any(bias + k0 + 16 * kt);
-    } else {
-#pragma unroll
-      for (int kt = 0; kt < kNt; ++kt)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) bv[kt][r] = k0 + 16 * kt + r < P.nk ? to_f32(bias[k0 + 16 * kt + r]) : 0.f;
-    }
+    bias_tile<T, kNt>(bias, blk * kRows + key_w + 4 * lg, P.nk, (blk + 1) * kRows <= P.nk, bv);
   };
-  if (bias && blk0 < blk1) load_bias(blk0);
+  if (bias) load_bias(blk0);
+  key_flags(blk0, 0);
+  key_flags(blk0 + 1, 1);
+  __syncthreads();
+  st.load(blk0 * kRows, flags[0].whole(), flags[0].on);
 
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  f32x4 o[2][kU];
+  // the sums of the weights: in bf16 a row of ones times their parts, on the
+  // matrix cores, which have the time; lane l gets its own row's
+  constexpr bool kOnes = sizeof(T) == 2;
+  F ones;
 #pragma unroll
-  for (int mp = 0; mp < 2; ++mp)
+  for (int e = 0; e < 8; ++e) ones[e] = from_f32<T>(1.f);
+  float m[2] = {-INFINITY, -INFINITY};
+  f32x4 l[2], o[2][kU];
+#pragma unroll
+  for (int mp = 0; mp < 2; ++mp) {
+    l[mp] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int u = 0; u < kU; ++u) o[mp][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
 
   st.store(tiles[0]);
-  key_flags(blk0, 0);
   __syncthreads();
 
+  int cur = 0;  // the block's flags
   for (int64_t blk = blk0; blk < blk1; ++blk) {
     const int buf = kBufs == 2 ? (int)(blk - blk0) & 1 : 0;
     const Tile& tile = tiles[buf];
     const bool more = blk + 1 < blk1;
+    const int next = cur == 2 ? 0 : cur + 1;
     f32x4 b[kNt];
 #pragma unroll
-    for (int kt = 0; kt < kNt; ++kt) {
-      b[kt] = *reinterpret_cast<const f32x4*>(&key_on[buf][key_w + 16 * kt + 4 * lg]);
-      if (bias) {
+    for (int kt = 0; kt < kNt; ++kt)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) b[kt][r] = fminf(bv[kt][r] * kLog2e, b[kt][r]);
-      }
-    }
+      for (int r = 0; r < 4; ++r) b[kt][r] = bias ? to_f32(bv[kt][r]) * P.inv_scale : 0.f;
+    flags[cur].apply(key_w, lg, b);
     if (more) {
-      st.load((blk + 1) * kRows, P.nk, mask);
+      st.load((blk + 1) * kRows, flags[next].whole(), flags[next].on);
       if (bias) load_bias(blk + 1);
+      key_flags(blk + 2, next == 2 ? 0 : next + 1);
+    }
+    cur = next;
+    f32x4 s[2][kNt];
+    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int kt = 0; kt < kNt; ++kt)
+#pragma unroll
+      for (int mp = 0; mp < 2; ++mp) {
+        s[mp][kt] = b[kt];
+#pragma unroll
+        for (int c = 0; c < kC; ++c) mma(s[mp][kt], load8(&tile.a[mp][key_w + 16 * kt + li][32 * c + 8 * lg]), qf[mp][c]);
+      }
+#pragma unroll
+    for (int kt = 0; kt < kNt; ++kt)
+#pragma unroll
+      for (int mp = 0; mp < 2; ++mp)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) top[mp] = fmaxf(top[mp], s[mp][kt][r]);
+    top[0] = group_max(top[0]) * P.scale_log2;
+    top[1] = group_max(top[1]) * P.scale_log2;
+    if (__builtin_amdgcn_ballot_w64(top[0] > m[0] + kSlack || top[1] > m[1] + kSlack)) {
+#pragma unroll
+      for (int mp = 0; mp < 2; ++mp) {
+        const float mn = fmaxf(m[mp], top[mp]);
+        const float alpha = __builtin_amdgcn_exp2f(m[mp] - exponent_base(mn));  // 0 where no key was before
+        m[mp] = mn;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          l[mp][r] *= alpha;
+#pragma unroll
+          for (int u = 0; u < kU; ++u) o[mp][u][r] *= alpha;
+        }
+      }
     }
     F pf[2][kNt / 2][kParts<T>];
 #pragma unroll
     for (int mp = 0; mp < 2; ++mp) {
-      f32x4 s[kNt];
-#pragma unroll
-      for (int kt = 0; kt < kNt; ++kt) {
-        s[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < kC; ++c) mma(s[kt], load8(&tile.a[mp][key_w + 16 * kt + li][32 * c + 8 * lg]), qf[mp][c]);
-      }
-      float top = -INFINITY;
-#pragma unroll
-      for (int kt = 0; kt < kNt; ++kt)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          s[kt][r] = fmaf(s[kt][r], P.scale_log2, b[kt][r]);
-          top = fmaxf(top, s[kt][r]);
-        }
-      top = group_max(top);
-      if (__builtin_amdgcn_ballot_w64(top > m[mp] + kSlack)) {
-        const float mn = fmaxf(m[mp], top);
-        const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[mp] - mn);
-        m[mp] = mn;
-        l[mp] *= alpha;
-#pragma unroll
-        for (int u = 0; u < kU; ++u)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) o[mp][u][r] *= alpha;
-      }
-      const float base = m[mp] == -INFINITY ? 0.f : m[mp];  // no key so far: every weight is 0
+      const float base = exponent_base(m[mp]);
       float p[kNt / 2][8];
 #pragma unroll
       for (int kt = 0; kt < kNt; ++kt)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float e = __builtin_amdgcn_exp2f(s[kt][r] - base);
-          l[mp] += e;
+          const float e = __builtin_amdgcn_exp2f(fmaf(s[mp][kt][r], P.scale_log2, -base));
+          if (!kOnes) l[mp][r] += e;
           p[kt >> 1][4 * (kt & 1) + r] = e;
         }
 #pragma unroll
-      for (int c = 0; c < kNt / 2; ++c) parts(p[c], pf[mp][c]);
+      for (int c = 0; c < kNt / 2; ++c) {
+        parts(p[c], pf[mp][c]);
+        if (kOnes) mma_parts(l[mp], ones, pf[mp][c]);
+      }
     }
 #pragma unroll
     for (int c = 0; c < kNt / 2; ++c)
@@ -184,12 +192,12 @@ __global__ __launch_bounds__(256) void diffattn_fwd_kernel(DiffAttnParams<T> P) 
     if (kBufs == 1) __syncthreads();
     if (more) {
       st.store(tiles[kBufs == 2 ? buf ^ 1 : 0]);
-      key_flags(blk + 1, kBufs == 2 ? buf ^ 1 : 0);
     }
     __syncthreads();
   }
-  l[0] = group_sum(l[0]);
-  l[1] = group_sum(l[1]);
+  float ls[2];
+#pragma unroll
+  for (int mp = 0; mp < 2; ++mp) ls[mp] = kOnes ? l[mp][0] : group_sum((l[mp][0] + l[mp][1]) + (l[mp][2] + l[mp][3]));
 
   if constexpr (KEYWISE) {
     // the waves' partial rows, on the largest of their maxima
@@ -199,25 +207,26 @@ __global__ __launch_bounds__(256) void diffattn_fwd_kernel(DiffAttnParams<T> P) 
     if (lg == 0)
       for (int mp = 0; mp < 2; ++mp) {
         ml[((wave * 2 + mp) * 16 + li) * 2] = m[mp];
-        ml[((wave * 2 + mp) * 16 + li) * 2 + 1] = l[mp];
+        ml[((wave * 2 + mp) * 16 + li) * 2 + 1] = ls[mp];
       }
     __syncthreads();
 #pragma unroll
     for (int mp = 0; mp < 2; ++mp) {
-      float mx = -INFINITY, ls = 0.f;
+      float mx = -INFINITY, sum = 0.f;
 #pragma unroll
       for (int w = 0; w < 4; ++w) mx = fmaxf(mx, ml[((w * 2 + mp) * 16 + li) * 2]);
-      const float base = mx == -INFINITY ? 0.f : mx;
+      const float base = exponent_base(mx);
 #pragma unroll
       for (int w = 0; w < 4; ++w)
-        ls = fmaf(ml[((w * 2 + mp) * 16 + li) * 2 + 1], __builtin_amdgcn_exp2f(ml[((w * 2 + mp) * 16 + li) * 2] - base), ls);
+        sum = fmaf(ml[((w * 2 + mp) * 16 + li) * 2 + 1],
+                   __builtin_amdgcn_exp2f(ml[((w * 2 + mp) * 16 + li) * 2] - base), sum);
       const float alpha = __builtin_amdgcn_exp2f(m[mp] - base);
 #pragma unroll
       for (int u = 0; u < kU; ++u)
 #pragma unroll
         for (int r = 0; r < 4; ++r) po[((wave * 2 + mp) * 16 + li) * kPo + 16 * u + 4 * lg + r] = o[mp][u][r] * alpha;
       m[mp] = mx;
-      l[mp] = ls;
+      ls[mp] = sum;
     }
     __syncthreads();
     // each wave takes kU / 4 of the tiles of 16 values
@@ -242,7 +251,7 @@ __global__ __launch_bounds__(256) void diffattn_fwd_kernel(DiffAttnParams<T> P) 
     const int64_t base = (split * (P.items * P.heads * P.nq) + at) * 2;
 #pragma unroll
     for (int mp = 0; mp < 2; ++mp) {
-      if (first) *reinterpret_cast<f32x2*>(P.part_ml + (base + mp) * 2) = f32x2{m[mp], l[mp]};
+      if (first) *reinterpret_cast<f32x2*>(P.part_ml + (base + mp) * 2) = f32x2{m[mp], ls[mp]};
 #pragma unroll
       for (int u = 0; u < kOwn; ++u)
         *reinterpret_cast<f32x4*>(P.part_o + (base + mp) * (2 * D) + 16 * (u0 + u) + 4 * lg) = o[mp][u];
@@ -252,9 +261,9 @@ __global__ __launch_bounds__(256) void diffattn_fwd_kernel(DiffAttnParams<T> P) 
   float inv[2];
 #pragma unroll
   for (int mp = 0; mp < 2; ++mp) {
-    inv[mp] = l[mp] == 0.f ? 0.f : 1.f / l[mp];  // a row without keys is zeros
+    inv[mp] = ls[mp] == 0.f ? 0.f : 1.f / ls[mp];  // a row without keys is zeros
     if (first && P.stats)  // +inf for such a row: its weights are zeros in the backward pass as well
-      P.stats[(item * 2 * P.heads + 2 * head + mp) * P.nq + qi] = l[mp] == 0.f ? INFINITY : m[mp] + log2f(l[mp]);
+      P.stats[(item * 2 * P.heads + 2 * head + mp) * P.nq + qi] = ls[mp] == 0.f ? INFINITY : m[mp] + log2f(ls[mp]);
   }
   inv[1] *= lam;
   T* out = P.out.p + item * P.out.item + head * P.out.head + qi * P.out.token;
@@ -285,7 +294,7 @@ __global__ __launch_bounds__(256) void diffattn_join_kernel(DiffAttnParams<T> P)
     for (int s = lane; s < P.splits; s += 64) mx = fmaxf(mx, P.part_ml[((s * rows + at) * 2 + mp) * 2]);
 #pragma unroll
     for (int x = 32; x >= 1; x >>= 1) mx = fmaxf(mx, shfl_xor(mx, x));
-    const float base = mx == -INFINITY ? 0.f : mx;
+    const float base = exponent_base(mx);
     float l = 0.f, o[2 * D / 64] = {};
 #pragma unroll 4
     for (int s = 0; s < P.splits; ++s) {
@@ -299,7 +308,7 @@ __global__ __launch_bounds__(256) void diffattn_join_kernel(DiffAttnParams<T> P)
     const float inv = (l == 0.f ? 0.f : 1.f / l) * (mp ? -lam : 1.f);
 #pragma unroll
     for (int j = 0; j < 2 * D / 64; ++j) res[j] = fmaf(o[j], inv, res[j]);
-    if (lane == 0 && P.stats) P.stats[(item * 2 * P.heads + 2 * head + mp) * P.nq + qi] = l == 0.f ? INFINITY : mx + log2f(l);
+    if (lane == 0 && P.stats) P.stats[(item * 2 * P.heads + 2 * head + mp) * P.nq + qi] = l == 0.f ? INFINITY : base + log2f(l);
   }
   T* out = P.out.p + item * P.out.item + head * P.out.head + qi * P.out.token;
 #pragma unroll

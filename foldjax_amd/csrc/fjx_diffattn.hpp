@@ -7,9 +7,11 @@
 // The heads of one key/value head are worked on together: its query rows are
 // the nq queries of each of the heads / kv_heads query heads, one after the
 // other, so that a single token's heads fill one 16-row tile and read the
-// cache once. Scores are in log2 units: scale log2(e) and log2(e) are folded
-// into one fma, and a bias whose product with log2(e) leaves float32's range
-// (the types' lowest values) is -inf, as a masked key is.
+// cache once. A score starts as bias / scale, in the accumulator of its matrix
+// instruction, and is left unscaled: the exponent of a weight is one fma,
+// 2^(s scale log2(e) - M), with the row's maximum M in log2 units. A bias whose
+// quotient by the scale or product with log2(e) leaves float32's range (-inf and
+// the types' lowest values) is no key.
 #pragma once
 
 #include "fjx_common.hpp"
@@ -34,7 +36,7 @@ struct DiffAttnParams {
   float* stats;                // [items][2 H][nq] row statistics, or null
   int64_t items, nq, nk, share;
   int heads, group;            // query heads, and those of one key/value head
-  float scale_log2, init;
+  float scale, scale_log2, inv_scale, init;  // scale_log2: times log2(e)
   // keys split over workgroups: key blocks of one split, and the partial
   // results [split][items][H nq rows][2 maps]: values [2 D], then (max, sum)
   int splits;
@@ -48,11 +50,14 @@ struct DiffAttnParams {
   const float* saved;          // the forward pass's stats
   float* delta;                // [items][2 H][nq]: rowsum(P_t dP)
   float* dlam;                 // [4][H][D]
+  float* part_lam;             // [H][parts] sums of D_2, or null: few rows
   float* part_bias;            // [chunks][planes][H][nq][nk] partial sums of dbias
   int64_t chunk_items;         // items of one chunk
   int chunks;
-  float scale;
 };
+
+// waves a SIMD that the registers are held to
+template <typename T, int D> constexpr int kDaWaves = sizeof(T) == 2 && D == 32 ? 2 : 1;
 
 constexpr int kDaKeys = 64;  // keys (or, for the keys' gradients, queries) of a staged block
 
@@ -92,17 +97,24 @@ __device__ __forceinline__ f32x8 col_frag(const float* tile, int pitch, int row0
 }
 
 // A float32 operand that the kernel computed (weights, dS) as the matrix
-// instructions take it: itself, or two bf16 parts (16 bits; the high one cut,
-// not rounded: the low one holds what is left either way), whose products take
+// instructions take it: itself, or two bf16 parts (17 bits), whose products take
 // twice the matrix instructions. These run beside the exponentials and the
-// vector work that bound the kernels.
+// vector work that bound the kernels. What is left of a pair of values beyond
+// their high parts is one v_dot2_f32_bf16 each, (h_0, h_1) . (-1, 0) + x_0 (exact),
+// where unpacking and subtracting takes two instructions. Its selector stays in a
+// register: as an inline constant it reached the instruction as the other half.
 template <typename T> constexpr int kParts = sizeof(T) == 2 ? 2 : 1;
 __device__ __forceinline__ void parts(const float* p, bf16x8 (&f)[2]) {
+  typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  uint32_t first = 0x0000bf80u, second = 0xbf800000u;
+  asm("" : "+s"(first), "+s"(second));
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float hi = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, p[e]) & 0xffff0000u);
-    f[0][e] = static_cast<bf16>(hi);
-    f[1][e] = static_cast<bf16>(p[e] - hi);
+  for (int e = 0; e < 8; e += 2) {
+    const bf16x2 h = {static_cast<bf16>(p[e]), static_cast<bf16>(p[e + 1])};
+    f[0][e] = h[0];
+    f[0][e + 1] = h[1];
+    f[1][e] = static_cast<bf16>(__builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(bf16x2, first), p[e], false));
+    f[1][e + 1] = static_cast<bf16>(__builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(bf16x2, second), p[e + 1], false));
   }
 }
 __device__ __forceinline__ void parts(const float* p, f32x8 (&f)[1]) { f[0] = pack8<float>(p); }
@@ -113,15 +125,60 @@ __device__ __forceinline__ void mma_parts(f32x4& o, const bf16x8& a, const bf16x
 __device__ __forceinline__ void mma_parts(f32x4& o, const f32x8& a, const f32x8 (&p)[1]) { mma(o, a, p[0]); }
 
 // 4 contiguous elements with element alignment only (rows of an odd length)
-__device__ __forceinline__ f32x4 load4_any(const bf16* p) {
-  typedef bf16x4 any4 __attribute__((aligned(2)));
-  const bf16x4 v = *reinterpret_cast<const any4*>(p);
-  return f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
+template <typename T> struct Quad;
+template <> struct Quad<bf16> { typedef bf16x4 type; typedef bf16x4 any __attribute__((aligned(2))); };
+template <> struct Quad<float> { typedef f32x4 type; typedef f32x4 any __attribute__((aligned(4))); };
+
+// the bias of a lane's 4 keys of each of NT tiles, from k0 on (its own 4 g
+// within); zeros past the last key, which its flag takes out
+template <typename T, int NT>
+__device__ __forceinline__ void bias_tile(const T* bias, int64_t k0, int64_t nk, bool whole, typename Quad<T>::type (&bv)[NT]) {
+  if (whole) {
+#pragma unroll
+    for (int kt = 0; kt < NT; ++kt) bv[kt] = *reinterpret_cast<const typename Quad<T>::any*>(bias + k0 + 16 * kt);
+  } else {
+#pragma unroll
+    for (int kt = 0; kt < NT; ++kt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) bv[kt][r] = k0 + 16 * kt + r < nk ? bias[k0 + 16 * kt + r] : from_f32<T>(0.f);
+  }
 }
-__device__ __forceinline__ f32x4 load4_any(const float* p) {
-  typedef f32x4 any4 __attribute__((aligned(4)));
-  return *reinterpret_cast<const any4*>(p);
-}
+
+// Which keys of a block take part: +inf, or -inf for one that does not, so
+// that the minimum with its bias (or 0) is -inf whatever the bias holds, a NaN
+// among it; and whether all of 64 do, the usual case.
+template <int ROWS>
+struct alignas(16) KeyFlags {
+  float on[ROWS];
+  int all[ROWS / 64];
+  // by threads 0 .. ROWS - 1
+  __device__ __forceinline__ void set(int t, bool part) {
+    on[t] = part ? INFINITY : -INFINITY;
+    const bool every = __builtin_amdgcn_ballot_w64(part) == ~0ull;
+    if ((t & 63) == 0) all[t >> 6] = every;
+  }
+  __device__ __forceinline__ bool whole() const {
+    int v = all[0];
+#pragma unroll
+    for (int i = 1; i < ROWS / 64; ++i) v &= all[i];
+    return __builtin_amdgcn_readfirstlane(v);
+  }
+  // b = min(b, flag) for a lane's keys
+  template <int NT>
+  __device__ __forceinline__ void apply(int key_w, int lg, f32x4 (&b)[NT]) const {
+    if (__builtin_amdgcn_readfirstlane(all[key_w >> 6])) return;
+#pragma unroll
+    for (int kt = 0; kt < NT; ++kt) {
+      const f32x4 f = *reinterpret_cast<const f32x4*>(&on[key_w + 16 * kt + 4 * lg]);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) b[kt][r] = fminf(b[kt][r], f[r]);
+    }
+  }
+};
+
+// what a row's maximum (in log2 units) subtracts in the exponent: itself, or 0
+// where the row has no key (every weight is then 2^-inf)
+__device__ __forceinline__ float exponent_base(float m) { return m == -INFINITY ? 0.f : m; }
 
 // max over the 4 lanes {l % 16 + 16 g}
 __device__ __forceinline__ float group_max(float x) {
@@ -180,21 +237,22 @@ struct DaStage {
     row = t / kPk;
     which = in / kPa;  // 0, 1: the a tiles; 2, 3: the halves of b
     col = (in % kPa) * kE + (which == 3 ? D : 0);
-    src = (which < 2 ? a + which * a_head : b) + col;
     pitch = which < 2 ? a_token : b_token;
+    src = (which < 2 ? a + which * a_head : b) + col + row * pitch;
   }
-  __device__ __forceinline__ void load(int64_t row0, int64_t n, const uint8_t* mask) {
-    bool on[kN];
+  // rows row0 .. row0 + ROWS - 1; `all`: every one is there and takes part,
+  // else on[x] says so of row x
+  __device__ __forceinline__ void load(int64_t row0, bool all, const float* on) {
+    const T* p = src + row0 * pitch;
+    if (all) {
 #pragma unroll
-    for (int i = 0; i < kN; ++i) {
-      const int64_t x = row0 + row + i * kStep;
-      on[i] = x < n;
-      if (on[i] && mask) on[i] = mask[x] != 0;
-    }
+      for (int i = 0; i < kN; ++i) r[i] = *reinterpret_cast<const u32x4*>(p + i * kStep * pitch);
+    } else {
 #pragma unroll
-    for (int i = 0; i < kN; ++i) {
-      r[i] = u32x4{0, 0, 0, 0};
-      if (on[i]) r[i] = *reinterpret_cast<const u32x4*>(src + (row0 + row + i * kStep) * pitch);
+      for (int i = 0; i < kN; ++i) {
+        r[i] = u32x4{0, 0, 0, 0};
+        if (on[row + i * kStep] > 0.f) r[i] = *reinterpret_cast<const u32x4*>(p + i * kStep * pitch);
+      }
     }
   }
   __device__ __forceinline__ void store(DaTile<T, D, ROWS>& tile) const {
@@ -210,6 +268,6 @@ struct DaStage {
 // workgroups in an order that keeps neighbours (the tiles of one item, which
 // read the same keys) on one of the 8 XCDs, to which the hardware deals block
 // after block in turn; grids are multiples of 8 blocks
-__device__ __forceinline__ int64_t xcd_order(int64_t blk, int64_t blocks) { return (blk & 7) * (blocks >> 3) + (blk >> 3); }
+__device__ __forceinline__ uint32_t xcd_order(uint32_t blk, uint32_t blocks) { return (blk & 7) * (blocks >> 3) + (blk >> 3); }
 
 }  // namespace fjx

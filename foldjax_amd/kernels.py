@@ -637,15 +637,14 @@ def triattn_core(
 def _launch(entry, args, x: torch.Tensor) -> None:
     """``entry`` on the current stream of ``x``'s device, whichever device is
     the current one."""
-    if torch.cuda.current_device() == x.get_device():
-        _lib.check(entry(ctypes.byref(args), _stream(x)))
+    dev = x.get_device()
+    if torch._C._cuda_getDevice() == dev:  # torch.cuda.current_device without its lazy start: x is there already
+        rc = entry(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(dev))
     else:
-        with torch.cuda.device(x.get_device()):
-            _lib.check(entry(ctypes.byref(args), _stream(x)))
-
-
-def _workspace(nbytes: int, x: torch.Tensor) -> torch.Tensor | None:
-    return torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+        with torch.cuda.device(dev):
+            rc = entry(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        _lib.check(rc)
 
 
 def _need_dtype(dtype: torch.dtype, **operands) -> None:
@@ -654,85 +653,123 @@ def _need_dtype(dtype: torch.dtype, **operands) -> None:
             raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
 
 
-def _rows_ok(t: torch.Tensor) -> bool:
-    """Whether the kernels' 16-byte accesses can take ``t``'s rows as they lie."""
-    es = t.element_size()
-    return (t.stride(-1) == 1 and t.data_ptr() % 16 == 0
-            and all(n == 1 or (s > 0 and s * es % 16 == 0) for n, s in zip(t.shape[:-1], t.stride()[:-1])))
+def _same_place(x: torch.Tensor, dtype: torch.dtype, **operands) -> None:
+    """Every operand there on ``x``'s device and of ``dtype``."""
+    dev = x.get_device()
+    for name, t in operands.items():
+        if t is not None and (t.dtype is not dtype or t.get_device() != dev):
+            _same_device(x, **{name: t})
+            _need_dtype(dtype, **{name: t})
 
 
-def _items(t: torch.Tensor, tail: int) -> torch.Tensor:
-    """The axes before the last ``tail`` folded into one."""
-    return t if t.dim() == tail + 1 else t.reshape((-1,) + tuple(t.shape[t.dim() - tail:]))
+def _folded(shape, strides):
+    """The stride of the axes taken as one, 0 for one element; None where they
+    do not fold."""
+    step, count = 0, 1
+    for n, s in zip(reversed(shape), reversed(strides)):
+        if n == 1:
+            continue
+        if s != step * count if count > 1 else s == 0:
+            return None
+        if count == 1:
+            step = s
+        count *= n
+    return step
 
 
-def _heads(t: torch.Tensor) -> torch.Tensor:
-    """[..., heads, tokens, width] as [items, heads, tokens, width] with rows
-    the kernels can take: a view wherever the strides allow one."""
-    t = _items(t, 3)
-    return t if _rows_ok(t) else t.clone(memory_format=torch.contiguous_format)
+def _head_rows(t: torch.Tensor, unit: int):
+    """Strides {item, head, token} of [..., heads, tokens, width] (0 for an
+    axis of one element), where the kernels can take its rows as they lie, whole
+    16-byte pieces of ``unit`` elements; None where not."""
+    shape, strides = t.shape, t.stride()
+    item = _folded(shape[:-3], strides[:-3])
+    if item is None or strides[-1] != 1 or t.data_ptr() & 15:
+        return None
+    head = strides[-3] if shape[-3] > 1 else 0
+    token = strides[-2] if shape[-2] > 1 else 0
+    if (item | head | token) % unit or (head == 0 and shape[-3] > 1) or (token == 0 and shape[-2] > 1):
+        return None
+    return item, head, token
 
 
-def _strides3(t: torch.Tensor):
-    """Strides of the first three axes; an axis of one element has none."""
-    return _lib._i64x3(*(0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride()[:3])))
+def _heads(t: torch.Tensor, unit: int):
+    """``t`` and its strides, a copy where its rows cannot be taken as they lie."""
+    st = _head_rows(t, unit)
+    if st is None:
+        t = t.clone(memory_format=torch.contiguous_format)
+        st = _head_rows(t, unit)
+    return t, st
+
+
+def _packed(shape):
+    """Strides {item, head, token} of a contiguous [..., heads, tokens, width]."""
+    width, tokens = shape[-1], shape[-2]
+    return shape[-3] * tokens * width, tokens * width, width
 
 
 def _diff_attention_args(q, k, v, lambda_vectors, lambda_init, scale, bias, mask):
     """The checked argument block that both directions share, and the tensors
-    it points to (q, k, v and bias as [items or planes, heads, tokens, ...])."""
-    _same_device(q, k=k, v=v, lambda_vectors=lambda_vectors, bias=bias, mask=mask)
-    code = _code(q.dtype)
-    _need_dtype(q.dtype, k=k, v=v, bias=bias)
-    _need_dtype(torch.float32, lambda_vectors=lambda_vectors)
-    if q.dim() < 3 or k.dim() != q.dim() or v.dim() != q.dim():
-        raise ValueError(f"q, k and v must be [..., heads, tokens, width] of as many axes, got {tuple(q.shape)}, "
-                         f"{tuple(k.shape)}, {tuple(v.shape)}")
-    lead = tuple(q.shape[:-3])
-    h2, nq, d = (int(n) for n in q.shape[-3:])
-    hk2, nk = int(k.shape[-3]), int(k.shape[-2])
+    it points to."""
+    dtype = q.dtype
+    code = _code(dtype)
+    _same_place(q, dtype, k=k, v=v, bias=bias)
+    _same_place(q, torch.float32, lambda_vectors=lambda_vectors)
+    _same_device(q, mask=mask)
+    qs, ks = q.shape, k.shape
+    if len(qs) < 3 or len(ks) != len(qs) or v.dim() != len(qs):
+        raise ValueError(f"q, k and v must be [..., heads, tokens, width] of as many axes, got {tuple(qs)}, "
+                         f"{tuple(ks)}, {tuple(v.shape)}")
+    lead = tuple(qs[:-3])
+    h2, nq, d = qs[-3:]
+    hk2, nk = ks[-3], ks[-2]
     if h2 % 2 or hk2 % 2:
         raise ValueError(f"q and k hold two maps a head: an even number of heads, got {h2} and {hk2}")
     heads, kv_heads = h2 // 2, hk2 // 2
     _need_shape("k", k, lead + (hk2, nk, d))
     _need_shape("v", v, lead + (kv_heads, nk, 2 * d))
     _need_shape("lambda_vectors", lambda_vectors, (4, heads, d))
-    q4, k4, v4 = _heads(q), _heads(k), _heads(v)
-    items = int(q4.shape[0])
-    lam = lambda_vectors.contiguous()
-    b4, share = None, 1
+    unit = 4 if dtype is torch.float32 else 8
+    items = 1
+    for n in lead:
+        items *= n
+    lam = lambda_vectors if lambda_vectors.is_contiguous() else lambda_vectors.contiguous()
+    bp, bst, share = None, (0, 0, 0), 1
     if bias is not None:
-        if bias.dim() < 3 or bias.dim() > q.dim() or tuple(bias.shape[-3:]) != (heads, nq, nk):
-            raise ValueError(f"bias must be [..., {heads}, {nq}, {nk}], got {tuple(bias.shape)}")
+        bs = bias.shape
+        if not 3 <= len(bs) <= len(qs) or bs[-1] != nk or bs[-2] != nq or bs[-3] != heads:
+            raise ValueError(f"bias must be [..., {heads}, {nq}, {nk}], got {tuple(bs)}")
         # planes for the leading items, then axes that share one
-        planes = (1,) * (len(lead) - bias.dim() + 3) + tuple(int(n) for n in bias.shape[:-3])
+        planes = (1,) * (len(qs) - len(bs)) + tuple(bs[:-3])
         axis = len(lead)
         while axis and planes[axis - 1] == 1:
             axis -= 1
             share *= lead[axis]
         if planes[:axis] != lead[:axis]:
             raise ValueError(f"bias must have one plane for each of q's leading axes {lead}, or share one over the last "
-                             f"of them, got {tuple(bias.shape[:-3])}")
-        b4 = _items(bias, 3)
-        if b4.stride(-1) != 1 and nk > 1 or min(b4.stride()) < 0:
-            b4 = b4.contiguous()
+                             f"of them, got {tuple(bs[:-3])}")
+        bst = bias.stride()
+        plane = _folded(bs[:-3], bst[:-3])
+        if plane is None or (bst[-1] != 1 and nk > 1) or min(bst) < 0:
+            bias = bias.contiguous()
+            bst = bias.stride()
+            plane = heads * nq * nk
+        bp, bst = bias.data_ptr(), (plane, bst[-3], bst[-2])
     m2 = None
     if mask is not None:
-        try:
-            m2 = torch.broadcast_to(mask, lead + (nk,))
-        except RuntimeError:
-            raise ValueError(f"mask of shape {tuple(mask.shape)} does not broadcast to {lead + (nk,)}") from None
-        m2 = (m2 if m2.dtype is torch.bool else m2.ne(0)).contiguous()
+        if mask.shape != lead + (nk,):
+            try:
+                mask = torch.broadcast_to(mask, lead + (nk,))
+            except RuntimeError:
+                raise ValueError(f"mask of shape {tuple(mask.shape)} does not broadcast to {lead + (nk,)}") from None
+        m2 = (mask if mask.dtype is torch.bool else mask.ne(0)).contiguous()
     _dev(q)
+    q, qst = _heads(q, unit)
+    k, kst = _heads(k, unit)
+    v, vst = _heads(v, unit)
     a = _lib.DiffAttentionArgs(
-        items=items, heads=heads, kv_heads=kv_heads, nq=nq, nk=nk, head_dim=d, bias_share=share, dtype=code,
-        scale=float(scale), lambda_init=float(lambda_init), q=_ptr(q4), k=_ptr(k4), v=_ptr(v4),
-        q_strides=_strides3(q4), k_strides=_strides3(k4), v_strides=_strides3(v4),
-        bias=_ptr(b4), mask=_ptr(m2), lambda_vectors=_ptr(lam),
-    )
-    if b4 is not None:
-        a.bias_strides = _strides3(b4)
-    return a, (q4, k4, v4, b4, m2, lam), lead
+        items, heads, kv_heads, nq, nk, d, share, code, scale, lambda_init, q.data_ptr(), k.data_ptr(), v.data_ptr(), None,
+        qst, kst, vst, (0, 0, 0), bp, bst, None if m2 is None else m2.data_ptr(), lam.data_ptr())
+    return a, (q, k, v, bias, m2, lam), lead, unit
 
 
 def diff_attention(
@@ -767,31 +804,29 @@ def diff_attention(
     Returns ``out`` ``[..., H, Q, 2 D]``; with ``return_lse`` also what
     ``diff_attention_backward`` needs to know of the rows. ``out``: write into
     this tensor (its rows whole 16-byte pieces, any order of the other axes)."""
-    a, (q4, *kept), lead = _diff_attention_args(q, k, v, lambda_vectors, lambda_init, scale, bias, mask)
+    a, kept, lead, unit = _diff_attention_args(q, k, v, lambda_vectors, lambda_init, scale, bias, mask)
     shape = lead + (a.heads, a.nq, 2 * a.head_dim)
     if out is None:
         out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        a.out_strides = _packed(shape)
     else:
         if out.shape != shape or out.dtype != q.dtype or out.device != q.device:
             raise ValueError(f"out must be a {q.dtype} tensor of shape {shape} on {q.device}, "
                              f"got {out.dtype} {tuple(out.shape)} on {out.device}")
-    o4 = out
-    if out.dim() != 4:
-        try:
-            o4 = out.view((a.items,) + shape[-3:])
-        except RuntimeError:
-            raise ValueError("out's leading axes must fold into one") from None
-    if not _rows_ok(o4):
-        raise ValueError("out must have rows of whole 16-byte pieces")
-    a.out, a.out_strides = _ptr(o4), _strides3(o4)
+        strides = _head_rows(out, unit)
+        if strides is None:
+            raise ValueError("out must have rows of whole 16-byte pieces, and leading axes that fold into one")
+        a.out_strides = strides
+    a.out = out.data_ptr()
     lse = None
     if return_lse:
         lse = torch.empty(lead + (2 * a.heads, a.nq), dtype=torch.float32, device=q.device)
-        a.stats = _ptr(lse)
+        a.stats = lse.data_ptr()
     lib = _lib.load()
     nbytes = lib.fjx_diff_attention_workspace_size(a.items, a.heads, a.kv_heads, a.nq, a.nk, a.head_dim, a.dtype)
-    ws = _workspace(nbytes, q)
-    a.workspace, a.workspace_bytes = _ptr(ws), nbytes
+    if nbytes:
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
     _launch(lib.fjx_diff_attention_fwd, a, q)
     return (out, lse) if return_lse else out
 
@@ -816,28 +851,28 @@ def diff_attention_backward(
     v and bias (dbias None without a bias or with ``bias_grad`` off; of a shared
     plane the sum over the items, of shared heads' k and v the sum over the
     query heads), dlambda float32 ``[4, H, D]``. The same bits each time."""
-    f, (q4, k4, v4, b4, *kept), lead = _diff_attention_args(q, k, v, lambda_vectors, lambda_init, scale, bias, mask)
-    _same_device(q, dout=dout, lse=lse)
-    _need_dtype(q.dtype, dout=dout)
-    _need_dtype(torch.float32, lse=lse)
+    f, kept, lead, unit = _diff_attention_args(q, k, v, lambda_vectors, lambda_init, scale, bias, mask)
+    _same_place(q, q.dtype, dout=dout)
+    _same_place(q, torch.float32, lse=lse)
     _need_shape("dout", dout, lead + (f.heads, f.nq, 2 * f.head_dim))
     _need_shape("lse", lse, lead + (2 * f.heads, f.nq))
-    do4 = _heads(dout)
-    lse = lse.contiguous()
-    f.out_strides, f.stats = _strides3(do4), _ptr(lse)
-    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-    dlam = torch.empty_like(lambda_vectors, memory_format=torch.contiguous_format)
-    g = _lib.DiffAttentionBwdArgs(dout=_ptr(do4), dq=_ptr(dq), dk=_ptr(dk), dv=_ptr(dv), dlambda=_ptr(dlam))
-    g.dq_strides, g.dk_strides, g.dv_strides = (_strides3(_items(t, 3)) for t in (dq, dk, dv))
-    dbias = None
+    dout, f.out_strides = _heads(dout, unit)
+    if not lse.is_contiguous():
+        lse = lse.contiguous()
+    f.stats = lse.data_ptr()
+    dev = q.device
+    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
+    dlam = torch.empty(lambda_vectors.shape, dtype=torch.float32, device=dev)
+    dbias, dbp, dbst = None, None, (0, 0, 0)
     if bias is not None and bias_grad:
-        dbias = torch.empty(bias.shape, dtype=bias.dtype, device=bias.device)
-        g.dbias, g.dbias_strides = _ptr(dbias), _strides3(_items(dbias, 3))
+        dbias = torch.empty(bias.shape, dtype=bias.dtype, device=dev)
+        dbp, dbst = dbias.data_ptr(), _packed(bias.shape)
     lib = _lib.load()
     nbytes = lib.fjx_diff_attention_bwd_workspace_size(f.items, f.heads, f.nq, f.nk, f.bias_share, dbias is not None)
-    ws = _workspace(nbytes, q)
-    f.workspace, f.workspace_bytes = _ptr(ws), nbytes
-    g.fwd = f
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    f.workspace, f.workspace_bytes = ws.data_ptr(), nbytes
+    g = _lib.DiffAttentionBwdArgs(f, dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _packed(q.shape),
+                                  _packed(k.shape), _packed(v.shape), dbp, dbst, dlam.data_ptr())
     _launch(lib.fjx_diff_attention_bwd, g, q)
     return dq, dk, dv, dbias, dlam
 
@@ -941,7 +976,7 @@ def rms_norm_backward(
     lib = _lib.load()
     rows = h.numel() // max(c, 1)
     nbytes = lib.fjx_rms_norm_bwd_workspace_size(rows, c)
-    ws = _workspace(nbytes, h)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=h.device)
     a = _lib.RmsNormBwdArgs(rows=rows, c=c, dtype=code, eps=float(eps), dy=_ptr(dyf), h=_ptr(hf), weight=_ptr(w),
                             dh=_ptr(dhf), dx=_ptr(dx), dweight=_ptr(dw), workspace=_ptr(ws), workspace_bytes=nbytes)
     _launch(lib.fjx_rms_norm_bwd, a, h)
