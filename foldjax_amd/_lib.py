@@ -204,6 +204,8 @@ class FjxError(RuntimeError):
 def load() -> ctypes.CDLL:
     """Load the library once; raise ``RuntimeError`` if it is not built."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib

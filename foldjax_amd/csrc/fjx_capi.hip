@@ -1142,21 +1142,23 @@ DiffPlan diff_plan(int64_t items, int64_t heads, int64_t kv_heads, int64_t nq, i
   return p;
 }
 
+#ifndef DA_CH
+#define DA_CH 512
+#endif
 // The bias gradient of shared planes: items of one chunk, so that the 64 x 64
 // tiles times the chunks are some workgroups a CU.
 struct DiffBwdPlan {
   int chunks;
   int64_t chunk_items;
-  size_t delta, lam, part;  // workspace bytes
+  size_t delta, part;  // workspace bytes
 };
 DiffBwdPlan diff_bwd_plan(int64_t items, int64_t heads, int64_t nq, int64_t nk, int64_t share, bool with_dbias) {
   DiffBwdPlan p = {};
   p.delta = align_up((size_t)items * 2 * heads * nq * sizeof(float));
-  p.lam = align_up(diffattn_lam_floats(items, (int)heads, nq) * sizeof(float));
   if (with_dbias && share > 1) {
     const int64_t planes = items / share;
     const int64_t tiles = planes * heads * ((nq + 63) / 64) * ((nk + 63) / 64);
-    const int64_t want = std::max<int64_t>(1, std::min<int64_t>((1024 + tiles - 1) / tiles, share));
+    const int64_t want = std::max<int64_t>(1, std::min<int64_t>((DA_CH + tiles - 1) / tiles, share));
     p.chunk_items = (share + want - 1) / want;
     p.chunks = (int)((share + p.chunk_items - 1) / p.chunk_items);
     p.part = align_up((size_t)p.chunks * planes * heads * nq * nk * sizeof(float));
@@ -1262,8 +1264,7 @@ int diff_bwd_run(const fjx_diff_attention_bwd_args* b, const DiffBwdPlan& plan, 
   p.saved = a->stats;
   p.dlam = b->dlambda;
   p.delta = at<float>(a->workspace, 0);
-  p.part_lam = plan.lam ? at<float>(a->workspace, plan.delta) : nullptr;
-  p.part_bias = at<float>(a->workspace, plan.delta + plan.lam);
+  p.part_bias = at<float>(a->workspace, plan.delta);
   p.chunks = plan.chunks;
   p.chunk_items = plan.chunk_items;
   return timed(K_DIFF_ATTENTION_BWD, st, "diff_attention_bwd",
@@ -1555,7 +1556,7 @@ size_t fjx_diff_attention_bwd_workspace_size(int64_t items, int64_t heads, int64
                                              int32_t with_dbias) {
   if (items < 1 || heads < 1 || nq < 1 || nk < 1 || (with_dbias && (bias_share < 1 || items % bias_share))) return 0;
   const DiffBwdPlan p = diff_bwd_plan(items, heads, nq, nk, bias_share, with_dbias != 0);
-  return p.delta + p.lam + p.part;
+  return p.delta + p.part;
 }
 
 int fjx_diff_attention_bwd(const fjx_diff_attention_bwd_args* b, hipStream_t st) {
@@ -1571,6 +1572,8 @@ int fjx_diff_attention_bwd(const fjx_diff_attention_bwd_args* b, hipStream_t st)
       !diff_strides_ok(b->dk_strides, a->items, 2 * a->kv_heads, a->nk, es, true) ||
       !diff_strides_ok(b->dv_strides, a->items, a->kv_heads, a->nk, es, true))
     return fail(FJX_ERR_INVALID, "%s: the gradients' strides must be positive multiples of 16 bytes", fn);
+  if (a->bias && (a->bias_strides[2] >= 1 << 26 || (b->dbias && b->dbias_strides[2] >= 1 << 26)))
+    return fail(FJX_ERR_UNSUPPORTED, "%s: rows of the bias must be less than 2^26 elements apart", fn);
   if (b->dbias) {
     const int64_t len[3] = {a->bias ? a->items / a->bias_share : 0, a->heads, a->nq};
     for (int i = 0; i < 3; ++i)
@@ -1583,7 +1586,7 @@ int fjx_diff_attention_bwd(const fjx_diff_attention_bwd_args* b, hipStream_t st)
   const double tiles = (double)std::max(plan.chunks, 1) * a->items * a->heads * (a->nq / 64 + 1.0) * (a->nk / 64 + 1.0) /
                        (a->bias ? a->bias_share : a->items);
   if (plan.chunks && tiles >= (1 << 23)) return fail(FJX_ERR_UNSUPPORTED, "%s: more bias than one launch takes", fn);
-  const size_t need = plan.delta + plan.lam + plan.part;
+  const size_t need = plan.delta + plan.part;
   if (!a->workspace || a->workspace_bytes < need)
     return fail(FJX_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", fn, need, a->workspace_bytes);
   if (!aligned16({a->workspace})) return fail(FJX_ERR_INVALID, "%s: the workspace must be 16-byte aligned", fn);

@@ -50,7 +50,6 @@ struct DiffAttnParams {
   const float* saved;          // the forward pass's stats
   float* delta;                // [items][2 H][nq]: rowsum(P_t dP)
   float* dlam;                 // [4][H][D]
-  float* part_lam;             // [H][parts] sums of D_2, or null: few rows
   float* part_bias;            // [chunks][planes][H][nq][nk] partial sums of dbias
   int64_t chunk_items;         // items of one chunk
   int chunks;

@@ -15,31 +15,33 @@ namespace fjx {
 
 namespace {
 
-// weights of the wave's 16 rows and a block's 64 keys, one map; b: bias / scale
-template <typename T, int D>
-__device__ __forceinline__ void tile_weights(const DaTile<T, D, kDaKeys>& tile, int mp, const typename Frag<T>::type (&qf)[D / 32],
-                                             const f32x4 (&b)[4], float scale_log2, float L, int li, int lg, f32x4 (&p)[4]) {
+// weights of the wave's 16 rows and NT key tiles from row `key_w` of a block on,
+// one map; b: bias / scale
+template <typename T, int D, int ROWS, int NT>
+__device__ __forceinline__ void tile_weights(const DaTile<T, D, ROWS>& tile, int mp, int key_w,
+                                             const typename Frag<T>::type (&qf)[D / 32], const f32x4 (&b)[NT],
+                                             float scale_log2, float L, int li, int lg, f32x4 (&p)[NT]) {
 #pragma unroll
-  for (int kt = 0; kt < 4; ++kt) {
+  for (int kt = 0; kt < NT; ++kt) {
     p[kt] = b[kt];
 #pragma unroll
-    for (int c = 0; c < D / 32; ++c) mma(p[kt], load8(&tile.a[mp][16 * kt + li][32 * c + 8 * lg]), qf[c]);
+    for (int c = 0; c < D / 32; ++c) mma(p[kt], load8(&tile.a[mp][key_w + 16 * kt + li][32 * c + 8 * lg]), qf[c]);
   }
 #pragma unroll
-  for (int kt = 0; kt < 4; ++kt)
+  for (int kt = 0; kt < NT; ++kt)
 #pragma unroll
     for (int r = 0; r < 4; ++r) p[kt][r] = __builtin_amdgcn_exp2f(fmaf(p[kt][r], scale_log2, -L));
 }
 
 // dP - c of the same
-template <typename T, int D>
-__device__ __forceinline__ void tile_dp(const DaTile<T, D, kDaKeys>& tile, const typename Frag<T>::type (&dof)[2 * D / 32], float c0,
-                                        int li, int lg, f32x4 (&dp)[4]) {
+template <typename T, int D, int ROWS, int NT>
+__device__ __forceinline__ void tile_dp(const DaTile<T, D, ROWS>& tile, int key_w, const typename Frag<T>::type (&dof)[2 * D / 32],
+                                        float c0, int li, int lg, f32x4 (&dp)[NT]) {
 #pragma unroll
-  for (int kt = 0; kt < 4; ++kt) {
+  for (int kt = 0; kt < NT; ++kt) {
     dp[kt] = f32x4{-c0, -c0, -c0, -c0};
 #pragma unroll
-    for (int c = 0; c < 2 * D / 32; ++c) mma(dp[kt], load8(&tile.b[16 * kt + li][32 * c + 8 * lg]), dof[c]);
+    for (int c = 0; c < 2 * D / 32; ++c) mma(dp[kt], load8(&tile.b[key_w + 16 * kt + li][32 * c + 8 * lg]), dof[c]);
   }
 }
 
@@ -51,32 +53,40 @@ __device__ __forceinline__ void tile_dp(const DaTile<T, D, kDaKeys>& tile, const
 // near the difference that is wanted. Against a first walk for D_t alone this
 // trades a second set of scores, dP and exponentials for the products W: 52 ->
 // 26 us at 4 x 499 tokens and 6 heads, 123 -> 75 us at 245 x 245 and 2.
-template <typename T, int D>
+//
+// SPLIT: the four waves share 16 rows and take 32 keys each of a 128-key
+// block, for calls with few rows; otherwise each has rows of its own.
+template <typename T, int D, bool SPLIT>
 __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dq_kernel(DiffAttnParams<T> P) {
+  constexpr int kRows = SPLIT ? 128 : 64, kNt = SPLIT ? 2 : 4, kBufs = SPLIT ? 1 : 2;
   constexpr int kC = D / 32, kU = D / 16;
   typedef typename Frag<T>::type F;
-  typedef DaTile<T, D, kDaKeys> Tile;
-  __shared__ __attribute__((aligned(16))) Tile tiles[2];
-  __shared__ __attribute__((aligned(16))) KeyFlags<kDaKeys> flags[3];  // of the block at hand and the next two
+  typedef DaTile<T, D, kRows> Tile;
+  constexpr int kPo = D + 2;
+  static_assert(!SPLIT || sizeof(Tile) >= 4 * 2 * 16 * kPo * sizeof(float), "the waves' sums");
+  __shared__ __attribute__((aligned(16))) Tile tiles[kBufs];
+  __shared__ __attribute__((aligned(16))) KeyFlags<kRows> flags[3];  // of the block at hand and the next two
+  __shared__ float joined[4][2][16];
 
   const int t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int kvh = P.heads / P.group;
-  const uint32_t nq = (uint32_t)P.nq, rows = P.group * nq, row_blocks = (rows + 63) / 64;
+  const uint32_t nq = (uint32_t)P.nq, rows = P.group * nq, row_blocks = SPLIT ? (rows + 15) / 16 : (rows + 63) / 64;
   uint32_t id = xcd_order(blockIdx.x, gridDim.x);
   if (id >= (uint32_t)P.items * kvh * row_blocks) return;
   const uint32_t rb = id % row_blocks;
   id /= row_blocks;
   const int kv = id % (uint32_t)kvh;
   const int64_t item = id / (uint32_t)kvh;
-  const uint32_t row = rb * 64 + 16 * wave + li;
+  const uint32_t row = SPLIT ? rb * 16 + li : rb * 64 + 16 * wave + li;
   const bool row_on = row < rows;
   const uint32_t row_c = row_on ? row : rows - 1;
   const int hg = row_c / nq;
   const int64_t qi = row_c - hg * nq;
   const int head = kv * P.group + hg;
+  const int key_w = SPLIT ? 32 * wave : 0;  // this wave's keys of a block
 
-  DaStage<T, D, kDaKeys, 256> st;
+  DaStage<T, D, kRows, 256> st;
   st.init(P.k.p + item * P.k.item + 2 * kv * P.k.head, P.k.head, P.k.token, P.v.p + item * P.v.item + kv * P.v.head,
           P.v.token, t);
   const uint8_t* mask = P.mask ? P.mask + item * P.nk : nullptr;
@@ -96,14 +106,17 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dq_kernel(Diff
     dof[c] = load8(P.dout.p + item * P.dout.item + head * P.dout.head + qi * P.dout.token + 32 * c + 8 * lg);
   const float lam = da_lambda<D>(P.lam, P.heads, head, P.init, lane);
   auto key_flags = [&](int64_t blk, int at) {
-    if (t < kDaKeys) {
-      const int64_t k = blk * kDaKeys + t;
+    if (t < kRows) {
+      const int64_t k = blk * kRows + t;
       flags[at].set(t, k < P.nk && (!mask || mask[k]));
     }
   };
-  typename Quad<T>::type bv[4];
-  const int64_t blocks = (P.nk + kDaKeys - 1) / kDaKeys;
-  if (bias) bias_tile<T, 4>(bias, 4 * lg, P.nk, kDaKeys <= P.nk, bv);
+  typename Quad<T>::type bv[kNt];
+  const int64_t blocks = (P.nk + kRows - 1) / kRows;
+  auto load_bias = [&](int64_t blk) {
+    bias_tile<T, kNt>(bias, blk * kRows + key_w + 4 * lg, P.nk, (blk + 1) * kRows <= P.nk, bv);
+  };
+  if (bias) load_bias(0);
 
   key_flags(0, 0);
   key_flags(1, 1);
@@ -119,31 +132,32 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dq_kernel(Diff
 
   st.store(tiles[0]);
   __syncthreads();
-  int buf = 0, at = 0;
-  for (int64_t blk = 0; blk < blocks; ++blk, buf ^= 1) {
+  int at = 0;
+  for (int64_t blk = 0; blk < blocks; ++blk) {
+    const int buf = kBufs == 2 ? (int)blk & 1 : 0;
     const Tile& tile = tiles[buf];
     const bool more = blk + 1 < blocks;
     const int next = at == 2 ? 0 : at + 1;
-    f32x4 b[4];
+    f32x4 b[kNt];
 #pragma unroll
-    for (int kt = 0; kt < 4; ++kt)
+    for (int kt = 0; kt < kNt; ++kt)
 #pragma unroll
       for (int r = 0; r < 4; ++r) b[kt][r] = bias ? to_f32(bv[kt][r]) * P.inv_scale : 0.f;
-    flags[at].apply(0, lg, b);
+    flags[at].apply(key_w, lg, b);
     if (more) {
-      st.load((blk + 1) * kDaKeys, flags[next].whole(), flags[next].on);
-      if (bias) bias_tile<T, 4>(bias, (blk + 1) * kDaKeys + 4 * lg, P.nk, (blk + 2) * kDaKeys <= P.nk, bv);
+      st.load((blk + 1) * kRows, flags[next].whole(), flags[next].on);
+      if (bias) load_bias(blk + 1);
       key_flags(blk + 2, next == 2 ? 0 : next + 1);
     }
     at = next;
-    f32x4 dp[4], p[2][4];
-    tile_dp<T, D>(tile, dof, c0, li, lg, dp);
+    f32x4 dp[kNt], p[2][kNt];
+    tile_dp<T, D, kRows, kNt>(tile, key_w, dof, c0, li, lg, dp);
 #pragma unroll
-    for (int m = 0; m < 2; ++m) tile_weights<T, D>(tile, m, qf[m], b, P.scale_log2, L[m], li, lg, p[m]);
+    for (int m = 0; m < 2; ++m) tile_weights<T, D, kRows, kNt>(tile, m, key_w, qf[m], b, P.scale_log2, L[m], li, lg, p[m]);
     if (blk == 0) {
       float sp = 0.f, sd = 0.f;
 #pragma unroll
-      for (int kt = 0; kt < 4; ++kt)
+      for (int kt = 0; kt < kNt; ++kt)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           sp += p[0][kt][r] + p[1][kt][r];
@@ -151,16 +165,22 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dq_kernel(Diff
         }
       sp = group_sum(sp);
       sd = group_sum(sd);
+      if constexpr (SPLIT) {
+        if (lg == 0) joined[wave][0][li] = sp, joined[wave][1][li] = sd;
+        __syncthreads();
+        sp = (joined[0][0][li] + joined[1][0][li]) + (joined[2][0][li] + joined[3][0][li]);
+        sd = (joined[0][1][li] + joined[1][1][li]) + (joined[2][1][li] + joined[3][1][li]);
+      }
       c0 = sp > 0.f ? sd / sp : 0.f;
 #pragma unroll
-      for (int kt = 0; kt < 4; ++kt)
+      for (int kt = 0; kt < kNt; ++kt)
 #pragma unroll
         for (int r = 0; r < 4; ++r) dp[kt][r] -= c0;
     }
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
+      for (int c = 0; c < kNt / 2; ++c) {
         float u8[8], w8[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -173,16 +193,51 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dq_kernel(Diff
         parts(w8, wf);
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
-          const F kf = col_frag(&tile.a[m][0][0], Tile::kA, 32 * c, 16 * u, lane);
+          const F kf = col_frag(&tile.a[m][0][0], Tile::kA, key_w + 32 * c, 16 * u, lane);
           mma_parts(us[m][u], kf, uf);
           mma_parts(ws[m][u], kf, wf);
         }
       }
-    if (more) st.store(tiles[buf ^ 1]);
+    if (kBufs == 1) __syncthreads();
+    if (more) st.store(tiles[kBufs == 2 ? buf ^ 1 : 0]);
     __syncthreads();
   }
 #pragma unroll
   for (int m = 0; m < 2; ++m) Dt[m] = group_sum(Dt[m]);
+  if constexpr (SPLIT) {  // the waves' sums, through the tile's memory
+    if (lg == 0) joined[wave][0][li] = Dt[0], joined[wave][1][li] = Dt[1];
+    __syncthreads();
+    float* po = reinterpret_cast<float*>(&tiles[0]);  // [wave][map][row][D + 2]
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      Dt[m] = (joined[0][m][li] + joined[1][m][li]) + (joined[2][m][li] + joined[3][m][li]);
+#pragma unroll
+      for (int u = 0; u < kU; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) po[((wave * 2 + m) * 16 + li) * kPo + 16 * u + 4 * lg + r] = us[m][u][r] - Dt[m] * ws[m][u][r];
+    }
+    __syncthreads();
+    // each wave writes half a map
+    const int m = wave >> 1;
+    if (!row_on) return;
+    if (lg == 0 && (wave & 1) == 0) P.delta[(item * 2 * P.heads + 2 * head + m) * P.nq + qi] = Dt[m] + c0;
+    const float by = P.scale * (m ? -lam : 1.f);
+    T* out = P.dq.p + item * P.dq.item + (2 * head + m) * P.dq.head + qi * P.dq.token;
+#pragma unroll
+    for (int u = 0; u < kU / 2; ++u) {
+      const int col = 16 * ((wave & 1) * (kU / 2) + u) + 4 * lg;
+      float v[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float x = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) x += po[((w * 2 + m) * 16 + li) * kPo + col + r];
+        v[r] = x * by;
+      }
+      store4f(out + col, v);
+    }
+    return;
+  }
   if (!row_on) return;
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
@@ -199,31 +254,73 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dq_kernel(Diff
   }
 }
 
+// dlambda_h = -sum over items and queries of D_2, and the four vectors'
+// gradients from it, by one workgroup a head: the first of the launch for dk
+// and dv, in whose shadow they run.
+template <typename T, int D>
+__device__ __forceinline__ void dlambda_of(const DiffAttnParams<T>& P, int head, float (&lds)[4]) {
+  const int t = threadIdx.x;
+  const int64_t n = P.items * P.nq;
+  float s = 0.f;
+#pragma unroll 8
+  for (int64_t i = t; i < n; i += 256) {
+    const int64_t item = n >> 32 ? i / P.nq : (uint32_t)i / (uint32_t)P.nq;
+    s += P.delta[(item * 2 * P.heads + 2 * head + 1) * P.nq + i - item * P.nq];
+  }
+#pragma unroll
+  for (int x = 32; x >= 1; x >>= 1) s += shfl_xor(s, x);
+  if ((t & 63) == 0) lds[t >> 6] = s;
+  __syncthreads();
+  if (t >= 64) return;
+  const float dl = -((lds[0] + lds[1]) + (lds[2] + lds[3]));
+  float e[2];
+  da_lambda<D>(P.lam, P.heads, head, P.init, t, e);
+  if (t < D) {
+    const int64_t st = (int64_t)P.heads * D, at = (int64_t)head * D + t;
+    const float g[2] = {dl * e[0], -dl * e[1]};
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      P.dlam[2 * m * st + at] = g[m] * P.lam[(2 * m + 1) * st + at];
+      P.dlam[(2 * m + 1) * st + at] = g[m] * P.lam[2 * m * st + at];
+    }
+  }
+}
+
 // dk and dv: a wave owns 16 keys (lane l key l % 16, its k and v in registers)
 // and walks the query blocks of every head that shares them. S_t = Q_t K_t^T
 // leaves the lane 4 queries of its key a tile, the operand of dS_t^T Q_t and of
 // (P_1 - lambda P_2)^T dO as they lie. It also writes dbias, where every item has
-// a plane of its own.
-template <typename T, int D>
+// a plane of its own. SPLIT: the four waves share 16 keys and take 32 queries
+// each of a 128-query block, for calls with few keys.
+template <typename T, int D, bool SPLIT>
 __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dkv_kernel(DiffAttnParams<T> P) {
-  constexpr int kC = D / 32, kU = D / 16, kQ = kDaKeys;
+  constexpr int kC = D / 32, kU = D / 16, kQ = SPLIT ? 128 : 64, kQt = SPLIT ? 2 : 4, kBufs = SPLIT ? 1 : 2;
   typedef typename Frag<T>::type F;
   typedef DaTile<T, D, kQ> Tile;
-  __shared__ __attribute__((aligned(16))) Tile tiles[2];
-  __shared__ __attribute__((aligned(16))) float row_stat[2][4][kQ];  // L_1, L_2, D_1, D_2
+  constexpr int kPo = 4 * D + 2;
+  static_assert(!SPLIT || sizeof(Tile) >= 4 * 16 * kPo * sizeof(float), "the waves' sums");
+  __shared__ __attribute__((aligned(16))) Tile tiles[kBufs];
+  __shared__ __attribute__((aligned(16))) float row_stat[kBufs][4][kQ];  // L_1, L_2, D_1, D_2
   __shared__ float query_on[kQ];
+  __shared__ float lam_lds[4];
 
   const int t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int kvh = P.heads / P.group;
-  const uint32_t key_blocks = (P.nk + 63) / 64;
-  uint32_t id = xcd_order(blockIdx.x, gridDim.x);
+  const uint32_t key_blocks = SPLIT ? (P.nk + 15) / 16 : (P.nk + 63) / 64;
+  const uint32_t lams = (P.heads + 7) / 8 * 8;
+  if (blockIdx.x < lams) {
+    if (blockIdx.x < (uint32_t)P.heads) dlambda_of<T, D>(P, blockIdx.x, lam_lds);
+    return;
+  }
+  uint32_t id = xcd_order(blockIdx.x - lams, gridDim.x - lams);
   if (id >= (uint32_t)P.items * kvh * key_blocks) return;
   const uint32_t kb = id % key_blocks;
   id /= key_blocks;
   const int kv = id % (uint32_t)kvh;
   const int64_t item = id / (uint32_t)kvh;
-  const int64_t key = kb * 64 + 16 * wave + li;
+  const int64_t key = SPLIT ? kb * 16 + li : kb * 64 + 16 * wave + li;
+  const int q_w = SPLIT ? 32 * wave : 0;  // this wave's queries of a block
   const bool in = key < P.nk;
   const bool part = in && (!P.mask || P.mask[item * P.nk + key]);
 
@@ -243,9 +340,11 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dkv_kernel(Dif
   const float key_on = part ? INFINITY : -INFINITY;
   const bool all_on = __builtin_amdgcn_ballot_w64(part) == ~0ull;
   const int64_t plane = biased ? item / P.share : 0;
-  const T* bias = biased ? P.bias.p + plane * P.bias.item + (in ? key : 0) : nullptr;
+  const T* bias = biased ? P.bias.p + plane * P.bias.item : nullptr;
+  const uint32_t key_c = in ? (uint32_t)key : 0;
 
-  T* dbias = P.dbias.p && P.share == 1 && in ? P.dbias.p + plane * P.dbias.item + key : nullptr;
+  T* dbias = P.dbias.p && P.share == 1 ? P.dbias.p + plane * P.dbias.item : nullptr;
+  const uint32_t lane_dbias = 4 * lg * (uint32_t)P.dbias.token + key_c;
 
   const int64_t q_blocks = (P.nq + kQ - 1) / kQ;
   DaStage<T, D, kQ, 256> st;
@@ -257,26 +356,47 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dkv_kernel(Dif
   // the last block's queries, as KeyFlags::on
   if (t < kQ) query_on[t] = (q_blocks - 1) * kQ + t < P.nq ? 1.f : -1.f;
   __syncthreads();
-  float stat;
+  constexpr int kStats = 4 * kQ / 256;  // statistics that a thread stages
+  float stat[kStats];
   auto fetch = [&](int hg, int64_t qb) {
     st.src = src0 + hg * head_step;
     st.load(qb * kQ, (qb + 1) * kQ <= P.nq, query_on);
-    const int which = t >> 6;
-    const int64_t q = qb * kQ + (t & 63);
-    const int64_t at = (item * 2 * P.heads + 2 * (h0 + hg) + (which & 1)) * P.nq + q;
-    stat = which < 2 ? INFINITY : 0.f;  // past the last query: weights of zero
-    if (q < P.nq) stat = which < 2 ? P.saved[at] : P.delta[at];
+#pragma unroll
+    for (int i = 0; i < kStats; ++i) {
+      const int which = (t + 256 * i) / kQ;
+      const int64_t q = qb * kQ + (t + 256 * i) % kQ;
+      const int64_t at = (item * 2 * P.heads + 2 * (h0 + hg) + (which & 1)) * P.nq + q;
+      stat[i] = which < 2 ? INFINITY : 0.f;  // past the last query: weights of zero
+      if (q < P.nq) stat[i] = which < 2 ? P.saved[at] : P.delta[at];
+    }
   };
-  T bq[4][4];
+  auto put = [&](int buf) {
+    st.store(tiles[buf]);
+#pragma unroll
+    for (int i = 0; i < kStats; ++i) row_stat[buf][(t + 256 * i) / kQ][(t + 256 * i) % kQ] = stat[i];
+  };
+  // a lane's rows of the bias: the row of a tile and r from the loop (scalar),
+  // 4 g rows and the key on top
+  const uint32_t lane_bias = 4 * lg * (uint32_t)P.bias.token;
+  T bq[kQt][4];
   auto fetch_bias = [&](int hg, int64_t qb) {
     const T* p = bias + (h0 + hg) * P.bias.head;
+    const int64_t q0 = qb * kQ + q_w;
+    if ((qb + 1) * kQ <= P.nq) {
+      p += q0 * P.bias.token;
 #pragma unroll
-    for (int qt = 0; qt < 4; ++qt)
+      for (int qt = 0; qt < kQt; ++qt)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int64_t q = qb * kQ + 16 * qt + 4 * lg + r;
-        bq[qt][r] = p[(q < P.nq ? q : P.nq - 1) * P.bias.token];
-      }
+        for (int r = 0; r < 4; ++r) bq[qt][r] = (p + (16 * qt + r) * P.bias.token)[lane_bias + key_c];
+    } else {
+#pragma unroll
+      for (int qt = 0; qt < kQt; ++qt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int64_t q = q0 + 16 * qt + 4 * lg + r;
+          bq[qt][r] = p[(q < P.nq ? q : P.nq - 1) * P.bias.token + key_c];
+        }
+    }
   };
 
   f32x4 dk[2][kU], dv[2 * kU];
@@ -289,24 +409,24 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dkv_kernel(Dif
 
   fetch(0, 0);
   if (biased) fetch_bias(0, 0);
-  st.store(tiles[0]);
-  row_stat[0][t >> 6][t & 63] = stat;
+  put(0);
   __syncthreads();
-  int buf = 0;
+  int turn = 0;
   for (int hg = 0; hg < P.group; ++hg) {
     const float lam = da_lambda<D>(P.lam, P.heads, h0 + hg, P.init, lane);
-    for (int64_t qb = 0; qb < q_blocks; ++qb, buf ^= 1) {
+    for (int64_t qb = 0; qb < q_blocks; ++qb, turn ^= 1) {
+      const int buf = kBufs == 2 ? turn : 0;
       const Tile& tile = tiles[buf];
       const bool same = qb + 1 < q_blocks;
       const bool more = same || hg + 1 < P.group;
-      f32x4 b[4];
+      f32x4 b[kQt];
 #pragma unroll
-      for (int qt = 0; qt < 4; ++qt)
+      for (int qt = 0; qt < kQt; ++qt)
 #pragma unroll
         for (int r = 0; r < 4; ++r) b[qt][r] = biased ? to_f32(bq[qt][r]) * P.inv_scale : 0.f;
       if (!all_on) {
 #pragma unroll
-        for (int qt = 0; qt < 4; ++qt)
+        for (int qt = 0; qt < kQt; ++qt)
 #pragma unroll
           for (int r = 0; r < 4; ++r) b[qt][r] = fminf(b[qt][r], key_on);
       }
@@ -315,7 +435,7 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dkv_kernel(Dif
         if (biased) fetch_bias(same ? hg : hg + 1, same ? qb + 1 : 0);
       }
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
+      for (int c = 0; c < kQt / 2; ++c) {
         float comb[8], ds[2][8];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -325,13 +445,13 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dkv_kernel(Dif
           for (int m = 0; m < 2; ++m) {
             s[m] = b[qt];
 #pragma unroll
-            for (int x = 0; x < kC; ++x) mma(s[m], load8(&tile.a[m][16 * qt + li][32 * x + 8 * lg]), kf[m][x]);
+            for (int x = 0; x < kC; ++x) mma(s[m], load8(&tile.a[m][q_w + 16 * qt + li][32 * x + 8 * lg]), kf[m][x]);
           }
 #pragma unroll
-          for (int x = 0; x < 2 * kC; ++x) mma(dp, load8(&tile.b[16 * qt + li][32 * x + 8 * lg]), vf[x]);
+          for (int x = 0; x < 2 * kC; ++x) mma(dp, load8(&tile.b[q_w + 16 * qt + li][32 * x + 8 * lg]), vf[x]);
           f32x4 rs[4];
 #pragma unroll
-          for (int w = 0; w < 4; ++w) rs[w] = *reinterpret_cast<const f32x4*>(&row_stat[buf][w][16 * qt + 4 * lg]);
+          for (int w = 0; w < 4; ++w) rs[w] = *reinterpret_cast<const f32x4*>(&row_stat[buf][w][q_w + 16 * qt + 4 * lg]);
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const float p1 = __builtin_amdgcn_exp2f(fmaf(s[0][r], P.scale_log2, -rs[0][r]));
@@ -340,12 +460,12 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dkv_kernel(Dif
             ds[0][4 * j + r] = p1 * (dp[r] - rs[2][r]);
             ds[1][4 * j + r] = p2 * (rs[3][r] - dp[r]);
           }
-          if (dbias) {
-            const int64_t q = qb * kQ + 16 * qt + 4 * lg;
+          if (dbias && in) {
+            const int64_t q = qb * kQ + q_w + 16 * qt;
             T* p = dbias + (h0 + hg) * P.dbias.head + q * P.dbias.token;
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-              if (q + r < P.nq) p[r * P.dbias.token] = from_f32<T>(ds[0][4 * j + r] + ds[1][4 * j + r]);
+              if (q + 4 * lg + r < P.nq) (p + r * P.dbias.token)[lane_dbias] = from_f32<T>(ds[0][4 * j + r] + ds[1][4 * j + r]);
           }
         }
         F cf[kParts<T>], df0[kParts<T>], df1[kParts<T>];
@@ -353,19 +473,43 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dkv_kernel(Dif
         parts(ds[0], df0);
         parts(ds[1], df1);
 #pragma unroll
-        for (int u = 0; u < 2 * kU; ++u) mma_parts(dv[u], col_frag(&tile.b[0][0], Tile::kB, 32 * c, 16 * u, lane), cf);
+        for (int u = 0; u < 2 * kU; ++u) mma_parts(dv[u], col_frag(&tile.b[0][0], Tile::kB, q_w + 32 * c, 16 * u, lane), cf);
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
-          mma_parts(dk[0][u], col_frag(&tile.a[0][0][0], Tile::kA, 32 * c, 16 * u, lane), df0);
-          mma_parts(dk[1][u], col_frag(&tile.a[1][0][0], Tile::kA, 32 * c, 16 * u, lane), df1);
+          mma_parts(dk[0][u], col_frag(&tile.a[0][0][0], Tile::kA, q_w + 32 * c, 16 * u, lane), df0);
+          mma_parts(dk[1][u], col_frag(&tile.a[1][0][0], Tile::kA, q_w + 32 * c, 16 * u, lane), df1);
         }
       }
-      if (more) {
-        st.store(tiles[buf ^ 1]);
-        row_stat[buf ^ 1][t >> 6][t & 63] = stat;
-      }
+      if (kBufs == 1) __syncthreads();
+      if (more) put(kBufs == 2 ? buf ^ 1 : 0);
       __syncthreads();
     }
+  }
+  if constexpr (SPLIT) {  // the waves' sums, through the tile's memory: [wave][key][dk_1, dk_2, dv]
+    float* po = reinterpret_cast<float*>(&tiles[0]);
+    float* own = po + (wave * 16 + li) * kPo + 4 * lg;
+#pragma unroll
+    for (int u = 0; u < 4 * kU; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) own[16 * u + r] = u < 2 * kU ? dk[u / kU][u % kU][r] : dv[u < 2 * kU ? 0 : u - 2 * kU][r];
+    __syncthreads();
+    if (!in) return;
+    // wave 0 writes dk_1, wave 1 dk_2, the others half of dv each
+    T* out = wave < 2 ? P.dk.p + item * P.dk.item + (2 * kv + wave) * P.dk.head + key * P.dk.token
+                      : P.dv.p + item * P.dv.item + kv * P.dv.head + key * P.dv.token + (wave - 2) * D;
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      float v[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float x = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) x += po[(w * 16 + li) * kPo + wave * D + 16 * u + 4 * lg + r];
+        v[r] = wave < 2 ? x * P.scale : x;
+      }
+      store4f(out + 16 * u + 4 * lg, v);
+    }
+    return;
   }
   if (!in) return;
 #pragma unroll
@@ -486,11 +630,11 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dbias_kernel(D
       key_flags(item + 2, at == 2 ? 0 : at + 1);
     }
     f32x4 dp[4];
-    tile_dp<T, D>(tile, dof, 0.f, li, lg, dp);
+    tile_dp<T, D, kDaKeys, 4>(tile, 0, dof, 0.f, li, lg, dp);
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
       f32x4 p[4];
-      tile_weights<T, D>(tile, m, qf[m], b, P.scale_log2, rs[m], li, lg, p);
+      tile_weights<T, D, kDaKeys, 4>(tile, m, 0, qf[m], b, P.scale_log2, rs[m], li, lg, p);
       const float by = m ? -lam : 1.f;
 #pragma unroll
       for (int kt = 0; kt < 4; ++kt)
@@ -515,90 +659,42 @@ __global__ __launch_bounds__(256) void diffattn_bias_sum_kernel(DiffAttnParams<T
   const int64_t per = P.items / P.share * P.heads * P.nq * P.nk;
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < per; i += gridDim.x * 256ll) {
     float s = 0.f;
+#pragma unroll 8
     for (int c = 0; c < P.chunks; ++c) s += P.part_bias[c * per + i];
     const int64_t k = i % P.nk, q = i / P.nk % P.nq, ph = i / (P.nk * P.nq);
     P.dbias.p[ph / P.heads * P.dbias.item + ph % P.heads * P.dbias.head + q * P.dbias.token + k] = from_f32<T>(s);
   }
 }
 
-// dlambda_h = -sum over items and queries of D_2, and the four vectors'
-// gradients from it. One workgroup a head; of many rows, kLamParts workgroups a
-// head leave their sums in `part_lam` first.
-constexpr int kLamParts = 32;
-__device__ __forceinline__ float lam_sum(const float* delta, int64_t items, int heads, int head, int64_t nq, int part,
-                                         int parts, float* lds) {
-  const int t = threadIdx.x;
-  const int64_t n = items * nq, per = (n + parts - 1) / parts;
-  const int64_t end = (part + 1) * per < n ? (part + 1) * per : n;
-  float s = 0.f;
-#pragma unroll 4
-  for (int64_t i = part * per + t; i < end; i += 1024) {
-    const int64_t item = n >> 32 ? i / nq : (uint32_t)i / (uint32_t)nq;
-    s += delta[(item * 2 * heads + 2 * head + 1) * nq + i - item * nq];
-  }
-#pragma unroll
-  for (int x = 32; x >= 1; x >>= 1) s += shfl_xor(s, x);
-  if ((t & 63) == 0) lds[t >> 6] = s;
-  __syncthreads();
-  s = 0.f;
-#pragma unroll
-  for (int w = 0; w < 16; ++w) s += lds[w];
-  return s;
-}
-__global__ __launch_bounds__(1024) void diffattn_lam_parts_kernel(const float* delta, float* part, int64_t items, int heads,
-                                                                  int64_t nq) {
-  __shared__ float lds[16];
-  const int head = blockIdx.x / kLamParts, p = blockIdx.x % kLamParts;
-  const float s = lam_sum(delta, items, heads, head, nq, p, kLamParts, lds);
-  if (threadIdx.x == 0) part[blockIdx.x] = s;
-}
-template <typename T, int D>
-__global__ __launch_bounds__(1024) void diffattn_dlam_kernel(DiffAttnParams<T> P) {
-  __shared__ float lds[16];
-  const int t = threadIdx.x, head = blockIdx.x;
-  float dl = 0.f;
-  if (P.part_lam) {
-#pragma unroll
-    for (int p = 0; p < kLamParts; ++p) dl -= P.part_lam[head * kLamParts + p];
-  } else {
-    dl = -lam_sum(P.delta, P.items, P.heads, head, P.nq, 0, 1, lds);
-  }
-  if (t >= 64) return;
-  float e[2];
-  da_lambda<D>(P.lam, P.heads, head, P.init, t, e);
-  if (t < D) {
-    const int64_t st = (int64_t)P.heads * D, at = (int64_t)head * D + t;
-    const float g[2] = {dl * e[0], -dl * e[1]};
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      P.dlam[2 * m * st + at] = g[m] * P.lam[(2 * m + 1) * st + at];
-      P.dlam[(2 * m + 1) * st + at] = g[m] * P.lam[2 * m * st + at];
-    }
-  }
-}
-
+#ifndef DA_SPLITQ
+#define DA_SPLITQ 192
+#define DA_SPLITK 224
+#endif
 unsigned eights(int64_t blocks) { return (unsigned)((blocks + 7) / 8 * 8); }
 
 template <typename T, int D>
 void bwd(const DiffAttnParams<T>& P, hipStream_t st) {
   const int64_t kvh = P.heads / P.group;
-  diffattn_dq_kernel<T, D><<<eights(P.items * kvh * ((P.group * P.nq + 63) / 64)), 256, 0, st>>>(P);
-  diffattn_dkv_kernel<T, D><<<eights(P.items * kvh * ((P.nk + 63) / 64)), 256, 0, st>>>(P);
+  // waves with rows (keys) of their own read each block once for 64 of them;
+  // they share 16 where that leaves fewer workgroups than two a CU
+  const int64_t heads = P.items * kvh, rows = P.group * P.nq;
+  if (heads * ((rows + 63) / 64) >= DA_SPLITQ)
+    diffattn_dq_kernel<T, D, false><<<eights(heads * ((rows + 63) / 64)), 256, 0, st>>>(P);
+  else
+    diffattn_dq_kernel<T, D, true><<<eights(heads * ((rows + 15) / 16)), 256, 0, st>>>(P);
+  if (heads * ((P.nk + 63) / 64) >= DA_SPLITK)
+    diffattn_dkv_kernel<T, D, false><<<eights(P.heads) + eights(heads * ((P.nk + 63) / 64)), 256, 0, st>>>(P);
+  else
+    diffattn_dkv_kernel<T, D, true><<<eights(P.heads) + eights(heads * ((P.nk + 15) / 16)), 256, 0, st>>>(P);
   if (P.dbias.p && P.share > 1) {
     const int64_t planes = P.items / P.share;
     diffattn_dbias_kernel<T, D><<<eights(planes * P.heads * P.chunks * ((P.nk + 63) / 64) * ((P.nq + 63) / 64)), 256, 0, st>>>(P);
     const int64_t blocks = (planes * P.heads * P.nq * P.nk + 255) / 256;
     diffattn_bias_sum_kernel<T><<<(unsigned)(blocks < 8192 ? blocks : 8192), 256, 0, st>>>(P);
   }
-  if (P.part_lam) diffattn_lam_parts_kernel<<<P.heads * kLamParts, 1024, 0, st>>>(P.delta, P.part_lam, P.items, P.heads, P.nq);
-  diffattn_dlam_kernel<T, D><<<P.heads, 1024, 0, st>>>(P);
 }
 
 }  // namespace
-
-size_t diffattn_lam_floats(int64_t items, int heads, int64_t nq) {
-  return items * nq > 8192 ? (size_t)heads * kLamParts : 0;
-}
 
 template <typename T>
 void launch_diffattn_bwd(const DiffAttnParams<T>& P, int d, hipStream_t st) {

@@ -339,8 +339,6 @@ template <typename T>
 struct DiffAttnParams;
 template <typename T>
 void launch_diffattn_fwd(const DiffAttnParams<T>& P, int d, bool keywise, hipStream_t st);
-// floats of DiffAttnParams::part_lam; 0: it stays null
-size_t diffattn_lam_floats(int64_t items, int heads, int64_t nq);
 template <typename T>
 void launch_diffattn_bwd(const DiffAttnParams<T>& P, int d, hipStream_t st);
 

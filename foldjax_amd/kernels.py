@@ -905,21 +905,21 @@ def rms_norm(
     kind = _CODES.get(codes) if codes is None or isinstance(codes, str) else None
     if kind is None:
         raise ValueError(f"codes must be None, 'e4m3' or 'int8', got {codes!r}")
-    _same_device(x, weight=weight, residual=residual, out=out, sum_out=sum_out)
-    code = _code(x.dtype)
-    _need_dtype(x.dtype, weight=weight, residual=residual)
-    if x.dim() < 1:
+    dtype, shape = x.dtype, x.shape
+    code = _code(dtype)
+    _same_place(x, dtype, weight=weight, residual=residual)
+    if not shape:
         raise ValueError("x must have a last axis to be normalised over")
-    c = int(x.shape[-1])
+    c = shape[-1]
     _need_shape("weight", weight, (c,))
     if residual is not None:
-        _need_shape("residual", residual, x.shape)
+        _need_shape("residual", residual, shape)
     elif sum_out is not None:
         raise ValueError("sum_out needs a residual")
     if group and codes is None:
         raise ValueError("group needs codes")
     _dev(x)
-    xf, res = x.contiguous(), None if residual is None else residual.contiguous()
+    xf, res = _like(x, dtype), _like(residual, dtype)
     scales = None
     if codes is None:
         y = _out_buffer(out, x, xf)
@@ -928,18 +928,18 @@ def rms_norm(
             raise ValueError("out is for a norm without codes")
         if group < 0 or (group and c % group):
             raise ValueError(f"group must divide the {c} channels, got {group}")
-        y = torch.empty(x.shape, dtype=kind[1], device=x.device)
-        scales = torch.empty(tuple(x.shape[:-1]) + (c // group if group else 1,), dtype=torch.float32, device=x.device)
+        y = torch.empty(shape, dtype=kind[1], device=x.device)
+        scales = torch.empty(shape[:-1] + (c // group if group else 1,), dtype=torch.float32, device=x.device)
     h = None if res is None else _out_buffer(sum_out, x, xf)
     if h is not None and h.data_ptr() == y.data_ptr():
         raise ValueError("out and sum_out must be two buffers")
-    w = weight.contiguous()
-    a = _lib.RmsNormArgs(rows=x.numel() // max(c, 1), c=c, dtype=code, eps=float(eps), x=_ptr(xf), residual=_ptr(res),
-                         weight=_ptr(w), sum_out=_ptr(h), out=_ptr(y), codes=kind[0], group=group, scales=_ptr(scales))
+    w = _like(weight, dtype)
+    a = _lib.RmsNormArgs(x.numel() // max(c, 1), c, code, eps, xf.data_ptr(), _ptr(res), w.data_ptr(), _ptr(h), y.data_ptr(),
+                         kind[0], group, _ptr(scales))
     _launch(_lib.load().fjx_rms_norm_fwd, a, x)
-    got = (y,) if scales is None else (y, scales)
-    got = got if h is None else got + (h,)
-    return got if len(got) > 1 else y
+    if scales is not None:
+        return (y, scales) if h is None else (y, scales, h)
+    return y if h is None else (y, h)
 
 
 def rms_norm_backward(
@@ -956,19 +956,17 @@ def rms_norm_backward(
     gradient too and includes ``dh``, what reaches h from elsewhere; dweight is
     float32, summed over the rows in one order. ``out``: write dx into this
     tensor, which may be ``dy`` or ``dh``."""
-    _same_device(h, dy=dy, weight=weight, dh=dh, out=out)
-    code = _code(h.dtype)
-    _need_dtype(h.dtype, dy=dy, weight=weight, dh=dh)
-    if h.dim() < 1:
+    dtype, shape = h.dtype, h.shape
+    code = _code(dtype)
+    _same_place(h, dtype, dy=dy, weight=weight, dh=dh)
+    if not shape:
         raise ValueError("h must have a last axis")
-    c = int(h.shape[-1])
+    c = shape[-1]
     _need_shape("weight", weight, (c,))
-    _need_shape("dy", dy, h.shape)
-    _need_shape("dh", dh, h.shape)
+    _need_shape("dy", dy, shape)
+    _need_shape("dh", dh, shape)
     _dev(h)
-    hf, dyf = h.contiguous(), dy.contiguous()
-    dhf = None if dh is None else dh.contiguous()
-    w = weight.contiguous()
+    hf, dyf, dhf, w = _like(h, dtype), _like(dy, dtype), _like(dh, dtype), _like(weight, dtype)
     if out is not None and out.data_ptr() == h.data_ptr():
         raise ValueError("out must not be h")
     dx = _out_buffer(out, h, hf)
@@ -977,8 +975,8 @@ def rms_norm_backward(
     rows = h.numel() // max(c, 1)
     nbytes = lib.fjx_rms_norm_bwd_workspace_size(rows, c)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=h.device)
-    a = _lib.RmsNormBwdArgs(rows=rows, c=c, dtype=code, eps=float(eps), dy=_ptr(dyf), h=_ptr(hf), weight=_ptr(w),
-                            dh=_ptr(dhf), dx=_ptr(dx), dweight=_ptr(dw), workspace=_ptr(ws), workspace_bytes=nbytes)
+    a = _lib.RmsNormBwdArgs(rows, c, code, eps, dyf.data_ptr(), hf.data_ptr(), w.data_ptr(), _ptr(dhf), dx.data_ptr(),
+                            dw.data_ptr(), ws.data_ptr(), nbytes)
     _launch(lib.fjx_rms_norm_bwd, a, h)
     return dx, dw
 
@@ -1010,31 +1008,32 @@ def dropout_add(
     one element on x's device, read by the kernel and added to ``offset``: a
     captured call then drops anew at each replay. ``out``: write into this
     tensor, which may be ``x`` and/or ``residual``."""
-    _same_device(x, residual=residual, out_mask=out_mask, step=step, out=out)
-    code = _code(x.dtype)
-    _need_dtype(x.dtype, residual=residual)
-    if x.dim() < 1:
+    dtype, shape = x.dtype, x.shape
+    code = _code(dtype)
+    _same_place(x, dtype, residual=residual)
+    dims = len(shape)
+    if not dims:
         raise ValueError("x must have a last axis")
     flags = 0
     for axis in shared:
-        if axis not in _SHARE or x.dim() < -axis:
-            raise ValueError(f"shared must name axes of x among -3, -2 and -1, got {shared!r} for {tuple(x.shape)}")
+        if axis not in _SHARE or dims < -axis:
+            raise ValueError(f"shared must name axes of x among -3, -2 and -1, got {shared!r} for {tuple(shape)}")
         flags |= _SHARE[axis]
     if residual is not None:
-        _need_shape("residual", residual, x.shape)
-    for name, n in (("seed", seed), ("offset", offset)):
-        if not 0 <= n < 2**64:
-            raise ValueError(f"{name} must be in [0, 2^64), got {n}")
+        _need_shape("residual", residual, shape)
+    if not (0 <= seed < 2**64 and 0 <= offset < 2**64):
+        raise ValueError(f"seed and offset must be in [0, 2^64), got {seed} and {offset}")
+    if out_mask is not None or step is not None:
+        _same_device(x, out_mask=out_mask, step=step)
     if step is not None and (step.dtype is not torch.int64 or step.numel() != 1):
         raise ValueError(f"step must be an int64 tensor of one element, got {step.dtype} {tuple(step.shape)}")
     _dev(x)
-    xf, res = x.contiguous(), None if residual is None else residual.contiguous()
-    om = _rows_of(out_mask, x.shape[:-1], x.dtype, "out_mask")
+    xf, res = _like(x, dtype), _like(residual, dtype)
+    om = None if out_mask is None else _rows_of(out_mask, shape[:-1], dtype, "out_mask")
     out = _out_buffer(out, x, xf)
-    n, m, c = (1, 1, *(int(v) for v in x.shape))[-3:]
-    a = _lib.DropoutArgs(batch=x.numel() // max(n * m * c, 1), n=n, m=m, c=c, dtype=code, shared=flags, p=float(p),
-                         seed=seed, offset=offset, step=_ptr(step), x=_ptr(xf), residual=_ptr(res), out_mask=_ptr(om),
-                         out=_ptr(out))
+    n, m, c = shape[-3:] if dims > 2 else (1, 1, *shape)[-3:]
+    a = _lib.DropoutArgs(x.numel() // max(n * m * c, 1), n, m, c, code, flags, p, seed, offset, _ptr(step), xf.data_ptr(),
+                         _ptr(res), _ptr(om), out.data_ptr())
     _launch(_lib.load().fjx_dropout_fwd, a, x)
     return out
 
