@@ -254,6 +254,8 @@ void by_width(int c, F f) {
 int rmsnorm_bwd_blocks(int64_t rows, int c) {
   int64_t blocks = 0;
   by_width(c, [&](auto team, auto) { blocks = (rows * team.value + 255) / 256; });
+  // a row a team while that leaves a workgroup a CU, then two and more
+  if (blocks > 256) blocks = blocks / 2 > 256 ? blocks / 2 : 256;
   return (int)(blocks < 1024 ? blocks : 1024);
 }
 
