@@ -177,13 +177,17 @@ def pairformer_layer_forward(
     attention_backend: str = "xla",
     triangle_backend: str = DEFAULT_BACKEND,
     glu_backend: str = "xla",
+    *,
+    dropout=None,
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """Boltz-2 ``pairformer_layer_forward`` (``B2K/pairformer.py:100-206``):
     every residual is fused into the producing kernel. ``params`` is the
-    Boltz-2 layer dict, or a ``foldjax_amd.pairformer.PairformerLayerWeights``."""
+    Boltz-2 layer dict, or a ``foldjax_amd.pairformer.PairformerLayerWeights``.
+    ``dropout``: a ``foldjax_amd.pairformer.PairDropout`` of the four triangle
+    updates."""
     w = _packed_layer(params, s, z)
     _check_layer_selectors(matmul_precision, triangle_backend)
-    return w.forward(s, z, mask, pair_mask, eps=eps)
+    return w.forward(s, z, mask, pair_mask, eps=eps, dropout=dropout)
 
 
 def _packed_layer(params, s: torch.Tensor, z: torch.Tensor):
@@ -276,6 +280,8 @@ def pairformer_module_forward(
     attention_backend: str = "xla",
     triangle_backend: str = DEFAULT_BACKEND,
     glu_backend: str = "xla",
+    *,
+    dropout=None,
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """Boltz-2 ``pairformer_module_forward`` (``B2K/pairformer.py:30-97``):
     the layers of ``params["layers"]`` applied in order, each one
@@ -288,11 +294,15 @@ def pairformer_module_forward(
     while every layer here streams through fused kernels with a fixed
     workspace. As the reference's scan donates its carry
     (``B2K/pairformer.py:74-96``), the first layer writes new s and z and
-    every later layer updates those in place."""
+    every later layer updates those in place. ``dropout``: a
+    ``foldjax_amd.pairformer.PairDropout`` of every layer's triangle updates."""
+    from foldjax_amd.pairformer import _block_dropout
+
     layers = params["layers"]
     if use_scan:
         layers = stack_layer_params(layers, z.dtype, z.device, single_dtype=s.dtype)
     _check_layer_selectors(matmul_precision, triangle_backend)
     for idx, layer in enumerate(layers):
-        s, z = _packed_layer(layer, s, z).forward(s, z, mask, pair_mask, eps=eps, donate=idx > 0)
+        s, z = _packed_layer(layer, s, z).forward(s, z, mask, pair_mask, eps=eps, donate=idx > 0,
+                                                  dropout=_block_dropout(dropout, idx))
     return s, z

@@ -19,7 +19,7 @@ import torch
 
 from foldjax_amd import kernels
 from foldjax_amd.kernels import SingleAttentionWeights, TransitionWeights, TriAttnWeights, TriMulWeights
-from foldjax_amd.pairformer import PairformerLayerWeights
+from foldjax_amd.pairformer import PairDropout, PairformerLayerWeights, _block_dropout
 from foldjax_amd.params import OpenFold3AttentionPairBiasParams as AttentionPairBiasParams
 from foldjax_amd.params import OpenFold3PairBlockParams as PairBlockParams
 from foldjax_amd.params import OpenFold3PairformerBlockParams as PairformerBlockParams
@@ -178,26 +178,28 @@ def pairformer_block(
     mask_transition: bool = True,
     eps: float = 1e-5,
     chunk_size: int | None = None,
+    dropout: PairDropout | None = None,
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """OpenFold3 ``pairformer_block`` (``OF3/pairformer.py:42-102``): z through
     the pair block, then s += attention with pair bias over the updated z
     and s += SwiGLU transition (update times ``single_mask`` when
     ``mask_transition``). ``params`` is a ``PairformerBlockParams`` or a packed
     ``PairformerLayerWeights``. When s and z share a dtype the attention's
-    pair bias comes out of the pair transition's epilogue."""
+    pair bias comes out of the pair transition's epilogue. ``dropout`` drops the
+    four triangle updates."""
     if chunk_size is not None and chunk_size <= 0:
         raise ValueError(f"chunk_size must be positive, got {chunk_size}")
     return _block_forward(s, z, params, single_mask, pair_mask, no_heads_pair, no_heads_pair_bias, inf,
-                          mask_transition, eps, donate=False)
+                          mask_transition, eps, donate=False, dropout=dropout)
 
 
 def _block_forward(s, z, params, single_mask, pair_mask, no_heads_pair, no_heads_pair_bias, inf, mask_transition,
-                   eps, *, donate):
+                   eps, *, donate, dropout):
     block = params if isinstance(params, PairformerLayerWeights) else PairformerLayerWeights.from_openfold3(
         params, z.dtype, z.device, single_dtype=s.dtype)
     _check_block_heads(block, no_heads_pair, no_heads_pair_bias)
     return block.forward_openfold3(s, z, single_mask, pair_mask, inf=inf, mask_transition=mask_transition, eps=eps,
-                                   donate=donate)
+                                   donate=donate, dropout=dropout)
 
 
 def can_scan(blocks) -> bool:
@@ -221,12 +223,14 @@ def pairformer_stack(
     eps: float = 1e-5,
     chunk_size: int | None = None,
     scan_blocks: bool = True,
+    dropout: PairDropout | None = None,
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """OpenFold3 ``pairformer_stack`` (``OF3/pairformer.py:105-171``): every
     block in order. ``params`` is a ``PairformerStackParams`` or a
     ``StackedLayers`` of packed blocks. Blocks are packed once; with
     ``scan_blocks`` a stackable list runs from one pre-stacked set of weights
-    (``_scan_blocks``), otherwise block by block. The kernels are the same."""
+    (``_scan_blocks``), otherwise block by block. The kernels are the same.
+    ``dropout`` drops every block's triangle updates."""
     blocks = params if isinstance(params, StackedLayers) else params.blocks
     if not isinstance(blocks, StackedLayers):
         blocks = [b if isinstance(b, PairformerLayerWeights)
@@ -240,5 +244,5 @@ def pairformer_stack(
     # place (the reference's scan donates its carry)
     for idx, block in enumerate(blocks):
         s, z = _block_forward(s, z, block, single_mask, pair_mask, no_heads_pair, no_heads_pair_bias, inf,
-                              mask_transition, eps, donate=idx > 0)
+                              mask_transition, eps, donate=idx > 0, dropout=_block_dropout(dropout, idx))
     return s, z

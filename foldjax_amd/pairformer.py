@@ -10,13 +10,45 @@ transition.
 
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 
 import torch
 
 from foldjax_amd import kernels
 from foldjax_amd import params as P
 from foldjax_amd import synthetic as syn
+
+
+@dataclass(frozen=True)
+class PairDropout:
+    """Dropout of the pair track's four triangle updates before they are added
+    to z, as the Pairformer is trained, and as it is left on to sample
+    structures: ``p`` of each update's mask entries are dropped. ``shared``:
+    the axes over which one entry serves, (-3,) for all rows (the ending node,
+    which works on the transposed grid, swaps -3 and -2), with -1 for all
+    channels too. A block draws its masks at ``offset`` .. ``offset + 3`` of the
+    generator of ``seed``, the block l of a stack 4 l further on; ``step`` (an
+    int64 device tensor) is added where the kernels run, so that a captured
+    block drops anew at each replay."""
+
+    p: float = 0.25
+    seed: int = 0
+    offset: int = 0
+    step: torch.Tensor | None = None
+    shared: tuple[int, ...] = (-3,)
+
+    def of_block(self, index: int) -> "PairDropout":
+        return replace(self, offset=self.offset + 4 * index)
+
+    def add(self, update: torch.Tensor, z: torch.Tensor, sublayer: int, ending: bool, out_mask, out) -> torch.Tensor:
+        """z + the dropped update, into ``out`` (or the update itself)."""
+        shared = tuple({-3: -2, -2: -3}.get(a, a) for a in self.shared) if ending else self.shared
+        return kernels.dropout_add(update, p=self.p, seed=self.seed, offset=self.offset + sublayer, step=self.step,
+                                   residual=z, shared=shared, out_mask=out_mask, out=update if out is None else out)
+
+
+def _block_dropout(dropout: PairDropout | None, index: int) -> PairDropout | None:
+    return None if dropout is None else dropout.of_block(index)
 
 
 @dataclass
@@ -28,7 +60,7 @@ class TriangleSublayers:
 
     def forward(self, z: torch.Tensor, mask: torch.Tensor | None, *, inf: float = 1e9, eps: float = 1e-5,
                 out_mask: torch.Tensor | None = None, tri_mul_first: bool = True,
-                donate: bool = False) -> torch.Tensor:
+                donate: bool = False, dropout: PairDropout | None = None) -> torch.Tensor:
         """z += each sublayer in turn (the residual fused into its epilogue);
         with ``out_mask`` every sublayer's output is multiplied by
         ``out_mask != 0`` (Protenix's ``z * pair_gate``). ``tri_mul_first``
@@ -41,7 +73,8 @@ class TriangleSublayers:
         tensor. ``donate``: the caller gives up ``z`` (a contiguous tensor it
         no longer reads, as the reference's scan donates its carry,
         ``B2K/pairformer.py:74-96``), and the first sublayer overwrites it as
-        well."""
+        well. ``dropout``: each update goes into a tensor of its own, and comes to
+        z through ``kernels.dropout_add``."""
         first = [True]
 
         def dest(z):
@@ -52,17 +85,21 @@ class TriangleSublayers:
                 return z if donate and z.is_contiguous() else None
             return z
 
+        def add(z, sublayer, ending, call):
+            # z + call's update
+            if dropout is None:
+                return call(z, residual=z, out_mask=out_mask, out=dest(z))
+            return dropout.add(call(z), z, sublayer, ending, out_mask, dest(z))
+
         def mul_pair(z):
-            z = kernels.trimul(z, mask, self.tri_mul_out, "outgoing", eps=eps, residual=z, out_mask=out_mask,
-                               out=dest(z))
-            return kernels.trimul(z, mask, self.tri_mul_in, "incoming", eps=eps, residual=z, out_mask=out_mask,
-                                  out=dest(z))
+            z = add(z, 0, False, lambda z, **k: kernels.trimul(z, mask, self.tri_mul_out, "outgoing", eps=eps, **k))
+            return add(z, 1, False, lambda z, **k: kernels.trimul(z, mask, self.tri_mul_in, "incoming", eps=eps, **k))
 
         def att_pair(z):
-            z = kernels.triattn(z, mask, self.tri_att_start, starting=True, inf=inf, eps=eps, residual=z,
-                                out_mask=out_mask, out=dest(z))
-            return kernels.triattn(z, mask, self.tri_att_end, starting=False, inf=inf, eps=eps, residual=z,
-                                   out_mask=out_mask, out=dest(z))
+            z = add(z, 2, False, lambda z, **k: kernels.triattn(z, mask, self.tri_att_start, starting=True, inf=inf,
+                                                                eps=eps, **k))
+            return add(z, 3, True, lambda z, **k: kernels.triattn(z, mask, self.tri_att_end, starting=False, inf=inf,
+                                                                  eps=eps, **k))
 
         return att_pair(mul_pair(z)) if tri_mul_first else mul_pair(att_pair(z))
 
@@ -118,7 +155,8 @@ class PairformerLayerWeights:
         return s if donate and s is not None and s.is_contiguous() else None
 
     def forward(self, s: torch.Tensor, z: torch.Tensor, mask: torch.Tensor | None, pair_mask: torch.Tensor | None,
-                eps: float = 1e-5, *, donate: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+                eps: float = 1e-5, *, donate: bool = False,
+                dropout: PairDropout | None = None) -> tuple[torch.Tensor, torch.Tensor]:
         """Boltz-2 ``pairformer_layer_forward`` (``B2K/pairformer.py:133-205``):
         z += tri-mul out, in, tri-attn start, end, transition; s +=
         attention(LN(s), z, mask); s += transition_s. The attention's pair
@@ -126,8 +164,9 @@ class PairformerLayerWeights:
         float32 when s is float32 over a bfloat16 z), so z is not read a
         further time. The block allocates one pair tensor and one single
         tensor for its outputs and updates them in place; with ``donate`` it
-        allocates neither and overwrites s and z (``TriangleSublayers.forward``)."""
-        z = self.triangle.forward(z, pair_mask, eps=eps, donate=donate)
+        allocates neither and overwrites s and z (``TriangleSublayers.forward``);
+        ``dropout`` as there."""
+        z = self.triangle.forward(z, pair_mask, eps=eps, donate=donate, dropout=dropout)
         z, bias = self._pair_transition(z, s, eps=eps)
         s = kernels.single_attention(s, None if bias is not None else z, mask, self.attention, residual=s, eps=eps,
                                      pair_bias=bias, out=self._s_dest(s, donate))
@@ -135,7 +174,7 @@ class PairformerLayerWeights:
         return s, z
 
     def forward_protenix(self, s: torch.Tensor | None, z: torch.Tensor,
-                         pair_mask: torch.Tensor | None, *, donate: bool = False
+                         pair_mask: torch.Tensor | None, *, donate: bool = False, dropout: PairDropout | None = None
                          ) -> tuple[torch.Tensor | None, torch.Tensor]:
         """Protenix ``pairformer_block`` (``PXK/pairformer.py:49-180``). Every
         sublayer's output is multiplied by ``pair_gate = bool(pair_mask)``
@@ -146,13 +185,13 @@ class PairformerLayerWeights:
         pair mask) is the single attention's key mask with ``inf = 1e10`` and
         gates its output and the single transition's; the reference's extra
         bias ``-1e10`` on invalid query rows changes only rows that the gate
-        then zeroes. ``donate`` as for ``forward``."""
+        then zeroes. ``donate`` and ``dropout`` as for ``forward``."""
         valid = None
         if pair_mask is not None:
             valid = torch.diagonal(pair_mask, dim1=-2, dim2=-1).ne(0)
             if s is not None:
                 valid = valid.to(s.dtype)  # once for the attention's two masks and the transition's
-        z = self.triangle.forward(z, pair_mask, out_mask=pair_mask, donate=donate)
+        z = self.triangle.forward(z, pair_mask, out_mask=pair_mask, donate=donate, dropout=dropout)
         z, bias = self._pair_transition(z, s, out_mask=pair_mask)
         if self.attention is None:
             if s is not None and valid is not None:
@@ -169,13 +208,14 @@ class PairformerLayerWeights:
 
     def forward_openfold3(self, s: torch.Tensor, z: torch.Tensor, single_mask: torch.Tensor | None,
                           pair_mask: torch.Tensor | None, *, inf: float = 1e9, mask_transition: bool = True,
-                          eps: float = 1e-5, donate: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+                          eps: float = 1e-5, donate: bool = False,
+                          dropout: PairDropout | None = None) -> tuple[torch.Tensor, torch.Tensor]:
         """OpenFold3 ``pairformer_block`` (``OF3/pairformer.py:42-102``): the
         pair block (``OF3/pair_block.py:106-190``), then s += attention with
         pair bias (key mask ``single_mask``, ``inf``) and the SwiGLU single
         transition, whose update is multiplied by ``single_mask`` when
-        ``mask_transition``. ``donate`` as for ``forward``."""
-        z = self.triangle.forward(z, pair_mask, inf=inf, eps=eps, donate=donate)
+        ``mask_transition``. ``donate`` and ``dropout`` as for ``forward``."""
+        z = self.triangle.forward(z, pair_mask, inf=inf, eps=eps, donate=donate, dropout=dropout)
         z, bias = self._pair_transition(z, s, row_mask=pair_mask if mask_transition else None, eps=eps)
         s = kernels.single_attention(s, None if bias is not None else z, single_mask, self.attention, inf=inf,
                                      eps=eps, residual=s, pair_bias=bias, out=self._s_dest(s, donate))

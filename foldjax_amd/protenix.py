@@ -26,7 +26,7 @@ import torch
 
 from foldjax_amd import kernels
 from foldjax_amd.kernels import SingleAttentionWeights, TransitionWeights, TriAttnWeights, TriMulWeights
-from foldjax_amd.pairformer import PairformerLayerWeights
+from foldjax_amd.pairformer import PairDropout, PairformerLayerWeights, _block_dropout
 from foldjax_amd.params import ProtenixAttentionPairBiasParams as AttentionPairBiasParams
 from foldjax_amd.params import ProtenixPairformerBlockParams as PairformerBlockParams
 from foldjax_amd.params import ProtenixPairformerStackParams as PairformerStackParams
@@ -177,6 +177,7 @@ def pairformer_block(
     single_att_q_chunk_size: int | None = None,
     single_attention_backend: str = "xla",
     triangle_attention_backend: str | None = None,
+    dropout: PairDropout | None = None,
 ) -> tuple[torch.Tensor | None, torch.Tensor]:
     """Protenix ``pairformer_block`` (``PXK/pairformer.py:49-180``): z through
     tri-mul out and in, tri-attn start and end, pair transition, each output
@@ -185,9 +186,10 @@ def pairformer_block(
     transition, each gated by that diagonal. ``params`` is a
     ``PairformerBlockParams`` (fields the reference's containers or packed
     weights) or a packed ``PairformerLayerWeights``. Chunk sizes are accepted
-    and unused; the backend selectors are validated as upstream."""
+    and unused; the backend selectors are validated as upstream. ``dropout``
+    drops the four triangle updates."""
     _check_block_selectors(single_attention_backend, triangle_attention_backend)
-    return _packed_block(params, s, z).forward_protenix(s, z, pair_mask)
+    return _packed_block(params, s, z).forward_protenix(s, z, pair_mask, dropout=dropout)
 
 
 def _check_block_selectors(single_attention_backend: str, triangle_attention_backend: str | None) -> None:
@@ -235,12 +237,14 @@ def pairformer_stack(
     single_att_q_chunk_size: int | None = None,
     single_attention_backend: str = "xla",
     triangle_attention_backend: str | None = None,
+    dropout: PairDropout | None = None,
 ) -> tuple[torch.Tensor | None, torch.Tensor]:
     """Protenix ``pairformer_stack`` (``PXK/pairformer.py:183-234``): the
     blocks in order. ``params`` is a ``PairformerStackParams`` or a
     ``StackedLayers`` of packed blocks. With ``use_scan`` the blocks are
     stacked once (``stack_pairformer_block_params``) and run from the stacked
-    weights; either way every block is the same chain of kernel launches."""
+    weights; either way every block is the same chain of kernel launches.
+    ``dropout`` drops every block's triangle updates."""
     blocks = params if isinstance(params, StackedLayers) else params.blocks
     if not blocks:
         raise ValueError("PairformerStack requires at least one block")
@@ -253,5 +257,6 @@ def pairformer_stack(
     # the first block writes new s and z, every later one updates them in
     # place (the reference's scan donates its carry)
     for idx, block in enumerate(blocks):
-        s, z = _packed_block(block, s, z).forward_protenix(s, z, pair_mask, donate=idx > 0)
+        s, z = _packed_block(block, s, z).forward_protenix(s, z, pair_mask, donate=idx > 0,
+                                                           dropout=_block_dropout(dropout, idx))
     return s, z
