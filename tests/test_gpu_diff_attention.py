@@ -369,3 +369,31 @@ def test_gradients_against_differences():
         have = float((got[name].double().cpu() * direction).sum())
         # float32 gradients: 1e-5 of their norm; the difference's own error is h^2
         assert abs(have - want) <= 1e-5 * float(got[name].double().norm()) * float(direction.norm()) + 1e-6, name
+
+
+def test_calls_of_one_layout_see_their_own_tensors():
+    """Calls of a layout seen before take their pointers anew: other tensors,
+    another scale, a tensor of the same strides off its 16 bytes, a mask whose
+    values changed in place."""
+    say("one layout, other tensors")
+    a, b = (make((2,), 2, 2, 33, 40, 32, BF, bias="plane", mask="holes", seed=s) for s in (1, 2))
+    for t in (a, b, a):
+        want, terms = reference(t, backward=True)
+        g = on_gpu(t)
+        out, lse = call(g, return_lse=True)
+        check("out", out, want["out"], terms["out"], BF)
+        got = grads(g, lse)
+        for name in ("dq", "dk", "dv", "dlam", "dbias"):
+            check(name, got[name], want[name], terms[name], BF)
+    g = on_gpu(b)
+    for name in ("q", "k", "v", "dout"):
+        off = torch.empty(g[name].numel() + 1, dtype=BF, device="cuda")[1:].view(g[name].shape)
+        moved = dict(g, **{name: off.copy_(g[name])})
+        o, l = call(moved, return_lse=True)
+        assert torch.equal(o, call(g)) and torch.equal(grads(moved, l)["dv"], grads(g, l)["dv"])
+    g["mask"][:, 5] ^= True
+    g["k"], g["v"], g["bias"] = (torch.nan_to_num(g[n], posinf=0.0) for n in ("k", "v", "bias"))
+    t = {n: x.cpu() if isinstance(x, torch.Tensor) else x for n, x in g.items()}
+    check("out", call(g), *(r["out"] for r in reference(t)), BF)
+    t["scale"] = g["scale"] = 0.1
+    check("out", call(g), *(r["out"] for r in reference(t)), BF)
