@@ -1122,13 +1122,20 @@ struct DiffPlan {
 DiffPlan diff_plan(int64_t items, int64_t heads, int64_t kv_heads, int64_t nq, int64_t nk, int64_t d) {
   const int64_t rows = heads / kv_heads * nq;
   DiffPlan p = {};
-  p.keywise = rows <= 16 || items * kv_heads * ((rows + 63) / 64) < 256;
+  // Keywise where the rows fill a quarter of a workgroup at most, or fill too few
+  // of the card's CUs; not for a single block of keys. us by rows / keywise, 6 heads:
+  // D = 32 bf16 at 48 workgroups (499 tokens) 18.3 / 11.4, 96 18.6 / 14.1, 144 18.9 /
+  // 17.6, 192 19.3 / 18.3, 288 26.6 / 28.7; D = 64 at 48 22.8 / 15.5, 96 23.2 / 29.5;
+  // float32 D = 32 at 48 38 / 18, 96 39 / 28, 144 40 / 41; 64 tokens 5.8 / 6.9.
+  const int64_t own = items * kv_heads * ((rows + 63) / 64);
+  p.keywise = nk > 64 && (rows <= 16 || own < (d == 32 ? 128 : 64));
   p.splits = 1;
   const int64_t blocks = p.keywise ? (nk + 127) / 128 : (nk + 63) / 64;
   p.split_blocks = blocks;
   if (p.keywise) {
     const int64_t wgs = items * kv_heads * ((rows + 15) / 16);
-    const int64_t want = std::min<int64_t>((512 + wgs - 1) / wgs, blocks / 2);  // two blocks a split at least
+    // more workgroups than that hide the join's launch no more (5 to 11 us)
+    const int64_t want = wgs <= 128 ? std::min<int64_t>(512 / wgs, blocks / 2) : 1;  // two blocks a split at least
     if (want > 1) {
       p.split_blocks = (blocks + want - 1) / want;
       p.splits = (int)((blocks + p.split_blocks - 1) / p.split_blocks);
@@ -1142,11 +1149,10 @@ DiffPlan diff_plan(int64_t items, int64_t heads, int64_t kv_heads, int64_t nq, i
   return p;
 }
 
-#ifndef DA_CH
-#define DA_CH 512
-#endif
 // The bias gradient of shared planes: items of one chunk, so that the 64 x 64
-// tiles times the chunks are some workgroups a CU.
+// tiles times the chunks are the workgroups that the card holds at once, two a
+// CU (245 x 245 tokens, 2 heads, 245 items; for 256 workgroups 71.8 us, 512 45.6,
+// 768 60.3, 1024 51.0).
 struct DiffBwdPlan {
   int chunks;
   int64_t chunk_items;
@@ -1158,7 +1164,7 @@ DiffBwdPlan diff_bwd_plan(int64_t items, int64_t heads, int64_t nq, int64_t nk, 
   if (with_dbias && share > 1) {
     const int64_t planes = items / share;
     const int64_t tiles = planes * heads * ((nq + 63) / 64) * ((nk + 63) / 64);
-    const int64_t want = std::max<int64_t>(1, std::min<int64_t>((DA_CH + tiles - 1) / tiles, share));
+    const int64_t want = std::max<int64_t>(1, std::min<int64_t>((512 + tiles - 1) / tiles, share));
     p.chunk_items = (share + want - 1) / want;
     p.chunks = (int)((share + p.chunk_items - 1) / p.chunk_items);
     p.part = align_up((size_t)p.chunks * planes * heads * nq * nk * sizeof(float));
@@ -1572,8 +1578,8 @@ int fjx_diff_attention_bwd(const fjx_diff_attention_bwd_args* b, hipStream_t st)
       !diff_strides_ok(b->dk_strides, a->items, 2 * a->kv_heads, a->nk, es, true) ||
       !diff_strides_ok(b->dv_strides, a->items, a->kv_heads, a->nk, es, true))
     return fail(FJX_ERR_INVALID, "%s: the gradients' strides must be positive multiples of 16 bytes", fn);
-  if (a->bias && (a->bias_strides[2] >= 1 << 26 || (b->dbias && b->dbias_strides[2] >= 1 << 26)))
-    return fail(FJX_ERR_UNSUPPORTED, "%s: rows of the bias must be less than 2^26 elements apart", fn);
+  if (a->bias && (a->bias_strides[2] >= 1 << 23 || (b->dbias && b->dbias_strides[2] >= 1 << 23)))
+    return fail(FJX_ERR_UNSUPPORTED, "%s: rows of the bias must be less than 2^23 elements apart", fn);
   if (b->dbias) {
     const int64_t len[3] = {a->bias ? a->items / a->bias_share : 0, a->heads, a->nq};
     for (int i = 0; i < 3; ++i)

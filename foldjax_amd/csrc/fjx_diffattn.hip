@@ -80,11 +80,15 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D> + (kDaWaves<T, D> > 1))) void 
       qf[m][c] = load8(P.q.p + item * P.q.item + (2 * head + m) * P.q.head + qi * P.q.token + 32 * c + 8 * lg);
   const float lam = da_lambda<D>(P.lam, P.heads, head, P.init, lane);
 
-  auto key_flags = [&](int64_t blk, int at) {
-    if (t < kRows) {
-      const int64_t k = blk * kRows + t;
-      flags[at].set(t, k < P.nk && (!mask || mask[k]));
-    }
+  // a block's flags in two steps: the mask on its way while a block is worked on
+  uint8_t part = 0;
+  auto look = [&](int64_t blk) {
+    const int64_t k = blk * kRows + t;
+    part = t < kRows && k < P.nk;
+    if (part && mask) part = mask[k];
+  };
+  auto put_flags = [&](int at) {
+    if (t < kRows) flags[at].set(t, part != 0);
   };
   const int key_w = KEYWISE ? 32 * wave : 0;  // this wave's keys of a block
   typename Quad<T>::type bv[kNt];
@@ -92,8 +96,10 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D> + (kDaWaves<T, D> > 1))) void 
     bias_tile<T, kNt>(bias, blk * kRows + key_w + 4 * lg, P.nk, (blk + 1) * kRows <= P.nk, bv);
   };
   if (bias) load_bias(blk0);
-  key_flags(blk0, 0);
-  key_flags(blk0 + 1, 1);
+  look(blk0);
+  put_flags(0);
+  look(blk0 + 1);
+  put_flags(1);
   __syncthreads();
   st.load(blk0 * kRows, flags[0].whole(), flags[0].on);
 
@@ -130,8 +136,9 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D> + (kDaWaves<T, D> > 1))) void 
     if (more) {
       st.load((blk + 1) * kRows, flags[next].whole(), flags[next].on);
       if (bias) load_bias(blk + 1);
-      key_flags(blk + 2, next == 2 ? 0 : next + 1);
+      look(blk + 2);
     }
+    const int after = next == 2 ? 0 : next + 1;
     cur = next;
     f32x4 s[2][kNt];
     float top[2] = {-INFINITY, -INFINITY};
@@ -195,6 +202,7 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D> + (kDaWaves<T, D> > 1))) void 
     if (kBufs == 1) __syncthreads();
     if (more) {
       st.store(tiles[kBufs == 2 ? buf ^ 1 : 0]);
+      put_flags(after);
     }
     __syncthreads();
   }

@@ -33,16 +33,20 @@ __device__ __forceinline__ void tile_weights(const DaTile<T, D, ROWS>& tile, int
     for (int r = 0; r < 4; ++r) p[kt][r] = __builtin_amdgcn_exp2f(fmaf(p[kt][r], scale_log2, -L));
 }
 
-// dP - c of the same
+// dP of the same
 template <typename T, int D, int ROWS, int NT>
 __device__ __forceinline__ void tile_dp(const DaTile<T, D, ROWS>& tile, int key_w, const typename Frag<T>::type (&dof)[2 * D / 32],
-                                        float c0, int li, int lg, f32x4 (&dp)[NT]) {
+                                        int li, int lg, f32x4 (&dp)[NT]) {
 #pragma unroll
   for (int kt = 0; kt < NT; ++kt) {
-    dp[kt] = f32x4{-c0, -c0, -c0, -c0};
+    dp[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < 2 * D / 32; ++c) mma(dp[kt], load8(&tile.b[key_w + 16 * kt + li][32 * c + 8 * lg]), dof[c]);
   }
+}
+
+__device__ __forceinline__ float sum8(const float (&x)[8]) {
+  return ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
 }
 
 // dq and D_t in one walk over the keys. A wave holds 16 query rows (lane l row
@@ -50,7 +54,10 @@ __device__ __forceinline__ void tile_dp(const DaTile<T, D, ROWS>& tile, int key_
 // are kept, U = sum P_t (dP - c) k and W = sum P_t k, and
 //   dq_t = scale (U - (D_t - c) W)
 // where c, the mean of dP under both maps' weights in the first block, keeps U
-// near the difference that is wanted. Against a first walk for D_t alone this
+// near the difference that is wanted. D_2 is divided by its weights' own sum, one
+// but for the rounding of L: lambda's gradient is the sum of all D_2, of either
+// sign, and shows what they have in common. (c is subtracted from dP here: as the
+// start of dP's accumulators it left D_2 off by 1e-6 in common.) Against a first walk for D_t alone this
 // trades a second set of scores, dP and exponentials for the products W: 52 ->
 // 26 us at 4 x 499 tokens and 6 heads, 123 -> 75 us at 245 x 245 and 2.
 //
@@ -66,7 +73,7 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dq_kernel(Diff
   static_assert(!SPLIT || sizeof(Tile) >= 4 * 2 * 16 * kPo * sizeof(float), "the waves' sums");
   __shared__ __attribute__((aligned(16))) Tile tiles[kBufs];
   __shared__ __attribute__((aligned(16))) KeyFlags<kRows> flags[3];  // of the block at hand and the next two
-  __shared__ float joined[4][2][16];
+  __shared__ float joined[4][3][16];
 
   const int t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -105,11 +112,15 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dq_kernel(Diff
   for (int c = 0; c < 2 * kC; ++c)
     dof[c] = load8(P.dout.p + item * P.dout.item + head * P.dout.head + qi * P.dout.token + 32 * c + 8 * lg);
   const float lam = da_lambda<D>(P.lam, P.heads, head, P.init, lane);
-  auto key_flags = [&](int64_t blk, int at) {
-    if (t < kRows) {
-      const int64_t k = blk * kRows + t;
-      flags[at].set(t, k < P.nk && (!mask || mask[k]));
-    }
+  // a block's flags in two steps: the mask on its way while a block is worked on
+  uint8_t part = 0;
+  auto look = [&](int64_t blk) {
+    const int64_t k = blk * kRows + t;
+    part = t < kRows && k < P.nk;
+    if (part && mask) part = mask[k];
+  };
+  auto put_flags = [&](int at) {
+    if (t < kRows) flags[at].set(t, part != 0);
   };
   typename Quad<T>::type bv[kNt];
   const int64_t blocks = (P.nk + kRows - 1) / kRows;
@@ -118,12 +129,14 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dq_kernel(Diff
   };
   if (bias) load_bias(0);
 
-  key_flags(0, 0);
-  key_flags(1, 1);
+  look(0);
+  put_flags(0);
+  look(1);
+  put_flags(1);
   __syncthreads();
   st.load(0, flags[0].whole(), flags[0].on);
 
-  float c0 = 0.f, Dt[2] = {0.f, 0.f};  // D_t - c
+  float c0 = 0.f, Dt[2] = {0.f, 0.f}, total = 0.f;  // D_t - c; the second map's weights
   f32x4 us[2][kU], ws[2][kU];
 #pragma unroll
   for (int m = 0; m < 2; ++m)
@@ -147,11 +160,12 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dq_kernel(Diff
     if (more) {
       st.load((blk + 1) * kRows, flags[next].whole(), flags[next].on);
       if (bias) load_bias(blk + 1);
-      key_flags(blk + 2, next == 2 ? 0 : next + 1);
+      look(blk + 2);
     }
+    const int after = next == 2 ? 0 : next + 1;
     at = next;
     f32x4 dp[kNt], p[2][kNt];
-    tile_dp<T, D, kRows, kNt>(tile, key_w, dof, c0, li, lg, dp);
+    tile_dp<T, D, kRows, kNt>(tile, key_w, dof, li, lg, dp);
 #pragma unroll
     for (int m = 0; m < 2; ++m) tile_weights<T, D, kRows, kNt>(tile, m, key_w, qf[m], b, P.scale_log2, L[m], li, lg, p[m]);
     if (blk == 0) {
@@ -172,11 +186,11 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dq_kernel(Diff
         sd = (joined[0][1][li] + joined[1][1][li]) + (joined[2][1][li] + joined[3][1][li]);
       }
       c0 = sp > 0.f ? sd / sp : 0.f;
-#pragma unroll
-      for (int kt = 0; kt < kNt; ++kt)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) dp[kt][r] -= c0;
     }
+#pragma unroll
+    for (int kt = 0; kt < kNt; ++kt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) dp[kt][r] -= c0;
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -186,8 +200,9 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dq_kernel(Diff
         for (int e = 0; e < 8; ++e) {
           w8[e] = p[m][2 * c + (e >> 2)][e & 3];
           u8[e] = w8[e] * dp[2 * c + (e >> 2)][e & 3];
-          Dt[m] += u8[e];
         }
+        Dt[m] += sum8(u8);
+        if (m == 1) total += sum8(w8);
         F uf[kParts<T>], wf[kParts<T>];
         parts(u8, uf);
         parts(w8, wf);
@@ -199,18 +214,24 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dq_kernel(Diff
         }
       }
     if (kBufs == 1) __syncthreads();
-    if (more) st.store(tiles[kBufs == 2 ? buf ^ 1 : 0]);
+    if (more) {
+      st.store(tiles[kBufs == 2 ? buf ^ 1 : 0]);
+      put_flags(after);
+    }
     __syncthreads();
   }
 #pragma unroll
   for (int m = 0; m < 2; ++m) Dt[m] = group_sum(Dt[m]);
+  total = group_sum(total);
   if constexpr (SPLIT) {  // the waves' sums, through the tile's memory
-    if (lg == 0) joined[wave][0][li] = Dt[0], joined[wave][1][li] = Dt[1];
+    if (lg == 0) joined[wave][0][li] = Dt[0], joined[wave][1][li] = Dt[1], joined[wave][2][li] = total;
     __syncthreads();
+    total = (joined[0][2][li] + joined[1][2][li]) + (joined[2][2][li] + joined[3][2][li]);
     float* po = reinterpret_cast<float*>(&tiles[0]);  // [wave][map][row][D + 2]
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
       Dt[m] = (joined[0][m][li] + joined[1][m][li]) + (joined[2][m][li] + joined[3][m][li]);
+      if (m == 1 && total > 0.f) Dt[m] /= total;
 #pragma unroll
       for (int u = 0; u < kU; ++u)
 #pragma unroll
@@ -238,6 +259,7 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dq_kernel(Diff
     }
     return;
   }
+  if (total > 0.f) Dt[1] /= total;
   if (!row_on) return;
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
@@ -258,21 +280,21 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dq_kernel(Diff
 // gradients from it, by one workgroup a head: the first of the launch for dk
 // and dv, in whose shadow they run.
 template <typename T, int D>
-__device__ __forceinline__ void dlambda_of(const DiffAttnParams<T>& P, int head, float (&lds)[4]) {
+__device__ __forceinline__ void dlambda_of(const DiffAttnParams<T>& P, int head, double (&lds)[4]) {
   const int t = threadIdx.x;
   const int64_t n = P.items * P.nq;
-  float s = 0.f;
+  double s = 0.;  // many numbers of either sign
 #pragma unroll 8
   for (int64_t i = t; i < n; i += 256) {
     const int64_t item = n >> 32 ? i / P.nq : (uint32_t)i / (uint32_t)P.nq;
     s += P.delta[(item * 2 * P.heads + 2 * head + 1) * P.nq + i - item * P.nq];
   }
 #pragma unroll
-  for (int x = 32; x >= 1; x >>= 1) s += shfl_xor(s, x);
+  for (int x = 32; x >= 1; x >>= 1) s += __shfl_xor(s, x, 64);
   if ((t & 63) == 0) lds[t >> 6] = s;
   __syncthreads();
   if (t >= 64) return;
-  const float dl = -((lds[0] + lds[1]) + (lds[2] + lds[3]));
+  const float dl = (float)-((lds[0] + lds[1]) + (lds[2] + lds[3]));
   float e[2];
   da_lambda<D>(P.lam, P.heads, head, P.init, t, e);
   if (t < D) {
@@ -292,7 +314,7 @@ __device__ __forceinline__ void dlambda_of(const DiffAttnParams<T>& P, int head,
 // (P_1 - lambda P_2)^T dO as they lie. It also writes dbias, where every item has
 // a plane of its own. SPLIT: the four waves share 16 keys and take 32 queries
 // each of a 128-query block, for calls with few keys.
-template <typename T, int D, bool SPLIT>
+template <typename T, int D, bool SPLIT, bool DBIAS>
 __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dkv_kernel(DiffAttnParams<T> P) {
   constexpr int kC = D / 32, kU = D / 16, kQ = SPLIT ? 128 : 64, kQt = SPLIT ? 2 : 4, kBufs = SPLIT ? 1 : 2;
   typedef typename Frag<T>::type F;
@@ -302,7 +324,7 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dkv_kernel(Dif
   __shared__ __attribute__((aligned(16))) Tile tiles[kBufs];
   __shared__ __attribute__((aligned(16))) float row_stat[kBufs][4][kQ];  // L_1, L_2, D_1, D_2
   __shared__ float query_on[kQ];
-  __shared__ float lam_lds[4];
+  __shared__ double lam_lds[4];
 
   const int t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -343,8 +365,7 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dkv_kernel(Dif
   const T* bias = biased ? P.bias.p + plane * P.bias.item : nullptr;
   const uint32_t key_c = in ? (uint32_t)key : 0;
 
-  T* dbias = P.dbias.p && P.share == 1 ? P.dbias.p + plane * P.dbias.item : nullptr;
-  const uint32_t lane_dbias = 4 * lg * (uint32_t)P.dbias.token + key_c;
+  T* dbias = DBIAS ? P.dbias.p + plane * P.dbias.item : nullptr;
 
   const int64_t q_blocks = (P.nq + kQ - 1) / kQ;
   DaStage<T, D, kQ, 256> st;
@@ -375,9 +396,10 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dkv_kernel(Dif
 #pragma unroll
     for (int i = 0; i < kStats; ++i) row_stat[buf][(t + 256 * i) / kQ][(t + 256 * i) % kQ] = stat[i];
   };
-  // a lane's rows of the bias: the row of a tile and r from the loop (scalar),
-  // 4 g rows and the key on top
-  const uint32_t lane_bias = 4 * lg * (uint32_t)P.bias.token;
+  // a lane's element of the bias in a tile's 16 rows (less than 2^23 elements
+  // apart): its row and its key; the tile's first row is scalar
+  const uint32_t bias_row = (uint32_t)P.bias.token, dbias_row = (uint32_t)P.dbias.token;
+  const uint32_t lane_bias = 4 * lg * bias_row + key_c, lane_dbias = 4 * lg * dbias_row + key_c;
   T bq[kQt][4];
   auto fetch_bias = [&](int hg, int64_t qb) {
     const T* p = bias + (h0 + hg) * P.bias.head;
@@ -387,7 +409,7 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dkv_kernel(Dif
 #pragma unroll
       for (int qt = 0; qt < kQt; ++qt)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) bq[qt][r] = (p + (16 * qt + r) * P.bias.token)[lane_bias + key_c];
+        for (int r = 0; r < 4; ++r) bq[qt][r] = (p + 16 * qt * P.bias.token)[lane_bias + r * bias_row];
     } else {
 #pragma unroll
       for (int qt = 0; qt < kQt; ++qt)
@@ -434,38 +456,37 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dkv_kernel(Dif
         fetch(same ? hg : hg + 1, same ? qb + 1 : 0);
         if (biased) fetch_bias(same ? hg : hg + 1, same ? qb + 1 : 0);
       }
+      f32x4 s[2][kQt], dp[kQt];
+#pragma unroll
+      for (int qt = 0; qt < kQt; ++qt) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          s[m][qt] = b[qt];
+#pragma unroll
+          for (int x = 0; x < kC; ++x) mma(s[m][qt], load8(&tile.a[m][q_w + 16 * qt + li][32 * x + 8 * lg]), kf[m][x]);
+        }
+        dp[qt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < 2 * kC; ++x) mma(dp[qt], load8(&tile.b[q_w + 16 * qt + li][32 * x + 8 * lg]), vf[x]);
+      }
+      T db[kQt][4];
 #pragma unroll
       for (int c = 0; c < kQt / 2; ++c) {
         float comb[8], ds[2][8];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const int qt = 2 * c + j;
-          f32x4 s[2], dp = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int m = 0; m < 2; ++m) {
-            s[m] = b[qt];
-#pragma unroll
-            for (int x = 0; x < kC; ++x) mma(s[m], load8(&tile.a[m][q_w + 16 * qt + li][32 * x + 8 * lg]), kf[m][x]);
-          }
-#pragma unroll
-          for (int x = 0; x < 2 * kC; ++x) mma(dp, load8(&tile.b[q_w + 16 * qt + li][32 * x + 8 * lg]), vf[x]);
           f32x4 rs[4];
 #pragma unroll
           for (int w = 0; w < 4; ++w) rs[w] = *reinterpret_cast<const f32x4*>(&row_stat[buf][w][q_w + 16 * qt + 4 * lg]);
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float p1 = __builtin_amdgcn_exp2f(fmaf(s[0][r], P.scale_log2, -rs[0][r]));
-            const float p2 = lam * __builtin_amdgcn_exp2f(fmaf(s[1][r], P.scale_log2, -rs[1][r]));
+            const float p1 = __builtin_amdgcn_exp2f(fmaf(s[0][qt][r], P.scale_log2, -rs[0][r]));
+            const float p2 = lam * __builtin_amdgcn_exp2f(fmaf(s[1][qt][r], P.scale_log2, -rs[1][r]));
             comb[4 * j + r] = p1 - p2;
-            ds[0][4 * j + r] = p1 * (dp[r] - rs[2][r]);
-            ds[1][4 * j + r] = p2 * (rs[3][r] - dp[r]);
-          }
-          if (dbias && in) {
-            const int64_t q = qb * kQ + q_w + 16 * qt;
-            T* p = dbias + (h0 + hg) * P.dbias.head + q * P.dbias.token;
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (q + 4 * lg + r < P.nq) (p + r * P.dbias.token)[lane_dbias] = from_f32<T>(ds[0][4 * j + r] + ds[1][4 * j + r]);
+            ds[0][4 * j + r] = p1 * (dp[qt][r] - rs[2][r]);
+            ds[1][4 * j + r] = p2 * (rs[3][r] - dp[qt][r]);
+            if (DBIAS) db[qt][r] = from_f32<T>(ds[0][4 * j + r] + ds[1][4 * j + r]);
           }
         }
         F cf[kParts<T>], df0[kParts<T>], df1[kParts<T>];
@@ -478,6 +499,22 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dkv_kernel(Dif
         for (int u = 0; u < kU; ++u) {
           mma_parts(dk[0][u], col_frag(&tile.a[0][0][0], Tile::kA, q_w + 32 * c, 16 * u, lane), df0);
           mma_parts(dk[1][u], col_frag(&tile.a[1][0][0], Tile::kA, q_w + 32 * c, 16 * u, lane), df1);
+        }
+      }
+      if (DBIAS && in) {
+        const int64_t q0 = qb * kQ + q_w;
+        T* p = dbias + (h0 + hg) * P.dbias.head + q0 * P.dbias.token;
+        if ((qb + 1) * kQ <= P.nq) {
+#pragma unroll
+          for (int qt = 0; qt < kQt; ++qt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) (p + (16 * qt + r) * P.dbias.token)[lane_dbias] = db[qt][r];
+        } else {
+#pragma unroll
+          for (int qt = 0; qt < kQt; ++qt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (q0 + 16 * qt + 4 * lg + r < P.nq) (p + (16 * qt + r) * P.dbias.token)[lane_dbias] = db[qt][r];
         }
       }
       if (kBufs == 1) __syncthreads();
@@ -591,17 +628,22 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dbias_kernel(D
     for (int c = 0; c < 2 * kC; ++c)
       don[c] = load8(P.dout.p + item * P.dout.item + head * P.dout.head + qc * P.dout.token + 32 * c + 8 * lg);
   };
-  auto key_flags = [&](int64_t item, int at) {
-    if (t < kDaKeys) {
-      const int64_t k = kb * 64 + t;
-      flags[at].set(t, item < i1 && k < P.nk && (!P.mask || P.mask[item * P.nk + k]));
-    }
+  uint8_t part = 0;  // as in the kernel for dq
+  auto look = [&](int64_t item) {
+    const int64_t k = kb * 64 + t;
+    part = t < kDaKeys && item < i1 && k < P.nk;
+    if (part && P.mask) part = P.mask[item * P.nk + k];
+  };
+  auto put_flags = [&](int at) {
+    if (t < kDaKeys) flags[at].set(t, part != 0);
   };
   f32x4 acc[4];
 #pragma unroll
   for (int kt = 0; kt < 4; ++kt) acc[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
-  key_flags(i0, 0);
-  key_flags(i0 + 1, 1);
+  look(i0);
+  put_flags(0);
+  look(i0 + 1);
+  put_flags(1);
   __syncthreads();
   fetch(i0, 0);
   st.store(tiles[0]);
@@ -627,10 +669,10 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dbias_kernel(D
     at = at == 2 ? 0 : at + 1;
     if (more) {
       fetch(item + 1, at);
-      key_flags(item + 2, at == 2 ? 0 : at + 1);
+      look(item + 2);
     }
     f32x4 dp[4];
-    tile_dp<T, D, kDaKeys, 4>(tile, 0, dof, 0.f, li, lg, dp);
+    tile_dp<T, D, kDaKeys, 4>(tile, 0, dof, li, lg, dp);
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
       f32x4 p[4];
@@ -641,7 +683,10 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dbias_kernel(D
 #pragma unroll
         for (int r = 0; r < 4; ++r) acc[kt][r] = fmaf(p[kt][r] * by, dp[kt][r] - rs[2 + m], acc[kt][r]);
     }
-    if (more) st.store(tiles[buf ^ 1]);
+    if (more) {
+      st.store(tiles[buf ^ 1]);
+      put_flags(at == 2 ? 0 : at + 1);
+    }
     __syncthreads();
   }
   if (qi >= P.nq) return;
@@ -666,26 +711,35 @@ __global__ __launch_bounds__(256) void diffattn_bias_sum_kernel(DiffAttnParams<T
   }
 }
 
-#ifndef DA_SPLITQ
-#define DA_SPLITQ 192
-#define DA_SPLITK 224
-#endif
 unsigned eights(int64_t blocks) { return (unsigned)((blocks + 7) / 8 * 8); }
 
 template <typename T, int D>
 void bwd(const DiffAttnParams<T>& P, hipStream_t st) {
   const int64_t kvh = P.heads / P.group;
-  // waves with rows (keys) of their own read each block once for 64 of them;
-  // they share 16 where that leaves fewer workgroups than two a CU
+  // Waves with rows (keys) of their own cost the least work; they share 16 where
+  // that leaves too few workgroups for the card's 256 CUs. D = 32, bf16, 6 heads,
+  // us own / shared: dq at 96 workgroups (2 x 499 tokens) 19.0 / 15.3, 144 19.1 /
+  // 22.1, 192 22.2 / 23.8, 240 19.9 / 26.6; dk and dv 28.3 / 17.4, 28.1 / 25.2, 29.7
+  // / 26.8, 29.2 / 30.5. float32 at 48 (2 x 256): 27.7 / 14.1 and 29.9 / 13.4.
   const int64_t heads = P.items * kvh, rows = P.group * P.nq;
-  if (heads * ((rows + 63) / 64) >= DA_SPLITQ)
+  if (heads * ((rows + 63) / 64) >= 128)
     diffattn_dq_kernel<T, D, false><<<eights(heads * ((rows + 63) / 64)), 256, 0, st>>>(P);
   else
     diffattn_dq_kernel<T, D, true><<<eights(heads * ((rows + 15) / 16)), 256, 0, st>>>(P);
-  if (heads * ((P.nk + 63) / 64) >= DA_SPLITK)
-    diffattn_dkv_kernel<T, D, false><<<eights(P.heads) + eights(heads * ((P.nk + 63) / 64)), 256, 0, st>>>(P);
-  else
-    diffattn_dkv_kernel<T, D, true><<<eights(P.heads) + eights(heads * ((P.nk + 15) / 16)), 256, 0, st>>>(P);
+  const bool own = P.dbias.p && P.share == 1;
+  if (heads * ((P.nk + 63) / 64) >= 224) {
+    const unsigned blocks = eights(P.heads) + eights(heads * ((P.nk + 63) / 64));
+    if (own)
+      diffattn_dkv_kernel<T, D, false, true><<<blocks, 256, 0, st>>>(P);
+    else
+      diffattn_dkv_kernel<T, D, false, false><<<blocks, 256, 0, st>>>(P);
+  } else {
+    const unsigned blocks = eights(P.heads) + eights(heads * ((P.nk + 15) / 16));
+    if (own)
+      diffattn_dkv_kernel<T, D, true, true><<<blocks, 256, 0, st>>>(P);
+    else
+      diffattn_dkv_kernel<T, D, true, false><<<blocks, 256, 0, st>>>(P);
+  }
   if (P.dbias.p && P.share > 1) {
     const int64_t planes = P.items / P.share;
     diffattn_dbias_kernel<T, D><<<eights(planes * P.heads * P.chunks * ((P.nk + 63) / 64) * ((P.nq + 63) / 64)), 256, 0, st>>>(P);
