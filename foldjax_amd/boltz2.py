@@ -218,6 +218,8 @@ def pairformer_no_seq_layer_forward(
     matmul_precision: str = "highest",
     triangle_backend: str = DEFAULT_BACKEND,
     glu_backend: str = "xla",
+    *,
+    dropout=None,
 ) -> torch.Tensor:
     """Boltz-2 ``pairformer_no_seq_layer_forward`` (``B2K/msa.py:467-539``),
     the MSA module's pair block: z += tri-mul outgoing, incoming, tri-attn
@@ -225,7 +227,8 @@ def pairformer_no_seq_layer_forward(
     transition, each residual fused into its kernel. ``params`` is the
     Boltz-2 dict with ``tri_mul_out``, ``tri_mul_in``, ``tri_att_start``,
     ``tri_att_end`` and ``transition_z``; the chunk arguments are accepted for
-    signature parity (the kernels stream with a fixed workspace)."""
+    signature parity (the kernels stream with a fixed workspace). ``dropout``: a
+    ``foldjax_amd.pairformer.PairDropout`` of the four triangle updates."""
     from foldjax_amd.pairformer import TriangleSublayers
 
     resolve_matmul_precision(matmul_precision)
@@ -240,7 +243,7 @@ def pairformer_no_seq_layer_forward(
         pack_triattn_boltz2(params["tri_att_start"], dt, dev),
         pack_triattn_boltz2(params["tri_att_end"], dt, dev),
     )
-    z = tri.forward(z, pair_mask)  # a new tensor, updated in place from here on
+    z = tri.forward(z, pair_mask, dropout=dropout)  # a new tensor, updated in place from here on
     return kernels.transition(z, pack_transition_boltz2(params["transition_z"], dt, dev), residual=z, eps=eps,
                               out=z)
 

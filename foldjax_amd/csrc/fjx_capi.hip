@@ -1578,7 +1578,7 @@ int fjx_diff_attention_bwd(const fjx_diff_attention_bwd_args* b, hipStream_t st)
       !diff_strides_ok(b->dk_strides, a->items, 2 * a->kv_heads, a->nk, es, true) ||
       !diff_strides_ok(b->dv_strides, a->items, a->kv_heads, a->nk, es, true))
     return fail(FJX_ERR_INVALID, "%s: the gradients' strides must be positive multiples of 16 bytes", fn);
-  if (a->bias && (a->bias_strides[2] >= 1 << 23 || (b->dbias && b->dbias_strides[2] >= 1 << 23)))
+  if (a->bias && a->nq > 1 && (a->bias_strides[2] >= 1 << 23 || (b->dbias && b->dbias_strides[2] >= 1 << 23)))
     return fail(FJX_ERR_UNSUPPORTED, "%s: rows of the bias must be less than 2^23 elements apart", fn);
   if (b->dbias) {
     const int64_t len[3] = {a->bias ? a->items / a->bias_share : 0, a->heads, a->nq};

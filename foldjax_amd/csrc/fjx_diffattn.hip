@@ -38,6 +38,7 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D> + (kDaWaves<T, D> > 1))) void 
   static_assert(!KEYWISE || kBytes >= kMerge, "the waves' sums");
   __shared__ __attribute__((aligned(16))) unsigned char raw[kBytes];
   __shared__ __attribute__((aligned(16))) KeyFlags<kRows> flags[3];  // of the block at hand and the next two
+  __shared__ float lams[4][16];  // of the waves' rows
   Tile* tiles = reinterpret_cast<Tile*>(raw);
 
   const int t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
@@ -59,7 +60,7 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D> + (kDaWaves<T, D> > 1))) void 
   const bool row_on = row < rows;
   const uint32_t row_c = row_on ? row : rows - 1;
   const int hg = row_c / nq;
-  const int64_t qi = row_c - hg * nq;
+  const uint32_t qi = row_c - hg * nq;
   const int head = kv * P.group + hg;
 
   DaStage<T, D, kRows, 256> st;
@@ -78,7 +79,9 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D> + (kDaWaves<T, D> > 1))) void 
 #pragma unroll
     for (int c = 0; c < kC; ++c)
       qf[m][c] = load8(P.q.p + item * P.q.item + (2 * head + m) * P.q.head + qi * P.q.token + 32 * c + 8 * lg);
-  const float lam = da_lambda<D>(P.lam, P.heads, head, P.init, lane);
+  // kept in LDS: in a register through the loop it was the one that spilled
+  const float lam_own = da_lambda<D>(P.lam, P.heads, head, P.init, lane);
+  if (lg == 0) lams[wave][li] = lam_own;
 
   // a block's flags in two steps: the mask on its way while a block is worked on
   uint8_t part = 0;
@@ -276,7 +279,7 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D> + (kDaWaves<T, D> > 1))) void 
     if (first && P.stats)  // +inf for such a row: its weights are zeros in the backward pass as well
       P.stats[(item * 2 * P.heads + 2 * head + mp) * P.nq + qi] = ls[mp] == 0.f ? INFINITY : m[mp] + log2f(ls[mp]);
   }
-  inv[1] *= lam;
+  inv[1] *= lams[wave][li];
   T* out = P.out.p + item * P.out.item + head * P.out.head + qi * P.out.token;
 #pragma unroll
   for (int u = 0; u < kOwn; ++u) {

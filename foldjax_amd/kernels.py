@@ -726,6 +726,7 @@ def _diff_attention_args(q, k, v, lambda_vectors, lambda_init, scale, bias, mask
     """The checked argument block that both directions share, the tensors it
     points to, the leading axes, the elements of a 16-byte piece, and (its key,
     the workspace of the forward call)."""
+    lambda_init, scale = float(lambda_init), float(scale)  # values, also of tensors: they are part of the key
     key = (_layout(q, k, v, lambda_vectors, bias, mask), lambda_init, scale)
     seen = _BLOCKS.get(key)
     if seen is not None:
@@ -761,7 +762,9 @@ def _diff_attention_args(q, k, v, lambda_vectors, lambda_init, scale, bias, mask
     items = 1
     for n in lead:
         items *= n
-    lam = lambda_vectors if lambda_vectors.is_contiguous() else lambda_vectors.contiguous()
+    lam = lambda_vectors
+    if not lam.is_contiguous() or lam.data_ptr() & 15:
+        lam = lam.clone(memory_format=torch.contiguous_format)
     bp, bst, share = None, (0, 0, 0), 1
     if bias is not None:
         bs = bias.shape
@@ -832,12 +835,14 @@ def diff_attention(
     over the last leading axes (1, or left out): ``[B, 1, H, J, J]`` for the
     rows of a triangle attention. ``mask`` broadcasts to ``[..., K]``: 0 takes
     a key out, whatever it holds. A bias of -inf, or of the dtype's lowest
-    value, takes a key out for one query (k and v finite there). A row without
-    keys is zeros.
+    value, takes a key out for one query (k and v finite there), any other
+    should leave bias / scale within float32's range. A row without keys is
+    zeros. ``scale`` in [1e-30, 1e30].
 
     Returns ``out`` ``[..., H, Q, 2 D]``; with ``return_lse`` also what
     ``diff_attention_backward`` needs to know of the rows. ``out``: write into
-    this tensor (its rows whole 16-byte pieces, any order of the other axes)."""
+    this tensor (its rows whole 16-byte pieces, any order of the other axes),
+    which overlaps no input."""
     a, kept, lead, unit, (_, nbytes) = _diff_attention_args(q, k, v, lambda_vectors, lambda_init, scale, bias, mask)
     shape = lead + (a.heads, a.nq, 2 * a.head_dim)
     if out is None:
@@ -847,6 +852,8 @@ def diff_attention(
         if out.shape != shape or out.dtype != q.dtype or out.device != q.device:
             raise ValueError(f"out must be a {q.dtype} tensor of shape {shape} on {q.device}, "
                              f"got {out.dtype} {tuple(out.shape)} on {out.device}")
+        if out.data_ptr() in (q.data_ptr(), k.data_ptr(), v.data_ptr()):
+            raise ValueError("out must not be q, k or v: other rows' results are taken from them")
         strides = _head_rows(out, unit)
         if strides is None:
             raise ValueError("out must have rows of whole 16-byte pieces, and leading axes that fold into one")
@@ -882,7 +889,8 @@ def diff_attention_backward(
     dv, dbias, dlambda)``: dq, dk, dv and dbias in the dtype and shape of q, k,
     v and bias (dbias None without a bias or with ``bias_grad`` off; of a shared
     plane the sum over the items, of shared heads' k and v the sum over the
-    query heads), dlambda float32 ``[4, H, D]``. The same bits each time."""
+    query heads), dlambda float32 ``[4, H, D]``. The same bits each time. Rows
+    of the bias are less than 2^23 elements apart."""
     f, kept, lead, unit, (key, _) = _diff_attention_args(q, k, v, lambda_vectors, lambda_init, scale, bias, mask)
     with_bias = bias is not None and bias_grad
     key = None if key is None else (key, _layout(dout, lse), with_bias)
@@ -944,7 +952,7 @@ def rms_norm(
     h)``; ``y ~ codes * scale``, scales ``[..., 1]`` or ``[..., C / group]``.
     ``out`` (without codes) and ``sum_out``: write y and h into these tensors
     (x's shape and dtype, contiguous); each may be ``x`` or ``residual``."""
-    key = None
+    key, eps = None, float(eps)
     if out is None and sum_out is None and (codes is None or isinstance(codes, str)):
         key = (_layout(x, weight, residual), eps, codes, group)
         seen = _BLOCKS.get(key)
@@ -1025,7 +1033,7 @@ def rms_norm_backward(
     gradient too and includes ``dh``, what reaches h from elsewhere; dweight is
     float32, summed over the rows in one order. ``out``: write dx into this
     tensor, which may be ``dy`` or ``dh``."""
-    key = None
+    key, eps = None, float(eps)
     if out is None:
         key = (_layout(dy, h, weight, dh), eps)
         seen = _BLOCKS.get(key)
@@ -1095,7 +1103,7 @@ def dropout_add(
     one element on x's device, read by the kernel and added to ``offset``: a
     captured call then drops anew at each replay. ``out``: write into this
     tensor, which may be ``x`` and/or ``residual``."""
-    key = None
+    key, p = None, float(p)
     shared = tuple(shared)
     if out_mask is None and step is None and out is None:
         key = (_layout(x, residual), p, shared)

@@ -108,6 +108,7 @@ def pair_block(
     tri_mul_first: bool = True,
     eps: float = 1e-5,
     chunk_size: int | None = None,
+    dropout: PairDropout | None = None,
 ) -> torch.Tensor:
     """OpenFold3 ``pair_block`` (``OF3/pair_block.py:106-190``): the updated
     ``z`` after tri-mul out and in, tri-attn start and end (``tri_mul_first``
@@ -117,17 +118,22 @@ def pair_block(
     module and transposes ``z`` and the mask around it; the ending-node kernel
     here addresses the transposed grid directly, which is the same update
     without the two transposed copies. ``chunk_size`` is accepted for
-    signature parity (the kernels stream rows with a fixed workspace)."""
+    signature parity (the kernels stream rows with a fixed workspace).
+    ``dropout`` drops the four triangle updates."""
+
+    def add(z, sublayer, update, *args, **more):
+        if dropout is None:
+            return update(z, *args, mask=pair_mask, eps=eps, residual=z, **more)
+        return dropout.add(update(z, *args, mask=pair_mask, eps=eps, **more), z, sublayer, sublayer == 3, None, None)
 
     def mul_pair(z):
-        z = triangle_multiplication(z, params.tri_mul_out, outgoing=True, mask=pair_mask, eps=eps, residual=z)
-        return triangle_multiplication(z, params.tri_mul_in, outgoing=False, mask=pair_mask, eps=eps, residual=z)
+        z = add(z, 0, triangle_multiplication, params.tri_mul_out, outgoing=True)
+        return add(z, 1, triangle_multiplication, params.tri_mul_in, outgoing=False)
 
     def att_pair(z):
-        z = triangle_attention(z, params.tri_att_start, no_heads=no_heads_pair, mask=pair_mask, starting=True,
-                               inf=inf, eps=eps, backend="hip", residual=z)
-        return triangle_attention(z, params.tri_att_end, no_heads=no_heads_pair, mask=pair_mask, starting=False,
-                                  inf=inf, eps=eps, backend="hip", residual=z)
+        more = {"no_heads": no_heads_pair, "inf": inf, "backend": "hip"}
+        z = add(z, 2, triangle_attention, params.tri_att_start, starting=True, **more)
+        return add(z, 3, triangle_attention, params.tri_att_end, starting=False, **more)
 
     z = att_pair(mul_pair(z)) if tri_mul_first else mul_pair(att_pair(z))
     return swiglu_transition(z, params.pair_transition, mask=pair_mask if mask_transition else None, eps=eps,

@@ -369,11 +369,13 @@ int fjx_single_attention_fwd(const fjx_single_attention_args* args, hipStream_t 
  * lie. bias [items / bias_share, heads, nq, nk] (strides {plane, head, query},
  * keys contiguous) serves bias_share consecutive items a plane: the rows of a
  * triangle attention share one.
- * A key takes part where mask ([items, nk] bytes, or NULL) is not 0 and the
- * bias is above float32's lowest value / log2(e), about -2.36e38: -inf and the
- * types' lowest values take a key out. A masked key's k, v and bias are never
+ * A key takes part where mask ([items, nk] bytes, or NULL) is not 0 and neither
+ * the bias's quotient by the scale nor its product with log2(e) is below
+ * float32's range: -inf and the types' lowest values take a key out, whatever
+ * the scale (which is in [1e-30, 1e30]). A masked key's k, v and bias are never
  * looked at (they may hold NaN), one that only the bias takes out needs finite
- * k and v. A row without a key is zeros, with zero gradients.
+ * k and v. A row without a key is zeros, with zero gradients. `out` overlaps no
+ * input.
  * stats ([items, 2 heads, nq] fp32, or NULL): what the backward pass needs to
  * know of a row. Supported: head_dim 32 or 64. Scores, weights and sums are fp32; the
  * maps' weights enter the products with v as two bf16 parts (fp32: as they are).
@@ -414,7 +416,8 @@ int fjx_diff_attention_fwd(const fjx_diff_attention_args* args, hipStream_t stre
  * The gradients of fjx_diff_attention_fwd. `fwd` holds that call's arguments
  * (out is not read; its strides are dout's), with the stats it wrote. Every
  * sum has one order: the same bits each time. dk and dv of a shared head are
- * summed over its query heads, dbias over its plane's items.
+ * summed over its query heads, dbias over its plane's items. Rows of bias and
+ * dbias are less than 2^23 elements apart (FJX_ERR_UNSUPPORTED otherwise).
  */
 typedef struct fjx_diff_attention_bwd_args {
   fjx_diff_attention_args fwd;

@@ -397,3 +397,25 @@ def test_calls_of_one_layout_see_their_own_tensors():
     check("out", call(g), *(r["out"] for r in reference(t)), BF)
     t["scale"] = g["scale"] = 0.1
     check("out", call(g), *(r["out"] for r in reference(t)), BF)
+
+
+def test_arguments_are_taken_by_value_and_never_written_over():
+    """A scale given as a tensor counts with what it holds at the call; lambda's
+    vectors may start at any element; an output over an input is refused."""
+    say("arguments by value")
+    t = on_gpu(make((2,), 2, 2, 40, 50, 32, BF))
+    scale, init = torch.tensor(0.2), torch.tensor(0.4)
+    more = {"bias": t["bias"], "mask": t["mask"]}
+    run = lambda s, i, lam=t["lam"]: kernels.diff_attention(t["q"], t["k"], t["v"], lam, scale=s, lambda_init=i, **more)  # noqa: E731
+    assert torch.equal(run(scale, init), run(float(scale), float(init)))
+    scale.mul_(2.0)
+    init.mul_(2.0)
+    assert torch.equal(run(scale, init), run(float(scale), float(init)))
+    assert not torch.equal(run(scale, init), run(0.2, 0.4))
+    lam = torch.empty(t["lam"].numel() + 1, device="cuda")[1:].view_as(t["lam"]).copy_(t["lam"])
+    assert torch.equal(run(0.2, 0.4, lam), run(0.2, 0.4))
+    x = torch.zeros(2, 2, 50, 64, dtype=BF, device="cuda")
+    q, k = x.view(2, 4, 50, 32), torch.randn(2, 4, 50, 32, device="cuda").to(BF)
+    for given in ((q, k, k.view(2, 2, 50, 64)), (k, q, k.view(2, 2, 50, 64)), (k, k, x)):
+        with pytest.raises(ValueError, match="out must not be"):
+            kernels.diff_attention(*given, t["lam"], scale=0.2, lambda_init=0.4, out=x)

@@ -14,6 +14,8 @@ import pytest
 import torch
 
 from foldjax_amd import boltz2, kernels, openfold3, protenix
+from foldjax_amd import params as P
+from foldjax_amd import synthetic as syn
 from foldjax_amd.pairformer import PairDropout, PairformerLayerWeights
 from tests.gpu_util import say
 from tests.test_gpu_dropout import mask_of
@@ -181,6 +183,25 @@ def test_stacks_move_the_offset_and_no_dropout_stays_as_it_was():
     o = openfold3.pairformer_block(s, z, blocks[0], single_mask=mask, pair_mask=pm, no_heads_pair=4, no_heads_pair_bias=16,
                                    dropout=drop)
     assert torch.equal(o[1], blocks[0].forward_openfold3(s, z, mask, pm, dropout=drop)[1])
+
+
+def test_pair_blocks_without_a_single_track():
+    """The same sublayers as a whole layer's: the same bits of z."""
+    say("pair blocks dropout")
+    params = P.pairformer_layer_to_boltz2(syn.pairformer_layer_weights(seed=31))
+    s, z, mask, pm = inputs(19, BF)
+    drop = PairDropout(p=0.25, seed=6, offset=12)
+    tri = {k: params[k] for k in ("tri_mul_out", "tri_mul_in", "tri_att_start", "tri_att_end", "transition_z")}
+    _, want = boltz2.pairformer_layer_forward(params, s, z, mask, pm, dropout=drop)
+    got = boltz2.pairformer_no_seq_layer_forward(tri, z, pm, dropout=drop)
+    assert torch.equal(got, want) and not torch.equal(got, boltz2.pairformer_no_seq_layer_forward(tri, z, pm))
+    layer = block(BF)
+    w = layer.triangle
+    of3 = openfold3.PairBlockParams(tri_mul_out=w.tri_mul_out, tri_mul_in=w.tri_mul_in, tri_att_start=w.tri_att_start,
+                                    tri_att_end=w.tri_att_end, pair_transition=layer.transition_z)
+    got = openfold3.pair_block(z, of3, pair_mask=pm, no_heads_pair=4, dropout=drop)
+    z1 = by_hand(w, z, pm, drop)
+    assert torch.equal(got, kernels.transition(z1, layer.transition_z, row_mask=pm, residual=z1))
 
 
 def test_a_captured_block_drops_anew():

@@ -121,6 +121,18 @@ def test_diff_attention_workspaces(lib):
     assert lib.fjx_diff_attention_bwd(None, None) == lib.fjx_diff_attention_fwd(None, None) == _lib.FJX_ERR_INVALID
 
 
+def test_backward_bias_rows_within_32_bits(lib):
+    """The kernels address a tile's rows of the bias with 32 bits."""
+    for bias_row, dbias_row, nq, code in ((2**23, 16, 8, "UNSUPPORTED"), (16, 2**23, 8, "UNSUPPORTED"),
+                                          (2**23 - 1, 2**23 - 1, 8, "WORKSPACE"), (2**23, 2**23, 1, "WORKSPACE")):
+        b = _lib.DiffAttentionBwdArgs(fwd=diff(nq=nq, stats=FAKE, out=None, bias=FAKE, bias_strides=(8, 8, bias_row)), dout=FAKE,
+                                      dq=FAKE, dk=FAKE, dv=FAKE, dlambda=FAKE, dbias=FAKE)
+        b.dq_strides, b.dk_strides, b.dv_strides = b.fwd.q_strides, b.fwd.k_strides, b.fwd.v_strides
+        b.dbias_strides = _lib._i64x3(8, 8, dbias_row)
+        assert lib.fjx_diff_attention_bwd(ctypes.byref(b), None) == getattr(_lib, f"FJX_ERR_{code}"), (bias_row, dbias_row)
+        assert "2^23" in lib.fjx_last_error().decode() or code == "WORKSPACE"
+
+
 def test_rms_norm_refusals(lib):
     ok = dict(rows=4, c=128, dtype=1, eps=1e-6, x=FAKE, weight=FAKE, out=2 * FAKE)
     for more, code in ((dict(rows=0), "INVALID"), (dict(c=12), "UNSUPPORTED"), (dict(c=8200), "UNSUPPORTED"),
