@@ -134,7 +134,7 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D> + (kDaWaves<T, D> > 1))) void 
 #pragma unroll
     for (int kt = 0; kt < kNt; ++kt)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) b[kt][r] = bias ? to_f32(bv[kt][r]) * P.inv_scale : 0.f;
+      for (int r = 0; r < 4; ++r) b[kt][r] = bias ? to_f32(bv[kt][r]) * bias_unit<T>(P.inv_scale) : 0.f;
     flags[cur].apply(key_w, lg, b);
     if (more) {
       st.load((blk + 1) * kRows, flags[next].whole(), flags[next].on);
@@ -149,7 +149,7 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D> + (kDaWaves<T, D> > 1))) void 
     for (int kt = 0; kt < kNt; ++kt)
 #pragma unroll
       for (int mp = 0; mp < 2; ++mp) {
-        s[mp][kt] = b[kt];
+        s[mp][kt] = score_start<T>(b[kt]);
 #pragma unroll
         for (int c = 0; c < kC; ++c) mma(s[mp][kt], load8(&tile.a[mp][key_w + 16 * kt + li][32 * c + 8 * lg]), qf[mp][c]);
       }
@@ -158,9 +158,12 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D> + (kDaWaves<T, D> > 1))) void 
 #pragma unroll
       for (int mp = 0; mp < 2; ++mp)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) top[mp] = fmaxf(top[mp], s[mp][kt][r]);
-    top[0] = group_max(top[0]) * P.scale_log2;
-    top[1] = group_max(top[1]) * P.scale_log2;
+        for (int r = 0; r < 4; ++r) {
+          if (!kBiasFirst<T>) s[mp][kt][r] = fmaf(s[mp][kt][r], P.scale_log2, b[kt][r]);
+          top[mp] = fmaxf(top[mp], s[mp][kt][r]);
+        }
+    top[0] = group_max(top[0]) * (kBiasFirst<T> ? P.scale_log2 : 1.f);
+    top[1] = group_max(top[1]) * (kBiasFirst<T> ? P.scale_log2 : 1.f);
     if (__builtin_amdgcn_ballot_w64(top[0] > m[0] + kSlack || top[1] > m[1] + kSlack)) {
 #pragma unroll
       for (int mp = 0; mp < 2; ++mp) {
@@ -184,7 +187,7 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D> + (kDaWaves<T, D> > 1))) void 
       for (int kt = 0; kt < kNt; ++kt)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float e = __builtin_amdgcn_exp2f(fmaf(s[mp][kt][r], P.scale_log2, -base));
+          const float e = __builtin_amdgcn_exp2f(kBiasFirst<T> ? fmaf(s[mp][kt][r], P.scale_log2, -base) : s[mp][kt][r] - base);
           if (!kOnes) l[mp][r] += e;
           p[kt >> 1][4 * (kt & 1) + r] = e;
         }

@@ -7,11 +7,12 @@
 // The heads of one key/value head are worked on together: its query rows are
 // the nq queries of each of the heads / kv_heads query heads, one after the
 // other, so that a single token's heads fill one 16-row tile and read the
-// cache once. A score starts as bias / scale, in the accumulator of its matrix
-// instruction, and is left unscaled: the exponent of a weight is one fma,
-// 2^(s scale log2(e) - M), with the row's maximum M in log2 units. A bias whose
-// quotient by the scale or product with log2(e) leaves float32's range (-inf and
-// the types' lowest values) is no key.
+// cache once. In bf16 a score starts as bias / scale, in the accumulator of its
+// matrix instruction, and is left unscaled: the exponent of a weight is one fma,
+// 2^(s scale log2(e) - M), with the row's maximum M in log2 units. Each of a
+// score's sums is then rounded at bias / scale's size, which float32 results show
+// (1e-6 of the output): there the bias comes to the scaled score, in log2 units.
+// A bias that is -inf in its unit (-inf and the types' lowest values) is no key.
 #pragma once
 
 #include "fjx_common.hpp"
@@ -57,6 +58,18 @@ struct DiffAttnParams {
 
 // waves a SIMD that the registers are held to
 template <typename T, int D> constexpr int kDaWaves = sizeof(T) == 2 && D == 32 ? 2 : 1;
+
+// a bias starts its score's sum, as bias / scale, or is added to the scaled score
+template <typename T> constexpr bool kBiasFirst = sizeof(T) == 2;
+template <typename T>
+__device__ __forceinline__ float bias_unit(float inv_scale) { return kBiasFirst<T> ? inv_scale : kLog2e; }
+template <typename T>
+__device__ __forceinline__ f32x4 score_start(const f32x4& b) { return kBiasFirst<T> ? b : f32x4{0.f, 0.f, 0.f, 0.f}; }
+// the exponent of a weight, less `base`, in log2 units, from its score's sum s
+template <typename T>
+__device__ __forceinline__ float exponent(float s, float b, float scale_log2, float base) {
+  return kBiasFirst<T> ? fmaf(s, scale_log2, -base) : fmaf(s, scale_log2, b) - base;
+}
 
 constexpr int kDaKeys = 64;  // keys (or, for the keys' gradients, queries) of a staged block
 

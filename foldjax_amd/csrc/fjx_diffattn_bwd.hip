@@ -16,21 +16,21 @@ namespace fjx {
 namespace {
 
 // weights of the wave's 16 rows and NT key tiles from row `key_w` of a block on,
-// one map; b: bias / scale
+// one map; b: bias in its unit
 template <typename T, int D, int ROWS, int NT>
 __device__ __forceinline__ void tile_weights(const DaTile<T, D, ROWS>& tile, int mp, int key_w,
                                              const typename Frag<T>::type (&qf)[D / 32], const f32x4 (&b)[NT],
                                              float scale_log2, float L, int li, int lg, f32x4 (&p)[NT]) {
 #pragma unroll
   for (int kt = 0; kt < NT; ++kt) {
-    p[kt] = b[kt];
+    p[kt] = score_start<T>(b[kt]);
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) mma(p[kt], load8(&tile.a[mp][key_w + 16 * kt + li][32 * c + 8 * lg]), qf[c]);
   }
 #pragma unroll
   for (int kt = 0; kt < NT; ++kt)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) p[kt][r] = __builtin_amdgcn_exp2f(fmaf(p[kt][r], scale_log2, -L));
+    for (int r = 0; r < 4; ++r) p[kt][r] = __builtin_amdgcn_exp2f(exponent<T>(p[kt][r], b[kt][r], scale_log2, L));
 }
 
 // dP of the same
@@ -155,7 +155,7 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dq_kernel(Diff
 #pragma unroll
     for (int kt = 0; kt < kNt; ++kt)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) b[kt][r] = bias ? to_f32(bv[kt][r]) * P.inv_scale : 0.f;
+      for (int r = 0; r < 4; ++r) b[kt][r] = bias ? to_f32(bv[kt][r]) * bias_unit<T>(P.inv_scale) : 0.f;
     flags[at].apply(key_w, lg, b);
     if (more) {
       st.load((blk + 1) * kRows, flags[next].whole(), flags[next].on);
@@ -445,7 +445,7 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dkv_kernel(Dif
 #pragma unroll
       for (int qt = 0; qt < kQt; ++qt)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) b[qt][r] = biased ? to_f32(bq[qt][r]) * P.inv_scale : 0.f;
+        for (int r = 0; r < 4; ++r) b[qt][r] = biased ? to_f32(bq[qt][r]) * bias_unit<T>(P.inv_scale) : 0.f;
       if (!all_on) {
 #pragma unroll
         for (int qt = 0; qt < kQt; ++qt)
@@ -461,7 +461,7 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dkv_kernel(Dif
       for (int qt = 0; qt < kQt; ++qt) {
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-          s[m][qt] = b[qt];
+          s[m][qt] = score_start<T>(b[qt]);
 #pragma unroll
           for (int x = 0; x < kC; ++x) mma(s[m][qt], load8(&tile.a[m][q_w + 16 * qt + li][32 * x + 8 * lg]), kf[m][x]);
         }
@@ -481,8 +481,8 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dkv_kernel(Dif
           for (int w = 0; w < 4; ++w) rs[w] = *reinterpret_cast<const f32x4*>(&row_stat[buf][w][q_w + 16 * qt + 4 * lg]);
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float p1 = __builtin_amdgcn_exp2f(fmaf(s[0][qt][r], P.scale_log2, -rs[0][r]));
-            const float p2 = lam * __builtin_amdgcn_exp2f(fmaf(s[1][qt][r], P.scale_log2, -rs[1][r]));
+            const float p1 = __builtin_amdgcn_exp2f(exponent<T>(s[0][qt][r], b[qt][r], P.scale_log2, rs[0][r]));
+            const float p2 = lam * __builtin_amdgcn_exp2f(exponent<T>(s[1][qt][r], b[qt][r], P.scale_log2, rs[1][r]));
             comb[4 * j + r] = p1 - p2;
             ds[0][4 * j + r] = p1 * (dp[qt][r] - rs[2][r]);
             ds[1][4 * j + r] = p2 * (rs[3][r] - dp[qt][r]);
@@ -664,7 +664,7 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dbias_kernel(D
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) b[kt][r] = to_f32(bv[kt][r]) * P.inv_scale;
+      for (int r = 0; r < 4; ++r) b[kt][r] = to_f32(bv[kt][r]) * bias_unit<T>(P.inv_scale);
     flags[at].apply(0, lg, b);
     at = at == 2 ? 0 : at + 1;
     if (more) {

@@ -369,10 +369,10 @@ int fjx_single_attention_fwd(const fjx_single_attention_args* args, hipStream_t 
  * lie. bias [items / bias_share, heads, nq, nk] (strides {plane, head, query},
  * keys contiguous) serves bias_share consecutive items a plane: the rows of a
  * triangle attention share one.
- * A key takes part where mask ([items, nk] bytes, or NULL) is not 0 and neither
- * the bias's quotient by the scale nor its product with log2(e) is below
- * float32's range: -inf and the types' lowest values take a key out, whatever
- * the scale (which is in [1e-30, 1e30]). A masked key's k, v and bias are never
+ * A key takes part where mask ([items, nk] bytes, or NULL) is not 0 and the
+ * bias's product with log2(e) (in bf16 also its quotient by the scale) is not
+ * below float32's range: -inf and the types' lowest values take a key out,
+ * whatever the scale (which is in [1e-30, 1e30]). A masked key's k, v and bias are never
  * looked at (they may hold NaN), one that only the bias takes out needs finite
  * k and v. A row without a key is zeros, with zero gradients. `out` overlaps no
  * input.
