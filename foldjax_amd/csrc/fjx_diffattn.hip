@@ -67,7 +67,8 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D> + (kDaWaves<T, D> > 1))) void 
   st.init(P.k.p + item * P.k.item + 2 * kv * P.k.head, P.k.head, P.k.token, P.v.p + item * P.v.item + kv * P.v.head,
           P.v.token, t);
   const uint8_t* mask = P.mask ? P.mask + item * P.nk : nullptr;
-  const T* bias = P.bias.p ? P.bias.p + (item / P.share) * P.bias.item + head * P.bias.head + qi * P.bias.token : nullptr;
+  const bool biased = P.bias.p != nullptr;
+  const T* bias = P.bias.p + (biased ? (item / P.share) * P.bias.item + head * P.bias.head + qi * P.bias.token : 0);
 
   const int64_t blocks = (P.nk + kRows - 1) / kRows;
   const int64_t blk0 = split * P.split_blocks;
@@ -94,11 +95,11 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D> + (kDaWaves<T, D> > 1))) void 
     if (t < kRows) flags[at].set(t, part != 0);
   };
   const int key_w = KEYWISE ? 32 * wave : 0;  // this wave's keys of a block
-  typename Quad<T>::type bv[kNt];
+  typename Quad<T>::type bv[kNt] = {};  // zeros without a bias
   auto load_bias = [&](int64_t blk) {
     bias_tile<T, kNt>(bias, blk * kRows + key_w + 4 * lg, P.nk, (blk + 1) * kRows <= P.nk, bv);
   };
-  if (bias) load_bias(blk0);
+  if (biased) load_bias(blk0);
   look(blk0);
   put_flags(0);
   look(blk0 + 1);
@@ -134,11 +135,11 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D> + (kDaWaves<T, D> > 1))) void 
 #pragma unroll
     for (int kt = 0; kt < kNt; ++kt)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) b[kt][r] = bias ? to_f32(bv[kt][r]) * bias_unit<T>(P.inv_scale) : 0.f;
+      for (int r = 0; r < 4; ++r) b[kt][r] = to_f32(bv[kt][r]) * bias_unit<T>(P.inv_scale);
     flags[cur].apply(key_w, lg, b);
     if (more) {
       st.load((blk + 1) * kRows, flags[next].whole(), flags[next].on);
-      if (bias) load_bias(blk + 1);
+      if (biased) load_bias(blk + 1);
       look(blk + 2);
     }
     const int after = next == 2 ? 0 : next + 1;
@@ -151,7 +152,7 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D> + (kDaWaves<T, D> > 1))) void 
       for (int mp = 0; mp < 2; ++mp) {
         s[mp][kt] = score_start<T>(b[kt]);
 #pragma unroll
-        for (int c = 0; c < kC; ++c) mma(s[mp][kt], load8(&tile.a[mp][key_w + 16 * kt + li][32 * c + 8 * lg]), qf[mp][c]);
+        for (int c = 0; c < kC; ++c) mma(s[mp][kt], load8(&tile.a[key_w + 16 * kt + li][D * mp + 32 * c + 8 * lg]), qf[mp][c]);
       }
 #pragma unroll
     for (int kt = 0; kt < kNt; ++kt)
@@ -201,7 +202,7 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D> + (kDaWaves<T, D> > 1))) void 
     for (int c = 0; c < kNt / 2; ++c)
 #pragma unroll
       for (int u = 0; u < kU; ++u) {
-        const F v = col_frag(&tile.b[0][0], Tile::kB, key_w + 32 * c, 16 * u, lane);
+        const F v = col_frag(&tile.b[0][0], Tile::kPitch, key_w + 32 * c, 16 * u, lane);
         mma_parts(o[0][u], v, pf[0][c]);
         mma_parts(o[1][u], v, pf[1][c]);
       }

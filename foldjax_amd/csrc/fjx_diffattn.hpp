@@ -73,14 +73,13 @@ __device__ __forceinline__ float exponent(float s, float b, float scale_log2, fl
 
 constexpr int kDaKeys = 64;  // keys (or, for the keys' gradients, queries) of a staged block
 
-// one staged block: two tiles of D columns and one of 2 D, rows padded by 16
-// bytes so that 16 rows' 16-byte pieces fall on distinct banks
+// one staged block: the two maps' D columns side by side, and 2 D columns; rows
+// padded by 16 bytes so that 16 rows' 16-byte pieces fall on distinct banks
 template <typename T, int D, int ROWS>
 struct DaTile {
-  static constexpr int kA = D + 16 / (int)sizeof(T);      // row pitch of the two
-  static constexpr int kB = 2 * D + 16 / (int)sizeof(T);  // of the third
-  T a[2][ROWS][kA];
-  T b[ROWS][kB];
+  static constexpr int kPitch = 2 * D + 16 / (int)sizeof(T);
+  T a[ROWS][kPitch];
+  T b[ROWS][kPitch];
 };
 
 // 8 k-slots of a column operand: rows row0 + 4 g + 0..3 and row0 + 16 + 4 g +
@@ -156,6 +155,19 @@ __device__ __forceinline__ void bias_tile(const T* bias, int64_t k0, int64_t nk,
   }
 }
 
+// One instruction where fminf and fmaxf quiet both operands first: for values
+// that no signalling NaN can be among, results of arithmetic.
+__device__ __forceinline__ float plain_min(float a, float b) {
+  float r;
+  asm("v_min_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
+}
+__device__ __forceinline__ float plain_max(float a, float b) {
+  float r;
+  asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
+}
+
 // Which keys of a block take part: +inf, or -inf for one that does not, so
 // that the minimum with its bias (or 0) is -inf whatever the bias holds, a NaN
 // among it; and whether all of 64 do, the usual case.
@@ -183,7 +195,7 @@ struct alignas(16) KeyFlags {
     for (int kt = 0; kt < NT; ++kt) {
       const f32x4 f = *reinterpret_cast<const f32x4*>(&on[key_w + 16 * kt + 4 * lg]);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) b[kt][r] = fminf(b[kt][r], f[r]);
+      for (int r = 0; r < 4; ++r) b[kt][r] = plain_min(b[kt][r], f[r]);
     }
   }
 };
@@ -197,10 +209,10 @@ __device__ __forceinline__ float group_max(float x) {
   const uint32_t u = __builtin_bit_cast(uint32_t, x);
   const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
   const uint32_t a0 = a[0], a1 = a[1];
-  const uint32_t v = __builtin_bit_cast(uint32_t, fmaxf(__builtin_bit_cast(float, a0), __builtin_bit_cast(float, a1)));
+  const uint32_t v = __builtin_bit_cast(uint32_t, plain_max(__builtin_bit_cast(float, a0), __builtin_bit_cast(float, a1)));
   const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
   const uint32_t b0 = b[0], b1 = b[1];
-  return fmaxf(__builtin_bit_cast(float, b0), __builtin_bit_cast(float, b1));
+  return plain_max(__builtin_bit_cast(float, b0), __builtin_bit_cast(float, b1));
 }
 
 // lambda of `head`, the lane's own; the 4 lanes of a row take a quarter of
@@ -240,7 +252,8 @@ struct DaStage {
   u32x4 r[kN];
   const T* src;
   int64_t pitch;
-  int row, which, col;
+  int row, which;
+  int lds;  // the first piece's place in the tile
 
   // a, b: the rows' bases; a_head: elements between the two a tiles
   __device__ __forceinline__ void init(const T* a, int64_t a_head, int64_t a_token, const T* b, int64_t b_token,
@@ -248,7 +261,8 @@ struct DaStage {
     const int in = t % kPk;
     row = t / kPk;
     which = in / kPa;  // 0, 1: the a tiles; 2, 3: the halves of b
-    col = (in % kPa) * kE + (which == 3 ? D : 0);
+    const int col = (in % kPa) * kE + (which == 3 ? D : 0);
+    lds = ((which >> 1) * ROWS + row) * DaTile<T, D, ROWS>::kPitch + in % (2 * kPa) * kE;
     pitch = which < 2 ? a_token : b_token;
     src = (which < 2 ? a + which * a_head : b) + col + row * pitch;
   }
@@ -269,11 +283,7 @@ struct DaStage {
   }
   __device__ __forceinline__ void store(DaTile<T, D, ROWS>& tile) const {
 #pragma unroll
-    for (int i = 0; i < kN; ++i) {
-      const int x = row + i * kStep;
-      T* d = which < 2 ? &tile.a[which & 1][x][col] : &tile.b[x][col];
-      *reinterpret_cast<u32x4*>(d) = r[i];
-    }
+    for (int i = 0; i < kN; ++i) *reinterpret_cast<u32x4*>(&tile.a[0][0] + lds + i * kStep * tile.kPitch) = r[i];
   }
 };
 

@@ -25,7 +25,7 @@ __device__ __forceinline__ void tile_weights(const DaTile<T, D, ROWS>& tile, int
   for (int kt = 0; kt < NT; ++kt) {
     p[kt] = score_start<T>(b[kt]);
 #pragma unroll
-    for (int c = 0; c < D / 32; ++c) mma(p[kt], load8(&tile.a[mp][key_w + 16 * kt + li][32 * c + 8 * lg]), qf[c]);
+    for (int c = 0; c < D / 32; ++c) mma(p[kt], load8(&tile.a[key_w + 16 * kt + li][D * mp + 32 * c + 8 * lg]), qf[c]);
   }
 #pragma unroll
   for (int kt = 0; kt < NT; ++kt)
@@ -97,7 +97,8 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dq_kernel(Diff
   st.init(P.k.p + item * P.k.item + 2 * kv * P.k.head, P.k.head, P.k.token, P.v.p + item * P.v.item + kv * P.v.head,
           P.v.token, t);
   const uint8_t* mask = P.mask ? P.mask + item * P.nk : nullptr;
-  const T* bias = P.bias.p ? P.bias.p + (item / P.share) * P.bias.item + head * P.bias.head + qi * P.bias.token : nullptr;
+  const bool biased = P.bias.p != nullptr;
+  const T* bias = P.bias.p + (biased ? (item / P.share) * P.bias.item + head * P.bias.head + qi * P.bias.token : 0);
 
   F qf[2][kC], dof[2 * kC];
   float L[2];
@@ -122,12 +123,12 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dq_kernel(Diff
   auto put_flags = [&](int at) {
     if (t < kRows) flags[at].set(t, part != 0);
   };
-  typename Quad<T>::type bv[kNt];
+  typename Quad<T>::type bv[kNt] = {};  // zeros without a bias
   const int64_t blocks = (P.nk + kRows - 1) / kRows;
   auto load_bias = [&](int64_t blk) {
     bias_tile<T, kNt>(bias, blk * kRows + key_w + 4 * lg, P.nk, (blk + 1) * kRows <= P.nk, bv);
   };
-  if (bias) load_bias(0);
+  if (biased) load_bias(0);
 
   look(0);
   put_flags(0);
@@ -155,11 +156,11 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dq_kernel(Diff
 #pragma unroll
     for (int kt = 0; kt < kNt; ++kt)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) b[kt][r] = bias ? to_f32(bv[kt][r]) * bias_unit<T>(P.inv_scale) : 0.f;
+      for (int r = 0; r < 4; ++r) b[kt][r] = to_f32(bv[kt][r]) * bias_unit<T>(P.inv_scale);
     flags[at].apply(key_w, lg, b);
     if (more) {
       st.load((blk + 1) * kRows, flags[next].whole(), flags[next].on);
-      if (bias) load_bias(blk + 1);
+      if (biased) load_bias(blk + 1);
       look(blk + 2);
     }
     const int after = next == 2 ? 0 : next + 1;
@@ -208,7 +209,7 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dq_kernel(Diff
         parts(w8, wf);
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
-          const F kf = col_frag(&tile.a[m][0][0], Tile::kA, key_w + 32 * c, 16 * u, lane);
+          const F kf = col_frag(&tile.a[0][D * m], Tile::kPitch, key_w + 32 * c, 16 * u, lane);
           mma_parts(us[m][u], kf, uf);
           mma_parts(ws[m][u], kf, wf);
         }
@@ -400,7 +401,7 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dkv_kernel(Dif
   // apart): its row and its key; the tile's first row is scalar
   const uint32_t bias_row = (uint32_t)P.bias.token, dbias_row = (uint32_t)P.dbias.token;
   const uint32_t lane_bias = 4 * lg * bias_row + key_c, lane_dbias = 4 * lg * dbias_row + key_c;
-  T bq[kQt][4];
+  T bq[kQt][4] = {};  // zeros without a bias
   auto fetch_bias = [&](int hg, int64_t qb) {
     const T* p = bias + (h0 + hg) * P.bias.head;
     const int64_t q0 = qb * kQ + q_w;
@@ -445,12 +446,12 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dkv_kernel(Dif
 #pragma unroll
       for (int qt = 0; qt < kQt; ++qt)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) b[qt][r] = biased ? to_f32(bq[qt][r]) * bias_unit<T>(P.inv_scale) : 0.f;
+        for (int r = 0; r < 4; ++r) b[qt][r] = to_f32(bq[qt][r]) * bias_unit<T>(P.inv_scale);
       if (!all_on) {
 #pragma unroll
         for (int qt = 0; qt < kQt; ++qt)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) b[qt][r] = fminf(b[qt][r], key_on);
+          for (int r = 0; r < 4; ++r) b[qt][r] = plain_min(b[qt][r], key_on);
       }
       if (more) {
         fetch(same ? hg : hg + 1, same ? qb + 1 : 0);
@@ -463,7 +464,7 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dkv_kernel(Dif
         for (int m = 0; m < 2; ++m) {
           s[m][qt] = score_start<T>(b[qt]);
 #pragma unroll
-          for (int x = 0; x < kC; ++x) mma(s[m][qt], load8(&tile.a[m][q_w + 16 * qt + li][32 * x + 8 * lg]), kf[m][x]);
+          for (int x = 0; x < kC; ++x) mma(s[m][qt], load8(&tile.a[q_w + 16 * qt + li][D * m + 32 * x + 8 * lg]), kf[m][x]);
         }
         dp[qt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -494,11 +495,11 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dkv_kernel(Dif
         parts(ds[0], df0);
         parts(ds[1], df1);
 #pragma unroll
-        for (int u = 0; u < 2 * kU; ++u) mma_parts(dv[u], col_frag(&tile.b[0][0], Tile::kB, q_w + 32 * c, 16 * u, lane), cf);
+        for (int u = 0; u < 2 * kU; ++u) mma_parts(dv[u], col_frag(&tile.b[0][0], Tile::kPitch, q_w + 32 * c, 16 * u, lane), cf);
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
-          mma_parts(dk[0][u], col_frag(&tile.a[0][0][0], Tile::kA, q_w + 32 * c, 16 * u, lane), df0);
-          mma_parts(dk[1][u], col_frag(&tile.a[1][0][0], Tile::kA, q_w + 32 * c, 16 * u, lane), df1);
+          mma_parts(dk[0][u], col_frag(&tile.a[0][0], Tile::kPitch, q_w + 32 * c, 16 * u, lane), df0);
+          mma_parts(dk[1][u], col_frag(&tile.a[0][D], Tile::kPitch, q_w + 32 * c, 16 * u, lane), df1);
         }
       }
       if (DBIAS && in) {
