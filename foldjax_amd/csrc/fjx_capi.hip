@@ -1122,13 +1122,13 @@ struct DiffPlan {
 DiffPlan diff_plan(int64_t items, int64_t heads, int64_t kv_heads, int64_t nq, int64_t nk, int64_t d) {
   const int64_t rows = heads / kv_heads * nq;
   DiffPlan p = {};
-  // Keywise where the rows fill a quarter of a workgroup at most, or fill too few
-  // of the card's CUs; not for a single block of keys. us by rows / keywise, 6 heads:
-  // D = 32 bf16 at 48 workgroups (499 tokens) 18.3 / 11.4, 96 18.6 / 14.1, 144 18.9 /
-  // 17.6, 192 19.3 / 18.3, 288 26.6 / 28.7; D = 64 at 48 22.8 / 15.5, 96 23.2 / 29.5;
-  // float32 D = 32 at 48 38 / 18, 96 39 / 28, 144 40 / 41; 64 tokens 5.8 / 6.9.
+  // Keywise where the rows fill a quarter of a workgroup at most, or few enough
+  // workgroups that four times as many are on the card at once; not for a single
+  // block of keys. us by rows / keywise, 499 tokens: D = 32 bf16 at 96 workgroups
+  // 17.5 / 13.9, 144 17.8 / 18.1; D = 64 120 23.7 / 22.4, 144 24.1 / 32.2; float32
+  // D = 32 120 40.1 / 28.3, 144 40.6 / 42.7, D = 64 120 68.9 / 61.8; 64 tokens 5.8 / 6.6.
   const int64_t own = items * kv_heads * ((rows + 63) / 64);
-  p.keywise = nk > 64 && (rows <= 16 || own < (d == 32 ? 128 : 64));
+  p.keywise = nk > 64 && (rows <= 16 || own < 128);
   p.splits = 1;
   const int64_t blocks = p.keywise ? (nk + 127) / 128 : (nk + 63) / 64;
   p.split_blocks = blocks;
@@ -1150,9 +1150,9 @@ DiffPlan diff_plan(int64_t items, int64_t heads, int64_t kv_heads, int64_t nq, i
 }
 
 // The bias gradient of shared planes: items of one chunk, so that the 64 x 64
-// tiles times the chunks are the workgroups that the card holds at once, two a
-// CU (245 x 245 tokens, 2 heads, 245 items; for 256 workgroups 71.8 us, 512 45.6,
-// 768 60.3, 1024 51.0).
+// tiles times the chunks are 512 workgroups, two a CU (a third fits in bf16 at
+// D = 32, and takes the odd ones). us with the chunks' sum, 2 heads, 245 x 245
+// tokens: 512 workgroups 46.9, 768 46.3, 1024 54.0; 300 rows of 350: 108, 119, 107.
 struct DiffBwdPlan {
   int chunks;
   int64_t chunk_items;

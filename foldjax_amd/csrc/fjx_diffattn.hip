@@ -20,6 +20,14 @@ namespace {
 // saves the outputs' rescaling in all but the first blocks of a row.
 constexpr float kSlack = 8.f;
 
+// What bounds it: vector instructions (an exponential, its fma and two bf16 parts
+// a weight and map: 6 to a matrix instruction) and the matrix instructions, which
+// on one SIMD run beside other waves' vector work only in part. 499 rows of 499
+// tokens, 2 heads with their bias: 315 us, the SIMDs 58 % in vector and 29 % in matrix
+// instructions; 245 rows of 245: 51 us, 44 and 18 %, a quarter of it the workgroups'
+// starts and ends (4 blocks of keys each). One token of 8 sequences against 16384
+// keys (134 MB, keywise and split): 26.5 us, the copy rate, and 4.3 for the join.
+//
 // KEYWISE: the four waves share one 16-row tile and take 32 keys each of a
 // 128-key block, for calls with few rows; otherwise each has 16 rows of its own
 // and walks every 64-key block.
@@ -74,16 +82,9 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D> + (kDaWaves<T, D> > 1))) void 
   const int64_t blk0 = split * P.split_blocks;
   const int64_t blk1 = blk0 + P.split_blocks < blocks ? blk0 + P.split_blocks : blocks;
 
-  F qf[2][kC];
-#pragma unroll
-  for (int m = 0; m < 2; ++m)
-#pragma unroll
-    for (int c = 0; c < kC; ++c)
-      qf[m][c] = load8(P.q.p + item * P.q.item + (2 * head + m) * P.q.head + qi * P.q.token + 32 * c + 8 * lg);
-  // kept in LDS: in a register through the loop it was the one that spilled
-  const float lam_own = da_lambda<D>(P.lam, P.heads, head, P.init, lane);
-  if (lg == 0) lams[wave][li] = lam_own;
-
+  // The loads on which others wait go first: the mask, whose flags say which rows of
+  // the block to load, then what the loop starts with; lambda's vectors come in
+  // while the block does.
   // a block's flags in two steps: the mask on its way while a block is worked on
   uint8_t part = 0;
   auto look = [&](int64_t blk) {
@@ -99,13 +100,23 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D> + (kDaWaves<T, D> > 1))) void 
   auto load_bias = [&](int64_t blk) {
     bias_tile<T, kNt>(bias, blk * kRows + key_w + 4 * lg, P.nk, (blk + 1) * kRows <= P.nk, bv);
   };
-  if (biased) load_bias(blk0);
   look(blk0);
-  put_flags(0);
+  const uint8_t part0 = part;
   look(blk0 + 1);
+  F qf[2][kC];
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int c = 0; c < kC; ++c)
+      qf[m][c] = load8(P.q.p + item * P.q.item + (2 * head + m) * P.q.head + qi * P.q.token + 32 * c + 8 * lg);
+  if (biased) load_bias(blk0);
+  if (t < kRows) flags[0].set(t, part0 != 0);
   put_flags(1);
   __syncthreads();
   st.load(blk0 * kRows, flags[0].whole(), flags[0].on);
+  // kept in LDS: in a register through the loop it was the one that spilled
+  const float lam_own = da_lambda<D>(P.lam, P.heads, head, P.init, lane);
+  if (lg == 0) lams[wave][li] = lam_own;
 
   // the sums of the weights: in bf16 a row of ones times their parts, on the
   // matrix cores, which have the time; lane l gets its own row's

@@ -57,9 +57,13 @@ __device__ __forceinline__ float sum8(const float (&x)[8]) {
 // near the difference that is wanted. D_2 is divided by its weights' own sum, one
 // but for the rounding of L: lambda's gradient is the sum of all D_2, of either
 // sign, and shows what they have in common. (c is subtracted from dP here: as the
-// start of dP's accumulators it left D_2 off by 1e-6 in common.) Against a first walk for D_t alone this
-// trades a second set of scores, dP and exponentials for the products W: 52 ->
-// 26 us at 4 x 499 tokens and 6 heads, 123 -> 75 us at 245 x 245 and 2.
+// start of dP's accumulators it left D_2 off by 1e-6 in common.) Against a first
+// walk for D_t alone this trades a second set of scores, dP and exponentials for
+// the products W, half the time. W takes two bf16 parts as well: where one key has
+// nearly all the weight, U and (D_t - c) W nearly cancel.
+// Bound like the forward kernel, with two waves a SIMD (256 registers): 65 us at 245
+// rows of 245 tokens and 2 heads, 46 % vector and 14 % matrix instructions, a quarter
+// of it starts and ends; 19 us at 4 x 499 tokens and 6 heads.
 //
 // SPLIT: the four waves share 16 rows and take 32 keys each of a 128-key
 // block, for calls with few rows; otherwise each has rows of its own.
@@ -100,20 +104,7 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dq_kernel(Diff
   const bool biased = P.bias.p != nullptr;
   const T* bias = P.bias.p + (biased ? (item / P.share) * P.bias.item + head * P.bias.head + qi * P.bias.token : 0);
 
-  F qf[2][kC], dof[2 * kC];
-  float L[2];
-#pragma unroll
-  for (int m = 0; m < 2; ++m) {
-    L[m] = P.saved[(item * 2 * P.heads + 2 * head + m) * P.nq + qi];
-#pragma unroll
-    for (int c = 0; c < kC; ++c)
-      qf[m][c] = load8(P.q.p + item * P.q.item + (2 * head + m) * P.q.head + qi * P.q.token + 32 * c + 8 * lg);
-  }
-#pragma unroll
-  for (int c = 0; c < 2 * kC; ++c)
-    dof[c] = load8(P.dout.p + item * P.dout.item + head * P.dout.head + qi * P.dout.token + 32 * c + 8 * lg);
-  const float lam = da_lambda<D>(P.lam, P.heads, head, P.init, lane);
-  // a block's flags in two steps: the mask on its way while a block is worked on
+  // as in the forward kernel: the mask's loads, on which the block's wait, go first
   uint8_t part = 0;
   auto look = [&](int64_t blk) {
     const int64_t k = blk * kRows + t;
@@ -128,14 +119,27 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dq_kernel(Diff
   auto load_bias = [&](int64_t blk) {
     bias_tile<T, kNt>(bias, blk * kRows + key_w + 4 * lg, P.nk, (blk + 1) * kRows <= P.nk, bv);
   };
-  if (biased) load_bias(0);
-
   look(0);
-  put_flags(0);
+  const uint8_t part0 = part;
   look(1);
+  F qf[2][kC], dof[2 * kC];
+  float L[2];
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    L[m] = P.saved[(item * 2 * P.heads + 2 * head + m) * P.nq + qi];
+#pragma unroll
+    for (int c = 0; c < kC; ++c)
+      qf[m][c] = load8(P.q.p + item * P.q.item + (2 * head + m) * P.q.head + qi * P.q.token + 32 * c + 8 * lg);
+  }
+#pragma unroll
+  for (int c = 0; c < 2 * kC; ++c)
+    dof[c] = load8(P.dout.p + item * P.dout.item + head * P.dout.head + qi * P.dout.token + 32 * c + 8 * lg);
+  if (biased) load_bias(0);
+  if (t < kRows) flags[0].set(t, part0 != 0);
   put_flags(1);
   __syncthreads();
   st.load(0, flags[0].whole(), flags[0].on);
+  const float lam = da_lambda<D>(P.lam, P.heads, head, P.init, lane);
 
   float c0 = 0.f, Dt[2] = {0.f, 0.f}, total = 0.f;  // D_t - c; the second map's weights
   f32x4 us[2][kU], ws[2][kU];
@@ -314,7 +318,8 @@ __device__ __forceinline__ void dlambda_of(const DiffAttnParams<T>& P, int head,
 // leaves the lane 4 queries of its key a tile, the operand of dS_t^T Q_t and of
 // (P_1 - lambda P_2)^T dO as they lie. It also writes dbias, where every item has
 // a plane of its own. SPLIT: the four waves share 16 keys and take 32 queries
-// each of a 128-query block, for calls with few keys.
+// each of a 128-query block, for calls with few keys. Bound like the kernel for
+// dq: 63 us at 245 rows of 245 tokens and 2 heads, 27 us with dbias at 4 x 499 and 6.
 template <typename T, int D, bool SPLIT, bool DBIAS>
 __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dkv_kernel(DiffAttnParams<T> P) {
   constexpr int kC = D / 32, kU = D / 16, kQ = SPLIT ? 128 : 64, kQt = SPLIT ? 2 : 4, kBufs = SPLIT ? 1 : 2;
@@ -345,21 +350,21 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dkv_kernel(Dif
   const int64_t key = SPLIT ? kb * 16 + li : kb * 64 + 16 * wave + li;
   const int q_w = SPLIT ? 32 * wave : 0;  // this wave's queries of a block
   const bool in = key < P.nk;
-  const bool part = in && (!P.mask || P.mask[item * P.nk + key]);
+  uint8_t there = in;
+  if (in && P.mask) there = P.mask[item * P.nk + key];
 
-  F kf[2][kC], vf[2 * kC];
-  F zero;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) zero[e] = from_f32<T>(0.f);
+  F kf[2][kC], vf[2 * kC];  // loaded beside the mask, and zeros where that takes the key out
+  const int64_t key_there = in ? key : 0;
 #pragma unroll
   for (int m = 0; m < 2; ++m)
 #pragma unroll
     for (int c = 0; c < kC; ++c)
-      kf[m][c] = part ? load8(P.k.p + item * P.k.item + (2 * kv + m) * P.k.head + key * P.k.token + 32 * c + 8 * lg) : zero;
+      kf[m][c] = load8(P.k.p + item * P.k.item + (2 * kv + m) * P.k.head + key_there * P.k.token + 32 * c + 8 * lg);
 #pragma unroll
   for (int c = 0; c < 2 * kC; ++c)
-    vf[c] = part ? load8(P.v.p + item * P.v.item + kv * P.v.head + key * P.v.token + 32 * c + 8 * lg) : zero;
+    vf[c] = load8(P.v.p + item * P.v.item + kv * P.v.head + key_there * P.v.token + 32 * c + 8 * lg);
   const bool biased = P.bias.p != nullptr;
+  const bool part = there != 0;
   const float key_on = part ? INFINITY : -INFINITY;
   const bool all_on = __builtin_amdgcn_ballot_w64(part) == ~0ull;
   const int64_t plane = biased ? item / P.share : 0;
@@ -432,11 +437,17 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dkv_kernel(Dif
 
   fetch(0, 0);
   if (biased) fetch_bias(0, 0);
+  float lam = da_lambda<D>(P.lam, P.heads, h0, P.init, lane);
+#pragma unroll
+  for (int c = 0; c < kC; ++c) {
+    if (!part) kf[0][c] = kf[1][c] = F{};
+    if (!part) vf[c] = vf[kC + c] = F{};
+  }
   put(0);
   __syncthreads();
   int turn = 0;
   for (int hg = 0; hg < P.group; ++hg) {
-    const float lam = da_lambda<D>(P.lam, P.heads, h0 + hg, P.init, lane);
+    if (hg) lam = da_lambda<D>(P.lam, P.heads, h0 + hg, P.init, lane);
     for (int64_t qb = 0; qb < q_blocks; ++qb, turn ^= 1) {
       const int buf = kBufs == 2 ? turn : 0;
       const Tile& tile = tiles[buf];
@@ -574,8 +585,11 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dkv_kernel(Dif
 // dbias of a plane that several items share (the rows of a triangle attention):
 // a workgroup owns 64 queries x 64 keys of one head and adds dS over the items
 // of its chunk in registers; the chunks' sums are added by diffattn_bias_sum.
+// What bounds it is the 32 KB of k, v, q and dO that each item of a tile brings from
+// L2: 42 us at 245 rows of 245 tokens and 2 heads, 6.1 TB/s (three waves a SIMD in
+// place of two change it by a few percent).
 template <typename T, int D>
-__global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dbias_kernel(DiffAttnParams<T> P) {
+__global__ __launch_bounds__(256, (kDaWaves<T, D> + (kDaWaves<T, D> > 1))) void diffattn_dbias_kernel(DiffAttnParams<T> P) {
   constexpr int kC = D / 32;
   typedef typename Frag<T>::type F;
   typedef DaTile<T, D, kDaKeys> Tile;
@@ -597,8 +611,8 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dbias_kernel(D
   const int chunk = id % (uint32_t)P.chunks;
   const int64_t plane = id / (uint32_t)P.chunks;
   const int kv = head / P.group;
-  const int64_t qi = qb * 64 + 16 * wave + li;
-  const int64_t qc = qi < P.nq ? qi : P.nq - 1;
+  const uint32_t qi = (uint32_t)qb * 64 + 16 * wave + li, nq = (uint32_t)P.nq;
+  const uint32_t qc = qi < nq ? qi : nq - 1;
   const int64_t i0 = plane * P.share + chunk * P.chunk_items;
   const int64_t i1 = i0 + P.chunk_items < (plane + 1) * P.share ? i0 + P.chunk_items : (plane + 1) * P.share;
 
@@ -678,11 +692,10 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dbias_kernel(D
     for (int m = 0; m < 2; ++m) {
       f32x4 p[4];
       tile_weights<T, D, kDaKeys, 4>(tile, m, 0, qf[m], b, P.scale_log2, rs[m], li, lg, p);
-      const float by = m ? -lam : 1.f;
 #pragma unroll
       for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) acc[kt][r] = fmaf(p[kt][r] * by, dp[kt][r] - rs[2 + m], acc[kt][r]);
+        for (int r = 0; r < 4; ++r) acc[kt][r] = fmaf(m ? p[kt][r] * -lam : p[kt][r], dp[kt][r] - rs[2 + m], acc[kt][r]);
     }
     if (more) {
       st.store(tiles[buf ^ 1]);
@@ -690,7 +703,7 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dbias_kernel(D
     }
     __syncthreads();
   }
-  if (qi >= P.nq) return;
+  if (qi >= nq) return;
   float* out = P.part_bias + (((int64_t)chunk * planes + plane) * P.heads + head) * P.nq * P.nk + qi * P.nk;
   const int64_t k0 = kb * 64 + 4 * lg;
 #pragma unroll
@@ -718,17 +731,20 @@ template <typename T, int D>
 void bwd(const DiffAttnParams<T>& P, hipStream_t st) {
   const int64_t kvh = P.heads / P.group;
   // Waves with rows (keys) of their own cost the least work; they share 16 where
-  // that leaves too few workgroups for the card's 256 CUs. D = 32, bf16, 6 heads,
-  // us own / shared: dq at 96 workgroups (2 x 499 tokens) 19.0 / 15.3, 144 19.1 /
-  // 22.1, 192 22.2 / 23.8, 240 19.9 / 26.6; dk and dv 28.3 / 17.4, 28.1 / 25.2, 29.7
-  // / 26.8, 29.2 / 30.5. float32 at 48 (2 x 256): 27.7 / 14.1 and 29.9 / 13.4.
+  // that leaves too few workgroups for the card's 256 CUs. us own / shared, 499
+  // tokens: dq in bf16 at D = 32 at 96 workgroups 18.8 / 14.9, 144 19.1 / 21.6; at
+  // D = 64 120 29.0 / 30.2; float32 D = 32 120 46.9 / 33.5, 144 48.0 / 47.6; D = 64
+  // 120 89 / 69. dk and dv in bf16 at D = 32 at 192 28.4 / 27.1, 240 29.4 / 31.1; at
+  // D = 64 120 37.8 / 34.7, 144 38.2 / 50.3; float32 D = 32 120 59.9 / 43.2, 144 61.1
+  // / 61.9.
+  constexpr int64_t kFewKeys = sizeof(T) == 2 && D == 32 ? 224 : 128;
   const int64_t heads = P.items * kvh, rows = P.group * P.nq;
   if (heads * ((rows + 63) / 64) >= 128)
     diffattn_dq_kernel<T, D, false><<<eights(heads * ((rows + 63) / 64)), 256, 0, st>>>(P);
   else
     diffattn_dq_kernel<T, D, true><<<eights(heads * ((rows + 15) / 16)), 256, 0, st>>>(P);
   const bool own = P.dbias.p && P.share == 1;
-  if (heads * ((P.nk + 63) / 64) >= 224) {
+  if (heads * ((P.nk + 63) / 64) >= kFewKeys) {
     const unsigned blocks = eights(P.heads) + eights(heads * ((P.nk + 63) / 64));
     if (own)
       diffattn_dkv_kernel<T, D, false, true><<<blocks, 256, 0, st>>>(P);
