@@ -28,25 +28,26 @@ constexpr float kSlack = 8.f;
 // starts and ends (4 blocks of keys each). One token of 8 sequences against 16384
 // keys (134 MB, keywise and split): 26.5 us, the copy rate, and 4.3 for the join.
 //
-// KEYWISE: the four waves share one 16-row tile and take 32 keys each of a
-// 128-key block, for calls with few rows; otherwise each has 16 rows of its own
-// and walks every 64-key block.
-template <typename T, int D, bool KEYWISE>
-__global__ __launch_bounds__(256, (kDaWaves<T, D> + (kDaWaves<T, D> > 1))) void diffattn_fwd_kernel(DiffAttnParams<T> P) {
-  constexpr int kRows = KEYWISE ? 128 : 64;    // keys of a block
-  constexpr int kNt = KEYWISE ? 2 : 4;         // key tiles of a wave in one
+// KS 4 (keywise): the four waves share one 16-row tile and take 32 keys each of a
+// 128-key block, for calls with few rows; KS 1: each has 16 rows of its own and
+// walks every 64-key block.
+template <typename T, int D, int KS>
+__global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D> + (kDaWaves<T, D> > 1))) void diffattn_fwd_kernel(DiffAttnParams<T> P) {
+  typedef DaForm<KS> Form;
+  constexpr int kRows = Form::kBlock;          // keys of a block
+  constexpr int kNt = kRows / KS / 16;         // key tiles of a wave in one
   // one block in LDS where the waves share it, for the sake of a second and third
   // workgroup on a CU (two blocks: 18.6 -> 23.5 us at 4 x 499 tokens)
-  constexpr int kBufs = KEYWISE ? 1 : 2;
+  constexpr int kBufs = KS == 4 ? 1 : 2;
   constexpr int kC = D / 32, kU = 2 * D / 16;  // k-steps of a score, tiles of 16 values
   typedef typename Frag<T>::type F;
   typedef DaTile<T, D, kRows> Tile;
-  constexpr size_t kMerge = 4 * 16 * 2 * (2 * D + 4) * sizeof(float);
+  constexpr size_t kMerge = Form::kWaves * 16 * 2 * (2 * D + 4) * sizeof(float);
   constexpr size_t kBytes = kBufs * sizeof(Tile);
-  static_assert(!KEYWISE || kBytes >= kMerge, "the waves' sums");
+  static_assert(KS == 1 || kBytes >= kMerge, "the waves' sums");
   __shared__ __attribute__((aligned(16))) unsigned char raw[kBytes];
   __shared__ __attribute__((aligned(16))) KeyFlags<kRows> flags[3];  // of the block at hand and the next two
-  __shared__ float lams[4][16];  // of the waves' rows
+  __shared__ float lams[Form::kWaves][16];  // of the waves' rows
   Tile* tiles = reinterpret_cast<Tile*>(raw);
 
   const int t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
@@ -54,7 +55,7 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D> + (kDaWaves<T, D> > 1))) void 
   const int kvh = P.heads / P.group;
   // 32 bits from here to the item: a launch has fewer than 2^23 workgroups
   const uint32_t nq = (uint32_t)P.nq, rows = P.group * nq;  // of one key/value head
-  const uint32_t row_blocks = KEYWISE ? (rows + 15) / 16 : (rows + 63) / 64;
+  const uint32_t row_blocks = (rows + Form::kTiles * 16 - 1) / (Form::kTiles * 16);
   uint32_t id = xcd_order(blockIdx.x, gridDim.x);
   if (id >= (uint32_t)P.items * kvh * row_blocks * P.splits) return;
   const uint32_t rb = id % row_blocks;
@@ -64,14 +65,15 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D> + (kDaWaves<T, D> > 1))) void 
   const int kv = id % (uint32_t)kvh;
   const int64_t item = id / (uint32_t)kvh;
 
-  const uint32_t row = KEYWISE ? rb * 16 + li : rb * 64 + 16 * wave + li;
+  const int tile_of = wave % Form::kTiles, ks = wave / Form::kTiles;  // its tile of 16 rows, and its part of a block's keys
+  const uint32_t row = (rb * Form::kTiles + tile_of) * 16 + li;
   const bool row_on = row < rows;
   const uint32_t row_c = row_on ? row : rows - 1;
   const int hg = row_c / nq;
   const uint32_t qi = row_c - hg * nq;
   const int head = kv * P.group + hg;
 
-  DaStage<T, D, kRows, 256> st;
+  DaStage<T, D, kRows, Form::kThreads> st;
   st.init(P.k.p + item * P.k.item + 2 * kv * P.k.head, P.k.head, P.k.token, P.v.p + item * P.v.item + kv * P.v.head,
           P.v.token, t);
   const uint8_t* mask = P.mask ? P.mask + item * P.nk : nullptr;
@@ -95,7 +97,7 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D> + (kDaWaves<T, D> > 1))) void 
   auto put_flags = [&](int at) {
     if (t < kRows) flags[at].set(t, part != 0);
   };
-  const int key_w = KEYWISE ? 32 * wave : 0;  // this wave's keys of a block
+  const int key_w = kRows / KS * ks;  // this wave's keys of a block
   typename Quad<T>::type bv[kNt] = {};  // zeros without a bias
   auto load_bias = [&](int64_t blk) {
     bias_tile<T, kNt>(bias, blk * kRows + key_w + 4 * lg, P.nk, (blk + 1) * kRows <= P.nk, bv);
@@ -228,53 +230,52 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D> + (kDaWaves<T, D> > 1))) void 
 #pragma unroll
   for (int mp = 0; mp < 2; ++mp) ls[mp] = kOnes ? l[mp][0] : group_sum((l[mp][0] + l[mp][1]) + (l[mp][2] + l[mp][3]));
 
-  if constexpr (KEYWISE) {
-    // the waves' partial rows, on the largest of their maxima
-    float* ml = reinterpret_cast<float*>(raw);                 // [wave][map][row][2]
-    float* po = ml + 4 * 2 * 16 * 2;                           // [wave][map][row][2 D + 2]
+  constexpr int kOwn = kU / KS;
+  const int u0 = ks * kOwn;
+  if constexpr (KS > 1) {
+    // the partial rows of the waves that share them, on the largest of their maxima
     constexpr int kPo = 2 * D + 2;
+    float* ml = reinterpret_cast<float*>(raw);       // [wave][map][row][2]
+    float* po = ml + Form::kWaves * 2 * 16 * 2;      // [wave][map][row][2 D + 2]
+    auto slot = [&](int j, int mp) { return ((Form::kTiles * j + tile_of) * 2 + mp) * 16 + li; };  // of the tile's j-th wave
     if (lg == 0)
       for (int mp = 0; mp < 2; ++mp) {
-        ml[((wave * 2 + mp) * 16 + li) * 2] = m[mp];
-        ml[((wave * 2 + mp) * 16 + li) * 2 + 1] = ls[mp];
+        ml[slot(ks, mp) * 2] = m[mp];
+        ml[slot(ks, mp) * 2 + 1] = ls[mp];
       }
     __syncthreads();
 #pragma unroll
     for (int mp = 0; mp < 2; ++mp) {
       float mx = -INFINITY, sum = 0.f;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) mx = fmaxf(mx, ml[((w * 2 + mp) * 16 + li) * 2]);
+      for (int j = 0; j < KS; ++j) mx = fmaxf(mx, ml[slot(j, mp) * 2]);
       const float base = exponent_base(mx);
 #pragma unroll
-      for (int w = 0; w < 4; ++w)
-        sum = fmaf(ml[((w * 2 + mp) * 16 + li) * 2 + 1],
-                   __builtin_amdgcn_exp2f(ml[((w * 2 + mp) * 16 + li) * 2] - base), sum);
+      for (int j = 0; j < KS; ++j) sum = fmaf(ml[slot(j, mp) * 2 + 1], __builtin_amdgcn_exp2f(ml[slot(j, mp) * 2] - base), sum);
       const float alpha = __builtin_amdgcn_exp2f(m[mp] - base);
 #pragma unroll
       for (int u = 0; u < kU; ++u)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) po[((wave * 2 + mp) * 16 + li) * kPo + 16 * u + 4 * lg + r] = o[mp][u][r] * alpha;
+        for (int r = 0; r < 4; ++r) po[slot(ks, mp) * kPo + 16 * u + 4 * lg + r] = o[mp][u][r] * alpha;
       m[mp] = mx;
       ls[mp] = sum;
     }
     __syncthreads();
-    // each wave takes kU / 4 of the tiles of 16 values
+    // each wave takes its share of the tiles of 16 values
 #pragma unroll
     for (int mp = 0; mp < 2; ++mp)
 #pragma unroll
-      for (int u = 0; u < kU / 4; ++u)
+      for (int u = 0; u < kOwn; ++u)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           float a = 0.f;
 #pragma unroll
-          for (int w = 0; w < 4; ++w) a += po[((w * 2 + mp) * 16 + li) * kPo + 16 * (wave * (kU / 4) + u) + 4 * lg + r];
+          for (int j = 0; j < KS; ++j) a += po[slot(j, mp) * kPo + 16 * (u0 + u) + 4 * lg + r];
           o[mp][u][r] = a;
         }
   }
   if (!row_on) return;
-  constexpr int kOwn = KEYWISE ? kU / 4 : kU;
-  const int u0 = KEYWISE ? wave * kOwn : 0;
-  const bool first = lg == 0 && (!KEYWISE || wave == 0);
+  const bool first = lg == 0 && ks == 0;
   const int64_t at = item * P.heads * P.nq + (int64_t)head * P.nq + qi;
   if (P.splits > 1) {
     const int64_t base = (split * (P.items * P.heads * P.nq) + at) * 2;
@@ -369,16 +370,21 @@ __global__ __launch_bounds__(256) void diffattn_join_kernel(DiffAttnParams<T> P)
   for (int j = 0; j < kV; ++j) out[64 * j + lane] = from_f32<T>(res[j]);
 }
 
+template <typename T, int D, int KS>
+void fwd_form(const DiffAttnParams<T>& P, hipStream_t st) {
+  constexpr int kTile = DaForm<KS>::kTiles * 16;
+  const int64_t blocks = P.items * (P.heads / P.group) * P.splits * ((P.group * P.nq + kTile - 1) / kTile);
+  diffattn_fwd_kernel<T, D, KS><<<(unsigned)((blocks + 7) / 8 * 8), DaForm<KS>::kThreads, 0, st>>>(P);
+}
+
 template <typename T, int D>
 void fwd(const DiffAttnParams<T>& P, bool keywise, hipStream_t st) {
-  const int64_t rows = P.group * P.nq;
-  const int64_t blocks = P.items * (P.heads / P.group) * P.splits * (keywise ? (rows + 15) / 16 : (rows + 63) / 64);
-  const dim3 grid((unsigned)((blocks + 7) / 8 * 8));
-  if (keywise)
-    diffattn_fwd_kernel<T, D, true><<<grid, 256, 0, st>>>(P);
-  else
-    diffattn_fwd_kernel<T, D, false><<<grid, 256, 0, st>>>(P);
-  if (P.splits > 1) diffattn_join_kernel<T, D><<<(unsigned)(P.items * P.heads * P.nq), 256, 0, st>>>(P);
+  if (keywise) {
+    fwd_form<T, D, 4>(P, st);
+    if (P.splits > 1) diffattn_join_kernel<T, D><<<(unsigned)(P.items * P.heads * P.nq), 256, 0, st>>>(P);
+    return;
+  }
+  fwd_form<T, D, 1>(P, st);
 }
 
 }  // namespace

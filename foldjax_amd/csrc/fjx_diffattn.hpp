@@ -71,6 +71,17 @@ __device__ __forceinline__ float exponent(float s, float b, float scale_log2, fl
   return kBiasFirst<T> ? fmaf(s, scale_log2, -base) : fmaf(s, scale_log2, b) - base;
 }
 
+// How the waves of a workgroup share its rows (for the keys' gradients: its keys)
+// and a staged block: KS of them have a tile of 16 rows and a KS-th of a block each.
+// KS 1: four waves, four tiles, blocks of 64; 4: four waves, one tile, blocks of
+// 128; 2: eight waves, four tiles, blocks of 128.
+template <int KS>
+struct DaForm {
+  static constexpr int kWaves = KS == 2 ? 8 : 4, kThreads = 64 * kWaves;
+  static constexpr int kTiles = kWaves / KS;
+  static constexpr int kBlock = KS == 1 ? 64 : 128;
+};
+
 constexpr int kDaKeys = 64;  // keys (or, for the keys' gradients, queries) of a staged block
 
 // one staged block: the two maps' D columns side by side, and 2 D columns; rows

@@ -65,39 +65,41 @@ __device__ __forceinline__ float sum8(const float (&x)[8]) {
 // rows of 245 tokens and 2 heads, 46 % vector and 14 % matrix instructions, a quarter
 // of it starts and ends; 19 us at 4 x 499 tokens and 6 heads.
 //
-// SPLIT: the four waves share 16 rows and take 32 keys each of a 128-key
-// block, for calls with few rows; otherwise each has rows of its own.
-template <typename T, int D, bool SPLIT>
-__global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dq_kernel(DiffAttnParams<T> P) {
-  constexpr int kRows = SPLIT ? 128 : 64, kNt = SPLIT ? 2 : 4, kBufs = SPLIT ? 1 : 2;
+// KS 4: the four waves share 16 rows and take 32 keys each of a 128-key block, for
+// calls with few rows; KS 1: each has rows of its own.
+template <typename T, int D, int KS>
+__global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diffattn_dq_kernel(DiffAttnParams<T> P) {
+  typedef DaForm<KS> Form;
+  constexpr int kRows = Form::kBlock, kNt = kRows / KS / 16, kBufs = KS == 4 ? 1 : 2;
   constexpr int kC = D / 32, kU = D / 16;
   typedef typename Frag<T>::type F;
   typedef DaTile<T, D, kRows> Tile;
   constexpr int kPo = D + 2;
-  static_assert(!SPLIT || sizeof(Tile) >= 4 * 2 * 16 * kPo * sizeof(float), "the waves' sums");
+  static_assert(KS == 1 || kBufs * sizeof(Tile) >= Form::kWaves * 2 * 16 * kPo * sizeof(float), "the waves' sums");
   __shared__ __attribute__((aligned(16))) Tile tiles[kBufs];
   __shared__ __attribute__((aligned(16))) KeyFlags<kRows> flags[3];  // of the block at hand and the next two
-  __shared__ float joined[4][3][16];
+  __shared__ float joined[Form::kWaves][3][16];
 
   const int t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int kvh = P.heads / P.group;
-  const uint32_t nq = (uint32_t)P.nq, rows = P.group * nq, row_blocks = SPLIT ? (rows + 15) / 16 : (rows + 63) / 64;
+  const uint32_t nq = (uint32_t)P.nq, rows = P.group * nq, row_blocks = (rows + Form::kTiles * 16 - 1) / (Form::kTiles * 16);
   uint32_t id = xcd_order(blockIdx.x, gridDim.x);
   if (id >= (uint32_t)P.items * kvh * row_blocks) return;
   const uint32_t rb = id % row_blocks;
   id /= row_blocks;
   const int kv = id % (uint32_t)kvh;
   const int64_t item = id / (uint32_t)kvh;
-  const uint32_t row = SPLIT ? rb * 16 + li : rb * 64 + 16 * wave + li;
+  const int tile_of = wave % Form::kTiles, ks = wave / Form::kTiles;  // its tile of 16 rows, and its part of a block's keys
+  const uint32_t row = (rb * Form::kTiles + tile_of) * 16 + li;
   const bool row_on = row < rows;
   const uint32_t row_c = row_on ? row : rows - 1;
   const int hg = row_c / nq;
   const int64_t qi = row_c - hg * nq;
   const int head = kv * P.group + hg;
-  const int key_w = SPLIT ? 32 * wave : 0;  // this wave's keys of a block
+  const int key_w = kRows / KS * ks;  // this wave's keys of a block
 
-  DaStage<T, D, kRows, 256> st;
+  DaStage<T, D, kRows, Form::kThreads> st;
   st.init(P.k.p + item * P.k.item + 2 * kv * P.k.head, P.k.head, P.k.token, P.v.p + item * P.v.item + kv * P.v.head,
           P.v.token, t);
   const uint8_t* mask = P.mask ? P.mask + item * P.nk : nullptr;
@@ -141,6 +143,15 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dq_kernel(Diff
   st.load(0, flags[0].whole(), flags[0].on);
   const float lam = da_lambda<D>(P.lam, P.heads, head, P.init, lane);
 
+  // the sum of the tile's waves' `joined`, in one order
+  auto of_tile = [&](int x) {
+    float v[KS];
+#pragma unroll
+    for (int j = 0; j < KS; ++j) v[j] = joined[Form::kTiles * j + tile_of][x][li];
+    if constexpr (KS == 4) return (v[0] + v[1]) + (v[2] + v[3]);
+    if constexpr (KS == 2) return v[0] + v[1];
+    return v[0];
+  };
   float c0 = 0.f, Dt[2] = {0.f, 0.f}, total = 0.f;  // D_t - c; the second map's weights
   f32x4 us[2][kU], ws[2][kU];
 #pragma unroll
@@ -184,11 +195,11 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dq_kernel(Diff
         }
       sp = group_sum(sp);
       sd = group_sum(sd);
-      if constexpr (SPLIT) {
+      if constexpr (KS > 1) {
         if (lg == 0) joined[wave][0][li] = sp, joined[wave][1][li] = sd;
         __syncthreads();
-        sp = (joined[0][0][li] + joined[1][0][li]) + (joined[2][0][li] + joined[3][0][li]);
-        sd = (joined[0][1][li] + joined[1][1][li]) + (joined[2][1][li] + joined[3][1][li]);
+        sp = of_tile(0);
+        sd = of_tile(1);
       }
       c0 = sp > 0.f ? sd / sp : 0.f;
     }
@@ -228,36 +239,38 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dq_kernel(Diff
 #pragma unroll
   for (int m = 0; m < 2; ++m) Dt[m] = group_sum(Dt[m]);
   total = group_sum(total);
-  if constexpr (SPLIT) {  // the waves' sums, through the tile's memory
+  if constexpr (KS > 1) {  // the waves' sums, through the tiles' memory
     if (lg == 0) joined[wave][0][li] = Dt[0], joined[wave][1][li] = Dt[1], joined[wave][2][li] = total;
     __syncthreads();
-    total = (joined[0][2][li] + joined[1][2][li]) + (joined[2][2][li] + joined[3][2][li]);
+    total = of_tile(2);
     float* po = reinterpret_cast<float*>(&tiles[0]);  // [wave][map][row][D + 2]
+    auto slot = [&](int j, int m) { return (((Form::kTiles * j + tile_of) * 2 + m) * 16 + li) * kPo; };  // of the tile's j-th wave
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
-      Dt[m] = (joined[0][m][li] + joined[1][m][li]) + (joined[2][m][li] + joined[3][m][li]);
+      Dt[m] = of_tile(m);
       if (m == 1 && total > 0.f) Dt[m] /= total;
 #pragma unroll
       for (int u = 0; u < kU; ++u)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) po[((wave * 2 + m) * 16 + li) * kPo + 16 * u + 4 * lg + r] = us[m][u][r] - Dt[m] * ws[m][u][r];
+        for (int r = 0; r < 4; ++r) po[slot(ks, m) + 16 * u + 4 * lg + r] = us[m][u][r] - Dt[m] * ws[m][u][r];
     }
     __syncthreads();
-    // each wave writes half a map
-    const int m = wave >> 1;
+    // each wave writes its share of the two maps' tiles of 16 columns
+    constexpr int kOwn = 2 * kU / KS;
+    const int m = ks * 2 / KS, first = ks * kOwn % kU;
     if (!row_on) return;
-    if (lg == 0 && (wave & 1) == 0) P.delta[(item * 2 * P.heads + 2 * head + m) * P.nq + qi] = Dt[m] + c0;
+    if (lg == 0 && first == 0) P.delta[(item * 2 * P.heads + 2 * head + m) * P.nq + qi] = Dt[m] + c0;
     const float by = P.scale * (m ? -lam : 1.f);
     T* out = P.dq.p + item * P.dq.item + (2 * head + m) * P.dq.head + qi * P.dq.token;
 #pragma unroll
-    for (int u = 0; u < kU / 2; ++u) {
-      const int col = 16 * ((wave & 1) * (kU / 2) + u) + 4 * lg;
+    for (int u = 0; u < kOwn; ++u) {
+      const int col = 16 * (first + u) + 4 * lg;
       float v[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         float x = 0.f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) x += po[((w * 2 + m) * 16 + li) * kPo + col + r];
+        for (int j = 0; j < KS; ++j) x += po[slot(j, m) + col + r];
         v[r] = x * by;
       }
       store4f(out + col, v);
@@ -284,13 +297,13 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dq_kernel(Diff
 // dlambda_h = -sum over items and queries of D_2, and the four vectors'
 // gradients from it, by one workgroup a head: the first of the launch for dk
 // and dv, in whose shadow they run.
-template <typename T, int D>
-__device__ __forceinline__ void dlambda_of(const DiffAttnParams<T>& P, int head, double (&lds)[4]) {
+template <typename T, int D, int WAVES>
+__device__ __forceinline__ void dlambda_of(const DiffAttnParams<T>& P, int head, double (&lds)[WAVES]) {
   const int t = threadIdx.x;
   const int64_t n = P.items * P.nq;
   double s = 0.;  // many numbers of either sign
 #pragma unroll 8
-  for (int64_t i = t; i < n; i += 256) {
+  for (int64_t i = t; i < n; i += 64 * WAVES) {
     const int64_t item = n >> 32 ? i / P.nq : (uint32_t)i / (uint32_t)P.nq;
     s += P.delta[(item * 2 * P.heads + 2 * head + 1) * P.nq + i - item * P.nq];
   }
@@ -299,7 +312,10 @@ __device__ __forceinline__ void dlambda_of(const DiffAttnParams<T>& P, int head,
   if ((t & 63) == 0) lds[t >> 6] = s;
   __syncthreads();
   if (t >= 64) return;
-  const float dl = (float)-((lds[0] + lds[1]) + (lds[2] + lds[3]));
+  double sum = 0.;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) sum += lds[w];
+  const float dl = (float)-sum;
   float e[2];
   da_lambda<D>(P.lam, P.heads, head, P.init, t, e);
   if (t < D) {
@@ -317,28 +333,31 @@ __device__ __forceinline__ void dlambda_of(const DiffAttnParams<T>& P, int head,
 // and walks the query blocks of every head that shares them. S_t = Q_t K_t^T
 // leaves the lane 4 queries of its key a tile, the operand of dS_t^T Q_t and of
 // (P_1 - lambda P_2)^T dO as they lie. It also writes dbias, where every item has
-// a plane of its own. SPLIT: the four waves share 16 keys and take 32 queries
-// each of a 128-query block, for calls with few keys. Bound like the kernel for
-// dq: 63 us at 245 rows of 245 tokens and 2 heads, 27 us with dbias at 4 x 499 and 6.
-template <typename T, int D, bool SPLIT, bool DBIAS>
-__global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dkv_kernel(DiffAttnParams<T> P) {
-  constexpr int kC = D / 32, kU = D / 16, kQ = SPLIT ? 128 : 64, kQt = SPLIT ? 2 : 4, kBufs = SPLIT ? 1 : 2;
+// a plane of its own. KS 4: the four waves share 16 keys and take 32 queries each
+// of a 128-query block, for calls with few keys; 2: two of eight share 16 and take
+// 64 each, so that a CU with one workgroup has two waves a SIMD. Bound like the
+// kernel for dq: 63 us at 245 rows of 245 tokens and 2 heads, 24 us with dbias at
+// 4 x 499 and 6.
+template <typename T, int D, int KS, bool DBIAS>
+__global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diffattn_dkv_kernel(DiffAttnParams<T> P) {
+  typedef DaForm<KS> Form;
+  constexpr int kC = D / 32, kU = D / 16, kQ = Form::kBlock, kQt = kQ / KS / 16, kBufs = KS == 4 ? 1 : 2;
   typedef typename Frag<T>::type F;
   typedef DaTile<T, D, kQ> Tile;
   constexpr int kPo = 4 * D + 2;
-  static_assert(!SPLIT || sizeof(Tile) >= 4 * 16 * kPo * sizeof(float), "the waves' sums");
+  static_assert(KS == 1 || kBufs * sizeof(Tile) >= Form::kWaves * 16 * kPo * sizeof(float), "the waves' sums");
   __shared__ __attribute__((aligned(16))) Tile tiles[kBufs];
   __shared__ __attribute__((aligned(16))) float row_stat[kBufs][4][kQ];  // L_1, L_2, D_1, D_2
   __shared__ float query_on[kQ];
-  __shared__ double lam_lds[4];
+  __shared__ double lam_lds[Form::kWaves];
 
   const int t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int kvh = P.heads / P.group;
-  const uint32_t key_blocks = SPLIT ? (P.nk + 15) / 16 : (P.nk + 63) / 64;
+  const uint32_t key_blocks = (P.nk + Form::kTiles * 16 - 1) / (Form::kTiles * 16);
   const uint32_t lams = (P.heads + 7) / 8 * 8;
   if (blockIdx.x < lams) {
-    if (blockIdx.x < (uint32_t)P.heads) dlambda_of<T, D>(P, blockIdx.x, lam_lds);
+    if (blockIdx.x < (uint32_t)P.heads) dlambda_of<T, D, Form::kWaves>(P, blockIdx.x, lam_lds);
     return;
   }
   uint32_t id = xcd_order(blockIdx.x - lams, gridDim.x - lams);
@@ -347,8 +366,9 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dkv_kernel(Dif
   id /= key_blocks;
   const int kv = id % (uint32_t)kvh;
   const int64_t item = id / (uint32_t)kvh;
-  const int64_t key = SPLIT ? kb * 16 + li : kb * 64 + 16 * wave + li;
-  const int q_w = SPLIT ? 32 * wave : 0;  // this wave's queries of a block
+  const int tile_of = wave % Form::kTiles, ks = wave / Form::kTiles;  // its tile of 16 keys, and its part of a block's queries
+  const int64_t key = ((int64_t)kb * Form::kTiles + tile_of) * 16 + li;
+  const int q_w = kQ / KS * ks;  // this wave's queries of a block
   const bool in = key < P.nk;
   uint8_t there = in;
   if (in && P.mask) there = P.mask[item * P.nk + key];
@@ -374,7 +394,7 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dkv_kernel(Dif
   T* dbias = DBIAS ? P.dbias.p + plane * P.dbias.item : nullptr;
 
   const int64_t q_blocks = (P.nq + kQ - 1) / kQ;
-  DaStage<T, D, kQ, 256> st;
+  DaStage<T, D, kQ, Form::kThreads> st;
   const int h0 = kv * P.group;
   st.init(P.q.p + item * P.q.item + 2 * h0 * P.q.head, P.q.head, P.q.token, P.dout.p + item * P.dout.item + h0 * P.dout.head,
           P.dout.token, t);
@@ -383,15 +403,15 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dkv_kernel(Dif
   // the last block's queries, as KeyFlags::on
   if (t < kQ) query_on[t] = (q_blocks - 1) * kQ + t < P.nq ? 1.f : -1.f;
   __syncthreads();
-  constexpr int kStats = 4 * kQ / 256;  // statistics that a thread stages
+  constexpr int kStats = 4 * kQ / Form::kThreads;  // statistics that a thread stages
   float stat[kStats];
   auto fetch = [&](int hg, int64_t qb) {
     st.src = src0 + hg * head_step;
     st.load(qb * kQ, (qb + 1) * kQ <= P.nq, query_on);
 #pragma unroll
     for (int i = 0; i < kStats; ++i) {
-      const int which = (t + 256 * i) / kQ;
-      const int64_t q = qb * kQ + (t + 256 * i) % kQ;
+      const int which = (t + Form::kThreads * i) / kQ;
+      const int64_t q = qb * kQ + (t + Form::kThreads * i) % kQ;
       const int64_t at = (item * 2 * P.heads + 2 * (h0 + hg) + (which & 1)) * P.nq + q;
       stat[i] = which < 2 ? INFINITY : 0.f;  // past the last query: weights of zero
       if (q < P.nq) stat[i] = which < 2 ? P.saved[at] : P.delta[at];
@@ -400,7 +420,7 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dkv_kernel(Dif
   auto put = [&](int buf) {
     st.store(tiles[buf]);
 #pragma unroll
-    for (int i = 0; i < kStats; ++i) row_stat[buf][(t + 256 * i) / kQ][(t + 256 * i) % kQ] = stat[i];
+    for (int i = 0; i < kStats; ++i) row_stat[buf][(t + Form::kThreads * i) / kQ][(t + Form::kThreads * i) % kQ] = stat[i];
   };
   // a lane's element of the bias in a tile's 16 rows (less than 2^23 elements
   // apart): its row and its key; the tile's first row is scalar
@@ -534,7 +554,7 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dkv_kernel(Dif
       __syncthreads();
     }
   }
-  if constexpr (SPLIT) {  // the waves' sums, through the tile's memory: [wave][key][dk_1, dk_2, dv]
+  if constexpr (KS > 1) {  // the waves' sums, through the tiles' memory: [wave][key][dk_1, dk_2, dv]
     float* po = reinterpret_cast<float*>(&tiles[0]);
     float* own = po + (wave * 16 + li) * kPo + 4 * lg;
 #pragma unroll
@@ -543,20 +563,24 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D>)) void diffattn_dkv_kernel(Dif
       for (int r = 0; r < 4; ++r) own[16 * u + r] = u < 2 * kU ? dk[u / kU][u % kU][r] : dv[u < 2 * kU ? 0 : u - 2 * kU][r];
     __syncthreads();
     if (!in) return;
-    // wave 0 writes dk_1, wave 1 dk_2, the others half of dv each
-    T* out = wave < 2 ? P.dk.p + item * P.dk.item + (2 * kv + wave) * P.dk.head + key * P.dk.token
-                      : P.dv.p + item * P.dv.item + kv * P.dv.head + key * P.dv.token + (wave - 2) * D;
+    // each wave writes 4 / KS of dk_1, dk_2 and the two halves of dv
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      float v[4];
+    for (int x = 0; x < 4 / KS; ++x) {
+      const int part_of = ks * (4 / KS) + x;
+      T* out = part_of < 2 ? P.dk.p + item * P.dk.item + (2 * kv + part_of) * P.dk.head + key * P.dk.token
+                           : P.dv.p + item * P.dv.item + kv * P.dv.head + key * P.dv.token + (part_of - 2) * D;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float x = 0.f;
+      for (int u = 0; u < kU; ++u) {
+        float v[4];
 #pragma unroll
-        for (int w = 0; w < 4; ++w) x += po[(w * 16 + li) * kPo + wave * D + 16 * u + 4 * lg + r];
-        v[r] = wave < 2 ? x * P.scale : x;
+        for (int r = 0; r < 4; ++r) {
+          float sum = 0.f;
+#pragma unroll
+          for (int j = 0; j < KS; ++j) sum += po[((Form::kTiles * j + tile_of) * 16 + li) * kPo + part_of * D + 16 * u + 4 * lg + r];
+          v[r] = part_of < 2 ? sum * P.scale : sum;
+        }
+        store4f(out + 16 * u + 4 * lg, v);
       }
-      store4f(out + 16 * u + 4 * lg, v);
     }
     return;
   }
@@ -727,36 +751,47 @@ __global__ __launch_bounds__(256) void diffattn_bias_sum_kernel(DiffAttnParams<T
 
 unsigned eights(int64_t blocks) { return (unsigned)((blocks + 7) / 8 * 8); }
 
+template <typename T, int D, int KS>
+void dq_form(const DiffAttnParams<T>& P, hipStream_t st) {
+  constexpr int kTile = DaForm<KS>::kTiles * 16;
+  const int64_t blocks = P.items * (P.heads / P.group) * ((P.group * P.nq + kTile - 1) / kTile);
+  diffattn_dq_kernel<T, D, KS><<<eights(blocks), DaForm<KS>::kThreads, 0, st>>>(P);
+}
+template <typename T, int D, int KS>
+void dkv_form(const DiffAttnParams<T>& P, hipStream_t st) {
+  constexpr int kTile = DaForm<KS>::kTiles * 16;
+  const unsigned blocks = eights(P.heads) + eights(P.items * (P.heads / P.group) * ((P.nk + kTile - 1) / kTile));
+  if (P.dbias.p && P.share == 1)
+    diffattn_dkv_kernel<T, D, KS, true><<<blocks, DaForm<KS>::kThreads, 0, st>>>(P);
+  else
+    diffattn_dkv_kernel<T, D, KS, false><<<blocks, DaForm<KS>::kThreads, 0, st>>>(P);
+}
+
 template <typename T, int D>
 void bwd(const DiffAttnParams<T>& P, hipStream_t st) {
   const int64_t kvh = P.heads / P.group;
   // Waves with rows (keys) of their own cost the least work; they share 16 where
-  // that leaves too few workgroups for the card's 256 CUs. us own / shared, 499
-  // tokens: dq in bf16 at D = 32 at 96 workgroups 18.8 / 14.9, 144 19.1 / 21.6; at
+  // that leaves too few workgroups for the card's 256 CUs. us own / shared by four,
+  // 499 tokens: dq in bf16 at D = 32 at 96 workgroups 18.8 / 14.9, 144 19.1 / 21.6; at
   // D = 64 120 29.0 / 30.2; float32 D = 32 120 46.9 / 33.5, 144 48.0 / 47.6; D = 64
-  // 120 89 / 69. dk and dv in bf16 at D = 32 at 192 28.4 / 27.1, 240 29.4 / 31.1; at
-  // D = 64 120 37.8 / 34.7, 144 38.2 / 50.3; float32 D = 32 120 59.9 / 43.2, 144 61.1
-  // / 61.9.
-  constexpr int64_t kFewKeys = sizeof(T) == 2 && D == 32 ? 224 : 128;
+  // 120 89 / 69. dk and dv at D = 64 120 37.8 / 34.7, 144 38.2 / 50.3; float32 D = 32
+  // 120 59.9 / 43.2, 144 61.1 / 61.9; bf16 at D = 32, own / by two / by four: 144 27.8 /
+  // 23.0 / 25.8, 192 28.4 / 24.3 / 27.1, 240 29.3 / 24.6 / 31.1 (one such workgroup
+  // fits a CU; the other types' registers leave one wave a SIMD). By two gains
+  // nothing in the forward kernel and dq (18.3 and 19.5 either way at 192).
+  constexpr bool kPaired = sizeof(T) == 2 && D == 32;
   const int64_t heads = P.items * kvh, rows = P.group * P.nq;
-  if (heads * ((rows + 63) / 64) >= 128)
-    diffattn_dq_kernel<T, D, false><<<eights(heads * ((rows + 63) / 64)), 256, 0, st>>>(P);
+  const int64_t row_wgs = heads * ((rows + 63) / 64), key_wgs = heads * ((P.nk + 63) / 64);
+  if (row_wgs < 128)
+    dq_form<T, D, 4>(P, st);
   else
-    diffattn_dq_kernel<T, D, true><<<eights(heads * ((rows + 15) / 16)), 256, 0, st>>>(P);
-  const bool own = P.dbias.p && P.share == 1;
-  if (heads * ((P.nk + 63) / 64) >= kFewKeys) {
-    const unsigned blocks = eights(P.heads) + eights(heads * ((P.nk + 63) / 64));
-    if (own)
-      diffattn_dkv_kernel<T, D, false, true><<<blocks, 256, 0, st>>>(P);
-    else
-      diffattn_dkv_kernel<T, D, false, false><<<blocks, 256, 0, st>>>(P);
-  } else {
-    const unsigned blocks = eights(P.heads) + eights(heads * ((P.nk + 15) / 16));
-    if (own)
-      diffattn_dkv_kernel<T, D, true, true><<<blocks, 256, 0, st>>>(P);
-    else
-      diffattn_dkv_kernel<T, D, true, false><<<blocks, 256, 0, st>>>(P);
-  }
+    dq_form<T, D, 1>(P, st);
+  if (key_wgs < 128)
+    dkv_form<T, D, 4>(P, st);
+  else if (kPaired && P.nq > 64 && key_wgs <= 256)
+    dkv_form<T, D, kPaired ? 2 : 1>(P, st);
+  else
+    dkv_form<T, D, 1>(P, st);
   if (P.dbias.p && P.share > 1) {
     const int64_t planes = P.items / P.share;
     diffattn_dbias_kernel<T, D><<<eights(planes * P.heads * P.chunks * ((P.nk + 63) / 64) * ((P.nq + 63) / 64)), 256, 0, st>>>(P);

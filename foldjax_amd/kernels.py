@@ -713,7 +713,7 @@ _BLOCKS: dict = {}
 
 
 def _layout(*tensors):
-    return tuple(None if t is None else (t.dtype, t.get_device(), t.shape, t.stride()) for t in tensors)
+    return tuple([None if t is None else (t.dtype, t.get_device(), t.shape, t.stride()) for t in tensors])
 
 
 def _remember(key, value) -> None:
@@ -1041,8 +1041,8 @@ def rms_norm_backward(
             block, nbytes, c = seen
             a = _lib.RmsNormBwdArgs.from_buffer_copy(block)
             dx = torch.empty_like(h)
-            dw = torch.empty((c,), dtype=torch.float32, device=h.device)
-            ws = torch.empty((nbytes,), dtype=torch.uint8, device=h.device)
+            dw = torch.empty(c, dtype=torch.float32, device=h.device)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=h.device)
             a.dy, a.h, a.weight, a.dx = dy.data_ptr(), h.data_ptr(), weight.data_ptr(), dx.data_ptr()
             a.dweight, a.workspace = dw.data_ptr(), ws.data_ptr()
             if dh is not None:

@@ -191,6 +191,25 @@ def test_forward_and_gradients(shape, bias, mask, dtype):
         check(name, got[name], want[name], terms[name], dtype)
 
 
+# as many rows and keys as make 64 of them a workgroup's, with waves that share a
+# block's keys (queries) and without
+MANY = [
+    ((4, 20), 4, 2, 70, 130, 32),
+    ((16,), 8, 8, 65, 130, 32),
+    ((11,), 6, 6, 129, 129, 32),
+    ((9,), 10, 5, 40, 256, 32),
+    ((24,), 6, 6, 66, 64, 32),
+    ((2, 10), 8, 4, 48, 100, 64),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("bias,mask", BIAS_MASK)
+@pytest.mark.parametrize("shape", MANY, ids=str)
+def test_many_rows(shape, bias, mask, dtype):
+    test_forward_and_gradients(shape, bias, mask, dtype)
+
+
 # few rows against many keys: the keys split over waves and workgroups
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("shape", [((3,), 8, 2, 1, 2000, 64), ((1,), 4, 4, 2, 4099, 32), ((2,), 8, 1, 3, 1023, 32),

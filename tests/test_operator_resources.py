@@ -45,4 +45,4 @@ def test_waves_a_simd_of_the_attention(resources):
             if re.search(r"(fwd|dq|dkv|dbias)_kernelI", name) and "DF16bLi32E" in name:
                 found += 1
                 assert m["vgpr_count"] <= most, (name, m)
-    assert found == 2 + 2 + 4 + 1
+    assert found == 2 + 2 + 6 + 1
