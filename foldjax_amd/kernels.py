@@ -723,14 +723,15 @@ def _remember(key, value) -> None:
 
 
 def _diff_attention_args(q, k, v, lambda_vectors, lambda_init, scale, bias, mask):
-    """The checked argument block that both directions share, the tensors it
-    points to, the leading axes, the elements of a 16-byte piece, and (its key,
-    the workspace of the forward call)."""
+    """The checked argument block that both directions share (its out strides
+    those of a contiguous output), the tensors it points to, the output's shape
+    and strides, the elements of a 16-byte piece, and (its key, the workspace of
+    the forward call)."""
     lambda_init, scale = float(lambda_init), float(scale)  # values, also of tensors: they are part of the key
     key = (_layout(q, k, v, lambda_vectors, bias, mask), lambda_init, scale)
     seen = _BLOCKS.get(key)
     if seen is not None:
-        block, lead, unit, nbytes = seen
+        block, shaped, unit, nbytes = seen
         a = _lib.DiffAttentionArgs.from_buffer_copy(block)
         a.q, a.k, a.v, a.lambda_vectors = qp, kp, vp, lp = q.data_ptr(), k.data_ptr(), v.data_ptr(), lambda_vectors.data_ptr()
         if not (qp | kp | vp | lp) & 15:
@@ -738,7 +739,7 @@ def _diff_attention_args(q, k, v, lambda_vectors, lambda_init, scale, bias, mask
                 a.bias = bias.data_ptr()
             if mask is not None:
                 a.mask = mask.data_ptr()
-            return a, (q, k, v, bias, mask, lambda_vectors), lead, unit, (key, nbytes)
+            return a, (q, k, v, bias, mask, lambda_vectors), shaped, unit, (key, nbytes)
     given = (q, k, v, bias, mask, lambda_vectors)
     dtype = q.dtype
     code = _code(dtype)
@@ -798,15 +799,21 @@ def _diff_attention_args(q, k, v, lambda_vectors, lambda_init, scale, bias, mask
     q, qst = _heads(q, unit)
     k, kst = _heads(k, unit)
     v, vst = _heads(v, unit)
+    shape = lead + (heads, nq, 2 * d)
+    packed = _packed(shape)
     a = _lib.DiffAttentionArgs(
         items, heads, kv_heads, nq, nk, d, share, code, scale, lambda_init, q.data_ptr(), k.data_ptr(), v.data_ptr(), None,
-        qst, kst, vst, (0, 0, 0), bp, bst, None if m2 is None else m2.data_ptr(), lam.data_ptr())
+        qst, kst, vst, packed, bp, bst, None if m2 is None else m2.data_ptr(), lam.data_ptr())
     kept = (q, k, v, bias, m2, lam)
     nbytes = _lib.load().fjx_diff_attention_workspace_size(items, heads, kv_heads, nq, nk, d, code)
+    strides = [1] * len(shape)
+    for i in range(len(shape) - 1, 0, -1):
+        strides[i - 1] = strides[i] * shape[i]
+    shaped = shape, tuple(strides)
     as_they_lie = all(x is y for x, y in zip(kept, given))
     if as_they_lie:
-        _remember(key, (bytes(a), lead, unit, nbytes))
-    return a, kept, lead, unit, (key if as_they_lie else None, nbytes)
+        _remember(key, (bytes(a), shaped, unit, nbytes))
+    return a, kept, shaped, unit, (key if as_they_lie else None, nbytes)
 
 
 def diff_attention(
@@ -843,11 +850,9 @@ def diff_attention(
     ``diff_attention_backward`` needs to know of the rows. ``out``: write into
     this tensor (its rows whole 16-byte pieces, any order of the other axes),
     which overlaps no input."""
-    a, kept, lead, unit, (_, nbytes) = _diff_attention_args(q, k, v, lambda_vectors, lambda_init, scale, bias, mask)
-    shape = lead + (a.heads, a.nq, 2 * a.head_dim)
+    a, kept, (shape, strides), unit, (_, nbytes) = _diff_attention_args(q, k, v, lambda_vectors, lambda_init, scale, bias, mask)
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=q.device)
-        a.out_strides = _packed(shape)
+        out = torch.empty_strided(shape, strides, dtype=q.dtype, device=q.device)
     else:
         if out.shape != shape or out.dtype != q.dtype or out.device != q.device:
             raise ValueError(f"out must be a {q.dtype} tensor of shape {shape} on {q.device}, "
@@ -861,7 +866,7 @@ def diff_attention(
     a.out = out.data_ptr()
     lse = None
     if return_lse:
-        lse = torch.empty(lead + (2 * a.heads, a.nq), dtype=torch.float32, device=q.device)
+        lse = torch.empty(shape[:-3] + (2 * a.heads, a.nq), dtype=torch.float32, device=q.device)
         a.stats = lse.data_ptr()
     if nbytes:
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
@@ -891,7 +896,7 @@ def diff_attention_backward(
     plane the sum over the items, of shared heads' k and v the sum over the
     query heads), dlambda float32 ``[4, H, D]``. The same bits each time. Rows
     of the bias are less than 2^23 elements apart."""
-    f, kept, lead, unit, (key, _) = _diff_attention_args(q, k, v, lambda_vectors, lambda_init, scale, bias, mask)
+    f, kept, (shape, _), unit, (key, _) = _diff_attention_args(q, k, v, lambda_vectors, lambda_init, scale, bias, mask)
     with_bias = bias is not None and bias_grad
     key = None if key is None else (key, _layout(dout, lse), with_bias)
     seen = None if key is None else _BLOCKS.get(key)
@@ -902,8 +907,8 @@ def diff_attention_backward(
     else:
         _same_place(q, q.dtype, dout=dout)
         _same_place(q, torch.float32, lse=lse)
-        _need_shape("dout", dout, lead + (f.heads, f.nq, 2 * f.head_dim))
-        _need_shape("lse", lse, lead + (2 * f.heads, f.nq))
+        _need_shape("dout", dout, shape)
+        _need_shape("lse", lse, shape[:-3] + (2 * f.heads, f.nq))
         given = dout, lse
         dout, f.out_strides = _heads(dout, unit)
         if not lse.is_contiguous():
