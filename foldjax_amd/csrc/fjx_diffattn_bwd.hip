@@ -51,22 +51,31 @@ __device__ __forceinline__ float sum8(const float (&x)[8]) {
 
 // dq and D_t in one walk over the keys. A wave holds 16 query rows (lane l row
 // l % 16) as in the forward pass. D_t is known only at the end, so two sums
-// are kept, U = sum P_t (dP - c) k and W = sum P_t k, and
-//   dq_t = scale (U - (D_t - c) W)
-// where c, the mean of dP under both maps' weights in the first block, keeps U
-// near the difference that is wanted. D_2 is divided by its weights' own sum, one
-// but for the rounding of L: lambda's gradient is the sum of all D_2, of either
-// sign, and shows what they have in common. (c is subtracted from dP here: as the
-// start of dP's accumulators it left D_2 off by 1e-6 in common.) Against a first
-// walk for D_t alone this trades a second set of scores, dP and exponentials for
-// the products W, half the time. W takes two bf16 parts as well: where one key has
-// nearly all the weight, U and (D_t - c) W nearly cancel.
-// Bound like the forward kernel, with two waves a SIMD (256 registers): 65 us at 245
-// rows of 245 tokens and 2 heads, 46 % vector and 14 % matrix instructions, a quarter
-// of it starts and ends; 19 us at 4 x 499 tokens and 6 heads.
+// are kept, U = sum P_t (dP - c_t) k and W = sum P_t k, and
+//   dq_t = scale (U - (D_t - c_t) W) / sum P_t
+// whatever c_t is; D_t - c_t comes from the sum of P_t (dP - c_t). (The weights'
+// own sum is one but for the rounding of L; lambda's gradient is the sum of all D_2,
+// of either sign, and shows what they have in common.) But the two terms cancel,
+// down to their operands' bits, unless c_t is near D_t: where one key has nearly
+// all the weight dq is what the others have left of it. So c_t is the mean of dP
+// under map t over the keys so far, moved before a block's own terms are formed,
+//   c -> c + e:  U -> U - e W,  sum P (dP - c) -> less e sum P,
+// until the keys it is taken from have kEnough of the weight: with A of it, it is
+// within sum P |dP - D| / A of D, and what is lost is 1 / A of the rounding of dS
+// itself. Rows are mostly there after a block or two; the waves that share a row each
+// have a centre of their own keys, joined at the end. (c is subtracted from dP here:
+// as the start of dP's accumulators it left D_2 off by 1e-6 in common.) Against a
+// first walk for D_t alone this trades a second set of scores, dP and exponentials
+// for the products W, half the time. W takes two bf16 parts as well.
+// Bound like the forward kernel, with two waves a SIMD (256 registers): 70 us at 245
+// rows of 245 tokens and 2 heads, mostly vector instructions, a quarter of it starts
+// and ends; 22 us at 4 x 499 tokens and 6 heads (64 and 20 with one centre of the first
+// block for both maps, which lost dq's digits in rows of one heavy key).
 //
 // KS 4: the four waves share 16 rows and take 32 keys each of a 128-key block, for
 // calls with few rows; KS 1: each has rows of its own.
+constexpr float kEnough = 1.f / 16;
+
 template <typename T, int D, int KS>
 __global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diffattn_dq_kernel(DiffAttnParams<T> P) {
   typedef DaForm<KS> Form;
@@ -78,7 +87,7 @@ __global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diff
   static_assert(KS == 1 || kBufs * sizeof(Tile) >= Form::kWaves * 2 * 16 * kPo * sizeof(float), "the waves' sums");
   __shared__ __attribute__((aligned(16))) Tile tiles[kBufs];
   __shared__ __attribute__((aligned(16))) KeyFlags<kRows> flags[3];  // of the block at hand and the next two
-  __shared__ float joined[Form::kWaves][3][16];
+  __shared__ float joined[Form::kWaves][2][3][16];  // of the waves' rows and maps: center, weight, off
 
   const int t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -143,16 +152,10 @@ __global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diff
   st.load(0, flags[0].whole(), flags[0].on);
   const float lam = da_lambda<D>(P.lam, P.heads, head, P.init, lane);
 
-  // the sum of the tile's waves' `joined`, in one order
-  auto of_tile = [&](int x) {
-    float v[KS];
-#pragma unroll
-    for (int j = 0; j < KS; ++j) v[j] = joined[Form::kTiles * j + tile_of][x][li];
-    if constexpr (KS == 4) return (v[0] + v[1]) + (v[2] + v[3]);
-    if constexpr (KS == 2) return v[0] + v[1];
-    return v[0];
-  };
-  float c0 = 0.f, Dt[2] = {0.f, 0.f}, total = 0.f;  // D_t - c; the second map's weights
+  // of each map: c_t, the lane's sums of P and of P (dP - c), and the row's weight
+  // that c_t was last taken from
+  float center[2] = {0.f, 0.f}, weight[2] = {0.f, 0.f}, off[2] = {0.f, 0.f};
+  float held[2] = {L[0] < INFINITY ? 0.f : 1.f, L[1] < INFINITY ? 0.f : 1.f};  // a row without keys needs none
   f32x4 us[2][kU], ws[2][kU];
 #pragma unroll
   for (int m = 0; m < 2; ++m)
@@ -184,29 +187,30 @@ __global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diff
     tile_dp<T, D, kRows, kNt>(tile, key_w, dof, li, lg, dp);
 #pragma unroll
     for (int m = 0; m < 2; ++m) tile_weights<T, D, kRows, kNt>(tile, m, key_w, qf[m], b, P.scale_log2, L[m], li, lg, p[m]);
-    if (blk == 0) {
-      float sp = 0.f, sd = 0.f;
+    if (__builtin_amdgcn_ballot_w64(held[0] < kEnough || held[1] < kEnough)) {
 #pragma unroll
-      for (int kt = 0; kt < kNt; ++kt)
+      for (int m = 0; m < 2; ++m) {
+        float sp = 0.f, sd = 0.f;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          sp += p[0][kt][r] + p[1][kt][r];
-          sd = fmaf(p[0][kt][r] + p[1][kt][r], dp[kt][r], sd);
-        }
-      sp = group_sum(sp);
-      sd = group_sum(sd);
-      if constexpr (KS > 1) {
-        if (lg == 0) joined[wave][0][li] = sp, joined[wave][1][li] = sd;
-        __syncthreads();
-        sp = of_tile(0);
-        sd = of_tile(1);
+        for (int kt = 0; kt < kNt; ++kt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            sp += p[m][kt][r];
+            sd = fmaf(p[m][kt][r], dp[kt][r] - center[m], sd);
+          }
+        sp = group_sum(sp) + held[m];
+        sd = group_sum(sd);
+        // the keys before it add nothing to sd: c_t is their mean
+        const float move = held[m] < kEnough && sp > 0.f ? sd / sp : 0.f;
+        held[m] = held[m] < kEnough ? sp : held[m];
+        center[m] += move;
+        off[m] = fmaf(-move, weight[m], off[m]);
+#pragma unroll
+        for (int u = 0; u < kU; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) us[m][u][r] = fmaf(-move, ws[m][u][r], us[m][u][r]);
       }
-      c0 = sp > 0.f ? sd / sp : 0.f;
     }
-#pragma unroll
-    for (int kt = 0; kt < kNt; ++kt)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) dp[kt][r] -= c0;
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -215,10 +219,10 @@ __global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diff
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           w8[e] = p[m][2 * c + (e >> 2)][e & 3];
-          u8[e] = w8[e] * dp[2 * c + (e >> 2)][e & 3];
+          u8[e] = w8[e] * (dp[2 * c + (e >> 2)][e & 3] - center[m]);
         }
-        Dt[m] += sum8(u8);
-        if (m == 1) total += sum8(w8);
+        off[m] += sum8(u8);
+        weight[m] += sum8(w8);
         F uf[kParts<T>], wf[kParts<T>];
         parts(u8, uf);
         parts(w8, wf);
@@ -237,30 +241,53 @@ __global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diff
     __syncthreads();
   }
 #pragma unroll
-  for (int m = 0; m < 2; ++m) Dt[m] = group_sum(Dt[m]);
-  total = group_sum(total);
+  for (int m = 0; m < 2; ++m) {
+    off[m] = group_sum(off[m]);
+    weight[m] = group_sum(weight[m]);
+  }
   if constexpr (KS > 1) {  // the waves' sums, through the tiles' memory
-    if (lg == 0) joined[wave][0][li] = Dt[0], joined[wave][1][li] = Dt[1], joined[wave][2][li] = total;
+    if (lg == 0)
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        joined[wave][m][0][li] = center[m];
+        joined[wave][m][1][li] = weight[m];
+        joined[wave][m][2][li] = off[m];
+      }
     __syncthreads();
-    total = of_tile(2);
+    // all the keys' weight, and their sum of P (dP - c) around this wave's centre
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      weight[m] = off[m] = 0.f;
+#pragma unroll
+      for (int j = 0; j < KS; ++j) {
+        const float (&of)[3][16] = joined[Form::kTiles * j + tile_of][m];
+        weight[m] += of[1][li];
+        off[m] += fmaf(of[1][li], of[0][li] - center[m], of[2][li]);
+      }
+    }
+  }
+  float by[2];  // and D_t - c_t in `off`
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    const float inv = weight[m] > 0.f ? 1.f / weight[m] : 0.f;  // a row without keys is zeros
+    off[m] *= inv;
+    by[m] = P.scale * inv * (m ? -lam : 1.f);
+  }
+  if constexpr (KS > 1) {
     float* po = reinterpret_cast<float*>(&tiles[0]);  // [wave][map][row][D + 2]
     auto slot = [&](int j, int m) { return (((Form::kTiles * j + tile_of) * 2 + m) * 16 + li) * kPo; };  // of the tile's j-th wave
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      Dt[m] = of_tile(m);
-      if (m == 1 && total > 0.f) Dt[m] /= total;
+    for (int m = 0; m < 2; ++m)
 #pragma unroll
       for (int u = 0; u < kU; ++u)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) po[slot(ks, m) + 16 * u + 4 * lg + r] = us[m][u][r] - Dt[m] * ws[m][u][r];
-    }
+        for (int r = 0; r < 4; ++r) po[slot(ks, m) + 16 * u + 4 * lg + r] = us[m][u][r] - off[m] * ws[m][u][r];
     __syncthreads();
     // each wave writes its share of the two maps' tiles of 16 columns
     constexpr int kOwn = 2 * kU / KS;
     const int m = ks * 2 / KS, first = ks * kOwn % kU;
     if (!row_on) return;
-    if (lg == 0 && first == 0) P.delta[(item * 2 * P.heads + 2 * head + m) * P.nq + qi] = Dt[m] + c0;
-    const float by = P.scale * (m ? -lam : 1.f);
+    if (lg == 0 && first == 0) P.delta[(item * 2 * P.heads + 2 * head + m) * P.nq + qi] = off[m] + center[m];
     T* out = P.dq.p + item * P.dq.item + (2 * head + m) * P.dq.head + qi * P.dq.token;
 #pragma unroll
     for (int u = 0; u < kOwn; ++u) {
@@ -271,24 +298,22 @@ __global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diff
         float x = 0.f;
 #pragma unroll
         for (int j = 0; j < KS; ++j) x += po[slot(j, m) + col + r];
-        v[r] = x * by;
+        v[r] = x * by[m];
       }
       store4f(out + col, v);
     }
     return;
   }
-  if (total > 0.f) Dt[1] /= total;
   if (!row_on) return;
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
-    if (lg == 0) P.delta[(item * 2 * P.heads + 2 * head + m) * P.nq + qi] = Dt[m] + c0;
-    const float by = P.scale * (m ? -lam : 1.f);
+    if (lg == 0) P.delta[(item * 2 * P.heads + 2 * head + m) * P.nq + qi] = off[m] + center[m];
     T* out = P.dq.p + item * P.dq.item + (2 * head + m) * P.dq.head + qi * P.dq.token;
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
       float v[4];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = (us[m][u][r] - Dt[m] * ws[m][u][r]) * by;
+      for (int r = 0; r < 4; ++r) v[r] = (us[m][u][r] - off[m] * ws[m][u][r]) * by[m];
       store4f(out + 16 * u + 4 * lg, v);
     }
   }
