@@ -23,7 +23,7 @@ constexpr float kSlack = 8.f;
 // What bounds it: vector instructions (an exponential, its fma and two bf16 parts
 // a weight and map: 6 to a matrix instruction) and the matrix instructions, which
 // on one SIMD run beside other waves' vector work only in part. 499 rows of 499
-// tokens, 2 heads with their bias: 315 us, the SIMDs 58 % in vector and 29 % in matrix
+// tokens, 2 heads with their bias: 318 us, the SIMDs 58 % in vector and 29 % in matrix
 // instructions; 245 rows of 245: 51 us, 44 and 18 %, a quarter of it the workgroups'
 // starts and ends (4 blocks of keys each). One token of 8 sequences against 16384
 // keys (134 MB, keywise and split): 26.5 us, the copy rate, and 4.3 for the join.
@@ -192,16 +192,23 @@ __global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D> + (kDaWaves
         }
       }
     }
+    const float bases[2] = {exponent_base(m[0]), exponent_base(m[1])};
+    float by = P.scale_log2;
+    if (kBiasFirst<T>) {
+      const bool far = __builtin_amdgcn_ballot_w64(fmaxf(fabsf(bases[0]), fabsf(bases[1])) > kFar);
+      by = far_scores(far, by, s[0]);
+      far_scores(far, P.scale_log2, s[1]);
+    }
     F pf[2][kNt / 2][kParts<T>];
 #pragma unroll
     for (int mp = 0; mp < 2; ++mp) {
-      const float base = exponent_base(m[mp]);
+      const float base = bases[mp];
       float p[kNt / 2][8];
 #pragma unroll
       for (int kt = 0; kt < kNt; ++kt)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float e = __builtin_amdgcn_exp2f(kBiasFirst<T> ? fmaf(s[mp][kt][r], P.scale_log2, -base) : s[mp][kt][r] - base);
+          const float e = __builtin_amdgcn_exp2f(kBiasFirst<T> ? fmaf(s[mp][kt][r], by, -base) : s[mp][kt][r] - base);
           if (!kOnes) l[mp][r] += e;
           p[kt >> 1][4 * (kt & 1) + r] = e;
         }
