@@ -1160,7 +1160,7 @@ struct DiffBwdPlan {
 };
 DiffBwdPlan diff_bwd_plan(int64_t items, int64_t heads, int64_t nq, int64_t nk, int64_t share, bool with_dbias) {
   DiffBwdPlan p = {};
-  p.delta = align_up((size_t)items * 2 * heads * nq * sizeof(float));
+  p.delta = align_up((size_t)items * 2 * heads * nq * sizeof(float));  // once more for the weights' sums
   if (with_dbias && share > 1) {
     const int64_t planes = items / share;
     const int64_t tiles = planes * heads * ((nq + 63) / 64) * ((nk + 63) / 64);
@@ -1270,7 +1270,8 @@ int diff_bwd_run(const fjx_diff_attention_bwd_args* b, const DiffBwdPlan& plan, 
   p.saved = a->stats;
   p.dlam = b->dlambda;
   p.delta = at<float>(a->workspace, 0);
-  p.part_bias = at<float>(a->workspace, plan.delta);
+  p.norm = at<float>(a->workspace, plan.delta);
+  p.part_bias = at<float>(a->workspace, 2 * plan.delta);
   p.chunks = plan.chunks;
   p.chunk_items = plan.chunk_items;
   return timed(K_DIFF_ATTENTION_BWD, st, "diff_attention_bwd",
@@ -1562,7 +1563,7 @@ size_t fjx_diff_attention_bwd_workspace_size(int64_t items, int64_t heads, int64
                                              int32_t with_dbias) {
   if (items < 1 || heads < 1 || nq < 1 || nk < 1 || (with_dbias && (bias_share < 1 || items % bias_share))) return 0;
   const DiffBwdPlan p = diff_bwd_plan(items, heads, nq, nk, bias_share, with_dbias != 0);
-  return p.delta + p.part;
+  return 2 * p.delta + p.part;
 }
 
 int fjx_diff_attention_bwd(const fjx_diff_attention_bwd_args* b, hipStream_t st) {
@@ -1592,7 +1593,7 @@ int fjx_diff_attention_bwd(const fjx_diff_attention_bwd_args* b, hipStream_t st)
   const double tiles = (double)std::max(plan.chunks, 1) * a->items * a->heads * (a->nq / 64 + 1.0) * (a->nk / 64 + 1.0) /
                        (a->bias ? a->bias_share : a->items);
   if (plan.chunks && tiles >= (1 << 23)) return fail(FJX_ERR_UNSUPPORTED, "%s: more bias than one launch takes", fn);
-  const size_t need = plan.delta + plan.part;
+  const size_t need = 2 * plan.delta + plan.part;
   if (!a->workspace || a->workspace_bytes < need)
     return fail(FJX_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", fn, need, a->workspace_bytes);
   if (!aligned16({a->workspace})) return fail(FJX_ERR_INVALID, "%s: the workspace must be 16-byte aligned", fn);

@@ -51,7 +51,8 @@ struct DiffAttnParams {
   HeadsView<T> dq, dk, dv;
   HeadsView<T> dbias;          // as bias, or null
   const float* saved;          // the forward pass's stats
-  float* delta;                // [items][2 H][nq]: rowsum(P_t dP)
+  float* delta;                // [items][2 H][nq]: rowsum(P_t dP) / rowsum(P_t)
+  float* norm;                 // the same: 1 / rowsum(P_t), 0 for a row without keys
   float* dlam;                 // [4][H][D]
   float* part_bias;            // [chunks][planes][H][nq][nk] partial sums of dbias
   int64_t chunk_items;         // items of one chunk

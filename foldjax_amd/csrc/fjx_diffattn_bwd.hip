@@ -3,7 +3,11 @@
 //   dq_t = scale dS_t k_t,  dk_t = scale dS_t^T q_t,  dv = (P_1 - lambda P_2)^T dO,
 //   dbias = dS_1 + dS_2,  dlambda = -sum D_2
 // The weights come again from the scores and the forward pass's row statistics
-// L_t = log2 sum 2^x: P_t = 2^(x - L_t). Every sum has one owner and one order:
+// L_t = log2 sum 2^x: P_t = 2^(x - L_t). L's own rounding is a factor of all of a row's
+// weights: 1e-6 of them at |L| = 32, but of the order of 1 under the biases of -1e5 and
+// beyond that masks add to whole rows (where L is the maximum alone, and the weights
+// add up to the number of keys). So the kernel for dq divides by the sum of P_t, and
+// leaves it for the others, which divide too wherever a row has |L| > kFarSum. Every sum has one owner and one order:
 // no atomics, and the same bits each time.
 //
 // dS's rows sum to zero, so its products may cancel: like the weights it goes
@@ -15,22 +19,31 @@ namespace fjx {
 
 namespace {
 
-// weights of the wave's 16 rows and NT key tiles from row `key_w` of a block on,
-// one map; b: bias in its unit
+constexpr float kFarSum = 256.f;  // there the factor is 1 + 5e-6
+// |L| beyond `most`, and not for want of keys
+__device__ __forceinline__ bool row_far(float L, float most) { return fabsf(L) > most && L < INFINITY; }
+
+// sums of the scores of the wave's 16 rows and NT key tiles from row `key_w` of a
+// block on, one map; b: bias in its unit
 template <typename T, int D, int ROWS, int NT>
-__device__ __forceinline__ void tile_weights(const DaTile<T, D, ROWS>& tile, int mp, int key_w,
-                                             const typename Frag<T>::type (&qf)[D / 32], const f32x4 (&b)[NT],
-                                             float scale_log2, float L, int li, int lg, f32x4 (&p)[NT]) {
+__device__ __forceinline__ void tile_scores(const DaTile<T, D, ROWS>& tile, int mp, int key_w,
+                                            const typename Frag<T>::type (&qf)[D / 32], const f32x4 (&b)[NT], int li, int lg,
+                                            f32x4 (&s)[NT]) {
 #pragma unroll
   for (int kt = 0; kt < NT; ++kt) {
-    p[kt] = score_start<T>(b[kt]);
+    s[kt] = score_start<T>(b[kt]);
 #pragma unroll
-    for (int c = 0; c < D / 32; ++c) mma(p[kt], load8(&tile.a[key_w + 16 * kt + li][D * mp + 32 * c + 8 * lg]), qf[c]);
+    for (int c = 0; c < D / 32; ++c) mma(s[kt], load8(&tile.a[key_w + 16 * kt + li][D * mp + 32 * c + 8 * lg]), qf[c]);
   }
+}
+
+// the weights in their place
+template <typename T, int NT>
+__device__ __forceinline__ void to_weights(const f32x4 (&b)[NT], float scale_log2, float L, f32x4 (&s)[NT]) {
 #pragma unroll
   for (int kt = 0; kt < NT; ++kt)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) p[kt][r] = __builtin_amdgcn_exp2f(exponent<T>(p[kt][r], b[kt][r], scale_log2, L));
+    for (int r = 0; r < 4; ++r) s[kt][r] = __builtin_amdgcn_exp2f(exponent<T>(s[kt][r], b[kt][r], scale_log2, L));
 }
 
 // dP of the same
@@ -155,7 +168,13 @@ __global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diff
   // of each map: c_t, the lane's sums of P and of P (dP - c), and the row's weight
   // that c_t was last taken from
   float center[2] = {0.f, 0.f}, weight[2] = {0.f, 0.f}, off[2] = {0.f, 0.f};
-  float held[2] = {L[0] < INFINITY ? 0.f : 1.f, L[1] < INFINITY ? 0.f : 1.f};  // a row without keys needs none
+  float held[2], enough[2];  // without keys none is needed; far rows' weights are not yet divided by their sum
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    held[m] = L[m] < INFINITY ? 0.f : INFINITY;
+    enough[m] = fabsf(L[m]) <= kFarSum ? kEnough : INFINITY;
+  }
+  const bool far = __builtin_amdgcn_ballot_w64(row_far(L[0], kFar) || row_far(L[1], kFar));
   f32x4 us[2][kU], ws[2][kU];
 #pragma unroll
   for (int m = 0; m < 2; ++m)
@@ -186,8 +205,15 @@ __global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diff
     f32x4 dp[kNt], p[2][kNt];
     tile_dp<T, D, kRows, kNt>(tile, key_w, dof, li, lg, dp);
 #pragma unroll
-    for (int m = 0; m < 2; ++m) tile_weights<T, D, kRows, kNt>(tile, m, key_w, qf[m], b, P.scale_log2, L[m], li, lg, p[m]);
-    if (__builtin_amdgcn_ballot_w64(held[0] < kEnough || held[1] < kEnough)) {
+    for (int m = 0; m < 2; ++m) tile_scores<T, D, kRows, kNt>(tile, m, key_w, qf[m], b, li, lg, p[m]);
+    float by = P.scale_log2;
+    if (kBiasFirst<T>) {
+      far_scores(far, P.scale_log2, p[0]);
+      by = far_scores(far, P.scale_log2, p[1]);
+    }
+#pragma unroll
+    for (int m = 0; m < 2; ++m) to_weights<T>(b, by, L[m], p[m]);
+    if (__builtin_amdgcn_ballot_w64(held[0] < enough[0] || held[1] < enough[1])) {
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
         float sp = 0.f, sd = 0.f;
@@ -201,8 +227,8 @@ __global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diff
         sp = group_sum(sp) + held[m];
         sd = group_sum(sd);
         // the keys before it add nothing to sd: c_t is their mean
-        const float move = held[m] < kEnough && sp > 0.f ? sd / sp : 0.f;
-        held[m] = held[m] < kEnough ? sp : held[m];
+        const float move = held[m] < enough[m] && sp > 0.f ? sd / sp : 0.f;
+        held[m] = held[m] < enough[m] ? sp : held[m];
         center[m] += move;
         off[m] = fmaf(-move, weight[m], off[m]);
 #pragma unroll
@@ -266,12 +292,12 @@ __global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diff
       }
     }
   }
-  float by[2];  // and D_t - c_t in `off`
+  float by[2];  // dq's factors; and D_t - c_t in `off`
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
-    const float inv = weight[m] > 0.f ? 1.f / weight[m] : 0.f;  // a row without keys is zeros
-    off[m] *= inv;
-    by[m] = P.scale * inv * (m ? -lam : 1.f);
+    weight[m] = weight[m] > 0.f ? 1.f / weight[m] : 0.f;  // a row without keys is zeros
+    off[m] *= weight[m];
+    by[m] = P.scale * weight[m] * (m ? -lam : 1.f);
   }
   if constexpr (KS > 1) {
     float* po = reinterpret_cast<float*>(&tiles[0]);  // [wave][map][row][D + 2]
@@ -287,7 +313,11 @@ __global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diff
     constexpr int kOwn = 2 * kU / KS;
     const int m = ks * 2 / KS, first = ks * kOwn % kU;
     if (!row_on) return;
-    if (lg == 0 && first == 0) P.delta[(item * 2 * P.heads + 2 * head + m) * P.nq + qi] = off[m] + center[m];
+    if (lg == 0 && first == 0) {
+      const int64_t at = (item * 2 * P.heads + 2 * head + m) * P.nq + qi;
+      P.delta[at] = off[m] + center[m];
+      P.norm[at] = weight[m];
+    }
     T* out = P.dq.p + item * P.dq.item + (2 * head + m) * P.dq.head + qi * P.dq.token;
 #pragma unroll
     for (int u = 0; u < kOwn; ++u) {
@@ -307,7 +337,11 @@ __global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diff
   if (!row_on) return;
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
-    if (lg == 0) P.delta[(item * 2 * P.heads + 2 * head + m) * P.nq + qi] = off[m] + center[m];
+    if (lg == 0) {
+      const int64_t at = (item * 2 * P.heads + 2 * head + m) * P.nq + qi;
+      P.delta[at] = off[m] + center[m];
+      P.norm[at] = weight[m];
+    }
     T* out = P.dq.p + item * P.dq.item + (2 * head + m) * P.dq.head + qi * P.dq.token;
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
@@ -373,6 +407,9 @@ __global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diff
   static_assert(KS == 1 || kBufs * sizeof(Tile) >= Form::kWaves * 16 * kPo * sizeof(float), "the waves' sums");
   __shared__ __attribute__((aligned(16))) Tile tiles[kBufs];
   __shared__ __attribute__((aligned(16))) float row_stat[kBufs][4][kQ];  // L_1, L_2, D_1, D_2
+  __shared__ __attribute__((aligned(16))) float far_norm[kBufs][2][kQ];  // log2 of rows' norms, 0 for |L| <= kFarSum
+  __shared__ int far_rows[kBufs][Form::kWaves];  // whether a wave staged such an L
+  __shared__ __attribute__((aligned(16))) float zeros[kQ];
   __shared__ float query_on[kQ];
   __shared__ double lam_lds[Form::kWaves];
 
@@ -426,10 +463,14 @@ __global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diff
   const int64_t head_step = st.which < 2 ? 2 * P.q.head : P.dout.head;
   const T* src0 = st.src;
   // the last block's queries, as KeyFlags::on
-  if (t < kQ) query_on[t] = (q_blocks - 1) * kQ + t < P.nq ? 1.f : -1.f;
+  if (t < kQ) {
+    query_on[t] = (q_blocks - 1) * kQ + t < P.nq ? 1.f : -1.f;
+    zeros[t] = 0.f;
+  }
   __syncthreads();
   constexpr int kStats = 4 * kQ / Form::kThreads;  // statistics that a thread stages
   float stat[kStats];
+  int64_t stat_at = 0;  // of the first one's row
   auto fetch = [&](int hg, int64_t qb) {
     st.src = src0 + hg * head_step;
     st.load(qb * kQ, (qb + 1) * kQ <= P.nq, query_on);
@@ -440,12 +481,19 @@ __global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diff
       const int64_t at = (item * 2 * P.heads + 2 * (h0 + hg) + (which & 1)) * P.nq + q;
       stat[i] = which < 2 ? INFINITY : 0.f;  // past the last query: weights of zero
       if (q < P.nq) stat[i] = which < 2 ? P.saved[at] : P.delta[at];
+      if (i == 0) stat_at = at;
     }
   };
   auto put = [&](int buf) {
     st.store(tiles[buf]);
 #pragma unroll
     for (int i = 0; i < kStats; ++i) row_stat[buf][(t + Form::kThreads * i) / kQ][(t + Form::kThreads * i) % kQ] = stat[i];
+    // kStats 1: L in the first half of the threads, 2: in the first of each one's
+    const bool is_L = kStats == 2 || t < 2 * kQ;
+    const bool far = is_L && row_far(stat[0], kFarSum);
+    const bool any = __builtin_amdgcn_ballot_w64(far);
+    if (lane == 0) far_rows[buf][wave] = any;
+    if (is_L) far_norm[buf][t / kQ][t % kQ] = far ? __builtin_amdgcn_logf(P.norm[stat_at]) : 0.f;
   };
   // a lane's element of the bias in a tile's 16 rows (less than 2^23 elements
   // apart): its row and its key; the tile's first row is scalar
@@ -526,6 +574,37 @@ __global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diff
 #pragma unroll
         for (int x = 0; x < 2 * kC; ++x) mma(dp[qt], load8(&tile.b[q_w + 16 * qt + li][32 * x + 8 * lg]), vf[x]);
       }
+      int far = 0;
+#pragma unroll
+      for (int w = 0; w < Form::kWaves; ++w) far |= far_rows[buf][w];
+      float by = P.scale_log2;
+      const float* ls = &row_stat[buf][0][0];  // L_1 and, `ls2` further on, L_2
+      int ls2 = kQ;
+      if (__builtin_amdgcn_readfirstlane(far)) {
+        // the exponents of divided weights in the scores' place, with no more to subtract
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int qt = 0; qt < kQt; ++qt) {
+            const f32x4 L = *reinterpret_cast<const f32x4*>(&row_stat[buf][m][q_w + 16 * qt + 4 * lg]);
+            const f32x4 n = *reinterpret_cast<const f32x4*>(&far_norm[buf][m][q_w + 16 * qt + 4 * lg]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              float e = exponent<T>(s[m][qt][r], b[qt][r], by, L[r]);
+              if (kBiasFirst<T> && row_far(L[r], kFar)) {
+                e = s[m][qt][r] * by;
+                asm("" : "+v"(e));  // rounded, as in far_scores
+                e -= L[r];
+              }
+              s[m][qt][r] = e + n[r];
+            }
+          }
+#pragma unroll
+        for (int qt = 0; qt < kQt; ++qt) b[qt] = f32x4{0.f, 0.f, 0.f, 0.f};
+        by = 1.f;
+        ls = zeros;
+        ls2 = 0;
+      }
       T db[kQt][4];
 #pragma unroll
       for (int c = 0; c < kQt / 2; ++c) {
@@ -535,11 +614,13 @@ __global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diff
           const int qt = 2 * c + j;
           f32x4 rs[4];
 #pragma unroll
-          for (int w = 0; w < 4; ++w) rs[w] = *reinterpret_cast<const f32x4*>(&row_stat[buf][w][q_w + 16 * qt + 4 * lg]);
+          for (int w = 0; w < 4; ++w)
+            rs[w] = *reinterpret_cast<const f32x4*>(w < 2 ? ls + w * ls2 + q_w + 16 * qt + 4 * lg
+                                                          : &row_stat[buf][w][q_w + 16 * qt + 4 * lg]);
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float p1 = __builtin_amdgcn_exp2f(exponent<T>(s[0][qt][r], b[qt][r], P.scale_log2, rs[0][r]));
-            const float p2 = lam * __builtin_amdgcn_exp2f(exponent<T>(s[1][qt][r], b[qt][r], P.scale_log2, rs[1][r]));
+            const float p1 = __builtin_amdgcn_exp2f(exponent<T>(s[0][qt][r], b[qt][r], by, rs[0][r]));
+            const float p2 = lam * __builtin_amdgcn_exp2f(exponent<T>(s[1][qt][r], b[qt][r], by, rs[1][r]));
             comb[4 * j + r] = p1 - p2;
             ds[0][4 * j + r] = p1 * (dp[qt][r] - rs[2][r]);
             ds[1][4 * j + r] = p2 * (rs[3][r] - dp[qt][r]);
@@ -735,12 +816,22 @@ __global__ __launch_bounds__(256, (kDaWaves<T, D> + (kDaWaves<T, D> > 1))) void 
       fetch(item + 1, at);
       look(item + 2);
     }
+    const bool far_sum = __builtin_amdgcn_ballot_w64(row_far(rs[0], kFarSum) || row_far(rs[1], kFarSum));
+    const bool far = far_sum && __builtin_amdgcn_ballot_w64(row_far(rs[0], kFar) || row_far(rs[1], kFar));
     f32x4 dp[4];
     tile_dp<T, D, kDaKeys, 4>(tile, 0, dof, li, lg, dp);
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
       f32x4 p[4];
-      tile_weights<T, D, kDaKeys, 4>(tile, m, 0, qf[m], b, P.scale_log2, rs[m], li, lg, p);
+      tile_scores<T, D, kDaKeys, 4>(tile, m, 0, qf[m], b, li, lg, p);
+      to_weights<T>(b, kBiasFirst<T> ? far_scores(far, P.scale_log2, p) : P.scale_log2, rs[m], p);
+      if (far_sum) {
+        const float n = P.norm[(item * 2 * P.heads + 2 * head + m) * P.nq + qc];
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) p[kt][r] *= n;
+      }
 #pragma unroll
       for (int kt = 0; kt < 4; ++kt)
 #pragma unroll

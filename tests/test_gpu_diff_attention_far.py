@@ -54,3 +54,36 @@ def test_one_token_against_far_keys(value, dtype):
     t["q"][1] = 0.0
     want, terms = reference(t)
     check("out", call(on_gpu(t)), want["out"], terms["out"], dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("value", FAR)
+@pytest.mark.parametrize("form", FORMS, ids=str)
+def test_gradients_of_rows_far_from_zero(form, value, dtype):
+    """The weights of such a row add up to one in the backward pass as well."""
+    say(f"far bias, gradients {form} {value} {dtype}")
+    t = far(*form, dtype, value)
+    t["bias"][..., 4, :] = t["bias"][..., 5, :] - 300.0  # distances at which scores still count
+    want, terms = reference(t, backward=True)
+    g = on_gpu(t)
+    got = grads(g, call(g, return_lse=True)[1])
+    for name in ("dq", "dk", "dv", "dlam", "dbias"):
+        check(name, got[name], want[name], terms[name], dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("value", [-1e5, -1e9, -1e30])
+@pytest.mark.parametrize("rows", [3, 40])
+def test_shared_bias_far_from_zero(rows, value, dtype):
+    """A plane that the rows of a pair tensor share, whole queries of it far."""
+    say(f"far shared bias {rows} {value} {dtype}")
+    t = make((2, rows), 2, 2, 70, 70, 32, dtype, bias="shared", mask="tail", seed=4)
+    t["bias"][..., 60:, :] = value
+    t["q"][..., 60:, :] = 0.0
+    want, terms = reference(t, backward=True)
+    g = on_gpu(t)
+    out, lse = call(g, return_lse=True)
+    check("out", out, want["out"], terms["out"], dtype)
+    got = grads(g, lse)
+    for name in ("dq", "dk", "dv", "dlam", "dbias"):
+        check(name, got[name], want[name], terms[name], dtype)
