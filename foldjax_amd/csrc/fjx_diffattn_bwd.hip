@@ -450,37 +450,42 @@ __global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diff
   const float key_on = part ? INFINITY : -INFINITY;
   const bool all_on = __builtin_amdgcn_ballot_w64(part) == ~0ull;
   const int64_t plane = biased ? item / P.share : 0;
-  const T* bias = biased ? P.bias.p + plane * P.bias.item : nullptr;
+  const int h0 = kv * P.group;
+  const T* bias = biased ? P.bias.p + plane * P.bias.item + h0 * P.bias.head : nullptr;
   const uint32_t key_c = in ? (uint32_t)key : 0;
 
-  T* dbias = DBIAS ? P.dbias.p + plane * P.dbias.item : nullptr;
+  T* dbias = DBIAS ? P.dbias.p + plane * P.dbias.item + h0 * P.dbias.head : nullptr;
 
-  const int64_t q_blocks = (P.nq + kQ - 1) / kQ;
+  const uint32_t nq = (uint32_t)P.nq;  // the queries in 32 bits: below 2^31
+  const int q_blocks = (nq + kQ - 1) / kQ;
   DaStage<T, D, kQ, Form::kThreads> st;
-  const int h0 = kv * P.group;
   st.init(P.q.p + item * P.q.item + 2 * h0 * P.q.head, P.q.head, P.q.token, P.dout.p + item * P.dout.item + h0 * P.dout.head,
           P.dout.token, t);
   const int64_t head_step = st.which < 2 ? 2 * P.q.head : P.dout.head;
   const T* src0 = st.src;
   // the last block's queries, as KeyFlags::on
   if (t < kQ) {
-    query_on[t] = (q_blocks - 1) * kQ + t < P.nq ? 1.f : -1.f;
+    query_on[t] = (uint32_t)(q_blocks - 1) * kQ + t < nq ? 1.f : -1.f;
     zeros[t] = 0.f;
   }
   __syncthreads();
   constexpr int kStats = 4 * kQ / Form::kThreads;  // statistics that a thread stages
   float stat[kStats];
-  int64_t stat_at = 0;  // of the first one's row
-  auto fetch = [&](int hg, int64_t qb) {
+  // of the first one's row; the statistics of this item's first head and map
+  uint32_t stat_at = 0;
+  const int64_t stats0 = (item * 2 * P.heads + 2 * h0) * (int64_t)nq;
+  const float *saved = P.saved + stats0, *delta = P.delta + stats0, *norm = P.norm + stats0;
+  auto fetch = [&](int hg, int qb) {
+    const uint32_t q0 = (uint32_t)qb * kQ;
     st.src = src0 + hg * head_step;
-    st.load(qb * kQ, (qb + 1) * kQ <= P.nq, query_on);
+    st.load(q0, q0 + kQ <= nq, query_on);
 #pragma unroll
     for (int i = 0; i < kStats; ++i) {
       const int which = (t + Form::kThreads * i) / kQ;
-      const int64_t q = qb * kQ + (t + Form::kThreads * i) % kQ;
-      const int64_t at = (item * 2 * P.heads + 2 * (h0 + hg) + (which & 1)) * P.nq + q;
+      const uint32_t q = q0 + (t + Form::kThreads * i) % kQ;
+      const uint32_t at = (2 * hg + (which & 1)) * nq + q;  // heads nq is below 2^27 a key/value head
       stat[i] = which < 2 ? INFINITY : 0.f;  // past the last query: weights of zero
-      if (q < P.nq) stat[i] = which < 2 ? P.saved[at] : P.delta[at];
+      if (q < nq) stat[i] = (which < 2 ? saved : delta)[at];
       if (i == 0) stat_at = at;
     }
   };
@@ -493,30 +498,32 @@ __global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diff
     const bool far = is_L && row_far(stat[0], kFarSum);
     const bool any = __builtin_amdgcn_ballot_w64(far);
     if (lane == 0) far_rows[buf][wave] = any;
-    if (is_L) far_norm[buf][t / kQ][t % kQ] = far ? __builtin_amdgcn_logf(P.norm[stat_at]) : 0.f;
+    if (is_L) far_norm[buf][t / kQ][t % kQ] = far ? __builtin_amdgcn_logf(norm[stat_at]) : 0.f;
   };
   // a lane's element of the bias in a tile's 16 rows (less than 2^23 elements
-  // apart): its row and its key; the tile's first row is scalar
+  // apart): its row and its key. The scalar address goes from tile to tile (of dbias
+  // from row to row) by a step that is not to be known before the loop: its multiples,
+  // kept there, took more scalars than there are
   const uint32_t bias_row = (uint32_t)P.bias.token, dbias_row = (uint32_t)P.dbias.token;
   const uint32_t lane_bias = 4 * lg * bias_row + key_c, lane_dbias = 4 * lg * dbias_row + key_c;
   T bq[kQt][4] = {};  // zeros without a bias
-  auto fetch_bias = [&](int hg, int64_t qb) {
-    const T* p = bias + (h0 + hg) * P.bias.head;
-    const int64_t q0 = qb * kQ + q_w;
-    if ((qb + 1) * kQ <= P.nq) {
-      p += q0 * P.bias.token;
+  auto fetch_bias = [&](int hg, int qb) {
+    const T* p = bias + hg * P.bias.head;
+    const uint32_t q0 = (uint32_t)qb * kQ + q_w;
+    uint32_t step = bias_row;
+    asm volatile("" : "+s"(step));
+    p += (uint64_t)q0 * step;
+    if ((uint32_t)(qb + 1) * kQ <= nq) {
 #pragma unroll
-      for (int qt = 0; qt < kQt; ++qt)
+      for (int qt = 0; qt < kQt; ++qt, p += 16 * step)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) bq[qt][r] = (p + 16 * qt * P.bias.token)[lane_bias + r * bias_row];
+        for (int r = 0; r < 4; ++r) bq[qt][r] = p[lane_bias + r * bias_row];
     } else {
+      const int left = (int)nq - (int)q0 - 4 * lg;
 #pragma unroll
-      for (int qt = 0; qt < kQt; ++qt)
+      for (int qt = 0; qt < kQt; ++qt, p += 16 * step)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int64_t q = q0 + 16 * qt + 4 * lg + r;
-          bq[qt][r] = p[(q < P.nq ? q : P.nq - 1) * P.bias.token + key_c];
-        }
+        for (int r = 0; r < 4; ++r) bq[qt][r] = 16 * qt + r < left ? p[lane_bias + r * bias_row] : from_f32<T>(0.f);
     }
   };
 
@@ -528,6 +535,9 @@ __global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diff
 #pragma unroll
   for (int u = 0; u < 2 * kU; ++u) dv[u] = f32x4{0.f, 0.f, 0.f, 0.f};
 
+  // for the end, a lane's: the loop has no scalar to spare
+  int to_item = (int)item, to_kv = kv;
+  asm("" : "+v"(to_item), "+v"(to_kv));
   fetch(0, 0);
   if (biased) fetch_bias(0, 0);
   float lam = da_lambda<D>(P.lam, P.heads, h0, P.init, lane);
@@ -541,7 +551,7 @@ __global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diff
   int turn = 0;
   for (int hg = 0; hg < P.group; ++hg) {
     if (hg) lam = da_lambda<D>(P.lam, P.heads, h0 + hg, P.init, lane);
-    for (int64_t qb = 0; qb < q_blocks; ++qb, turn ^= 1) {
+    for (int qb = 0; qb < q_blocks; ++qb, turn ^= 1) {
       const int buf = kBufs == 2 ? turn : 0;
       const Tile& tile = tiles[buf];
       const bool same = qb + 1 < q_blocks;
@@ -640,19 +650,22 @@ __global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diff
         }
       }
       if (DBIAS && in) {
-        const int64_t q0 = qb * kQ + q_w;
-        T* p = dbias + (h0 + hg) * P.dbias.head + q0 * P.dbias.token;
-        if ((qb + 1) * kQ <= P.nq) {
+        const uint32_t q0 = (uint32_t)qb * kQ + q_w;
+        uint32_t step = dbias_row;
+        asm volatile("" : "+s"(step));
+        T* p = dbias + hg * P.dbias.head + (uint64_t)q0 * step;
+        if ((uint32_t)(qb + 1) * kQ <= nq) {
 #pragma unroll
-          for (int qt = 0; qt < kQt; ++qt)
+          for (int qt = 0; qt < kQt; ++qt, p += 12 * step)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) (p + (16 * qt + r) * P.dbias.token)[lane_dbias] = db[qt][r];
+            for (int r = 0; r < 4; ++r, p += step) p[lane_dbias] = db[qt][r];
         } else {
+          const int left = (int)nq - (int)q0 - 4 * lg;
 #pragma unroll
-          for (int qt = 0; qt < kQt; ++qt)
+          for (int qt = 0; qt < kQt; ++qt, p += 12 * step)
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (q0 + 16 * qt + 4 * lg + r < P.nq) (p + (16 * qt + r) * P.dbias.token)[lane_dbias] = db[qt][r];
+            for (int r = 0; r < 4; ++r, p += step)
+              if (16 * qt + r < left) p[lane_dbias] = db[qt][r];
         }
       }
       if (kBufs == 1) __syncthreads();
@@ -673,8 +686,8 @@ __global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diff
 #pragma unroll
     for (int x = 0; x < 4 / KS; ++x) {
       const int part_of = ks * (4 / KS) + x;
-      T* out = part_of < 2 ? P.dk.p + item * P.dk.item + (2 * kv + part_of) * P.dk.head + key * P.dk.token
-                           : P.dv.p + item * P.dv.item + kv * P.dv.head + key * P.dv.token + (part_of - 2) * D;
+      T* out = part_of < 2 ? P.dk.p + to_item * P.dk.item + (2 * to_kv + part_of) * P.dk.head + key * P.dk.token
+                           : P.dv.p + to_item * P.dv.item + to_kv * P.dv.head + key * P.dv.token + (part_of - 2) * D;
 #pragma unroll
       for (int u = 0; u < kU; ++u) {
         float v[4];
@@ -693,7 +706,7 @@ __global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diff
   if (!in) return;
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
-    T* out = P.dk.p + item * P.dk.item + (2 * kv + m) * P.dk.head + key * P.dk.token;
+    T* out = P.dk.p + to_item * P.dk.item + (2 * to_kv + m) * P.dk.head + key * P.dk.token;
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
       float v[4];
@@ -702,7 +715,7 @@ __global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diff
       store4f(out + 16 * u + 4 * lg, v);
     }
   }
-  T* out = P.dv.p + item * P.dv.item + kv * P.dv.head + key * P.dv.token;
+  T* out = P.dv.p + to_item * P.dv.item + to_kv * P.dv.head + key * P.dv.token;
 #pragma unroll
   for (int u = 0; u < 2 * kU; ++u) {
     float v[4];
