@@ -1106,7 +1106,9 @@ def dropout_add(
     one mask entry serves, as the Pairformer drops an update for all rows
     (``(-3,)``) or for all columns (``(-2,)``). ``step``: an int64 tensor of
     one element on x's device, read by the kernel and added to ``offset``: a
-    captured call then drops anew at each replay. ``out``: write into this
+    captured call then drops anew at each replay (calls with one seed and one
+    step need offsets further apart than the step counts, or the later draws
+    what the other drew). ``out``: write into this
     tensor, which may be ``x`` and/or ``residual``."""
     key, p = None, float(p)
     shared = tuple(shared)

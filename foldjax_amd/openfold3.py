@@ -120,6 +120,7 @@ def pair_block(
     without the two transposed copies. ``chunk_size`` is accepted for
     signature parity (the kernels stream rows with a fixed workspace).
     ``dropout`` drops the four triangle updates."""
+    dropout = None if dropout is None else dropout.drawn()
 
     def add(z, sublayer, update, *args, **more):
         if dropout is None:

@@ -27,9 +27,11 @@ class PairDropout:
     the axes over which one entry serves, (-3,) for all rows (the ending node,
     which works on the transposed grid, swaps -3 and -2), with -1 for all
     channels too. A block draws its masks at ``offset`` .. ``offset + 3`` of the
-    generator of ``seed``, the block l of a stack 4 l further on; ``step`` (an
-    int64 device tensor) is added where the kernels run, so that a captured
-    block drops anew at each replay."""
+    generator of ``seed``, the block l of a stack l 2^32 further on (up to 2^28
+    blocks). ``step`` (an int64 device tensor of one element) is read where the
+    kernels run, so that a captured block or stack drops anew at each replay:
+    any other value, below 2^32, gives every update another mask, whether the
+    caller counts by 1 or more."""
 
     p: float = 0.25
     seed: int = 0
@@ -37,13 +39,24 @@ class PairDropout:
     step: torch.Tensor | None = None
     shared: tuple[int, ...] = (-3,)
 
+    def __post_init__(self):
+        if not (0 <= self.seed < 2**64 and 0 <= self.offset < 2**64):
+            raise ValueError(f"seed and offset must be in [0, 2^64), got {self.seed} and {self.offset}")
+
     def of_block(self, index: int) -> "PairDropout":
-        return replace(self, offset=self.offset + 4 * index)
+        return replace(self, offset=(self.offset + (index << 32)) % 2**64)
+
+    def drawn(self) -> "PairDropout":
+        """``step`` as a block's four updates add it to their offsets, which
+        differ in the two lowest bits: the step's own two become the highest."""
+        if self.step is None or self.step.dtype is not torch.int64:
+            return self
+        return replace(self, step=(self.step & -4) | (self.step << 62))
 
     def add(self, update: torch.Tensor, z: torch.Tensor, sublayer: int, ending: bool, out_mask, out) -> torch.Tensor:
-        """z + the dropped update, into ``out`` (or the update itself)."""
+        """z + the dropped update, into ``out`` (or the update itself); of ``drawn()``."""
         shared = tuple({-3: -2, -2: -3}.get(a, a) for a in self.shared) if ending else self.shared
-        return kernels.dropout_add(update, p=self.p, seed=self.seed, offset=self.offset + sublayer, step=self.step,
+        return kernels.dropout_add(update, p=self.p, seed=self.seed, offset=(self.offset + sublayer) % 2**64, step=self.step,
                                    residual=z, shared=shared, out_mask=out_mask, out=update if out is None else out)
 
 
@@ -76,6 +89,7 @@ class TriangleSublayers:
         well. ``dropout``: each update goes into a tensor of its own, and comes to
         z through ``kernels.dropout_add``."""
         first = [True]
+        dropout = None if dropout is None else dropout.drawn()
 
         def dest(z):
             # the output buffer of the next sublayer: z itself, except for the

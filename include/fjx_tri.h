@@ -498,7 +498,8 @@ int fjx_rms_norm_bwd(const fjx_rms_norm_bwd_args* args, hipStream_t stream);
  * for all rows, or for all columns after the ending node), and its element i
  * is kept where word i % 4 of Philox 4x32-10 of the counter (i / 4, offset)
  * under the key `seed` is at least p 2^32. `step` (a device value added to the
- * offset) gives each replay of a captured call a mask of its own. The same
+ * offset) gives each replay of a captured call a mask of its own; calls with one
+ * seed and one step need offsets further apart than the step counts. The same
  * call without a residual on the output's gradient is the backward pass.
  */
 enum { FJX_SHARE_N = 1, FJX_SHARE_M = 2, FJX_SHARE_C = 4 };
