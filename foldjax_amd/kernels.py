@@ -759,6 +759,8 @@ def _diff_attention_args(q, k, v, lambda_vectors, lambda_init, scale, bias, mask
     _need_shape("k", k, lead + (hk2, nk, d))
     _need_shape("v", v, lead + (kv_heads, nk, 2 * d))
     _need_shape("lambda_vectors", lambda_vectors, (4, heads, d))
+    if d not in (32, 64):
+        raise ValueError(f"q and k must have a width (head_dim) of 32 or 64, got {d}")
     unit = 4 if dtype is torch.float32 else 8
     items = 1
     for n in lead:
