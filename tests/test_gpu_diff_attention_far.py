@@ -73,13 +73,33 @@ def test_gradients_of_rows_far_from_zero(form, value, dtype):
 
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("value", [-1e5, -1e9, -1e30])
-@pytest.mark.parametrize("rows", [3, 40])
+@pytest.mark.parametrize("rows", [3, 20, 40])
 def test_shared_bias_far_from_zero(rows, value, dtype):
     """A plane that the rows of a pair tensor share, whole queries of it far."""
     say(f"far shared bias {rows} {value} {dtype}")
     t = make((2, rows), 2, 2, 70, 70, 32, dtype, bias="shared", mask="tail", seed=4)
     t["bias"][..., 60:, :] = value
     t["q"][..., 60:, :] = 0.0
+    want, terms = reference(t, backward=True)
+    g = on_gpu(t)
+    out, lse = call(g, return_lse=True)
+    check("out", out, want["out"], terms["out"], dtype)
+    got = grads(g, lse)
+    for name in ("dq", "dk", "dv", "dlam", "dbias"):
+        check(name, got[name], want[name], terms[name], dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("value", [-1e5, -1e10])
+@pytest.mark.parametrize("lead,heads,kv", [((48,), 2, 2), ((24,), 6, 3), ((2,), 8, 2), ((70,), 4, 2)], ids=str)
+def test_gradients_of_far_rows_in_several_blocks(lead, heads, kv, value, dtype):
+    """Query blocks with far rows and without, of heads that share keys, in the
+    forms of every number of workgroups."""
+    say(f"far blocks {lead} {heads} {kv} {value} {dtype}")
+    t = make(lead, heads, kv, 150, 90, 32, dtype, bias="plane", mask="none", seed=heads)
+    for rows in (slice(20, 22), slice(140, 150)):  # blocks 0 and 2 of 64, 0 and 1 of 128
+        t["bias"][..., heads - 1, rows, :] = value
+        t["q"][..., -2:, rows, :] = 0.0
     want, terms = reference(t, backward=True)
     g = on_gpu(t)
     out, lse = call(g, return_lse=True)
