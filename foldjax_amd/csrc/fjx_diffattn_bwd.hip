@@ -90,7 +90,7 @@ __device__ __forceinline__ float sum8(const float (&x)[8]) {
 constexpr float kEnough = 1.f / 16;
 
 template <typename T, int D, int KS>
-__global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diffattn_dq_kernel(DiffAttnParams<T> P) {
+__global__ __launch_bounds__((DaForm<KS>::kThreads), (D == 32 ? 2 : 1)) void diffattn_dq_kernel(DiffAttnParams<T> P) {
   typedef DaForm<KS> Form;
   constexpr int kRows = Form::kBlock, kNt = kRows / KS / 16, kBufs = KS == 4 ? 1 : 2;
   constexpr int kC = D / 32, kU = D / 16;
@@ -100,6 +100,7 @@ __global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diff
   static_assert(KS == 1 || kBufs * sizeof(Tile) >= Form::kWaves * 2 * 16 * kPo * sizeof(float), "the waves' sums");
   __shared__ __attribute__((aligned(16))) Tile tiles[kBufs];
   __shared__ __attribute__((aligned(16))) KeyFlags<kRows> flags[3];  // of the block at hand and the next two
+  __shared__ float lams[Form::kWaves][16];  // of the waves' rows
   __shared__ float joined[Form::kWaves][2][3][16];  // of the waves' rows and maps: center, weight, off
 
   const int t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
@@ -117,7 +118,7 @@ __global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diff
   const bool row_on = row < rows;
   const uint32_t row_c = row_on ? row : rows - 1;
   const int hg = row_c / nq;
-  const int64_t qi = row_c - hg * nq;
+  const uint32_t qi = row_c - hg * nq;
   const int head = kv * P.group + hg;
   const int key_w = kRows / KS * ks;  // this wave's keys of a block
 
@@ -163,17 +164,14 @@ __global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diff
   put_flags(1);
   __syncthreads();
   st.load(0, flags[0].whole(), flags[0].on);
-  const float lam = da_lambda<D>(P.lam, P.heads, head, P.init, lane);
+  const float lam_own = da_lambda<D>(P.lam, P.heads, head, P.init, lane);  // kept in LDS, as there
+  if (lg == 0) lams[wave][li] = lam_own;
 
-  // of each map: c_t, the lane's sums of P and of P (dP - c), and the row's weight
-  // that c_t was last taken from
+  // of each map: c_t, the lane's sums of P and of P (dP - c), and whether c_t is to
+  // move yet (not in a row without keys, to the end in a far one, whose weights are not
+  // yet divided by their sum)
   float center[2] = {0.f, 0.f}, weight[2] = {0.f, 0.f}, off[2] = {0.f, 0.f};
-  float held[2], enough[2];  // without keys none is needed; far rows' weights are not yet divided by their sum
-#pragma unroll
-  for (int m = 0; m < 2; ++m) {
-    held[m] = L[m] < INFINITY ? 0.f : INFINITY;
-    enough[m] = fabsf(L[m]) <= kFarSum ? kEnough : INFINITY;
-  }
+  bool moves[2] = {L[0] < INFINITY, L[1] < INFINITY};
   const bool far = __builtin_amdgcn_ballot_w64(row_far(L[0], kFar) || row_far(L[1], kFar));
   f32x4 us[2][kU], ws[2][kU];
 #pragma unroll
@@ -183,6 +181,8 @@ __global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diff
 
   st.store(tiles[0]);
   __syncthreads();
+  uint32_t row_e = row_c;
+  asm("" : "+v"(row_e));
   int at = 0;
   for (int64_t blk = 0; blk < blocks; ++blk) {
     const int buf = kBufs == 2 ? (int)blk & 1 : 0;
@@ -213,7 +213,7 @@ __global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diff
     }
 #pragma unroll
     for (int m = 0; m < 2; ++m) to_weights<T>(b, by, L[m], p[m]);
-    if (__builtin_amdgcn_ballot_w64(held[0] < enough[0] || held[1] < enough[1])) {
+    if (__builtin_amdgcn_ballot_w64(moves[0] || moves[1])) {
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
         float sp = 0.f, sd = 0.f;
@@ -224,11 +224,11 @@ __global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diff
             sp += p[m][kt][r];
             sd = fmaf(p[m][kt][r], dp[kt][r] - center[m], sd);
           }
-        sp = group_sum(sp) + held[m];
+        sp = group_sum(sp + weight[m]);
         sd = group_sum(sd);
         // the keys before it add nothing to sd: c_t is their mean
-        const float move = held[m] < enough[m] && sp > 0.f ? sd / sp : 0.f;
-        held[m] = held[m] < enough[m] ? sp : held[m];
+        const float move = moves[m] && sp > 0.f ? sd / sp : 0.f;
+        moves[m] = moves[m] && !(sp >= kEnough && fabsf(L[m]) <= kFarSum);
         center[m] += move;
         off[m] = fmaf(-move, weight[m], off[m]);
 #pragma unroll
@@ -292,12 +292,16 @@ __global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diff
       }
     }
   }
+  // the row's head and query again: through the loop they took the registers that a
+  // second wave a SIMD needs
+  const uint32_t hg_e = row_e / nq, qi_e = row_e - hg_e * nq;
+  const int head_e = kv * P.group + hg_e;
   float by[2];  // dq's factors; and D_t - c_t in `off`
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
     weight[m] = weight[m] > 0.f ? 1.f / weight[m] : 0.f;  // a row without keys is zeros
     off[m] *= weight[m];
-    by[m] = P.scale * weight[m] * (m ? -lam : 1.f);
+    by[m] = P.scale * weight[m] * (m ? -lams[wave][li] : 1.f);
   }
   if constexpr (KS > 1) {
     float* po = reinterpret_cast<float*>(&tiles[0]);  // [wave][map][row][D + 2]
@@ -314,11 +318,11 @@ __global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diff
     const int m = ks * 2 / KS, first = ks * kOwn % kU;
     if (!row_on) return;
     if (lg == 0 && first == 0) {
-      const int64_t at = (item * 2 * P.heads + 2 * head + m) * P.nq + qi;
+      const int64_t at = (item * 2 * P.heads + 2 * head_e + m) * P.nq + qi_e;
       P.delta[at] = off[m] + center[m];
       P.norm[at] = weight[m];
     }
-    T* out = P.dq.p + item * P.dq.item + (2 * head + m) * P.dq.head + qi * P.dq.token;
+    T* out = P.dq.p + item * P.dq.item + (2 * head_e + m) * P.dq.head + qi_e * P.dq.token;
 #pragma unroll
     for (int u = 0; u < kOwn; ++u) {
       const int col = 16 * (first + u) + 4 * lg;
@@ -338,11 +342,11 @@ __global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diff
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
     if (lg == 0) {
-      const int64_t at = (item * 2 * P.heads + 2 * head + m) * P.nq + qi;
+      const int64_t at = (item * 2 * P.heads + 2 * head_e + m) * P.nq + qi_e;
       P.delta[at] = off[m] + center[m];
       P.norm[at] = weight[m];
     }
-    T* out = P.dq.p + item * P.dq.item + (2 * head + m) * P.dq.head + qi * P.dq.token;
+    T* out = P.dq.p + item * P.dq.item + (2 * head_e + m) * P.dq.head + qi_e * P.dq.token;
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
       float v[4];
