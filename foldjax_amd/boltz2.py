@@ -181,7 +181,8 @@ def pairformer_layer_forward(
     dropout=None,
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """Boltz-2 ``pairformer_layer_forward`` (``B2K/pairformer.py:100-206``):
-    every residual is fused into the producing kernel. ``params`` is the
+    every residual is fused into the producing kernel (with ``dropout`` the four
+    triangle updates are added by ``kernels.dropout_add``). ``params`` is the
     Boltz-2 layer dict, or a ``foldjax_amd.pairformer.PairformerLayerWeights``.
     ``dropout``: a ``foldjax_amd.pairformer.PairDropout`` of the four triangle
     updates."""
@@ -224,7 +225,8 @@ def pairformer_no_seq_layer_forward(
     """Boltz-2 ``pairformer_no_seq_layer_forward`` (``B2K/msa.py:467-539``),
     the MSA module's pair block: z += tri-mul outgoing, incoming, tri-attn
     starting, ending (all with ``pair_mask``) and the unmasked pair
-    transition, each residual fused into its kernel. ``params`` is the
+    transition, each residual fused into its kernel (the triangle updates' not
+    with ``dropout``). ``params`` is the
     Boltz-2 dict with ``tri_mul_out``, ``tri_mul_in``, ``tri_att_start``,
     ``tri_att_end`` and ``transition_z``; the chunk arguments are accepted for
     signature parity (the kernels stream with a fixed workspace). ``dropout``: a

@@ -23,10 +23,11 @@ constexpr float kSlack = 8.f;
 // What bounds it: vector instructions (an exponential, its fma and two bf16 parts
 // a weight and map: 6 to a matrix instruction) and the matrix instructions, which
 // on one SIMD run beside other waves' vector work only in part. 499 rows of 499
-// tokens, 2 heads with their bias: 318 us, the SIMDs 58 % in vector and 29 % in matrix
-// instructions; 245 rows of 245: 51 us, 44 and 18 %, a quarter of it the workgroups'
+// tokens, 2 heads with their bias: 280 us (at the clock that the card has after a
+// hundred passes, as all figures here), the SIMDs 60 % in vector and 29 % in matrix
+// instructions; 245 rows of 245: 47 us, 45 and 18 %, a quarter of it the workgroups'
 // starts and ends (4 blocks of keys each). One token of 8 sequences against 16384
-// keys (134 MB, keywise and split): 26.5 us, the copy rate, and 4.3 for the join.
+// keys (134 MB, keywise and split): 25.7 us, the copy rate, and 4.8 for the join.
 //
 // KS 4 (keywise): the four waves share one 16-row tile and take 32 keys each of a
 // 128-key block, for calls with few rows; KS 1: each has 16 rows of its own and

@@ -7,8 +7,8 @@
 // weights: 1e-6 of them at |L| = 32, but of the order of 1 under the biases of -1e5 and
 // beyond that masks add to whole rows (where L is the maximum alone, and the weights
 // add up to the number of keys). So the kernel for dq divides by the sum of P_t, and
-// leaves it for the others, which divide too wherever a row has |L| > kFarSum. Every sum has one owner and one order:
-// no atomics, and the same bits each time.
+// leaves it for the others, which divide too wherever a row has |L| > kFarSum. Every
+// sum has one owner and one order: no atomics, and the same bits each time.
 //
 // dS's rows sum to zero, so its products may cancel: like the weights it goes
 // into them as two bf16 parts, and a gradient is off by its own rounding. With
@@ -80,10 +80,12 @@ __device__ __forceinline__ float sum8(const float (&x)[8]) {
 // as the start of dP's accumulators it left D_2 off by 1e-6 in common.) Against a
 // first walk for D_t alone this trades a second set of scores, dP and exponentials
 // for the products W, half the time. W takes two bf16 parts as well.
-// Bound like the forward kernel, with two waves a SIMD (256 registers): 70 us at 245
-// rows of 245 tokens and 2 heads, mostly vector instructions, a quarter of it starts
-// and ends; 22 us at 4 x 499 tokens and 6 heads (64 and 20 with one centre of the first
-// block for both maps, which lost dq's digits in rows of one heavy key).
+// Bound like the forward kernel, with two waves a SIMD (256 registers; at 64 channels
+// one): 69 us at 245 rows of 245 tokens and 2 heads, 50 % vector and 13 % matrix
+// instructions, a quarter of it starts and ends; 23 us at 4 x 499 tokens and 6 heads (62
+// and 19 with one centre of the first block for both maps, which lost dq's digits in
+// rows of one heavy key, and without far rows). 64 of a block's vector instructions are
+// copies still: the sums of P and P (dP - c) come after parts() has overwritten them.
 //
 // KS 4: the four waves share 16 rows and take 32 keys each of a 128-key block, for
 // calls with few rows; KS 1: each has rows of its own.
@@ -399,8 +401,8 @@ __device__ __forceinline__ void dlambda_of(const DiffAttnParams<T>& P, int head,
 // a plane of its own. KS 4: the four waves share 16 keys and take 32 queries each
 // of a 128-query block, for calls with few keys; 2: two of eight share 16 and take
 // 64 each, so that a CU with one workgroup has two waves a SIMD. Bound like the
-// kernel for dq: 63 us at 245 rows of 245 tokens and 2 heads, 24 us with dbias at
-// 4 x 499 and 6.
+// kernel for dq (41 % vector, 14 % matrix instructions): 62 us at 245 rows of 245
+// tokens and 2 heads, 22 us with dbias at 4 x 499 and 6.
 template <typename T, int D, int KS, bool DBIAS>
 __global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diffattn_dkv_kernel(DiffAttnParams<T> P) {
   typedef DaForm<KS> Form;
@@ -733,7 +735,7 @@ __global__ __launch_bounds__((DaForm<KS>::kThreads), (kDaWaves<T, D>)) void diff
 // a workgroup owns 64 queries x 64 keys of one head and adds dS over the items
 // of its chunk in registers; the chunks' sums are added by diffattn_bias_sum.
 // What bounds it is the 32 KB of k, v, q and dO that each item of a tile brings from
-// L2: 42 us at 245 rows of 245 tokens and 2 heads, 6.1 TB/s (three waves a SIMD in
+// L2: 40 us at 245 rows of 245 tokens and 2 heads, 6.4 TB/s (three waves a SIMD in
 // place of two change it by a few percent).
 template <typename T, int D>
 __global__ __launch_bounds__(256, (kDaWaves<T, D> + (kDaWaves<T, D> > 1))) void diffattn_dbias_kernel(DiffAttnParams<T> P) {
@@ -905,13 +907,15 @@ void bwd(const DiffAttnParams<T>& P, hipStream_t st) {
   const int64_t kvh = P.heads / P.group;
   // Waves with rows (keys) of their own cost the least work; they share 16 where
   // that leaves too few workgroups for the card's 256 CUs. us own / shared by four,
-  // 499 tokens: dq in bf16 at D = 32 at 96 workgroups 18.8 / 14.9, 144 19.1 / 21.6; at
-  // D = 64 120 29.0 / 30.2; float32 D = 32 120 46.9 / 33.5, 144 48.0 / 47.6; D = 64
-  // 120 89 / 69. dk and dv at D = 64 120 37.8 / 34.7, 144 38.2 / 50.3; float32 D = 32
-  // 120 59.9 / 43.2, 144 61.1 / 61.9; bf16 at D = 32, own / by two / by four: 144 27.8 /
-  // 23.0 / 25.8, 192 28.4 / 24.3 / 27.1, 240 29.3 / 24.6 / 31.1 (one such workgroup
-  // fits a CU; the other types' registers leave one wave a SIMD). By two gains
-  // nothing in the forward kernel and dq (18.3 and 19.5 either way at 192).
+  // 499 tokens: dq in bf16 at D = 32 at 120 workgroups 22.9 / 16.9, 144 22.4 / 25.6; at
+  // D = 64 120 29.8 / 34.0 (the one form that would rather change over earlier), 144
+  // 29.7 / 48.4; float32 D = 32 120 49.0 / 34.4, 144 49.0 / 48.4; D = 64 120 86.9 / 70.7,
+  // 144 88 / 102. dk and dv in bf16 at D = 64 120 39.2 / 35.3, 144 39.6 / 51.6; float32 D =
+  // 32 120 54.2 / 45.9, 144 55.1 / 66.5; D = 64 120 94 / 73, 144 95 / 106; bf16 at D = 32,
+  // own / by two / by four: 120 24.9 / 20.9 / 16.5, 144 25.5 / 21.3 / 25.3, 192 26.4 /
+  // 22.0 / 26.2, 240 27.1 / 23.6 / 29.9 (one such workgroup fits a CU; the other types'
+  // registers leave one wave a SIMD). By two gained nothing in the forward kernel and dq
+  // (18.3 and 19.5 either way at 192).
   constexpr bool kPaired = sizeof(T) == 2 && D == 32;
   const int64_t heads = P.items * kvh, rows = P.group * P.nq;
   const int64_t row_wgs = heads * ((rows + 63) / 64), key_wgs = heads * ((P.nk + 63) / 64);

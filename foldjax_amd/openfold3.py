@@ -119,7 +119,8 @@ def pair_block(
     here addresses the transposed grid directly, which is the same update
     without the two transposed copies. ``chunk_size`` is accepted for
     signature parity (the kernels stream rows with a fixed workspace).
-    ``dropout`` drops the four triangle updates."""
+    ``dropout`` drops the four triangle updates, which ``kernels.dropout_add``
+    then adds."""
     dropout = None if dropout is None else dropout.drawn()
 
     def add(z, sublayer, update, *args, **more):
