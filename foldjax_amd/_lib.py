@@ -22,6 +22,8 @@ FJX_INCOMING = 1
 FJX_CODES_NONE = 0
 FJX_CODES_E4M3 = 1
 FJX_CODES_INT8 = 2
+FJX_INDEX_I32 = 0
+FJX_INDEX_I64 = 1
 FJX_SHARE_N = 1
 FJX_SHARE_M = 2
 FJX_SHARE_C = 4
@@ -31,7 +33,7 @@ FJX_ERR_UNSUPPORTED = 2
 FJX_ERR_WORKSPACE = 3
 FJX_ERR_HIP = 4
 
-ABI_VERSION = 7
+ABI_VERSION = 8
 NOALLOC_SCRATCH_BYTES = 3 * 591 * 640 * 256
 
 _vp = ctypes.c_void_p
@@ -40,7 +42,9 @@ _i32 = ctypes.c_int32
 _f32 = ctypes.c_float
 _sz = ctypes.c_size_t
 _u64 = ctypes.c_uint64
+_i64x2 = _i64 * 2
 _i64x3 = _i64 * 3
+_i64x4 = _i64 * 4
 
 
 class TriMulArgs(ctypes.Structure):
@@ -154,6 +158,44 @@ class DropoutArgs(ctypes.Structure):
     ]
 
 
+class PackedAttentionArgs(ctypes.Structure):
+    _fields_ = [
+        ("tokens_q", _i64), ("tokens_k", _i64), ("sequences", _i64), ("heads", _i64), ("kv_heads", _i64), ("head_dim", _i64),
+        ("dtype", _i32), ("index_dtype", _i32), ("causal", _i32), ("zero_tail", _i32), ("scale", _f32),
+        ("q", _vp), ("k", _vp), ("v", _vp), ("out", _vp),
+        ("q_strides", _i64x2), ("k_strides", _i64x2), ("v_strides", _i64x2), ("out_strides", _i64x2),
+        ("q_starts", _vp), ("k_starts", _vp), ("k_lengths", _vp),
+        ("lse", _vp), ("rest", _vp), ("rest_strides", _i64x2),
+        ("workspace", _vp), ("workspace_bytes", _sz),
+    ]
+
+
+class PackedAttentionBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("fwd", PackedAttentionArgs),
+        ("dout", _vp), ("dq", _vp), ("dk", _vp), ("dv", _vp),
+        ("dout_strides", _i64x2), ("dq_strides", _i64x2), ("dk_strides", _i64x2), ("dv_strides", _i64x2),
+    ]
+
+
+class HeadNormRotaryArgs(ctypes.Structure):
+    _fields_ = [
+        ("items", _i64), ("heads", _i64), ("kv_heads", _i64), ("tokens", _i64), ("head_dim", _i64),
+        ("dtype", _i32), ("index_dtype", _i32), ("neighbours", _i32), ("axes", _i32), ("sections", _i64x4), ("eps", _f32),
+        ("q", _vp), ("k", _vp), ("q_weight", _vp), ("k_weight", _vp),
+        ("positions", _vp), ("position_strides", _i64x2), ("frequencies", _vp), ("q_out", _vp), ("k_out", _vp),
+        ("q_strides", _i64x3), ("k_strides", _i64x3), ("q_out_strides", _i64x3), ("k_out_strides", _i64x3),
+    ]
+
+
+class HeadNormRotaryBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("fwd", HeadNormRotaryArgs),
+        ("dq", _vp), ("dk", _vp), ("dq_strides", _i64x3), ("dk_strides", _i64x3),
+        ("dq_weight", _vp), ("dk_weight", _vp), ("workspace", _vp), ("workspace_bytes", _sz),
+    ]
+
+
 # every symbol the header declares, with its ctypes signature
 SYMBOLS = {
     "fjx_trimul_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i32]),
@@ -176,6 +218,13 @@ SYMBOLS = {
     "fjx_rms_norm_bwd_workspace_size": (_sz, [_i64, _i64]),
     "fjx_rms_norm_bwd": (ctypes.c_int, [ctypes.POINTER(RmsNormBwdArgs), _vp]),
     "fjx_dropout_fwd": (ctypes.c_int, [ctypes.POINTER(DropoutArgs), _vp]),
+    "fjx_packed_attention_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64, _i32]),
+    "fjx_packed_attention_fwd": (ctypes.c_int, [ctypes.POINTER(PackedAttentionArgs), _vp]),
+    "fjx_packed_attention_bwd_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64, _i32]),
+    "fjx_packed_attention_bwd": (ctypes.c_int, [ctypes.POINTER(PackedAttentionBwdArgs), _vp]),
+    "fjx_head_norm_rotary_fwd": (ctypes.c_int, [ctypes.POINTER(HeadNormRotaryArgs), _vp]),
+    "fjx_head_norm_rotary_bwd_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i64]),
+    "fjx_head_norm_rotary_bwd": (ctypes.c_int, [ctypes.POINTER(HeadNormRotaryBwdArgs), _vp]),
     "fjx_last_error": (ctypes.c_char_p, []),
     "fjx_abi_version": (ctypes.c_int, []),
     "fjx_prof_enable": (ctypes.c_int, [ctypes.c_int]),

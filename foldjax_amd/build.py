@@ -55,6 +55,8 @@ def _hipcc() -> str:
 FILE_FLAGS = {
     "fjx_diffattn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "fjx_diffattn_bwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "fjx_packed.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "fjx_packed_bwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "fjx_single_flash.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],
     "fjx_flash.hip": ["-fno-honor-nans", "-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "fjx_rowproj.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1", "-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],

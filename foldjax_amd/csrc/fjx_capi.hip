@@ -13,6 +13,7 @@
 #include "fjx_common.hpp"
 #include "fjx_diffattn.hpp"
 #include "fjx_kernels.hpp"
+#include "fjx_packed.hpp"
 
 using namespace fjx;
 
@@ -64,6 +65,10 @@ enum KernelId {
   K_RMS_NORM_FWD,
   K_RMS_NORM_BWD,
   K_DROPOUT,
+  K_PACKED_ATTENTION_FWD,
+  K_PACKED_ATTENTION_BWD,
+  K_HEAD_NORM_FWD,
+  K_HEAD_NORM_BWD,
   K_COUNT
 };
 const char* kKernelNames[K_COUNT] = {"trimul_prologue", "trimul_contract", "trimul_epilogue",
@@ -71,7 +76,9 @@ const char* kKernelNames[K_COUNT] = {"trimul_prologue", "trimul_contract", "trim
                                      "triattn_core_prep", "transition",     "single_proj",
                                      "single_pair_bias", "single_flash",   "single_out",
                                      "single_transition", "diff_attention_fwd", "diff_attention_bwd",
-                                     "rms_norm_fwd",     "rms_norm_bwd",   "dropout"};
+                                     "rms_norm_fwd",     "rms_norm_bwd",   "dropout",
+                                     "packed_attention_fwd", "packed_attention_bwd", "head_norm_rotary_fwd",
+                                     "head_norm_rotary_bwd"};
 
 struct Prof {
   std::mutex mu;
@@ -1278,6 +1285,263 @@ int diff_bwd_run(const fjx_diff_attention_bwd_args* b, const DiffBwdPlan& plan, 
                [&] { launch_diffattn_bwd<T>(p, (int)a->head_dim, st); });
 }
 
+// ------------------------------------------------------ packed attention
+// How a call is cut. The host knows how many sequences and tokens there are, not how
+// long each is: `own` counts the workgroups of R tiles a wave if all lengths were alike.
+struct PackedPlan {
+  PackedForm rows, keys;
+  int splits;                // of the keys (forward, keywise), of the heads that share keys (dk, dv)
+  size_t part_o, part_ml;    // workspace bytes: forward; backward: one of dk, dv and D
+};
+int packed_width(int64_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
+PackedForm packed_form(int64_t tokens, int64_t seqs, int64_t per, int64_t kvh, int64_t other, int32_t dtype) {
+  const int64_t rows = tokens * per;
+  auto own = [&](int64_t tile) { return kvh * ((rows + tile - 1) / tile); };
+  PackedForm f = {};
+  f.keywise = other > 64 * seqs && (rows <= 16 * seqs || own(64) < 128);
+  f.tiles = !f.keywise && dtype == FJX_DTYPE_BF16 && own(128) >= 256 ? 2 : 1;
+  const int64_t tile = f.keywise ? 16 : 64 * f.tiles;
+  const int64_t count = rows / tile + seqs + 1;
+  f.count = (int)std::min<int64_t>(count, 1 << 30);
+  return f;
+}
+PackedPlan packed_fwd_plan(int64_t tq, int64_t tk, int64_t seqs, int64_t heads, int64_t kvh, int64_t d, int32_t dtype) {
+  const int64_t group = heads / kvh;
+  PackedPlan p = {};
+  p.rows = packed_form(tq, seqs, group, kvh, tk, dtype);
+  p.splits = 1;
+  if (p.rows.keywise) {
+    const int64_t wgs = kvh * std::max(seqs, tq * group / 16);
+    // two blocks of 128 keys a split at least, were the lengths alike
+    const int64_t want = wgs <= 128 ? std::min<int64_t>(512 / wgs, tk / seqs / 256) : 1;
+    if (want > 1) {
+      p.splits = (int)want;
+      const size_t r = (size_t)heads * tq * p.splits;
+      p.part_o = align_up(r * packed_width(d) * sizeof(float));
+      p.part_ml = align_up(r * 2 * sizeof(float));
+    }
+  }
+  return p;
+}
+PackedPlan packed_bwd_plan(int64_t tq, int64_t tk, int64_t seqs, int64_t heads, int64_t kvh, int64_t d, int32_t dtype) {
+  const int64_t group = heads / kvh;
+  PackedPlan p = {};
+  p.rows = packed_form(tq, seqs, group, kvh, tk, dtype);
+  p.keys = packed_form(tk, seqs, 1, kvh, tq * group, dtype);
+  if (!tq) p.rows.count = 0;
+  if (!tk) p.keys.count = 0;
+  p.splits = 1;
+  // workgroups that walk long and, causal, uneven ways: the heads that share keys in parts
+  const int64_t wgs = kvh * ((tk + 64 * p.keys.tiles - 1) / (64 * p.keys.tiles));
+  if (!p.keys.keywise && group > 1 && tk && wgs < 1024) {
+    p.splits = (int)std::min<int64_t>(group, (1024 + wgs - 1) / wgs);
+    p.part_o = align_up((size_t)p.splits * kvh * tk * packed_width(d) * sizeof(float));
+  }
+  p.part_ml = align_up((size_t)heads * tq * sizeof(float));
+  return p;
+}
+
+// {head, token} strides that the kernels' 16-byte accesses of rows take
+bool packed_strides_ok(const int64_t* s, int64_t heads, int64_t tokens, int64_t d, size_t es) {
+  if (heads > 1 && (s[0] < 1 || s[0] * (int64_t)es % 16)) return false;
+  return tokens < 2 || (s[1] >= d && s[1] * (int64_t)es % 16 == 0 && s[1] * (int64_t)es < 1 << 24);
+}
+
+int packed_check(const fjx_packed_attention_args* a, const char* fn) {
+  if (a->tokens_q < 0 || a->tokens_k < 0 || a->sequences < 1 || a->heads < 1 || a->kv_heads < 1)
+    return fail(FJX_ERR_INVALID, "%s: sequences, heads and kv_heads must be >= 1, tokens >= 0", fn);
+  if (!dtype_ok(a->dtype)) return fail(FJX_ERR_INVALID, "%s: unknown dtype %d", fn, a->dtype);
+  if (a->index_dtype != FJX_INDEX_I32 && a->index_dtype != FJX_INDEX_I64)
+    return fail(FJX_ERR_INVALID, "%s: unknown index_dtype %d", fn, a->index_dtype);
+  if (a->head_dim < 8 || a->head_dim % 8 || a->head_dim > 128 || a->heads > 1024)
+    return fail(FJX_ERR_UNSUPPORTED, "%s: this build supports head_dim in multiples of 8 up to 128 and at most 1024 heads, got %lld and %lld",
+                fn, (long long)a->head_dim, (long long)a->heads);
+  if (a->heads % a->kv_heads)
+    return fail(FJX_ERR_INVALID, "%s: kv_heads must divide heads, got %lld and %lld", fn, (long long)a->kv_heads,
+                (long long)a->heads);
+  if (!(a->scale >= 1e-30f && a->scale <= 1e30f))
+    return fail(FJX_ERR_INVALID, "%s: scale must be in [1e-30, 1e30], got %g", fn, (double)a->scale);
+  if ((a->tokens_q && (!a->q || !a->out)) || (a->tokens_k && (!a->k || !a->v)) || !a->q_starts || !a->k_starts)
+    return fail(FJX_ERR_INVALID, "%s: a required pointer is NULL", fn);
+  if (!aligned16({a->q, a->k, a->v, a->out, a->rest}) || reinterpret_cast<uintptr_t>(a->lse) % 8)
+    return fail(FJX_ERR_INVALID, "%s: tensors must be 16-byte aligned", fn);
+  const uintptr_t is = a->index_dtype == FJX_INDEX_I64 ? 8 : 4;
+  if (reinterpret_cast<uintptr_t>(a->q_starts) % is || reinterpret_cast<uintptr_t>(a->k_starts) % is ||
+      reinterpret_cast<uintptr_t>(a->k_lengths) % is)
+    return fail(FJX_ERR_INVALID, "%s: offsets must be aligned to their elements", fn);
+  if (a->rest && a->dtype == FJX_DTYPE_F32)
+    return fail(FJX_ERR_INVALID, "%s: rest is of bf16 outputs", fn);
+  constexpr int64_t kLong = (int64_t)1 << 31;
+  if (a->tokens_q * a->heads >= kLong || a->tokens_k >= kLong || a->sequences >= 1 << 22)
+    return fail(FJX_ERR_UNSUPPORTED, "%s: tokens_q * heads and tokens_k must be below 2^31, sequences below 2^22", fn);
+  const size_t es = esize(a->dtype);
+  const int64_t d = a->head_dim;
+  if (!packed_strides_ok(a->q_strides, a->heads, a->tokens_q, d, es) ||
+      !packed_strides_ok(a->k_strides, a->kv_heads, a->tokens_k, d, es) ||
+      !packed_strides_ok(a->v_strides, a->kv_heads, a->tokens_k, d, es) ||
+      !packed_strides_ok(a->out_strides, a->heads, a->tokens_q, d, es) ||
+      (a->rest && !packed_strides_ok(a->rest_strides, a->heads, a->tokens_q, d, es)))
+    return fail(FJX_ERR_INVALID, "%s: strides must be positive multiples of 16 bytes, a token's at least head_dim and below 2^24 bytes", fn);
+  return FJX_OK;
+}
+int packed_launch_ok(const char* fn, const PackedForm& f, int64_t kvh, int splits) {
+  if ((double)f.count * kvh * splits >= (1 << 23)) return fail(FJX_ERR_UNSUPPORTED, "%s: more rows than one launch takes", fn);
+  return FJX_OK;
+}
+
+template <typename T>
+PackedParams<T> packed_params(const fjx_packed_attention_args* a) {
+  PackedParams<T> p = {};
+  // one token has no stride of its own: rows behind it must not be taken for it
+  auto view = [&](const void* ptr, const int64_t* s, int64_t tokens) {
+    return PackedView<const T>{static_cast<const T*>(ptr), s[0], tokens > 1 ? s[1] : a->head_dim};
+  };
+  p.q = view(a->q, a->q_strides, a->tokens_q);
+  p.k = view(a->k, a->k_strides, a->tokens_k);
+  p.v = view(a->v, a->v_strides, a->tokens_k);
+  const int wide = a->index_dtype == FJX_INDEX_I64;
+  p.q_starts = {a->q_starts, wide};
+  p.k_starts = {a->k_starts, wide};
+  p.k_lengths = {a->k_lengths, wide};
+  p.tq = a->tokens_q;
+  p.tk = a->tokens_k;
+  p.seqs = (int)a->sequences;
+  p.heads = (int)a->heads;
+  p.group = (int)(a->heads / a->kv_heads);
+  p.d = (int)a->head_dim;
+  p.scale = a->scale;
+  p.scale_log2 = a->scale * kLog2e;
+  p.causal = a->causal != 0;
+  p.zero_tail = a->zero_tail != 0;
+  p.lse = a->lse;
+  return p;
+}
+
+template <typename T>
+int packed_fwd_run(const fjx_packed_attention_args* a, const PackedPlan& plan, hipStream_t st) {
+  PackedParams<T> p = packed_params<T>(a);
+  p.out = {static_cast<T*>(a->out), a->out_strides[0], a->out_strides[1]};
+  p.rest = {static_cast<T*>(a->rest), a->rest_strides[0], a->rest_strides[1]};
+  p.tiles = plan.rows.count;
+  p.splits = plan.splits;
+  p.part_o = at<float>(a->workspace, 0);
+  p.part_ml = at<float>(a->workspace, plan.part_o);
+  PackedForm form = plan.rows;
+  form.count *= plan.splits;
+  return timed(K_PACKED_ATTENTION_FWD, st, "packed_attention_fwd", [&] { launch_packed_fwd<T>(p, form, st); });
+}
+
+template <typename T>
+int packed_bwd_run(const fjx_packed_attention_bwd_args* b, const PackedPlan& plan, hipStream_t st) {
+  const fjx_packed_attention_args* a = &b->fwd;
+  PackedParams<T> p = packed_params<T>(a);
+  auto in = [&](const void* ptr, const int64_t* s) {
+    return PackedView<const T>{static_cast<const T*>(ptr), s[0], a->tokens_q > 1 ? s[1] : a->head_dim};
+  };
+  auto out = [](void* ptr, const int64_t* s) { return PackedView<T>{static_cast<T*>(ptr), s[0], s[1]}; };
+  p.dout = in(b->dout, b->dout_strides);
+  p.o = in(a->out, a->out_strides);
+  p.o_rest = in(a->rest, a->rest_strides);
+  p.dq = out(b->dq, b->dq_strides);
+  p.dk = out(b->dk, b->dk_strides);
+  p.dv = out(b->dv, b->dv_strides);
+  p.zero_tail = 1;
+  p.splits = plan.splits;
+  p.part_dk = at<float>(a->workspace, 0);
+  p.part_dv = at<float>(a->workspace, plan.part_o);
+  p.delta = at<float>(a->workspace, 2 * plan.part_o);
+  return timed(K_PACKED_ATTENTION_BWD, st, "packed_attention_bwd",
+               [&] { launch_packed_bwd<T>(p, plan.rows, plan.keys, st); });
+}
+
+// ------------------------------------------------- heads' norm and rotation
+// `writes`: q_out and k_out are outputs (in the backward pass gradients that are read)
+int head_norm_check(const fjx_head_norm_rotary_args* a, const char* fn, bool writes) {
+  if (a->items < 1 || a->tokens < 1 || a->heads < 1 || a->kv_heads < 0)
+    return fail(FJX_ERR_INVALID, "%s: items, tokens and heads must be >= 1, kv_heads >= 0", fn);
+  if (!dtype_ok(a->dtype)) return fail(FJX_ERR_INVALID, "%s: unknown dtype %d", fn, a->dtype);
+  if (a->index_dtype != FJX_INDEX_I32 && a->index_dtype != FJX_INDEX_I64)
+    return fail(FJX_ERR_INVALID, "%s: unknown index_dtype %d", fn, a->index_dtype);
+  if (a->head_dim < 8 || a->head_dim % 8 || a->head_dim > 256 || a->heads > 1024 || a->kv_heads > 1024)
+    return fail(FJX_ERR_UNSUPPORTED, "%s: this build supports head_dim in multiples of 8 up to 256 and at most 1024 heads, got %lld and %lld",
+                fn, (long long)a->head_dim, (long long)std::max(a->heads, a->kv_heads));
+  if (a->axes < 1 || a->axes > 4) return fail(FJX_ERR_INVALID, "%s: axes must be 1 to 4, got %d", fn, a->axes);
+  int64_t pairs = 0;
+  for (int i = 0; i < a->axes; ++i) {
+    if (a->sections[i] < 0 || a->sections[i] > a->head_dim / 2)
+      return fail(FJX_ERR_INVALID, "%s: sections must be in [0, head_dim / 2]", fn);
+    pairs += a->sections[i];
+  }
+  if (pairs % 4 || 2 * pairs > a->head_dim)
+    return fail(FJX_ERR_UNSUPPORTED, "%s: the rotated pairs must be a multiple of 4 and at most head_dim / 2, got %lld", fn,
+                (long long)pairs);
+  if (a->items >= (int64_t)1 << 31 || a->tokens >= (int64_t)1 << 31 || (double)a->items * a->tokens >= 0x1p40)
+    return fail(FJX_ERR_UNSUPPORTED, "%s: too many rows", fn);
+  if (!a->q || !a->q_out || (a->kv_heads && (!a->k || !a->k_out)) || (pairs && (!a->positions || !a->frequencies)))
+    return fail(FJX_ERR_INVALID, "%s: a required pointer is NULL", fn);
+  if (!aligned16({a->q, a->k, a->q_weight, a->k_weight, a->q_out, a->k_out}))
+    return fail(FJX_ERR_INVALID, "%s: tensors must be 16-byte aligned", fn);
+  if (reinterpret_cast<uintptr_t>(a->positions) % (a->index_dtype == FJX_INDEX_I64 ? 8 : 4) ||
+      reinterpret_cast<uintptr_t>(a->frequencies) % 8)
+    return fail(FJX_ERR_INVALID, "%s: positions and frequencies must be aligned to their elements", fn);
+  const size_t es = esize(a->dtype);
+  if (!diff_strides_ok(a->q_strides, a->items, a->heads, a->tokens, es, false) ||
+      !diff_strides_ok(a->q_out_strides, a->items, a->heads, a->tokens, es, writes) ||
+      (a->kv_heads && (!diff_strides_ok(a->k_strides, a->items, a->kv_heads, a->tokens, es, false) ||
+                       !diff_strides_ok(a->k_out_strides, a->items, a->kv_heads, a->tokens, es, writes))))
+    return fail(FJX_ERR_INVALID, "%s: strides must be multiples of 16 bytes, not negative (an output's: positive)", fn);
+  return FJX_OK;
+}
+
+template <typename T>
+HeadNormParams<T> head_norm_params(const fjx_head_norm_rotary_args* a) {
+  HeadNormParams<T> p = {};
+  auto in = [](const void* ptr, const int64_t* s) { return HeadNormView<const T>{static_cast<const T*>(ptr), s[0], s[1], s[2]}; };
+  auto out = [](void* ptr, const int64_t* s) { return HeadNormView<T>{static_cast<T*>(ptr), s[0], s[1], s[2]}; };
+  p.x[0] = in(a->q, a->q_strides);
+  p.x[1] = in(a->k, a->k_strides);
+  p.y[0] = out(a->q_out, a->q_out_strides);
+  p.y[1] = out(a->k_out, a->k_out_strides);
+  p.w[0] = static_cast<const T*>(a->q_weight);
+  p.w[1] = static_cast<const T*>(a->k_weight);
+  p.positions = a->positions;
+  p.pos_wide = a->index_dtype == FJX_INDEX_I64;
+  p.pos_axis = a->position_strides[0];
+  p.pos_item = a->position_strides[1];
+  int64_t end = 0;
+  for (int i = 0; i < 3; ++i) {
+    if (i < a->axes) end += a->sections[i];
+    p.axis_end[i] = i < a->axes - 1 ? (int)end : 1 << 30;
+  }
+  p.pairs = (int)(end + (a->axes == 4 ? a->sections[3] : 0));
+  p.frequencies = a->frequencies;
+  p.d = (int)a->head_dim;
+  p.neighbours = a->neighbours != 0;
+  p.items = a->items;
+  p.tokens = a->tokens;
+  p.heads[0] = (int)a->heads;
+  p.heads[1] = (int)a->kv_heads;
+  p.eps = a->eps;
+  return p;
+}
+
+template <typename T>
+int head_norm_run(const fjx_head_norm_rotary_args* a, hipStream_t st) {
+  const HeadNormParams<T> p = head_norm_params<T>(a);
+  return timed(K_HEAD_NORM_FWD, st, "head_norm_rotary_fwd", [&] { launch_headnorm<T>(p, st); });
+}
+
+template <typename T>
+int head_norm_bwd_run(const fjx_head_norm_rotary_bwd_args* b, hipStream_t st) {
+  HeadNormParams<T> p = head_norm_params<T>(&b->fwd);
+  auto out = [](void* ptr, const int64_t* s) { return HeadNormView<T>{static_cast<T*>(ptr), s[0], s[1], s[2]}; };
+  p.g[0] = out(b->dq, b->dq_strides);
+  p.g[1] = out(b->dk, b->dk_strides);
+  p.part = p.w[0] || p.w[1] ? static_cast<float*>(b->workspace) : nullptr;
+  return timed(K_HEAD_NORM_BWD, st, "head_norm_rotary_bwd",
+               [&] { launch_headnorm_bwd<T>(p, b->dq_weight, b->dk_weight, st); });
+}
+
 // -------------------------------------------------------------- RMS norm
 template <typename T>
 int rms_norm_run(const fjx_rms_norm_args* a, hipStream_t st) {
@@ -1651,6 +1915,98 @@ int fjx_dropout_fwd(const fjx_dropout_args* a, hipStream_t st) {
   if (!aligned16({a->x, a->residual, a->out})) return fail(FJX_ERR_INVALID, "%s: tensors must be 16-byte aligned", fn);
   if (reinterpret_cast<uintptr_t>(a->step) % 8) return fail(FJX_ERR_INVALID, "%s: step must be 8-byte aligned", fn);
   return a->dtype == FJX_DTYPE_BF16 ? dropout_run<bf16>(a, st) : dropout_run<float>(a, st);
+}
+
+size_t fjx_packed_attention_workspace_size(int64_t tokens_q, int64_t tokens_k, int64_t sequences, int64_t heads,
+                                           int64_t kv_heads, int64_t head_dim, int32_t dtype) {
+  if (tokens_q < 1 || tokens_k < 0 || sequences < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || head_dim < 1 ||
+      !dtype_ok(dtype))
+    return 0;
+  const PackedPlan p = packed_fwd_plan(tokens_q, tokens_k, sequences, heads, kv_heads, head_dim, dtype);
+  return p.part_o + p.part_ml;
+}
+
+int fjx_packed_attention_fwd(const fjx_packed_attention_args* a, hipStream_t st) {
+  const char* fn = "fjx_packed_attention_fwd";
+  g_err.clear();
+  if (!a) return fail(FJX_ERR_INVALID, "%s: args is NULL", fn);
+  if (int rc = packed_check(a, fn)) return rc;
+  if (!a->tokens_q) return FJX_OK;
+  const PackedPlan plan = packed_fwd_plan(a->tokens_q, a->tokens_k, a->sequences, a->heads, a->kv_heads, a->head_dim, a->dtype);
+  if (int rc = packed_launch_ok(fn, plan.rows, a->kv_heads, plan.splits)) return rc;
+  const size_t need = plan.part_o + plan.part_ml;
+  if (need && (!a->workspace || a->workspace_bytes < need))
+    return fail(FJX_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", fn, need, a->workspace_bytes);
+  if (need && !aligned16({a->workspace})) return fail(FJX_ERR_INVALID, "%s: the workspace must be 16-byte aligned", fn);
+  return a->dtype == FJX_DTYPE_BF16 ? packed_fwd_run<bf16>(a, plan, st) : packed_fwd_run<float>(a, plan, st);
+}
+
+size_t fjx_packed_attention_bwd_workspace_size(int64_t tokens_q, int64_t tokens_k, int64_t sequences, int64_t heads,
+                                               int64_t kv_heads, int64_t head_dim, int32_t dtype) {
+  if (tokens_q < 0 || tokens_k < 0 || sequences < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || head_dim < 1 ||
+      !dtype_ok(dtype))
+    return 0;
+  const PackedPlan p = packed_bwd_plan(tokens_q, tokens_k, sequences, heads, kv_heads, head_dim, dtype);
+  return 2 * p.part_o + p.part_ml;
+}
+
+int fjx_packed_attention_bwd(const fjx_packed_attention_bwd_args* b, hipStream_t st) {
+  const char* fn = "fjx_packed_attention_bwd";
+  g_err.clear();
+  if (!b) return fail(FJX_ERR_INVALID, "%s: args is NULL", fn);
+  const fjx_packed_attention_args* a = &b->fwd;
+  if (int rc = packed_check(a, fn)) return rc;
+  if ((a->tokens_q && (!b->dout || !b->dq || !a->lse)) || (a->tokens_k && (!b->dk || !b->dv)))
+    return fail(FJX_ERR_INVALID, "%s: a required pointer is NULL", fn);
+  if (!aligned16({b->dout, b->dq, b->dk, b->dv})) return fail(FJX_ERR_INVALID, "%s: tensors must be 16-byte aligned", fn);
+  const size_t es = esize(a->dtype);
+  if (!packed_strides_ok(b->dout_strides, a->heads, a->tokens_q, a->head_dim, es) ||
+      !packed_strides_ok(b->dq_strides, a->heads, a->tokens_q, a->head_dim, es) ||
+      !packed_strides_ok(b->dk_strides, a->kv_heads, a->tokens_k, a->head_dim, es) ||
+      !packed_strides_ok(b->dv_strides, a->kv_heads, a->tokens_k, a->head_dim, es))
+    return fail(FJX_ERR_INVALID, "%s: the gradients' strides must be positive multiples of 16 bytes, a token's at least head_dim and below 2^24 bytes", fn);
+  if (!a->tokens_q && !a->tokens_k) return FJX_OK;
+  const PackedPlan plan = packed_bwd_plan(a->tokens_q, a->tokens_k, a->sequences, a->heads, a->kv_heads, a->head_dim, a->dtype);
+  if (int rc = packed_launch_ok(fn, plan.rows, a->kv_heads, 1)) return rc;
+  if (int rc = packed_launch_ok(fn, plan.keys, a->kv_heads, plan.splits)) return rc;
+  const size_t need = 2 * plan.part_o + plan.part_ml;
+  if (need && (!a->workspace || a->workspace_bytes < need))
+    return fail(FJX_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", fn, need, a->workspace_bytes);
+  if (need && !aligned16({a->workspace})) return fail(FJX_ERR_INVALID, "%s: the workspace must be 16-byte aligned", fn);
+  return a->dtype == FJX_DTYPE_BF16 ? packed_bwd_run<bf16>(b, plan, st) : packed_bwd_run<float>(b, plan, st);
+}
+
+int fjx_head_norm_rotary_fwd(const fjx_head_norm_rotary_args* a, hipStream_t st) {
+  const char* fn = "fjx_head_norm_rotary_fwd";
+  g_err.clear();
+  if (!a) return fail(FJX_ERR_INVALID, "%s: args is NULL", fn);
+  if (int rc = head_norm_check(a, fn, true)) return rc;
+  return a->dtype == FJX_DTYPE_BF16 ? head_norm_run<bf16>(a, st) : head_norm_run<float>(a, st);
+}
+
+size_t fjx_head_norm_rotary_bwd_workspace_size(int64_t items, int64_t heads, int64_t kv_heads, int64_t tokens,
+                                               int64_t head_dim) {
+  if (items < 1 || heads < 1 || kv_heads < 0 || tokens < 1 || head_dim < 8 || head_dim % 8 || head_dim > 256) return 0;
+  return align_up((size_t)headnorm_bwd_blocks(items, tokens, (int)(heads + kv_heads), (int)head_dim) * 2 * head_dim * sizeof(float));
+}
+
+int fjx_head_norm_rotary_bwd(const fjx_head_norm_rotary_bwd_args* b, hipStream_t st) {
+  const char* fn = "fjx_head_norm_rotary_bwd";
+  g_err.clear();
+  if (!b) return fail(FJX_ERR_INVALID, "%s: args is NULL", fn);
+  const fjx_head_norm_rotary_args* a = &b->fwd;
+  if (int rc = head_norm_check(a, fn, false)) return rc;
+  if (!b->dq || (a->kv_heads && !b->dk) || (a->q_weight && !b->dq_weight) || (a->kv_heads && a->k_weight && !b->dk_weight))
+    return fail(FJX_ERR_INVALID, "%s: a required pointer is NULL", fn);
+  if (!aligned16({b->dq, b->dk, b->workspace})) return fail(FJX_ERR_INVALID, "%s: tensors must be 16-byte aligned", fn);
+  const size_t es = esize(a->dtype);
+  if (!diff_strides_ok(b->dq_strides, a->items, a->heads, a->tokens, es, true) ||
+      (a->kv_heads && !diff_strides_ok(b->dk_strides, a->items, a->kv_heads, a->tokens, es, true)))
+    return fail(FJX_ERR_INVALID, "%s: the gradients' strides must be positive multiples of 16 bytes", fn);
+  const size_t need = fjx_head_norm_rotary_bwd_workspace_size(a->items, a->heads, a->kv_heads, a->tokens, a->head_dim);
+  if ((a->q_weight || a->k_weight) && (!b->workspace || b->workspace_bytes < need))
+    return fail(FJX_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", fn, need, b->workspace_bytes);
+  return a->dtype == FJX_DTYPE_BF16 ? head_norm_bwd_run<bf16>(b, st) : head_norm_bwd_run<float>(b, st);
 }
 
 int fjx_prof_enable(int on) {

@@ -333,6 +333,38 @@ struct DropoutParams {
 template <typename T>
 void launch_dropout(const DropoutParams<T>& p, hipStream_t st);
 
+// the heads' norm and rotation (fjx_headnorm.hip); [0]: queries, [1]: keys. Strides in elements
+template <typename T>
+struct HeadNormView {
+  T* p;
+  int64_t item, head, token;
+};
+template <typename T>
+struct HeadNormParams {
+  HeadNormView<const T> x[2];
+  HeadNormView<T> y[2];    // outputs; backward: the outputs' gradients (not written)
+  HeadNormView<T> g[2];    // backward: the inputs' gradients
+  const T* w[2];           // [d], or null: no norm
+  const void* positions;   // int32 or int64, [axes][items or 1][tokens]
+  int pos_wide;
+  int64_t pos_axis, pos_item;
+  int axis_end[3];         // the pairs before these are of axes 0, 1, 2
+  const double* frequencies;  // [pairs], radians a position
+  int pairs, d;
+  bool neighbours;         // pairs (2 i, 2 i + 1) instead of (i, i + pairs)
+  int64_t items, tokens;
+  int heads[2];
+  float eps;
+  float* part;             // backward: [blocks][2][d] partial sums of the weights' gradients, or null
+  int chunks, per_chunk;   // teams of a token, and heads of one (set at the launch)
+  int64_t first;           // block of this launch
+};
+template <typename T>
+void launch_headnorm(HeadNormParams<T> p, hipStream_t st);
+int headnorm_bwd_blocks(int64_t items, int64_t tokens, int heads, int d);
+template <typename T>
+void launch_headnorm_bwd(HeadNormParams<T> p, float* dwq, float* dwk, hipStream_t st);
+
 // differential attention (fjx_diffattn.hip, fjx_diffattn_bwd.hip); the
 // parameters are in fjx_diffattn.hpp
 template <typename T>

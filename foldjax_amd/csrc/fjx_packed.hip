@@ -1,0 +1,356 @@
+// Packed attention, forward: one pass over a row's keys with the running maximum
+// and sum of the softmax.
+#include "fjx_packed.hpp"
+
+namespace fjx {
+
+namespace {
+
+// A wave holds R tiles of 16 rows, lane l row l % 16 of each, and walks the keys in
+// tiles of 16: S^T = K Q^T leaves the lane 4 keys of its own row a tile (keys 4 g + r,
+// g = l / 16), so a row's maximum and sum are the lane's own values and two lane swaps,
+// and the weights of two key tiles are the operand of O^T = V^T P^T as they lie.
+//
+// A bf16 weight is rounded once (half a step, 2^-9 of itself), and the row's sum is
+// that of the rounded weights, taken by the matrix cores as a row of ones times them:
+// the weights that are applied add up to one, and an output is off by less than its own
+// rounding. A weight may exceed 1 by up to 2^kSlack before the maximum is moved, which
+// saves the outputs' rescaling in all but the first blocks of a row.
+constexpr float kSlack = 8.f;
+
+// An exponent is the rounding of s scale log2(e) - M with M rounded: off by up to half
+// a step of M for all of a row's keys alike, which cancels in the softmax while 2 to that
+// is a number. Rows with |M| beyond take products rounded by themselves, whose largest is
+// M exactly.
+constexpr float kFar = 16777216.f;
+
+template <typename T, int DP, int KS, int R>
+__global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1)) void packed_fwd_kernel(PackedParams<T> P) {
+  typedef PkForm<KS> Form;
+  typedef PkRows<T, DP> Rows;
+  typedef typename Frag<T>::type F;
+  constexpr int kC = Rows::kC, kU = Rows::kU;
+  constexpr int kNt = Form::kBlock / KS / 16;  // key tiles of a wave in a block
+  constexpr int kTileRows = 16 * R * (KS == 1 ? 4 : 1), kShift = __builtin_ctz(kTileRows);
+  constexpr int kOperand = Form::kStage * Rows::kRowBytes;
+  constexpr int kSets = KS == 1 ? 1 : 4;       // of staged rows
+  constexpr int kStages = 4 * kOperand * kSets <= 160 * 1024 ? 2 : 1;
+  constexpr int kPo = DP + 2;
+  static_assert(KS == 1 || kStages * 2 * kOperand * kSets >= 4 * 16 * R * (kPo + 2) * 4, "the waves' sums");
+  __shared__ __attribute__((aligned(16))) unsigned char raw[kStages * 2 * kOperand * kSets];
+
+  const int t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int kvh = P.heads / P.group;
+  const int kv = blockIdx.x % kvh;
+  const uint32_t rest_id = blockIdx.x / kvh;
+  const int split = rest_id / (uint32_t)P.tiles;
+  const int tile_id = P.tiles - 1 - (int)(rest_id % (uint32_t)P.tiles);  // causal rows with the most keys first
+  PackedSpan sp;
+  if (!packed_span(P, false, P.group, kShift, tile_id, lane, sp)) return;
+  if (sp.seq == P.seqs && !P.zero_tail) return;
+  const int rows = sp.nq * P.group;
+  const int row0 = sp.tile * kTileRows;
+  if (row0 >= rows) return;
+  const int row_w = row0 + (KS == 1 ? 16 * R * wave : 0);
+
+  // of the lane's rows: head, token, and the keys that it sees: those before lim
+  int head[R], token[R], lim[R];
+  F qf[R][kC];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int row = row_w + 16 * r + li < rows ? row_w + 16 * r + li : rows - 1;
+    const int qi = row / P.group;
+    head[r] = kv * P.group + row - qi * P.group;
+    token[r] = sp.q0 + qi;
+    lim[r] = P.causal ? qi + sp.nk - sp.nq + 1 : sp.nk;
+    const T* q = P.q.p + head[r] * P.q.head + token[r] * P.q.token + 8 * lg;
+#pragma unroll
+    for (int c = 0; c < kC; ++c) qf[r][c] = 32 * c + 8 * lg < P.d ? load8(q + 32 * c) : F{};
+  }
+  const int last = (row0 + kTileRows < rows ? row0 + kTileRows : rows) - 1;
+  const int most = P.causal ? last / P.group + sp.nk - sp.nq + 1 : sp.nk;  // keys that the workgroup's rows see
+  const int lim_lo = __builtin_amdgcn_readfirstlane(lim[0]);               // that all of the wave's rows see,
+  const int lim_hi = row_w < rows ? __builtin_amdgcn_readlane(lim[R - 1], 15) : 0;  // and that any does
+  const int64_t blocks = most > 0 ? (most + Form::kBlock - 1) / Form::kBlock : 0;
+  const int blk0 = (int)(blocks * split / P.splits), blk1 = (int)(blocks * (split + 1) / P.splits);
+
+  unsigned char* const mine = raw + (KS == 1 ? 0 : wave * kStages * 2 * kOperand);
+  const int stager = KS == 1 ? wave : 0;
+  const int key_w = KS == 1 ? 0 : 32 * wave;  // the wave's (staged) keys of a block
+  PkCopy<T, DP, Form::kStage, Form::kOwners> kcopy, vcopy;
+  kcopy.init(P.k.token, P.d, stager, lane);
+  vcopy.init(P.v.token, P.d, stager, lane);
+  const T* ks = P.k.p + kv * P.k.head + (int64_t)sp.k0 * P.k.token;
+  const T* vs = P.v.p + kv * P.v.head + (int64_t)sp.k0 * P.v.token;
+  auto stage = [&](int blk, int at) {
+    unsigned char* s = mine + at * 2 * kOperand;
+    kcopy.issue(ks, (int64_t)blk * Form::kBlock + key_w, sp.nk, P.d, s, stager);
+    vcopy.issue(vs, (int64_t)blk * Form::kBlock + key_w, sp.nk, P.d, s + kOperand, stager);
+  };
+  PkLane<T, DP> at;
+  at.init(lane);
+
+  constexpr bool kOnes = sizeof(T) == 2;
+  F ones;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) ones[e] = from_f32<T>(1.f);
+  float m[R];
+  f32x4 l[R], o[R][kU];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    m[r] = -INFINITY;
+    l[r] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < kU; ++u) o[r][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  bool far = false;
+
+  if (kStages == 2) {
+    if (blk0 < blk1) stage(blk0, 0);
+    pk_sync<KS>();
+  }
+  for (int blk = blk0; blk < blk1; ++blk) {
+    const int cur = kStages == 2 ? (blk - blk0) & 1 : 0;
+    if (kStages == 1) {
+      stage(blk, 0);
+      pk_sync<KS>();
+    } else if (blk + 1 < blk1) {
+      stage(blk + 1, cur ^ 1);
+    }
+    const unsigned char* kt_ = mine + cur * 2 * kOperand;
+    const unsigned char* vt_ = kt_ + kOperand;
+    const int key0 = blk * Form::kBlock + key_w;
+    if (key0 < lim_hi) {
+      f32x4 s[R][kNt];
+#pragma unroll
+      for (int kt = 0; kt < kNt; ++kt) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) s[r][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < kC; ++c) {
+          const F kf = at.at_row(kt_, 16 * kt, c);
+#pragma unroll
+          for (int r = 0; r < R; ++r) mma(s[r][kt], kf, qf[r][c]);
+        }
+      }
+      if (key0 + 16 * kNt > lim_lo) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const int left = lim[r] - key0 - 4 * lg;
+#pragma unroll
+          for (int kt = 0; kt < kNt; ++kt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[r][kt][e] = 16 * kt + e < left ? s[r][kt][e] : -INFINITY;
+        }
+      }
+      float top[R];
+      bool moved = false;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        top[r] = -INFINITY;
+#pragma unroll
+        for (int kt = 0; kt < kNt; ++kt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top[r] = fmaxf(top[r], s[r][kt][e]);
+        top[r] = lanes4_max(top[r]) * P.scale_log2;
+        moved = moved || top[r] > m[r] + kSlack;
+      }
+      if (__builtin_amdgcn_ballot_w64(moved)) {
+        bool any = false;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const float mn = fmaxf(m[r], top[r]);
+          const float alpha = __builtin_amdgcn_exp2f(m[r] - pk_base(mn));  // 0 where no key was before
+          m[r] = mn;
+          any = any || fabsf(pk_base(mn)) > kFar;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            l[r][e] *= alpha;
+#pragma unroll
+            for (int u = 0; u < kU; ++u) o[r][u][e] *= alpha;
+          }
+        }
+        far = __builtin_amdgcn_ballot_w64(any);
+      }
+      float by = P.scale_log2;
+      if (far) {
+        by = 1.f;
+#pragma unroll
+        for (int r = 0; r < R; ++r) pk_round(P.scale_log2, s[r]);
+      }
+      F pf[R][kNt / 2];
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float base = pk_base(m[r]);
+#pragma unroll
+        for (int c = 0; c < kNt / 2; ++c) {
+          float p[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            p[e] = __builtin_amdgcn_exp2f(fmaf(s[r][2 * c + (e >> 2)][e & 3], by, -base));
+            if (!kOnes) l[r][e & 3] += p[e];
+          }
+          pf[r][c] = pack8<T>(p);
+          if (kOnes) mma(l[r], ones, pf[r][c]);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < kNt / 2; ++c)
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+          const F vf = at.at_col(vt_, 32 * c, u);
+#pragma unroll
+          for (int r = 0; r < R; ++r) mma(o[r][u], vf, pf[r][c]);
+        }
+    }
+    pk_sync<KS>();
+  }
+  float ls[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) ls[r] = kOnes ? l[r][0] : group_sum((l[r][0] + l[r][1]) + (l[r][2] + l[r][3]));
+
+  if constexpr (KS > 1) {
+    // the waves' partial rows, on the largest of their maxima
+    float* ml = reinterpret_cast<float*>(raw);  // [wave][row][2], then the outputs
+    auto slot = [&](int j, int r) { return (j * R + r) * 16 + li; };
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (lg == 0) {
+        ml[slot(wave, r) * 2] = m[r];
+        ml[slot(wave, r) * 2 + 1] = ls[r];
+      }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float mx = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) mx = fmaxf(mx, ml[slot(j, r) * 2]);
+      const float base = pk_base(mx);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum = fmaf(ml[slot(j, r) * 2 + 1], __builtin_amdgcn_exp2f(ml[slot(j, r) * 2] - base), sum);
+      const float alpha = __builtin_amdgcn_exp2f(m[r] - base);
+#pragma unroll
+      for (int u = 0; u < kU; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[r][u][e] *= alpha;
+      m[r] = mx;
+      ls[r] = sum;
+    }
+    pk_sum_waves<R, kU, kPo>(ml + 4 * 16 * R * 2, wave, li, lg, o);
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    if (row_w + 16 * r + li >= rows) continue;
+    const int64_t at_row = (int64_t)head[r] * P.tq + token[r];
+    const bool first = lg == 0 && (KS == 1 || wave == 0);
+    if (P.splits > 1) {
+      const int64_t base = (int64_t)split * P.heads * P.tq + at_row;
+      if (first) *reinterpret_cast<f32x2*>(P.part_ml + base * 2) = f32x2{m[r], ls[r]};
+#pragma unroll
+      for (int u = 0; u < kU; ++u)
+        if (KS == 1 || u % 4 == wave) *reinterpret_cast<f32x4*>(P.part_o + base * DP + 16 * u + 4 * lg) = o[r][u];
+      continue;
+    }
+    if (first && P.lse) *reinterpret_cast<f32x2*>(P.lse + at_row * 2) = pk_stats(m[r], ls[r]);
+    const float inv = ls[r] == 0.f ? 0.f : 1.f / ls[r];  // a row without keys is zeros
+    T* out = P.out.p + head[r] * P.out.head + token[r] * P.out.token;
+    T* rest = P.rest.p + head[r] * P.rest.head + token[r] * P.rest.token;
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      if (KS > 1 && u % 4 != wave) continue;
+      const int col = 16 * u + 4 * lg;
+      if (col >= P.d) continue;
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = o[r][u][e] * inv;
+      store4f(out + col, v);
+      if (P.rest.p) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] -= round_to<T>(v[e]);
+        store4f(rest + col, v);
+      }
+    }
+  }
+}
+
+// The splits of a row joined: a workgroup a row, wave w taking every fourth split
+// from w on, lane l holding DP / 64 values (of DP = 32 half the lanes one).
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void packed_join_kernel(PackedParams<T> P) {
+  constexpr int kV = DP > 64 ? DP / 64 : 1;
+  __shared__ float lds_o[4][DP];
+  __shared__ float lds_l[4];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t rows = P.heads * P.tq, at = blockIdx.x;
+  const int64_t token = at % P.tq;
+  const int head = (int)(at / P.tq);
+  // rows of no sequence have no parts
+  if (token >= packed_int(P.q_starts, P.seqs, P.tq) && !P.zero_tail) return;
+  float mx = -INFINITY;
+  for (int s = lane; s < P.splits; s += 64) mx = fmaxf(mx, P.part_ml[(s * rows + at) * 2]);
+#pragma unroll
+  for (int x = 32; x >= 1; x >>= 1) mx = fmaxf(mx, shfl_xor(mx, x));
+  const float base = pk_base(mx);
+  float l = 0.f, o[kV] = {};
+#pragma unroll 8
+  for (int s = wave; s < P.splits; s += 4) {
+    const int64_t i = s * rows + at;
+    const f32x2 v = *reinterpret_cast<const f32x2*>(P.part_ml + i * 2);
+    const float w = __builtin_amdgcn_exp2f(v[0] - base);
+    l = fmaf(v[1], w, l);
+#pragma unroll
+    for (int j = 0; j < kV; ++j)
+      if (64 * j + lane < DP) o[j] = fmaf(P.part_o[i * DP + 64 * j + lane], w, o[j]);
+  }
+  if (lane == 0) lds_l[wave] = l;
+#pragma unroll
+  for (int j = 0; j < kV; ++j)
+    if (64 * j + lane < DP) lds_o[wave][64 * j + lane] = o[j];
+  __syncthreads();
+  if (wave) return;
+  const float sum = (lds_l[0] + lds_l[1]) + (lds_l[2] + lds_l[3]);
+  if (lane == 0 && P.lse) *reinterpret_cast<f32x2*>(P.lse + at * 2) = pk_stats(mx, sum);
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  T* out = P.out.p + head * P.out.head + token * P.out.token;
+  T* rest = P.rest.p + head * P.rest.head + token * P.rest.token;
+#pragma unroll
+  for (int j = 0; j < kV; ++j) {
+    const int x = 64 * j + lane;
+    if (x >= P.d) continue;
+    const float v = ((lds_o[0][x] + lds_o[1][x]) + (lds_o[2][x] + lds_o[3][x])) * inv;
+    out[x] = from_f32<T>(v);
+    if (P.rest.p) rest[x] = from_f32<T>(v - round_to<T>(v));
+  }
+}
+
+template <typename T, int DP>
+void fwd(const PackedParams<T>& P, const PackedForm& form, hipStream_t st) {
+  const unsigned blocks = (unsigned)((int64_t)form.count * (P.heads / P.group));
+  if (form.keywise) {
+    packed_fwd_kernel<T, DP, 4, 1><<<blocks, 256, 0, st>>>(P);
+    if (P.splits > 1) packed_join_kernel<T, DP><<<(unsigned)(P.heads * P.tq), 256, 0, st>>>(P);
+  } else if (form.tiles == 2) {
+    if constexpr (sizeof(T) == 2) packed_fwd_kernel<T, DP, 1, 2><<<blocks, 256, 0, st>>>(P);
+  } else {
+    packed_fwd_kernel<T, DP, 1, 1><<<blocks, 256, 0, st>>>(P);
+  }
+}
+
+}  // namespace
+
+template <typename T>
+void launch_packed_fwd(const PackedParams<T>& P, const PackedForm& form, hipStream_t st) {
+  if (P.d <= 32)
+    fwd<T, 32>(P, form, st);
+  else if (P.d <= 64)
+    fwd<T, 64>(P, form, st);
+  else
+    fwd<T, 128>(P, form, st);
+}
+template void launch_packed_fwd<bf16>(const PackedParams<bf16>&, const PackedForm&, hipStream_t);
+template void launch_packed_fwd<float>(const PackedParams<float>&, const PackedForm&, hipStream_t);
+
+}  // namespace fjx

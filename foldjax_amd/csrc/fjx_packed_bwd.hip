@@ -1,0 +1,505 @@
+// Packed attention, backward. With dP = dO v^T and D = rowsum(dO out):
+//   dS = P (dP - D),  dq = scale dS k,  dk = scale dS^T q,  dv = P^T dO
+// The weights come again from the scores and the forward pass's row statistics, the
+// maximum M and log2 of the sum l, kept apart: P = 2^((s scale log2(e) - M) - log2 l).
+// Every sum has one owner and one order: no atomics, and the same bits each time. So
+// dq and the keys' gradients are two walks with the scores and dP taken twice, seven
+// products in place of five.
+//
+// dS's rows sum to zero. Where one key has nearly all of a row's weight dP - D is what
+// the others have left of it, and D must be known to more bits than a bf16 output has:
+// it is taken from the output and what its rounding left (17 bits; the forward pass
+// applies rounded weights, but in D they are off in proportion to dS itself). Weights
+// and dS enter their products rounded once to bf16, each relative to itself.
+#include "fjx_packed.hpp"
+
+namespace fjx {
+
+namespace {
+
+constexpr float kFar = 16777216.f;  // as in the forward pass
+
+// a weight's exponent from its score's sum s: by = 1 for scores that were multiplied
+__device__ __forceinline__ float pk_weight(float s, float by, float m, float log_sum) {
+  return __builtin_amdgcn_exp2f(fmaf(s, by, -m) - log_sum);
+}
+
+// dq, and D for the other kernel: rows and blocks as in the forward pass.
+template <typename T, int DP, int KS, int R>
+__global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1)) void packed_dq_kernel(PackedParams<T> P) {
+  typedef PkForm<KS> Form;
+  typedef PkRows<T, DP> Rows;
+  typedef typename Frag<T>::type F;
+  constexpr int kC = Rows::kC, kU = Rows::kU;
+  constexpr int kNt = Form::kBlock / KS / 16;
+  constexpr int kTileRows = 16 * R * (KS == 1 ? 4 : 1), kShift = __builtin_ctz(kTileRows);
+  constexpr int kOperand = Form::kStage * Rows::kRowBytes;
+  constexpr int kSets = KS == 1 ? 1 : 4;
+  constexpr int kStages = 4 * kOperand * kSets <= 160 * 1024 ? 2 : 1;
+  constexpr int kPo = DP + 2;
+  static_assert(KS == 1 || kStages * 2 * kOperand * kSets >= 4 * 16 * R * kPo * 4, "the waves' sums");
+  __shared__ __attribute__((aligned(16))) unsigned char raw[kStages * 2 * kOperand * kSets];
+
+  const int t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int kvh = P.heads / P.group;
+  const int kv = blockIdx.x % kvh;
+  const int tile_id = P.tiles - 1 - (int)(blockIdx.x / kvh);
+  PackedSpan sp;
+  if (!packed_span(P, false, P.group, kShift, tile_id, lane, sp)) return;
+  const int rows = sp.nq * P.group;
+  const int row0 = sp.tile * kTileRows;
+  if (row0 >= rows) return;
+  const int row_w = row0 + (KS == 1 ? 16 * R * wave : 0);
+
+  int head[R], token[R], lim[R];
+  F qf[R][kC], dof[R][kC];
+  float m[R], log_sum[R], delta[R];
+  bool any_far = false;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int row = row_w + 16 * r + li < rows ? row_w + 16 * r + li : rows - 1;
+    const int qi = row / P.group;
+    head[r] = kv * P.group + row - qi * P.group;
+    token[r] = sp.q0 + qi;
+    lim[r] = P.causal ? qi + sp.nk - sp.nq + 1 : sp.nk;
+    const T* q = P.q.p + head[r] * P.q.head + token[r] * P.q.token + 8 * lg;
+    const T* dout = P.dout.p + head[r] * P.dout.head + token[r] * P.dout.token + 8 * lg;
+    const T* o = P.o.p + head[r] * P.o.head + token[r] * P.o.token + 8 * lg;
+    const T* rest = P.o_rest.p + head[r] * P.o_rest.head + token[r] * P.o_rest.token + 8 * lg;
+    float d = 0.f;
+#pragma unroll
+    for (int c = 0; c < kC; ++c) {
+      qf[r][c] = dof[r][c] = F{};
+      if (32 * c + 8 * lg >= P.d) continue;
+      qf[r][c] = load8(q + 32 * c);
+      dof[r][c] = load8(dout + 32 * c);
+      float x[8], y[8];
+      to_f32x8(dof[r][c], x);
+      to_f32x8(load8(o + 32 * c), y);
+      if (P.o_rest.p) {
+        float z[8];
+        to_f32x8(load8(rest + 32 * c), z);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] += z[e];
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) d = fmaf(x[e], y[e], d);
+    }
+    delta[r] = group_sum(d);
+    const int64_t at_row = (int64_t)head[r] * P.tq + token[r];
+    const f32x2 stats = *reinterpret_cast<const f32x2*>(P.lse + at_row * 2);
+    m[r] = stats[0];
+    log_sum[r] = stats[1];
+    any_far = any_far || fabsf(m[r]) > kFar;
+    if (lg == 0 && (KS == 1 || wave == 0) && row_w + 16 * r + li < rows) P.delta[at_row] = delta[r];
+  }
+  const bool far = __builtin_amdgcn_ballot_w64(any_far);
+  const int last = (row0 + kTileRows < rows ? row0 + kTileRows : rows) - 1;
+  const int most = P.causal ? last / P.group + sp.nk - sp.nq + 1 : sp.nk;
+  const int lim_lo = __builtin_amdgcn_readfirstlane(lim[0]);
+  const int lim_hi = row_w < rows ? __builtin_amdgcn_readlane(lim[R - 1], 15) : 0;
+  const int blocks = most > 0 ? (int)(((int64_t)most + Form::kBlock - 1) / Form::kBlock) : 0;
+
+  unsigned char* const mine = raw + (KS == 1 ? 0 : wave * kStages * 2 * kOperand);
+  const int stager = KS == 1 ? wave : 0;
+  const int key_w = KS == 1 ? 0 : 32 * wave;
+  PkCopy<T, DP, Form::kStage, Form::kOwners> kcopy, vcopy;
+  kcopy.init(P.k.token, P.d, stager, lane);
+  vcopy.init(P.v.token, P.d, stager, lane);
+  const T* ks = P.k.p + kv * P.k.head + (int64_t)sp.k0 * P.k.token;
+  const T* vs = P.v.p + kv * P.v.head + (int64_t)sp.k0 * P.v.token;
+  auto stage = [&](int blk, int at) {
+    unsigned char* s = mine + at * 2 * kOperand;
+    kcopy.issue(ks, (int64_t)blk * Form::kBlock + key_w, sp.nk, P.d, s, stager);
+    vcopy.issue(vs, (int64_t)blk * Form::kBlock + key_w, sp.nk, P.d, s + kOperand, stager);
+  };
+  PkLane<T, DP> at;
+  at.init(lane);
+  f32x4 dq[R][kU];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int u = 0; u < kU; ++u) dq[r][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  if (kStages == 2) {
+    if (blocks) stage(0, 0);
+    pk_sync<KS>();
+  }
+  for (int blk = 0; blk < blocks; ++blk) {
+    const int cur = kStages == 2 ? blk & 1 : 0;
+    if (kStages == 1) {
+      stage(blk, 0);
+      pk_sync<KS>();
+    } else if (blk + 1 < blocks) {
+      stage(blk + 1, cur ^ 1);
+    }
+    const unsigned char* kt_ = mine + cur * 2 * kOperand;
+    const unsigned char* vt_ = kt_ + kOperand;
+    const int key0 = blk * Form::kBlock + key_w;
+    if (key0 < lim_hi) {
+      const bool masked = key0 + 16 * kNt > lim_lo;
+#pragma unroll
+      for (int pair = 0; pair < kNt / 2; ++pair) {
+        f32x4 s[R][2], dp[R][2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+          for (int r = 0; r < R; ++r) s[r][j] = dp[r][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < kC; ++c) {
+            const F kf = at.at_row(kt_, 32 * pair + 16 * j, c);
+#pragma unroll
+            for (int r = 0; r < R; ++r) mma(s[r][j], kf, qf[r][c]);
+          }
+#pragma unroll
+          for (int c = 0; c < kC; ++c) {
+            const F vf = at.at_row(vt_, 32 * pair + 16 * j, c);
+#pragma unroll
+            for (int r = 0; r < R; ++r) mma(dp[r][j], vf, dof[r][c]);
+          }
+        }
+        float by = P.scale_log2;
+        if (far) {
+          by = 1.f;
+#pragma unroll
+          for (int r = 0; r < R; ++r) pk_round(P.scale_log2, s[r]);
+        }
+        if (masked) {
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            const int left = lim[r] - key0 - 32 * pair - 4 * lg;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[r][j][e] = 16 * j + e < left ? s[r][j][e] : -INFINITY;
+          }
+        }
+        F dsf[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          float ds[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            ds[e] = pk_weight(s[r][e >> 2][e & 3], by, m[r], log_sum[r]) * (dp[r][e >> 2][e & 3] - delta[r]);
+          dsf[r] = pack8<T>(ds);
+        }
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+          const F kf = at.at_col(kt_, 32 * pair, u);
+#pragma unroll
+          for (int r = 0; r < R; ++r) mma(dq[r][u], kf, dsf[r]);
+        }
+      }
+    }
+    pk_sync<KS>();
+  }
+  if constexpr (KS > 1) pk_sum_waves<R, kU, kPo>(reinterpret_cast<float*>(raw), wave, li, lg, dq);
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    if (row_w + 16 * r + li >= rows) continue;
+    T* out = P.dq.p + head[r] * P.dq.head + token[r] * P.dq.token;
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const int col = 16 * u + 4 * lg;
+      if ((KS > 1 && u % 4 != wave) || col >= P.d) continue;
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = dq[r][u][e] * P.scale;
+      store4f(out + col, v);
+    }
+  }
+}
+
+// dk and dv: a wave holds R tiles of 16 keys, lane l key l % 16 of each, and walks the
+// queries of every head that shares them in tiles of 16: S = Q K^T and dP = dO V^T leave
+// the lane 4 queries of its own keys, as the operands of dV^T = dO^T P and dK^T = Q^T dS.
+// KS 1: four waves with keys of their own; 4: the waves share keys and split the queries.
+template <typename T, int DP, int KS, int R>
+__global__ __launch_bounds__(256, (sizeof(T) == 2 && DP * R <= 128 ? 2 : 1)) void packed_dkv_kernel(PackedParams<T> P) {
+  typedef PkForm<KS> Form;
+  typedef PkRows<T, DP> Rows;
+  typedef typename Frag<T>::type F;
+  constexpr int kC = Rows::kC, kU = Rows::kU;
+  constexpr int kNt = Form::kBlock / KS / 16;  // query tiles of a wave in a block
+  constexpr int kTileKeys = 16 * R * (KS == 1 ? 4 : 1), kShift = __builtin_ctz(kTileKeys);
+  constexpr int kOperand = Form::kStage * Rows::kRowBytes;
+  constexpr int kSets = KS == 1 ? 1 : 4;
+  constexpr int kStages = 4 * kOperand * kSets <= 156 * 1024 ? 2 : 1;
+  constexpr int kPo = DP + 2;
+  static_assert(KS == 1 || kStages * 2 * kOperand * kSets >= 4 * 16 * R * kPo * 4, "the waves' sums");
+  __shared__ __attribute__((aligned(16))) unsigned char raw[kStages * 2 * kOperand * kSets];
+  __shared__ __attribute__((aligned(16))) float rowstat[kSets][kStages][3][Form::kStage];  // M, log2 of the sum, D
+  __shared__ int rowfar[kSets][kStages];
+
+  const int t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int kvh = P.heads / P.group;
+  const int kv = blockIdx.x % kvh;
+  const uint32_t rest_id = blockIdx.x / kvh;
+  const int split = rest_id / (uint32_t)P.tiles;
+  PackedSpan sp;
+  if (!packed_span(P, true, 1, kShift, (int)(rest_id % (uint32_t)P.tiles), lane, sp)) return;
+  const int key0 = sp.tile * kTileKeys;
+  if (key0 >= sp.cap) return;
+  const int key_w = key0 + (KS == 1 ? 16 * R * wave : 0);
+  const int shift = sp.nq - sp.nk;  // a causal row i sees the keys up to i - shift
+
+  F kf[R][kC], vf[R][kC];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int key = key_w + 16 * r + li;
+    const int64_t token = (int64_t)sp.k0 + key;
+    const T* k = P.k.p + kv * P.k.head + token * P.k.token + 8 * lg;
+    const T* v = P.v.p + kv * P.v.head + token * P.v.token + 8 * lg;
+#pragma unroll
+    for (int c = 0; c < kC; ++c) {
+      const bool in = key < sp.nk && 32 * c + 8 * lg < P.d;
+      kf[r][c] = in ? load8(k + 32 * c) : F{};
+      vf[r][c] = in ? load8(v + 32 * c) : F{};
+    }
+  }
+  // the heads of this part, and the query blocks in which any row sees the first key
+  const int h0 = P.group * split / P.splits, h1 = P.group * (split + 1) / P.splits;
+  const int q_first = P.causal && key0 + shift > 0 ? key0 + shift : 0;
+  const int qb0 = q_first / Form::kBlock;
+  const int qb1 = key0 < sp.nk ? (int)(((int64_t)sp.nq + Form::kBlock - 1) / Form::kBlock) : 0;
+  const int turns = qb1 > qb0 ? (h1 - h0) * (qb1 - qb0) : 0;
+
+  const int set = KS == 1 ? 0 : wave, stager = KS == 1 ? wave : 0;
+  unsigned char* const mine = raw + set * kStages * 2 * kOperand;
+  const int q_w = KS == 1 ? 0 : 32 * wave;
+  PkCopy<T, DP, Form::kStage, Form::kOwners> qcopy, ocopy;
+  qcopy.init(P.q.token, P.d, stager, lane);
+  ocopy.init(P.dout.token, P.d, stager, lane);
+  int next_h = h0, next_b = qb0;  // of the next block to stage
+  f32x2 st_m = {0.f, INFINITY};
+  float st_d = 0.f;
+  auto stage = [&](int at) {
+    const int head = kv * P.group + next_h;
+    const int64_t row0 = (int64_t)next_b * Form::kBlock + q_w;
+    unsigned char* s = mine + at * 2 * kOperand;
+    qcopy.issue(P.q.p + head * P.q.head + (int64_t)sp.q0 * P.q.token, row0, sp.nq, P.d, s, stager);
+    ocopy.issue(P.dout.p + head * P.dout.head + (int64_t)sp.q0 * P.dout.token, row0, sp.nq, P.d, s + kOperand, stager);
+    st_m = f32x2{0.f, INFINITY};  // rows past the last: weights of zero
+    st_d = 0.f;
+    const int r = KS == 1 ? t : lane;
+    if (r < Form::kStage && row0 + r < sp.nq) {
+      const int64_t at_row = (int64_t)head * P.tq + sp.q0 + row0 + r;
+      st_m = *reinterpret_cast<const f32x2*>(P.lse + at_row * 2);
+      st_d = P.delta[at_row];
+    }
+    if (++next_b == qb1) {
+      next_b = qb0;
+      ++next_h;
+    }
+  };
+  auto put_stats = [&](int at) {
+    const int r = KS == 1 ? t : lane;
+    if (r < Form::kStage) {
+      rowstat[set][at][0][r] = st_m[0];
+      rowstat[set][at][1][r] = st_m[1];
+      rowstat[set][at][2][r] = st_d;
+      const bool far = __builtin_amdgcn_ballot_w64(fabsf(st_m[0]) > kFar);
+      if (r == 0) rowfar[set][at] = far;
+    }
+  };
+  PkLane<T, DP> at;
+  at.init(lane);
+  f32x4 dk[R][kU], dv[R][kU];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int u = 0; u < kU; ++u) dk[r][u] = dv[r][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  if (kStages == 2) {
+    if (turns) {
+      stage(0);
+      put_stats(0);
+    }
+    pk_sync<KS>();
+  }
+  int qb = qb0;
+  for (int turn = 0; turn < turns; ++turn) {
+    const int cur = kStages == 2 ? turn & 1 : 0;
+    if (kStages == 1) {
+      stage(0);
+      put_stats(0);
+      pk_sync<KS>();
+    } else if (turn + 1 < turns) {
+      stage(cur ^ 1);
+    }
+    const unsigned char* qt_ = mine + cur * 2 * kOperand;
+    const unsigned char* ot_ = qt_ + kOperand;
+    const int row0 = qb * Form::kBlock + q_w;
+    // rows from key + shift on see a key
+    if (!P.causal || row0 + 16 * kNt > key_w + shift) {
+      const bool masked = P.causal && row0 < key_w + 16 * R - 1 + shift;
+      const bool far = __builtin_amdgcn_readfirstlane(rowfar[set][cur]);
+#pragma unroll
+      for (int pair = 0; pair < kNt / 2; ++pair) {
+        f32x4 s[R][2], dp[R][2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+          for (int r = 0; r < R; ++r) s[r][j] = dp[r][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < kC; ++c) {
+            const F qf = at.at_row(qt_, 32 * pair + 16 * j, c);
+#pragma unroll
+            for (int r = 0; r < R; ++r) mma(s[r][j], qf, kf[r][c]);
+          }
+#pragma unroll
+          for (int c = 0; c < kC; ++c) {
+            const F of = at.at_row(ot_, 32 * pair + 16 * j, c);
+#pragma unroll
+            for (int r = 0; r < R; ++r) mma(dp[r][j], of, vf[r][c]);
+          }
+        }
+        float by = P.scale_log2;
+        if (far) {
+          by = 1.f;
+#pragma unroll
+          for (int r = 0; r < R; ++r) pk_round(P.scale_log2, s[r]);
+        }
+        if (masked) {
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            const int from = key_w + 16 * r + li + shift - row0 - 32 * pair - 4 * lg;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[r][j][e] = 16 * j + e >= from ? s[r][j][e] : -INFINITY;
+          }
+        }
+        F pf[R], dsf[R];
+        float p[R][8], ds[R][8];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int row = 32 * pair + 16 * j + 4 * lg;
+          const f32x4 m4 = *reinterpret_cast<const f32x4*>(&rowstat[set][cur][0][row]);
+          const f32x4 l4 = *reinterpret_cast<const f32x4*>(&rowstat[set][cur][1][row]);
+          const f32x4 d4 = *reinterpret_cast<const f32x4*>(&rowstat[set][cur][2][row]);
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              p[r][4 * j + e] = pk_weight(s[r][j][e], by, m4[e], l4[e]);
+              ds[r][4 * j + e] = p[r][4 * j + e] * (dp[r][j][e] - d4[e]);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          pf[r] = pack8<T>(p[r]);
+          dsf[r] = pack8<T>(ds[r]);
+        }
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+          const F of = at.at_col(ot_, 32 * pair, u);
+#pragma unroll
+          for (int r = 0; r < R; ++r) mma(dv[r][u], of, pf[r]);
+          const F qf = at.at_col(qt_, 32 * pair, u);
+#pragma unroll
+          for (int r = 0; r < R; ++r) mma(dk[r][u], qf, dsf[r]);
+        }
+      }
+    }
+    if (++qb == qb1) qb = qb0;
+    if (kStages == 2 && turn + 1 < turns) put_stats(cur ^ 1);
+    pk_sync<KS>();
+  }
+  if constexpr (KS > 1) {
+    pk_sum_waves<R, kU, kPo>(reinterpret_cast<float*>(raw), wave, li, lg, dk);
+    pk_sum_waves<R, kU, kPo>(reinterpret_cast<float*>(raw), wave, li, lg, dv);
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int key = key_w + 16 * r + li;
+    if (key >= sp.cap) continue;
+    const bool real = key < sp.nk;  // the others' gradients are zeros
+    const int64_t token = (int64_t)sp.k0 + key;
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const int col = 16 * u + 4 * lg;
+      if (KS > 1 && u % 4 != wave) continue;
+      if (P.splits > 1) {
+        const int64_t at_key = (((int64_t)split * kvh + kv) * P.tk + token) * DP + col;
+        *reinterpret_cast<f32x4*>(P.part_dk + at_key) = real ? dk[r][u] : f32x4{0.f, 0.f, 0.f, 0.f};
+        *reinterpret_cast<f32x4*>(P.part_dv + at_key) = real ? dv[r][u] : f32x4{0.f, 0.f, 0.f, 0.f};
+        continue;
+      }
+      if (col >= P.d) continue;
+      float a[4], b[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        a[e] = real ? dk[r][u][e] * P.scale : 0.f;
+        b[e] = real ? dv[r][u][e] : 0.f;
+      }
+      store4f(P.dk.p + kv * P.dk.head + token * P.dk.token + col, a);
+      store4f(P.dv.p + kv * P.dv.head + token * P.dv.token + col, b);
+    }
+  }
+}
+
+// The parts of dk and dv (a part has some of the heads that share them) added: 4
+// elements a thread.
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void packed_dkv_join_kernel(PackedParams<T> P) {
+  const int kvh = P.heads / P.group;
+  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, all = (int64_t)kvh * P.tk * DP;
+  if (at >= all || at % DP >= P.d) return;
+  f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
+  for (int s = 0; s < P.splits; ++s) {
+    a += *reinterpret_cast<const f32x4*>(P.part_dk + s * all + at);
+    b += *reinterpret_cast<const f32x4*>(P.part_dv + s * all + at);
+  }
+  const int64_t row = at / DP, token = row % P.tk, kv = row / P.tk, col = at % DP;
+  const float x[4] = {a[0] * P.scale, a[1] * P.scale, a[2] * P.scale, a[3] * P.scale}, y[4] = {b[0], b[1], b[2], b[3]};
+  store4f(P.dk.p + kv * P.dk.head + token * P.dk.token + col, x);
+  store4f(P.dv.p + kv * P.dv.head + token * P.dv.token + col, y);
+}
+
+template <typename T, int DP>
+void bwd(PackedParams<T> P, const PackedForm& rows, const PackedForm& keys, hipStream_t st) {
+  const int kvh = P.heads / P.group;
+  const int splits = P.splits;
+  P.splits = 1;
+  P.tiles = rows.count;
+  if (rows.count) {
+    const unsigned blocks = (unsigned)((int64_t)rows.count * kvh);
+    if (rows.keywise)
+      packed_dq_kernel<T, DP, 4, 1><<<blocks, 256, 0, st>>>(P);
+    else if (rows.tiles == 2) {
+      if constexpr (sizeof(T) == 2) packed_dq_kernel<T, DP, 1, 2><<<blocks, 256, 0, st>>>(P);
+    } else
+      packed_dq_kernel<T, DP, 1, 1><<<blocks, 256, 0, st>>>(P);
+  }
+  if (!keys.count) return;
+  P.splits = splits;
+  P.tiles = keys.count;
+  const unsigned blocks = (unsigned)((int64_t)keys.count * kvh * splits);
+  if (keys.keywise)
+    packed_dkv_kernel<T, DP, 4, 1><<<blocks, 256, 0, st>>>(P);
+  else if (keys.tiles == 2) {
+    if constexpr (sizeof(T) == 2) packed_dkv_kernel<T, DP, 1, 2><<<blocks, 256, 0, st>>>(P);
+  } else
+    packed_dkv_kernel<T, DP, 1, 1><<<blocks, 256, 0, st>>>(P);
+  if (splits > 1)
+    packed_dkv_join_kernel<T, DP><<<(unsigned)(((int64_t)kvh * P.tk * DP / 4 + 255) / 256), 256, 0, st>>>(P);
+}
+
+}  // namespace
+
+template <typename T>
+void launch_packed_bwd(const PackedParams<T>& P, const PackedForm& rows, const PackedForm& keys, hipStream_t st) {
+  if (P.d <= 32)
+    bwd<T, 32>(P, rows, keys, st);
+  else if (P.d <= 64)
+    bwd<T, 64>(P, rows, keys, st);
+  else
+    bwd<T, 128>(P, rows, keys, st);
+}
+template void launch_packed_bwd<bf16>(const PackedParams<bf16>&, const PackedForm&, const PackedForm&, hipStream_t);
+template void launch_packed_bwd<float>(const PackedParams<float>&, const PackedForm&, const PackedForm&, hipStream_t);
+
+}  // namespace fjx

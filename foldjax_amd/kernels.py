@@ -934,6 +934,419 @@ def diff_attention_backward(
     return dq, dk, dv, dbias, dlam
 
 
+_INDEX = {torch.int32: _lib.FJX_INDEX_I32, torch.int64: _lib.FJX_INDEX_I64}
+
+
+def _packed_rows(t: torch.Tensor, unit: int):
+    """Strides {head, token} of [heads, tokens, width] where the kernels can take
+    its rows as they lie, None where not."""
+    st = _head_rows(t, unit)
+    if st is None or (t.shape[1] > 1 and not t.shape[2] <= st[2] < (1 << 24) // t.element_size()):
+        return None
+    return st[1], st[2]
+
+
+def _packed_heads(t: torch.Tensor, unit: int):
+    """``t`` and its strides, a copy where its rows cannot be taken as they lie."""
+    st = _packed_rows(t, unit)
+    if st is None:
+        t = t.clone(memory_format=torch.contiguous_format)
+        st = _packed_rows(t, unit)
+    return t, st
+
+
+def _token_major(heads: int, tokens: int, width: int, like: torch.Tensor) -> torch.Tensor:
+    """A new [heads, tokens, width] whose memory has a token's heads side by side,
+    as the projections before and behind an attention have them."""
+    return torch.empty_strided((heads, tokens, width), (width, heads * width, 1), dtype=like.dtype, device=like.device)
+
+
+def _packed_attention_args(q, k, v, q_starts, scale, causal, k_starts, k_lengths):
+    """The checked argument block that both directions share, the tensors it points
+    to, the elements of a 16-byte piece, and (its key, the forward call's workspace)."""
+    scale, causal = float(scale), bool(causal)
+    key = (_layout(q, k, v, q_starts, k_starts, k_lengths), scale, causal)
+    seen = _BLOCKS.get(key)
+    if seen is not None:
+        block, unit, nbytes = seen
+        a = _lib.PackedAttentionArgs.from_buffer_copy(block)
+        a.q, a.k, a.v = qp, kp, vp = q.data_ptr(), k.data_ptr(), v.data_ptr()
+        if not (qp | kp | vp) & 15:
+            a.q_starts = q_starts.data_ptr()
+            a.k_starts = a.q_starts if k_starts is None else k_starts.data_ptr()
+            if k_lengths is not None:
+                a.k_lengths = k_lengths.data_ptr()
+            return a, (q, k, v, q_starts, k_starts, k_lengths), unit, (key, nbytes)
+    dtype = q.dtype
+    code = _code(dtype)
+    _same_place(q, dtype, k=k, v=v)
+    _same_device(q, q_starts=q_starts, k_starts=k_starts, k_lengths=k_lengths)
+    qs, ks = q.shape, k.shape
+    if len(qs) != 3 or len(ks) != 3:
+        raise ValueError(f"q, k and v must be [heads, tokens, width], got {tuple(qs)}, {tuple(ks)}, {tuple(v.shape)}")
+    heads, tq, d = qs
+    kv_heads, tk = ks[:2]
+    _need_shape("k", k, (kv_heads, tk, d))
+    _need_shape("v", v, (kv_heads, tk, d))
+    if d % 8 or not 8 <= d <= 128:
+        raise ValueError(f"q, k and v must have a width (head_dim) that is a multiple of 8 up to 128, got {d}")
+    if not kv_heads or heads % kv_heads:
+        raise ValueError(f"q's heads must be a multiple of k's, got {heads} and {kv_heads}")
+    if q_starts.dim() != 1 or q_starts.shape[0] < 2:
+        raise ValueError(f"q_starts must hold an offset more than there are sequences, one at least, got {tuple(q_starts.shape)}")
+    seqs = q_starts.shape[0] - 1
+    if k_starts is None:
+        if tk != tq:
+            raise ValueError(f"k_starts must be given where k has other tokens than q, got {tk} and {tq}")
+    else:
+        _need_shape("k_starts", k_starts, (seqs + 1,))
+    _need_shape("k_lengths", k_lengths, (seqs,))
+    index = _INDEX.get(q_starts.dtype)
+    if index is None:
+        raise ValueError(f"q_starts must be int32 or int64, got {q_starts.dtype}")
+    for name, t in (("k_starts", k_starts), ("k_lengths", k_lengths)):
+        if t is not None and t.dtype not in _INDEX:
+            raise ValueError(f"{name} must be int32 or int64, got {t.dtype}")
+    _dev(q)
+    given = (q, k, v, q_starts, k_starts, k_lengths)
+    q_starts, k_starts, k_lengths = (_like(t, q_starts.dtype) for t in (q_starts, k_starts, k_lengths))
+    unit = 4 if dtype is torch.float32 else 8
+    q, qst = _packed_heads(q, unit)
+    k, kst = _packed_heads(k, unit)
+    v, vst = _packed_heads(v, unit)
+    a = _lib.PackedAttentionArgs(
+        tq, tk, seqs, heads, kv_heads, d, code, index, causal, 0, scale, q.data_ptr(), k.data_ptr(), v.data_ptr(), None,
+        qst, kst, vst, (d, heads * d), q_starts.data_ptr(), (q_starts if k_starts is None else k_starts).data_ptr(),
+        _ptr(k_lengths), None, None, (d, heads * d))
+    kept = (q, k, v, q_starts, k_starts, k_lengths)
+    nbytes = _lib.load().fjx_packed_attention_workspace_size(tq, tk, seqs, heads, kv_heads, d, code)
+    as_they_lie = all(x is y for x, y in zip(kept, given))
+    if as_they_lie:
+        _remember(key, (bytes(a), unit, nbytes))
+    return a, kept, unit, (key if as_they_lie else None, nbytes)
+
+
+def packed_attention(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    q_starts: torch.Tensor,
+    *,
+    scale: float,
+    causal: bool = False,
+    k_starts: torch.Tensor | None = None,
+    k_lengths: torch.Tensor | None = None,
+    return_lse: bool = False,
+    out: torch.Tensor | None = None,
+):
+    """Attention over sequences of different lengths packed one behind the other
+    (``fjx_packed_attention_fwd``): ``softmax(scale q k^T) v`` within each.
+
+    q ``[H, Tq, D]``, k and v ``[Hk, Tk, D]`` (Hk divides H: heads may share keys
+    and values), D a multiple of 8 up to 128; any strides whose rows are whole
+    16-byte pieces are taken as they lie, others are copied. Sequence s has the
+    queries ``q_starts[s] .. q_starts[s + 1] - 1`` and, of k and v, the tokens
+    ``k_starts[s] .. k_starts[s + 1] - 1`` (left out: those of its queries), with
+    ``k_lengths`` only the first ``k_lengths[s]`` of them: a cache with room for
+    more, whose unused places may hold anything. The offsets are int32 or int64
+    device tensors, from 0 on and not descending; they are read on the device, so
+    that a captured call takes new lengths at each replay. ``causal``: query i of
+    nq sees key j of nk where ``j <= i + nk - nq``: each token those before it, new
+    tokens their cache. A row without keys is zeros. k and v are finite. ``scale``
+    in [1e-30, 1e30].
+
+    Returns ``out`` ``[H, Tq, D]``, a token's heads side by side in memory; rows
+    behind the last sequence are zeros. With ``return_lse`` ``(out, lse, rest)``,
+    the latter two for ``packed_attention_backward``: what it needs to know of the
+    rows, and what the rounding of a bfloat16 output left (None of float32).
+    ``out``: write into this tensor (its rows whole 16-byte pieces), which overlaps
+    no input; its rows behind the last sequence are left as they are."""
+    a, kept, unit, (_, nbytes) = _packed_attention_args(q, k, v, q_starts, scale, causal, k_starts, k_lengths)
+    if out is None:
+        out = _token_major(a.heads, a.tokens_q, a.head_dim, q)
+        a.zero_tail = 1
+    else:
+        if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
+            raise ValueError(f"out must be a {q.dtype} tensor of shape {tuple(q.shape)} on {q.device}, "
+                             f"got {out.dtype} {tuple(out.shape)} on {out.device}")
+        if a.tokens_q and out.data_ptr() in (q.data_ptr(), k.data_ptr(), v.data_ptr()):
+            raise ValueError("out must not be q, k or v: other rows' results are taken from them")
+        strides = _packed_rows(out, unit)
+        if strides is None:
+            raise ValueError("out must have rows of whole 16-byte pieces that do not overlap")
+        a.out_strides = strides
+    a.out = out.data_ptr()
+    lse = rest = None
+    if return_lse:
+        lse = torch.empty((a.heads, a.tokens_q, 2), dtype=torch.float32, device=q.device)
+        a.lse = lse.data_ptr()
+        if q.dtype is torch.bfloat16:
+            rest = _token_major(a.heads, a.tokens_q, a.head_dim, q)
+            a.rest = rest.data_ptr()
+    if nbytes:
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
+    _launch(_lib.load().fjx_packed_attention_fwd, a, q)
+    return (out, lse, rest) if return_lse else out
+
+
+def packed_attention_backward(
+    dout: torch.Tensor,
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    out: torch.Tensor,
+    lse: torch.Tensor,
+    rest: torch.Tensor | None,
+    q_starts: torch.Tensor,
+    *,
+    scale: float,
+    causal: bool = False,
+    k_starts: torch.Tensor | None = None,
+    k_lengths: torch.Tensor | None = None,
+):
+    """Gradients of ``packed_attention`` (``fjx_packed_attention_bwd``) at the same
+    arguments; ``out``, ``lse`` and ``rest`` are what the forward call returned.
+    Returns ``(dq, dk, dv)`` in the dtype and shape of q, k and v, a token's heads
+    side by side in memory; gradients of shared heads are summed over the query
+    heads, those of tokens of no sequence and of a cache's unused places are zeros.
+    The same bits each time. Without ``rest`` bfloat16 gradients of rows in which
+    one key has nearly all the weight lose digits."""
+    a, kept, unit, (key, _) = _packed_attention_args(q, k, v, q_starts, scale, causal, k_starts, k_lengths)
+    key = None if key is None else (key, _layout(dout, out, lse, rest))
+    seen = None if key is None else _BLOCKS.get(key)
+    if seen is not None and not (dout.data_ptr() | out.data_ptr() | (0 if rest is None else rest.data_ptr())) & 15:
+        block, nbytes = seen
+        g = _lib.PackedAttentionBwdArgs.from_buffer_copy(block)
+        a.out_strides, a.rest_strides = g.fwd.out_strides, g.fwd.rest_strides
+    else:
+        _same_place(q, q.dtype, dout=dout, out=out, rest=rest)
+        _same_place(q, torch.float32, lse=lse)
+        _need_shape("dout", dout, q.shape)
+        _need_shape("out", out, q.shape)
+        _need_shape("rest", rest, q.shape)
+        _need_shape("lse", lse, (a.heads, a.tokens_q, 2))
+        if rest is not None and q.dtype is not torch.bfloat16:
+            raise ValueError("rest is of bfloat16 outputs")
+        given = dout, out, lse, rest
+        lse = lse.contiguous()
+        dout, dst = _packed_heads(dout, unit)
+        out, a.out_strides = _packed_heads(out, unit)
+        if rest is not None:
+            rest, a.rest_strides = _packed_heads(rest, unit)
+        by_q, by_k = (a.head_dim, a.heads * a.head_dim), (a.head_dim, a.kv_heads * a.head_dim)
+        g = _lib.PackedAttentionBwdArgs(a, None, None, None, None, dst, by_q, by_k, by_k)
+        nbytes = _lib.load().fjx_packed_attention_bwd_workspace_size(a.tokens_q, a.tokens_k, a.sequences, a.heads, a.kv_heads,
+                                                                     a.head_dim, a.dtype)
+        if key is not None and all(x is y for x, y in zip((dout, out, lse, rest), given)):
+            _remember(key, (bytes(g), nbytes))
+    dq, dk, dv = (_token_major(*t.shape, q) for t in (q, k, v))
+    a.out, a.lse, a.rest = out.data_ptr(), lse.data_ptr(), _ptr(rest)
+    if nbytes:
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
+    g.fwd = a
+    g.dout, g.dq, g.dk, g.dv = dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+    _launch(_lib.load().fjx_packed_attention_bwd, g, q)
+    return dq, dk, dv
+
+
+def _like_heads(t: torch.Tensor) -> torch.Tensor:
+    """A new tensor of ``t``'s shape [..., heads, tokens, width] whose memory has a
+    token's heads side by side."""
+    *lead, heads, tokens, width = t.shape
+    st, step = [width, heads * width, 1], tokens * heads * width
+    for n in reversed(lead):
+        st.insert(0, step)
+        step *= n
+    return torch.empty_strided(t.shape, st, dtype=t.dtype, device=t.device)
+
+
+def _rotary_args(q, k, positions, frequencies, q_weight, k_weight, eps, sections, interleaved):
+    """The checked argument block that both directions share, the tensors it points
+    to, the elements of a 16-byte piece, and its key."""
+    eps, interleaved = float(eps), bool(interleaved)
+    sections = None if sections is None else tuple(int(n) for n in sections)
+    key = (_layout(q, k, positions, frequencies, q_weight, k_weight), eps, sections, interleaved, "rotary")
+    seen = _BLOCKS.get(key)
+    if seen is not None:
+        block, unit = seen
+        a = _lib.HeadNormRotaryArgs.from_buffer_copy(block)
+        a.q, a.positions, a.frequencies = qp, _, _ = q.data_ptr(), positions.data_ptr(), frequencies.data_ptr()
+        for name, t in (("k", k), ("q_weight", q_weight), ("k_weight", k_weight)):
+            if t is not None:
+                p = t.data_ptr()
+                setattr(a, name, p)
+                qp |= p
+        if not qp & 15:
+            return a, (q, k, positions, frequencies, q_weight, k_weight), unit, key
+    dtype, shape = q.dtype, q.shape
+    code = _code(dtype)
+    _same_place(q, dtype, k=k, q_weight=q_weight, k_weight=k_weight)
+    _same_place(q, torch.float64, frequencies=frequencies)
+    _same_device(q, positions=positions)
+    if len(shape) < 3:
+        raise ValueError(f"q must be [..., heads, tokens, width], got {tuple(shape)}")
+    lead, (heads, tokens, d) = tuple(shape[:-3]), shape[-3:]
+    kv_heads = 0
+    if k is not None:
+        kv_heads = k.shape[-3] if k.dim() > 2 else 0
+        _need_shape("k", k, lead + (kv_heads, tokens, d))
+    elif k_weight is not None:
+        raise ValueError("k_weight needs k")
+    _need_shape("q_weight", q_weight, (d,))
+    _need_shape("k_weight", k_weight, (d,))
+    if d % 8 or not 8 <= d <= 256:
+        raise ValueError(f"q and k must have a width (head_dim) that is a multiple of 8 up to 256, got {d}")
+    if frequencies.dim() != 1 or frequencies.shape[0] % 4 or 2 * frequencies.shape[0] > d:
+        raise ValueError(f"frequencies must be a multiple of 4 and at most half of the {d} channels, got {tuple(frequencies.shape)}")
+    pairs = frequencies.shape[0]
+    sections_ = (pairs,) if sections is None else sections
+    if not 1 <= len(sections_) <= 4 or min(sections_) < 0 or sum(sections_) != pairs:
+        raise ValueError(f"sections must be 1 to 4 numbers that add up to the {pairs} frequencies, got {sections}")
+    index = _INDEX.get(positions.dtype)
+    if index is None:
+        raise ValueError(f"positions must be int32 or int64, got {positions.dtype}")
+    axes = len(sections_)
+    shared = positions.dim() == 2
+    _need_shape("positions", positions, (axes, tokens) if shared else (axes, *lead, tokens))
+    _dev(q)
+    given = (q, k, positions, frequencies, q_weight, k_weight)
+    positions, frequencies = positions.contiguous(), frequencies.contiguous()
+    wq, wk = (None if w is None else _aligned(w.contiguous()) for w in (q_weight, k_weight))
+    unit = 4 if dtype is torch.float32 else 8
+    q, qst = _heads(q, unit)
+    k, kst = (None, (0, 0, 0)) if k is None else _heads(k, unit)
+    items = 1
+    for n in lead:
+        items *= n
+    a = _lib.HeadNormRotaryArgs(
+        items, heads, kv_heads, tokens, d, code, index, interleaved, axes, sections_, eps, q.data_ptr(), _ptr(k), _ptr(wq),
+        _ptr(wk), positions.data_ptr(), (positions.stride(0), 0 if shared else tokens), frequencies.data_ptr(), None, None,
+        qst, kst, (tokens * heads * d, d, heads * d), (tokens * kv_heads * d, d, kv_heads * d))
+    kept = (q, k, positions, frequencies, wq, wk)
+    as_they_lie = all(x is y for x, y in zip(kept, given))
+    if as_they_lie:
+        _remember(key, (bytes(a), unit))
+    return a, kept, unit, key if as_they_lie else None
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    return t.clone() if t.data_ptr() & 15 else t
+
+
+def head_norm_rotary(
+    q: torch.Tensor,
+    k: torch.Tensor | None,
+    positions: torch.Tensor,
+    frequencies: torch.Tensor,
+    *,
+    q_weight: torch.Tensor | None = None,
+    k_weight: torch.Tensor | None = None,
+    eps: float = 1e-6,
+    sections: tuple[int, ...] | None = None,
+    interleaved: bool = False,
+    q_out: torch.Tensor | None = None,
+    k_out: torch.Tensor | None = None,
+):
+    """The root-mean-square norm of each head's queries and keys and their rotation
+    by position, in one pass (``fjx_head_norm_rotary_fwd``).
+
+    q ``[..., H, T, D]``, k ``[..., Hk, T, D]`` (or None), D a multiple of 8 up to
+    256; any strides whose rows are whole 16-byte pieces are taken as they lie,
+    others are copied. ``q_weight`` and ``k_weight`` ``[D]``: ``x / sqrt(mean(x^2) +
+    eps) * weight``; None: no norm. ``frequencies`` float64 ``[P]``, in radians a
+    position: pair i, the channels (i, i + P) or with ``interleaved`` (2 i, 2 i + 1),
+    is turned by position times ``frequencies[i]``, an angle that is taken in 64 bits;
+    channels from 2 P on are left (P a multiple of 4, 0 for the norm alone).
+    ``positions`` int32 or int64 ``[A, ..., T]``, or ``[A, T]`` for all items alike:
+    axis a's for the ``sections[a]`` pairs behind those of the axes before it
+    (residue, chain and copy of a token, for instance; up to 4 axes; left out: one).
+
+    Returns ``(q', k')``, a token's heads side by side in memory (k' None without k).
+    ``q_out``, ``k_out``: write into these tensors (of q's and k's shape, their rows
+    whole 16-byte pieces: places in a cache, for one), each of which may be its input."""
+    a, kept, unit, _ = _rotary_args(q, k, positions, frequencies, q_weight, k_weight, eps, sections, interleaved)
+    if q_out is None:
+        q_out = _like_heads(q)
+    else:
+        a.q_out_strides = _rotary_out("q_out", q_out, q, unit)
+    a.q_out = q_out.data_ptr()
+    if k is None:
+        if k_out is not None:
+            raise ValueError("k_out needs k")
+    else:
+        if k_out is None:
+            k_out = _like_heads(k)
+        else:
+            a.k_out_strides = _rotary_out("k_out", k_out, k, unit)
+            if k_out.data_ptr() == a.q_out or (k_out.data_ptr() == a.q and a.q != a.k):
+                raise ValueError("q_out and k_out must be two buffers, neither the other's input")
+        if a.q_out == a.k:
+            raise ValueError("q_out and k_out must be two buffers, neither the other's input")
+        a.k_out = k_out.data_ptr()
+    _launch(_lib.load().fjx_head_norm_rotary_fwd, a, q)
+    return q_out, k_out
+
+
+def _rotary_out(name: str, out: torch.Tensor, x: torch.Tensor, unit: int):
+    if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
+        raise ValueError(f"{name} must be a {x.dtype} tensor of shape {tuple(x.shape)} on {x.device}, "
+                         f"got {out.dtype} {tuple(out.shape)} on {out.device}")
+    strides = _head_rows(out, unit)
+    if strides is None:
+        raise ValueError(f"{name} must have rows of whole 16-byte pieces, and leading axes that fold into one")
+    return strides
+
+
+def head_norm_rotary_backward(
+    dq: torch.Tensor,
+    dk: torch.Tensor | None,
+    q: torch.Tensor,
+    k: torch.Tensor | None,
+    positions: torch.Tensor,
+    frequencies: torch.Tensor,
+    *,
+    q_weight: torch.Tensor | None = None,
+    k_weight: torch.Tensor | None = None,
+    eps: float = 1e-6,
+    sections: tuple[int, ...] | None = None,
+    interleaved: bool = False,
+):
+    """Gradients of ``head_norm_rotary`` (``fjx_head_norm_rotary_bwd``) at the same
+    arguments, dq and dk being those of its outputs (dk None without k). Returns
+    ``(dx_q, dx_k, dq_weight, dk_weight)``: the inputs' in their dtype and shape, a
+    token's heads side by side in memory, the weights' float32 ``[D]``, summed over
+    tokens and heads in one order; None for what is not there."""
+    a, kept, unit, _ = _rotary_args(q, k, positions, frequencies, q_weight, k_weight, eps, sections, interleaved)
+    if (dk is None) != (k is None):
+        raise ValueError("dk must be given where k is, and only there")
+    _same_place(q, q.dtype, dq=dq, dk=dk)
+    _need_shape("dq", dq, q.shape)
+    if k is not None:
+        _need_shape("dk", dk, k.shape)
+    gk, k_strides = None, (0, 0, 0)
+    dq, a.q_out_strides = _heads(dq, unit)
+    a.q_out = dq.data_ptr()
+    if dk is not None:
+        dk, a.k_out_strides = _heads(dk, unit)
+        a.k_out = dk.data_ptr()
+    gq = _like_heads(q)
+    packed = lambda h: (a.tokens * h * a.head_dim, a.head_dim, h * a.head_dim)  # noqa: E731
+    if k is not None:
+        gk, k_strides = _like_heads(k), packed(a.kv_heads)
+    new = lambda w: None if w is None else torch.empty((a.head_dim,), dtype=torch.float32, device=q.device)  # noqa: E731
+    dwq, dwk = new(q_weight), new(k_weight)
+    b = _lib.HeadNormRotaryBwdArgs(a, gq.data_ptr(), _ptr(gk), packed(a.heads), k_strides, _ptr(dwq), _ptr(dwk))
+    lib = _lib.load()
+    if dwq is not None or dwk is not None:
+        nbytes = lib.fjx_head_norm_rotary_bwd_workspace_size(a.items, a.heads, a.kv_heads, a.tokens, a.head_dim)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        b.workspace, b.workspace_bytes = ws.data_ptr(), nbytes
+    _launch(lib.fjx_head_norm_rotary_bwd, b, q)
+    return gq, gk, dwq, dwk
+
+
 _CODES = {None: (_lib.FJX_CODES_NONE, None), "e4m3": (_lib.FJX_CODES_E4M3, torch.float8_e4m3fn),
           "int8": (_lib.FJX_CODES_INT8, torch.int8)}
 

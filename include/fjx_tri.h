@@ -49,7 +49,7 @@
 extern "C" {
 #endif
 
-#define FJX_ABI_VERSION 7
+#define FJX_ABI_VERSION 8
 
 /* element types of activations, masks and weights */
 enum { FJX_DTYPE_F32 = 0, FJX_DTYPE_BF16 = 1 };
@@ -522,6 +522,155 @@ typedef struct fjx_dropout_args {
 } fjx_dropout_args;
 
 int fjx_dropout_fwd(const fjx_dropout_args* args, hipStream_t stream);
+
+/* element types of token offsets and positions */
+enum { FJX_INDEX_I32 = 0, FJX_INDEX_I64 = 1 };
+
+/*
+ * Attention over sequences of different lengths that lie one behind the other,
+ * each against itself or against a cache of its own. Beside fjx_triattn_core and
+ * fjx_diff_attention_fwd, whose items have one length; no counterpart in the
+ * reference.
+ *   out = softmax(scale q k^T) v   over the keys that a row sees
+ * q [heads, tokens_q, head_dim], k and v [kv_heads, tokens_k, head_dim], out as
+ * q; *_strides are {head, token} in elements, the last axis contiguous. Query
+ * heads heads / kv_heads * j and on share key/value head j. Sequence s has the
+ * queries q_starts[s] .. q_starts[s + 1] - 1 and the keys k_starts[s] ..
+ * k_starts[s + 1] - 1, of which only the first k_lengths[s] are there when that
+ * is given (what lies behind them, as in a cache with room, is never looked at).
+ * Offsets are device values, read by the kernels: [sequences + 1] from 0 on, not
+ * descending; offsets that lead out of the buffers are taken as their ends (the
+ * results are then undefined, nothing outside is touched). causal: of nq queries
+ * and nk keys, query i sees key j where j <= i + nk - nq (the last query sees all);
+ * rows without a key are zeros, with zero gradients. k and v of a sequence's keys
+ * are finite. Rows of out behind the last sequence are left as they are, or with
+ * zero_tail written as zeros. `out` overlaps no input.
+ * For the backward pass: lse [heads, tokens_q, 2] fp32, and `rest` (as out, of
+ * bf16), what the output's rounding left.
+ * Supported: head_dim a multiple of 8 up to 128. Scores, statistics and sums are
+ * fp32; bf16 weights enter the product with v rounded once, and their sum with them.
+ */
+typedef struct fjx_packed_attention_args {
+  int64_t tokens_q;
+  int64_t tokens_k;       /* may be 0 */
+  int64_t sequences;
+  int64_t heads;
+  int64_t kv_heads;       /* a divisor of heads */
+  int64_t head_dim;
+  int32_t dtype;          /* of q, k, v, out and rest */
+  int32_t index_dtype;    /* of q_starts, k_starts and k_lengths */
+  int32_t causal;
+  int32_t zero_tail;
+  float scale;            /* in [1e-30, 1e30] */
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  int64_t q_strides[2];
+  int64_t k_strides[2];
+  int64_t v_strides[2];
+  int64_t out_strides[2];
+  const void* q_starts;   /* [sequences + 1] */
+  const void* k_starts;   /* [sequences + 1] */
+  const void* k_lengths;  /* [sequences] or NULL */
+  float* lse;             /* or NULL */
+  void* rest;             /* or NULL; fp32: NULL */
+  int64_t rest_strides[2];
+  void* workspace;        /* may be NULL when the size is 0 */
+  size_t workspace_bytes;
+} fjx_packed_attention_args;
+
+size_t fjx_packed_attention_workspace_size(int64_t tokens_q, int64_t tokens_k, int64_t sequences, int64_t heads,
+                                           int64_t kv_heads, int64_t head_dim, int32_t dtype);
+int fjx_packed_attention_fwd(const fjx_packed_attention_args* args, hipStream_t stream);
+
+/*
+ * The gradients of fjx_packed_attention_fwd. `fwd` holds that call's arguments with
+ * the out, lse and rest that it wrote (rest may be NULL in bf16: the gradients of
+ * rows with one heavy key then lose digits). Every row of dq, dk and dv is written,
+ * those of no sequence as zeros. Every sum has one order: the same bits each time.
+ */
+typedef struct fjx_packed_attention_bwd_args {
+  fjx_packed_attention_args fwd;
+  const void* dout;
+  void* dq;
+  void* dk;
+  void* dv;
+  int64_t dout_strides[2];
+  int64_t dq_strides[2];
+  int64_t dk_strides[2];
+  int64_t dv_strides[2];
+} fjx_packed_attention_bwd_args;
+
+size_t fjx_packed_attention_bwd_workspace_size(int64_t tokens_q, int64_t tokens_k, int64_t sequences, int64_t heads,
+                                               int64_t kv_heads, int64_t head_dim, int32_t dtype);
+int fjx_packed_attention_bwd(const fjx_packed_attention_bwd_args* args, hipStream_t stream);
+
+/*
+ * The root-mean-square norm of each head's queries and keys and their rotation by
+ * position, in one pass. No counterpart in the reference, whose tokens know their
+ * places from the pair track.
+ *   n = x / sqrt(mean(x^2) + eps) * weight       (x itself where the weight is NULL)
+ *   y = each pair (a, b) of n turned: (a cos t - b sin t, a sin t + b cos t)
+ * Pairs are channels (i, i + pairs), with `neighbours` (2 i, 2 i + 1); channels
+ * from 2 pairs on are left as they are. t = position * frequencies[i], in 64 bits,
+ * the position being that of pair i's axis: the first sections[0] pairs have axis 0,
+ * the next sections[1] axis 1, and so on (up to 4 axes, for instance residue, chain
+ * and copy). q [items, heads, tokens, head_dim], k [items, kv_heads, tokens, head_dim]
+ * (kv_heads 0: none); *_strides are {item, head, token} in elements, the last axis
+ * contiguous. An output may be its input. Supported: head_dim a multiple of 8 up to
+ * 256, pairs a multiple of 4 (0: the norm alone).
+ */
+typedef struct fjx_head_norm_rotary_args {
+  int64_t items;
+  int64_t heads;
+  int64_t kv_heads;
+  int64_t tokens;
+  int64_t head_dim;
+  int32_t dtype;             /* of q, k, the weights and the outputs */
+  int32_t index_dtype;       /* of positions */
+  int32_t neighbours;
+  int32_t axes;              /* 1 to 4 */
+  int64_t sections[4];       /* pairs of each axis; their sum is the number of pairs */
+  float eps;
+  const void* q;
+  const void* k;
+  const void* q_weight;      /* [head_dim] or NULL */
+  const void* k_weight;      /* [head_dim] or NULL */
+  const void* positions;     /* [axes, items or 1, tokens] */
+  int64_t position_strides[2]; /* {axis, item}: 0 for positions that the items share */
+  const double* frequencies; /* [pairs], radians a position */
+  void* q_out;
+  void* k_out;
+  int64_t q_strides[3];
+  int64_t k_strides[3];
+  int64_t q_out_strides[3];
+  int64_t k_out_strides[3];
+} fjx_head_norm_rotary_args;
+
+int fjx_head_norm_rotary_fwd(const fjx_head_norm_rotary_args* args, hipStream_t stream);
+
+/*
+ * The gradients: `fwd` holds the forward call's arguments, with the outputs'
+ * gradients in the place of q_out and k_out (they are only read). q and k are not
+ * looked at where there is no weight. dq and dk may be the outputs' gradients. The
+ * weights' gradients are fp32, summed over tokens and heads in one order.
+ */
+typedef struct fjx_head_norm_rotary_bwd_args {
+  fjx_head_norm_rotary_args fwd;
+  void* dq;
+  void* dk;
+  int64_t dq_strides[3];
+  int64_t dk_strides[3];
+  float* dq_weight;          /* [head_dim], with q_weight */
+  float* dk_weight;          /* [head_dim], with k_weight */
+  void* workspace;
+  size_t workspace_bytes;
+} fjx_head_norm_rotary_bwd_args;
+
+size_t fjx_head_norm_rotary_bwd_workspace_size(int64_t items, int64_t heads, int64_t kv_heads, int64_t tokens,
+                                               int64_t head_dim);
+int fjx_head_norm_rotary_bwd(const fjx_head_norm_rotary_bwd_args* args, hipStream_t stream);
 
 /* Message for the last error on the calling thread ("" if none). */
 const char* fjx_last_error(void);
