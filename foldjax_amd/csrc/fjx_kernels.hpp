@@ -356,7 +356,8 @@ struct HeadNormParams {
   int heads[2];
   float eps;
   float* part;             // backward: [blocks][2][d] partial sums of the weights' gradients, or null
-  int chunks, per_chunk;   // teams of a token, and heads of one (set at the launch)
+  int chunks, per_chunk;   // workgroups that share a token's heads, and heads of one (set at the launch, as the next)
+  float inv_d;
   int64_t first;           // block of this launch
 };
 template <typename T>

@@ -1151,35 +1151,44 @@ def packed_attention_backward(
     return dq, dk, dv
 
 
-def _like_heads(t: torch.Tensor) -> torch.Tensor:
-    """A new tensor of ``t``'s shape [..., heads, tokens, width] whose memory has a
-    token's heads side by side."""
-    *lead, heads, tokens, width = t.shape
+def _side_by_side(shape):
+    """Strides of [..., heads, tokens, width] whose memory has a token's heads side
+    by side."""
+    *lead, heads, tokens, width = shape
     st, step = [width, heads * width, 1], tokens * heads * width
     for n in reversed(lead):
         st.insert(0, step)
         step *= n
-    return torch.empty_strided(t.shape, st, dtype=t.dtype, device=t.device)
+    return tuple(st)
+
+
+def _like_heads(t: torch.Tensor, strides) -> torch.Tensor:
+    return torch.empty_strided(t.shape, strides, dtype=t.dtype, device=t.device)
 
 
 def _rotary_args(q, k, positions, frequencies, q_weight, k_weight, eps, sections, interleaved):
     """The checked argument block that both directions share, the tensors it points
-    to, the elements of a 16-byte piece, and its key."""
+    to, the elements of a 16-byte piece, the strides of outputs like q and k, and its
+    key."""
     eps, interleaved = float(eps), bool(interleaved)
     sections = None if sections is None else tuple(int(n) for n in sections)
     key = (_layout(q, k, positions, frequencies, q_weight, k_weight), eps, sections, interleaved, "rotary")
     seen = _BLOCKS.get(key)
     if seen is not None:
-        block, unit = seen
+        block, unit, like = seen
         a = _lib.HeadNormRotaryArgs.from_buffer_copy(block)
-        a.q, a.positions, a.frequencies = qp, _, _ = q.data_ptr(), positions.data_ptr(), frequencies.data_ptr()
-        for name, t in (("k", k), ("q_weight", q_weight), ("k_weight", k_weight)):
-            if t is not None:
-                p = t.data_ptr()
-                setattr(a, name, p)
-                qp |= p
-        if not qp & 15:
-            return a, (q, k, positions, frequencies, q_weight, k_weight), unit, key
+        a.q, a.positions, a.frequencies = p, _, _ = q.data_ptr(), positions.data_ptr(), frequencies.data_ptr()
+        if k is not None:
+            a.k = kp = k.data_ptr()
+            p |= kp
+        if q_weight is not None:
+            a.q_weight = wp = q_weight.data_ptr()
+            p |= wp
+        if k_weight is not None:
+            a.k_weight = wp = k_weight.data_ptr()
+            p |= wp
+        if not p & 15:
+            return a, (q, k, positions, frequencies, q_weight, k_weight), unit, like, key
     dtype, shape = q.dtype, q.shape
     code = _code(dtype)
     _same_place(q, dtype, k=k, q_weight=q_weight, k_weight=k_weight)
@@ -1226,9 +1235,10 @@ def _rotary_args(q, k, positions, frequencies, q_weight, k_weight, eps, sections
         qst, kst, (tokens * heads * d, d, heads * d), (tokens * kv_heads * d, d, kv_heads * d))
     kept = (q, k, positions, frequencies, wq, wk)
     as_they_lie = all(x is y for x, y in zip(kept, given))
+    like = _side_by_side(shape), None if k is None else _side_by_side(k.shape)
     if as_they_lie:
-        _remember(key, (bytes(a), unit))
-    return a, kept, unit, key if as_they_lie else None
+        _remember(key, (bytes(a), unit, like))
+    return a, kept, unit, like, key if as_they_lie else None
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
@@ -1266,9 +1276,9 @@ def head_norm_rotary(
     Returns ``(q', k')``, a token's heads side by side in memory (k' None without k).
     ``q_out``, ``k_out``: write into these tensors (of q's and k's shape, their rows
     whole 16-byte pieces: places in a cache, for one), each of which may be its input."""
-    a, kept, unit, _ = _rotary_args(q, k, positions, frequencies, q_weight, k_weight, eps, sections, interleaved)
+    a, kept, unit, like, _ = _rotary_args(q, k, positions, frequencies, q_weight, k_weight, eps, sections, interleaved)
     if q_out is None:
-        q_out = _like_heads(q)
+        q_out = _like_heads(q, like[0])
     else:
         a.q_out_strides = _rotary_out("q_out", q_out, q, unit)
     a.q_out = q_out.data_ptr()
@@ -1277,7 +1287,7 @@ def head_norm_rotary(
             raise ValueError("k_out needs k")
     else:
         if k_out is None:
-            k_out = _like_heads(k)
+            k_out = _like_heads(k, like[1])
         else:
             a.k_out_strides = _rotary_out("k_out", k_out, k, unit)
             if k_out.data_ptr() == a.q_out or (k_out.data_ptr() == a.q and a.q != a.k):
@@ -1318,31 +1328,48 @@ def head_norm_rotary_backward(
     ``(dx_q, dx_k, dq_weight, dk_weight)``: the inputs' in their dtype and shape, a
     token's heads side by side in memory, the weights' float32 ``[D]``, summed over
     tokens and heads in one order; None for what is not there."""
-    a, kept, unit, _ = _rotary_args(q, k, positions, frequencies, q_weight, k_weight, eps, sections, interleaved)
-    if (dk is None) != (k is None):
-        raise ValueError("dk must be given where k is, and only there")
-    _same_place(q, q.dtype, dq=dq, dk=dk)
-    _need_shape("dq", dq, q.shape)
-    if k is not None:
-        _need_shape("dk", dk, k.shape)
-    gk, k_strides = None, (0, 0, 0)
-    dq, a.q_out_strides = _heads(dq, unit)
-    a.q_out = dq.data_ptr()
-    if dk is not None:
-        dk, a.k_out_strides = _heads(dk, unit)
-        a.k_out = dk.data_ptr()
-    gq = _like_heads(q)
-    packed = lambda h: (a.tokens * h * a.head_dim, a.head_dim, h * a.head_dim)  # noqa: E731
-    if k is not None:
-        gk, k_strides = _like_heads(k), packed(a.kv_heads)
-    new = lambda w: None if w is None else torch.empty((a.head_dim,), dtype=torch.float32, device=q.device)  # noqa: E731
-    dwq, dwk = new(q_weight), new(k_weight)
-    b = _lib.HeadNormRotaryBwdArgs(a, gq.data_ptr(), _ptr(gk), packed(a.heads), k_strides, _ptr(dwq), _ptr(dwk))
+    a, kept, unit, like, key = _rotary_args(q, k, positions, frequencies, q_weight, k_weight, eps, sections, interleaved)
+    key = None if key is None else (key, _layout(dq, dk))
+    seen = None if key is None else _BLOCKS.get(key)
     lib = _lib.load()
-    if dwq is not None or dwk is not None:
-        nbytes = lib.fjx_head_norm_rotary_bwd_workspace_size(a.items, a.heads, a.kv_heads, a.tokens, a.head_dim)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    if seen is not None and not (dq.data_ptr() | (0 if dk is None else dk.data_ptr())) & 15:
+        block, nbytes = seen
+        b = _lib.HeadNormRotaryBwdArgs.from_buffer_copy(block)
+        a.q_out_strides, a.k_out_strides = b.fwd.q_out_strides, b.fwd.k_out_strides
+    else:
+        if (dk is None) != (k is None):
+            raise ValueError("dk must be given where k is, and only there")
+        _same_place(q, q.dtype, dq=dq, dk=dk)
+        _need_shape("dq", dq, q.shape)
+        if k is not None:
+            _need_shape("dk", dk, k.shape)
+        given = dq, dk
+        dq, a.q_out_strides = _heads(dq, unit)
+        if dk is not None:
+            dk, a.k_out_strides = _heads(dk, unit)
+        packed = lambda h: (a.tokens * h * a.head_dim, a.head_dim, h * a.head_dim)  # noqa: E731
+        b = _lib.HeadNormRotaryBwdArgs(a, None, None, packed(a.heads), packed(a.kv_heads))
+        nbytes = 0
+        if q_weight is not None or k_weight is not None:
+            nbytes = lib.fjx_head_norm_rotary_bwd_workspace_size(a.items, a.heads, a.kv_heads, a.tokens, a.head_dim)
+        if key is not None and dq is given[0] and dk is given[1]:
+            _remember(key, (bytes(b), nbytes))
+    dev = q.device
+    gq, gk, dwq, dwk = _like_heads(q, like[0]), None, None, None
+    a.q_out, b.dq = dq.data_ptr(), gq.data_ptr()
+    if k is not None:
+        gk = _like_heads(k, like[1])
+        a.k_out, b.dk = dk.data_ptr(), gk.data_ptr()
+    if q_weight is not None:
+        dwq = torch.empty(a.head_dim, dtype=torch.float32, device=dev)
+        b.dq_weight = dwq.data_ptr()
+    if k_weight is not None:
+        dwk = torch.empty(a.head_dim, dtype=torch.float32, device=dev)
+        b.dk_weight = dwk.data_ptr()
+    if nbytes:
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         b.workspace, b.workspace_bytes = ws.data_ptr(), nbytes
+    b.fwd = a
     _launch(lib.fjx_head_norm_rotary_bwd, b, q)
     return gq, gk, dwq, dwk
 
