@@ -1287,33 +1287,57 @@ int diff_bwd_run(const fjx_diff_attention_bwd_args* b, const DiffBwdPlan& plan, 
 
 // ------------------------------------------------------ packed attention
 // How a call is cut. The host knows how many sequences and tokens there are, not how
-// long each is: `own` counts the workgroups of R tiles a wave if all lengths were alike.
+// long each is: the rules take all lengths as alike.
 struct PackedPlan {
   PackedForm rows, keys;
   int splits;                // of the keys (forward, keywise), of the heads that share keys (dk, dv)
   size_t part_o, part_ml;    // workspace bytes: forward; backward: one of dk, dv and D
+  size_t rows_order, keys_order;
 };
 int packed_width(int64_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
-PackedForm packed_form(int64_t tokens, int64_t seqs, int64_t per, int64_t kvh, int64_t other, int32_t dtype) {
-  const int64_t rows = tokens * per;
-  auto own = [&](int64_t tile) { return kvh * ((rows + tile - 1) / tile); };
+// `wgs`: workgroups of 64 rows (keys) there are, `walk`: keys (rows) that one walks.
+// us by form, KS 4 / KS 2 / KS 1 with one tile / KS 2 / KS 1 with two:
+//   forward  126 workgroups 1003 keys d 64        9.3 / 12.2 / 15.4 /   - /   -
+//            216            850       128        25.7 / 17.4 / 20.9 / 24.3 / 29.6
+//            258            700        64        20.2 / 15.3 / 17.1 / 17.7 / 21.2
+//            496            245        24        15.7 / 11.5 /  9.8 / 11.8 / 10.5
+//            520            4099      128         123 / 62.7 / 70.5 / 69.6 / 98.2
+//           1024            1640      128         188 /   92 /   81 /   77 /  106
+//           2048            2730      128         660 /  320 /  285 /  249 /  234
+//   float32  132 workgroups 700 keys   64        41.5 / 41.9 / 45.6;  256, 2048, d 128  112 / 160 / 156
+// (the last two of the forward rows sorted). `most`: tiles of a wave at most.
+PackedForm packed_form(int64_t rows, int64_t seqs, int64_t wgs, int64_t walk, int most, int64_t few) {
   PackedForm f = {};
-  f.keywise = other > 64 * seqs && (rows <= 16 * seqs || own(64) < 128);
-  f.tiles = !f.keywise && dtype == FJX_DTYPE_BF16 && own(128) >= 256 ? 2 : 1;
-  const int64_t tile = f.keywise ? 16 : 64 * f.tiles;
-  const int64_t count = rows / tile + seqs + 1;
-  f.count = (int)std::min<int64_t>(count, 1 << 30);
+  f.tiles = 1;
+  if (walk > 64 && (rows <= 16 * seqs || wgs < few))
+    f.ks = 4;
+  else if (walk < 320 || wgs < 128)
+    f.ks = 1;
+  else if (wgs < 1024 || most < 2)
+    f.ks = 2;
+  else {
+    f.ks = wgs < 2048 ? 2 : 1;
+    f.tiles = 2;
+  }
+  f.count = (int)std::min<int64_t>(rows / f.rows() + seqs + 1, 1 << 30);
   return f;
 }
+// Sorting the tiles by their work takes a launch, 4 us: for calls of several sequences
+// that walk 16384 blocks of 64 and more in all (the forward pass of 5 causal sequences,
+// 8192 tokens, 85 -> 77 us with it, of 6 with 16384 254 -> 234)
+bool packed_sorted(const PackedForm& f, int64_t seqs, int64_t wgs, int64_t walk) {
+  return !f.keywise() && f.count && f.count <= kPackedOrder && seqs > 1 && wgs * walk >= (int64_t)16384 * 64;
+}
 PackedPlan packed_fwd_plan(int64_t tq, int64_t tk, int64_t seqs, int64_t heads, int64_t kvh, int64_t d, int32_t dtype) {
-  const int64_t group = heads / kvh;
+  const int64_t group = heads / kvh, rows = tq * group, wgs = kvh * ((rows + 63) / 64), walk = tk / seqs;
+  const bool bf = dtype == FJX_DTYPE_BF16;
   PackedPlan p = {};
-  p.rows = packed_form(tq, seqs, group, kvh, tk, dtype);
+  p.rows = packed_form(rows, seqs, wgs, walk, bf ? 2 : 1, bf ? 128 : d <= 64 ? 256 : 512);
   p.splits = 1;
-  if (p.rows.keywise) {
-    const int64_t wgs = kvh * std::max(seqs, tq * group / 16);
+  if (p.rows.keywise()) {
+    const int64_t tiles = kvh * std::max(seqs, rows / 16);
     // two blocks of 128 keys a split at least, were the lengths alike
-    const int64_t want = wgs <= 128 ? std::min<int64_t>(512 / wgs, tk / seqs / 256) : 1;
+    const int64_t want = tiles <= 128 ? std::min<int64_t>(512 / tiles, walk / 256) : 1;
     if (want > 1) {
       p.splits = (int)want;
       const size_t r = (size_t)heads * tq * p.splits;
@@ -1321,23 +1345,24 @@ PackedPlan packed_fwd_plan(int64_t tq, int64_t tk, int64_t seqs, int64_t heads, 
       p.part_ml = align_up(r * 2 * sizeof(float));
     }
   }
+  if (packed_sorted(p.rows, seqs, wgs, walk)) p.rows_order = align_up((size_t)p.rows.count * sizeof(int2));
   return p;
 }
 PackedPlan packed_bwd_plan(int64_t tq, int64_t tk, int64_t seqs, int64_t heads, int64_t kvh, int64_t d, int32_t dtype) {
-  const int64_t group = heads / kvh;
+  const int64_t group = heads / kvh, rows = tq * group, wgs = kvh * ((rows + 63) / 64), walk = tk / seqs;
+  const int64_t key_wgs = kvh * ((tk + 63) / 64);
+  const bool bf = dtype == FJX_DTYPE_BF16;
   PackedPlan p = {};
-  p.rows = packed_form(tq, seqs, group, kvh, tk, dtype);
-  p.keys = packed_form(tk, seqs, 1, kvh, tq * group, dtype);
-  if (!tq) p.rows.count = 0;
-  if (!tk) p.keys.count = 0;
   p.splits = 1;
   // workgroups that walk long and, causal, uneven ways: the heads that share keys in parts
-  const int64_t wgs = kvh * ((tk + 64 * p.keys.tiles - 1) / (64 * p.keys.tiles));
-  if (!p.keys.keywise && group > 1 && tk && wgs < 1024) {
-    p.splits = (int)std::min<int64_t>(group, (1024 + wgs - 1) / wgs);
-    p.part_o = align_up((size_t)p.splits * kvh * tk * packed_width(d) * sizeof(float));
-  }
+  if (group > 1 && tk && key_wgs < 1024) p.splits = (int)std::min<int64_t>(group, (1024 + key_wgs - 1) / key_wgs);
+  if (tq) p.rows = packed_form(rows, seqs, wgs, walk, bf ? 2 : 1, bf ? 128 : 256);
+  // two tiles of keys a wave would take more registers than two waves a SIMD have at 128 channels
+  if (tk) p.keys = packed_form(tk, seqs, key_wgs * p.splits, tq / seqs, bf && d <= 64 ? 2 : 1, bf ? 128 : 256);
+  if (p.splits > 1) p.part_o = align_up((size_t)p.splits * kvh * tk * packed_width(d) * sizeof(float));
   p.part_ml = align_up((size_t)heads * tq * sizeof(float));
+  if (packed_sorted(p.rows, seqs, wgs, walk)) p.rows_order = align_up((size_t)p.rows.count * sizeof(int2));
+  if (packed_sorted(p.keys, seqs, key_wgs * group, tq / seqs)) p.keys_order = align_up((size_t)p.keys.count * sizeof(int2));
   return p;
 }
 
@@ -1427,7 +1452,7 @@ int packed_fwd_run(const fjx_packed_attention_args* a, const PackedPlan& plan, h
   p.part_o = at<float>(a->workspace, 0);
   p.part_ml = at<float>(a->workspace, plan.part_o);
   PackedForm form = plan.rows;
-  form.count *= plan.splits;
+  p.order = form.order = plan.rows_order ? at<int2>(a->workspace, plan.part_o + plan.part_ml) : nullptr;
   return timed(K_PACKED_ATTENTION_FWD, st, "packed_attention_fwd", [&] { launch_packed_fwd<T>(p, form, st); });
 }
 
@@ -1450,8 +1475,11 @@ int packed_bwd_run(const fjx_packed_attention_bwd_args* b, const PackedPlan& pla
   p.part_dk = at<float>(a->workspace, 0);
   p.part_dv = at<float>(a->workspace, plan.part_o);
   p.delta = at<float>(a->workspace, 2 * plan.part_o);
-  return timed(K_PACKED_ATTENTION_BWD, st, "packed_attention_bwd",
-               [&] { launch_packed_bwd<T>(p, plan.rows, plan.keys, st); });
+  PackedForm rows = plan.rows, keys = plan.keys;
+  const size_t end = 2 * plan.part_o + plan.part_ml;
+  rows.order = plan.rows_order ? at<int2>(a->workspace, end) : nullptr;
+  keys.order = plan.keys_order ? at<int2>(a->workspace, end + plan.rows_order) : nullptr;
+  return timed(K_PACKED_ATTENTION_BWD, st, "packed_attention_bwd", [&] { launch_packed_bwd<T>(p, rows, keys, st); });
 }
 
 // ------------------------------------------------- heads' norm and rotation
@@ -1923,7 +1951,7 @@ size_t fjx_packed_attention_workspace_size(int64_t tokens_q, int64_t tokens_k, i
       !dtype_ok(dtype))
     return 0;
   const PackedPlan p = packed_fwd_plan(tokens_q, tokens_k, sequences, heads, kv_heads, head_dim, dtype);
-  return p.part_o + p.part_ml;
+  return p.part_o + p.part_ml + p.rows_order;
 }
 
 int fjx_packed_attention_fwd(const fjx_packed_attention_args* a, hipStream_t st) {
@@ -1934,7 +1962,7 @@ int fjx_packed_attention_fwd(const fjx_packed_attention_args* a, hipStream_t st)
   if (!a->tokens_q) return FJX_OK;
   const PackedPlan plan = packed_fwd_plan(a->tokens_q, a->tokens_k, a->sequences, a->heads, a->kv_heads, a->head_dim, a->dtype);
   if (int rc = packed_launch_ok(fn, plan.rows, a->kv_heads, plan.splits)) return rc;
-  const size_t need = plan.part_o + plan.part_ml;
+  const size_t need = plan.part_o + plan.part_ml + plan.rows_order;
   if (need && (!a->workspace || a->workspace_bytes < need))
     return fail(FJX_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", fn, need, a->workspace_bytes);
   if (need && !aligned16({a->workspace})) return fail(FJX_ERR_INVALID, "%s: the workspace must be 16-byte aligned", fn);
@@ -1947,7 +1975,7 @@ size_t fjx_packed_attention_bwd_workspace_size(int64_t tokens_q, int64_t tokens_
       !dtype_ok(dtype))
     return 0;
   const PackedPlan p = packed_bwd_plan(tokens_q, tokens_k, sequences, heads, kv_heads, head_dim, dtype);
-  return 2 * p.part_o + p.part_ml;
+  return 2 * p.part_o + p.part_ml + p.rows_order + p.keys_order;
 }
 
 int fjx_packed_attention_bwd(const fjx_packed_attention_bwd_args* b, hipStream_t st) {
@@ -1969,7 +1997,7 @@ int fjx_packed_attention_bwd(const fjx_packed_attention_bwd_args* b, hipStream_t
   const PackedPlan plan = packed_bwd_plan(a->tokens_q, a->tokens_k, a->sequences, a->heads, a->kv_heads, a->head_dim, a->dtype);
   if (int rc = packed_launch_ok(fn, plan.rows, a->kv_heads, 1)) return rc;
   if (int rc = packed_launch_ok(fn, plan.keys, a->kv_heads, plan.splits)) return rc;
-  const size_t need = 2 * plan.part_o + plan.part_ml;
+  const size_t need = 2 * plan.part_o + plan.part_ml + plan.rows_order + plan.keys_order;
   if (need && (!a->workspace || a->workspace_bytes < need))
     return fail(FJX_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", fn, need, a->workspace_bytes);
   if (need && !aligned16({a->workspace})) return fail(FJX_ERR_INVALID, "%s: the workspace must be 16-byte aligned", fn);

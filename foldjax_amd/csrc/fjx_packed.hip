@@ -25,34 +25,36 @@ constexpr float kSlack = 8.f;
 constexpr float kFar = 16777216.f;
 
 template <typename T, int DP, int KS, int R>
-__global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1)) void packed_fwd_kernel(PackedParams<T> P) {
+__global__ __launch_bounds__(PkForm<KS>::kThreads, (PkForm<KS>::template kSimd<T, DP>)) void packed_fwd_kernel(PackedParams<T> P) {
   typedef PkForm<KS> Form;
   typedef PkRows<T, DP> Rows;
   typedef typename Frag<T>::type F;
   constexpr int kC = Rows::kC, kU = Rows::kU;
-  constexpr int kNt = Form::kBlock / KS / 16;  // key tiles of a wave in a block
-  constexpr int kTileRows = 16 * R * (KS == 1 ? 4 : 1), kShift = __builtin_ctz(kTileRows);
+  constexpr int kNt = Form::kOwn / 16;  // key tiles of a wave in a block
+  constexpr int kTileRows = 16 * R * Form::kGroups, kShift = __builtin_ctz(kTileRows);
   constexpr int kOperand = Form::kStage * Rows::kRowBytes;
-  constexpr int kSets = KS == 1 ? 1 : 4;       // of staged rows
+  constexpr int kSets = Form::kSets;
   constexpr int kStages = 4 * kOperand * kSets <= 160 * 1024 ? 2 : 1;
   constexpr int kPo = DP + 2;
-  static_assert(KS == 1 || kStages * 2 * kOperand * kSets >= 4 * 16 * R * (kPo + 2) * 4, "the waves' sums");
+  static_assert(KS == 1 || kStages * 2 * kOperand * kSets >= 4 * 16 * R * kPo * 4 + Form::kWaves * 16 * R * 8, "the waves' sums");
   __shared__ __attribute__((aligned(16))) unsigned char raw[kStages * 2 * kOperand * kSets];
 
   const int t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const Form form(wave);
   const int kvh = P.heads / P.group;
   const int kv = blockIdx.x % kvh;
   const uint32_t rest_id = blockIdx.x / kvh;
   const int split = rest_id / (uint32_t)P.tiles;
-  const int tile_id = P.tiles - 1 - (int)(rest_id % (uint32_t)P.tiles);  // causal rows with the most keys first
+  // without an order of their work, from the last tile on: causal rows with the most keys first
+  const int nth = rest_id % (uint32_t)P.tiles, tile_id = P.order ? nth : P.tiles - 1 - nth;
   PackedSpan sp;
   if (!packed_span(P, false, P.group, kShift, tile_id, lane, sp)) return;
   if (sp.seq == P.seqs && !P.zero_tail) return;
   const int rows = sp.nq * P.group;
   const int row0 = sp.tile * kTileRows;
   if (row0 >= rows) return;
-  const int row_w = row0 + (KS == 1 ? 16 * R * wave : 0);
+  const int row_w = row0 + 16 * R * form.group;
 
   // of the lane's rows: head, token, and the keys that it sees: those before lim
   int head[R], token[R], lim[R];
@@ -75,18 +77,17 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1)) void packed_fwd_kern
   const int64_t blocks = most > 0 ? (most + Form::kBlock - 1) / Form::kBlock : 0;
   const int blk0 = (int)(blocks * split / P.splits), blk1 = (int)(blocks * (split + 1) / P.splits);
 
-  unsigned char* const mine = raw + (KS == 1 ? 0 : wave * kStages * 2 * kOperand);
-  const int stager = KS == 1 ? wave : 0;
-  const int key_w = KS == 1 ? 0 : 32 * wave;  // the wave's (staged) keys of a block
+  unsigned char* const mine = raw + (KS == 4 ? wave * kStages * 2 * kOperand : 0);
   PkCopy<T, DP, Form::kStage, Form::kOwners> kcopy, vcopy;
-  kcopy.init(P.k.token, P.d, stager, lane);
-  vcopy.init(P.v.token, P.d, stager, lane);
+  kcopy.init(P.k.token, P.d, form.stager, lane);
+  vcopy.init(P.v.token, P.d, form.stager, lane);
   const T* ks = P.k.p + kv * P.k.head + (int64_t)sp.k0 * P.k.token;
   const T* vs = P.v.p + kv * P.v.head + (int64_t)sp.k0 * P.v.token;
   auto stage = [&](int blk, int at) {
     unsigned char* s = mine + at * 2 * kOperand;
-    kcopy.issue(ks, (int64_t)blk * Form::kBlock + key_w, sp.nk, P.d, s, stager);
-    vcopy.issue(vs, (int64_t)blk * Form::kBlock + key_w, sp.nk, P.d, s + kOperand, stager);
+    const int64_t key = (int64_t)blk * Form::kBlock + (KS == 4 ? Form::kOwn * form.part : 0);
+    kcopy.issue(ks, key, sp.nk, P.d, s, form.stager);
+    vcopy.issue(vs, key, sp.nk, P.d, s + kOperand, form.stager);
   };
   PkLane<T, DP> at;
   at.init(lane);
@@ -118,9 +119,9 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1)) void packed_fwd_kern
     } else if (blk + 1 < blk1) {
       stage(blk + 1, cur ^ 1);
     }
-    const unsigned char* kt_ = mine + cur * 2 * kOperand;
+    const unsigned char* kt_ = mine + cur * 2 * kOperand + form.at * Rows::kRowBytes;
     const unsigned char* vt_ = kt_ + kOperand;
-    const int key0 = blk * Form::kBlock + key_w;
+    const int key0 = blk * Form::kBlock + Form::kOwn * form.part;
     if (key0 < lim_hi) {
       f32x4 s[R][kNt];
 #pragma unroll
@@ -211,25 +212,25 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1)) void packed_fwd_kern
   for (int r = 0; r < R; ++r) ls[r] = kOnes ? l[r][0] : group_sum((l[r][0] + l[r][1]) + (l[r][2] + l[r][3]));
 
   if constexpr (KS > 1) {
-    // the waves' partial rows, on the largest of their maxima
+    // the partial rows of the waves that share them, on the largest of their maxima
     float* ml = reinterpret_cast<float*>(raw);  // [wave][row][2], then the outputs
-    auto slot = [&](int j, int r) { return (j * R + r) * 16 + li; };
+    auto slot = [&](int j, int r) { return ((KS == 4 ? j : 4 * j + form.group) * R + r) * 16 + li; };  // of the rows' j-th wave
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < R; ++r)
       if (lg == 0) {
-        ml[slot(wave, r) * 2] = m[r];
-        ml[slot(wave, r) * 2 + 1] = ls[r];
+        ml[slot(form.part, r) * 2] = m[r];
+        ml[slot(form.part, r) * 2 + 1] = ls[r];
       }
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       float mx = -INFINITY, sum = 0.f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) mx = fmaxf(mx, ml[slot(j, r) * 2]);
+      for (int j = 0; j < KS; ++j) mx = fmaxf(mx, ml[slot(j, r) * 2]);
       const float base = pk_base(mx);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sum = fmaf(ml[slot(j, r) * 2 + 1], __builtin_amdgcn_exp2f(ml[slot(j, r) * 2] - base), sum);
+      for (int j = 0; j < KS; ++j) sum = fmaf(ml[slot(j, r) * 2 + 1], __builtin_amdgcn_exp2f(ml[slot(j, r) * 2] - base), sum);
       const float alpha = __builtin_amdgcn_exp2f(m[r] - base);
 #pragma unroll
       for (int u = 0; u < kU; ++u)
@@ -238,19 +239,19 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1)) void packed_fwd_kern
       m[r] = mx;
       ls[r] = sum;
     }
-    pk_sum_waves<R, kU, kPo>(ml + 4 * 16 * R * 2, wave, li, lg, o);
+    pk_sum_waves<KS, R, kU, kPo>(ml + Form::kWaves * 16 * R * 2, form, li, lg, o);
   }
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     if (row_w + 16 * r + li >= rows) continue;
     const int64_t at_row = (int64_t)head[r] * P.tq + token[r];
-    const bool first = lg == 0 && (KS == 1 || wave == 0);
+    const bool first = lg == 0 && form.part == 0;
     if (P.splits > 1) {
       const int64_t base = (int64_t)split * P.heads * P.tq + at_row;
       if (first) *reinterpret_cast<f32x2*>(P.part_ml + base * 2) = f32x2{m[r], ls[r]};
 #pragma unroll
       for (int u = 0; u < kU; ++u)
-        if (KS == 1 || u % 4 == wave) *reinterpret_cast<f32x4*>(P.part_o + base * DP + 16 * u + 4 * lg) = o[r][u];
+        if (form.writes(u)) *reinterpret_cast<f32x4*>(P.part_o + base * DP + 16 * u + 4 * lg) = o[r][u];
       continue;
     }
     if (first && P.lse) *reinterpret_cast<f32x2*>(P.lse + at_row * 2) = pk_stats(m[r], ls[r]);
@@ -259,7 +260,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1)) void packed_fwd_kern
     T* rest = P.rest.p + head[r] * P.rest.head + token[r] * P.rest.token;
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      if (KS > 1 && u % 4 != wave) continue;
+      if (!form.writes(u)) continue;
       const int col = 16 * u + 4 * lg;
       if (col >= P.d) continue;
       float v[4];
@@ -326,23 +327,113 @@ __global__ __launch_bounds__(256) void packed_join_kernel(PackedParams<T> P) {
   }
 }
 
+// The tiles of one key/value head by their work, longest first: they are dealt to the
+// card in this order, and the last to end are short ones (8 causal sequences of one
+// length leave half the card idle at the end else, a long one that comes last more).
+// One workgroup: a tile's work, the number of key blocks (dk, dv: query blocks) that
+// it walks, kept in LDS, then a counting sort by 256 classes of it. The order within a
+// class changes nothing but who starts first.
+template <typename T>
+__global__ __launch_bounds__(1024) void packed_order_kernel(PackedParams<T> P, PackedForm by_rows, PackedForm of_keys) {
+  // a workgroup for each order that is asked for
+  const bool by_keys = !by_rows.order || blockIdx.x;
+  const PackedForm form = by_keys ? of_keys : by_rows;
+  int2* const order = form.order;
+  const int count = form.count, shift = __builtin_ctz(form.rows());
+  constexpr int kClasses = 256;
+  __shared__ int work[kPackedOrder], seqs[kPackedOrder];
+  __shared__ int classes[kClasses], most;
+  const int t = threadIdx.x;
+  if (t < kClasses) classes[t] = 0;
+  if (t == 0) most = 0;
+  __syncthreads();
+  const PackedInts& starts = by_keys ? P.k_starts : P.q_starts;
+  const int64_t tokens = by_keys ? P.tk : P.tq;
+  const int per = by_keys ? 1 : P.group;
+  auto first = [&](int s) { return (int)((packed_start(starts, s, tokens) * per) >> shift) + s; };
+  for (int i = t; i < count; i += 1024) {
+    int lo = 0, hi = P.seqs + 1;  // the last s whose first tile is not behind i
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (first(mid) <= i)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    PackedSpan s;
+    s.seq = lo;
+    s.tile = i - first(lo);
+    packed_sequence(P, by_keys, s);
+    const int64_t row0 = (int64_t)s.tile << shift, rows = by_keys ? s.cap : (int64_t)s.nq * P.group;
+    int blocks = -1;
+    if (s.tile >= 0 && row0 < rows && (s.seq < P.seqs || P.zero_tail)) {
+      int64_t walk;
+      if (by_keys) {
+        const int64_t from = P.causal && row0 + s.nq - s.nk > 0 ? row0 + s.nq - s.nk : 0;  // the first query
+        walk = row0 < s.nk && from < s.nq ? s.nq - from : 0;
+      } else {
+        const int64_t last = (row0 + (1 << shift) < rows ? row0 + (1 << shift) : rows) - 1;
+        walk = P.causal ? last / P.group + s.nk - s.nq + 1 : s.nk;
+      }
+      blocks = walk > 0 ? (int)((walk + 63) / 64) : 0;
+      atomicMax(&most, blocks);
+    }
+    work[i] = blocks;
+    seqs[i] = s.seq;
+  }
+  __syncthreads();
+  const int top = most + 1;
+  auto class_of = [&](int w) { return kClasses - 1 - (int)((int64_t)w * kClasses / top); };
+  for (int i = t; i < count; i += 1024)
+    if (work[i] >= 0) atomicAdd(&classes[class_of(work[i])], 1);
+  __syncthreads();
+  if (t < 64) {  // where each class begins
+    int c[4], sum = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      c[j] = sum;
+      sum += classes[4 * t + j];
+    }
+    int before = sum;
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) {
+      const int o = __shfl_up(before, x, 64);
+      if (t >= x) before += o;
+    }
+    before -= sum;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) classes[4 * t + j] = before + c[j];
+    if (t == 63) most = before + sum;
+  }
+  __syncthreads();
+  for (int i = t; i < count; i += 1024)
+    if (work[i] >= 0) order[atomicAdd(&classes[class_of(work[i])], 1)] = make_int2(seqs[i], i - first(seqs[i]));
+  for (int i = most + t; i < count; i += 1024) order[i] = make_int2(-1, 0);
+}
+
 template <typename T, int DP>
 void fwd(const PackedParams<T>& P, const PackedForm& form, hipStream_t st) {
-  const unsigned blocks = (unsigned)((int64_t)form.count * (P.heads / P.group));
-  if (form.keywise) {
-    packed_fwd_kernel<T, DP, 4, 1><<<blocks, 256, 0, st>>>(P);
-    if (P.splits > 1) packed_join_kernel<T, DP><<<(unsigned)(P.heads * P.tq), 256, 0, st>>>(P);
-  } else if (form.tiles == 2) {
-    if constexpr (sizeof(T) == 2) packed_fwd_kernel<T, DP, 1, 2><<<blocks, 256, 0, st>>>(P);
-  } else {
-    packed_fwd_kernel<T, DP, 1, 1><<<blocks, 256, 0, st>>>(P);
-  }
+  const unsigned blocks = (unsigned)((int64_t)form.count * P.splits * (P.heads / P.group));
+  pk_form<T>(form, [&](auto ks, auto r) {
+    constexpr int KS = decltype(ks)::value, R = decltype(r)::value;
+    packed_fwd_kernel<T, DP, KS, R><<<blocks, PkForm<KS>::kThreads, 0, st>>>(P);
+  });
+  if (P.splits > 1) packed_join_kernel<T, DP><<<(unsigned)(P.heads * P.tq), 256, 0, st>>>(P);
 }
 
 }  // namespace
 
 template <typename T>
+void launch_packed_order(const PackedParams<T>& P, const PackedForm& rows, const PackedForm& keys, hipStream_t st) {
+  const int orders = (rows.order != nullptr) + (keys.order != nullptr);
+  if (orders) packed_order_kernel<T><<<orders, 1024, 0, st>>>(P, rows, keys);
+}
+template void launch_packed_order<bf16>(const PackedParams<bf16>&, const PackedForm&, const PackedForm&, hipStream_t);
+template void launch_packed_order<float>(const PackedParams<float>&, const PackedForm&, const PackedForm&, hipStream_t);
+
+template <typename T>
 void launch_packed_fwd(const PackedParams<T>& P, const PackedForm& form, hipStream_t st) {
+  launch_packed_order(P, form, PackedForm{}, st);
   if (P.d <= 32)
     fwd<T, 32>(P, form, st);
   else if (P.d <= 64)

@@ -36,12 +36,16 @@ struct PackedInts {
   int wide;
 };
 
-// how a call is cut: its rows over waves or its keys (keywise), 16-row tiles of a wave
+// how a call is cut
 struct PackedForm {
-  bool keywise;
-  int tiles;
-  int count;  // workgroups for one key/value head
+  int ks;       // 1, 2 or 4: how many waves share a tile (PkForm)
+  int tiles;    // 16-row tiles of a wave
+  __host__ __device__ bool keywise() const { return ks == 4; }
+  __host__ __device__ int rows() const { return ks == 4 ? 16 : 64 * tiles; }  // of a workgroup
+  int count;    // workgroups for one key/value head
+  int2* order;  // [count], to be filled with the tiles in the order of their work, or null
 };
+constexpr int kPackedOrder = 12288;  // tiles that are sorted at most
 
 template <typename T>
 struct PackedParams {
@@ -56,6 +60,7 @@ struct PackedParams {
   int causal;
   int zero_tail;                // rows of no sequence are written as zeros
   int tiles;                    // of a launch, for one key/value head
+  const int2* order;            // [tiles] {sequence, its tile}, those with the most work first; or null
   // keys (dk, dv: the group's heads) over several workgroups, whose sums a second kernel joins
   int splits;
   float* part_o;                // [splits][H][tq][DP]
@@ -105,11 +110,9 @@ __device__ __forceinline__ bool packed_find(const PackedInts& a, int seqs, int64
   return at >= 0;
 }
 
+// what there is of sequence s.seq
 template <typename T>
-__device__ __forceinline__ bool packed_span(const PackedParams<T>& P, bool by_keys, int per, int shift, int tile, int lane,
-                                            PackedSpan& s) {
-  if (!packed_find(by_keys ? P.k_starts : P.q_starts, P.seqs, by_keys ? P.tk : P.tq, per, shift, tile, lane, s.seq, s.tile))
-    return false;
+__device__ __forceinline__ void packed_sequence(const PackedParams<T>& P, bool by_keys, PackedSpan& s) {
   const int64_t q0 = packed_start(P.q_starts, s.seq, P.tq), k0 = packed_start(P.k_starts, s.seq, P.tk);
   int64_t q1 = P.tq, k1 = P.tk, nk = 0;
   if (s.seq < P.seqs) {
@@ -118,23 +121,61 @@ __device__ __forceinline__ bool packed_span(const PackedParams<T>& P, bool by_ke
     if (k1 < k0) k1 = k0;
     nk = P.k_lengths.p ? packed_int(P.k_lengths, s.seq, k1 - k0) : k1 - k0;
   }
-  s.q0 = __builtin_amdgcn_readfirstlane((int)q0);
-  s.nq = s.seq < P.seqs || !by_keys ? __builtin_amdgcn_readfirstlane((int)(q1 > q0 ? q1 - q0 : 0)) : 0;
-  s.k0 = __builtin_amdgcn_readfirstlane((int)k0);
-  s.nk = __builtin_amdgcn_readfirstlane((int)nk);
-  s.cap = __builtin_amdgcn_readfirstlane((int)(k1 > k0 ? k1 - k0 : 0));
+  s.q0 = (int)q0;
+  s.nq = s.seq < P.seqs || !by_keys ? (int)(q1 > q0 ? q1 - q0 : 0) : 0;
+  s.k0 = (int)k0;
+  s.nk = (int)nk;
+  s.cap = (int)(k1 > k0 ? k1 - k0 : 0);
+}
+
+// the sequence and the tile of a workgroup, the `at`-th of a key/value head
+template <typename T>
+__device__ __forceinline__ bool packed_span(const PackedParams<T>& P, bool by_keys, int per, int shift, int at, int lane,
+                                            PackedSpan& s) {
+  if (P.order) {
+    const int2 o = P.order[at];
+    s.seq = __builtin_amdgcn_readfirstlane(o.x);
+    s.tile = __builtin_amdgcn_readfirstlane(o.y);
+    if (s.seq < 0) return false;
+  } else if (!packed_find(by_keys ? P.k_starts : P.q_starts, P.seqs, by_keys ? P.tk : P.tq, per, shift, at, lane, s.seq, s.tile)) {
+    return false;
+  }
+  packed_sequence(P, by_keys, s);
+  s.q0 = __builtin_amdgcn_readfirstlane(s.q0);
+  s.nq = __builtin_amdgcn_readfirstlane(s.nq);
+  s.k0 = __builtin_amdgcn_readfirstlane(s.k0);
+  s.nk = __builtin_amdgcn_readfirstlane(s.nk);
+  s.cap = __builtin_amdgcn_readfirstlane(s.cap);
   return true;
 }
 
-// How the waves of a workgroup share its rows (for the keys' gradients: its keys)
-// and the blocks that it walks: KS 1: four waves with tiles of their own, blocks of
-// 64 staged for all; 4: four waves, one set of tiles, each wave staging 32 of a
-// block of 128 for itself.
+// How the waves of a workgroup share its rows (for the keys' gradients: its keys) and the
+// blocks that it walks. KS 1: four waves with tiles of their own, blocks of 64 staged for
+// all; 2: eight waves, two to the same tiles, each with half of a block of 128; 4: four
+// waves that share one set of tiles, each staging 32 of a block of 128 for itself.
 template <int KS>
 struct PkForm {
-  static constexpr int kBlock = KS == 1 ? 64 : 128;  // of all waves
-  static constexpr int kStage = KS == 1 ? 64 : 32;   // rows staged together
-  static constexpr int kOwners = KS == 1 ? 4 : 1;    // waves that stage them
+  static constexpr int kWaves = KS == 2 ? 8 : 4, kThreads = 64 * kWaves;
+  static constexpr int kGroups = KS == 4 ? 1 : 4;        // of waves with the same tiles
+  static constexpr int kBlock = KS == 1 ? 64 : 128;      // of all waves
+  static constexpr int kOwn = kBlock / KS;               // of one
+  static constexpr int kStage = KS == 4 ? 32 : kBlock;   // rows staged together
+  static constexpr int kSets = KS == 4 ? 4 : 1;          // of such rows
+  static constexpr int kOwners = KS == 4 ? 1 : kWaves;   // waves that stage them
+  static constexpr int kRest = (kStage + 63) / 64;       // waves that fetch a value for each
+  // waves a SIMD that the registers are held to, where a workgroup's LDS (two stages of
+  // two operands) leaves room for as many
+  template <typename T, int DP>
+  static constexpr int kSimd = kWaves / 4 * (sizeof(T) == 2 && 2 * 4 * kStage * kSets * DP * (int)sizeof(T) <= 150 * 1024 ? 2 : 1) >= 2
+                                   ? 2 : 1;
+  // the wave's place: its group, its part of a block, where that begins among its
+  // staged rows, and as which of the owners it stages
+  int group, part, at, stager;
+  __device__ __forceinline__ explicit PkForm(int wave)
+      : group(KS == 4 ? 0 : wave & 3), part(KS == 1 ? 0 : KS == 2 ? wave >> 2 : wave), at(KS == 2 ? kOwn * part : 0),
+        stager(KS == 4 ? 0 : wave) {}
+  // which of the waves with the same rows writes column tile u, after their sums were joined
+  __device__ __forceinline__ bool writes(int u) const { return KS == 1 || (KS == 2 ? part == 0 : (u & 3) == part); }
 };
 
 // Rows of DP elements in LDS, 16-byte piece c of row r in slot c ^ f(r) of its row.
@@ -266,7 +307,7 @@ struct PkCopy {
 template <int KS>
 __device__ __forceinline__ void pk_sync() {
   lds_wait<0>();
-  if constexpr (KS == 1) lds_barrier();
+  if constexpr (KS != 4) lds_barrier();
   asm volatile("" ::: "memory");
 }
 
@@ -294,29 +335,31 @@ __device__ __forceinline__ void pk_round(float by, f32x4 (&s)[NT]) {
     }
 }
 
-// The four waves' accumulators of the same rows added, through LDS; wave w gets the
-// column tiles u with u % 4 == w.
-template <int R, int U, int PITCH>
-__device__ __forceinline__ void pk_sum_waves(float* lds, int wave, int li, int lg, f32x4 (&x)[R][U]) {
+// The accumulators of the waves with the same rows added, through LDS (PITCH floats a
+// row): KS 2: the first of two gets them, 4: wave w the column tiles u with u % 4 == w.
+template <int KS, int R, int U, int PITCH>
+__device__ __forceinline__ void pk_sum_waves(float* lds, const PkForm<KS>& f, int li, int lg, f32x4 (&x)[R][U]) {
   auto slot = [&](int j, int r) { return ((j * R + r) * 16 + li) * PITCH + 4 * lg; };
   __syncthreads();
+  if (KS == 4 || f.part) {
 #pragma unroll
-  for (int r = 0; r < R; ++r)
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) lds[slot(wave, r) + 16 * u + e] = x[r][u][e];
+        for (int e = 0; e < 4; ++e) lds[slot(KS == 4 ? f.part : f.group, r) + 16 * u + e] = x[r][u][e];
+  }
   __syncthreads();
 #pragma unroll
   for (int r = 0; r < R; ++r)
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (u % 4 != wave) continue;
+      if (!f.writes(u)) continue;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        float a = 0.f;
+        float a = KS == 4 ? 0.f : x[r][u][e];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) a += lds[slot(j, r) + 16 * u + e];
+        for (int j = 0; j < (KS == 4 ? 4 : 1); ++j) a += lds[slot(KS == 4 ? j : f.group, r) + 16 * u + e];
         x[r][u][e] = a;
       }
     }
@@ -333,6 +376,22 @@ __device__ __forceinline__ float lanes4_max(float x) {
   return fmaxf(__builtin_bit_cast(float, b0), __builtin_bit_cast(float, b1));
 }
 
+// f(KS, R) for a form; float32 has one tile a wave
+template <typename T, typename F>
+void pk_form(const PackedForm& form, F f) {
+  typedef std::integral_constant<int, 1> One;
+  typedef std::integral_constant<int, 2> Two;
+  if (form.ks == 4) return f(std::integral_constant<int, 4>{}, One{});
+  if constexpr (sizeof(T) == 2) {
+    if (form.tiles == 2) return form.ks == 2 ? f(Two{}, Two{}) : f(One{}, Two{});
+  }
+  if (form.ks == 2) return f(Two{}, One{});
+  f(One{}, One{});
+}
+
+// the orders that `rows` and `keys` ask for
+template <typename T>
+void launch_packed_order(const PackedParams<T>& P, const PackedForm& rows, const PackedForm& keys, hipStream_t st);
 template <typename T>
 void launch_packed_fwd(const PackedParams<T>& P, const PackedForm& form, hipStream_t st);
 template <typename T>

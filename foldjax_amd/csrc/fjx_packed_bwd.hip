@@ -26,15 +26,15 @@ __device__ __forceinline__ float pk_weight(float s, float by, float m, float log
 
 // dq, and D for the other kernel: rows and blocks as in the forward pass.
 template <typename T, int DP, int KS, int R>
-__global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1)) void packed_dq_kernel(PackedParams<T> P) {
+__global__ __launch_bounds__(PkForm<KS>::kThreads, (PkForm<KS>::template kSimd<T, DP>)) void packed_dq_kernel(PackedParams<T> P) {
   typedef PkForm<KS> Form;
   typedef PkRows<T, DP> Rows;
   typedef typename Frag<T>::type F;
   constexpr int kC = Rows::kC, kU = Rows::kU;
-  constexpr int kNt = Form::kBlock / KS / 16;
-  constexpr int kTileRows = 16 * R * (KS == 1 ? 4 : 1), kShift = __builtin_ctz(kTileRows);
+  constexpr int kNt = Form::kOwn / 16;
+  constexpr int kTileRows = 16 * R * Form::kGroups, kShift = __builtin_ctz(kTileRows);
   constexpr int kOperand = Form::kStage * Rows::kRowBytes;
-  constexpr int kSets = KS == 1 ? 1 : 4;
+  constexpr int kSets = Form::kSets;
   constexpr int kStages = 4 * kOperand * kSets <= 160 * 1024 ? 2 : 1;
   constexpr int kPo = DP + 2;
   static_assert(KS == 1 || kStages * 2 * kOperand * kSets >= 4 * 16 * R * kPo * 4, "the waves' sums");
@@ -42,15 +42,16 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1)) void packed_dq_kerne
 
   const int t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const Form form(wave);
   const int kvh = P.heads / P.group;
   const int kv = blockIdx.x % kvh;
-  const int tile_id = P.tiles - 1 - (int)(blockIdx.x / kvh);
+  const int nth = blockIdx.x / kvh, tile_id = P.order ? nth : P.tiles - 1 - nth;  // as in the forward pass
   PackedSpan sp;
   if (!packed_span(P, false, P.group, kShift, tile_id, lane, sp)) return;
   const int rows = sp.nq * P.group;
   const int row0 = sp.tile * kTileRows;
   if (row0 >= rows) return;
-  const int row_w = row0 + (KS == 1 ? 16 * R * wave : 0);
+  const int row_w = row0 + 16 * R * form.group;
 
   int head[R], token[R], lim[R];
   F qf[R][kC], dof[R][kC];
@@ -92,7 +93,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1)) void packed_dq_kerne
     m[r] = stats[0];
     log_sum[r] = stats[1];
     any_far = any_far || fabsf(m[r]) > kFar;
-    if (lg == 0 && (KS == 1 || wave == 0) && row_w + 16 * r + li < rows) P.delta[at_row] = delta[r];
+    if (lg == 0 && form.part == 0 && row_w + 16 * r + li < rows) P.delta[at_row] = delta[r];
   }
   const bool far = __builtin_amdgcn_ballot_w64(any_far);
   const int last = (row0 + kTileRows < rows ? row0 + kTileRows : rows) - 1;
@@ -101,18 +102,17 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1)) void packed_dq_kerne
   const int lim_hi = row_w < rows ? __builtin_amdgcn_readlane(lim[R - 1], 15) : 0;
   const int blocks = most > 0 ? (int)(((int64_t)most + Form::kBlock - 1) / Form::kBlock) : 0;
 
-  unsigned char* const mine = raw + (KS == 1 ? 0 : wave * kStages * 2 * kOperand);
-  const int stager = KS == 1 ? wave : 0;
-  const int key_w = KS == 1 ? 0 : 32 * wave;
+  unsigned char* const mine = raw + (KS == 4 ? wave * kStages * 2 * kOperand : 0);
   PkCopy<T, DP, Form::kStage, Form::kOwners> kcopy, vcopy;
-  kcopy.init(P.k.token, P.d, stager, lane);
-  vcopy.init(P.v.token, P.d, stager, lane);
+  kcopy.init(P.k.token, P.d, form.stager, lane);
+  vcopy.init(P.v.token, P.d, form.stager, lane);
   const T* ks = P.k.p + kv * P.k.head + (int64_t)sp.k0 * P.k.token;
   const T* vs = P.v.p + kv * P.v.head + (int64_t)sp.k0 * P.v.token;
   auto stage = [&](int blk, int at) {
     unsigned char* s = mine + at * 2 * kOperand;
-    kcopy.issue(ks, (int64_t)blk * Form::kBlock + key_w, sp.nk, P.d, s, stager);
-    vcopy.issue(vs, (int64_t)blk * Form::kBlock + key_w, sp.nk, P.d, s + kOperand, stager);
+    const int64_t key = (int64_t)blk * Form::kBlock + (KS == 4 ? Form::kOwn * form.part : 0);
+    kcopy.issue(ks, key, sp.nk, P.d, s, form.stager);
+    vcopy.issue(vs, key, sp.nk, P.d, s + kOperand, form.stager);
   };
   PkLane<T, DP> at;
   at.init(lane);
@@ -134,9 +134,9 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1)) void packed_dq_kerne
     } else if (blk + 1 < blocks) {
       stage(blk + 1, cur ^ 1);
     }
-    const unsigned char* kt_ = mine + cur * 2 * kOperand;
+    const unsigned char* kt_ = mine + cur * 2 * kOperand + form.at * Rows::kRowBytes;
     const unsigned char* vt_ = kt_ + kOperand;
-    const int key0 = blk * Form::kBlock + key_w;
+    const int key0 = blk * Form::kBlock + Form::kOwn * form.part;
     if (key0 < lim_hi) {
       const bool masked = key0 + 16 * kNt > lim_lo;
 #pragma unroll
@@ -194,7 +194,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1)) void packed_dq_kerne
     }
     pk_sync<KS>();
   }
-  if constexpr (KS > 1) pk_sum_waves<R, kU, kPo>(reinterpret_cast<float*>(raw), wave, li, lg, dq);
+  if constexpr (KS > 1) pk_sum_waves<KS, R, kU, kPo>(reinterpret_cast<float*>(raw), form, li, lg, dq);
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     if (row_w + 16 * r + li >= rows) continue;
@@ -202,7 +202,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1)) void packed_dq_kerne
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
       const int col = 16 * u + 4 * lg;
-      if ((KS > 1 && u % 4 != wave) || col >= P.d) continue;
+      if (!form.writes(u) || col >= P.d) continue;
       float v[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = dq[r][u][e] * P.scale;
@@ -216,24 +216,25 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1)) void packed_dq_kerne
 // the lane 4 queries of its own keys, as the operands of dV^T = dO^T P and dK^T = Q^T dS.
 // KS 1: four waves with keys of their own; 4: the waves share keys and split the queries.
 template <typename T, int DP, int KS, int R>
-__global__ __launch_bounds__(256, (sizeof(T) == 2 && DP * R <= 128 ? 2 : 1)) void packed_dkv_kernel(PackedParams<T> P) {
+__global__ __launch_bounds__(PkForm<KS>::kThreads, (PkForm<KS>::template kSimd<T, DP>)) void packed_dkv_kernel(PackedParams<T> P) {
   typedef PkForm<KS> Form;
   typedef PkRows<T, DP> Rows;
   typedef typename Frag<T>::type F;
   constexpr int kC = Rows::kC, kU = Rows::kU;
-  constexpr int kNt = Form::kBlock / KS / 16;  // query tiles of a wave in a block
-  constexpr int kTileKeys = 16 * R * (KS == 1 ? 4 : 1), kShift = __builtin_ctz(kTileKeys);
+  constexpr int kNt = Form::kOwn / 16;  // query tiles of a wave in a block
+  constexpr int kTileKeys = 16 * R * Form::kGroups, kShift = __builtin_ctz(kTileKeys);
   constexpr int kOperand = Form::kStage * Rows::kRowBytes;
-  constexpr int kSets = KS == 1 ? 1 : 4;
+  constexpr int kSets = Form::kSets;
   constexpr int kStages = 4 * kOperand * kSets <= 156 * 1024 ? 2 : 1;
   constexpr int kPo = DP + 2;
   static_assert(KS == 1 || kStages * 2 * kOperand * kSets >= 4 * 16 * R * kPo * 4, "the waves' sums");
   __shared__ __attribute__((aligned(16))) unsigned char raw[kStages * 2 * kOperand * kSets];
   __shared__ __attribute__((aligned(16))) float rowstat[kSets][kStages][3][Form::kStage];  // M, log2 of the sum, D
-  __shared__ int rowfar[kSets][kStages];
+  __shared__ int rowfar[kSets][kStages][Form::kRest];
 
   const int t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const Form form(wave);
   const int kvh = P.heads / P.group;
   const int kv = blockIdx.x % kvh;
   const uint32_t rest_id = blockIdx.x / kvh;
@@ -242,7 +243,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP * R <= 128 ? 2 : 1)) voi
   if (!packed_span(P, true, 1, kShift, (int)(rest_id % (uint32_t)P.tiles), lane, sp)) return;
   const int key0 = sp.tile * kTileKeys;
   if (key0 >= sp.cap) return;
-  const int key_w = key0 + (KS == 1 ? 16 * R * wave : 0);
+  const int key_w = key0 + 16 * R * form.group;
   const int shift = sp.nq - sp.nk;  // a causal row i sees the keys up to i - shift
 
   F kf[R][kC], vf[R][kC];
@@ -266,26 +267,25 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP * R <= 128 ? 2 : 1)) voi
   const int qb1 = key0 < sp.nk ? (int)(((int64_t)sp.nq + Form::kBlock - 1) / Form::kBlock) : 0;
   const int turns = qb1 > qb0 ? (h1 - h0) * (qb1 - qb0) : 0;
 
-  const int set = KS == 1 ? 0 : wave, stager = KS == 1 ? wave : 0;
+  const int set = KS == 4 ? wave : 0;
   unsigned char* const mine = raw + set * kStages * 2 * kOperand;
-  const int q_w = KS == 1 ? 0 : 32 * wave;
+  const int stat_row = KS == 4 ? lane : t;  // of a staged block, of which the thread fetches the statistics
   PkCopy<T, DP, Form::kStage, Form::kOwners> qcopy, ocopy;
-  qcopy.init(P.q.token, P.d, stager, lane);
-  ocopy.init(P.dout.token, P.d, stager, lane);
+  qcopy.init(P.q.token, P.d, form.stager, lane);
+  ocopy.init(P.dout.token, P.d, form.stager, lane);
   int next_h = h0, next_b = qb0;  // of the next block to stage
   f32x2 st_m = {0.f, INFINITY};
   float st_d = 0.f;
   auto stage = [&](int at) {
     const int head = kv * P.group + next_h;
-    const int64_t row0 = (int64_t)next_b * Form::kBlock + q_w;
+    const int64_t row0 = (int64_t)next_b * Form::kBlock + (KS == 4 ? Form::kOwn * form.part : 0);
     unsigned char* s = mine + at * 2 * kOperand;
-    qcopy.issue(P.q.p + head * P.q.head + (int64_t)sp.q0 * P.q.token, row0, sp.nq, P.d, s, stager);
-    ocopy.issue(P.dout.p + head * P.dout.head + (int64_t)sp.q0 * P.dout.token, row0, sp.nq, P.d, s + kOperand, stager);
+    qcopy.issue(P.q.p + head * P.q.head + (int64_t)sp.q0 * P.q.token, row0, sp.nq, P.d, s, form.stager);
+    ocopy.issue(P.dout.p + head * P.dout.head + (int64_t)sp.q0 * P.dout.token, row0, sp.nq, P.d, s + kOperand, form.stager);
     st_m = f32x2{0.f, INFINITY};  // rows past the last: weights of zero
     st_d = 0.f;
-    const int r = KS == 1 ? t : lane;
-    if (r < Form::kStage && row0 + r < sp.nq) {
-      const int64_t at_row = (int64_t)head * P.tq + sp.q0 + row0 + r;
+    if (stat_row < Form::kStage && row0 + stat_row < sp.nq) {
+      const int64_t at_row = (int64_t)head * P.tq + sp.q0 + row0 + stat_row;
       st_m = *reinterpret_cast<const f32x2*>(P.lse + at_row * 2);
       st_d = P.delta[at_row];
     }
@@ -295,13 +295,12 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP * R <= 128 ? 2 : 1)) voi
     }
   };
   auto put_stats = [&](int at) {
-    const int r = KS == 1 ? t : lane;
-    if (r < Form::kStage) {
-      rowstat[set][at][0][r] = st_m[0];
-      rowstat[set][at][1][r] = st_m[1];
-      rowstat[set][at][2][r] = st_d;
+    if (stat_row < Form::kStage) {
+      rowstat[set][at][0][stat_row] = st_m[0];
+      rowstat[set][at][1][stat_row] = st_m[1];
+      rowstat[set][at][2][stat_row] = st_d;
       const bool far = __builtin_amdgcn_ballot_w64(fabsf(st_m[0]) > kFar);
-      if (r == 0) rowfar[set][at] = far;
+      if (stat_row % 64 == 0) rowfar[set][at][stat_row / 64] = far;
     }
   };
   PkLane<T, DP> at;
@@ -329,54 +328,53 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP * R <= 128 ? 2 : 1)) voi
     } else if (turn + 1 < turns) {
       stage(cur ^ 1);
     }
-    const unsigned char* qt_ = mine + cur * 2 * kOperand;
+    const unsigned char* qt_ = mine + cur * 2 * kOperand + form.at * Rows::kRowBytes;
     const unsigned char* ot_ = qt_ + kOperand;
-    const int row0 = qb * Form::kBlock + q_w;
+    const int row0 = qb * Form::kBlock + Form::kOwn * form.part;
     // rows from key + shift on see a key
     if (!P.causal || row0 + 16 * kNt > key_w + shift) {
       const bool masked = P.causal && row0 < key_w + 16 * R - 1 + shift;
-      const bool far = __builtin_amdgcn_readfirstlane(rowfar[set][cur]);
+      int any_far = 0;
+#pragma unroll
+      for (int i = 0; i < Form::kRest; ++i) any_far |= rowfar[set][cur][i];
+      const bool far = __builtin_amdgcn_readfirstlane(any_far);
 #pragma unroll
       for (int pair = 0; pair < kNt / 2; ++pair) {
-        f32x4 s[R][2], dp[R][2];
+        // one tile of 16 queries after the other: the scores of both took more registers
+        // than two waves a SIMD have
+        F pf[R], dsf[R];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
+          f32x4 s[R][1], dp[R];
 #pragma unroll
-          for (int r = 0; r < R; ++r) s[r][j] = dp[r][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+          for (int r = 0; r < R; ++r) s[r][0] = dp[r] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int c = 0; c < kC; ++c) {
             const F qf = at.at_row(qt_, 32 * pair + 16 * j, c);
 #pragma unroll
-            for (int r = 0; r < R; ++r) mma(s[r][j], qf, kf[r][c]);
+            for (int r = 0; r < R; ++r) mma(s[r][0], qf, kf[r][c]);
           }
 #pragma unroll
           for (int c = 0; c < kC; ++c) {
             const F of = at.at_row(ot_, 32 * pair + 16 * j, c);
 #pragma unroll
-            for (int r = 0; r < R; ++r) mma(dp[r][j], of, vf[r][c]);
+            for (int r = 0; r < R; ++r) mma(dp[r], of, vf[r][c]);
           }
-        }
-        float by = P.scale_log2;
-        if (far) {
-          by = 1.f;
+          float by = P.scale_log2;
+          if (far) {
+            by = 1.f;
 #pragma unroll
-          for (int r = 0; r < R; ++r) pk_round(P.scale_log2, s[r]);
-        }
-        if (masked) {
-#pragma unroll
-          for (int r = 0; r < R; ++r) {
-            const int from = key_w + 16 * r + li + shift - row0 - 32 * pair - 4 * lg;
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) s[r][j][e] = 16 * j + e >= from ? s[r][j][e] : -INFINITY;
+            for (int r = 0; r < R; ++r) pk_round(P.scale_log2, s[r]);
           }
-        }
-        F pf[R], dsf[R];
-        float p[R][8], ds[R][8];
+          if (masked) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int row = 32 * pair + 16 * j + 4 * lg;
+            for (int r = 0; r < R; ++r) {
+              const int from = key_w + 16 * r + li + shift - row0 - 32 * pair - 16 * j - 4 * lg;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[r][0][e] = e >= from ? s[r][0][e] : -INFINITY;
+            }
+          }
+          const int row = form.at + 32 * pair + 16 * j + 4 * lg;
           const f32x4 m4 = *reinterpret_cast<const f32x4*>(&rowstat[set][cur][0][row]);
           const f32x4 l4 = *reinterpret_cast<const f32x4*>(&rowstat[set][cur][1][row]);
           const f32x4 d4 = *reinterpret_cast<const f32x4*>(&rowstat[set][cur][2][row]);
@@ -384,14 +382,10 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP * R <= 128 ? 2 : 1)) voi
           for (int r = 0; r < R; ++r)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              p[r][4 * j + e] = pk_weight(s[r][j][e], by, m4[e], l4[e]);
-              ds[r][4 * j + e] = p[r][4 * j + e] * (dp[r][j][e] - d4[e]);
+              const float p = pk_weight(s[r][0][e], by, m4[e], l4[e]);
+              pf[r][4 * j + e] = from_f32<T>(p);
+              dsf[r][4 * j + e] = from_f32<T>(p * (dp[r][e] - d4[e]));
             }
-        }
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-          pf[r] = pack8<T>(p[r]);
-          dsf[r] = pack8<T>(ds[r]);
         }
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
@@ -409,8 +403,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP * R <= 128 ? 2 : 1)) voi
     pk_sync<KS>();
   }
   if constexpr (KS > 1) {
-    pk_sum_waves<R, kU, kPo>(reinterpret_cast<float*>(raw), wave, li, lg, dk);
-    pk_sum_waves<R, kU, kPo>(reinterpret_cast<float*>(raw), wave, li, lg, dv);
+    pk_sum_waves<KS, R, kU, kPo>(reinterpret_cast<float*>(raw), form, li, lg, dk);
+    pk_sum_waves<KS, R, kU, kPo>(reinterpret_cast<float*>(raw), form, li, lg, dv);
   }
 #pragma unroll
   for (int r = 0; r < R; ++r) {
@@ -421,7 +415,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP * R <= 128 ? 2 : 1)) voi
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
       const int col = 16 * u + 4 * lg;
-      if (KS > 1 && u % 4 != wave) continue;
+      if (!form.writes(u)) continue;
       if (P.splits > 1) {
         const int64_t at_key = (((int64_t)split * kvh + kv) * P.tk + token) * DP + col;
         *reinterpret_cast<f32x4*>(P.part_dk + at_key) = real ? dk[r][u] : f32x4{0.f, 0.f, 0.f, 0.f};
@@ -463,27 +457,25 @@ template <typename T, int DP>
 void bwd(PackedParams<T> P, const PackedForm& rows, const PackedForm& keys, hipStream_t st) {
   const int kvh = P.heads / P.group;
   const int splits = P.splits;
+  launch_packed_order(P, rows, keys, st);
   P.splits = 1;
   P.tiles = rows.count;
+  P.order = rows.order;
   if (rows.count) {
-    const unsigned blocks = (unsigned)((int64_t)rows.count * kvh);
-    if (rows.keywise)
-      packed_dq_kernel<T, DP, 4, 1><<<blocks, 256, 0, st>>>(P);
-    else if (rows.tiles == 2) {
-      if constexpr (sizeof(T) == 2) packed_dq_kernel<T, DP, 1, 2><<<blocks, 256, 0, st>>>(P);
-    } else
-      packed_dq_kernel<T, DP, 1, 1><<<blocks, 256, 0, st>>>(P);
+    pk_form<T>(rows, [&](auto ks, auto r) {
+      constexpr int KS = decltype(ks)::value, R = decltype(r)::value;
+      packed_dq_kernel<T, DP, KS, R><<<(unsigned)((int64_t)rows.count * kvh), PkForm<KS>::kThreads, 0, st>>>(P);
+    });
   }
   if (!keys.count) return;
   P.splits = splits;
   P.tiles = keys.count;
-  const unsigned blocks = (unsigned)((int64_t)keys.count * kvh * splits);
-  if (keys.keywise)
-    packed_dkv_kernel<T, DP, 4, 1><<<blocks, 256, 0, st>>>(P);
-  else if (keys.tiles == 2) {
-    if constexpr (sizeof(T) == 2) packed_dkv_kernel<T, DP, 1, 2><<<blocks, 256, 0, st>>>(P);
-  } else
-    packed_dkv_kernel<T, DP, 1, 1><<<blocks, 256, 0, st>>>(P);
+  P.order = keys.order;
+  pk_form<T>(keys, [&](auto ks, auto r) {
+    constexpr int KS = decltype(ks)::value, R = decltype(r)::value;
+    if constexpr (DP * R <= 128)
+      packed_dkv_kernel<T, DP, KS, R><<<(unsigned)((int64_t)keys.count * kvh * splits), PkForm<KS>::kThreads, 0, st>>>(P);
+  });
   if (splits > 1)
     packed_dkv_join_kernel<T, DP><<<(unsigned)(((int64_t)kvh * P.tk * DP / 4 + 255) / 256), 256, 0, st>>>(P);
 }
