@@ -1308,9 +1308,10 @@ int packed_width(int64_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
 // (the last two of the forward rows sorted). `most`: tiles of a wave at most.
 PackedForm packed_form(int64_t rows, int64_t seqs, int64_t wgs, int64_t walk, int most, int64_t few) {
   PackedForm f = {};
+  f.groups = 4;
   f.tiles = 1;
   if (walk > 64 && (rows <= 16 * seqs || wgs < few))
-    f.ks = 4;
+    f.groups = 1, f.ks = 4;
   else if (walk < 320 || wgs < 128)
     f.ks = 1;
   else if (wgs < 1024 || most < 2)
@@ -1326,7 +1327,7 @@ PackedForm packed_form(int64_t rows, int64_t seqs, int64_t wgs, int64_t walk, in
 // that walk 16384 blocks of 64 and more in all (the forward pass of 5 causal sequences,
 // 8192 tokens, 85 -> 77 us with it, of 6 with 16384 254 -> 234)
 bool packed_sorted(const PackedForm& f, int64_t seqs, int64_t wgs, int64_t walk) {
-  return !f.keywise() && f.count && f.count <= kPackedOrder && seqs > 1 && wgs * walk >= (int64_t)16384 * 64;
+  return f.groups > 1 && f.count && f.count <= kPackedOrder && seqs > 1 && wgs * walk >= (int64_t)16384 * 64;
 }
 PackedPlan packed_fwd_plan(int64_t tq, int64_t tk, int64_t seqs, int64_t heads, int64_t kvh, int64_t d, int32_t dtype) {
   const int64_t group = heads / kvh, rows = tq * group, wgs = kvh * ((rows + 63) / 64), walk = tk / seqs;
@@ -1334,7 +1335,7 @@ PackedPlan packed_fwd_plan(int64_t tq, int64_t tk, int64_t seqs, int64_t heads, 
   PackedPlan p = {};
   p.rows = packed_form(rows, seqs, wgs, walk, bf ? 2 : 1, bf ? 128 : d <= 64 ? 256 : 512);
   p.splits = 1;
-  if (p.rows.keywise()) {
+  if (p.rows.groups == 1) {
     const int64_t tiles = kvh * std::max(seqs, rows / 16);
     // two blocks of 128 keys a split at least, were the lengths alike
     const int64_t want = tiles <= 128 ? std::min<int64_t>(512 / tiles, walk / 256) : 1;

@@ -24,19 +24,19 @@ constexpr float kSlack = 8.f;
 // M exactly.
 constexpr float kFar = 16777216.f;
 
-template <typename T, int DP, int KS, int R>
-__global__ __launch_bounds__(PkForm<KS>::kThreads, (PkForm<KS>::template kSimd<T, DP>)) void packed_fwd_kernel(PackedParams<T> P) {
-  typedef PkForm<KS> Form;
+template <typename T, int DP, int G, int KS, int R>
+__global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkForm<G, KS>::template kSimd<T, DP>)) void packed_fwd_kernel(PackedParams<T> P) {
+  typedef PkForm<G, KS> Form;
   typedef PkRows<T, DP> Rows;
   typedef typename Frag<T>::type F;
   constexpr int kC = Rows::kC, kU = Rows::kU;
   constexpr int kNt = Form::kOwn / 16;  // key tiles of a wave in a block
-  constexpr int kTileRows = 16 * R * Form::kGroups, kShift = __builtin_ctz(kTileRows);
+  constexpr int kTileRows = 16 * R * G, kShift = __builtin_ctz(kTileRows);
   constexpr int kOperand = Form::kStage * Rows::kRowBytes;
   constexpr int kSets = Form::kSets;
   constexpr int kStages = 4 * kOperand * kSets <= 160 * 1024 ? 2 : 1;
   constexpr int kPo = DP + 2;
-  static_assert(KS == 1 || kStages * 2 * kOperand * kSets >= 4 * 16 * R * kPo * 4 + Form::kWaves * 16 * R * 8, "the waves' sums");
+  static_assert(KS == 1 || kStages * 2 * kOperand * kSets >= kPkSumBytes<G, KS, kPo> + Form::kWaves * 16 * R * 8, "the waves' sums");
   __shared__ __attribute__((aligned(16))) unsigned char raw[kStages * 2 * kOperand * kSets];
 
   const int t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
@@ -77,7 +77,7 @@ __global__ __launch_bounds__(PkForm<KS>::kThreads, (PkForm<KS>::template kSimd<T
   const int64_t blocks = most > 0 ? (most + Form::kBlock - 1) / Form::kBlock : 0;
   const int blk0 = (int)(blocks * split / P.splits), blk1 = (int)(blocks * (split + 1) / P.splits);
 
-  unsigned char* const mine = raw + (KS == 4 ? wave * kStages * 2 * kOperand : 0);
+  unsigned char* const mine = raw + (Form::kPrivate ? wave * kStages * 2 * kOperand : 0);
   PkCopy<T, DP, Form::kStage, Form::kOwners> kcopy, vcopy;
   kcopy.init(P.k.token, P.d, form.stager, lane);
   vcopy.init(P.v.token, P.d, form.stager, lane);
@@ -85,7 +85,7 @@ __global__ __launch_bounds__(PkForm<KS>::kThreads, (PkForm<KS>::template kSimd<T
   const T* vs = P.v.p + kv * P.v.head + (int64_t)sp.k0 * P.v.token;
   auto stage = [&](int blk, int at) {
     unsigned char* s = mine + at * 2 * kOperand;
-    const int64_t key = (int64_t)blk * Form::kBlock + (KS == 4 ? Form::kOwn * form.part : 0);
+    const int64_t key = (int64_t)blk * Form::kBlock + form.staged();
     kcopy.issue(ks, key, sp.nk, P.d, s, form.stager);
     vcopy.issue(vs, key, sp.nk, P.d, s + kOperand, form.stager);
   };
@@ -109,13 +109,13 @@ __global__ __launch_bounds__(PkForm<KS>::kThreads, (PkForm<KS>::template kSimd<T
 
   if (kStages == 2) {
     if (blk0 < blk1) stage(blk0, 0);
-    pk_sync<KS>();
+    pk_sync<Form>();
   }
   for (int blk = blk0; blk < blk1; ++blk) {
     const int cur = kStages == 2 ? (blk - blk0) & 1 : 0;
     if (kStages == 1) {
       stage(blk, 0);
-      pk_sync<KS>();
+      pk_sync<Form>();
     } else if (blk + 1 < blk1) {
       stage(blk + 1, cur ^ 1);
     }
@@ -125,16 +125,14 @@ __global__ __launch_bounds__(PkForm<KS>::kThreads, (PkForm<KS>::template kSimd<T
     if (key0 < lim_hi) {
       f32x4 s[R][kNt];
 #pragma unroll
-      for (int kt = 0; kt < kNt; ++kt) {
+      for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int r = 0; r < R; ++r) s[r][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int kt = 0; kt < kNt; ++kt) s[r][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      pk_ahead<kNt * kC>([&](int i) { return at.at_row(kt_, 16 * (i / kC), i % kC); },
+                         [&](int i, const F& kf) {
 #pragma unroll
-        for (int c = 0; c < kC; ++c) {
-          const F kf = at.at_row(kt_, 16 * kt, c);
-#pragma unroll
-          for (int r = 0; r < R; ++r) mma(s[r][kt], kf, qf[r][c]);
-        }
-      }
+                           for (int r = 0; r < R; ++r) mma(s[r][i / kC], kf, qf[r][i % kC]);
+                         });
       if (key0 + 16 * kNt > lim_lo) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
@@ -196,16 +194,13 @@ __global__ __launch_bounds__(PkForm<KS>::kThreads, (PkForm<KS>::template kSimd<T
           if (kOnes) mma(l[r], ones, pf[r][c]);
         }
       }
+      pk_ahead<kNt / 2 * kU>([&](int i) { return at.at_col(vt_, 32 * (i / kU), i % kU); },
+                             [&](int i, const F& vf) {
 #pragma unroll
-      for (int c = 0; c < kNt / 2; ++c)
-#pragma unroll
-        for (int u = 0; u < kU; ++u) {
-          const F vf = at.at_col(vt_, 32 * c, u);
-#pragma unroll
-          for (int r = 0; r < R; ++r) mma(o[r][u], vf, pf[r][c]);
-        }
+                               for (int r = 0; r < R; ++r) mma(o[r][i % kU], vf, pf[r][i / kU]);
+                             });
     }
-    pk_sync<KS>();
+    pk_sync<Form>();
   }
   float ls[R];
 #pragma unroll
@@ -214,7 +209,7 @@ __global__ __launch_bounds__(PkForm<KS>::kThreads, (PkForm<KS>::template kSimd<T
   if constexpr (KS > 1) {
     // the partial rows of the waves that share them, on the largest of their maxima
     float* ml = reinterpret_cast<float*>(raw);  // [wave][row][2], then the outputs
-    auto slot = [&](int j, int r) { return ((KS == 4 ? j : 4 * j + form.group) * R + r) * 16 + li; };  // of the rows' j-th wave
+    auto slot = [&](int j, int r) { return ((j * G + form.group) * R + r) * 16 + li; };  // of the rows' j-th wave
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < R; ++r)
@@ -239,7 +234,7 @@ __global__ __launch_bounds__(PkForm<KS>::kThreads, (PkForm<KS>::template kSimd<T
       m[r] = mx;
       ls[r] = sum;
     }
-    pk_sum_waves<KS, R, kU, kPo>(ml + Form::kWaves * 16 * R * 2, form, li, lg, o);
+    pk_sum_waves<G, KS, R, kU, kPo>(ml + Form::kWaves * 16 * R * 2, form, li, lg, o);
   }
 #pragma unroll
   for (int r = 0; r < R; ++r) {
@@ -414,9 +409,9 @@ __global__ __launch_bounds__(1024) void packed_order_kernel(PackedParams<T> P, P
 template <typename T, int DP>
 void fwd(const PackedParams<T>& P, const PackedForm& form, hipStream_t st) {
   const unsigned blocks = (unsigned)((int64_t)form.count * P.splits * (P.heads / P.group));
-  pk_form<T>(form, [&](auto ks, auto r) {
-    constexpr int KS = decltype(ks)::value, R = decltype(r)::value;
-    packed_fwd_kernel<T, DP, KS, R><<<blocks, PkForm<KS>::kThreads, 0, st>>>(P);
+  pk_form<T>(form, [&](auto g, auto ks, auto r) {
+    constexpr int G = decltype(g)::value, KS = decltype(ks)::value, R = decltype(r)::value;
+    packed_fwd_kernel<T, DP, G, KS, R><<<blocks, PkForm<G, KS>::kThreads, 0, st>>>(P);
   });
   if (P.splits > 1) packed_join_kernel<T, DP><<<(unsigned)(P.heads * P.tq), 256, 0, st>>>(P);
 }

@@ -36,14 +36,12 @@ struct PackedInts {
   int wide;
 };
 
-// how a call is cut
+// how a call is cut (PkForm), 16-row tiles of a wave
 struct PackedForm {
-  int ks;       // 1, 2 or 4: how many waves share a tile (PkForm)
-  int tiles;    // 16-row tiles of a wave
-  __host__ __device__ bool keywise() const { return ks == 4; }
-  __host__ __device__ int rows() const { return ks == 4 ? 16 : 64 * tiles; }  // of a workgroup
+  int groups, ks, tiles;
   int count;    // workgroups for one key/value head
   int2* order;  // [count], to be filled with the tiles in the order of their work, or null
+  __host__ __device__ int rows() const { return 16 * groups * tiles; }  // of a workgroup
 };
 constexpr int kPackedOrder = 12288;  // tiles that are sorted at most
 
@@ -150,32 +148,34 @@ __device__ __forceinline__ bool packed_span(const PackedParams<T>& P, bool by_ke
 }
 
 // How the waves of a workgroup share its rows (for the keys' gradients: its keys) and the
-// blocks that it walks. KS 1: four waves with tiles of their own, blocks of 64 staged for
-// all; 2: eight waves, two to the same tiles, each with half of a block of 128; 4: four
-// waves that share one set of tiles, each staging 32 of a block of 128 for itself.
-template <int KS>
+// blocks that it walks: G groups of waves with tiles of their own, KS waves in each with
+// the same tiles and a KS-th of a block. Every group reads a whole block from LDS, so that
+// few groups of many rows read least. One group: its waves have staged rows of their own,
+// and need no barrier.
+template <int G, int KS>
 struct PkForm {
-  static constexpr int kWaves = KS == 2 ? 8 : 4, kThreads = 64 * kWaves;
-  static constexpr int kGroups = KS == 4 ? 1 : 4;        // of waves with the same tiles
-  static constexpr int kBlock = KS == 1 ? 64 : 128;      // of all waves
-  static constexpr int kOwn = kBlock / KS;               // of one
-  static constexpr int kStage = KS == 4 ? 32 : kBlock;   // rows staged together
-  static constexpr int kSets = KS == 4 ? 4 : 1;          // of such rows
-  static constexpr int kOwners = KS == 4 ? 1 : kWaves;   // waves that stage them
-  static constexpr int kRest = (kStage + 63) / 64;       // waves that fetch a value for each
+  static constexpr int kWaves = G * KS, kThreads = 64 * kWaves;
+  static constexpr bool kPrivate = G == 1;
+  static constexpr int kBlock = KS == 1 ? 64 : 128;             // of all waves
+  static constexpr int kOwn = kBlock / KS;                      // of one
+  static constexpr int kStage = kPrivate ? kOwn : kBlock;       // rows staged together
+  static constexpr int kSets = kPrivate ? KS : 1;               // of such rows
+  static constexpr int kOwners = kPrivate ? 1 : kWaves;         // waves that stage them
+  static constexpr int kRest = (kStage + 63) / 64;              // waves that fetch a value for each
   // waves a SIMD that the registers are held to, where a workgroup's LDS (two stages of
   // two operands) leaves room for as many
   template <typename T, int DP>
-  static constexpr int kSimd = kWaves / 4 * (sizeof(T) == 2 && 2 * 4 * kStage * kSets * DP * (int)sizeof(T) <= 150 * 1024 ? 2 : 1) >= 2
-                                   ? 2 : 1;
+  static constexpr int kSimd =
+      kWaves / 4 * (sizeof(T) == 2 && 2 * 2 * kStage * kSets * DP * (int)sizeof(T) <= 75 * 1024 ? 2 : 1) >= 2 ? 2 : 1;
   // the wave's place: its group, its part of a block, where that begins among its
   // staged rows, and as which of the owners it stages
   int group, part, at, stager;
   __device__ __forceinline__ explicit PkForm(int wave)
-      : group(KS == 4 ? 0 : wave & 3), part(KS == 1 ? 0 : KS == 2 ? wave >> 2 : wave), at(KS == 2 ? kOwn * part : 0),
-        stager(KS == 4 ? 0 : wave) {}
+      : group(wave % G), part(wave / G), at(kPrivate ? 0 : kOwn * (wave / G)), stager(kPrivate ? 0 : wave) {}
+  // the first of the wave's staged rows in a block
+  __device__ __forceinline__ int staged() const { return kPrivate ? kOwn * part : 0; }
   // which of the waves with the same rows writes column tile u, after their sums were joined
-  __device__ __forceinline__ bool writes(int u) const { return KS == 1 || (KS == 2 ? part == 0 : (u & 3) == part); }
+  __device__ __forceinline__ bool writes(int u) const { return u % KS == part; }
 };
 
 // Rows of DP elements in LDS, 16-byte piece c of row r in slot c ^ f(r) of its row.
@@ -302,12 +302,36 @@ struct PkCopy {
   }
 };
 
+// N products use(i, load(i)) whose fragments come from LDS: those of the next four are on
+// their way while four are worked on. Left to itself the compiler reads one or two ahead,
+// and a wave waits for LDS between any two products.
+template <int N, typename L, typename U>
+__device__ __forceinline__ void pk_ahead(L load, U use) {
+  typedef decltype(load(0)) F;
+  constexpr int kGroup = sizeof(F) > 16 ? 2 : 4, kGroups = (N + kGroup - 1) / kGroup;
+  F f[2][kGroup];
+#pragma unroll
+  for (int j = 0; j < kGroup; ++j)
+    if (j < N) f[0][j] = load(j);
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) {
+#pragma unroll
+    for (int j = 0; j < kGroup; ++j)
+      if (kGroup * (g + 1) + j < N) f[(g + 1) & 1][j] = load(kGroup * (g + 1) + j);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < kGroup; ++j)
+      if (kGroup * g + j < N) use(kGroup * g + j, f[g & 1][j]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
 // Behind the use of a stage and the issue of the next: what this wave has in flight is
 // complete, its fragment reads too, and where waves share stages, theirs.
-template <int KS>
+template <typename Form>
 __device__ __forceinline__ void pk_sync() {
   lds_wait<0>();
-  if constexpr (KS != 4) lds_barrier();
+  if constexpr (!Form::kPrivate) lds_barrier();
   asm volatile("" ::: "memory");
 }
 
@@ -335,35 +359,34 @@ __device__ __forceinline__ void pk_round(float by, f32x4 (&s)[NT]) {
     }
 }
 
-// The accumulators of the waves with the same rows added, through LDS (PITCH floats a
-// row): KS 2: the first of two gets them, 4: wave w the column tiles u with u % 4 == w.
-template <int KS, int R, int U, int PITCH>
-__device__ __forceinline__ void pk_sum_waves(float* lds, const PkForm<KS>& f, int li, int lg, f32x4 (&x)[R][U]) {
-  auto slot = [&](int j, int r) { return ((j * R + r) * 16 + li) * PITCH + 4 * lg; };
-  __syncthreads();
-  if (KS == 4 || f.part) {
+// The accumulators of a group's waves added, through LDS (PITCH floats a row), 16 rows of
+// each at a time; wave j of a group gets the column tiles u with u % KS == j.
+template <int G, int KS, int R, int U, int PITCH>
+__device__ __forceinline__ void pk_sum_waves(float* lds, const PkForm<G, KS>& f, int li, int lg, f32x4 (&x)[R][U]) {
+  auto slot = [&](int j) { return ((j * G + f.group) * 16 + li) * PITCH + 4 * lg; };
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+  for (int r = 0; r < R; ++r) {
+    __syncthreads();
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) lds[slot(KS == 4 ? f.part : f.group, r) + 16 * u + e] = x[r][u][e];
-  }
-  __syncthreads();
-#pragma unroll
-  for (int r = 0; r < R; ++r)
+      for (int e = 0; e < 4; ++e) lds[slot(f.part) + 16 * u + e] = x[r][u][e];
+    __syncthreads();
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (!f.writes(u)) continue;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        float a = KS == 4 ? 0.f : x[r][u][e];
+        float a = 0.f;
 #pragma unroll
-        for (int j = 0; j < (KS == 4 ? 4 : 1); ++j) a += lds[slot(KS == 4 ? j : f.group, r) + 16 * u + e];
+        for (int j = 0; j < KS; ++j) a += lds[slot(j) + 16 * u + e];
         x[r][u][e] = a;
       }
     }
+  }
 }
+template <int G, int KS, int PITCH>
+constexpr int kPkSumBytes = G * KS * 16 * PITCH * 4;
 
 // max over the 4 lanes {l % 16 + 16 g}
 __device__ __forceinline__ float lanes4_max(float x) {
@@ -376,17 +399,19 @@ __device__ __forceinline__ float lanes4_max(float x) {
   return fmaxf(__builtin_bit_cast(float, b0), __builtin_bit_cast(float, b1));
 }
 
-// f(KS, R) for a form; float32 has one tile a wave
+// f(G, KS, R) for the forms that packed_form chooses; float32 has one tile a wave
 template <typename T, typename F>
 void pk_form(const PackedForm& form, F f) {
   typedef std::integral_constant<int, 1> One;
   typedef std::integral_constant<int, 2> Two;
-  if (form.ks == 4) return f(std::integral_constant<int, 4>{}, One{});
+  typedef std::integral_constant<int, 4> Four;
+  if (form.groups == 1) return f(One{}, Four{}, One{});
   if constexpr (sizeof(T) == 2) {
-    if (form.tiles == 2) return form.ks == 2 ? f(Two{}, Two{}) : f(One{}, Two{});
+    if (form.groups == 2) return f(Two{}, Four{}, Two{});
+    if (form.tiles == 2) return form.ks == 2 ? f(Four{}, Two{}, Two{}) : f(Four{}, One{}, Two{});
   }
-  if (form.ks == 2) return f(Two{}, One{});
-  f(One{}, One{});
+  if (form.ks == 2) return f(Four{}, Two{}, One{});
+  f(Four{}, One{}, One{});
 }
 
 // the orders that `rows` and `keys` ask for

@@ -25,19 +25,19 @@ __device__ __forceinline__ float pk_weight(float s, float by, float m, float log
 }
 
 // dq, and D for the other kernel: rows and blocks as in the forward pass.
-template <typename T, int DP, int KS, int R>
-__global__ __launch_bounds__(PkForm<KS>::kThreads, (PkForm<KS>::template kSimd<T, DP>)) void packed_dq_kernel(PackedParams<T> P) {
-  typedef PkForm<KS> Form;
+template <typename T, int DP, int G, int KS, int R>
+__global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkForm<G, KS>::template kSimd<T, DP>)) void packed_dq_kernel(PackedParams<T> P) {
+  typedef PkForm<G, KS> Form;
   typedef PkRows<T, DP> Rows;
   typedef typename Frag<T>::type F;
   constexpr int kC = Rows::kC, kU = Rows::kU;
   constexpr int kNt = Form::kOwn / 16;
-  constexpr int kTileRows = 16 * R * Form::kGroups, kShift = __builtin_ctz(kTileRows);
+  constexpr int kTileRows = 16 * R * G, kShift = __builtin_ctz(kTileRows);
   constexpr int kOperand = Form::kStage * Rows::kRowBytes;
   constexpr int kSets = Form::kSets;
   constexpr int kStages = 4 * kOperand * kSets <= 160 * 1024 ? 2 : 1;
   constexpr int kPo = DP + 2;
-  static_assert(KS == 1 || kStages * 2 * kOperand * kSets >= 4 * 16 * R * kPo * 4, "the waves' sums");
+  static_assert(KS == 1 || kStages * 2 * kOperand * kSets >= kPkSumBytes<G, KS, kPo>, "the waves' sums");
   __shared__ __attribute__((aligned(16))) unsigned char raw[kStages * 2 * kOperand * kSets];
 
   const int t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
@@ -102,7 +102,7 @@ __global__ __launch_bounds__(PkForm<KS>::kThreads, (PkForm<KS>::template kSimd<T
   const int lim_hi = row_w < rows ? __builtin_amdgcn_readlane(lim[R - 1], 15) : 0;
   const int blocks = most > 0 ? (int)(((int64_t)most + Form::kBlock - 1) / Form::kBlock) : 0;
 
-  unsigned char* const mine = raw + (KS == 4 ? wave * kStages * 2 * kOperand : 0);
+  unsigned char* const mine = raw + (Form::kPrivate ? wave * kStages * 2 * kOperand : 0);
   PkCopy<T, DP, Form::kStage, Form::kOwners> kcopy, vcopy;
   kcopy.init(P.k.token, P.d, form.stager, lane);
   vcopy.init(P.v.token, P.d, form.stager, lane);
@@ -110,7 +110,7 @@ __global__ __launch_bounds__(PkForm<KS>::kThreads, (PkForm<KS>::template kSimd<T
   const T* vs = P.v.p + kv * P.v.head + (int64_t)sp.k0 * P.v.token;
   auto stage = [&](int blk, int at) {
     unsigned char* s = mine + at * 2 * kOperand;
-    const int64_t key = (int64_t)blk * Form::kBlock + (KS == 4 ? Form::kOwn * form.part : 0);
+    const int64_t key = (int64_t)blk * Form::kBlock + form.staged();
     kcopy.issue(ks, key, sp.nk, P.d, s, form.stager);
     vcopy.issue(vs, key, sp.nk, P.d, s + kOperand, form.stager);
   };
@@ -124,13 +124,13 @@ __global__ __launch_bounds__(PkForm<KS>::kThreads, (PkForm<KS>::template kSimd<T
 
   if (kStages == 2) {
     if (blocks) stage(0, 0);
-    pk_sync<KS>();
+    pk_sync<Form>();
   }
   for (int blk = 0; blk < blocks; ++blk) {
     const int cur = kStages == 2 ? blk & 1 : 0;
     if (kStages == 1) {
       stage(blk, 0);
-      pk_sync<KS>();
+      pk_sync<Form>();
     } else if (blk + 1 < blocks) {
       stage(blk + 1, cur ^ 1);
     }
@@ -143,22 +143,19 @@ __global__ __launch_bounds__(PkForm<KS>::kThreads, (PkForm<KS>::template kSimd<T
       for (int pair = 0; pair < kNt / 2; ++pair) {
         f32x4 s[R][2], dp[R][2];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int r = 0; r < R; ++r)
 #pragma unroll
-          for (int r = 0; r < R; ++r) s[r][j] = dp[r][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+          for (int j = 0; j < 2; ++j) s[r][j] = dp[r][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        pk_ahead<2 * kC>([&](int i) { return at.at_row(kt_, 32 * pair + 16 * (i / kC), i % kC); },
+                         [&](int i, const F& kf) {
 #pragma unroll
-          for (int c = 0; c < kC; ++c) {
-            const F kf = at.at_row(kt_, 32 * pair + 16 * j, c);
+                           for (int r = 0; r < R; ++r) mma(s[r][i / kC], kf, qf[r][i % kC]);
+                         });
+        pk_ahead<2 * kC>([&](int i) { return at.at_row(vt_, 32 * pair + 16 * (i / kC), i % kC); },
+                         [&](int i, const F& vf) {
 #pragma unroll
-            for (int r = 0; r < R; ++r) mma(s[r][j], kf, qf[r][c]);
-          }
-#pragma unroll
-          for (int c = 0; c < kC; ++c) {
-            const F vf = at.at_row(vt_, 32 * pair + 16 * j, c);
-#pragma unroll
-            for (int r = 0; r < R; ++r) mma(dp[r][j], vf, dof[r][c]);
-          }
-        }
+                           for (int r = 0; r < R; ++r) mma(dp[r][i / kC], vf, dof[r][i % kC]);
+                         });
         float by = P.scale_log2;
         if (far) {
           by = 1.f;
@@ -184,17 +181,16 @@ __global__ __launch_bounds__(PkForm<KS>::kThreads, (PkForm<KS>::template kSimd<T
             ds[e] = pk_weight(s[r][e >> 2][e & 3], by, m[r], log_sum[r]) * (dp[r][e >> 2][e & 3] - delta[r]);
           dsf[r] = pack8<T>(ds);
         }
+        pk_ahead<kU>([&](int u) { return at.at_col(kt_, 32 * pair, u); },
+                     [&](int u, const F& kf) {
 #pragma unroll
-        for (int u = 0; u < kU; ++u) {
-          const F kf = at.at_col(kt_, 32 * pair, u);
-#pragma unroll
-          for (int r = 0; r < R; ++r) mma(dq[r][u], kf, dsf[r]);
-        }
+                       for (int r = 0; r < R; ++r) mma(dq[r][u], kf, dsf[r]);
+                     });
       }
     }
-    pk_sync<KS>();
+    pk_sync<Form>();
   }
-  if constexpr (KS > 1) pk_sum_waves<KS, R, kU, kPo>(reinterpret_cast<float*>(raw), form, li, lg, dq);
+  if constexpr (KS > 1) pk_sum_waves<G, KS, R, kU, kPo>(reinterpret_cast<float*>(raw), form, li, lg, dq);
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     if (row_w + 16 * r + li >= rows) continue;
@@ -215,22 +211,26 @@ __global__ __launch_bounds__(PkForm<KS>::kThreads, (PkForm<KS>::template kSimd<T
 // queries of every head that shares them in tiles of 16: S = Q K^T and dP = dO V^T leave
 // the lane 4 queries of its own keys, as the operands of dV^T = dO^T P and dK^T = Q^T dS.
 // KS 1: four waves with keys of their own; 4: the waves share keys and split the queries.
-template <typename T, int DP, int KS, int R>
-__global__ __launch_bounds__(PkForm<KS>::kThreads, (PkForm<KS>::template kSimd<T, DP>)) void packed_dkv_kernel(PackedParams<T> P) {
-  typedef PkForm<KS> Form;
+template <typename T, int DP, int G, int KS, int R>
+__global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkForm<G, KS>::template kSimd<T, DP>)) void packed_dkv_kernel(PackedParams<T> P) {
+  typedef PkForm<G, KS> Form;
   typedef PkRows<T, DP> Rows;
   typedef typename Frag<T>::type F;
   constexpr int kC = Rows::kC, kU = Rows::kU;
   constexpr int kNt = Form::kOwn / 16;  // query tiles of a wave in a block
-  constexpr int kTileKeys = 16 * R * Form::kGroups, kShift = __builtin_ctz(kTileKeys);
+  constexpr int kTileKeys = 16 * R * G, kShift = __builtin_ctz(kTileKeys);
   constexpr int kOperand = Form::kStage * Rows::kRowBytes;
   constexpr int kSets = Form::kSets;
   constexpr int kStages = 4 * kOperand * kSets <= 156 * 1024 ? 2 : 1;
   constexpr int kPo = DP + 2;
-  static_assert(KS == 1 || kStages * 2 * kOperand * kSets >= 4 * 16 * R * kPo * 4, "the waves' sums");
+  static_assert(KS == 1 || kStages * 2 * kOperand * kSets >= kPkSumBytes<G, KS, kPo>, "the waves' sums");
   __shared__ __attribute__((aligned(16))) unsigned char raw[kStages * 2 * kOperand * kSets];
   __shared__ __attribute__((aligned(16))) float rowstat[kSets][kStages][3][Form::kStage];  // M, log2 of the sum, D
   __shared__ int rowfar[kSets][kStages][Form::kRest];
+  // two tiles of keys a wave at 128 channels: with their values in registers as well there
+  // would be more of them than two waves a SIMD have
+  constexpr bool kValues = DP * R > 128;
+  __shared__ __attribute__((aligned(16))) unsigned char values[kValues ? kTileKeys * Rows::kRowBytes : 16];
 
   const int t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -246,7 +246,7 @@ __global__ __launch_bounds__(PkForm<KS>::kThreads, (PkForm<KS>::template kSimd<T
   const int key_w = key0 + 16 * R * form.group;
   const int shift = sp.nq - sp.nk;  // a causal row i sees the keys up to i - shift
 
-  F kf[R][kC], vf[R][kC];
+  F kf[R][kC], vf[kValues ? 1 : R][kC];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const int key = key_w + 16 * r + li;
@@ -257,8 +257,13 @@ __global__ __launch_bounds__(PkForm<KS>::kThreads, (PkForm<KS>::template kSimd<T
     for (int c = 0; c < kC; ++c) {
       const bool in = key < sp.nk && 32 * c + 8 * lg < P.d;
       kf[r][c] = in ? load8(k + 32 * c) : F{};
-      vf[r][c] = in ? load8(v + 32 * c) : F{};
+      if constexpr (!kValues) vf[r][c] = in ? load8(v + 32 * c) : F{};
     }
+  }
+  if constexpr (kValues) {
+    PkCopy<T, DP, kTileKeys, Form::kOwners> copy;
+    copy.init(P.v.token, P.d, form.stager, lane);
+    copy.issue(P.v.p + kv * P.v.head + (int64_t)sp.k0 * P.v.token, key0, sp.nk, P.d, values, form.stager);
   }
   // the heads of this part, and the query blocks in which any row sees the first key
   const int h0 = P.group * split / P.splits, h1 = P.group * (split + 1) / P.splits;
@@ -267,9 +272,9 @@ __global__ __launch_bounds__(PkForm<KS>::kThreads, (PkForm<KS>::template kSimd<T
   const int qb1 = key0 < sp.nk ? (int)(((int64_t)sp.nq + Form::kBlock - 1) / Form::kBlock) : 0;
   const int turns = qb1 > qb0 ? (h1 - h0) * (qb1 - qb0) : 0;
 
-  const int set = KS == 4 ? wave : 0;
+  const int set = Form::kPrivate ? wave : 0;
   unsigned char* const mine = raw + set * kStages * 2 * kOperand;
-  const int stat_row = KS == 4 ? lane : t;  // of a staged block, of which the thread fetches the statistics
+  const int stat_row = Form::kPrivate ? lane : t;  // of a staged block, of which the thread fetches the statistics
   PkCopy<T, DP, Form::kStage, Form::kOwners> qcopy, ocopy;
   qcopy.init(P.q.token, P.d, form.stager, lane);
   ocopy.init(P.dout.token, P.d, form.stager, lane);
@@ -278,7 +283,7 @@ __global__ __launch_bounds__(PkForm<KS>::kThreads, (PkForm<KS>::template kSimd<T
   float st_d = 0.f;
   auto stage = [&](int at) {
     const int head = kv * P.group + next_h;
-    const int64_t row0 = (int64_t)next_b * Form::kBlock + (KS == 4 ? Form::kOwn * form.part : 0);
+    const int64_t row0 = (int64_t)next_b * Form::kBlock + form.staged();
     unsigned char* s = mine + at * 2 * kOperand;
     qcopy.issue(P.q.p + head * P.q.head + (int64_t)sp.q0 * P.q.token, row0, sp.nq, P.d, s, form.stager);
     ocopy.issue(P.dout.p + head * P.dout.head + (int64_t)sp.q0 * P.dout.token, row0, sp.nq, P.d, s + kOperand, form.stager);
@@ -316,7 +321,7 @@ __global__ __launch_bounds__(PkForm<KS>::kThreads, (PkForm<KS>::template kSimd<T
       stage(0);
       put_stats(0);
     }
-    pk_sync<KS>();
+    pk_sync<Form>();
   }
   int qb = qb0;
   for (int turn = 0; turn < turns; ++turn) {
@@ -324,7 +329,7 @@ __global__ __launch_bounds__(PkForm<KS>::kThreads, (PkForm<KS>::template kSimd<T
     if (kStages == 1) {
       stage(0);
       put_stats(0);
-      pk_sync<KS>();
+      pk_sync<Form>();
     } else if (turn + 1 < turns) {
       stage(cur ^ 1);
     }
@@ -340,40 +345,55 @@ __global__ __launch_bounds__(PkForm<KS>::kThreads, (PkForm<KS>::template kSimd<T
       const bool far = __builtin_amdgcn_readfirstlane(any_far);
 #pragma unroll
       for (int pair = 0; pair < kNt / 2; ++pair) {
-        // one tile of 16 queries after the other: the scores of both took more registers
-        // than two waves a SIMD have
+        f32x4 s[R][2], dp[R][2];
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) s[r][j] = dp[r][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        pk_ahead<2 * kC>([&](int i) { return at.at_row(qt_, 32 * pair + 16 * (i / kC), i % kC); },
+                         [&](int i, const F& qf) {
+#pragma unroll
+                           for (int r = 0; r < R; ++r) mma(s[r][i / kC], qf, kf[r][i % kC]);
+                         });
+        if constexpr (kValues) {
+#pragma unroll
+          for (int c = 0; c < kC; ++c) {
+            F vc[R];
+#pragma unroll
+            for (int r = 0; r < R; ++r) vc[r] = at.at_row(values, 16 * (R * form.group + r), c);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const F of = at.at_row(ot_, 32 * pair + 16 * j, c);
+#pragma unroll
+              for (int r = 0; r < R; ++r) mma(dp[r][j], of, vc[r]);
+            }
+          }
+        } else {
+          pk_ahead<2 * kC>([&](int i) { return at.at_row(ot_, 32 * pair + 16 * (i / kC), i % kC); },
+                           [&](int i, const F& of) {
+#pragma unroll
+                             for (int r = 0; r < R; ++r) mma(dp[r][i / kC], of, vf[r][i % kC]);
+                           });
+        }
+        float by = P.scale_log2;
+        if (far) {
+          by = 1.f;
+#pragma unroll
+          for (int r = 0; r < R; ++r) pk_round(P.scale_log2, s[r]);
+        }
+        if (masked) {
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            const int from = key_w + 16 * r + li + shift - row0 - 32 * pair - 4 * lg;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[r][j][e] = 16 * j + e >= from ? s[r][j][e] : -INFINITY;
+          }
+        }
         F pf[R], dsf[R];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          f32x4 s[R][1], dp[R];
-#pragma unroll
-          for (int r = 0; r < R; ++r) s[r][0] = dp[r] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int c = 0; c < kC; ++c) {
-            const F qf = at.at_row(qt_, 32 * pair + 16 * j, c);
-#pragma unroll
-            for (int r = 0; r < R; ++r) mma(s[r][0], qf, kf[r][c]);
-          }
-#pragma unroll
-          for (int c = 0; c < kC; ++c) {
-            const F of = at.at_row(ot_, 32 * pair + 16 * j, c);
-#pragma unroll
-            for (int r = 0; r < R; ++r) mma(dp[r], of, vf[r][c]);
-          }
-          float by = P.scale_log2;
-          if (far) {
-            by = 1.f;
-#pragma unroll
-            for (int r = 0; r < R; ++r) pk_round(P.scale_log2, s[r]);
-          }
-          if (masked) {
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-              const int from = key_w + 16 * r + li + shift - row0 - 32 * pair - 16 * j - 4 * lg;
-#pragma unroll
-              for (int e = 0; e < 4; ++e) s[r][0][e] = e >= from ? s[r][0][e] : -INFINITY;
-            }
-          }
           const int row = form.at + 32 * pair + 16 * j + 4 * lg;
           const f32x4 m4 = *reinterpret_cast<const f32x4*>(&rowstat[set][cur][0][row]);
           const f32x4 l4 = *reinterpret_cast<const f32x4*>(&rowstat[set][cur][1][row]);
@@ -382,29 +402,30 @@ __global__ __launch_bounds__(PkForm<KS>::kThreads, (PkForm<KS>::template kSimd<T
           for (int r = 0; r < R; ++r)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float p = pk_weight(s[r][0][e], by, m4[e], l4[e]);
+              const float p = pk_weight(s[r][j][e], by, m4[e], l4[e]);
               pf[r][4 * j + e] = from_f32<T>(p);
-              dsf[r][4 * j + e] = from_f32<T>(p * (dp[r][e] - d4[e]));
+              dsf[r][4 * j + e] = from_f32<T>(p * (dp[r][j][e] - d4[e]));
             }
         }
+        pk_ahead<2 * kU>([&](int i) { return at.at_col(i & 1 ? qt_ : ot_, 32 * pair, i / 2); },
+                         [&](int i, const F& f) {
 #pragma unroll
-        for (int u = 0; u < kU; ++u) {
-          const F of = at.at_col(ot_, 32 * pair, u);
-#pragma unroll
-          for (int r = 0; r < R; ++r) mma(dv[r][u], of, pf[r]);
-          const F qf = at.at_col(qt_, 32 * pair, u);
-#pragma unroll
-          for (int r = 0; r < R; ++r) mma(dk[r][u], qf, dsf[r]);
-        }
+                           for (int r = 0; r < R; ++r) {
+                             if (i & 1)
+                               mma(dk[r][i / 2], f, dsf[r]);
+                             else
+                               mma(dv[r][i / 2], f, pf[r]);
+                           }
+                         });
       }
     }
     if (++qb == qb1) qb = qb0;
     if (kStages == 2 && turn + 1 < turns) put_stats(cur ^ 1);
-    pk_sync<KS>();
+    pk_sync<Form>();
   }
   if constexpr (KS > 1) {
-    pk_sum_waves<KS, R, kU, kPo>(reinterpret_cast<float*>(raw), form, li, lg, dk);
-    pk_sum_waves<KS, R, kU, kPo>(reinterpret_cast<float*>(raw), form, li, lg, dv);
+    pk_sum_waves<G, KS, R, kU, kPo>(reinterpret_cast<float*>(raw), form, li, lg, dk);
+    pk_sum_waves<G, KS, R, kU, kPo>(reinterpret_cast<float*>(raw), form, li, lg, dv);
   }
 #pragma unroll
   for (int r = 0; r < R; ++r) {
@@ -462,19 +483,19 @@ void bwd(PackedParams<T> P, const PackedForm& rows, const PackedForm& keys, hipS
   P.tiles = rows.count;
   P.order = rows.order;
   if (rows.count) {
-    pk_form<T>(rows, [&](auto ks, auto r) {
-      constexpr int KS = decltype(ks)::value, R = decltype(r)::value;
-      packed_dq_kernel<T, DP, KS, R><<<(unsigned)((int64_t)rows.count * kvh), PkForm<KS>::kThreads, 0, st>>>(P);
+    pk_form<T>(rows, [&](auto g, auto ks, auto r) {
+      constexpr int G = decltype(g)::value, KS = decltype(ks)::value, R = decltype(r)::value;
+      packed_dq_kernel<T, DP, G, KS, R><<<(unsigned)((int64_t)rows.count * kvh), PkForm<G, KS>::kThreads, 0, st>>>(P);
     });
   }
   if (!keys.count) return;
   P.splits = splits;
   P.tiles = keys.count;
   P.order = keys.order;
-  pk_form<T>(keys, [&](auto ks, auto r) {
-    constexpr int KS = decltype(ks)::value, R = decltype(r)::value;
-    if constexpr (DP * R <= 128)
-      packed_dkv_kernel<T, DP, KS, R><<<(unsigned)((int64_t)keys.count * kvh * splits), PkForm<KS>::kThreads, 0, st>>>(P);
+  pk_form<T>(keys, [&](auto g, auto ks, auto r) {
+    constexpr int G = decltype(g)::value, KS = decltype(ks)::value, R = decltype(r)::value;
+    if constexpr (DP * R <= 128 || G == 2)
+      packed_dkv_kernel<T, DP, G, KS, R><<<(unsigned)((int64_t)keys.count * kvh * splits), PkForm<G, KS>::kThreads, 0, st>>>(P);
   });
   if (splits > 1)
     packed_dkv_join_kernel<T, DP><<<(unsigned)(((int64_t)kvh * P.tk * DP / 4 + 255) / 256), 256, 0, st>>>(P);
