@@ -1346,7 +1346,7 @@ PackedPlan packed_fwd_plan(int64_t tq, int64_t tk, int64_t seqs, int64_t heads, 
       p.part_ml = align_up(r * 2 * sizeof(float));
     }
   }
-  if (packed_sorted(p.rows, seqs, wgs, walk)) p.rows_order = align_up((size_t)p.rows.count * sizeof(int2));
+  if (packed_sorted(p.rows, seqs, wgs, walk)) p.rows_order = align_up((size_t)p.rows.count * sizeof(PackedTile));
   return p;
 }
 PackedPlan packed_bwd_plan(int64_t tq, int64_t tk, int64_t seqs, int64_t heads, int64_t kvh, int64_t d, int32_t dtype) {
@@ -1362,8 +1362,8 @@ PackedPlan packed_bwd_plan(int64_t tq, int64_t tk, int64_t seqs, int64_t heads, 
   if (tk) p.keys = packed_form(tk, seqs, key_wgs * p.splits, tq / seqs, bf && d <= 64 ? 2 : 1, bf ? 128 : 256);
   if (p.splits > 1) p.part_o = align_up((size_t)p.splits * kvh * tk * packed_width(d) * sizeof(float));
   p.part_ml = align_up((size_t)heads * tq * sizeof(float));
-  if (packed_sorted(p.rows, seqs, wgs, walk)) p.rows_order = align_up((size_t)p.rows.count * sizeof(int2));
-  if (packed_sorted(p.keys, seqs, key_wgs * group, tq / seqs)) p.keys_order = align_up((size_t)p.keys.count * sizeof(int2));
+  if (packed_sorted(p.rows, seqs, wgs, walk)) p.rows_order = align_up((size_t)p.rows.count * sizeof(PackedTile));
+  if (packed_sorted(p.keys, seqs, key_wgs * group, tq / seqs)) p.keys_order = align_up((size_t)p.keys.count * sizeof(PackedTile));
   return p;
 }
 
@@ -1434,6 +1434,7 @@ PackedParams<T> packed_params(const fjx_packed_attention_args* a) {
   p.seqs = (int)a->sequences;
   p.heads = (int)a->heads;
   p.group = (int)(a->heads / a->kv_heads);
+  p.group_inv = (1u << 21) / p.group + 1;
   p.d = (int)a->head_dim;
   p.scale = a->scale;
   p.scale_log2 = a->scale * kLog2e;
@@ -1453,7 +1454,7 @@ int packed_fwd_run(const fjx_packed_attention_args* a, const PackedPlan& plan, h
   p.part_o = at<float>(a->workspace, 0);
   p.part_ml = at<float>(a->workspace, plan.part_o);
   PackedForm form = plan.rows;
-  p.order = form.order = plan.rows_order ? at<int2>(a->workspace, plan.part_o + plan.part_ml) : nullptr;
+  p.order = form.order = plan.rows_order ? at<PackedTile>(a->workspace, plan.part_o + plan.part_ml) : nullptr;
   return timed(K_PACKED_ATTENTION_FWD, st, "packed_attention_fwd", [&] { launch_packed_fwd<T>(p, form, st); });
 }
 
@@ -1478,8 +1479,8 @@ int packed_bwd_run(const fjx_packed_attention_bwd_args* b, const PackedPlan& pla
   p.delta = at<float>(a->workspace, 2 * plan.part_o);
   PackedForm rows = plan.rows, keys = plan.keys;
   const size_t end = 2 * plan.part_o + plan.part_ml;
-  rows.order = plan.rows_order ? at<int2>(a->workspace, end) : nullptr;
-  keys.order = plan.keys_order ? at<int2>(a->workspace, end + plan.rows_order) : nullptr;
+  rows.order = plan.rows_order ? at<PackedTile>(a->workspace, end) : nullptr;
+  keys.order = plan.keys_order ? at<PackedTile>(a->workspace, end + plan.rows_order) : nullptr;
   return timed(K_PACKED_ATTENTION_BWD, st, "packed_attention_bwd", [&] { launch_packed_bwd<T>(p, rows, keys, st); });
 }
 

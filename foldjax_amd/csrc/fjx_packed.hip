@@ -25,8 +25,8 @@ constexpr float kSlack = 8.f;
 constexpr float kFar = 16777216.f;
 
 template <typename T, int DP, int G, int KS, int R>
-__global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkForm<G, KS>::template kSimd<T, DP>)) void packed_fwd_kernel(PackedParams<T> P) {
-  typedef PkForm<G, KS> Form;
+__global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkFormOf<T, DP, G, KS>::type::template kSimd<T, DP>)) void packed_fwd_kernel(PackedParams<T> P) {
+  typedef typename PkFormOf<T, DP, G, KS>::type Form;
   typedef PkRows<T, DP> Rows;
   typedef typename Frag<T>::type F;
   constexpr int kC = Rows::kC, kU = Rows::kU;
@@ -35,59 +35,64 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkForm<G, KS>::template
   constexpr int kOperand = Form::kStage * Rows::kRowBytes;
   constexpr int kSets = Form::kSets;
   constexpr int kStages = 4 * kOperand * kSets <= 160 * 1024 ? 2 : 1;
-  constexpr int kPo = DP + 2;
-  static_assert(KS == 1 || kStages * 2 * kOperand * kSets >= kPkSumBytes<G, KS, kPo> + Form::kWaves * 16 * R * 8, "the waves' sums");
-  __shared__ __attribute__((aligned(16))) unsigned char raw[kStages * 2 * kOperand * kSets];
+  typedef PkOut<Form, DP> Out;
+  constexpr int kRaw = kStages * 2 * kOperand * kSets;  // and at the end the outputs' way
+  __shared__ __attribute__((aligned(16))) unsigned char raw[kRaw > Out::kBytes ? kRaw : Out::kBytes];
+  __shared__ f32x2 wave_ml[R][KS][16 * G];  // maxima and sums
+  __shared__ int2 places[R][16 * G];        // the rows' heads and tokens; head -1: no such row
 
   const int t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const Form form(wave);
-  const int kvh = P.heads / P.group;
-  const int kv = blockIdx.x % kvh;
-  const uint32_t rest_id = blockIdx.x / kvh;
-  const int split = rest_id / (uint32_t)P.tiles;
+  const int kv = blockIdx.x, split = blockIdx.z;
   // without an order of their work, from the last tile on: causal rows with the most keys first
-  const int nth = rest_id % (uint32_t)P.tiles, tile_id = P.order ? nth : P.tiles - 1 - nth;
-  PackedSpan sp;
-  if (!packed_span(P, false, P.group, kShift, tile_id, lane, sp)) return;
+  const int nth = P.tile0 + blockIdx.y;
+  PackedTile sp;
+  if (!packed_tile(P, false, P.group, kShift, P.order ? nth : P.tiles - 1 - nth, lane, sp)) return;
   if (sp.seq == P.seqs && !P.zero_tail) return;
-  const int rows = sp.nq * P.group;
-  const int row0 = sp.tile * kTileRows;
-  if (row0 >= rows) return;
-  const int row_w = row0 + 16 * R * form.group;
+  const int row0 = sp.tile * kTileRows, rows = sp.nq * P.group - row0;  // those from row0 on
+  if (rows <= 0) return;
+  const int row_w = 16 * R * form.group;
+  const PackedRows place(P, row0);
 
   // of the lane's rows: head, token, and the keys that it sees: those before lim
-  int head[R], token[R], lim[R];
+  int lim[R];
   F qf[R][kC];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const int row = row_w + 16 * r + li < rows ? row_w + 16 * r + li : rows - 1;
-    const int qi = row / P.group;
-    head[r] = kv * P.group + row - qi * P.group;
-    token[r] = sp.q0 + qi;
+    const int x = row_w + 16 * r + li;
+    int qi, head;
+    place.at(x < rows ? x : rows - 1, qi, head);
+    head += kv * P.group;
     lim[r] = P.causal ? qi + sp.nk - sp.nq + 1 : sp.nk;
-    const T* q = P.q.p + head[r] * P.q.head + token[r] * P.q.token + 8 * lg;
+    if (lg == 0 && form.part == 0) places[r][16 * form.group + li] = make_int2(x < rows ? head : -1, sp.q0 + qi);
+    const T* q = P.q.p + head * P.q.head + (int64_t)(sp.q0 + qi) * P.q.token + 8 * lg;
 #pragma unroll
     for (int c = 0; c < kC; ++c) qf[r][c] = 32 * c + 8 * lg < P.d ? load8(q + 32 * c) : F{};
   }
-  const int last = (row0 + kTileRows < rows ? row0 + kTileRows : rows) - 1;
-  const int most = P.causal ? last / P.group + sp.nk - sp.nq + 1 : sp.nk;  // keys that the workgroup's rows see
-  const int lim_lo = __builtin_amdgcn_readfirstlane(lim[0]);               // that all of the wave's rows see,
+  int q_last, h_last;
+  place.at((kTileRows < rows ? kTileRows : rows) - 1, q_last, h_last);
+  const int most = P.causal ? q_last + sp.nk - sp.nq + 1 : sp.nk;  // keys that the workgroup's rows see
+  const int lim_lo = __builtin_amdgcn_readfirstlane(lim[0]);      // that all of the wave's rows see,
   const int lim_hi = row_w < rows ? __builtin_amdgcn_readlane(lim[R - 1], 15) : 0;  // and that any does
-  const int64_t blocks = most > 0 ? (most + Form::kBlock - 1) / Form::kBlock : 0;
-  const int blk0 = (int)(blocks * split / P.splits), blk1 = (int)(blocks * (split + 1) / P.splits);
+  const int blocks = most > 0 ? (int)((uint32_t)(most + Form::kBlock - 1) / Form::kBlock) : 0;
+  int blk0 = 0, blk1 = blocks;
+  if (P.splits > 1) {
+    const int each = (blocks + P.splits - 1) / P.splits;
+    blk0 = split * each < blocks ? split * each : blocks;
+    blk1 = blk0 + each < blocks ? blk0 + each : blocks;
+  }
 
   unsigned char* const mine = raw + (Form::kPrivate ? wave * kStages * 2 * kOperand : 0);
   PkCopy<T, DP, Form::kStage, Form::kOwners> kcopy, vcopy;
   kcopy.init(P.k.token, P.d, form.stager, lane);
   vcopy.init(P.v.token, P.d, form.stager, lane);
-  const T* ks = P.k.p + kv * P.k.head + (int64_t)sp.k0 * P.k.token;
-  const T* vs = P.v.p + kv * P.v.head + (int64_t)sp.k0 * P.v.token;
-  auto stage = [&](int blk, int at) {
+  kcopy.begin(P.k.p + kv * P.k.head + (int64_t)sp.k0 * P.k.token, blk0 * Form::kBlock + form.staged(), sp.nk);
+  vcopy.begin(P.v.p + kv * P.v.head + (int64_t)sp.k0 * P.v.token, blk0 * Form::kBlock + form.staged(), sp.nk);
+  auto stage = [&](int at) {  // the next block
     unsigned char* s = mine + at * 2 * kOperand;
-    const int64_t key = (int64_t)blk * Form::kBlock + form.staged();
-    kcopy.issue(ks, key, sp.nk, P.d, s, form.stager);
-    vcopy.issue(vs, key, sp.nk, P.d, s + kOperand, form.stager);
+    kcopy.issue(s, form.stager, Form::kBlock);
+    vcopy.issue(s + kOperand, form.stager, Form::kBlock);
   };
   PkLane<T, DP> at;
   at.init(lane);
@@ -108,16 +113,16 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkForm<G, KS>::template
   bool far = false;
 
   if (kStages == 2) {
-    if (blk0 < blk1) stage(blk0, 0);
+    if (blk0 < blk1) stage(0);
     pk_sync<Form>();
   }
   for (int blk = blk0; blk < blk1; ++blk) {
     const int cur = kStages == 2 ? (blk - blk0) & 1 : 0;
     if (kStages == 1) {
-      stage(blk, 0);
+      stage(0);
       pk_sync<Form>();
     } else if (blk + 1 < blk1) {
-      stage(blk + 1, cur ^ 1);
+      stage(cur ^ 1);
     }
     const unsigned char* kt_ = mine + cur * 2 * kOperand + form.at * Rows::kRowBytes;
     const unsigned char* vt_ = kt_ + kOperand;
@@ -202,73 +207,50 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkForm<G, KS>::template
     }
     pk_sync<Form>();
   }
-  float ls[R];
 #pragma unroll
-  for (int r = 0; r < R; ++r) ls[r] = kOnes ? l[r][0] : group_sum((l[r][0] + l[r][1]) + (l[r][2] + l[r][3]));
-
-  if constexpr (KS > 1) {
-    // the partial rows of the waves that share them, on the largest of their maxima
-    float* ml = reinterpret_cast<float*>(raw);  // [wave][row][2], then the outputs
-    auto slot = [&](int j, int r) { return ((j * G + form.group) * R + r) * 16 + li; };  // of the rows' j-th wave
-    __syncthreads();
+  for (int r = 0; r < R; ++r)
+    if (lg == 0 || !kOnes) {
+      const float sum = kOnes ? l[r][0] : group_sum((l[r][0] + l[r][1]) + (l[r][2] + l[r][3]));
+      if (lg == 0) wave_ml[r][form.part][16 * form.group + li] = f32x2{m[r], sum};
+    }
+  // rows come together on the largest of their waves' maxima
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-      if (lg == 0) {
-        ml[slot(form.part, r) * 2] = m[r];
-        ml[slot(form.part, r) * 2 + 1] = ls[r];
-      }
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
+  for (int r = 0; r < R; ++r)
+    Out::write(raw, form, t, o[r], [&](int row, int c, const float* x) {
+      const int2 to = places[r][row];
+      if (to.x < 0) return;
       float mx = -INFINITY, sum = 0.f;
 #pragma unroll
-      for (int j = 0; j < KS; ++j) mx = fmaxf(mx, ml[slot(j, r) * 2]);
-      const float base = pk_base(mx);
+      for (int j = 0; j < KS; ++j) mx = fmaxf(mx, wave_ml[r][j][row][0]);
+      f32x8 v = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < KS; ++j) sum = fmaf(ml[slot(j, r) * 2 + 1], __builtin_amdgcn_exp2f(ml[slot(j, r) * 2] - base), sum);
-      const float alpha = __builtin_amdgcn_exp2f(m[r] - base);
+      for (int j = 0; j < KS; ++j) {
+        const f32x2 ml = wave_ml[r][j][row];
+        const float w = __builtin_amdgcn_exp2f(ml[0] - pk_base(mx));
+        const f32x8 y = load8(x + j * Out::kPart);
+        sum = fmaf(ml[1], w, sum);
 #pragma unroll
-      for (int u = 0; u < kU; ++u)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[r][u][e] *= alpha;
-      m[r] = mx;
-      ls[r] = sum;
-    }
-    pk_sum_waves<G, KS, R, kU, kPo>(ml + Form::kWaves * 16 * R * 2, form, li, lg, o);
-  }
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    if (row_w + 16 * r + li >= rows) continue;
-    const int64_t at_row = (int64_t)head[r] * P.tq + token[r];
-    const bool first = lg == 0 && form.part == 0;
-    if (P.splits > 1) {
-      const int64_t base = (int64_t)split * P.heads * P.tq + at_row;
-      if (first) *reinterpret_cast<f32x2*>(P.part_ml + base * 2) = f32x2{m[r], ls[r]};
-#pragma unroll
-      for (int u = 0; u < kU; ++u)
-        if (form.writes(u)) *reinterpret_cast<f32x4*>(P.part_o + base * DP + 16 * u + 4 * lg) = o[r][u];
-      continue;
-    }
-    if (first && P.lse) *reinterpret_cast<f32x2*>(P.lse + at_row * 2) = pk_stats(m[r], ls[r]);
-    const float inv = ls[r] == 0.f ? 0.f : 1.f / ls[r];  // a row without keys is zeros
-    T* out = P.out.p + head[r] * P.out.head + token[r] * P.out.token;
-    T* rest = P.rest.p + head[r] * P.rest.head + token[r] * P.rest.token;
-#pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      if (!form.writes(u)) continue;
-      const int col = 16 * u + 4 * lg;
-      if (col >= P.d) continue;
-      float v[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = o[r][u][e] * inv;
-      store4f(out + col, v);
-      if (P.rest.p) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] -= round_to<T>(v[e]);
-        store4f(rest + col, v);
+        for (int e = 0; e < 8; ++e) v[e] = fmaf(y[e], w, v[e]);
       }
-    }
-  }
+      const int64_t at_row = (int64_t)to.x * P.tq + to.y;
+      if (P.splits > 1) {
+        const int64_t part = (int64_t)split * P.heads * P.tq + at_row;
+        if (c == 0) *reinterpret_cast<f32x2*>(P.part_ml + part * 2) = f32x2{mx, sum};
+        store8(P.part_o + part * DP + c, v);
+        return;
+      }
+      if (c == 0 && P.lse) *reinterpret_cast<f32x2*>(P.lse + at_row * 2) = pk_stats(mx, sum);
+      if (c >= P.d) return;
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row without keys is zeros
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = v[e] * inv;
+      store8(P.out.p + to.x * P.out.head + to.y * P.out.token + c, pack8<T>(y));
+      if (!P.rest.p) return;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] -= round_to<T>(y[e]);
+      store8(P.rest.p + to.x * P.rest.head + to.y * P.rest.token + c, pack8<T>(y));
+    });
 }
 
 // The splits of a row joined: a workgroup a row, wave w taking every fourth split
@@ -333,7 +315,7 @@ __global__ __launch_bounds__(1024) void packed_order_kernel(PackedParams<T> P, P
   // a workgroup for each order that is asked for
   const bool by_keys = !by_rows.order || blockIdx.x;
   const PackedForm form = by_keys ? of_keys : by_rows;
-  int2* const order = form.order;
+  PackedTile* const order = form.order;
   const int count = form.count, shift = __builtin_ctz(form.rows());
   constexpr int kClasses = 256;
   __shared__ int work[kPackedOrder], seqs[kPackedOrder];
@@ -346,6 +328,17 @@ __global__ __launch_bounds__(1024) void packed_order_kernel(PackedParams<T> P, P
   const int64_t tokens = by_keys ? P.tk : P.tq;
   const int per = by_keys ? 1 : P.group;
   auto first = [&](int s) { return (int)((packed_start(starts, s, tokens) * per) >> shift) + s; };
+  auto tile_of = [&](int i, int seq) {
+    PackedTile s;
+    const int next = seq < P.seqs ? seq + 1 : seq;
+    s.seq = seq;
+    s.tile = i - first(seq);
+    s.pad = 0;
+    packed_tokens(P, by_keys, (int)packed_start(P.q_starts, seq, P.tq), (int)packed_start(P.q_starts, next, P.tq),
+                  (int)packed_start(P.k_starts, seq, P.tk), (int)packed_start(P.k_starts, next, P.tk),
+                  P.k_lengths.p && seq < P.seqs ? (int)packed_int(P.k_lengths, seq, P.tk) : 0x7fffffff, s);
+    return s;
+  };
   for (int i = t; i < count; i += 1024) {
     int lo = 0, hi = P.seqs + 1;  // the last s whose first tile is not behind i
     while (hi - lo > 1) {
@@ -355,10 +348,7 @@ __global__ __launch_bounds__(1024) void packed_order_kernel(PackedParams<T> P, P
       else
         hi = mid;
     }
-    PackedSpan s;
-    s.seq = lo;
-    s.tile = i - first(lo);
-    packed_sequence(P, by_keys, s);
+    const PackedTile s = tile_of(i, lo);
     const int64_t row0 = (int64_t)s.tile << shift, rows = by_keys ? s.cap : (int64_t)s.nq * P.group;
     int blocks = -1;
     if (s.tile >= 0 && row0 < rows && (s.seq < P.seqs || P.zero_tail)) {
@@ -402,16 +392,17 @@ __global__ __launch_bounds__(1024) void packed_order_kernel(PackedParams<T> P, P
   }
   __syncthreads();
   for (int i = t; i < count; i += 1024)
-    if (work[i] >= 0) order[atomicAdd(&classes[class_of(work[i])], 1)] = make_int2(seqs[i], i - first(seqs[i]));
-  for (int i = most + t; i < count; i += 1024) order[i] = make_int2(-1, 0);
+    if (work[i] >= 0) order[atomicAdd(&classes[class_of(work[i])], 1)] = tile_of(i, seqs[i]);
+  for (int i = most + t; i < count; i += 1024) order[i].seq = -1;
 }
 
 template <typename T, int DP>
 void fwd(const PackedParams<T>& P, const PackedForm& form, hipStream_t st) {
-  const unsigned blocks = (unsigned)((int64_t)form.count * P.splits * (P.heads / P.group));
   pk_form<T>(form, [&](auto g, auto ks, auto r) {
     constexpr int G = decltype(g)::value, KS = decltype(ks)::value, R = decltype(r)::value;
-    packed_fwd_kernel<T, DP, G, KS, R><<<blocks, PkForm<G, KS>::kThreads, 0, st>>>(P);
+    pk_grid(P, [&](const PackedParams<T>& Q, dim3 grid) {
+      packed_fwd_kernel<T, DP, G, KS, R><<<grid, PkForm<G, KS>::kThreads, 0, st>>>(Q);
+    });
   });
   if (P.splits > 1) packed_join_kernel<T, DP><<<(unsigned)(P.heads * P.tq), 256, 0, st>>>(P);
 }

@@ -36,15 +36,21 @@ struct PackedInts {
   int wide;
 };
 
+constexpr int kPackedOrder = 12288;  // tiles that are sorted at most
+
+// a tile of a sequence: first query, queries, first key, keys, and keys with the unused
+// ones behind them. Sequence `seqs`: the rows behind the last one
+struct alignas(16) PackedTile {
+  int seq, tile, q0, nq, k0, nk, cap, pad;
+};
+
 // how a call is cut (PkForm), 16-row tiles of a wave
 struct PackedForm {
   int groups, ks, tiles;
-  int count;    // workgroups for one key/value head
-  int2* order;  // [count], to be filled with the tiles in the order of their work, or null
+  int count;          // tiles for one key/value head
+  PackedTile* order;  // [count], to be filled with the tiles in the order of their work, or null
   __host__ __device__ int rows() const { return 16 * groups * tiles; }  // of a workgroup
 };
-constexpr int kPackedOrder = 12288;  // tiles that are sorted at most
-
 template <typename T>
 struct PackedParams {
   PackedView<const T> q, k, v;  // [H][tq][d], [Hk][tk][d], [Hk][tk][d]
@@ -54,11 +60,13 @@ struct PackedParams {
   PackedInts q_starts, k_starts, k_lengths;  // [seqs + 1], [seqs + 1], [seqs] or null
   int64_t tq, tk;
   int seqs, heads, group, d;
+  uint32_t group_inv;           // x / group = (x group_inv) >> 21 for x < group + 128
   float scale, scale_log2;      // scale_log2: times log2(e)
   int causal;
   int zero_tail;                // rows of no sequence are written as zeros
   int tiles;                    // of a launch, for one key/value head
-  const int2* order;            // [tiles] {sequence, its tile}, those with the most work first; or null
+  const PackedTile* order;      // [tiles], those with the most work first; or null
+  int tile0;                    // the first tile of this launch
   // keys (dk, dv: the group's heads) over several workgroups, whose sums a second kernel joins
   int splits;
   float* part_o;                // [splits][H][tq][DP]
@@ -80,83 +88,108 @@ __device__ __forceinline__ int64_t packed_start(const PackedInts& a, int s, int6
   return s == 0 ? 0 : packed_int(a, s, tokens);
 }
 
-struct PackedSpan {
-  int seq;         // seqs: the rows behind the last sequence
-  int tile;        // of the sequence
-  int q0, nq, k0, nk, cap;  // first query, queries, first key, keys, and keys with the unused ones behind them
-};
+// the sequence's tokens, from its offsets as they are
+template <typename T>
+__device__ __forceinline__ void packed_tokens(const PackedParams<T>& P, bool by_keys, int q0, int q1, int k0, int k1, int length,
+                                              PackedTile& s) {
+  const bool real = s.seq < P.seqs;
+  if (!real) q1 = (int)P.tq, k1 = (int)P.tk;
+  s.q0 = q0;
+  s.nq = (real || !by_keys) && q1 > q0 ? q1 - q0 : 0;
+  s.k0 = k0;
+  s.cap = k1 > k0 ? k1 - k0 : 0;
+  s.nk = !real ? 0 : length < s.cap ? length : s.cap;
+}
 
-// The sequence of `tile` among tiles of 2^shift rows of which a token has `per`,
-// counted over a's offsets: 64 probes at a time. False for a tile past the last.
-__device__ __forceinline__ bool packed_find(const PackedInts& a, int seqs, int64_t tokens, int per, int shift, int tile,
-                                            int lane, int& seq, int& at) {
-  auto first = [&](int s) { return (int)((packed_start(a, s, tokens) * per) >> shift) + s; };
-  int lo = 0, n = seqs + 1;  // the last s of [lo, lo + n) whose first tile is not behind `tile`; s = 0 starts at 0
+// The sequence of tile `at` among tiles of 2^shift rows of which a token has `per`
+// (by_keys: of keys). False for a tile past the last. For up to 63 sequences a lane has
+// the offsets of one, and one trip to memory tells all there is to know.
+template <typename T>
+__device__ __forceinline__ bool packed_find(const PackedParams<T>& P, bool by_keys, int per, int shift, int at, int lane,
+                                            PackedTile& s) {
+  const PackedInts& own = by_keys ? P.k_starts : P.q_starts;
+  const int64_t tokens = by_keys ? P.tk : P.tq;
+  auto first = [&](int64_t start, int seq) { return (int)((start * per) >> shift) + seq; };
+  if (P.seqs < 64) {
+    const int i = lane < P.seqs ? lane : P.seqs;
+    const int qv = (int)packed_start(P.q_starts, i, P.tq), kv = (int)packed_start(P.k_starts, i, P.tk);
+    const int lv = P.k_lengths.p ? (int)packed_int(P.k_lengths, lane < P.seqs ? lane : 0, P.tk) : 0x7fffffff;
+    const int f = first(by_keys ? kv : qv, i);
+    const uint64_t votes = __builtin_amdgcn_ballot_w64(lane <= P.seqs && f <= at);
+    // offsets that descend leave votes behind a gap: the first run counts
+    const int run = (int)__builtin_ctzll(~votes);
+    const int seq = run > 0 ? run - 1 : 0, next = seq < P.seqs ? seq + 1 : seq;
+    s.seq = seq;
+    s.tile = at - __builtin_amdgcn_readlane(f, seq);
+    packed_tokens(P, by_keys, __builtin_amdgcn_readlane(qv, seq), __builtin_amdgcn_readlane(qv, next),
+                  __builtin_amdgcn_readlane(kv, seq), __builtin_amdgcn_readlane(kv, next), __builtin_amdgcn_readlane(lv, seq), s);
+    return s.tile >= 0;
+  }
+  int lo = 0, n = P.seqs + 1;  // the last s of [lo, lo + n) whose first tile is not behind `at`; s = 0 starts at 0
   while (n > 1) {
     const int step = (n + 63) / 64;
-    const int s = lo + lane * step;
-    const bool in = lane * step < n && first(s) <= tile;
+    const int seq = lo + lane * step;
+    const bool in = lane * step < n && first(packed_start(own, seq, tokens), seq) <= at;
     const uint64_t votes = __builtin_amdgcn_ballot_w64(in);
-    // offsets that descend leave votes behind a gap: the first run counts
     const int run = votes == ~0ull ? 64 : (int)__builtin_ctzll(~votes);
     const int hop = run > 0 ? run - 1 : 0;
     lo += hop * step;
     n = n - hop * step < step ? n - hop * step : step;
   }
-  seq = __builtin_amdgcn_readfirstlane(lo);
-  at = tile - __builtin_amdgcn_readfirstlane(first(seq));
-  return at >= 0;
-}
-
-// what there is of sequence s.seq
-template <typename T>
-__device__ __forceinline__ void packed_sequence(const PackedParams<T>& P, bool by_keys, PackedSpan& s) {
-  const int64_t q0 = packed_start(P.q_starts, s.seq, P.tq), k0 = packed_start(P.k_starts, s.seq, P.tk);
-  int64_t q1 = P.tq, k1 = P.tk, nk = 0;
-  if (s.seq < P.seqs) {
-    q1 = packed_int(P.q_starts, s.seq + 1, P.tq);
-    k1 = packed_int(P.k_starts, s.seq + 1, P.tk);
-    if (k1 < k0) k1 = k0;
-    nk = P.k_lengths.p ? packed_int(P.k_lengths, s.seq, k1 - k0) : k1 - k0;
-  }
-  s.q0 = (int)q0;
-  s.nq = s.seq < P.seqs || !by_keys ? (int)(q1 > q0 ? q1 - q0 : 0) : 0;
-  s.k0 = (int)k0;
-  s.nk = (int)nk;
-  s.cap = (int)(k1 > k0 ? k1 - k0 : 0);
+  s.seq = __builtin_amdgcn_readfirstlane(lo);
+  const int next = s.seq < P.seqs ? s.seq + 1 : s.seq;
+  const int q0 = (int)packed_start(P.q_starts, s.seq, P.tq), k0 = (int)packed_start(P.k_starts, s.seq, P.tk);
+  s.tile = at - __builtin_amdgcn_readfirstlane(first(by_keys ? k0 : q0, s.seq));
+  packed_tokens(P, by_keys, __builtin_amdgcn_readfirstlane(q0),
+                __builtin_amdgcn_readfirstlane((int)packed_start(P.q_starts, next, P.tq)), __builtin_amdgcn_readfirstlane(k0),
+                __builtin_amdgcn_readfirstlane((int)packed_start(P.k_starts, next, P.tk)),
+                P.k_lengths.p && s.seq < P.seqs ? __builtin_amdgcn_readfirstlane((int)packed_int(P.k_lengths, s.seq, P.tk)) : 0x7fffffff,
+                s);
+  return s.tile >= 0;
 }
 
 // the sequence and the tile of a workgroup, the `at`-th of a key/value head
 template <typename T>
-__device__ __forceinline__ bool packed_span(const PackedParams<T>& P, bool by_keys, int per, int shift, int at, int lane,
-                                            PackedSpan& s) {
-  if (P.order) {
-    const int2 o = P.order[at];
-    s.seq = __builtin_amdgcn_readfirstlane(o.x);
-    s.tile = __builtin_amdgcn_readfirstlane(o.y);
-    if (s.seq < 0) return false;
-  } else if (!packed_find(by_keys ? P.k_starts : P.q_starts, P.seqs, by_keys ? P.tk : P.tq, per, shift, at, lane, s.seq, s.tile)) {
-    return false;
-  }
-  packed_sequence(P, by_keys, s);
-  s.q0 = __builtin_amdgcn_readfirstlane(s.q0);
-  s.nq = __builtin_amdgcn_readfirstlane(s.nq);
-  s.k0 = __builtin_amdgcn_readfirstlane(s.k0);
-  s.nk = __builtin_amdgcn_readfirstlane(s.nk);
-  s.cap = __builtin_amdgcn_readfirstlane(s.cap);
-  return true;
+__device__ __forceinline__ bool packed_tile(const PackedParams<T>& P, bool by_keys, int per, int shift, int at, int lane,
+                                            PackedTile& s) {
+  if (!P.order) return packed_find(P, by_keys, per, shift, at, lane, s);
+  const PackedTile o = P.order[at];
+  s.seq = __builtin_amdgcn_readfirstlane(o.seq);
+  s.tile = __builtin_amdgcn_readfirstlane(o.tile);
+  s.q0 = __builtin_amdgcn_readfirstlane(o.q0);
+  s.nq = __builtin_amdgcn_readfirstlane(o.nq);
+  s.k0 = __builtin_amdgcn_readfirstlane(o.k0);
+  s.nk = __builtin_amdgcn_readfirstlane(o.nk);
+  s.cap = __builtin_amdgcn_readfirstlane(o.cap);
+  return s.seq >= 0;
 }
+
+// A workgroup's rows from row0 on: query and head (of the group) of its x-th. One
+// division for them all; those of a lane by a product (group_inv).
+struct PackedRows {
+  int query, rest, group;
+  uint32_t inv;
+  template <typename T>
+  __device__ __forceinline__ PackedRows(const PackedParams<T>& P, int row0) : group(P.group), inv(P.group_inv) {
+    query = row0 / group;
+    rest = row0 - query * group;
+  }
+  __device__ __forceinline__ void at(int x, int& q, int& head) const {
+    const uint32_t y = rest + x, n = (y * inv) >> 21;
+    q = query + n;
+    head = y - n * group;
+  }
+};
 
 // How the waves of a workgroup share its rows (for the keys' gradients: its keys) and the
 // blocks that it walks: G groups of waves with tiles of their own, KS waves in each with
-// the same tiles and a KS-th of a block. Every group reads a whole block from LDS, so that
-// few groups of many rows read least. One group: its waves have staged rows of their own,
-// and need no barrier.
-template <int G, int KS>
+// the same tiles and a KS-th of a block. One group: its waves have staged rows of their own, and
+// need no barrier.
+template <int G, int KS, int BLOCK = KS == 1 ? 64 : 128>
 struct PkForm {
-  static constexpr int kWaves = G * KS, kThreads = 64 * kWaves;
+  static constexpr int kG = G, kKS = KS, kWaves = G * KS, kThreads = 64 * kWaves;
   static constexpr bool kPrivate = G == 1;
-  static constexpr int kBlock = KS == 1 ? 64 : 128;             // of all waves
+  static constexpr int kBlock = BLOCK;                          // of all waves
   static constexpr int kOwn = kBlock / KS;                      // of one
   static constexpr int kStage = kPrivate ? kOwn : kBlock;       // rows staged together
   static constexpr int kSets = kPrivate ? KS : 1;               // of such rows
@@ -174,8 +207,19 @@ struct PkForm {
       : group(wave % G), part(wave / G), at(kPrivate ? 0 : kOwn * (wave / G)), stager(kPrivate ? 0 : wave) {}
   // the first of the wave's staged rows in a block
   __device__ __forceinline__ int staged() const { return kPrivate ? kOwn * part : 0; }
-  // which of the waves with the same rows writes column tile u, after their sums were joined
-  __device__ __forceinline__ bool writes(int u) const { return u % KS == part; }
+};
+
+// The kernel's arguments, read from memory where they are used (each packed kernel has them as its only ones).
+template <typename T>
+__device__ __forceinline__ const __attribute__((address_space(4))) PackedParams<T>* pk_late() {
+  auto* p = (const __attribute__((address_space(4))) PackedParams<T>*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return p;
+}
+
+template <typename T, int DP, int G, int KS>
+struct PkFormOf {
+  typedef PkForm<G, KS, KS == 1 || (KS == 2 && DP * sizeof(T) >= 512) ? 64 : 128> type;
 };
 
 // Rows of DP elements in LDS, 16-byte piece c of row r in slot c ^ f(r) of its row.
@@ -258,9 +302,9 @@ struct PkLane {
 };
 
 // Copies ROWS rows of d <= DP elements from memory to LDS without registers
-// (buffer_load ... lds: a wave's 64 pieces side by side). Rows past the last and
-// columns past d come as zeros, from past the resource's end: a weight of zero times
-// what lies there must stay zero. WAVES waves share the work.
+// (buffer_load ... lds: a wave's 64 pieces side by side), one block after the other. Rows
+// past the last and columns past d come as zeros, from past the resource's end: a weight of
+// zero times what lies there must stay zero. WAVES waves share the work.
 template <typename T, int DP, int ROWS, int WAVES>
 struct PkCopy {
   typedef PkRows<T, DP> Rows;
@@ -270,9 +314,12 @@ struct PkCopy {
   static constexpr int kSub = kG > WAVES ? kG / WAVES : 1;             // distinct offsets of a lane
   static_assert(Rows::kCh <= 64 && ROWS % 16 == 0 && kN >= 1, "whole instructions");
   uint32_t off[kSub];
-  uint32_t pitch;  // bytes between rows
+  uint32_t pitch;    // bytes between rows
+  uint64_t from;     // address of the next block's first row
+  int left, row;     // rows from there on; bytes of a row
   __device__ __forceinline__ void init(int64_t token, int d, int wave, int lane) {
     pitch = (uint32_t)(token * (int64_t)sizeof(T));
+    row = d * (int)sizeof(T);
 #pragma unroll
     for (int i = 0; i < kSub; ++i) {
       const int sub = WAVES >= kG ? wave % kG : wave + WAVES * i;
@@ -281,24 +328,29 @@ struct PkCopy {
       off[i] = c * Rows::kE < d ? r * pitch + 16 * c : 0x80000000u;
     }
   }
-  // rows row0 .. of `src` (row 0 at src, n rows in all) to `tile`
-  __device__ __forceinline__ void issue(const T* src, int64_t row0, int64_t n, int d, unsigned char* tile, int wave) const {
-    const int64_t left = n - row0;
-    const int64_t rows = left < ROWS ? left : ROWS;
-    const int bytes = rows > 0 ? (int)((rows - 1) * pitch + d * (int)sizeof(T)) : 0;
-    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<char*>(reinterpret_cast<const char*>(src) + row0 * (int64_t)pitch), (short)0, bytes, 0x00020000);
+  // begins at row row0 of the n at src
+  __device__ __forceinline__ void begin(const T* src, int row0, int n) {
+    from = (uint64_t)(uintptr_t)src + (uint64_t)row0 * pitch;
+    left = n - row0;
+  }
+  // a block to `tile`; the next one is `step` rows on
+  __device__ __forceinline__ void issue(unsigned char* tile, int wave, int step) {
+    const uint32_t bytes = left <= 0 ? 0u : (uint32_t)((left < ROWS ? left : ROWS) - 1) * pitch + (uint32_t)row;
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<char*>((uintptr_t)from), (short)0, (int)bytes, 0x00020000);
     // their sums, kept through a loop, took more scalars than there are
     typedef __attribute__((address_space(3))) unsigned char lds_byte;
-    uint32_t step = pitch, to = (uint32_t)(uintptr_t)(lds_byte*)tile;
-    asm volatile("" : "+s"(step), "+s"(to));
+    uint32_t by = pitch, to = (uint32_t)(uintptr_t)(lds_byte*)tile;
+    asm volatile("" : "+s"(by), "+s"(to));
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
       // 16-row group and place of instruction `wave + WAVES i`
       const int group = WAVES >= kG ? wave / kG + i * (WAVES / kG) : i / kSub;
       const uint32_t o = off[WAVES >= kG ? 0 : i % kSub];
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_byte*)(uintptr_t)(to + (wave + WAVES * i) * 1024), 16, o + (uint32_t)(16 * group) * step, 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_byte*)(uintptr_t)(to + (wave + WAVES * i) * 1024), 16,
+                                               o + (uint32_t)(16 * group) * by, 0, 0, 0);
     }
+    from += (uint64_t)step * pitch;
+    left -= step;
   }
 };
 
@@ -359,34 +411,41 @@ __device__ __forceinline__ void pk_round(float by, f32x4 (&s)[NT]) {
     }
 }
 
-// The accumulators of a group's waves added, through LDS (PITCH floats a row), 16 rows of
-// each at a time; wave j of a group gets the column tiles u with u % KS == j.
-template <int G, int KS, int R, int U, int PITCH>
-__device__ __forceinline__ void pk_sum_waves(float* lds, const PkForm<G, KS>& f, int li, int lg, f32x4 (&x)[R][U]) {
-  auto slot = [&](int j) { return ((j * G + f.group) * 16 + li) * PITCH + 4 * lg; };
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
+// A workgroup's accumulators to memory by way of LDS: 16 rows of each wave, then put(row,
+// c, x) for each row of the groups and its 8 columns from c on, x being where they lie, the
+// j-th wave's of a group j * kPart floats on. Few instructions, where each lane's stores
+// to its own rows were most of a small call's time, and whole rows of memory.
+template <typename Form, int DP>
+struct PkOut {
+  static constexpr int kPitch = DP + 4, kRows = 16 * Form::kG, kPart = kRows * kPitch;
+  static constexpr int kBytes = Form::kKS * kPart * 4;
+  template <int U, typename Put>
+  __device__ static __forceinline__ void write(unsigned char* raw, const Form& f, int t, const f32x4 (&x)[U], Put put) {
+    float* lds = reinterpret_cast<float*>(raw);
+    const int li = t & 15, lg = (t >> 4) & 3;
     __syncthreads();
+    float* mine = lds + f.part * kPart + (16 * f.group + li) * kPitch + 4 * lg;
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) lds[slot(f.part) + 16 * u + e] = x[r][u][e];
+    for (int u = 0; u < U; ++u) *reinterpret_cast<f32x4*>(mine + 16 * u) = x[u];
     __syncthreads();
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (!f.writes(u)) continue;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float a = 0.f;
-#pragma unroll
-        for (int j = 0; j < KS; ++j) a += lds[slot(j) + 16 * u + e];
-        x[r][u][e] = a;
-      }
+#pragma unroll 1
+    for (int i = t; i < kRows * (DP / 8); i += Form::kThreads) {
+      const int row = i / (DP / 8), c = i % (DP / 8) * 8;
+      put(row, c, lds + row * kPitch + c);
     }
   }
-}
-template <int G, int KS, int PITCH>
-constexpr int kPkSumBytes = G * KS * 16 * PITCH * 4;
+  // the sum of a group's waves
+  __device__ static __forceinline__ f32x8 sum(const float* x) {
+    f32x8 v = load8(x);
+#pragma unroll
+    for (int j = 1; j < Form::kKS; ++j) {
+      const f32x8 o = load8(x + j * kPart);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += o[e];
+    }
+    return v;
+  }
+};
 
 // max over the 4 lanes {l % 16 + 16 g}
 __device__ __forceinline__ float lanes4_max(float x) {
@@ -399,6 +458,15 @@ __device__ __forceinline__ float lanes4_max(float x) {
   return fmaxf(__builtin_bit_cast(float, b0), __builtin_bit_cast(float, b1));
 }
 
+// launch(P, grid) for a call's workgroups: key/value heads, tiles and parts, in as many
+// launches as a grid's second axis takes
+template <typename T, typename F>
+void pk_grid(PackedParams<T> P, F launch) {
+  constexpr int kMost = 65535;
+  for (P.tile0 = 0; P.tile0 < P.tiles; P.tile0 += kMost)
+    launch(P, dim3(P.heads / P.group, P.tiles - P.tile0 < kMost ? P.tiles - P.tile0 : kMost, P.splits));
+}
+
 // f(G, KS, R) for the forms that packed_form chooses; float32 has one tile a wave
 template <typename T, typename F>
 void pk_form(const PackedForm& form, F f) {
@@ -407,7 +475,6 @@ void pk_form(const PackedForm& form, F f) {
   typedef std::integral_constant<int, 4> Four;
   if (form.groups == 1) return f(One{}, Four{}, One{});
   if constexpr (sizeof(T) == 2) {
-    if (form.groups == 2) return f(Two{}, Four{}, Two{});
     if (form.tiles == 2) return form.ks == 2 ? f(Four{}, Two{}, Two{}) : f(Four{}, One{}, Two{});
   }
   if (form.ks == 2) return f(Four{}, Two{}, One{});

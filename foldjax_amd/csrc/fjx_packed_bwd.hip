@@ -26,8 +26,8 @@ __device__ __forceinline__ float pk_weight(float s, float by, float m, float log
 
 // dq, and D for the other kernel: rows and blocks as in the forward pass.
 template <typename T, int DP, int G, int KS, int R>
-__global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkForm<G, KS>::template kSimd<T, DP>)) void packed_dq_kernel(PackedParams<T> P) {
-  typedef PkForm<G, KS> Form;
+__global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkFormOf<T, DP, G, KS>::type::template kSimd<T, DP>)) void packed_dq_kernel(PackedParams<T> P) {
+  typedef typename PkFormOf<T, DP, G, KS>::type Form;
   typedef PkRows<T, DP> Rows;
   typedef typename Frag<T>::type F;
   constexpr int kC = Rows::kC, kU = Rows::kU;
@@ -36,38 +36,40 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkForm<G, KS>::template
   constexpr int kOperand = Form::kStage * Rows::kRowBytes;
   constexpr int kSets = Form::kSets;
   constexpr int kStages = 4 * kOperand * kSets <= 160 * 1024 ? 2 : 1;
-  constexpr int kPo = DP + 2;
-  static_assert(KS == 1 || kStages * 2 * kOperand * kSets >= kPkSumBytes<G, KS, kPo>, "the waves' sums");
-  __shared__ __attribute__((aligned(16))) unsigned char raw[kStages * 2 * kOperand * kSets];
+  typedef PkOut<Form, DP> Out;
+  constexpr int kRaw = kStages * 2 * kOperand * kSets;  // and at the end the outputs' way
+  __shared__ __attribute__((aligned(16))) unsigned char raw[kRaw > Out::kBytes ? kRaw : Out::kBytes];
+  __shared__ int2 places[R][16 * G];  // the rows' heads and tokens; head -1: no such row
 
   const int t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const Form form(wave);
-  const int kvh = P.heads / P.group;
-  const int kv = blockIdx.x % kvh;
-  const int nth = blockIdx.x / kvh, tile_id = P.order ? nth : P.tiles - 1 - nth;  // as in the forward pass
-  PackedSpan sp;
-  if (!packed_span(P, false, P.group, kShift, tile_id, lane, sp)) return;
-  const int rows = sp.nq * P.group;
-  const int row0 = sp.tile * kTileRows;
-  if (row0 >= rows) return;
-  const int row_w = row0 + 16 * R * form.group;
+  const int kv = blockIdx.x;
+  const int nth = P.tile0 + blockIdx.y;  // in the forward pass's order
+  PackedTile sp;
+  if (!packed_tile(P, false, P.group, kShift, P.order ? nth : P.tiles - 1 - nth, lane, sp)) return;
+  const int row0 = sp.tile * kTileRows, rows = sp.nq * P.group - row0;  // those from row0 on
+  if (rows <= 0) return;
+  const int row_w = 16 * R * form.group;
+  const PackedRows place(P, row0);
 
-  int head[R], token[R], lim[R];
+  int lim[R];
   F qf[R][kC], dof[R][kC];
   float m[R], log_sum[R], delta[R];
   bool any_far = false;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const int row = row_w + 16 * r + li < rows ? row_w + 16 * r + li : rows - 1;
-    const int qi = row / P.group;
-    head[r] = kv * P.group + row - qi * P.group;
-    token[r] = sp.q0 + qi;
+    const int x = row_w + 16 * r + li;
+    int qi, head;
+    place.at(x < rows ? x : rows - 1, qi, head);
+    head += kv * P.group;
+    const int64_t token = sp.q0 + qi;
     lim[r] = P.causal ? qi + sp.nk - sp.nq + 1 : sp.nk;
-    const T* q = P.q.p + head[r] * P.q.head + token[r] * P.q.token + 8 * lg;
-    const T* dout = P.dout.p + head[r] * P.dout.head + token[r] * P.dout.token + 8 * lg;
-    const T* o = P.o.p + head[r] * P.o.head + token[r] * P.o.token + 8 * lg;
-    const T* rest = P.o_rest.p + head[r] * P.o_rest.head + token[r] * P.o_rest.token + 8 * lg;
+    if (lg == 0 && form.part == 0) places[r][16 * form.group + li] = make_int2(x < rows ? head : -1, (int)token);
+    const T* q = P.q.p + head * P.q.head + token * P.q.token + 8 * lg;
+    const T* dout = P.dout.p + head * P.dout.head + token * P.dout.token + 8 * lg;
+    const T* o = P.o.p + head * P.o.head + token * P.o.token + 8 * lg;
+    const T* rest = P.o_rest.p + head * P.o_rest.head + token * P.o_rest.token + 8 * lg;
     float d = 0.f;
 #pragma unroll
     for (int c = 0; c < kC; ++c) {
@@ -88,31 +90,31 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkForm<G, KS>::template
       for (int e = 0; e < 8; ++e) d = fmaf(x[e], y[e], d);
     }
     delta[r] = group_sum(d);
-    const int64_t at_row = (int64_t)head[r] * P.tq + token[r];
+    const int64_t at_row = (int64_t)head * P.tq + token;
     const f32x2 stats = *reinterpret_cast<const f32x2*>(P.lse + at_row * 2);
     m[r] = stats[0];
     log_sum[r] = stats[1];
     any_far = any_far || fabsf(m[r]) > kFar;
-    if (lg == 0 && form.part == 0 && row_w + 16 * r + li < rows) P.delta[at_row] = delta[r];
+    if (lg == 0 && form.part == 0 && x < rows) P.delta[at_row] = delta[r];
   }
   const bool far = __builtin_amdgcn_ballot_w64(any_far);
-  const int last = (row0 + kTileRows < rows ? row0 + kTileRows : rows) - 1;
-  const int most = P.causal ? last / P.group + sp.nk - sp.nq + 1 : sp.nk;
+  int q_last, h_last;
+  place.at((kTileRows < rows ? kTileRows : rows) - 1, q_last, h_last);
+  const int most = P.causal ? q_last + sp.nk - sp.nq + 1 : sp.nk;
   const int lim_lo = __builtin_amdgcn_readfirstlane(lim[0]);
   const int lim_hi = row_w < rows ? __builtin_amdgcn_readlane(lim[R - 1], 15) : 0;
-  const int blocks = most > 0 ? (int)(((int64_t)most + Form::kBlock - 1) / Form::kBlock) : 0;
+  const int blocks = most > 0 ? (int)((uint32_t)(most + Form::kBlock - 1) / Form::kBlock) : 0;
 
   unsigned char* const mine = raw + (Form::kPrivate ? wave * kStages * 2 * kOperand : 0);
   PkCopy<T, DP, Form::kStage, Form::kOwners> kcopy, vcopy;
   kcopy.init(P.k.token, P.d, form.stager, lane);
   vcopy.init(P.v.token, P.d, form.stager, lane);
-  const T* ks = P.k.p + kv * P.k.head + (int64_t)sp.k0 * P.k.token;
-  const T* vs = P.v.p + kv * P.v.head + (int64_t)sp.k0 * P.v.token;
-  auto stage = [&](int blk, int at) {
+  kcopy.begin(P.k.p + kv * P.k.head + (int64_t)sp.k0 * P.k.token, form.staged(), sp.nk);
+  vcopy.begin(P.v.p + kv * P.v.head + (int64_t)sp.k0 * P.v.token, form.staged(), sp.nk);
+  auto stage = [&](int at) {  // the next block
     unsigned char* s = mine + at * 2 * kOperand;
-    const int64_t key = (int64_t)blk * Form::kBlock + form.staged();
-    kcopy.issue(ks, key, sp.nk, P.d, s, form.stager);
-    vcopy.issue(vs, key, sp.nk, P.d, s + kOperand, form.stager);
+    kcopy.issue(s, form.stager, Form::kBlock);
+    vcopy.issue(s + kOperand, form.stager, Form::kBlock);
   };
   PkLane<T, DP> at;
   at.init(lane);
@@ -123,16 +125,16 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkForm<G, KS>::template
     for (int u = 0; u < kU; ++u) dq[r][u] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   if (kStages == 2) {
-    if (blocks) stage(0, 0);
+    if (blocks) stage(0);
     pk_sync<Form>();
   }
   for (int blk = 0; blk < blocks; ++blk) {
     const int cur = kStages == 2 ? blk & 1 : 0;
     if (kStages == 1) {
-      stage(blk, 0);
+      stage(0);
       pk_sync<Form>();
     } else if (blk + 1 < blocks) {
-      stage(blk + 1, cur ^ 1);
+      stage(cur ^ 1);
     }
     const unsigned char* kt_ = mine + cur * 2 * kOperand + form.at * Rows::kRowBytes;
     const unsigned char* vt_ = kt_ + kOperand;
@@ -190,21 +192,17 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkForm<G, KS>::template
     }
     pk_sync<Form>();
   }
-  if constexpr (KS > 1) pk_sum_waves<G, KS, R, kU, kPo>(reinterpret_cast<float*>(raw), form, li, lg, dq);
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    if (row_w + 16 * r + li >= rows) continue;
-    T* out = P.dq.p + head[r] * P.dq.head + token[r] * P.dq.token;
+  for (int r = 0; r < R; ++r)
+    Out::write(raw, form, t, dq[r], [&](int row, int c, const float* x) {
+      const int2 to = places[r][row];
+      if (to.x < 0 || c >= P.d) return;
+      const f32x8 v = Out::sum(x);
+      float y[8];
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const int col = 16 * u + 4 * lg;
-      if (!form.writes(u) || col >= P.d) continue;
-      float v[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = dq[r][u][e] * P.scale;
-      store4f(out + col, v);
-    }
-  }
+      for (int e = 0; e < 8; ++e) y[e] = v[e] * P.scale;
+      store8(P.dq.p + to.x * P.dq.head + to.y * P.dq.token + c, pack8<T>(y));
+    });
 }
 
 // dk and dv: a wave holds R tiles of 16 keys, lane l key l % 16 of each, and walks the
@@ -212,8 +210,8 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkForm<G, KS>::template
 // the lane 4 queries of its own keys, as the operands of dV^T = dO^T P and dK^T = Q^T dS.
 // KS 1: four waves with keys of their own; 4: the waves share keys and split the queries.
 template <typename T, int DP, int G, int KS, int R>
-__global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkForm<G, KS>::template kSimd<T, DP>)) void packed_dkv_kernel(PackedParams<T> P) {
-  typedef PkForm<G, KS> Form;
+__global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkFormOf<T, DP, G, KS>::type::template kSimd<T, DP>)) void packed_dkv_kernel(PackedParams<T> P) {
+  typedef typename PkFormOf<T, DP, G, KS>::type Form;
   typedef PkRows<T, DP> Rows;
   typedef typename Frag<T>::type F;
   constexpr int kC = Rows::kC, kU = Rows::kU;
@@ -222,31 +220,24 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkForm<G, KS>::template
   constexpr int kOperand = Form::kStage * Rows::kRowBytes;
   constexpr int kSets = Form::kSets;
   constexpr int kStages = 4 * kOperand * kSets <= 156 * 1024 ? 2 : 1;
-  constexpr int kPo = DP + 2;
-  static_assert(KS == 1 || kStages * 2 * kOperand * kSets >= kPkSumBytes<G, KS, kPo>, "the waves' sums");
-  __shared__ __attribute__((aligned(16))) unsigned char raw[kStages * 2 * kOperand * kSets];
+  typedef PkOut<Form, DP> Out;
+  constexpr int kRaw = kStages * 2 * kOperand * kSets;  // and at the end the outputs' way
+  __shared__ __attribute__((aligned(16))) unsigned char raw[kRaw > Out::kBytes ? kRaw : Out::kBytes];
   __shared__ __attribute__((aligned(16))) float rowstat[kSets][kStages][3][Form::kStage];  // M, log2 of the sum, D
   __shared__ int rowfar[kSets][kStages][Form::kRest];
-  // two tiles of keys a wave at 128 channels: with their values in registers as well there
-  // would be more of them than two waves a SIMD have
-  constexpr bool kValues = DP * R > 128;
-  __shared__ __attribute__((aligned(16))) unsigned char values[kValues ? kTileKeys * Rows::kRowBytes : 16];
 
   const int t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const Form form(wave);
-  const int kvh = P.heads / P.group;
-  const int kv = blockIdx.x % kvh;
-  const uint32_t rest_id = blockIdx.x / kvh;
-  const int split = rest_id / (uint32_t)P.tiles;
-  PackedSpan sp;
-  if (!packed_span(P, true, 1, kShift, (int)(rest_id % (uint32_t)P.tiles), lane, sp)) return;
+  const int kvh = P.heads / P.group, kv = blockIdx.x, split = blockIdx.z;
+  PackedTile sp;
+  if (!packed_tile(P, true, 1, kShift, P.tile0 + blockIdx.y, lane, sp)) return;
   const int key0 = sp.tile * kTileKeys;
   if (key0 >= sp.cap) return;
   const int key_w = key0 + 16 * R * form.group;
   const int shift = sp.nq - sp.nk;  // a causal row i sees the keys up to i - shift
 
-  F kf[R][kC], vf[kValues ? 1 : R][kC];
+  F kf[R][kC], vf[R][kC];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const int key = key_w + 16 * r + li;
@@ -257,19 +248,15 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkForm<G, KS>::template
     for (int c = 0; c < kC; ++c) {
       const bool in = key < sp.nk && 32 * c + 8 * lg < P.d;
       kf[r][c] = in ? load8(k + 32 * c) : F{};
-      if constexpr (!kValues) vf[r][c] = in ? load8(v + 32 * c) : F{};
+      vf[r][c] = in ? load8(v + 32 * c) : F{};
     }
   }
-  if constexpr (kValues) {
-    PkCopy<T, DP, kTileKeys, Form::kOwners> copy;
-    copy.init(P.v.token, P.d, form.stager, lane);
-    copy.issue(P.v.p + kv * P.v.head + (int64_t)sp.k0 * P.v.token, key0, sp.nk, P.d, values, form.stager);
-  }
   // the heads of this part, and the query blocks in which any row sees the first key
-  const int h0 = P.group * split / P.splits, h1 = P.group * (split + 1) / P.splits;
-  const int q_first = P.causal && key0 + shift > 0 ? key0 + shift : 0;
+  int h0 = 0, h1 = P.group;
+  if (P.splits > 1) h0 = P.group * split / P.splits, h1 = P.group * (split + 1) / P.splits;
+  const uint32_t q_first = P.causal && key0 + shift > 0 ? key0 + shift : 0;
   const int qb0 = q_first / Form::kBlock;
-  const int qb1 = key0 < sp.nk ? (int)(((int64_t)sp.nq + Form::kBlock - 1) / Form::kBlock) : 0;
+  const int qb1 = key0 < sp.nk ? (int)((uint32_t)(sp.nq + Form::kBlock - 1) / Form::kBlock) : 0;
   const int turns = qb1 > qb0 ? (h1 - h0) * (qb1 - qb0) : 0;
 
   const int set = Form::kPrivate ? wave : 0;
@@ -282,11 +269,14 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkForm<G, KS>::template
   f32x2 st_m = {0.f, INFINITY};
   float st_d = 0.f;
   auto stage = [&](int at) {
-    const int head = kv * P.group + next_h;
-    const int64_t row0 = (int64_t)next_b * Form::kBlock + form.staged();
+    const int head = kv * P.group + next_h, row0 = next_b * Form::kBlock + form.staged();
+    if (next_b == qb0) {
+      qcopy.begin(P.q.p + head * P.q.head + (int64_t)sp.q0 * P.q.token, row0, sp.nq);
+      ocopy.begin(P.dout.p + head * P.dout.head + (int64_t)sp.q0 * P.dout.token, row0, sp.nq);
+    }
     unsigned char* s = mine + at * 2 * kOperand;
-    qcopy.issue(P.q.p + head * P.q.head + (int64_t)sp.q0 * P.q.token, row0, sp.nq, P.d, s, form.stager);
-    ocopy.issue(P.dout.p + head * P.dout.head + (int64_t)sp.q0 * P.dout.token, row0, sp.nq, P.d, s + kOperand, form.stager);
+    qcopy.issue(s, form.stager, Form::kBlock);
+    ocopy.issue(s + kOperand, form.stager, Form::kBlock);
     st_m = f32x2{0.f, INFINITY};  // rows past the last: weights of zero
     st_d = 0.f;
     if (stat_row < Form::kStage && row0 + stat_row < sp.nq) {
@@ -355,26 +345,11 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkForm<G, KS>::template
 #pragma unroll
                            for (int r = 0; r < R; ++r) mma(s[r][i / kC], qf, kf[r][i % kC]);
                          });
-        if constexpr (kValues) {
+        pk_ahead<2 * kC>([&](int i) { return at.at_row(ot_, 32 * pair + 16 * (i / kC), i % kC); },
+                         [&](int i, const F& of) {
 #pragma unroll
-          for (int c = 0; c < kC; ++c) {
-            F vc[R];
-#pragma unroll
-            for (int r = 0; r < R; ++r) vc[r] = at.at_row(values, 16 * (R * form.group + r), c);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const F of = at.at_row(ot_, 32 * pair + 16 * j, c);
-#pragma unroll
-              for (int r = 0; r < R; ++r) mma(dp[r][j], of, vc[r]);
-            }
-          }
-        } else {
-          pk_ahead<2 * kC>([&](int i) { return at.at_row(ot_, 32 * pair + 16 * (i / kC), i % kC); },
-                           [&](int i, const F& of) {
-#pragma unroll
-                             for (int r = 0; r < R; ++r) mma(dp[r][i / kC], of, vf[r][i % kC]);
-                           });
-        }
+                           for (int r = 0; r < R; ++r) mma(dp[r][i / kC], of, vf[r][i % kC]);
+                         });
         float by = P.scale_log2;
         if (far) {
           by = 1.f;
@@ -423,37 +398,31 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkForm<G, KS>::template
     if (kStages == 2 && turn + 1 < turns) put_stats(cur ^ 1);
     pk_sync<Form>();
   }
-  if constexpr (KS > 1) {
-    pk_sum_waves<G, KS, R, kU, kPo>(reinterpret_cast<float*>(raw), form, li, lg, dk);
-    pk_sum_waves<G, KS, R, kU, kPo>(reinterpret_cast<float*>(raw), form, li, lg, dv);
-  }
+  // The arguments are read again here: kept through the walk, they would spill scalar registers.
+  const auto* L = pk_late<T>();
+  // dk, then dv; keys that are not there have zeros
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int key = key_w + 16 * r + li;
-    if (key >= sp.cap) continue;
-    const bool real = key < sp.nk;  // the others' gradients are zeros
-    const int64_t token = (int64_t)sp.k0 + key;
+  for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const int col = 16 * u + 4 * lg;
-      if (!form.writes(u)) continue;
-      if (P.splits > 1) {
-        const int64_t at_key = (((int64_t)split * kvh + kv) * P.tk + token) * DP + col;
-        *reinterpret_cast<f32x4*>(P.part_dk + at_key) = real ? dk[r][u] : f32x4{0.f, 0.f, 0.f, 0.f};
-        *reinterpret_cast<f32x4*>(P.part_dv + at_key) = real ? dv[r][u] : f32x4{0.f, 0.f, 0.f, 0.f};
-        continue;
-      }
-      if (col >= P.d) continue;
-      float a[4], b[4];
+    for (int r = 0; r < R; ++r)
+      Out::write(raw, form, t, i ? dv[r] : dk[r], [&](int row, int c, const float* x) {
+        const int key = key0 + 16 * (R * (row / 16) + r) + row % 16;
+        if (key >= sp.cap) return;
+        const f32x8 v = Out::sum(x);
+        const int64_t token = (int64_t)sp.k0 + key;
+        const float by = key < sp.nk ? i || L->splits > 1 ? 1.f : L->scale : 0.f;
+        float y[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        a[e] = real ? dk[r][u][e] * P.scale : 0.f;
-        b[e] = real ? dv[r][u][e] : 0.f;
-      }
-      store4f(P.dk.p + kv * P.dk.head + token * P.dk.token + col, a);
-      store4f(P.dv.p + kv * P.dv.head + token * P.dv.token + col, b);
-    }
-  }
+        for (int e = 0; e < 8; ++e) y[e] = by == 0.f ? 0.f : v[e] * by;
+        if (L->splits > 1) {
+          store8((i ? L->part_dv : L->part_dk) + (((int64_t)split * kvh + kv) * L->tk + token) * DP + c, pack8<float>(y));
+          return;
+        }
+        if (c >= L->d) return;
+        T* to = i ? L->dv.p : L->dk.p;
+        const int64_t head = i ? L->dv.head : L->dk.head, step = i ? L->dv.token : L->dk.token;
+        store8(to + kv * head + token * step + c, pack8<T>(y));
+      });
 }
 
 // The parts of dk and dv (a part has some of the heads that share them) added: 4
@@ -482,20 +451,23 @@ void bwd(PackedParams<T> P, const PackedForm& rows, const PackedForm& keys, hipS
   P.splits = 1;
   P.tiles = rows.count;
   P.order = rows.order;
-  if (rows.count) {
-    pk_form<T>(rows, [&](auto g, auto ks, auto r) {
-      constexpr int G = decltype(g)::value, KS = decltype(ks)::value, R = decltype(r)::value;
-      packed_dq_kernel<T, DP, G, KS, R><<<(unsigned)((int64_t)rows.count * kvh), PkForm<G, KS>::kThreads, 0, st>>>(P);
+  pk_form<T>(rows, [&](auto g, auto ks, auto r) {
+    constexpr int G = decltype(g)::value, KS = decltype(ks)::value, R = decltype(r)::value;
+    pk_grid(P, [&](const PackedParams<T>& Q, dim3 grid) {
+      packed_dq_kernel<T, DP, G, KS, R><<<grid, PkForm<G, KS>::kThreads, 0, st>>>(Q);
     });
-  }
+  });
   if (!keys.count) return;
   P.splits = splits;
   P.tiles = keys.count;
   P.order = keys.order;
   pk_form<T>(keys, [&](auto g, auto ks, auto r) {
     constexpr int G = decltype(g)::value, KS = decltype(ks)::value, R = decltype(r)::value;
-    if constexpr (DP * R <= 128 || G == 2)
-      packed_dkv_kernel<T, DP, G, KS, R><<<(unsigned)((int64_t)keys.count * kvh * splits), PkForm<G, KS>::kThreads, 0, st>>>(P);
+    // two tiles of keys a wave at 128 channels would take more registers than two waves a SIMD have
+    if constexpr (DP * R <= 128)
+      pk_grid(P, [&](const PackedParams<T>& Q, dim3 grid) {
+        packed_dkv_kernel<T, DP, G, KS, R><<<grid, PkForm<G, KS>::kThreads, 0, st>>>(Q);
+      });
   });
   if (splits > 1)
     packed_dkv_join_kernel<T, DP><<<(unsigned)(((int64_t)kvh * P.tk * DP / 4 + 255) / 256), 256, 0, st>>>(P);
