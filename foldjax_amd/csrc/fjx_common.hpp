@@ -194,6 +194,34 @@ template <> __device__ __forceinline__ f32x8 pack8<float>(const float* f) {
   return v;
 }
 
+// A float32 operand that the kernel computed (weights, dS) as the matrix
+// instructions take it: itself, or two bf16 parts (17 bits), whose products take
+// twice the matrix instructions. In the attention kernels these run beside the
+// exponentials and the vector work that bound them. What is left of a pair of values beyond
+// their high parts is one v_dot2_f32_bf16 each, (h_0, h_1) . (-1, 0) + x_0 (exact),
+// where unpacking and subtracting takes two instructions. Its selector stays in a
+// register: as an inline constant it reached the instruction as the other half.
+template <typename T> constexpr int kParts = sizeof(T) == 2 ? 2 : 1;
+__device__ __forceinline__ void parts(const float* p, bf16x8 (&f)[2]) {
+  typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  uint32_t first = 0x0000bf80u, second = 0xbf800000u;
+  asm("" : "+s"(first), "+s"(second));
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    const bf16x2 h = {static_cast<bf16>(p[e]), static_cast<bf16>(p[e + 1])};
+    f[0][e] = h[0];
+    f[0][e + 1] = h[1];
+    f[1][e] = static_cast<bf16>(__builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(bf16x2, first), p[e], false));
+    f[1][e + 1] = static_cast<bf16>(__builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(bf16x2, second), p[e + 1], false));
+  }
+}
+__device__ __forceinline__ void parts(const float* p, f32x8 (&f)[1]) { f[0] = pack8<float>(p); }
+__device__ __forceinline__ void mma_parts(f32x4& o, const bf16x8& a, const bf16x8 (&p)[2]) {
+  mma(o, a, p[1]);
+  mma(o, a, p[0]);
+}
+__device__ __forceinline__ void mma_parts(f32x4& o, const f32x8& a, const f32x8 (&p)[1]) { mma(o, a, p[0]); }
+
 __device__ __forceinline__ float fast_sigmoid(float x) {
   // 1 / (1 + 2^(-x log2 e)) on the hardware v_exp_f32 / v_rcp_f32 (about 1 ulp
   // each); saturates cleanly to 0 (2^big = inf, rcp(inf) = 0) and to 1
