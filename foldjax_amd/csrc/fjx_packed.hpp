@@ -117,7 +117,7 @@ __device__ __forceinline__ bool packed_find(const PackedParams<T>& P, bool by_ke
     const int f = first(by_keys ? kv : qv, i);
     const uint64_t votes = __builtin_amdgcn_ballot_w64(lane <= P.seqs && f <= at);
     // offsets that descend leave votes behind a gap: the first run counts
-    const int run = (int)__builtin_ctzll(~votes);
+    const int run = votes == ~0ull ? 64 : (int)__builtin_ctzll(~votes);
     const int seq = run > 0 ? run - 1 : 0, next = seq < P.seqs ? seq + 1 : seq;
     s.seq = seq;
     s.tile = at - __builtin_amdgcn_readlane(f, seq);
