@@ -1327,7 +1327,7 @@ PackedForm packed_form(int64_t rows, int64_t seqs, int64_t wgs, int64_t walk, in
 // that walk 16384 blocks of 64 and more in all (the forward pass of 5 causal sequences,
 // 8192 tokens, 85 -> 77 us with it, of 6 with 16384 254 -> 234)
 bool packed_sorted(const PackedForm& f, int64_t seqs, int64_t wgs, int64_t walk) {
-  return f.groups > 1 && f.count && f.count <= kPackedOrder && seqs > 1 && wgs * walk >= (int64_t)16384 * 64;
+  return f.groups > 1 && f.count && f.count <= kPackedOrder && seqs > 1 && seqs <= kPackedOrderSeqs && wgs * walk >= (int64_t)16384 * 64;
 }
 PackedPlan packed_fwd_plan(int64_t tq, int64_t tk, int64_t seqs, int64_t heads, int64_t kvh, int64_t d, int32_t dtype) {
   const int64_t group = heads / kvh, rows = tq * group, wgs = kvh * ((rows + 63) / 64), walk = tk / seqs;

@@ -320,23 +320,27 @@ __global__ __launch_bounds__(1024) void packed_order_kernel(PackedParams<T> P, P
   constexpr int kClasses = 256;
   __shared__ int work[kPackedOrder], seqs[kPackedOrder];
   __shared__ int classes[kClasses], most;
+  __shared__ int q_at[kPackedOrderSeqs + 1], k_at[kPackedOrderSeqs + 1], length[kPackedOrderSeqs + 1];
   const int t = threadIdx.x;
   if (t < kClasses) classes[t] = 0;
   if (t == 0) most = 0;
   __syncthreads();
-  const PackedInts& starts = by_keys ? P.k_starts : P.q_starts;
-  const int64_t tokens = by_keys ? P.tk : P.tq;
   const int per = by_keys ? 1 : P.group;
-  auto first = [&](int s) { return (int)((packed_start(starts, s, tokens) * per) >> shift) + s; };
+  // the offsets, fetched once: the search and both passes over the tiles wait for no memory
+  for (int s = t; s <= P.seqs; s += 1024) {
+    q_at[s] = (int)packed_start(P.q_starts, s, P.tq);
+    k_at[s] = (int)packed_start(P.k_starts, s, P.tk);
+    length[s] = P.k_lengths.p && s < P.seqs ? (int)packed_int(P.k_lengths, s, P.tk) : 0x7fffffff;
+  }
+  __syncthreads();
+  auto first = [&](int s) { return (int)(((int64_t)(by_keys ? k_at : q_at)[s] * per) >> shift) + s; };
   auto tile_of = [&](int i, int seq) {
     PackedTile s;
     const int next = seq < P.seqs ? seq + 1 : seq;
     s.seq = seq;
     s.tile = i - first(seq);
     s.pad = 0;
-    packed_tokens(P, by_keys, (int)packed_start(P.q_starts, seq, P.tq), (int)packed_start(P.q_starts, next, P.tq),
-                  (int)packed_start(P.k_starts, seq, P.tk), (int)packed_start(P.k_starts, next, P.tk),
-                  P.k_lengths.p && seq < P.seqs ? (int)packed_int(P.k_lengths, seq, P.tk) : 0x7fffffff, s);
+    packed_tokens(P, by_keys, q_at[seq], q_at[next], k_at[seq], k_at[next], length[seq], s);
     return s;
   };
   for (int i = t; i < count; i += 1024) {

@@ -36,7 +36,7 @@ struct PackedInts {
   int wide;
 };
 
-constexpr int kPackedOrder = 12288;  // tiles that are sorted at most
+constexpr int kPackedOrder = 12288, kPackedOrderSeqs = 1023;  // tiles that are sorted at most, and their sequences
 
 // a tile of a sequence: first query, queries, first key, keys, and keys with the unused
 // ones behind them. Sequence `seqs`: the rows behind the last one
