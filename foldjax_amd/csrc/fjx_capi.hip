@@ -1295,18 +1295,26 @@ struct PackedPlan {
   size_t rows_order, keys_order;
 };
 int packed_width(int64_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
-// `wgs`: workgroups of 64 rows (keys) there are, `walk`: keys (rows) that one walks.
-// us by form, KS 4 / KS 2 / KS 1 with one tile / KS 2 / KS 1 with two:
-//   forward  126 workgroups 1003 keys d 64        9.3 / 12.2 / 15.4 /   - /   -
-//            216            850       128        25.7 / 17.4 / 20.9 / 24.3 / 29.6
-//            258            700        64        20.2 / 15.3 / 17.1 / 17.7 / 21.2
-//            496            245        24        15.7 / 11.5 /  9.8 / 11.8 / 10.5
-//            520            4099      128         123 / 62.7 / 70.5 / 69.6 / 98.2
-//           1024            1640      128         188 /   92 /   81 /   77 /  106
-//           2048            2730      128         660 /  320 /  285 /  249 /  234
-//   float32  132 workgroups 700 keys   64        41.5 / 41.9 / 45.6;  256, 2048, d 128  112 / 160 / 156
-// (the last two of the forward rows sorted). `most`: tiles of a wave at most.
-PackedForm packed_form(int64_t rows, int64_t seqs, int64_t wgs, int64_t walk, int most, int64_t few) {
+// `wgs`: workgroups of 64 rows (keys) there are, `walk`: keys (rows) that one walks;
+// `few`: so few wgs are one wave's rows with its own keys each; `pairs`: from so many on a
+// wave has two tiles. us by form, KS 4 / KS 2 / KS 1 with one tile / KS 2 / KS 1 with two:
+//   forward  126 workgroups 1003 keys d 64         8.7 / 10.9 / 14.6 / 15.6 / 20.5
+//            216            851       128         21.0 / 15.4 / 19.4 / 22.2 / 27.6
+//            258            686        64         17.5 / 13.4 / 16.4 / 16.0 / 20.8
+//            496            245        24         14.1 /  9.4 /  8.9 / 10.3 / 10.2
+//            520            4099      128          107 / 56.6 / 64.9 / 64.1 / 87.9
+//           1024            1638      128          160 / 83.4 / 75.9 / 70.8 / 96.1
+//           2048            2730      128          586 /  296 /  264 /  230 /  219
+//           4096            8192       64          641 /  370 /  349 /  301 /  295
+//   dk, dv (the backward pass with them, dq's form the same)
+//           1016            4049       64          251 /  202 /  238 /  216 /  231
+//           1024            4096       64         1101 /  849 / 1035 /  889 / 1182
+//           4096            8192       64         1580 / 1177 / 1135 / 1122 / 1090
+//   float32  132            701        64           36 /   39 /   42
+//            256            2048      128          107 /  144 /  148
+//            456            1774      128          163 /  147 /  149
+// (rows of several long sequences sorted).
+PackedForm packed_form(int64_t rows, int64_t seqs, int64_t wgs, int64_t walk, int64_t few, int64_t pairs) {
   PackedForm f = {};
   f.groups = 4;
   f.tiles = 1;
@@ -1314,12 +1322,10 @@ PackedForm packed_form(int64_t rows, int64_t seqs, int64_t wgs, int64_t walk, in
     f.groups = 1, f.ks = 4;
   else if (walk < 320 || wgs < 128)
     f.ks = 1;
-  else if (wgs < 1024 || most < 2)
+  else if (wgs < pairs)
     f.ks = 2;
-  else {
-    f.ks = wgs < 2048 ? 2 : 1;
-    f.tiles = 2;
-  }
+  else
+    f.ks = wgs < 2048 ? 2 : 1, f.tiles = 2;
   f.count = (int)std::min<int64_t>(rows / f.rows() + seqs + 1, 1 << 30);
   return f;
 }
@@ -1329,11 +1335,12 @@ PackedForm packed_form(int64_t rows, int64_t seqs, int64_t wgs, int64_t walk, in
 bool packed_sorted(const PackedForm& f, int64_t seqs, int64_t wgs, int64_t walk) {
   return f.groups > 1 && f.count && f.count <= kPackedOrder && seqs > 1 && seqs <= kPackedOrderSeqs && wgs * walk >= (int64_t)16384 * 64;
 }
+int64_t packed_few(bool bf, int64_t d) { return bf ? 128 : d <= 64 ? 256 : 384; }
 PackedPlan packed_fwd_plan(int64_t tq, int64_t tk, int64_t seqs, int64_t heads, int64_t kvh, int64_t d, int32_t dtype) {
   const int64_t group = heads / kvh, rows = tq * group, wgs = kvh * ((rows + 63) / 64), walk = tk / seqs;
   const bool bf = dtype == FJX_DTYPE_BF16;
   PackedPlan p = {};
-  p.rows = packed_form(rows, seqs, wgs, walk, bf ? 2 : 1, bf ? 128 : d <= 64 ? 256 : 512);
+  p.rows = packed_form(rows, seqs, wgs, walk, packed_few(bf, d), bf ? 1024 : INT64_MAX);
   p.splits = 1;
   if (p.rows.groups == 1) {
     const int64_t tiles = kvh * std::max(seqs, rows / 16);
@@ -1357,9 +1364,9 @@ PackedPlan packed_bwd_plan(int64_t tq, int64_t tk, int64_t seqs, int64_t heads, 
   p.splits = 1;
   // workgroups that walk long and, causal, uneven ways: the heads that share keys in parts
   if (group > 1 && tk && key_wgs < 1024) p.splits = (int)std::min<int64_t>(group, (1024 + key_wgs - 1) / key_wgs);
-  if (tq) p.rows = packed_form(rows, seqs, wgs, walk, bf ? 2 : 1, bf ? 128 : 256);
+  if (tq) p.rows = packed_form(rows, seqs, wgs, walk, packed_few(bf, d), bf ? 1024 : INT64_MAX);
   // two tiles of keys a wave would take more registers than two waves a SIMD have at 128 channels
-  if (tk) p.keys = packed_form(tk, seqs, key_wgs * p.splits, tq / seqs, bf && d <= 64 ? 2 : 1, bf ? 128 : 256);
+  if (tk) p.keys = packed_form(tk, seqs, key_wgs * p.splits, tq / seqs, packed_few(bf, d), bf && d <= 64 ? 2048 : INT64_MAX);
   if (p.splits > 1) p.part_o = align_up((size_t)p.splits * kvh * tk * packed_width(d) * sizeof(float));
   p.part_ml = align_up((size_t)heads * tq * sizeof(float));
   if (packed_sorted(p.rows, seqs, wgs, walk)) p.rows_order = align_up((size_t)p.rows.count * sizeof(PackedTile));

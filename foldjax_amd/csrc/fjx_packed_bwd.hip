@@ -466,8 +466,9 @@ void bwd(PackedParams<T> P, const PackedForm& rows, const PackedForm& keys, hipS
   P.order = keys.order;
   pk_form<T>(keys, [&](auto g, auto ks, auto r) {
     constexpr int G = decltype(g)::value, KS = decltype(ks)::value, R = decltype(r)::value;
-    // two tiles of keys a wave at 128 channels would take more registers than two waves a SIMD have
-    if constexpr (DP * R <= 128)
+    // two tiles of keys a wave: at 128 channels they would take more registers than two waves
+    // a SIMD have, and are taken only where workgroups are many
+    if constexpr (DP * R <= 128 && (KS * R <= 2 || G == 1))
       pk_grid(P, [&](const PackedParams<T>& Q, dim3 grid) {
         packed_dkv_kernel<T, DP, G, KS, R><<<grid, PkForm<G, KS>::kThreads, 0, st>>>(Q);
       });

@@ -143,3 +143,14 @@ def test_writes_stay_in_the_workspace(lens, room, h, kv, d, dtype):
     assert asked == [n for n in sizes if n]
     assert all((t[:guard] == 0xA5).all() and (t[-guard:] == 0xA5).all() for t in around)
     assert all(torch.equal(got[n], want[n]) for n in want)
+
+
+# so many workgroups that a wave has two tiles of rows, and of keys; and float32 with two waves a tile
+@pytest.mark.parametrize("lens,h,kv,d,dtype", [([330] * 20 + [1700], 16, 16, 24, BF16), ([400, 37, 363] * 11, 16, 16, 64, BF16),
+                                               ([900, 1, 700], 16, 16, 128, FP32), ([2000, 1100], 16, 8, 128, FP32)])
+@pytest.mark.parametrize("causal", [False, True], ids=["all", "causal"])
+def test_many_workgroups(lens, h, kv, d, dtype, causal):
+    say(f"packed many workgroups {len(lens)} {d} {dtype} {causal}")
+    q, k, v, dout = inputs(lens, h, kv, d, dtype, seed=27)
+    more = {"scale": d**-0.5, "causal": causal}
+    compare(run(q, k, v, ints(starts(lens)), dout, **more), O.attention(q, k, v, starts(lens), dout=dout, **more))
