@@ -1404,9 +1404,11 @@ int packed_check(const fjx_packed_attention_args* a, const char* fn) {
     return fail(FJX_ERR_INVALID, "%s: offsets must be aligned to their elements", fn);
   if (a->rest && a->dtype == FJX_DTYPE_F32)
     return fail(FJX_ERR_INVALID, "%s: rest is of bf16 outputs", fn);
-  constexpr int64_t kLong = (int64_t)1 << 31;
-  if (a->tokens_q * a->heads >= kLong || a->tokens_k >= kLong || a->sequences >= 1 << 22)
-    return fail(FJX_ERR_UNSUPPORTED, "%s: tokens_q * heads and tokens_k must be below 2^31, sequences below 2^22", fn);
+  // 32-bit row numbers, also of the last tile of 128 rows that begins in each sequence
+  if (a->sequences >= 1 << 22) return fail(FJX_ERR_UNSUPPORTED, "%s: sequences must be below 2^22", fn);
+  const int64_t most = ((int64_t)1 << 31) - 128 * (a->sequences + 2);
+  if (a->tokens_q >= most || a->tokens_q * a->heads >= most || a->tokens_k >= most)
+    return fail(FJX_ERR_UNSUPPORTED, "%s: tokens_q * heads and tokens_k must be below 2^31 - 128 (sequences + 2)", fn);
   const size_t es = esize(a->dtype);
   const int64_t d = a->head_dim;
   if (!packed_strides_ok(a->q_strides, a->heads, a->tokens_q, d, es) ||

@@ -64,7 +64,7 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkFormOf<T, DP, G, KS>:
     int qi, head;
     place.at(x < rows ? x : rows - 1, qi, head);
     head += kv * P.group;
-    lim[r] = P.causal ? qi + sp.nk - sp.nq + 1 : sp.nk;
+    lim[r] = P.causal ? qi + (sp.nk - sp.nq) + 1 : sp.nk;
     if (lg == 0 && form.part == 0) places[r][16 * form.group + li] = make_int2(x < rows ? head : -1, sp.q0 + qi);
     const T* q = P.q.p + head * P.q.head + (int64_t)(sp.q0 + qi) * P.q.token + 8 * lg;
 #pragma unroll
@@ -72,7 +72,7 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkFormOf<T, DP, G, KS>:
   }
   int q_last, h_last;
   place.at((kTileRows < rows ? kTileRows : rows) - 1, q_last, h_last);
-  const int most = P.causal ? q_last + sp.nk - sp.nq + 1 : sp.nk;  // keys that the workgroup's rows see
+  const int most = P.causal ? q_last + (sp.nk - sp.nq) + 1 : sp.nk;  // keys that the workgroup's rows see
   const int lim_lo = __builtin_amdgcn_readfirstlane(lim[0]);      // that all of the wave's rows see,
   const int lim_hi = row_w < rows ? __builtin_amdgcn_readlane(lim[R - 1], 15) : 0;  // and that any does
   const int blocks = most > 0 ? (int)((uint32_t)(most + Form::kBlock - 1) / Form::kBlock) : 0;

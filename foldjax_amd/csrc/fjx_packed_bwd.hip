@@ -67,7 +67,7 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkFormOf<T, DP, G, KS>:
     place.at(x < rows ? x : rows - 1, qi, head);
     head += kv * P.group;
     const int64_t token = sp.q0 + qi;
-    lim[r] = P.causal ? qi + sp.nk - sp.nq + 1 : sp.nk;
+    lim[r] = P.causal ? qi + (sp.nk - sp.nq) + 1 : sp.nk;
     if (lg == 0 && form.part == 0) places[r][16 * form.group + li] = make_int2(x < rows ? head : -1, (int)token);
     const T* q = P.q.p + head * P.q.head + token * P.q.token + 8 * lg;
     const T* dout = P.dout.p + head * P.dout.head + token * P.dout.token + 8 * lg;
@@ -103,7 +103,7 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkFormOf<T, DP, G, KS>:
   const bool far = __builtin_amdgcn_ballot_w64(any_far);
   int q_last, h_last;
   place.at((kTileRows < rows ? kTileRows : rows) - 1, q_last, h_last);
-  const int most = P.causal ? q_last + sp.nk - sp.nq + 1 : sp.nk;
+  const int most = P.causal ? q_last + (sp.nk - sp.nq) + 1 : sp.nk;
   const int lim_lo = __builtin_amdgcn_readfirstlane(lim[0]);
   const int lim_hi = row_w < rows ? __builtin_amdgcn_readlane(lim[R - 1], 15) : 0;
   const int blocks = most > 0 ? (int)((uint32_t)(most + Form::kBlock - 1) / Form::kBlock) : 0;

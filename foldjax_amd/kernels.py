@@ -1110,7 +1110,7 @@ def packed_attention_backward(
     Returns ``(dq, dk, dv)`` in the dtype and shape of q, k and v, a token's heads
     side by side in memory; gradients of shared heads are summed over the query
     heads, those of tokens of no sequence and of a cache's unused places are zeros.
-    The same bits each time. Without ``rest`` bfloat16 gradients of rows in which
+    dout is finite. The same bits each time. Without ``rest`` bfloat16 gradients of rows in which
     one key has nearly all the weight lose digits."""
     a, kept, unit, (key, _) = _packed_attention_args(q, k, v, q_starts, scale, causal, k_starts, k_lengths)
     key = None if key is None else (key, _layout(dout, out, lse, rest))

@@ -543,11 +543,12 @@ enum { FJX_INDEX_I32 = 0, FJX_INDEX_I64 = 1 };
  * results are then undefined, nothing outside is touched). causal: of nq queries
  * and nk keys, query i sees key j where j <= i + nk - nq (the last query sees all);
  * rows without a key are zeros, with zero gradients. k and v of a sequence's keys
- * are finite. Rows of out behind the last sequence are left as they are, or with
+ * (backward: dout too) are finite. Rows of out behind the last sequence are left as they are, or with
  * zero_tail written as zeros. `out` overlaps no input.
  * For the backward pass: lse [heads, tokens_q, 2] fp32, and `rest` (as out, of
  * bf16), what the output's rounding left.
- * Supported: head_dim a multiple of 8 up to 128. Scores, statistics and sums are
+ * Supported: head_dim a multiple of 8 up to 128, tokens_q * heads and tokens_k below
+ * 2^31 - 128 (sequences + 2), sequences below 2^22. Scores, statistics and sums are
  * fp32; bf16 weights enter the product with v rounded once, and their sum with them.
  */
 typedef struct fjx_packed_attention_args {

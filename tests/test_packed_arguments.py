@@ -226,3 +226,15 @@ def test_no_scratch_and_no_spills(src):
     assert found
     for name, m in found.items():
         assert m["private_segment_fixed_size"] == 0 and m["vgpr_spill_count"] == 0 and m["sgpr_spill_count"] == 0, (name, m)
+
+
+@pytest.mark.parametrize("more", [
+    {"tokens_q": 1 << 61}, {"tokens_q": (1 << 29) - 64}, {"tokens_k": (1 << 31) - 512}, {"tokens_k": (1 << 31) - 1},
+    {"sequences": (1 << 22) - 1, "tokens_q": (3 << 27)},
+], ids=str)
+def test_row_numbers_fit_32_bits(lib, more):
+    """Rows are numbered in 32 bits, up to the end of a tile of 128 behind each sequence."""
+    for call, a in ((lib.fjx_packed_attention_fwd, packed(**more)),
+                    (lib.fjx_packed_attention_bwd, _lib.PackedAttentionBwdArgs(fwd=packed(**more)))):
+        assert call(ctypes.byref(a), None) == 2
+        assert "2^31" in lib.fjx_last_error().decode()
