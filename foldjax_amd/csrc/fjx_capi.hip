@@ -1362,8 +1362,15 @@ PackedPlan packed_bwd_plan(int64_t tq, int64_t tk, int64_t seqs, int64_t heads, 
   const bool bf = dtype == FJX_DTYPE_BF16;
   PackedPlan p = {};
   p.splits = 1;
-  // workgroups that walk long and, causal, uneven ways: the heads that share keys in parts
-  if (group > 1 && tk && key_wgs < 1024) p.splits = (int)std::min<int64_t>(group, (1024 + key_wgs - 1) / key_wgs);
+  // Workgroups that walk long and, causal, uneven ways: the heads that share keys in parts,
+  // two rounds of the workgroups that the card holds (of 128 channels one a CU, else two), and
+  // two parts at least. us of the backward pass with 1 / 2 / 4 parts, causal: 64 workgroups of
+  // 2048 keys, d 128  179 / 117 / 87; 256, 1638, d 128  408 / 292 / 298; 512, 4096, d 128
+  // 961 / 901 / 912; 254, 4049, d 64  280 / 237 / 201
+  if (group > 1 && tk && key_wgs < 1024) {
+    const int64_t all = d > 64 ? 512 : 1024;
+    p.splits = (int)std::min(group, std::max<int64_t>(2, (all + key_wgs - 1) / key_wgs));
+  }
   if (tq) p.rows = packed_form(rows, seqs, wgs, walk, packed_few(bf, d), bf ? 1024 : INT64_MAX);
   // two tiles of keys a wave would take more registers than two waves a SIMD have at 128 channels
   if (tk) p.keys = packed_form(tk, seqs, key_wgs * p.splits, tq / seqs, packed_few(bf, d), bf && d <= 64 ? 2048 : INT64_MAX);
