@@ -1292,6 +1292,7 @@ struct PackedPlan {
   PackedForm rows, keys;
   int splits;                // of the keys (forward, keywise), of the heads that share keys (dk, dv)
   size_t part_o, part_ml;    // workspace bytes: forward; backward: one of dk, dv and D
+  int part_rows;
   size_t rows_order, keys_order;
 };
 int packed_width(int64_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
@@ -1362,14 +1363,15 @@ PackedPlan packed_bwd_plan(int64_t tq, int64_t tk, int64_t seqs, int64_t heads, 
   const bool bf = dtype == FJX_DTYPE_BF16;
   PackedPlan p = {};
   p.splits = 1;
-  // Workgroups that walk long and, causal, uneven ways: the heads that share keys in parts,
-  // two rounds of the workgroups that the card holds (of 128 channels one a CU, else two), and
-  // two parts at least. us of the backward pass with 1 / 2 / 4 parts, causal: 64 workgroups of
-  // 2048 keys, d 128  179 / 117 / 87; 256, 1638, d 128  408 / 292 / 298; 512, 4096, d 128
-  // 961 / 901 / 912; 254, 4049, d 64  280 / 237 / 201
+  // Workgroups that walk long and, causal, uneven ways: the heads that share keys in parts, of
+  // an eighth of a workgroup's share of the card (of 128 channels one a CU, else two) were the
+  // lengths alike. us of the backward pass with every tile in 4 parts / with parts of a half /
+  // an eighth / a 16th, causal: 8192 tokens in 5 sequences, d 128 (2 parts: 283)  291 / 316 /
+  // 270 / 270; one sequence of 8192, d 64  353 / 384 / 330 / 332; 4099 and 4000, d 64
+  // 199 / 210 / 188 / 187; one of 1003, d 64  30.4 / 32 / 31.0 / 31
   if (group > 1 && tk && key_wgs < 1024) {
-    const int64_t all = d > 64 ? 512 : 1024;
-    p.splits = (int)std::min(group, std::max<int64_t>(2, (all + key_wgs - 1) / key_wgs));
+    p.splits = (int)std::min(group, std::max<int64_t>(2, (1024 + key_wgs - 1) / key_wgs));
+    p.part_rows = (int)std::max<int64_t>(256, tq * group / seqs * key_wgs / (d > 64 ? 256 : 512) / 8);
   }
   if (tq) p.rows = packed_form(rows, seqs, wgs, walk, packed_few(bf, d), bf ? 1024 : INT64_MAX);
   // two tiles of keys a wave would take more registers than two waves a SIMD have at 128 channels
@@ -1490,6 +1492,7 @@ int packed_bwd_run(const fjx_packed_attention_bwd_args* b, const PackedPlan& pla
   p.dv = out(b->dv, b->dv_strides);
   p.zero_tail = 1;
   p.splits = plan.splits;
+  p.part_rows = plan.part_rows;
   p.part_dk = at<float>(a->workspace, 0);
   p.part_dv = at<float>(a->workspace, plan.part_o);
   p.delta = at<float>(a->workspace, 2 * plan.part_o);

@@ -12,6 +12,11 @@
 // channels, which half a row lies between when pairs are (i, i + half)). Angles are
 // taken in 64 bits and reduced in turns: float32 would lose 1e-2 of an angle at position
 // 1e5. A row stays in registers.
+//
+// Memory bounds it: queries and keys of 16384 tokens, 8 + 2 heads of 128, 17.1 us (84 MB,
+// 4.9 TB/s; a copy of as many bytes 16.1); with gradients at 8192 tokens 11.5 and 16.2, and
+// 3.8 for the workgroups' sums of the weights' gradients; smaller calls the latency of a
+// token's chain (positions, cosines in 64 bits, a row), 4.2.
 #include <type_traits>
 
 #include "fjx_common.hpp"

@@ -77,6 +77,7 @@ struct PackedParams {
   float* delta;                 // [H][tq]: rowsum(dO out)
   float* part_dk;               // [splits][Hk][tk][DP]
   float* part_dv;
+  int part_rows;                // rows of all heads that a part of a key tile walks, about
 };
 
 __device__ __forceinline__ int64_t packed_int(const PackedInts& a, int i, int64_t most) {

@@ -14,6 +14,15 @@
 // lose no longer sums to zero, and times the keys' common part it was as large as dq's
 // own rounding (0.0026 of dq against 0.0017). dk and dv sum over rows, where nothing
 // cancels so: weights and dS enter their products rounded once, relative to themselves.
+//
+// us of dq / dk and dv: a step of 8192 causal tokens in 5 sequences of 43 to 4099, 8 heads
+// of 128 on 2: 110 / 160 and the join; of 6 crops of 1 to 1003 residues, 16 heads of 24:
+// 19.8 / 18.4. No one thing bounds
+// them. In variants of the first that left out work, half the column fragments' reads were 3 % of
+// both, the exponentials and dS 4 %, the staging of further blocks 8 %, and all blocks but
+// the first left a quarter to a third: finding the tile, the first loads, the outputs.
+// Two tiles of keys a wave at 128 channels, on one wave a SIMD, halve the reads and
+// took 360 us where this takes 299.
 #include "fjx_packed.hpp"
 
 namespace fjx {
@@ -208,6 +217,25 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkFormOf<T, DP, G, KS>:
     });
 }
 
+// A key tile's walk: the blocks of queries in which any row sees its first key, and in how
+// many parts the heads that share it are dealt to workgroups: a tile's walk depends on its
+// sequence and, causal, its place in that, so that long ones have parts and short ones none.
+struct PkWalk {
+  int first, last, parts;
+  template <typename T>
+  __device__ __forceinline__ PkWalk(const PackedParams<T>& P, const PackedTile& sp, int key0, int block) {
+    const int shift = sp.nq - sp.nk;
+    first = (uint32_t)(P.causal && key0 + shift > 0 ? key0 + shift : 0) / block;
+    last = key0 < sp.nk ? (int)((uint32_t)(sp.nq + block - 1) / block) : 0;
+    if (last < first) last = first;
+    parts = 1;
+    if (P.splits > 1) {
+      const int n = (int)(((uint32_t)(last - first) * block * P.group + P.part_rows - 1) / P.part_rows);
+      parts = n < 1 ? 1 : n < P.splits ? n : P.splits;
+    }
+  }
+};
+
 // dk and dv: a wave holds R tiles of 16 keys, lane l key l % 16 of each, and walks the
 // queries of every head that shares them in tiles of 16: S = Q K^T and dP = dO V^T leave
 // the lane 4 queries of its own keys, as the operands of dV^T = dO^T P and dK^T = Q^T dS.
@@ -232,11 +260,14 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkFormOf<T, DP, G, KS>:
   const int t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const Form form(wave);
-  const int kvh = P.heads / P.group, kv = blockIdx.x, split = blockIdx.z;
+  const int kv = blockIdx.x / P.splits, part = blockIdx.x - kv * P.splits;
   PackedTile sp;
   if (!packed_tile(P, true, 1, kShift, P.tile0 + blockIdx.y, lane, sp)) return;
   const int key0 = sp.tile * kTileKeys;
   if (key0 >= sp.cap) return;
+  const PkWalk walk(P, sp, key0, Form::kBlock);
+  const int parts = __builtin_amdgcn_readfirstlane(walk.parts);
+  if (part >= parts) return;
   const int key_w = key0 + 16 * R * form.group;
   const int shift = sp.nq - sp.nk;  // a causal row i sees the keys up to i - shift
 
@@ -254,12 +285,8 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkFormOf<T, DP, G, KS>:
       vf[r][c] = in ? load8(v + 32 * c) : F{};
     }
   }
-  // the heads of this part, and the query blocks in which any row sees the first key
-  int h0 = 0, h1 = P.group;
-  if (P.splits > 1) h0 = P.group * split / P.splits, h1 = P.group * (split + 1) / P.splits;
-  const uint32_t q_first = P.causal && key0 + shift > 0 ? key0 + shift : 0;
-  const int qb0 = q_first / Form::kBlock;
-  const int qb1 = key0 < sp.nk ? (int)((uint32_t)(sp.nq + Form::kBlock - 1) / Form::kBlock) : 0;
+  const int h0 = P.group * part / parts, h1 = P.group * (part + 1) / parts;  // the heads of this part
+  const int qb0 = walk.first, qb1 = walk.last;
   const int turns = qb1 > qb0 ? (h1 - h0) * (qb1 - qb0) : 0;
 
   const int set = Form::kPrivate ? wave : 0;
@@ -413,12 +440,13 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkFormOf<T, DP, G, KS>:
         if (key >= sp.cap) return;
         const f32x8 v = Out::sum(x);
         const int64_t token = (int64_t)sp.k0 + key;
-        const float by = key < sp.nk ? i || L->splits > 1 ? 1.f : L->scale : 0.f;
+        const float by = key < sp.nk ? i || parts > 1 ? 1.f : L->scale : 0.f;
         float y[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) y[e] = by == 0.f ? 0.f : v[e] * by;
-        if (L->splits > 1) {
-          store8((i ? L->part_dv : L->part_dk) + (((int64_t)split * kvh + kv) * L->tk + token) * DP + c, pack8<float>(y));
+        if (parts > 1) {
+          const int kvh = L->heads / L->group;
+          store8((i ? L->part_dv : L->part_dk) + (((int64_t)part * kvh + kv) * L->tk + token) * DP + c, pack8<float>(y));
           return;
         }
         if (c >= L->d) return;
@@ -428,27 +456,33 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkFormOf<T, DP, G, KS>:
       });
 }
 
-// The parts of dk and dv (a part has some of the heads that share them) added: 4
-// elements a thread.
+// The parts of dk and dv added, where a tile (of 2^shift keys) has several: a workgroup 16
+// keys, 8 elements a thread.
 template <typename T, int DP>
-__global__ __launch_bounds__(256) void packed_dkv_join_kernel(PackedParams<T> P) {
-  const int kvh = P.heads / P.group;
-  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, all = (int64_t)kvh * P.tk * DP;
-  if (at >= all || at % DP >= P.d) return;
-  f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
-  for (int s = 0; s < P.splits; ++s) {
-    a += *reinterpret_cast<const f32x4*>(P.part_dk + s * all + at);
-    b += *reinterpret_cast<const f32x4*>(P.part_dv + s * all + at);
+__global__ __launch_bounds__(2 * DP) void packed_dkv_join_kernel(PackedParams<T> P, int shift, int block) {
+  PackedTile sp;
+  if (!packed_tile(P, true, 1, shift, P.tile0 + blockIdx.y, threadIdx.x & 63, sp)) return;
+  const int key0 = sp.tile << shift, kv = blockIdx.x, key = key0 + 16 * blockIdx.z + threadIdx.x / (DP / 8);
+  const int c = threadIdx.x % (DP / 8) * 8;
+  if (key >= sp.cap || c >= P.d) return;
+  const int parts = PkWalk(P, sp, key0, block).parts;
+  if (parts == 1) return;
+  const int64_t all = (int64_t)(P.heads / P.group) * P.tk * DP, token = (int64_t)sp.k0 + key;
+  const int64_t at = (kv * P.tk + token) * DP + c;
+  f32x8 a = load8(P.part_dk + at), b = load8(P.part_dv + at);
+  for (int s = 1; s < parts; ++s) {
+    a += load8(P.part_dk + s * all + at);
+    b += load8(P.part_dv + s * all + at);
   }
-  const int64_t row = at / DP, token = row % P.tk, kv = row / P.tk, col = at % DP;
-  const float x[4] = {a[0] * P.scale, a[1] * P.scale, a[2] * P.scale, a[3] * P.scale}, y[4] = {b[0], b[1], b[2], b[3]};
-  store4f(P.dk.p + kv * P.dk.head + token * P.dk.token + col, x);
-  store4f(P.dv.p + kv * P.dv.head + token * P.dv.token + col, y);
+  float x[8], y[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = a[e] * P.scale, y[e] = b[e];
+  store8(P.dk.p + kv * P.dk.head + token * P.dk.token + c, pack8<T>(x));
+  store8(P.dv.p + kv * P.dv.head + token * P.dv.token + c, pack8<T>(y));
 }
 
 template <typename T, int DP>
 void bwd(PackedParams<T> P, const PackedForm& rows, const PackedForm& keys, hipStream_t st) {
-  const int kvh = P.heads / P.group;
   const int splits = P.splits;
   launch_packed_order(P, rows, keys, st);
   P.splits = 1;
@@ -470,11 +504,13 @@ void bwd(PackedParams<T> P, const PackedForm& rows, const PackedForm& keys, hipS
     // a SIMD have, and are taken only where workgroups are many
     if constexpr (DP * R <= 128 && (KS * R <= 2 || G == 1))
       pk_grid(P, [&](const PackedParams<T>& Q, dim3 grid) {
-        packed_dkv_kernel<T, DP, G, KS, R><<<grid, PkForm<G, KS>::kThreads, 0, st>>>(Q);
+        // a tile's parts side by side, so that the longest tiles begin with all of theirs
+        packed_dkv_kernel<T, DP, G, KS, R><<<dim3(grid.x * splits, grid.y), PkForm<G, KS>::kThreads, 0, st>>>(Q);
+        if (splits > 1)
+          packed_dkv_join_kernel<T, DP><<<dim3(grid.x, grid.y, G * R), 2 * DP, 0, st>>>(Q, __builtin_ctz(keys.rows()),
+                                                                                        PkFormOf<T, DP, G, KS>::type::kBlock);
       });
   });
-  if (splits > 1)
-    packed_dkv_join_kernel<T, DP><<<(unsigned)(((int64_t)kvh * P.tk * DP / 4 + 255) / 256), 256, 0, st>>>(P);
 }
 
 }  // namespace
