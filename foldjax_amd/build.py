@@ -51,7 +51,8 @@ def _hipcc() -> str:
 # attention's flash kernel 27 % faster with iterative-ilp; the other files
 # measured no better or slower with either. Differential attention's kernels
 # read every accumulator they make as well (a token against 16384 keys 33.7 ->
-# 31.5 us, the float32 gradients 3 % faster, the rest within 1 %).
+# 31.5 us, the float32 gradients 3 % faster, the rest within 1 %), and so do
+# packed attention's.
 FILE_FLAGS = {
     "fjx_diffattn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "fjx_diffattn_bwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],

@@ -16,8 +16,8 @@
 // cancels so: weights and dS enter their products rounded once, relative to themselves.
 //
 // us of dq / dk and dv: a step of 8192 causal tokens in 5 sequences of 43 to 4099, 8 heads
-// of 128 on 2: 110 / 160 and the join; of 6 crops of 1 to 1003 residues, 16 heads of 24:
-// 19.8 / 18.4. No one thing bounds
+// of 128 on 2: 110 / 143 and the join's 13; of 6 crops of 1 to 1003 residues, 16 heads of 24:
+// 19.3 / 18.5. No one thing bounds
 // them. In variants of the first that left out work, half the column fragments' reads were 3 % of
 // both, the exponentials and dS 4 %, the staging of further blocks 8 %, and all blocks but
 // the first left a quarter to a third: finding the tile, the first loads, the outputs.
