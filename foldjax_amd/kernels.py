@@ -1001,15 +1001,15 @@ def _packed_attention_args(q, k, v, q_starts, scale, causal, k_starts, k_lengths
     else:
         _need_shape("k_starts", k_starts, (seqs + 1,))
     _need_shape("k_lengths", k_lengths, (seqs,))
-    index = _INDEX.get(q_starts.dtype)
-    if index is None:
-        raise ValueError(f"q_starts must be int32 or int64, got {q_starts.dtype}")
-    for name, t in (("k_starts", k_starts), ("k_lengths", k_lengths)):
+    offsets = (q_starts, k_starts, k_lengths)
+    for name, t in zip(("q_starts", "k_starts", "k_lengths"), offsets):
         if t is not None and t.dtype not in _INDEX:
             raise ValueError(f"{name} must be int32 or int64, got {t.dtype}")
+    wide = torch.int64 if any(t is not None and t.dtype is torch.int64 for t in offsets) else torch.int32
+    index = _INDEX[wide]
     _dev(q)
-    given = (q, k, v, q_starts, k_starts, k_lengths)
-    q_starts, k_starts, k_lengths = (_like(t, q_starts.dtype) for t in (q_starts, k_starts, k_lengths))
+    given = (q, k, v, *offsets)
+    q_starts, k_starts, k_lengths = (_like(t, wide) for t in offsets)
     unit = 4 if dtype is torch.float32 else 8
     q, qst = _packed_heads(q, unit)
     k, kst = _packed_heads(k, unit)
@@ -1110,7 +1110,8 @@ def packed_attention_backward(
     Returns ``(dq, dk, dv)`` in the dtype and shape of q, k and v, a token's heads
     side by side in memory; gradients of shared heads are summed over the query
     heads, those of tokens of no sequence and of a cache's unused places are zeros.
-    dout is finite. The same bits each time. Without ``rest`` bfloat16 gradients of rows in which
+    dout is finite; other values than numbers in a row of q may reach the gradients of all
+    its sequence's keys. The same bits each time. Without ``rest`` bfloat16 gradients of rows in which
     one key has nearly all the weight lose digits."""
     a, kept, unit, (key, _) = _packed_attention_args(q, k, v, q_starts, scale, causal, k_starts, k_lengths)
     key = None if key is None else (key, _layout(dout, out, lse, rest))

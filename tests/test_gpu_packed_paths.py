@@ -154,3 +154,49 @@ def test_many_workgroups(lens, h, kv, d, dtype, causal):
     q, k, v, dout = inputs(lens, h, kv, d, dtype, seed=27)
     more = {"scale": d**-0.5, "causal": causal}
     compare(run(q, k, v, ints(starts(lens)), dout, **more), O.attention(q, k, v, starts(lens), dout=dout, **more))
+
+
+@pytest.mark.parametrize("h,kv", [(1024, 1), (96, 1), (90, 2), (1000, 1000)])
+def test_many_heads(h, kv):
+    """Groups of heads that are no powers of two and of more heads than a tile has rows."""
+    say(f"packed heads {h} {kv}")
+    lens = [3, 1, 17]
+    q, k, v, dout = inputs(lens, h, kv, 8, BF16, tail=2, seed=h)
+    more = {"scale": 0.35, "causal": True}
+    compare(run(q, k, v, ints(starts(lens)), dout, **more), O.attention(q, k, v, starts(lens), dout=dout, **more))
+    room = [100, 90, 300]  # a cache, walked by waves with keys of their own
+    g = torch.Generator(device="cuda").manual_seed(h)
+    k, v = (heads(g, sum(room), kv, 8, BF16) for _ in range(2))
+    got = run(q, k, v, ints(starts(lens)), dout, k_starts=ints(starts(room)), **more)
+    compare(got, O.attention(q, k, v, starts(lens), k_starts=starts(room), dout=dout, **more))
+
+
+def test_gradients_of_keys_without_queries():
+    say("packed no queries")
+    k = torch.ones(2, 50, 32, dtype=BF16, device="cuda")
+    q = torch.ones(4, 0, 32, dtype=BF16, device="cuda")
+    more = {"k_starts": ints([0, 20, 45]), "scale": 1.0}
+    out, lse, rest = kernels.packed_attention(q, k, k, ints([0, 0, 0]), return_lse=True, **more)
+    for t in kernels.packed_attention_backward(q, q, k, k, out, lse, rest, ints([0, 0, 0]), **more):
+        assert t.shape[1] in (0, 50) and (t == 0).all()
+
+
+def test_offsets_of_two_types_and_of_every_second_place():
+    say("packed offsets of two types")
+    lens, d = [40, 25, 30], 32
+    q, k, v, dout = inputs(lens, 4, 2, d, BF16, seed=28)
+    st = starts(lens)
+    want = run(q, k, v, ints(st), dout, scale=0.2, k_starts=ints(st), k_lengths=ints([40, 20, 30]))
+    apart = torch.stack([ints(st), ints(st) - 7], 1)[:, 0]
+    got = run(q, k, v, apart, dout, scale=0.2, k_starts=ints([*st[:-1], 2**40], torch.int64), k_lengths=ints([40, 20, 2**33 + 1], torch.int64))
+    assert all(torch.equal(got[n], want[n]) for n in want)
+
+
+def test_heads_that_are_one():
+    """k and v broadcast over heads, q over tokens: taken by copies, gradients of each place."""
+    say("packed broadcast")
+    lens, d = [30, 9], 16
+    q, k, v, dout = inputs(lens, 4, 4, d, FP32, seed=29)
+    q, k, v = q[:, :1].expand(-1, 39, -1), k[:1].expand(4, -1, -1), v[:1].expand(4, -1, -1)
+    got = run(q, k, v, ints(starts(lens)), dout, scale=0.3, causal=True)
+    compare(got, O.attention(q, k, v, starts(lens), scale=0.3, causal=True, dout=dout))
