@@ -1113,14 +1113,27 @@ def packed_attention_backward(
     dout is finite; other values than numbers in a row of q may reach the gradients of all
     its sequence's keys. The same bits each time. Without ``rest`` bfloat16 gradients of rows in which
     one key has nearly all the weight lose digits."""
-    a, kept, unit, (key, _) = _packed_attention_args(q, k, v, q_starts, scale, causal, k_starts, k_lengths)
-    key = None if key is None else (key, _layout(dout, out, lse, rest))
-    seen = None if key is None else _BLOCKS.get(key)
-    if seen is not None and not (dout.data_ptr() | out.data_ptr() | (0 if rest is None else rest.data_ptr())) & 15:
+    scale, causal = float(scale), bool(causal)
+    key = (_layout(q, k, v, q_starts, k_starts, k_lengths, dout, out, lse, rest), scale, causal)
+    seen = _BLOCKS.get(key)
+    fits = False
+    if seen is not None:
         block, nbytes = seen
         g = _lib.PackedAttentionBwdArgs.from_buffer_copy(block)
-        a.out_strides, a.rest_strides = g.fwd.out_strides, g.fwd.rest_strides
+        a = g.fwd
+        a.q, a.k, a.v, a.out, g.dout = qp, kp, vp, op, dp = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                                                             dout.data_ptr())
+        if rest is not None:
+            a.rest = rp = rest.data_ptr()
+            op |= rp
+        fits = not (qp | kp | vp | op | dp) & 15
+    if fits:
+        a.lse, a.q_starts = lse.data_ptr(), q_starts.data_ptr()
+        a.k_starts = a.q_starts if k_starts is None else k_starts.data_ptr()
+        if k_lengths is not None:
+            a.k_lengths = k_lengths.data_ptr()
     else:
+        a, kept, unit, (as_they_lie, _) = _packed_attention_args(q, k, v, q_starts, scale, causal, k_starts, k_lengths)
         _same_place(q, q.dtype, dout=dout, out=out, rest=rest)
         _same_place(q, torch.float32, lse=lse)
         _need_shape("dout", dout, q.shape)
@@ -1136,18 +1149,18 @@ def packed_attention_backward(
         if rest is not None:
             rest, a.rest_strides = _packed_heads(rest, unit)
         by_q, by_k = (a.head_dim, a.heads * a.head_dim), (a.head_dim, a.kv_heads * a.head_dim)
-        g = _lib.PackedAttentionBwdArgs(a, None, None, None, None, dst, by_q, by_k, by_k)
+        a.out, a.lse, a.rest = out.data_ptr(), lse.data_ptr(), _ptr(rest)
+        g = _lib.PackedAttentionBwdArgs(a, dout.data_ptr(), None, None, None, dst, by_q, by_k, by_k)
         nbytes = _lib.load().fjx_packed_attention_bwd_workspace_size(a.tokens_q, a.tokens_k, a.sequences, a.heads, a.kv_heads,
                                                                      a.head_dim, a.dtype)
-        if key is not None and all(x is y for x, y in zip((dout, out, lse, rest), given)):
+        if as_they_lie is not None and all(x is y for x, y in zip((dout, out, lse, rest), given)):
             _remember(key, (bytes(g), nbytes))
+        a = g.fwd
     dq, dk, dv = (_token_major(*t.shape, q) for t in (q, k, v))
-    a.out, a.lse, a.rest = out.data_ptr(), lse.data_ptr(), _ptr(rest)
     if nbytes:
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
         a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
-    g.fwd = a
-    g.dout, g.dq, g.dk, g.dv = dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+    g.dq, g.dk, g.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
     _launch(_lib.load().fjx_packed_attention_bwd, g, q)
     return dq, dk, dv
 
@@ -1172,7 +1185,7 @@ def _rotary_args(q, k, positions, frequencies, q_weight, k_weight, eps, sections
     to, the elements of a 16-byte piece, the strides of outputs like q and k, and its
     key."""
     eps, interleaved = float(eps), bool(interleaved)
-    sections = None if sections is None else tuple(int(n) for n in sections)
+    sections = None if sections is None else tuple([int(n) for n in sections])
     key = (_layout(q, k, positions, frequencies, q_weight, k_weight), eps, sections, interleaved, "rotary")
     seen = _BLOCKS.get(key)
     if seen is not None:
@@ -1329,15 +1342,31 @@ def head_norm_rotary_backward(
     ``(dx_q, dx_k, dq_weight, dk_weight)``: the inputs' in their dtype and shape, a
     token's heads side by side in memory, the weights' float32 ``[D]``, summed over
     tokens and heads in one order; None for what is not there."""
-    a, kept, unit, like, key = _rotary_args(q, k, positions, frequencies, q_weight, k_weight, eps, sections, interleaved)
-    key = None if key is None else (key, _layout(dq, dk))
-    seen = None if key is None else _BLOCKS.get(key)
-    lib = _lib.load()
-    if seen is not None and not (dq.data_ptr() | (0 if dk is None else dk.data_ptr())) & 15:
-        block, nbytes = seen
+    eps, interleaved = float(eps), bool(interleaved)
+    sections = None if sections is None else tuple([int(n) for n in sections])
+    key = (_layout(q, k, positions, frequencies, q_weight, k_weight, dq, dk), eps, sections, interleaved)
+    seen = _BLOCKS.get(key)
+    fits = False
+    if seen is not None:
+        block, nbytes, like = seen
         b = _lib.HeadNormRotaryBwdArgs.from_buffer_copy(block)
-        a.q_out_strides, a.k_out_strides = b.fwd.q_out_strides, b.fwd.k_out_strides
+        a = b.fwd
+        a.q, a.q_out = p, yp = q.data_ptr(), dq.data_ptr()
+        p |= yp
+        if k is not None:
+            a.k, a.k_out = kp, yp = k.data_ptr(), dk.data_ptr()
+            p |= kp | yp
+        if q_weight is not None:
+            a.q_weight = wp = q_weight.data_ptr()
+            p |= wp
+        if k_weight is not None:
+            a.k_weight = wp = k_weight.data_ptr()
+            p |= wp
+        fits = not p & 15
+    if fits:
+        a.positions, a.frequencies = positions.data_ptr(), frequencies.data_ptr()
     else:
+        a, kept, unit, like, as_they_lie = _rotary_args(q, k, positions, frequencies, q_weight, k_weight, eps, sections, interleaved)
         if (dk is None) != (k is None):
             raise ValueError("dk must be given where k is, and only there")
         _same_place(q, q.dtype, dq=dq, dk=dk)
@@ -1346,32 +1375,33 @@ def head_norm_rotary_backward(
             _need_shape("dk", dk, k.shape)
         given = dq, dk
         dq, a.q_out_strides = _heads(dq, unit)
+        a.q_out = dq.data_ptr()
         if dk is not None:
             dk, a.k_out_strides = _heads(dk, unit)
+            a.k_out = dk.data_ptr()
         packed = lambda h: (a.tokens * h * a.head_dim, a.head_dim, h * a.head_dim)  # noqa: E731
         b = _lib.HeadNormRotaryBwdArgs(a, None, None, packed(a.heads), packed(a.kv_heads))
         nbytes = 0
         if q_weight is not None or k_weight is not None:
-            nbytes = lib.fjx_head_norm_rotary_bwd_workspace_size(a.items, a.heads, a.kv_heads, a.tokens, a.head_dim)
-        if key is not None and dq is given[0] and dk is given[1]:
-            _remember(key, (bytes(b), nbytes))
-    dev = q.device
+            nbytes = _lib.load().fjx_head_norm_rotary_bwd_workspace_size(a.items, a.heads, a.kv_heads, a.tokens, a.head_dim)
+        if as_they_lie is not None and dq is given[0] and dk is given[1]:
+            _remember(key, (bytes(b), nbytes, like))
+    dev, d = q.device, q.shape[-1]
     gq, gk, dwq, dwk = _like_heads(q, like[0]), None, None, None
-    a.q_out, b.dq = dq.data_ptr(), gq.data_ptr()
+    b.dq = gq.data_ptr()
     if k is not None:
         gk = _like_heads(k, like[1])
-        a.k_out, b.dk = dk.data_ptr(), gk.data_ptr()
+        b.dk = gk.data_ptr()
     if q_weight is not None:
-        dwq = torch.empty(a.head_dim, dtype=torch.float32, device=dev)
+        dwq = torch.empty(d, dtype=torch.float32, device=dev)
         b.dq_weight = dwq.data_ptr()
     if k_weight is not None:
-        dwk = torch.empty(a.head_dim, dtype=torch.float32, device=dev)
+        dwk = torch.empty(d, dtype=torch.float32, device=dev)
         b.dk_weight = dwk.data_ptr()
     if nbytes:
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         b.workspace, b.workspace_bytes = ws.data_ptr(), nbytes
-    b.fwd = a
-    _launch(lib.fjx_head_norm_rotary_bwd, b, q)
+    _launch(_lib.load().fjx_head_norm_rotary_bwd, b, q)
     return gq, gk, dwq, dwk
 
 
