@@ -165,7 +165,7 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkFormOf<T, DP, G, KS>:
 #pragma unroll
         for (int kt = 0; kt < kNt; ++kt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) top[r] = fmaxf(top[r], s[r][kt][e]);
+          for (int e = 0; e < 4; ++e) top[r] = pk_most(top[r], s[r][kt][e]);
         top[r] = lanes4_max(top[r]) * P.scale_log2;
         moved = moved || top[r] > m[r] + kSlack;
       }

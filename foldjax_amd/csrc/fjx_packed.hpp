@@ -448,15 +448,19 @@ struct PkOut {
   }
 };
 
+// The larger of two, NaN if either is: unlike fmaxf it takes values as they come, three at a
+// time (17 -> 13 instructions for 16 scores and the lanes; 1 % of the forward pass).
+__device__ __forceinline__ float pk_most(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
 // max over the 4 lanes {l % 16 + 16 g}
 __device__ __forceinline__ float lanes4_max(float x) {
   const uint32_t u = __builtin_bit_cast(uint32_t, x);
   const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
   const uint32_t a0 = a[0], a1 = a[1];
-  const uint32_t v = __builtin_bit_cast(uint32_t, fmaxf(__builtin_bit_cast(float, a0), __builtin_bit_cast(float, a1)));
+  const uint32_t v = __builtin_bit_cast(uint32_t, pk_most(__builtin_bit_cast(float, a0), __builtin_bit_cast(float, a1)));
   const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
   const uint32_t b0 = b[0], b1 = b[1];
-  return fmaxf(__builtin_bit_cast(float, b0), __builtin_bit_cast(float, b1));
+  return pk_most(__builtin_bit_cast(float, b0), __builtin_bit_cast(float, b1));
 }
 
 // launch(P, grid) for a call's workgroups: key/value heads, tiles and parts, in as many

@@ -31,9 +31,20 @@ namespace {
 
 constexpr float kFar = 16777216.f;  // as in the forward pass
 
-// a weight's exponent from its score's sum s: by = 1 for scores that were multiplied
-__device__ __forceinline__ float pk_weight(float s, float by, float m, float log_sum) {
-  return __builtin_amdgcn_exp2f(fmaf(s, by, -m) - log_sum);
+// The exponent of a weight is s scale log2(e) - M - log2 l. bf16 rows whose |M| is up to
+// kNear take M + log2 l as one number, half a step of which, 2^-13, is a 16th of a weight's
+// own rounding: one fma. Others have M subtracted from their scores (rounded products where
+// they are far, as in the forward pass) and the logarithm apart.
+constexpr float kNear = 2048.f;
+template <typename T> constexpr bool kJoined = sizeof(T) == 2;
+template <int N, typename M>
+__device__ __forceinline__ void pk_less(float scale, bool far, M m, f32x4 (&s)[N]) {
+  if (far) pk_round(scale, s);
+  const float by = far ? 1.f : scale;
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[j][e] = fmaf(s[j][e], by, -m(j, e));
 }
 
 // dq, and D for the other kernel: rows and blocks as in the forward pass.
@@ -68,7 +79,7 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkFormOf<T, DP, G, KS>:
   int lim[R];
   F qf[R][kC], dof[R][kC];
   float m[R], log_sum[R], delta[R];
-  bool any_far = false;
+  bool any_far = false, any_off = false;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const int x = row_w + 16 * r + li;
@@ -107,9 +118,14 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkFormOf<T, DP, G, KS>:
     m[r] = stats[0];
     log_sum[r] = stats[1];
     any_far = any_far || fabsf(m[r]) > kFar;
+    any_off = any_off || !kJoined<T> || fabsf(m[r]) > kNear;
     if (lg == 0 && form.part == 0 && x < rows) P.delta[at_row] = delta[r];
   }
-  const bool far = __builtin_amdgcn_ballot_w64(any_far);
+  const bool far = __builtin_amdgcn_ballot_w64(any_far), off = __builtin_amdgcn_ballot_w64(any_off);
+  const float by = off ? 1.f : P.scale_log2;
+  float base[R];  // what is still to be subtracted from a score times by
+#pragma unroll
+  for (int r = 0; r < R; ++r) base[r] = off ? log_sum[r] : m[r] + log_sum[r];
   int q_last, h_last;
   place.at((kTileRows < rows ? kTileRows : rows) - 1, q_last, h_last);
   const int most = P.causal ? q_last + (sp.nk - sp.nq) + 1 : sp.nk;
@@ -159,7 +175,10 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkFormOf<T, DP, G, KS>:
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) s[r][j] = dp[r][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+          for (int j = 0; j < 2; ++j) {
+            s[r][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            dp[r][j] = f32x4{-delta[r], -delta[r], -delta[r], -delta[r]};  // dP - D from the start
+          }
         pk_ahead<2 * kC>([&](int i) { return at.at_row(kt_, 32 * pair + 16 * (i / kC), i % kC); },
                          [&](int i, const F& kf) {
 #pragma unroll
@@ -170,11 +189,9 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkFormOf<T, DP, G, KS>:
 #pragma unroll
                            for (int r = 0; r < R; ++r) mma(dp[r][i / kC], vf, dof[r][i % kC]);
                          });
-        float by = P.scale_log2;
-        if (far) {
-          by = 1.f;
+        if (off) {
 #pragma unroll
-          for (int r = 0; r < R; ++r) pk_round(P.scale_log2, s[r]);
+          for (int r = 0; r < R; ++r) pk_less(P.scale_log2, far, [&](int, int) { return m[r]; }, s[r]);
         }
         if (masked) {
 #pragma unroll
@@ -192,7 +209,7 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkFormOf<T, DP, G, KS>:
           float ds[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            ds[e] = pk_weight(s[r][e >> 2][e & 3], by, m[r], log_sum[r]) * (dp[r][e >> 2][e & 3] - delta[r]);
+            ds[e] = __builtin_amdgcn_exp2f(fmaf(s[r][e >> 2][e & 3], by, -base[r])) * dp[r][e >> 2][e & 3];
           parts(ds, dsf[r]);
         }
         pk_ahead<kU>([&](int u) { return at.at_col(kt_, 32 * pair, u); },
@@ -254,8 +271,8 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkFormOf<T, DP, G, KS>:
   typedef PkOut<Form, DP> Out;
   constexpr int kRaw = kStages * 2 * kOperand * kSets;  // and at the end the outputs' way
   __shared__ __attribute__((aligned(16))) unsigned char raw[kRaw > Out::kBytes ? kRaw : Out::kBytes];
-  __shared__ __attribute__((aligned(16))) float rowstat[kSets][kStages][3][Form::kStage];  // M, log2 of the sum, D
-  __shared__ int rowfar[kSets][kStages][Form::kRest];
+  __shared__ __attribute__((aligned(16))) float rowstat[kSets][kStages][3 + kJoined<T>][Form::kStage];  // M, log2 of the sum, -D, M + the second
+  __shared__ int rowfar[kSets][kStages][Form::kRest];  // 1: a row past kNear, 2: one past kFar
 
   const int t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -323,8 +340,10 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkFormOf<T, DP, G, KS>:
     if (stat_row < Form::kStage) {
       rowstat[set][at][0][stat_row] = st_m[0];
       rowstat[set][at][1][stat_row] = st_m[1];
-      rowstat[set][at][2][stat_row] = st_d;
-      const bool far = __builtin_amdgcn_ballot_w64(fabsf(st_m[0]) > kFar);
+      rowstat[set][at][2][stat_row] = -st_d;
+      if constexpr (kJoined<T>) rowstat[set][at][3][stat_row] = st_m[0] + st_m[1];
+      const int far = (__builtin_amdgcn_ballot_w64(!kJoined<T> || fabsf(st_m[0]) > kNear) ? 1 : 0) |
+                      (__builtin_amdgcn_ballot_w64(fabsf(st_m[0]) > kFar) ? 2 : 0);
       if (stat_row % 64 == 0) rowfar[set][at][stat_row / 64] = far;
     }
   };
@@ -362,14 +381,24 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkFormOf<T, DP, G, KS>:
       int any_far = 0;
 #pragma unroll
       for (int i = 0; i < Form::kRest; ++i) any_far |= rowfar[set][cur][i];
-      const bool far = __builtin_amdgcn_readfirstlane(any_far);
+      const int flags = __builtin_amdgcn_readfirstlane(any_far);
+      const bool off = flags & 1, far = flags & 2;
+      const float by = off ? 1.f : P.scale_log2;
+      const float* const stats = rowstat[set][cur][0];
+      const float* const bases = rowstat[set][cur][kJoined<T> && !off ? 3 : 1];
 #pragma unroll
       for (int pair = 0; pair < kNt / 2; ++pair) {
         f32x4 s[R][2], dp[R][2];
+        const int row = form.at + 32 * pair + 4 * lg;
 #pragma unroll
-        for (int r = 0; r < R; ++r)
+        for (int j = 0; j < 2; ++j) {
+          const f32x4 d4 = *reinterpret_cast<const f32x4*>(stats + 2 * Form::kStage + row + 16 * j);
 #pragma unroll
-          for (int j = 0; j < 2; ++j) s[r][j] = dp[r][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+          for (int r = 0; r < R; ++r) {
+            s[r][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            dp[r][j] = d4;  // dP - D from the start
+          }
+        }
         pk_ahead<2 * kC>([&](int i) { return at.at_row(qt_, 32 * pair + 16 * (i / kC), i % kC); },
                          [&](int i, const F& qf) {
 #pragma unroll
@@ -380,11 +409,12 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkFormOf<T, DP, G, KS>:
 #pragma unroll
                            for (int r = 0; r < R; ++r) mma(dp[r][i / kC], of, vf[r][i % kC]);
                          });
-        float by = P.scale_log2;
-        if (far) {
-          by = 1.f;
+        if (off) {
+          f32x4 m4[2];
 #pragma unroll
-          for (int r = 0; r < R; ++r) pk_round(P.scale_log2, s[r]);
+          for (int j = 0; j < 2; ++j) m4[j] = *reinterpret_cast<const f32x4*>(stats + row + 16 * j);
+#pragma unroll
+          for (int r = 0; r < R; ++r) pk_less(P.scale_log2, far, [&](int j, int e) { return m4[j][e]; }, s[r]);
         }
         if (masked) {
 #pragma unroll
@@ -399,17 +429,14 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkFormOf<T, DP, G, KS>:
         F pf[R], dsf[R];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const int row = form.at + 32 * pair + 16 * j + 4 * lg;
-          const f32x4 m4 = *reinterpret_cast<const f32x4*>(&rowstat[set][cur][0][row]);
-          const f32x4 l4 = *reinterpret_cast<const f32x4*>(&rowstat[set][cur][1][row]);
-          const f32x4 d4 = *reinterpret_cast<const f32x4*>(&rowstat[set][cur][2][row]);
+          const f32x4 b4 = *reinterpret_cast<const f32x4*>(bases + row + 16 * j);
 #pragma unroll
           for (int r = 0; r < R; ++r)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float p = pk_weight(s[r][j][e], by, m4[e], l4[e]);
+              const float p = __builtin_amdgcn_exp2f(fmaf(s[r][j][e], by, -b4[e]));
               pf[r][4 * j + e] = from_f32<T>(p);
-              dsf[r][4 * j + e] = from_f32<T>(p * (dp[r][j][e] - d4[e]));
+              dsf[r][4 * j + e] = from_f32<T>(p * dp[r][j][e]);
             }
         }
         pk_ahead<2 * kU>([&](int i) { return at.at_col(i & 1 ? qt_ : ot_, 32 * pair, i / 2); },

@@ -200,3 +200,23 @@ def test_heads_that_are_one():
     q, k, v = q[:, :1].expand(-1, 39, -1), k[:1].expand(4, -1, -1), v[:1].expand(4, -1, -1)
     got = run(q, k, v, ints(starts(lens)), dout, scale=0.3, causal=True)
     compare(got, O.attention(q, k, v, starts(lens), scale=0.3, causal=True, dout=dout))
+
+
+@DTYPES
+@pytest.mark.parametrize("size", [2.0**10, 2.0**12, 2.0**20, 2.0**23])
+def test_equal_scores_of_any_size(size, dtype):
+    """Scores that are all the same have the same weights, 1 / 20, however far from zero, beside
+    rows of small scores: the weight's own rounding, a sum of 20 and the output's."""
+    say(f"packed equal scores {size} {dtype}")
+    n, d = 20, 32
+    root = 2.0 ** int(torch.tensor(size).log2().item() // 2)
+    q, k = (torch.zeros(2, n, d, dtype=dtype, device="cuda") for _ in range(2))
+    q[0, :, 0], k[..., 0] = size / root, root
+    g = torch.Generator(device="cuda").manual_seed(30)
+    v, dout = (torch.randn(2, n, d, generator=g, device="cuda").to(dtype) for _ in range(2))
+    got = run(q, k, v, ints([0, n]), dout, scale=0.7)
+    u = torch.finfo(dtype).eps / 2 + 40 * 2.0**-24
+    want, room = v.double().mean(1, keepdim=True), v.double().abs().mean(1, keepdim=True)
+    assert ((got["out"].double() - want).abs() <= u * (2 * room + want.abs())).all()
+    want, room = dout.double().mean(1, keepdim=True), dout.double().abs().mean(1, keepdim=True)
+    assert ((got["dv"].double() - want).abs() <= u * (2 * room + want.abs())).all()
