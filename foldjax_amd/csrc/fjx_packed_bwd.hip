@@ -1,7 +1,7 @@
 // Packed attention, backward. With dP = dO v^T and D = rowsum(dO out):
 //   dS = P (dP - D),  dq = scale dS k,  dk = scale dS^T q,  dv = P^T dO
 // The weights come again from the scores and the forward pass's row statistics, the
-// maximum M and log2 of the sum l, kept apart: P = 2^((s scale log2(e) - M) - log2 l).
+// maximum M and log2 of the sum l: P = 2^(s scale log2(e) - M - log2 l).
 // Every sum has one owner and one order: no atomics, and the same bits each time. So
 // dq and the keys' gradients are two walks with the scores and dP taken twice, seven
 // products in place of five.
@@ -16,13 +16,14 @@
 // cancels so: weights and dS enter their products rounded once, relative to themselves.
 //
 // us of dq / dk and dv: a step of 8192 causal tokens in 5 sequences of 43 to 4099, 8 heads
-// of 128 on 2: 110 / 143 and the join's 13; of 6 crops of 1 to 1003 residues, 16 heads of 24:
-// 19.3 / 18.5. No one thing bounds
-// them. In variants of the first that left out work, half the column fragments' reads were 3 % of
-// both, the exponentials and dS 4 %, the staging of further blocks 8 %, and all blocks but
-// the first left a quarter to a third: finding the tile, the first loads, the outputs.
-// Two tiles of keys a wave at 128 channels, on one wave a SIMD, halve the reads and
-// took 360 us where this takes 299.
+// of 128 on 2: 106 / 142 and the join's 13; of 6 crops of 1 to 1003 residues, 16 heads of
+// 24: 18.7 / 17.9. No one thing bounds them. In variants of the first that left out work,
+// half the column fragments' reads were 3 % of both, the exponentials and dS 4 %, the
+// staging of further blocks 8 %, and all blocks but the first left a quarter to a third:
+// finding the tile, the first loads, the outputs. Vector instructions a score, one of them
+// an exponential: 5 for dq, 4 for dk and dv (7 and 6 with D and the logarithm subtracted
+// by themselves: 5 % and 2 % slower). Two tiles of keys a wave at 128 channels, on one
+// wave a SIMD, halve the reads and took 360 us where two waves take 299.
 #include "fjx_packed.hpp"
 
 namespace fjx {
