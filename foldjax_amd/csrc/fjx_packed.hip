@@ -21,9 +21,9 @@ namespace {
 // from LDS a product ahead. What bounds it: long prompts the issue of vector beside matrix
 // instructions (16384 causal tokens in 6 sequences of up to 9001, 8 heads of 128 on 2: 226 us,
 // 970 TFLOP/s, where a large product reaches 1400); narrow heads the vector instructions,
-// 5 a score and one of them an exponential, against two matrix products of 24 channels, and the ways in and out (6 crops
-// of 1 to 1003 residues, 16 heads of 24: 14.3 us, of them 3.4 until a workgroup's first
-// block is there and 5.8 walking); single tokens memory (8 caches of 9 to 16384 tokens:
+// 5 a score and one of them an exponential, against two matrix products of 24 channels,
+// and the ways in and out (6 crops of 1 to 1003 residues, 16 heads of 24: 14.3 us, of them
+// 3.4 until a workgroup's first block is there and 5.8 walking); single tokens memory (8 caches of 9 to 16384 tokens:
 // 19.0 us, 4.6 TB/s, and the join 4.4).
 constexpr float kSlack = 8.f;
 
