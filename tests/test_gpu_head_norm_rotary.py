@@ -179,3 +179,34 @@ def test_streams_graphs_and_the_same_bits():
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(held, step()))
         q.float().sum().item()
+
+
+@pytest.mark.parametrize("interleaved", [False, True], ids=["halves", "neighbours"])
+def test_gradients_against_differences(interleaved):
+    """The gradient along a direction of length 1 is the change of sum(y dy) along it, in
+    float32: the difference's own error is its third derivative's, h^2, and 2^-22 / h of the
+    terms' absolute sum."""
+    say(f"rotary differences {interleaved}")
+    g = gen(31)
+    d, tokens = 24, 40
+    q, dq = (heads(g, (2,), 3, tokens, d, torch.float32) for _ in range(2))
+    k, dk = (heads(g, (2,), 1, tokens, d, torch.float32) for _ in range(2))
+    wq, wk = weights(g, d, torch.float32)
+    pos, fr, more = places(2, tokens), freqs(12), {"sections": (4, 8), "interleaved": interleaved}
+    grads = kernels.head_norm_rotary_backward(dq, dk, q, k, pos, fr, q_weight=wq, k_weight=wk, **more)
+    inputs = [q, k, wq, wk]
+
+    def value(args):
+        y = kernels.head_norm_rotary(args[0], args[1], pos, fr, q_weight=args[2], k_weight=args[3], **more)
+        return sum((a.double() * b.double()).sum() for a, b in zip(y, (dq, dk))), sum(
+            (a.double() * b.double()).abs().sum() for a, b in zip(y, (dq, dk)))
+
+    step = 1e-2
+    size = value(inputs)[1]
+    for i, t in enumerate(inputs):
+        way = torch.randn(t.shape, generator=g, device="cuda")
+        way /= way.norm()
+        ends = [value([x + sign * step * way if x is t else x for x in inputs])[0] for sign in (1, -1)]
+        slope = (ends[0] - ends[1]) / (2 * step)
+        want = (grads[i].double() * way.double()).sum()
+        assert abs(slope - want) <= 2.0**-22 / step * size + 10 * step**2 * grads[i].double().norm(), i

@@ -220,3 +220,29 @@ def test_equal_scores_of_any_size(size, dtype):
     assert ((got["out"].double() - want).abs() <= u * (2 * room + want.abs())).all()
     want, room = dout.double().mean(1, keepdim=True), dout.double().abs().mean(1, keepdim=True)
     assert ((got["dv"].double() - want).abs() <= u * (2 * room + want.abs())).all()
+
+
+def test_captured_with_other_lengths():
+    """A captured step whose tiles are sorted and whose key tiles have parts: a replay orders
+    and deals them by the lengths that are there; two such graphs at once keep their own."""
+    say("packed captured sorted")
+    tokens, more = 6200, {"scale": 0.18, "causal": True}
+    q, k, v, dout = inputs([tokens], 8, 2, 32, BF16, seed=32)
+    plans = [[3000, 2100, 1000], [40, 6000, 100], [6100, 0, 100], [2000, 2000, 2200]]
+    sides = []
+    for i in range(2):
+        st, graph = ints(starts(plans[i])), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = run(q, k, v, st, dout, **more)
+        sides.append((st, graph, held, torch.cuda.Stream()))
+    for turn in range(4):
+        for i, (st, graph, _, stream) in enumerate(sides):
+            st.copy_(ints(starts(plans[(turn + i) % 4])))
+        for _, graph, _, stream in sides:
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for st, _, held, _ in sides:
+            want = run(q, k, v, st, dout, **more)
+            assert all(torch.equal(held[n], want[n]) for n in want), turn
