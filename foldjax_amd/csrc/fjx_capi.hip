@@ -13,6 +13,7 @@
 #include "fjx_common.hpp"
 #include "fjx_diffattn.hpp"
 #include "fjx_kernels.hpp"
+#include "fjx_overlap.hpp"
 #include "fjx_packed.hpp"
 
 using namespace fjx;
@@ -1542,6 +1543,30 @@ int head_norm_check(const fjx_head_norm_rotary_args* a, const char* fn, bool wri
   return FJX_OK;
 }
 
+// Heads and tokens are dealt to workgroups, so that a row written where another's input
+// lies would be read by some before and by others after. `y` [2]: what a call writes, may be
+// null; `x` [count][2]: what it reads, null where it does not. Queries, keys.
+int head_norm_apart(const fjx_head_norm_rotary_args* a, const char* fn, const char* names, const void* const* y,
+                    const int64_t* const* y_strides, const void* const (*x)[2], const int64_t* const (*x_strides)[2], int count) {
+  const int64_t es = (int64_t)esize(a->dtype);
+  auto rows = [&](const void* p, const int64_t* s, int i) {
+    return RowSet{reinterpret_cast<uintptr_t>(p), {a->items, i ? a->kv_heads : a->heads, a->tokens},
+                  {s[0] * es, s[1] * es, s[2] * es}, a->head_dim * es};
+  };
+  auto refuse = [&] {
+    return fail(FJX_ERR_INVALID, "%s: %s must be two buffers, neither the other's input, each its own only in its place", fn, names);
+  };
+  if (a->kv_heads && rows_meet(rows(y[0], y_strides[0], 0), rows(y[1], y_strides[1], 1))) return refuse();
+  for (int i = 0; i < (a->kv_heads ? 2 : 1); ++i)
+    for (int c = 0; c < count; ++c)
+      for (int j = 0; j < (a->kv_heads ? 2 : 1); ++j) {
+        if (!x[c][j]) continue;
+        const RowSet out = rows(y[i], y_strides[i], i), in = rows(x[c][j], x_strides[c][j], j);
+        if (!(i == j && rows_equal(out, in)) && rows_meet(out, in)) return refuse();
+      }
+  return FJX_OK;
+}
+
 template <typename T>
 HeadNormParams<T> head_norm_params(const fjx_head_norm_rotary_args* a) {
   HeadNormParams<T> p = {};
@@ -2030,6 +2055,9 @@ int fjx_head_norm_rotary_fwd(const fjx_head_norm_rotary_args* a, hipStream_t st)
   g_err.clear();
   if (!a) return fail(FJX_ERR_INVALID, "%s: args is NULL", fn);
   if (int rc = head_norm_check(a, fn, true)) return rc;
+  const void *const y[2] = {a->q_out, a->k_out}, *const x[1][2] = {{a->q, a->k}};
+  const int64_t *const ys[2] = {a->q_out_strides, a->k_out_strides}, *const xs[1][2] = {{a->q_strides, a->k_strides}};
+  if (int rc = head_norm_apart(a, fn, "q_out and k_out", y, ys, x, xs, 1)) return rc;
   return a->dtype == FJX_DTYPE_BF16 ? head_norm_run<bf16>(a, st) : head_norm_run<float>(a, st);
 }
 
@@ -2055,6 +2083,12 @@ int fjx_head_norm_rotary_bwd(const fjx_head_norm_rotary_bwd_args* b, hipStream_t
   const size_t need = fjx_head_norm_rotary_bwd_workspace_size(a->items, a->heads, a->kv_heads, a->tokens, a->head_dim);
   if ((a->q_weight || a->k_weight) && (!b->workspace || b->workspace_bytes < need))
     return fail(FJX_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", fn, need, b->workspace_bytes);
+  // q and k are read for the norm alone
+  const void *const y[2] = {b->dq, b->dk};
+  const void *const x[2][2] = {{a->q_out, a->k_out}, {a->q_weight ? a->q : nullptr, a->k_weight ? a->k : nullptr}};
+  const int64_t *const ys[2] = {b->dq_strides, b->dk_strides};
+  const int64_t *const xs[2][2] = {{a->q_out_strides, a->k_out_strides}, {a->q_strides, a->k_strides}};
+  if (int rc = head_norm_apart(a, fn, "dq and dk", y, ys, x, xs, 2)) return rc;
   return a->dtype == FJX_DTYPE_BF16 ? head_norm_bwd_run<bf16>(b, st) : head_norm_bwd_run<float>(b, st);
 }
 

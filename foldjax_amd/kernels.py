@@ -1289,7 +1289,8 @@ def head_norm_rotary(
 
     Returns ``(q', k')``, a token's heads side by side in memory (k' None without k).
     ``q_out``, ``k_out``: write into these tensors (of q's and k's shape, their rows
-    whole 16-byte pieces: places in a cache, for one), each of which may be its input."""
+    whole 16-byte pieces: places in a cache, for one), each of which may be its input, in
+    its very place; they share no other memory with an input or each other (refused)."""
     a, kept, unit, like, _ = _rotary_args(q, k, positions, frequencies, q_weight, k_weight, eps, sections, interleaved)
     if q_out is None:
         q_out = _like_heads(q, like[0])
@@ -1304,10 +1305,6 @@ def head_norm_rotary(
             k_out = _like_heads(k, like[1])
         else:
             a.k_out_strides = _rotary_out("k_out", k_out, k, unit)
-            if k_out.data_ptr() == a.q_out or (k_out.data_ptr() == a.q and a.q != a.k):
-                raise ValueError("q_out and k_out must be two buffers, neither the other's input")
-        if a.q_out == a.k:
-            raise ValueError("q_out and k_out must be two buffers, neither the other's input")
         a.k_out = k_out.data_ptr()
     _launch(_lib.load().fjx_head_norm_rotary_fwd, a, q)
     return q_out, k_out

@@ -619,7 +619,8 @@ int fjx_packed_attention_bwd(const fjx_packed_attention_bwd_args* args, hipStrea
  * the next sections[1] axis 1, and so on (up to 4 axes, for instance residue, chain
  * and copy). q [items, heads, tokens, head_dim], k [items, kv_heads, tokens, head_dim]
  * (kv_heads 0: none); *_strides are {item, head, token} in elements, the last axis
- * contiguous. An output may be its input. Supported: head_dim a multiple of 8 up to
+ * contiguous. An output may be its input, in its very place; outputs share no other
+ * memory with an input or each other (refused). Supported: head_dim a multiple of 8 up to
  * 256, pairs a multiple of 4 (0: the norm alone).
  */
 typedef struct fjx_head_norm_rotary_args {
@@ -654,7 +655,7 @@ int fjx_head_norm_rotary_fwd(const fjx_head_norm_rotary_args* args, hipStream_t 
 /*
  * The gradients: `fwd` holds the forward call's arguments, with the outputs'
  * gradients in the place of q_out and k_out (they are only read). q and k are not
- * looked at where there is no weight. dq and dk may be the outputs' gradients. The
+ * looked at where there is no weight. dq and dk may be the outputs' gradients, as above. The
  * weights' gradients are fp32, summed over tokens and heads in one order.
  */
 typedef struct fjx_head_norm_rotary_bwd_args {
