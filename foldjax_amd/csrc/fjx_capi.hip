@@ -1434,6 +1434,18 @@ int packed_launch_ok(const char* fn, const PackedForm& f, int64_t kvh, int split
   return FJX_OK;
 }
 
+// `out` shares no memory with q, k or v
+bool packed_apart(const fjx_packed_attention_args* a) {
+  const int64_t es = (int64_t)esize(a->dtype);
+  auto rows = [&](const void* p, const int64_t* s, int64_t heads, int64_t tokens) {
+    return RowSet{reinterpret_cast<uintptr_t>(p), {1, heads, tokens}, {0, s[0] * es, s[1] * es}, a->head_dim * es};
+  };
+  const RowSet out = rows(a->out, a->out_strides, a->heads, a->tokens_q);
+  return !rows_meet(out, rows(a->q, a->q_strides, a->heads, a->tokens_q)) &&
+         !rows_meet(out, rows(a->k, a->k_strides, a->kv_heads, a->tokens_k)) &&
+         !rows_meet(out, rows(a->v, a->v_strides, a->kv_heads, a->tokens_k));
+}
+
 template <typename T>
 PackedParams<T> packed_params(const fjx_packed_attention_args* a) {
   PackedParams<T> p = {};
@@ -2012,6 +2024,7 @@ int fjx_packed_attention_fwd(const fjx_packed_attention_args* a, hipStream_t st)
   if (need && (!a->workspace || a->workspace_bytes < need))
     return fail(FJX_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", fn, need, a->workspace_bytes);
   if (need && !aligned16({a->workspace})) return fail(FJX_ERR_INVALID, "%s: the workspace must be 16-byte aligned", fn);
+  if (!packed_apart(a)) return fail(FJX_ERR_INVALID, "%s: out must not overlap q, k or v: other rows' results are taken from them", fn);
   return a->dtype == FJX_DTYPE_BF16 ? packed_fwd_run<bf16>(a, plan, st) : packed_fwd_run<float>(a, plan, st);
 }
 

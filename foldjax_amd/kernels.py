@@ -1059,8 +1059,8 @@ def packed_attention(
     behind the last sequence are zeros. With ``return_lse`` ``(out, lse, rest)``,
     the latter two for ``packed_attention_backward``: what it needs to know of the
     rows, and what the rounding of a bfloat16 output left (None of float32).
-    ``out``: write into this tensor (its rows whole 16-byte pieces), which overlaps
-    no input; its rows behind the last sequence are left as they are."""
+    ``out``: write into this tensor (its rows whole 16-byte pieces), which shares
+    no memory with an input (refused); its rows behind the last sequence are left as they are."""
     a, kept, unit, (_, nbytes) = _packed_attention_args(q, k, v, q_starts, scale, causal, k_starts, k_lengths)
     if out is None:
         out = _token_major(a.heads, a.tokens_q, a.head_dim, q)
@@ -1069,8 +1069,6 @@ def packed_attention(
         if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
             raise ValueError(f"out must be a {q.dtype} tensor of shape {tuple(q.shape)} on {q.device}, "
                              f"got {out.dtype} {tuple(out.shape)} on {out.device}")
-        if a.tokens_q and out.data_ptr() in (q.data_ptr(), k.data_ptr(), v.data_ptr()):
-            raise ValueError("out must not be q, k or v: other rows' results are taken from them")
         strides = _packed_rows(out, unit)
         if strides is None:
             raise ValueError("out must have rows of whole 16-byte pieces that do not overlap")

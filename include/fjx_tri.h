@@ -544,7 +544,7 @@ enum { FJX_INDEX_I32 = 0, FJX_INDEX_I64 = 1 };
  * and nk keys, query i sees key j where j <= i + nk - nq (the last query sees all);
  * rows without a key are zeros, with zero gradients. k and v of a sequence's keys
  * (backward: dout too) are finite. Rows of out behind the last sequence are left as they are, or with
- * zero_tail written as zeros. `out` overlaps no input.
+ * zero_tail written as zeros. `out` shares no memory with q, k or v (refused).
  * For the backward pass: lse [heads, tokens_q, 2] fp32, and `rest` (as out, of
  * bf16), what the output's rounding left.
  * Supported: head_dim a multiple of 8 up to 128, tokens_q * heads and tokens_k below

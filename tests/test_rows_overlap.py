@@ -137,3 +137,26 @@ def test_gradients_over_inputs_are_refused(dq, dk, more):
     b = _lib.HeadNormRotaryBwdArgs(rotary(**more), dq, dk, (1024, 32, 128), (1024, 32, 128), 0x40000, 0x41000, 0x50000, size)
     assert lib.fjx_head_norm_rotary_bwd(ctypes.byref(b), None) == 1
     assert "two buffers" in lib.fjx_last_error().decode()
+
+
+def packed(**more):
+    """40 tokens in 2 sequences, 4 query heads on 2, 32 channels in bf16, token by token."""
+    a = _lib.PackedAttentionArgs(tokens_q=40, tokens_k=40, sequences=2, heads=4, kv_heads=2, head_dim=32, dtype=1, scale=1.0,
+                                 q=0x10000, k=0x14000, v=0x18000, out=0x1C000, q_starts=0x20000, k_starts=0x20000)
+    for name in ("q_strides", "k_strides", "v_strides", "out_strides", "rest_strides"):
+        setattr(a, name, (32, 128))
+    for n, v in more.items():
+        setattr(a, n, v)
+    return a
+
+
+@pytest.mark.parametrize("more", [
+    {"out": 0x10000}, {"out": 0x10000 + 256}, {"out": 0x10000 - 39 * 256},  # the queries, a token on, their first token
+    {"out": 0x10000, "out_strides": (40 * 32, 32)},                        # turned
+    {"out": 0x14000 - 2 * 64}, {"out": 0x18000 + 39 * 256},                # a head of keys, the last token's values
+    {"k": 0x10000 + 4 * 64, "k_strides": (32, 256), "q_strides": (32, 256), "out": 0x10000 + 3 * 64, "out_strides": (32, 256)},
+], ids=str)
+def test_attention_over_its_inputs_is_refused(more):
+    lib = _lib.load()
+    assert lib.fjx_packed_attention_fwd(ctypes.byref(packed(**more)), None) == 1
+    assert "out must not overlap" in lib.fjx_last_error().decode()
