@@ -1285,10 +1285,11 @@ def head_norm_rotary(
     axis a's for the ``sections[a]`` pairs behind those of the axes before it
     (residue, chain and copy of a token, for instance; up to 4 axes; left out: one).
 
-    Returns ``(q', k')``, a token's heads side by side in memory (k' None without k).
-    ``q_out``, ``k_out``: write into these tensors (of q's and k's shape, their rows
-    whole 16-byte pieces: places in a cache, for one), each of which may be its input, in
-    its very place; they share no other memory with an input or each other (refused)."""
+    Returns ``(q', k')``, a token's heads side by side in memory (k' None without k);
+    no tokens or no items are allowed. ``q_out``, ``k_out``: write into these tensors
+    (of q's and k's shape, their rows whole 16-byte pieces: places in a cache, for
+    one), each of which may be its input, in its very place; they share no other
+    memory with an input or each other (refused)."""
     a, kept, unit, like, _ = _rotary_args(q, k, positions, frequencies, q_weight, k_weight, eps, sections, interleaved)
     if q_out is None:
         q_out = _like_heads(q, like[0])
@@ -1304,7 +1305,8 @@ def head_norm_rotary(
         else:
             a.k_out_strides = _rotary_out("k_out", k_out, k, unit)
         a.k_out = k_out.data_ptr()
-    _launch(_lib.load().fjx_head_norm_rotary_fwd, a, q)
+    if a.items and a.tokens:
+        _launch(_lib.load().fjx_head_norm_rotary_fwd, a, q)
     return q_out, k_out
 
 
@@ -1383,6 +1385,9 @@ def head_norm_rotary_backward(
             _remember(key, (bytes(b), nbytes, like))
     dev, d = q.device, q.shape[-1]
     gq, gk, dwq, dwk = _like_heads(q, like[0]), None, None, None
+    if not (b.fwd.items and b.fwd.tokens):  # no rows: sums of nothing
+        return gq, None if k is None else _like_heads(k, like[1]), *(
+            None if w is None else torch.zeros(d, dtype=torch.float32, device=dev) for w in (q_weight, k_weight))
     b.dq = gq.data_ptr()
     if k is not None:
         gk = _like_heads(k, like[1])
