@@ -1287,103 +1287,6 @@ int diff_bwd_run(const fjx_diff_attention_bwd_args* b, const DiffBwdPlan& plan, 
 }
 
 // ------------------------------------------------------ packed attention
-// How a call is cut. The host knows how many sequences and tokens there are, not how
-// long each is: the rules take all lengths as alike.
-struct PackedPlan {
-  PackedForm rows, keys;
-  int splits;                // of the keys (forward, keywise), of the heads that share keys (dk, dv)
-  size_t part_o, part_ml;    // workspace bytes: forward; backward: one of dk, dv and D
-  int part_rows;
-  size_t rows_order, keys_order;
-};
-int packed_width(int64_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
-// `wgs`: workgroups of 64 rows (keys) there are, `walk`: keys (rows) that one walks;
-// `few`: so few wgs are one wave's rows with its own keys each; `pairs`: from so many on a
-// wave has two tiles. us by form, KS 4 / KS 2 / KS 1 with one tile / KS 2 / KS 1 with two:
-//   forward  126 workgroups 1003 keys d 64         8.7 / 10.9 / 14.6 / 15.6 / 20.5
-//            216            851       128         21.0 / 15.4 / 19.4 / 22.2 / 27.6
-//            258            686        64         17.5 / 13.4 / 16.4 / 16.0 / 20.8
-//            496            245        24         14.1 /  9.4 /  8.9 / 10.3 / 10.2
-//            520            4099      128          107 / 56.6 / 64.9 / 64.1 / 87.9
-//           1024            1638      128          160 / 83.4 / 75.9 / 70.8 / 96.1
-//           2048            2730      128          586 /  296 /  264 /  230 /  219
-//           4096            8192       64          641 /  370 /  349 /  301 /  295
-//   dk, dv (the backward pass with them, dq's form the same)
-//           1016            4049       64          251 /  202 /  238 /  216 /  231
-//           1024            4096       64         1101 /  849 / 1035 /  889 / 1182
-//           4096            8192       64         1580 / 1177 / 1135 / 1122 / 1090
-//   float32  132            701        64           36 /   39 /   42
-//            256            2048      128          107 /  144 /  148
-//            456            1774      128          163 /  147 /  149
-// (rows of several long sequences sorted).
-PackedForm packed_form(int64_t rows, int64_t seqs, int64_t wgs, int64_t walk, int64_t few, int64_t pairs) {
-  PackedForm f = {};
-  f.groups = 4;
-  f.tiles = 1;
-  if (walk > 64 && (rows <= 16 * seqs || wgs < few))
-    f.groups = 1, f.ks = 4;
-  else if (walk < 320 || wgs < 128)
-    f.ks = 1;
-  else if (wgs < pairs)
-    f.ks = 2;
-  else
-    f.ks = wgs < 2048 ? 2 : 1, f.tiles = 2;
-  f.count = (int)std::min<int64_t>(rows / f.rows() + seqs + 1, 1 << 30);
-  return f;
-}
-// Sorting the tiles by their work takes a launch, 4 us: for calls of several sequences
-// that walk 16384 blocks of 64 and more in all (the forward pass of 5 causal sequences,
-// 8192 tokens, 85 -> 77 us with it, of 6 with 16384 254 -> 234)
-bool packed_sorted(const PackedForm& f, int64_t seqs, int64_t wgs, int64_t walk) {
-  return f.groups > 1 && f.count && f.count <= kPackedOrder && seqs > 1 && seqs <= kPackedOrderSeqs && wgs * walk >= (int64_t)16384 * 64;
-}
-int64_t packed_few(bool bf, int64_t d) { return bf ? 128 : d <= 64 ? 256 : 384; }
-PackedPlan packed_fwd_plan(int64_t tq, int64_t tk, int64_t seqs, int64_t heads, int64_t kvh, int64_t d, int32_t dtype) {
-  const int64_t group = heads / kvh, rows = tq * group, wgs = kvh * ((rows + 63) / 64), walk = tk / seqs;
-  const bool bf = dtype == FJX_DTYPE_BF16;
-  PackedPlan p = {};
-  p.rows = packed_form(rows, seqs, wgs, walk, packed_few(bf, d), bf ? 1024 : INT64_MAX);
-  p.splits = 1;
-  if (p.rows.groups == 1) {
-    const int64_t tiles = kvh * std::max(seqs, rows / 16);
-    // two blocks of 128 keys a split at least, were the lengths alike
-    const int64_t want = tiles <= 128 ? std::min<int64_t>(512 / tiles, walk / 256) : 1;
-    if (want > 1) {
-      p.splits = (int)want;
-      const size_t r = (size_t)heads * tq * p.splits;
-      p.part_o = align_up(r * packed_width(d) * sizeof(float));
-      p.part_ml = align_up(r * 2 * sizeof(float));
-    }
-  }
-  if (packed_sorted(p.rows, seqs, wgs, walk)) p.rows_order = align_up((size_t)p.rows.count * sizeof(PackedTile));
-  return p;
-}
-PackedPlan packed_bwd_plan(int64_t tq, int64_t tk, int64_t seqs, int64_t heads, int64_t kvh, int64_t d, int32_t dtype) {
-  const int64_t group = heads / kvh, rows = tq * group, wgs = kvh * ((rows + 63) / 64), walk = tk / seqs;
-  const int64_t key_wgs = kvh * ((tk + 63) / 64);
-  const bool bf = dtype == FJX_DTYPE_BF16;
-  PackedPlan p = {};
-  p.splits = 1;
-  // Workgroups that walk long and, causal, uneven ways: the heads that share keys in parts, of
-  // an eighth of a workgroup's share of the card (of 128 channels one a CU, else two) were the
-  // lengths alike. us of the backward pass with every tile in 4 parts / with parts of a half /
-  // an eighth / a 16th, causal: 8192 tokens in 5 sequences, d 128 (2 parts: 283)  291 / 316 /
-  // 270 / 270; one sequence of 8192, d 64  353 / 384 / 330 / 332; 4099 and 4000, d 64
-  // 199 / 210 / 188 / 187; one of 1003, d 64  30.4 / 32 / 31.0 / 31
-  if (group > 1 && tk && key_wgs < 1024) {
-    p.splits = (int)std::min(group, std::max<int64_t>(2, (1024 + key_wgs - 1) / key_wgs));
-    p.part_rows = (int)std::max<int64_t>(256, tq * group / seqs * key_wgs / (d > 64 ? 256 : 512) / 8);
-  }
-  if (tq) p.rows = packed_form(rows, seqs, wgs, walk, packed_few(bf, d), bf ? 1024 : INT64_MAX);
-  // two tiles of keys a wave would take more registers than two waves a SIMD have at 128 channels
-  if (tk) p.keys = packed_form(tk, seqs, key_wgs * p.splits, tq / seqs, packed_few(bf, d), bf && d <= 64 ? 2048 : INT64_MAX);
-  if (p.splits > 1) p.part_o = align_up((size_t)p.splits * kvh * tk * packed_width(d) * sizeof(float));
-  p.part_ml = align_up((size_t)heads * tq * sizeof(float));
-  if (packed_sorted(p.rows, seqs, wgs, walk)) p.rows_order = align_up((size_t)p.rows.count * sizeof(PackedTile));
-  if (packed_sorted(p.keys, seqs, key_wgs * group, tq / seqs)) p.keys_order = align_up((size_t)p.keys.count * sizeof(PackedTile));
-  return p;
-}
-
 // {head, token} strides that the kernels' 16-byte accesses of rows take
 bool packed_strides_ok(const int64_t* s, int64_t heads, int64_t tokens, int64_t d, size_t es) {
   if (heads > 1 && (s[0] < 1 || s[0] * (int64_t)es % 16)) return false;
@@ -2008,7 +1911,7 @@ size_t fjx_packed_attention_workspace_size(int64_t tokens_q, int64_t tokens_k, i
   if (tokens_q < 1 || tokens_k < 0 || sequences < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || head_dim < 1 ||
       !dtype_ok(dtype))
     return 0;
-  const PackedPlan p = packed_fwd_plan(tokens_q, tokens_k, sequences, heads, kv_heads, head_dim, dtype);
+  const PackedPlan p = packed_fwd_plan(tokens_q, tokens_k, sequences, heads, kv_heads, head_dim, dtype == FJX_DTYPE_BF16);
   return p.part_o + p.part_ml + p.rows_order;
 }
 
@@ -2018,7 +1921,7 @@ int fjx_packed_attention_fwd(const fjx_packed_attention_args* a, hipStream_t st)
   if (!a) return fail(FJX_ERR_INVALID, "%s: args is NULL", fn);
   if (int rc = packed_check(a, fn)) return rc;
   if (!a->tokens_q) return FJX_OK;
-  const PackedPlan plan = packed_fwd_plan(a->tokens_q, a->tokens_k, a->sequences, a->heads, a->kv_heads, a->head_dim, a->dtype);
+  const PackedPlan plan = packed_fwd_plan(a->tokens_q, a->tokens_k, a->sequences, a->heads, a->kv_heads, a->head_dim, a->dtype == FJX_DTYPE_BF16);
   if (int rc = packed_launch_ok(fn, plan.rows, a->kv_heads, plan.splits)) return rc;
   const size_t need = plan.part_o + plan.part_ml + plan.rows_order;
   if (need && (!a->workspace || a->workspace_bytes < need))
@@ -2033,7 +1936,7 @@ size_t fjx_packed_attention_bwd_workspace_size(int64_t tokens_q, int64_t tokens_
   if (tokens_q < 0 || tokens_k < 0 || sequences < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || head_dim < 1 ||
       !dtype_ok(dtype))
     return 0;
-  const PackedPlan p = packed_bwd_plan(tokens_q, tokens_k, sequences, heads, kv_heads, head_dim, dtype);
+  const PackedPlan p = packed_bwd_plan(tokens_q, tokens_k, sequences, heads, kv_heads, head_dim, dtype == FJX_DTYPE_BF16);
   return 2 * p.part_o + p.part_ml + p.rows_order + p.keys_order;
 }
 
@@ -2053,7 +1956,7 @@ int fjx_packed_attention_bwd(const fjx_packed_attention_bwd_args* b, hipStream_t
       !packed_strides_ok(b->dv_strides, a->kv_heads, a->tokens_k, a->head_dim, es))
     return fail(FJX_ERR_INVALID, "%s: the gradients' strides must be positive multiples of 16 bytes, a token's at least head_dim and below 2^24 bytes", fn);
   if (!a->tokens_q && !a->tokens_k) return FJX_OK;
-  const PackedPlan plan = packed_bwd_plan(a->tokens_q, a->tokens_k, a->sequences, a->heads, a->kv_heads, a->head_dim, a->dtype);
+  const PackedPlan plan = packed_bwd_plan(a->tokens_q, a->tokens_k, a->sequences, a->heads, a->kv_heads, a->head_dim, a->dtype == FJX_DTYPE_BF16);
   if (int rc = packed_launch_ok(fn, plan.rows, a->kv_heads, 1)) return rc;
   if (int rc = packed_launch_ok(fn, plan.keys, a->kv_heads, plan.splits)) return rc;
   const size_t need = 2 * plan.part_o + plan.part_ml + plan.rows_order + plan.keys_order;

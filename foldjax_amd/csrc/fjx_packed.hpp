@@ -20,6 +20,7 @@
 
 #include "fjx_common.hpp"
 #include "fjx_kernels.hpp"
+#include "fjx_packed_plan.hpp"
 
 namespace fjx {
 
@@ -36,21 +37,6 @@ struct PackedInts {
   int wide;
 };
 
-constexpr int kPackedOrder = 12288, kPackedOrderSeqs = 1023;  // tiles that are sorted at most, and their sequences
-
-// a tile of a sequence: first query, queries, first key, keys, and keys with the unused
-// ones behind them. Sequence `seqs`: the rows behind the last one
-struct alignas(16) PackedTile {
-  int seq, tile, q0, nq, k0, nk, cap, pad;
-};
-
-// how a call is cut (PkForm), 16-row tiles of a wave
-struct PackedForm {
-  int groups, ks, tiles;
-  int count;          // tiles for one key/value head
-  PackedTile* order;  // [count], to be filled with the tiles in the order of their work, or null
-  __host__ __device__ int rows() const { return 16 * groups * tiles; }  // of a workgroup
-};
 template <typename T>
 struct PackedParams {
   PackedView<const T> q, k, v;  // [H][tq][d], [Hk][tk][d], [Hk][tk][d]
