@@ -1387,6 +1387,7 @@ int packed_fwd_run(const fjx_packed_attention_args* a, const PackedPlan& plan, h
   p.splits = plan.splits;
   p.part_o = at<float>(a->workspace, 0);
   p.part_ml = at<float>(a->workspace, plan.part_o);
+  p.part_l = p.part_ml + 2 * (size_t)a->heads * a->tokens_q * plan.splits;
   PackedForm form = plan.rows;
   p.order = form.order = plan.rows_order ? at<PackedTile>(a->workspace, plan.part_o + plan.part_ml) : nullptr;
   return timed(K_PACKED_ATTENTION_FWD, st, "packed_attention_fwd", [&] { launch_packed_fwd<T>(p, form, st); });

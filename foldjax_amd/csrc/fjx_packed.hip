@@ -11,8 +11,8 @@ namespace {
 // g = l / 16), so a row's maximum and sum are the lane's own values and two lane swaps,
 // and the weights of two key tiles are the operand of O^T = V^T P^T as they lie.
 //
-// A bf16 weight is rounded once (half a step, 2^-9 of itself), and the row's sum is
-// that of the rounded weights, taken by the matrix cores as a row of ones times them:
+// A bf16 weight is rounded once (half a step, 2^-8 of itself at most), and the outputs'
+// sum is that of the rounded weights, taken by the matrix cores as a row of ones times them:
 // the weights that are applied add up to one, and an output is off by less than its own
 // rounding. A weight may exceed 1 by up to 2^kSlack before the maximum is moved, which
 // saves the outputs' rescaling in all but the first blocks of a row.
@@ -33,7 +33,11 @@ constexpr float kSlack = 8.f;
 // M exactly.
 constexpr float kFar = 16777216.f;
 
-template <typename T, int DP, int G, int KS, int R>
+// SUMS: also the sum of the weights before their rounding, for the statistics. The rounded
+// ones' is off by up to half a step of bf16 where a few keys have the weight (0.3 % measured),
+// and the gradients' weights, which come anew, would all be off by that: a vector
+// instruction a score more, where statistics are asked for.
+template <typename T, int DP, int G, int KS, int R, bool SUMS>
 __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkFormOf<T, DP, G, KS>::type::template kSimd<T, DP>)) void packed_fwd_kernel(PackedParams<T> P) {
   typedef typename PkFormOf<T, DP, G, KS>::type Form;
   typedef PkRows<T, DP> Rows;
@@ -48,6 +52,7 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkFormOf<T, DP, G, KS>:
   constexpr int kRaw = kStages * 2 * kOperand * kSets;  // and at the end the outputs' way
   __shared__ __attribute__((aligned(16))) unsigned char raw[kRaw > Out::kBytes ? kRaw : Out::kBytes];
   __shared__ f32x2 wave_ml[R][KS][16 * G];  // maxima and sums
+  __shared__ float wave_l[SUMS ? R : 1][KS][16 * G];  // sums of unrounded weights
   __shared__ int2 places[R][16 * G];        // the rows' heads and tokens; head -1: no such row
 
   const int t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
@@ -110,11 +115,12 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkFormOf<T, DP, G, KS>:
   F ones;
 #pragma unroll
   for (int e = 0; e < 8; ++e) ones[e] = from_f32<T>(1.f);
-  float m[R];
+  float m[R], unrounded[R];
   f32x4 l[R], o[R][kU];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     m[r] = -INFINITY;
+    unrounded[r] = 0.f;
     l[r] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int u = 0; u < kU; ++u) o[r][u] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -177,6 +183,7 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkFormOf<T, DP, G, KS>:
           const float alpha = __builtin_amdgcn_exp2f(m[r] - pk_base(mn));  // 0 where no key was before
           m[r] = mn;
           any = any || fabsf(pk_base(mn)) > kFar;
+          if (SUMS) unrounded[r] *= alpha;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             l[r][e] *= alpha;
@@ -204,6 +211,7 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkFormOf<T, DP, G, KS>:
             p[e] = __builtin_amdgcn_exp2f(fmaf(s[r][2 * c + (e >> 2)][e & 3], by, -base));
             if (!kOnes) l[r][e & 3] += p[e];
           }
+          if (SUMS) unrounded[r] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
           pf[r][c] = pack8<T>(p);
           if (kOnes) mma(l[r], ones, pf[r][c]);
         }
@@ -217,18 +225,23 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkFormOf<T, DP, G, KS>:
     pk_sync<Form>();
   }
 #pragma unroll
-  for (int r = 0; r < R; ++r)
+  for (int r = 0; r < R; ++r) {
+    if (SUMS) {
+      const float sum = group_sum(unrounded[r]);
+      if (lg == 0) wave_l[r][form.part][16 * form.group + li] = sum;
+    }
     if (lg == 0 || !kOnes) {
       const float sum = kOnes ? l[r][0] : group_sum((l[r][0] + l[r][1]) + (l[r][2] + l[r][3]));
       if (lg == 0) wave_ml[r][form.part][16 * form.group + li] = f32x2{m[r], sum};
     }
+  }
   // rows come together on the largest of their waves' maxima
 #pragma unroll
   for (int r = 0; r < R; ++r)
     Out::write(raw, form, t, o[r], [&](int row, int c, const float* x) {
       const int2 to = places[r][row];
       if (to.x < 0) return;
-      float mx = -INFINITY, sum = 0.f;
+      float mx = -INFINITY, sum = 0.f, all = 0.f;
 #pragma unroll
       for (int j = 0; j < KS; ++j) mx = fmaxf(mx, wave_ml[r][j][row][0]);
       f32x8 v = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -238,6 +251,7 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkFormOf<T, DP, G, KS>:
         const float w = __builtin_amdgcn_exp2f(ml[0] - pk_base(mx));
         const f32x8 y = load8(x + j * Out::kPart);
         sum = fmaf(ml[1], w, sum);
+        if (SUMS) all = fmaf(wave_l[r][j][row], w, all);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = fmaf(y[e], w, v[e]);
       }
@@ -245,10 +259,11 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkFormOf<T, DP, G, KS>:
       if (P.splits > 1) {
         const int64_t part = (int64_t)split * P.heads * P.tq + at_row;
         if (c == 0) *reinterpret_cast<f32x2*>(P.part_ml + part * 2) = f32x2{mx, sum};
+        if (SUMS && c == 0) P.part_l[part] = all;
         store8(P.part_o + part * DP + c, v);
         return;
       }
-      if (c == 0 && P.lse) *reinterpret_cast<f32x2*>(P.lse + at_row * 2) = pk_stats(mx, sum);
+      if (c == 0 && P.lse) *reinterpret_cast<f32x2*>(P.lse + at_row * 2) = pk_stats(mx, SUMS ? all : sum);
       if (c >= P.d) return;
       const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row without keys is zeros
       float y[8];
@@ -264,11 +279,12 @@ __global__ __launch_bounds__((PkForm<G, KS>::kThreads), (PkFormOf<T, DP, G, KS>:
 
 // The splits of a row joined: a workgroup a row, wave w taking every fourth split
 // from w on, lane l holding DP / 64 values (of DP = 32 half the lanes one).
-template <typename T, int DP>
+template <typename T, int DP, bool SUMS>
 __global__ __launch_bounds__(256) void packed_join_kernel(PackedParams<T> P) {
   constexpr int kV = DP > 64 ? DP / 64 : 1;
   __shared__ float lds_o[4][DP];
   __shared__ float lds_l[4];
+  __shared__ float lds_all[SUMS ? 4 : 1];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t rows = P.heads * P.tq, at = blockIdx.x;
@@ -281,25 +297,28 @@ __global__ __launch_bounds__(256) void packed_join_kernel(PackedParams<T> P) {
 #pragma unroll
   for (int x = 32; x >= 1; x >>= 1) mx = fmaxf(mx, shfl_xor(mx, x));
   const float base = pk_base(mx);
-  float l = 0.f, o[kV] = {};
+  float l = 0.f, all = 0.f, o[kV] = {};
 #pragma unroll 8
   for (int s = wave; s < P.splits; s += 4) {
     const int64_t i = s * rows + at;
     const f32x2 v = *reinterpret_cast<const f32x2*>(P.part_ml + i * 2);
     const float w = __builtin_amdgcn_exp2f(v[0] - base);
     l = fmaf(v[1], w, l);
+    if (SUMS) all = fmaf(P.part_l[i], w, all);
 #pragma unroll
     for (int j = 0; j < kV; ++j)
       if (64 * j + lane < DP) o[j] = fmaf(P.part_o[i * DP + 64 * j + lane], w, o[j]);
   }
   if (lane == 0) lds_l[wave] = l;
+  if (SUMS && lane == 0) lds_all[wave] = all;
 #pragma unroll
   for (int j = 0; j < kV; ++j)
     if (64 * j + lane < DP) lds_o[wave][64 * j + lane] = o[j];
   __syncthreads();
   if (wave) return;
   const float sum = (lds_l[0] + lds_l[1]) + (lds_l[2] + lds_l[3]);
-  if (lane == 0 && P.lse) *reinterpret_cast<f32x2*>(P.lse + at * 2) = pk_stats(mx, sum);
+  if (lane == 0 && P.lse)
+    *reinterpret_cast<f32x2*>(P.lse + at * 2) = pk_stats(mx, SUMS ? (lds_all[0] + lds_all[1]) + (lds_all[2] + lds_all[3]) : sum);
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   T* out = P.out.p + head * P.out.head + token * P.out.token;
   T* rest = P.rest.p + head * P.rest.head + token * P.rest.token;
@@ -409,15 +428,21 @@ __global__ __launch_bounds__(1024) void packed_order_kernel(PackedParams<T> P, P
   for (int i = most + t; i < count; i += 1024) order[i].seq = -1;
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool SUMS>
 void fwd(const PackedParams<T>& P, const PackedForm& form, hipStream_t st) {
   pk_form<T>(form, [&](auto g, auto ks, auto r) {
     constexpr int G = decltype(g)::value, KS = decltype(ks)::value, R = decltype(r)::value;
     pk_grid(P, [&](const PackedParams<T>& Q, dim3 grid) {
-      packed_fwd_kernel<T, DP, G, KS, R><<<grid, PkForm<G, KS>::kThreads, 0, st>>>(Q);
+      packed_fwd_kernel<T, DP, G, KS, R, SUMS><<<grid, PkForm<G, KS>::kThreads, 0, st>>>(Q);
     });
   });
-  if (P.splits > 1) packed_join_kernel<T, DP><<<(unsigned)(P.heads * P.tq), 256, 0, st>>>(P);
+  if (P.splits > 1) packed_join_kernel<T, DP, SUMS><<<(unsigned)(P.heads * P.tq), 256, 0, st>>>(P);
+}
+template <typename T, int DP>
+void fwd(const PackedParams<T>& P, const PackedForm& form, hipStream_t st) {
+  if constexpr (sizeof(T) == 2)
+    if (P.lse) return fwd<T, DP, true>(P, form, st);
+  fwd<T, DP, false>(P, form, st);
 }
 
 }  // namespace

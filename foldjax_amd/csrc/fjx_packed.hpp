@@ -42,7 +42,7 @@ struct PackedParams {
   PackedView<const T> q, k, v;  // [H][tq][d], [Hk][tk][d], [Hk][tk][d]
   PackedView<T> out;            // [H][tq][d]
   PackedView<T> rest;           // what out's rounding left, or null
-  float* lse;                   // [H][tq][2]: the row's maximum and log2 of its sum (log2 units), or null
+  float* lse;                   // [H][tq][2]: the row's maximum and log2 of its sum, unrounded (log2 units), or null
   PackedInts q_starts, k_starts, k_lengths;  // [seqs + 1], [seqs + 1], [seqs] or null
   int64_t tq, tk;
   int seqs, heads, group, d;
@@ -57,6 +57,7 @@ struct PackedParams {
   int splits;
   float* part_o;                // [splits][H][tq][DP]
   float* part_ml;               // [splits][H][tq][2]
+  float* part_l;                // [splits][H][tq]: sums of unrounded bf16 weights, where lse is asked for
   // backward
   PackedView<const T> dout, o, o_rest;
   PackedView<T> dq, dk, dv;

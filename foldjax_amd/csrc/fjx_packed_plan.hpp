@@ -91,7 +91,7 @@ inline PackedPlan packed_fwd_plan(int64_t tq, int64_t tk, int64_t seqs, int64_t 
       p.splits = (int)want;
       const size_t r = (size_t)heads * tq * p.splits;
       p.part_o = packed_bytes(r * packed_width(d) * sizeof(float));
-      p.part_ml = packed_bytes(r * 2 * sizeof(float));
+      p.part_ml = packed_bytes(r * 3 * sizeof(float));  // maxima and sums, and the statistics' sums
     }
   }
   if (packed_sorted(p.rows, seqs, wgs, walk)) p.rows_order = packed_bytes((size_t)p.rows.count * sizeof(PackedTile));

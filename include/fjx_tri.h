@@ -549,7 +549,8 @@ enum { FJX_INDEX_I32 = 0, FJX_INDEX_I64 = 1 };
  * bf16), what the output's rounding left.
  * Supported: head_dim a multiple of 8 up to 128, tokens_q * heads and tokens_k below
  * 2^31 - 128 (sequences + 2), sequences below 2^22. Scores, statistics and sums are
- * fp32; bf16 weights enter the product with v rounded once, and their sum with them.
+ * fp32; bf16 weights enter the product with v rounded once, and the outputs' sum with them
+ * (the sum in lse is that of the weights as they were).
  */
 typedef struct fjx_packed_attention_args {
   int64_t tokens_q;
