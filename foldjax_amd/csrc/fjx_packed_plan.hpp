@@ -39,7 +39,8 @@ inline size_t packed_bytes(size_t n) { return (n + 255) / 256 * 256; }  // a wor
 inline int packed_width(int64_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
 // `wgs`: workgroups of 64 rows (keys) there are, `walk`: keys (rows) that one walks;
 // `few`: so few wgs are one wave's rows with its own keys each; `pairs`: from so many on a
-// wave has two tiles. us by form, KS 4 / KS 2 / KS 1 with one tile / KS 2 / KS 1 with two:
+// wave has two tiles; `alone`: from so many on also all keys of a block. us by form, KS 4 /
+// KS 2 / KS 1 with one tile / KS 2 / KS 1 with two:
 //   forward  126 workgroups 1003 keys d 64         8.7 / 10.9 / 14.6 / 15.6 / 20.5
 //            216            851       128         21.0 / 15.4 / 19.4 / 22.2 / 27.6
 //            258            686        64         17.5 / 13.4 / 16.4 / 16.0 / 20.8
@@ -55,8 +56,28 @@ inline int packed_width(int64_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
 //   float32  132            701        64           36 /   39 /   42
 //            256            2048      128          107 /  144 /  148
 //            456            1774      128          163 /  147 /  149
-// (rows of several long sequences sorted).
-inline PackedForm packed_form(int64_t rows, int64_t seqs, int64_t wgs, int64_t walk, int64_t few, int64_t pairs) {
+// (rows of several long sequences sorted). Where `pairs` and `alone` lie, KS 2 with one / KS 2 /
+// KS 1 with two tiles, four sequences, causal and all keys (d 128: 8 heads, d 64: 16 on 4):
+//   forward  640  d 128    43 /  45 /  59   68 /  60 /  66
+//            768           57 /  55 /  74   90 /  81 /  77
+//           1024           86 /  70 /  95  145 / 135 / 126
+//           1536          167 / 130 / 144  287 / 226 / 211
+//           2048          269 / 209 / 198  503 / 386 / 402
+//            768  d 64     21 /  21 /  28   31 /  29 /  34
+//           1024           30 /  33 /  41   48 /  46 /  52
+//           1280           40 /  40 /  50   64 /  60 /  65
+//           2048           79 /  67 /  78  138 / 127 / 132
+//           3200          167 / 138 / 138  321 / 260 / 256
+//           4096          262 / 218 / 210  494 / 404 / 413
+//   dq (the backward pass with it)
+//            768  d 128   167 / 169 / 194  272 / 265 / 259
+//           2048          841 / 785 / 766  1590 / 1492 / 1501
+//           1280  d 64    128 / 131 / 137  202 / 202 / 206
+//           2048          247 / 253 / 249  448 / 459 / 454
+//           3200          530 / 537 / 510  979 / 974 / 943
+// Up to d 64 two tiles begin to pay at 1280 to 2048 where it is causal and at 640 to 768 with all
+// keys, which a workspace's size does not know: 1024 lies between (all keys, d 24, 1264: 54 / 48).
+inline PackedForm packed_form(int64_t rows, int64_t seqs, int64_t wgs, int64_t walk, int64_t few, int64_t pairs, int64_t alone) {
   PackedForm f = {};
   f.groups = 4;
   f.tiles = 1;
@@ -67,7 +88,7 @@ inline PackedForm packed_form(int64_t rows, int64_t seqs, int64_t wgs, int64_t w
   else if (wgs < pairs)
     f.ks = 2;
   else
-    f.ks = wgs < 2048 ? 2 : 1, f.tiles = 2;
+    f.ks = wgs < alone ? 2 : 1, f.tiles = 2;
   f.count = (int)std::min<int64_t>(rows / f.rows() + seqs + 1, 1 << 30);
   return f;
 }
@@ -78,10 +99,11 @@ inline bool packed_sorted(const PackedForm& f, int64_t seqs, int64_t wgs, int64_
   return f.groups > 1 && f.count && f.count <= kPackedOrder && seqs > 1 && seqs <= kPackedOrderSeqs && wgs * walk >= (int64_t)16384 * 64;
 }
 inline int64_t packed_few(bool bf, int64_t d) { return bf ? 128 : d <= 64 ? 256 : 384; }
+inline int64_t packed_pairs(bool bf, int64_t d) { return !bf ? INT64_MAX : d <= 64 ? 1024 : 768; }
 inline PackedPlan packed_fwd_plan(int64_t tq, int64_t tk, int64_t seqs, int64_t heads, int64_t kvh, int64_t d, bool bf) {
   const int64_t group = heads / kvh, rows = tq * group, wgs = kvh * ((rows + 63) / 64), walk = tk / seqs;
   PackedPlan p = {};
-  p.rows = packed_form(rows, seqs, wgs, walk, packed_few(bf, d), bf ? 1024 : INT64_MAX);
+  p.rows = packed_form(rows, seqs, wgs, walk, packed_few(bf, d), packed_pairs(bf, d), d <= 64 ? 3200 : 2048);
   p.splits = 1;
   if (p.rows.groups == 1) {
     const int64_t tiles = kvh * std::max(seqs, rows / 16);
@@ -112,9 +134,10 @@ inline PackedPlan packed_bwd_plan(int64_t tq, int64_t tk, int64_t seqs, int64_t 
     p.splits = (int)std::min(group, std::max<int64_t>(2, (1024 + key_wgs - 1) / key_wgs));
     p.part_rows = (int)std::max<int64_t>(256, tq * group / seqs * key_wgs / (d > 64 ? 256 : 512) / 8);
   }
-  if (tq) p.rows = packed_form(rows, seqs, wgs, walk, packed_few(bf, d), bf ? 1024 : INT64_MAX);
+  if (tq) p.rows = packed_form(rows, seqs, wgs, walk, packed_few(bf, d), packed_pairs(bf, d), 2048);
   // two tiles of keys a wave would take more registers than two waves a SIMD have at 128 channels
-  if (tk) p.keys = packed_form(tk, seqs, key_wgs * p.splits, tq / seqs, packed_few(bf, d), bf && d <= 64 ? 2048 : INT64_MAX);
+  if (tk) p.keys = packed_form(tk, seqs, key_wgs * p.splits, tq / seqs, packed_few(bf, d),
+                                bf && d <= 64 ? 2048 : INT64_MAX, 0);
   if (p.splits > 1) p.part_o = packed_bytes((size_t)p.splits * kvh * tk * packed_width(d) * sizeof(float));
   p.part_ml = packed_bytes((size_t)heads * tq * sizeof(float));
   if (packed_sorted(p.rows, seqs, wgs, walk)) p.rows_order = packed_bytes((size_t)p.rows.count * sizeof(PackedTile));

@@ -35,3 +35,13 @@ def test_tiles_cover_the_rows():
     for (tq, tk, seqs, heads, kv, _, _), p in zip(some, plans(some)):
         for form, rows in ((p.forward, tq * heads // kv), (p.dq, tq * heads // kv), (p.keys, tk)):
             assert form.count == rows // (16 * form.groups * form.tiles) + seqs + 1
+
+
+def test_two_tiles_a_wave_where_they_were_measured_faster():
+    """Forward: from 768 workgroups of 64 rows on at more than 64 channels, 1024 below; a wave
+    has all keys of a block from 2048 and 3200 on."""
+    for d, pairs, alone in ((128, 768, 2048), (72, 768, 2048), (64, 1024, 3200), (24, 1024, 3200)):
+        wgs = [640, pairs - 2, pairs, alone - 2, alone, 2 * alone]
+        got = plans([(n * 16, n * 16, 4, 4, 2, d, True) for n in wgs])
+        assert [p.forward[1:3] for p in got] == [(2, 1), (2, 1), (2, 2), (2, 2), (1, 2), (1, 2)], d
+        assert all(p.forward.tiles == 1 for p in plans([(n * 16, n * 16, 4, 4, 2, d, False) for n in wgs]))
