@@ -1333,7 +1333,10 @@ int packed_check(const fjx_packed_attention_args* a, const char* fn) {
   return FJX_OK;
 }
 int packed_launch_ok(const char* fn, const PackedForm& f, int64_t kvh, int splits) {
-  if ((double)f.count * kvh * splits >= (1 << 23)) return fail(FJX_ERR_UNSUPPORTED, "%s: more rows than one launch takes", fn);
+  if ((double)f.count * kvh * splits >= (1 << 23))
+    return fail(FJX_ERR_UNSUPPORTED,
+                "%s: 2^23 workgroups and more in a launch; tokens_q * heads and tokens_k * kv_heads up to 2^28 with heads * (sequences + 1) up to 2^20 fit",
+                fn);
   return FJX_OK;
 }
 

@@ -1053,7 +1053,8 @@ def packed_attention(
     that a captured call takes new lengths at each replay. ``causal``: query i of
     nq sees key j of nk where ``j <= i + nk - nq``: each token those before it, new
     tokens their cache. A row without keys is zeros. k and v are finite. ``scale``
-    in [1e-30, 1e30].
+    in [1e-30, 1e30]. Calls of up to 2^28 rows of queries (H Tq) and of keys (Hk Tk),
+    H times the offsets up to 2^20, are always taken, larger ones up to 2^23 workgroups.
 
     Returns ``out`` ``[H, Tq, D]``, a token's heads side by side in memory; rows
     behind the last sequence are zeros. With ``return_lse`` ``(out, lse, rest)``,

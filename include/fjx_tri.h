@@ -548,7 +548,10 @@ enum { FJX_INDEX_I32 = 0, FJX_INDEX_I64 = 1 };
  * For the backward pass: lse [heads, tokens_q, 2] fp32, and `rest` (as out, of
  * bf16), what the output's rounding left.
  * Supported: head_dim a multiple of 8 up to 128, tokens_q * heads and tokens_k below
- * 2^31 - 128 (sequences + 2), sequences below 2^22. Scores, statistics and sums are
+ * 2^31 - 128 (sequences + 2), sequences below 2^22, and below 2^23 workgroups in a launch:
+ * tiles of 16 to 128 rows (backward also keys, for each part of the heads that share
+ * them), one at least a sequence, for each key/value head. tokens_q * heads and
+ * tokens_k * kv_heads up to 2^28 with heads * (sequences + 1) up to 2^20 always fit. Scores, statistics and sums are
  * fp32; bf16 weights enter the product with v rounded once, and the outputs' sum with them
  * (the sum in lse is that of the weights as they were).
  */
