@@ -19,12 +19,14 @@ namespace {
 //
 // Blocks of keys and values come by LDS DMA, the next while one is worked on, fragments
 // from LDS a product ahead. What bounds it: long prompts the issue of vector beside matrix
-// instructions (16384 causal tokens in 6 sequences of up to 9001, 8 heads of 128 on 2: 226 us,
-// 970 TFLOP/s, where a large product reaches 1400); narrow heads the vector instructions,
+// instructions (16384 causal tokens in 6 sequences of up to 9001, 8 heads of 128 on 2: 220 us,
+// 990 TFLOP/s, where a large product reaches 1400; the matrix cores busy in 47 % of the cycles,
+// 3.4 vector instructions to one of theirs, waves issuing in 41 % of theirs and waiting to
+// issue in as many); narrow heads the vector instructions,
 // 5 a score and one of them an exponential, against two matrix products of 24 channels,
-// and the ways in and out (6 crops of 1 to 1003 residues, 16 heads of 24: 14.3 us, of them
-// 3.4 until a workgroup's first block is there and 5.8 walking); single tokens memory (8 caches of 9 to 16384 tokens:
-// 19.0 us, 4.6 TB/s, and the join 4.4).
+// and the ways in and out (6 crops of 1 to 1003 residues, 16 heads of 24: 13.8 us, of them
+// 3.4 until a workgroup's first block is there and 5.8 walking; 14.8 with the statistics);
+// single tokens memory (8 caches of 9 to 16384 tokens: 19.5 us, 4.5 TB/s, and the join 3.8).
 constexpr float kSlack = 8.f;
 
 // An exponent is the rounding of s scale log2(e) - M with M rounded: off by up to half

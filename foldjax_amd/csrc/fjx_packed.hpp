@@ -12,8 +12,8 @@
 // The host knows the number of sequences and of tokens, not the lengths. Sequence s
 // has the tiles from t(s) = floor(first row / R) + s on: t(s + 1) - t(s) is at least
 // its rows / R rounded up, so that no two share a tile, and there are at most
-// (rows / R) + sequences in all; a tile finds its sequence by a search in t, and one
-// that has no rows returns.
+// floor(rows / R) + sequences + 1 in all, the one more for the rows behind the last
+// sequence; a tile finds its sequence by a search in t, and one that has no rows returns.
 #pragma once
 
 #include <type_traits>

@@ -11,13 +11,14 @@
 // it is taken from the output and what its rounding left (17 bits; the forward pass
 // applies rounded weights, but in D they are off in proportion to dS itself). For the
 // same reason dq takes bf16's dS in two parts (17 bits): rounded once, what a row's dS
-// lose no longer sums to zero, and times the keys' common part it was as large as dq's
-// own rounding (0.0026 of dq against 0.0017). dk and dv sum over rows, where nothing
+// lose is as large as dq's own rounding (0.0026 of dq against 0.0017). What the applied
+// weights' rounding leaves in D stays, times the keys' weighted mean: where all keys share a
+// part of 4 times their spread dq is off by 0.0056 (0.0083 with one part). dk and dv sum over rows, where nothing
 // cancels so: weights and dS enter their products rounded once, relative to themselves.
 //
 // us of dq / dk and dv: a step of 8192 causal tokens in 5 sequences of 43 to 4099, 8 heads
-// of 128 on 2: 106 / 142 and the join's 13; of 6 crops of 1 to 1003 residues, 16 heads of
-// 24: 18.7 / 17.9. No one thing bounds them. In variants of the first that left out work,
+// of 128 on 2: 106 / 142 and the join's 11; of 6 crops of 1 to 1003 residues, 16 heads of
+// 24: 19.0 / 17.7. No one thing bounds them. In variants of the first that left out work,
 // half the column fragments' reads were 3 % of both, the exponentials and dS 4 %, the
 // staging of further blocks 8 %, and all blocks but the first left a quarter to a third:
 // finding the tile, the first loads, the outputs. Vector instructions a score, one of them

@@ -1049,8 +1049,10 @@ def packed_attention(
     ``k_starts[s] .. k_starts[s + 1] - 1`` (left out: those of its queries), with
     ``k_lengths`` only the first ``k_lengths[s]`` of them: a cache with room for
     more, whose unused places may hold anything. The offsets are int32 or int64
-    device tensors, from 0 on and not descending; they are read on the device, so
-    that a captured call takes new lengths at each replay. ``causal``: query i of
+    device tensors, from 0 on and not descending (the first counts as 0, whatever it
+    holds: a slice of longer offsets goes with its first one subtracted and the
+    tokens from there on); they are read on the device, so that a captured call
+    takes new lengths at each replay. ``causal``: query i of
     nq sees key j of nk where ``j <= i + nk - nq``: each token those before it, new
     tokens their cache. A row without keys is zeros. k and v are finite. ``scale``
     in [1e-30, 1e30]. Calls of up to 2^28 rows of queries (H Tq) and of keys (Hk Tk),

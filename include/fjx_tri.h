@@ -539,7 +539,7 @@ enum { FJX_INDEX_I32 = 0, FJX_INDEX_I64 = 1 };
  * k_starts[s + 1] - 1, of which only the first k_lengths[s] are there when that
  * is given (what lies behind them, as in a cache with room, is never looked at).
  * Offsets are device values, read by the kernels: [sequences + 1] from 0 on, not
- * descending; offsets that lead out of the buffers are taken as their ends (the
+ * descending (the first counts as 0, whatever it holds); offsets that lead out of the buffers are taken as their ends (the
  * results are then undefined, nothing outside is touched). causal: of nq queries
  * and nk keys, query i sees key j where j <= i + nk - nq (the last query sees all);
  * rows without a key are zeros, with zero gradients. k and v of a sequence's keys
